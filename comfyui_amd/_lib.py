@@ -22,6 +22,7 @@ SRC_F32 = 2
 ACT_NONE = 0
 ACT_GELU = 1
 MAX_EXPERTS = 16
+BLOCK_MAX_EXPERTS = 32
 E_NULL, E_SHAPE, E_WORKSPACE, E_LAUNCH = -1, -2, -3, -4
 TOPK = 2
 NUM_STAGES = 6
@@ -88,6 +89,28 @@ class LayerLayout(ctypes.Structure):
                  "a", "h", "y", "normed", "partials", "flags", "total")]
 
 
+class BlockWeights(ctypes.Structure):
+    """hdmoe_block_weights"""
+    _fields_ = [("weight", c_void_p), ("scale", c_void_p), ("weight3", c_void_p), ("scale3", c_void_p), ("bias", c_void_p)]
+
+
+class BlockRows(ctypes.Structure):
+    """hdmoe_block_rows"""
+    _fields_ = [("a", c_void_p), ("scale_a", c_void_p), ("scale_a_stride", c_int64),
+                ("out", c_void_p), ("scale_out", c_void_p), ("scale_out_stride", c_int64)]
+
+
+class BlockArgs(ctypes.Structure):
+    """hdmoe_block_args"""
+    _fields_ = [
+        ("out_dtype", c_int), ("E", c_int), ("rows", c_int), ("T", c_int), ("K", c_int), ("N", c_int),
+        ("rows_static", c_int), ("K_static", c_int), ("N_static", c_int),
+        ("perm", c_void_p), ("offsets", c_void_p),
+        ("experts", ctypes.POINTER(BlockWeights)), ("shared", ctypes.POINTER(BlockWeights)),
+        ("routed", BlockRows), ("fixed", BlockRows),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/hdmoe.h declares
 SIGNATURES = {
     "hdmoe_version": (c_int, []),
@@ -150,6 +173,9 @@ SIGNATURES = {
                                  ctypes.POINTER(FfnWeights), c_void_p, c_void_p, c_size_t, c_void_p]),
     "hdmoe_ffn_swiglu": (c_int, [c_int, c_void_p, c_int, c_int, c_int, ctypes.POINTER(FfnWeights), c_void_p, c_void_p,
                                  c_size_t, c_void_p]),
+    "hdmoe_quant_block_fp8": (c_int, [c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
+    "hdmoe_block_linear": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
+    "hdmoe_block_swiglu": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
     "hdmoe_layer_layout_get": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(LayerLayout)]),
 }
 

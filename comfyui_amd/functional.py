@@ -546,3 +546,217 @@ def moe_ffn(x2d, gate_w, experts, shared, H, Hs, weight_dtype, out=None, workspa
     if want_routing:
         return out, idx, tw
     return out
+
+
+# ---- e4m3fn with a scale for each block of 128 -------------------------------------------------------------------
+
+BLOCK = 128
+
+
+def _blocks(n):
+    return -(-n // BLOCK)
+
+
+def block_scales(rows, K, device):
+    """Room for the scales of [rows, K] activations: fp32 [rows, ceil(K / 128)], the scales of one block next to each other."""
+    return torch.empty((_blocks(K), rows), dtype=torch.float32, device=device).t()
+
+
+def quant_block_fp8(x):
+    """Cast of 16-bit rows with a scale for every 128 values: x [..., K] bf16 or fp16, K a multiple of 16 ->
+    (float8_e4m3fn of x's shape, fp32 scales [rows, ceil(K / 128)] as block_scales lays them out).
+    scale = max(max|x|, 2^-96) / 448, value = e4m3fn(x * (448 / max(max|x|, 2^-96)))."""
+    dt = _act_dtype(x, "quant_block_fp8 x")
+    _need_hip(x, "quant_block_fp8 x")
+    K = x.shape[-1]
+    rows = x.numel() // K if K > 0 else 0
+    with torch.cuda.device(x.device):
+        q = torch.empty(x.shape, dtype=FP8, device=x.device)
+        s = block_scales(rows, K, x.device)
+        check(lib.hdmoe_quant_block_fp8(W_BF16 if dt == BF16 else _lib.W_F16, ptr(x), rows, K, ptr(q), ptr(s), rows, _stream(x)))
+    return q, s
+
+
+def _block_rows(a, scale_a, what):
+    """(e4m3fn rows, scales laid out as block_scales) of activations: e4m3fn with their scales, or 16-bit ones, which are cast."""
+    if a.dim() != 2:
+        raise ValueError(f"{what}: expected [rows, K] activations, got {tuple(a.shape)}")
+    if a.dtype != FP8:
+        if scale_a is not None:
+            raise TypeError(f"{what}: scales belong to float8_e4m3fn activations, got {a.dtype}")
+        return quant_block_fp8(a)
+    _need_hip(a, what, FP8)
+    if scale_a is None:
+        raise TypeError(f"{what}: float8_e4m3fn activations need their scales")
+    rows, K = a.shape
+    if scale_a.device != a.device or scale_a.dtype != torch.float32 or tuple(scale_a.shape) != (rows, _blocks(K)):
+        raise ValueError(f"{what}: scales must be float32 [{rows}, {_blocks(K)}] on {a.device}, got {scale_a.dtype} "
+                         f"{tuple(scale_a.shape)} on {scale_a.device}")
+    if not scale_a.t().is_contiguous():
+        scale_a = scale_a.t().contiguous().t()
+    return a, scale_a
+
+
+def _block_matrix(weight, scale, K, device, what):
+    """N of a weight [N, K] with scales [ceil(N / 128), ceil(K / 128)]."""
+    if weight.dtype != FP8 or weight.device != device or weight.dim() != 2 or weight.shape[1] != K or not weight.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous float8_e4m3fn weight [N, {K}] on {device}, got {weight.dtype} "
+                         f"{tuple(weight.shape)} on {weight.device}")
+    N = weight.shape[0]
+    if (scale.dtype != torch.float32 or scale.device != device or tuple(scale.shape) != (_blocks(N), _blocks(K))
+            or not scale.is_contiguous()):
+        raise ValueError(f"{what}: expected contiguous float32 scales [{_blocks(N)}, {_blocks(K)}] on {device}, got "
+                         f"{scale.dtype} {tuple(scale.shape)} on {scale.device}")
+    return N
+
+
+def _block_bias(bias, N, dtype, device, what):
+    if bias is not None and (bias.dtype != dtype or bias.device != device or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
+        raise ValueError(f"{what}: expected a contiguous {dtype} bias [{N}] on {device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+    return bias
+
+
+def _block_weights(entry, K, dtype, device, what):
+    """BlockWeights and N of (weight, scale, bias or None) or, for gate/up (dtype None), (w1, scale1, w3, scale3)."""
+    if dtype is None:
+        w1, s1, w3, s3 = entry
+        N = _block_matrix(w1, s1, K, device, what + " w1")
+        if _block_matrix(w3, s3, K, device, what + " w3") != N:
+            raise ValueError(f"{what}: w1 {tuple(w1.shape)} and w3 {tuple(w3.shape)} differ")
+        return _lib.BlockWeights(ptr(w1), ptr(s1), ptr(w3), ptr(s3), None), N
+    w, s, b = entry
+    N = _block_matrix(w, s, K, device, what)
+    return _lib.BlockWeights(ptr(w), ptr(s), None, None, ptr(_block_bias(b, N, dtype, device, what))), N
+
+
+def _block_out_dtype(a, out_dtype, what):
+    if out_dtype is None:
+        out_dtype = BF16 if a.dtype == FP8 else a.dtype
+    if out_dtype not in ACT_DTYPES:
+        raise TypeError(f"{what}: out_dtype must be bfloat16 or float16, got {out_dtype}")
+    return out_dtype
+
+
+def _block_segments(a, offsets, experts, perm, what):
+    """Rows of the experts' segments; checks offsets and perm."""
+    E = len(experts)
+    if not 1 <= E <= _lib.BLOCK_MAX_EXPERTS:
+        raise ValueError(f"{what}: {E} experts (1 to {_lib.BLOCK_MAX_EXPERTS})")
+    if offsets.dtype != torch.int32 or offsets.device != a.device or tuple(offsets.shape) != (E + 1,) or not offsets.is_contiguous():
+        raise ValueError(f"{what}: offsets must be contiguous int32 [{E + 1}] on {a.device}")
+    if perm is None:
+        return a.shape[0]
+    rows = a.shape[0] * _lib.TOPK
+    if perm.dtype != torch.int32 or perm.device != a.device or tuple(perm.shape) != (rows,) or not perm.is_contiguous():
+        raise ValueError(f"{what}: perm must be contiguous int32 [{rows}] on {a.device}")
+    return rows
+
+
+def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype=None):
+    """x [rows, K] times weight [N, K]^T (+ bias [N]): weight float8_e4m3fn with fp32 scales scale_weight
+    [ceil(N / 128), ceil(K / 128)]; x bf16 or fp16 (cast as quant_block_fp8 does), or float8_e4m3fn with its scales scale_x
+    [rows, ceil(K / 128)]. -> [rows, N] of x's type (out_dtype, bf16 unless given, for float8_e4m3fn x). K and N are multiples
+    of 16. The sums are fp32; bias joins them before the one rounding."""
+    what = "linear_block_fp8"
+    dt = _block_out_dtype(x, out_dtype, what)
+    q, s = _block_rows(x, scale_x, what + " x")
+    rows, K = q.shape
+    w, N = _block_weights((weight, scale_weight, bias), K, dt, q.device, what)
+    with torch.cuda.device(q.device):
+        out = torch.empty((rows, N), dtype=dt, device=q.device)
+        if rows == 0:
+            return out
+        args = _lib.BlockArgs()
+        args.out_dtype = W_BF16 if dt == BF16 else _lib.W_F16
+        args.rows_static, args.K_static, args.N_static = rows, K, N
+        args.shared = ctypes.pointer(w)
+        args.fixed = _lib.BlockRows(ptr(q), ptr(s), rows, ptr(out), None, 0)
+        check(lib.hdmoe_block_linear(ctypes.byref(args), _stream(q)))
+    return out
+
+
+def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, perm=None, shared=None, a_static=None,
+                             scale_static=None):
+    """linear_block_fp8 of every expert over its row segment [offsets[e], offsets[e + 1]) of a [rows, K]. experts: list of
+    (weight [N, K], scale, bias [N] or None), at most 32; offsets: int32 [E + 1] on the device, ascending. a as in linear_block_fp8.
+    perm: the dispatch's permutation, sorted row r being row perm[r] // 2 of a [T, K]; the output then has 2T rows. Rows that no
+    segment holds are not written. -> out [rows, N].
+    shared: one more (weight, scale, bias) over all rows of a_static (with scale_static), of sizes of its own, in the same launch;
+    -> (out, out_static)."""
+    what = "grouped_linear_block_fp8"
+    dt = _block_out_dtype(a, out_dtype, what)
+    a, sa = _block_rows(a, scale_a, what + " a")
+    dev = a.device
+    rows = _block_segments(a, offsets, experts, perm, what)
+    K = a.shape[1]
+    packed = [_block_weights(e, K, dt, dev, what) for e in experts]
+    N = packed[0][1]
+    if any(n != N for _, n in packed):
+        raise ValueError(f"{what}: the experts' weights differ in size")
+    with torch.cuda.device(dev):
+        args = _lib.BlockArgs()
+        args.out_dtype = W_BF16 if dt == BF16 else _lib.W_F16
+        out = torch.empty((rows, N), dtype=dt, device=dev)
+        if rows > 0:
+            args.E, args.rows, args.K, args.N = len(experts), rows, K, N
+            if perm is not None:
+                args.perm, args.T = ptr(perm), a.shape[0]
+            args.offsets = ptr(offsets)
+            args.experts = (_lib.BlockWeights * len(experts))(*(w for w, _ in packed))
+            args.routed = _lib.BlockRows(ptr(a), ptr(sa), a.shape[0], ptr(out), None, 0)
+        out_static = None
+        if shared is not None:
+            if a_static is None:
+                raise ValueError(f"{what}: shared needs a_static")
+            q, s = _block_rows(a_static, scale_static, what + " a_static")
+            if q.device != dev:
+                raise ValueError(f"{what}: a_static is on {q.device}")
+            n, Ks = q.shape
+            w, Ns = _block_weights(shared, Ks, dt, dev, what + " shared")
+            out_static = torch.empty((n, Ns), dtype=dt, device=dev)
+            if n > 0:
+                args.rows_static, args.K_static, args.N_static = n, Ks, Ns
+                args.shared = ctypes.pointer(w)
+                args.fixed = _lib.BlockRows(ptr(q), ptr(s), n, ptr(out_static), None, 0)
+        check(lib.hdmoe_block_linear(ctypes.byref(args), _stream(a)))
+    return out if shared is None else (out, out_static)
+
+
+def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, shared=None):
+    """First half of every expert's SwiGLU feed-forward, silu(a w1^T) * (a w3^T), cast as quant_block_fp8 does:
+    experts: list of (w1 [H, K], scale1, w3 [H, K], scale3); a, scale_a, offsets, perm as in grouped_linear_block_fp8.
+    -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]); everything before the cast is fp32.
+    shared: one more (w1, scale1, w3, scale3) over all rows of a, with a width of its own, in the same launch;
+    -> (h, scales, h_shared, scales_shared)."""
+    what = "grouped_swiglu_block_fp8"
+    a, sa = _block_rows(a, scale_a, what + " a")
+    dev = a.device
+    rows = _block_segments(a, offsets, experts, perm, what)
+    n, K = a.shape
+    packed = [_block_weights(e, K, None, dev, what) for e in experts]
+    H = packed[0][1]
+    if any(h != H for _, h in packed):
+        raise ValueError(f"{what}: the experts' weights differ in size")
+    with torch.cuda.device(dev):
+        args = _lib.BlockArgs()
+        args.out_dtype = W_BF16
+        h = torch.empty((rows, H), dtype=FP8, device=dev)
+        sh = block_scales(rows, H, dev)
+        h_shared = sh_shared = None
+        if rows > 0:
+            args.E, args.rows, args.K, args.N = len(experts), rows, K, H
+            if perm is not None:
+                args.perm, args.T = ptr(perm), n
+            args.offsets = ptr(offsets)
+            args.experts = (_lib.BlockWeights * len(experts))(*(w for w, _ in packed))
+            args.routed = _lib.BlockRows(ptr(a), ptr(sa), n, ptr(h), ptr(sh), rows)
+        if shared is not None:
+            w, Hs = _block_weights(shared, K, None, dev, what + " shared")
+            h_shared = torch.empty((n, Hs), dtype=FP8, device=dev)
+            sh_shared = block_scales(n, Hs, dev)
+            if n > 0:
+                args.rows_static, args.K_static, args.N_static = n, K, Hs
+                args.shared = ctypes.pointer(w)
+                args.fixed = _lib.BlockRows(ptr(a), ptr(sa), n, ptr(h_shared), ptr(sh_shared), n)
+        check(lib.hdmoe_block_swiglu(ctypes.byref(args), _stream(a)))
+    return (h, sh) if shared is None else (h, sh, h_shared, sh_shared)

@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define HDMOE_VERSION 116
+#define HDMOE_VERSION 117
 
 #define HDMOE_OK 0
 #define HDMOE_E_NULL (-1)      /* required pointer is NULL */
@@ -366,6 +366,62 @@ int hdmoe_combine_gated_residual(const void* y_sorted_bf16, const int32_t* inv_p
  * out[t] = bf16( bf16(gate[t / tokens_per_batch] * y[t]) + residual[t] ). */
 int hdmoe_gated_residual_bf16(const void* y_bf16, const void* gate_bf16, const void* residual_bf16,
                               int tokens_per_batch, int T, int D, void* out_bf16, hdmoe_stream_t stream);
+
+/* ---- e4m3fn with a scale for each block of 128 --------------------------------- */
+
+/* Linears whose weights carry one fp32 scale for every 128 x 128 block and whose activations carry one for every 128
+ * consecutive values of a row (the last block of a row or column may be short). The reference's scaled-fp8 Linear has one scale
+ * for a whole tensor (comfy/ops.py:379-428); it has nothing of this kind.
+ *
+ * hdmoe_quant_block_fp8 casts rows: for every block, with fp32 arithmetic,
+ *   top = max(max|x|, 2^-96),  scale = top / 448,  out = e4m3fn(x * (448 / top))
+ * so that x is about out * scale. A block that holds NaN or an infinity becomes NaN. x [rows,K] bf16 or fp16 (src_dtype
+ * HDMOE_W_BF16 / HDMOE_W_F16), 16-byte aligned; out [rows,K]; the scale of block b of row r is scale[b * scale_stride + r]
+ * (scale_stride >= rows). K % 16 == 0. */
+int hdmoe_quant_block_fp8(int src_dtype, const void* x, int64_t rows, int K, void* out_e4m3fn, float* scale,
+                          int64_t scale_stride, hdmoe_stream_t stream);
+
+#define HDMOE_BLOCK_MAX_EXPERTS 32
+typedef struct hdmoe_block_weights {
+  const void* weight;   /* e4m3fn [N,K]; gate/up: w1 */
+  const float* scale;   /* [ceil(N/128), ceil(K/128)], device */
+  const void* weight3;  /* gate/up: w3 [N,K] */
+  const float* scale3;  /* gate/up: its scales */
+  const void* bias;     /* [N] of out_dtype or NULL (not read by gate/up) */
+} hdmoe_block_weights;
+typedef struct hdmoe_block_rows {
+  const void* a;            /* e4m3fn [rows,K] */
+  const float* scale_a;     /* of block b of row r at scale_a[b * scale_a_stride + r] */
+  int64_t scale_a_stride;
+  void* out;                /* [rows,N] of out_dtype; gate/up: e4m3fn [rows,N] */
+  float* scale_out;         /* gate/up: of block b of row r at scale_out[b * scale_out_stride + r] */
+  int64_t scale_out_stride;
+} hdmoe_block_rows;
+/* Experts over the row segments of a dispatched batch, and optionally one more group over all rows of another input (a shared
+ * expert, or the one weight of a dense Linear). Expert e takes rows [offsets[e], offsets[e + 1]) (ascending, device; bounds beyond
+ * 0 .. rows are cut off); rows in no segment are left as they were. perm (NULL = the rows are in segment order): sorted row r is
+ * row perm[r] / 2 of routed.a [T,K] and its scales. All matrices start on 16 bytes; K % 16 == 0, N % 16 == 0. */
+typedef struct hdmoe_block_args {
+  int out_dtype;      /* HDMOE_W_BF16 or HDMOE_W_F16 (hdmoe_block_linear: output and bias) */
+  int E;              /* experts, 0 = none, at most HDMOE_BLOCK_MAX_EXPERTS */
+  int rows;           /* rows of the segments together (rows of routed.out) */
+  int T;              /* rows of routed.a when perm is set (rows == 2 T) */
+  int K, N;
+  int rows_static;    /* rows of the static group, 0 = none */
+  int K_static, N_static;
+  const int32_t* perm;
+  const int32_t* offsets;             /* [E+1], device */
+  const hdmoe_block_weights* experts; /* host array [E] */
+  const hdmoe_block_weights* shared;  /* of the static group */
+  hdmoe_block_rows routed, fixed;     /* the experts' rows, the static group's */
+} hdmoe_block_args;
+
+/* out[r, n] = round( sum_b scale_a[r, b] * scale[n / 128, b] * sum_{k in block b} a[r, k] * weight[n, k]  + bias[n] ); the sums over
+ * a block are the matrix cores', the one over blocks is fp32, and there is one rounding to out_dtype. */
+int hdmoe_block_linear(const hdmoe_block_args* args, hdmoe_stream_t stream);
+/* The first half of a SwiGLU feed-forward: h = silu(g) * u with g and u such sums over w1 and w3, all in fp32, and the cast of h's rows
+ * as hdmoe_quant_block_fp8 makes it (out, scale_out). */
+int hdmoe_block_swiglu(const hdmoe_block_args* args, hdmoe_stream_t stream);
 
 /* ---- whole layer -------------------------------------------------------------- */
 
