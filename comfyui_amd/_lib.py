@@ -103,11 +103,12 @@ class BlockRows(ctypes.Structure):
 class BlockArgs(ctypes.Structure):
     """hdmoe_block_args"""
     _fields_ = [
-        ("out_dtype", c_int), ("E", c_int), ("rows", c_int), ("T", c_int), ("K", c_int), ("N", c_int),
+        ("a_dtype", c_int), ("out_dtype", c_int), ("E", c_int), ("rows", c_int), ("T", c_int), ("K", c_int), ("N", c_int),
         ("rows_static", c_int), ("K_static", c_int), ("N_static", c_int),
         ("perm", c_void_p), ("offsets", c_void_p),
         ("experts", ctypes.POINTER(BlockWeights)), ("shared", ctypes.POINTER(BlockWeights)),
         ("routed", BlockRows), ("fixed", BlockRows),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 
 
@@ -174,6 +175,7 @@ SIGNATURES = {
     "hdmoe_ffn_swiglu": (c_int, [c_int, c_void_p, c_int, c_int, c_int, ctypes.POINTER(FfnWeights), c_void_p, c_void_p,
                                  c_size_t, c_void_p]),
     "hdmoe_quant_block_fp8": (c_int, [c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
+    "hdmoe_block_workspace_bytes": (c_size_t, [c_int] * 6),
     "hdmoe_block_linear": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
     "hdmoe_block_swiglu": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
     "hdmoe_layer_layout_get": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(LayerLayout)]),

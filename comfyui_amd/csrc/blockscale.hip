@@ -71,7 +71,7 @@ struct Group {
 
 // Rows and sizes that the experts' groups share, and those of the static one.
 struct Operand {
-  const uint8_t* a;     // e4m3fn rows of K bytes
+  const uint8_t* a;     // e4m3fn rows of K bytes (few rows, cast inside: 16-bit rows of K values)
   const float* sa;      // scale of block b of row r at sa[b * ld_sa + r]
   const int32_t* gather;  // NULL, or sorted row r is row gather[r] >> 1 of a
   long long ld_sa;
@@ -88,6 +88,7 @@ struct BlockArgs {
   Operand op[2];        // the experts' operand, the static group's
   const int32_t* offsets;
   int E;
+  int lds_rows;         // few rows, cast inside: rows that a tile can have (the tile's height at most)
 };
 
 __device__ __forceinline__ int swz(int row) { return ((row >> 1) & 7) ^ ((row & 1) << 2); }
@@ -359,6 +360,226 @@ __global__ __launch_bounds__(64 * WF * WT) void block_gemm_kernel(const BlockArg
 #endif
 }
 
+// ---- few rows -----------------------------------------------------------------------------------------------------
+// Segments of up to a few dozen rows: the weights are read once from memory into registers, no tile of them passes through LDS, and
+// many 16-byte loads are on their way at once. A wave multiplies 16 weight rows (a strip) with TT * 16 tokens.
+//   Linear:  the NW waves of a block share one strip and deal its K blocks out; their sums meet in LDS.
+//   gate/up: 16 waves hold the 8 + 8 strips of w1 and w3 behind one block of the cast output, each over all of K.
+// CAST: the activations are 16-bit rows; the block casts its own into LDS (rows of K + 16 bytes: 16 rows then hit all banks) while the
+// first weights are on their way, instead of a launch of its own in front.
+template <class Act>
+__device__ __forceinline__ void cast_unit(const uint16_t* x, int k, bool in, uint32_t (&o)[2], float& s) {
+  u32x4 v = {0, 0, 0, 0};
+  if (in) v = *reinterpret_cast<const u32x4*>(x + k);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, max(v[i] & 0x7fffu, (v[i] >> 16) & 0x7fffu));
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 16));
+  const float top_in = Act::lo(m);
+  const float top = top_in < TOP_FLOOR ? TOP_FLOOR : top_in;
+  const float r = 448.0f / top;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    o[i] = hdmoe_dev_pack4_e4m3fn(Act::lo(v[2 * i]) * r, Act::hi(v[2 * i]) * r, Act::lo(v[2 * i + 1]) * r, Act::hi(v[2 * i + 1]) * r);
+  s = top / 448.0f;
+}
+
+template <class Act, bool SWIGLU, int TT, bool CAST>
+__global__ __launch_bounds__(SWIGLU ? 1024 : 512) void block_stream_kernel(const BlockArgs args) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int NW = SWIGLU ? 16 : 8;
+  constexpr int BM = TT * 16;
+  constexpr int FEAT = SWIGLU ? BLK : 16;
+  constexpr int DEPTH = SWIGLU ? (TT == 1 || CAST ? 4 : 2) : (TT == 1 ? 6 : 4);   // K blocks on their way (in registers: 16 waves have 128 each)
+  constexpr int OUTSIDE = (int)0x80000000u;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, quad = lane >> 4;
+
+  const Tiles<BM, FEAT> tiles(args, lane);
+  const int per_xcd = (tiles.total + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD;
+  const int slot = blockIdx.x / HDMOE_NUM_XCD;
+  const int L = (int)(blockIdx.x % HDMOE_NUM_XCD) * per_xcd + slot;
+  if (slot >= per_xcd || L >= tiles.total) return;
+  const Tile t = tiles.get(L);
+  const Group& grp = args.g[t.g];
+  const Operand& op = args.op[t.g == args.E ? 1 : 0];
+  const int K = op.K, N = op.N;
+  const int KB = (K + BLK - 1) / BLK;
+  const bool gathers = op.gather != nullptr;
+
+  // weights: lane = row fr of the strip, 16-byte chunks quad and quad + 4 of a K block
+  const int strip = SWIGLU ? wave & 7 : 0;
+  const bool third = SWIGLU && wave >= 8;
+  const uint8_t* const wp = (third ? grp.w1 : grp.w0) + (size_t)(t.n0 + strip * 16) * K;
+  const bool has_strip = t.n0 + strip * 16 < N;            // N is a multiple of 16
+  const __amdgpu_buffer_rsrc_t rw = make_rsrc(has_strip ? wp : nullptr, has_strip ? 16u * (uint32_t)K : 0u);
+  const float* const sw = (third ? grp.s1 : grp.s0) + (size_t)(t.n0 / BLK) * KB;
+  const int kb_first = SWIGLU ? 0 : wave, kb_step = SWIGLU ? 1 : NW;
+
+  // tokens: column fr of each tile
+  int row[TT];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) {
+    const int r = tt * 16 + fr;
+    row[tt] = -1;
+    if (r < t.rows_here) {
+      row[tt] = gathers ? op.gather[t.row0 + r] >> 1 : t.row0 + r;
+      if ((unsigned)row[tt] >= (unsigned)op.a_rows) row[tt] = -1;
+    }
+  }
+
+  struct Step { v4i w[2]; v4i x[TT][2]; float sw, sx[TT]; };
+  auto load = [&](Step& st, int kb) {
+    const int k = kb * BLK + quad * 16;
+    st.w[0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, k < K ? fr * K + k : OUTSIDE, 0, 0));
+    st.w[1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, k + 64 < K ? fr * K + k + 64 : OUTSIDE, 0, 0));
+    st.sw = kb < KB ? sw[kb] : 0.0f;
+    if constexpr (!CAST) {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+        const uint8_t* const xr = op.a + (size_t)max(row[tt], 0) * K + k;
+        st.x[tt][0] = st.x[tt][1] = v4i{0, 0, 0, 0};
+        if (row[tt] >= 0 && k < K) st.x[tt][0] = *reinterpret_cast<const v4i*>(xr);
+        if (row[tt] >= 0 && k + 64 < K) st.x[tt][1] = *reinterpret_cast<const v4i*>(xr + 64);
+        st.sx[tt] = row[tt] >= 0 && kb < KB ? op.sa[(size_t)kb * op.ld_sa + row[tt]] : 0.0f;
+      }
+    }
+  };
+  Step st[DEPTH];
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i) load(st[i], kb_first + i * kb_step);
+
+  // [rows][ld_x] cast rows, [KB][rows] scales; a column without a row reads the last one's and is never stored
+  const int ld_x = KB * BLK + 16, R = args.lds_rows;
+  uint8_t* const lx = smem;
+  float* const ls = reinterpret_cast<float*>(smem + (size_t)R * ld_x);
+  if constexpr (CAST) {
+    const uint16_t* const x16 = reinterpret_cast<const uint16_t*>(op.a);
+    const int units = R * KB;
+    for (int u = tid >> 4; u < units; u += NW * 4) {
+      const int r = u / KB, b = u - r * KB;
+      int from = -1;
+      if (r < t.rows_here) {
+        from = gathers ? op.gather[t.row0 + r] >> 1 : t.row0 + r;
+        if ((unsigned)from >= (unsigned)op.a_rows) from = -1;
+      }
+      const int k = b * BLK + (tid & 15) * 8;
+      uint32_t o[2];
+      float s;
+      cast_unit<Act>(x16 + (size_t)max(from, 0) * K, k, from >= 0 && k < K, o, s);
+      *reinterpret_cast<u32x2*>(lx + r * ld_x + k) = u32x2{o[0], o[1]};
+      if ((tid & 15) == 0) ls[b * R + r] = from >= 0 ? s : 0.0f;
+    }
+    __syncthreads();
+  }
+
+  v4f acc[TT];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) acc[tt] = v4f{0, 0, 0, 0};
+  auto multiply = [&](const Step& st, int kb) {
+    const v8i fa = {st.w[0].x, st.w[0].y, st.w[0].z, st.w[0].w, st.w[1].x, st.w[1].y, st.w[1].z, st.w[1].w};
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      v4i x0, x1;
+      float sx;
+      if constexpr (CAST) {
+        const int r = min(tt * 16 + fr, R - 1);
+        const uint8_t* const xr = lx + r * ld_x + kb * BLK + quad * 16;
+        x0 = *reinterpret_cast<const v4i*>(xr);
+        x1 = *reinterpret_cast<const v4i*>(xr + 64);
+        sx = ls[kb * R + r];
+      } else {
+        x0 = st.x[tt][0];
+        x1 = st.x[tt][1];
+        sx = st.sx[tt];
+      }
+      const v8i fb = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+      const v4f p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb, v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+      const float m = sx * st.sw;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[tt][i] = __builtin_fmaf(p[i], m, acc[tt][i]);
+    }
+  };
+  for (int kb0 = kb_first; kb0 < KB; kb0 += DEPTH * kb_step) {
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      const int kb = kb0 + i * kb_step;
+      if (kb < KB) multiply(st[i], kb);
+      load(st[i], kb + DEPTH * kb_step);
+    }
+  }
+  __syncthreads();   // the cast rows are read no more
+
+  if constexpr (!SWIGLU) {
+    // the waves' sums, [NW][TT][64] of 16 bytes; then wave w forms token tile w
+    v4f* const parts = reinterpret_cast<v4f*>(smem);
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) parts[(wave * TT + tt) * 64 + lane] = acc[tt];
+    __syncthreads();
+    if (wave >= TT) return;
+    v4f y = parts[wave * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      const v4f v = parts[(w * TT + wave) * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] += v[i];
+    }
+    const int r = wave * 16 + fr, f = t.n0 + quad * 4;
+    if (r >= t.rows_here) return;
+    if (grp.bias != nullptr) {
+      const u32x2 b = *reinterpret_cast<const u32x2*>(grp.bias + f);
+      y[0] += Act::lo(b.x); y[1] += Act::hi(b.x); y[2] += Act::lo(b.y); y[3] += Act::hi(b.y);
+    }
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(op.out) + (size_t)(t.row0 + r) * N + f) = u32x2{Act::pack(y[0], y[1]), Act::pack(y[2], y[3])};
+  } else {
+    // u from the upper eight waves to the lower ones, which form silu(g) * u, its largest value of a token and the cast
+    v4f* const us = reinterpret_cast<v4f*>(smem);                                   // [8][TT][64]
+    uint32_t* const tops = reinterpret_cast<uint32_t*>(smem + 8 * TT * 64 * 16);    // [8][BM]
+    if (third) {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) us[(strip * TT + tt) * 64 + lane] = acc[tt];
+    }
+    __syncthreads();
+    if (!third) {
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+        const v4f u = us[(strip * TT + tt) * 64 + lane];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float g = acc[tt][i];
+          acc[tt][i] = g / (1.0f + __expf(-g)) * u[i];
+          top = max(top, __float_as_uint(acc[tt][i]) & 0x7fffffffu);
+        }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+        if (quad == 0) tops[strip * BM + tt * 16 + fr] = top;
+      }
+    }
+    __syncthreads();
+    if (third) return;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      const int r = tt * 16 + fr;
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, tops[j * BM + r]);
+      const float both = __uint_as_float(top);
+      const float tp = both < TOP_FLOOR ? TOP_FLOOR : both;
+      const float m = 448.0f / tp;
+      if (r >= t.rows_here) continue;
+      if (wave == 0 && quad == 0) op.s_out[(size_t)(t.n0 / BLK) * op.ld_out + t.row0 + r] = tp / 448.0f;
+      if (!has_strip) continue;
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(op.out) + (size_t)(t.row0 + r) * N + t.n0 + strip * 16 + quad * 4) =
+          hdmoe_dev_pack4_e4m3fn(acc[tt][0] * m, acc[tt][1] * m, acc[tt][2] * m, acc[tt][3] * m);
+    }
+  }
+#endif
+}
+
 // ---- launch -------------------------------------------------------------------------------------------------------
 // The opt-in for more than 64 KiB of LDS, once per kernel and device.
 template <class Kernel>
@@ -373,19 +594,43 @@ int allow_lds(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done, const ch
   return HDMOE_OK;
 }
 
+// At most this many tiles, whatever the segments: every one of them can end in a tile that is not full. Rounded up to the XCDs.
+long long grid_of(const BlockArgs& args, int bm, int feat) {
+  long long tiles = 0;
+  if (args.E > 0) {
+    const long long rows = args.op[0].rows, ends = rows < args.E ? rows : args.E;   // the ends take a row each at least
+    tiles += ((rows - ends) / bm + ends) * ((args.op[0].N + feat - 1) / feat);
+  }
+  tiles += ((long long)args.op[1].rows + bm - 1) / bm * ((args.op[1].N + feat - 1) / feat);
+  return (tiles + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD * HDMOE_NUM_XCD;
+}
+
 template <class Act, bool SWIGLU, int WF, int WT, int TT>
 int launch_gemm(const BlockArgs& args, const char* what, hipStream_t stream) {
   constexpr int BM = WT * TT * 16, FEAT = SWIGLU ? WF * BLK / 2 : WF * BLK;
   constexpr size_t SMEM = 2 * (size_t)(BM + WF * BLK) * BLK;
   static std::atomic<uint64_t> done{0};
   if (int rc = allow_lds(block_gemm_kernel<Act, SWIGLU, WF, WT, TT>, SMEM, done, what)) return rc;
-  // at most this many tiles, whatever the segments: every one of them can end in a tile that is not full
-  long long tiles = 0;
-  if (args.E > 0) tiles += ((long long)args.op[0].rows / BM + (args.op[0].rows < args.E ? args.op[0].rows : args.E)) * ((args.op[0].N + FEAT - 1) / FEAT);
-  tiles += ((long long)args.op[1].rows + BM - 1) / BM * ((args.op[1].N + FEAT - 1) / FEAT);
-  const long long grid = (tiles + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD * HDMOE_NUM_XCD;
-  if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, tiles);
+  const long long grid = grid_of(args, BM, FEAT);
+  if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
   block_gemm_kernel<Act, SWIGLU, WF, WT, TT><<<(unsigned)grid, 64 * WF * WT, SMEM, stream>>>(args);
+  return hdmoe_check_launch(what);
+}
+
+// LDS of a few-row block: cast rows and their scales, later the exchange between waves
+size_t stream_lds(bool swiglu, int tt, int lds_rows, int K) {
+  const size_t exchange = (size_t)tt * 64 * 16 * 8 + (swiglu ? (size_t)8 * tt * 16 * 4 : 0);
+  const size_t KB = (K + BLK - 1) / BLK;
+  const size_t rows = (size_t)lds_rows * (KB * BLK + 16 + KB * 4);
+  return rows > exchange ? rows : exchange;
+}
+
+template <class Act, bool SWIGLU, int TT, bool CAST>
+int launch_stream(const BlockArgs& args, const char* what, hipStream_t stream) {
+  const int K = args.op[0].K > args.op[1].K ? args.op[0].K : args.op[1].K;
+  const long long grid = grid_of(args, TT * 16, SWIGLU ? BLK : 16);
+  if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
+  block_stream_kernel<Act, SWIGLU, TT, CAST><<<(unsigned)grid, SWIGLU ? 1024 : 512, stream_lds(SWIGLU, TT, CAST ? args.lds_rows : 0, K), stream>>>(args);
   return hdmoe_check_launch(what);
 }
 
@@ -427,10 +672,34 @@ extern "C" int hdmoe_quant_block_fp8(int src_dtype, const void* x, int64_t rows,
 
 namespace {
 
-// Arguments of both contractions -> those of the kernels; checks everything but what only the device knows.
-int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& args) {
+// How a call runs: the few-row kernels on tiles of 16 * tt rows (tt > 0; with the cast inside or not), or the tiles of
+// block_gemm_kernel.
+struct Plan { int tt; bool cast_inside; int lds_rows; };
+
+Plan plan_of(bool swiglu, bool x16, int rows, int E, int rows_static, int K) {
+  Plan p = {0, false, 0};
+  const int per = E > 0 ? (rows + E - 1) / E : 0, most = per > rows_static ? per : rows_static;   // rows of a segment, if they are even
+  if (most <= 16) p.tt = 1;
+  else if (most <= 32) p.tt = 2;
+  if (p.tt > 0 && x16) {
+    // a block casts for itself where that takes its threads a few trips at most
+    const int whole = rows > rows_static ? rows : rows_static;
+    p.lds_rows = whole < 16 * p.tt ? whole : 16 * p.tt;
+    p.cast_inside = (long long)p.lds_rows * ((K + BLK - 1) / BLK) * 16 <= 4 * (swiglu ? 1024 : 512);
+  }
+  return p;
+}
+
+size_t cast_bytes(long long rows, int K) { return hdmoe_align_up((size_t)rows * K, 256) + (size_t)rows * ((K + BLK - 1) / BLK) * 4; }
+
+// Arguments of both contractions -> those of the kernels; checks everything but what only the device knows. 16-bit activations are
+// cast into the workspace here unless the contraction does that itself.
+int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& args, Plan& plan, hipStream_t stream) {
   HDMOE_REQUIRE_PTR(p);
-  if (p->out_dtype != HDMOE_W_BF16 && p->out_dtype != HDMOE_W_F16) return hdmoe_fail(HDMOE_E_SHAPE, "%s: out_dtype=%d", what, p->out_dtype);
+  const bool x16 = p->a_dtype == HDMOE_W_BF16 || p->a_dtype == HDMOE_W_F16;
+  if ((p->out_dtype != HDMOE_W_BF16 && p->out_dtype != HDMOE_W_F16) || (!x16 && p->a_dtype != HDMOE_W_E4M3FN) ||
+      (x16 && !swiglu && p->a_dtype != p->out_dtype))
+    return hdmoe_fail(HDMOE_E_SHAPE, "%s: a_dtype=%d out_dtype=%d", what, p->a_dtype, p->out_dtype);
   if (p->E < 0 || p->E > MAX_E || p->rows < 0 || p->rows_static < 0 || (p->E == 0 && p->rows > 0))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: E=%d (at most %d) rows=%d rows_static=%d", what, p->E, MAX_E, p->rows, p->rows_static);
   args = BlockArgs{};
@@ -448,10 +717,10 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
   };
   auto operand = [&](const hdmoe_block_rows& r, int rows, int K, int N, const int32_t* perm, int T, Operand& op) -> int {
     const int a_rows = perm != nullptr ? T : rows;
-    if (r.a == nullptr || r.scale_a == nullptr || r.out == nullptr || (swiglu && r.scale_out == nullptr))
+    if (r.a == nullptr || (!x16 && r.scale_a == nullptr) || r.out == nullptr || (swiglu && r.scale_out == nullptr))
       return hdmoe_fail(HDMOE_E_NULL, "%s: activations, their scales or the output are NULL", what);
     if (!aligned16(r.a) || !aligned16(r.out)) return hdmoe_fail(HDMOE_E_SHAPE, "%s: activations and outputs must start on 16 bytes", what);
-    if (r.scale_a_stride < a_rows || (swiglu && r.scale_out_stride < rows))
+    if ((!x16 && r.scale_a_stride < a_rows) || (swiglu && r.scale_out_stride < rows))
       return hdmoe_fail(HDMOE_E_SHAPE, "%s: scale strides %lld, %lld for %d rows", what, (long long)r.scale_a_stride, (long long)r.scale_out_stride, a_rows);
     if (perm != nullptr && (long long)a_rows * K > 0x7fffffffll)
       return hdmoe_fail(HDMOE_E_SHAPE, "%s: %d rows of K=%d read through a permutation: at most 2 GiB", what, a_rows, K);
@@ -468,7 +737,8 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
     op.ld_out = r.scale_out_stride;
     return HDMOE_OK;
   };
-  if (p->E > 0 && p->rows > 0) {
+  const bool routed = p->E > 0 && p->rows > 0;
+  if (routed) {
     if (int rc = check_sizes(what, "", p->rows, p->K, p->N)) return rc;
     HDMOE_REQUIRE_PTR(p->offsets);
     HDMOE_REQUIRE_PTR(p->experts);
@@ -486,23 +756,59 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
     if (int rc = weights(*p->shared, args.g[args.E])) return rc;
     if (int rc = operand(p->fixed, p->rows_static, p->K_static, p->N_static, nullptr, 0, args.op[1])) return rc;
   }
+  const int a_rows = routed ? args.op[0].a_rows : p->rows_static, K = routed ? p->K : p->K_static;
+  if (x16 && routed && p->rows_static > 0 && (p->fixed.a != p->routed.a || p->rows_static != a_rows || p->K_static != K))
+    return hdmoe_fail(HDMOE_E_SHAPE, "%s: 16-bit activations of the experts and of the static group must be the same rows", what);
+  plan = plan_of(swiglu, x16, routed ? p->rows : 0, routed ? p->E : 0, p->rows_static, K);
+  args.lds_rows = plan.lds_rows;
+  if (a_rows > 0 && x16 && !plan.cast_inside) {
+    if (p->workspace == nullptr || p->workspace_bytes < cast_bytes(a_rows, K) || (reinterpret_cast<uintptr_t>(p->workspace) & 255))
+      return hdmoe_fail(HDMOE_E_WORKSPACE, "%s: workspace %zu bytes, need %zu (256-byte aligned)", what, p->workspace_bytes, cast_bytes(a_rows, K));
+    uint8_t* const q = static_cast<uint8_t*>(p->workspace);
+    float* const s = reinterpret_cast<float*>(q + hdmoe_align_up((size_t)a_rows * K, 256));
+    if (int rc = hdmoe_quant_block_fp8(p->a_dtype, routed ? p->routed.a : p->fixed.a, a_rows, K, q, s, a_rows, stream)) return rc;
+    for (Operand& op : args.op) {
+      op.a = q;
+      op.sa = s;
+      op.ld_sa = a_rows;
+    }
+  }
   return HDMOE_OK;
+}
+
+template <class Act, bool SWIGLU>
+int launch_few(const BlockArgs& args, const Plan& plan, const char* what, hipStream_t s) {
+  if (plan.cast_inside) return plan.tt == 1 ? launch_stream<Act, SWIGLU, 1, true>(args, what, s) : launch_stream<Act, SWIGLU, 2, true>(args, what, s);
+  return plan.tt == 1 ? launch_stream<Act, SWIGLU, 1, false>(args, what, s) : launch_stream<Act, SWIGLU, 2, false>(args, what, s);
 }
 
 }  // namespace
 
+extern "C" size_t hdmoe_block_workspace_bytes(int swiglu, int rows, int E, int T, int rows_static, int K) {
+  if (rows < 0 || E < 0 || T < 0 || rows_static < 0 || K <= 0) return 0;
+  return plan_of(swiglu != 0, true, rows, E, rows_static, K).cast_inside ? 0 : cast_bytes(rows > 0 ? (T > 0 ? T : rows) : rows_static, K);
+}
+
 extern "C" int hdmoe_block_linear(const hdmoe_block_args* p, hdmoe_stream_t stream) {
+  const char* what = "hdmoe_block_linear";
   BlockArgs args;
-  if (int rc = fill("hdmoe_block_linear", p, false, args)) return rc;
-  if (args.op[0].rows + (long long)args.op[1].rows == 0) return HDMOE_OK;
+  Plan plan;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return p->out_dtype == HDMOE_W_BF16 ? launch_gemm<HdmoeBf16, false, 2, 4, 4>(args, "hdmoe_block_linear", s)
-                                      : launch_gemm<HdmoeF16, false, 2, 4, 4>(args, "hdmoe_block_linear", s);
+  if (int rc = fill(what, p, false, args, plan, s)) return rc;
+  if (args.op[0].rows + (long long)args.op[1].rows == 0) return HDMOE_OK;
+  const bool bf16 = p->out_dtype == HDMOE_W_BF16;
+  if (plan.tt > 0) return bf16 ? launch_few<HdmoeBf16, false>(args, plan, what, s) : launch_few<HdmoeF16, false>(args, plan, what, s);
+  return bf16 ? launch_gemm<HdmoeBf16, false, 2, 4, 4>(args, what, s) : launch_gemm<HdmoeF16, false, 2, 4, 4>(args, what, s);
 }
 
 extern "C" int hdmoe_block_swiglu(const hdmoe_block_args* p, hdmoe_stream_t stream) {
+  const char* what = "hdmoe_block_swiglu";
   BlockArgs args;
-  if (int rc = fill("hdmoe_block_swiglu", p, true, args)) return rc;
+  Plan plan;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (int rc = fill(what, p, true, args, plan, s)) return rc;
   if (args.op[0].rows + (long long)args.op[1].rows == 0) return HDMOE_OK;
-  return launch_gemm<HdmoeBf16, true, 2, 4, 4>(args, "hdmoe_block_swiglu", static_cast<hipStream_t>(stream));
+  if (plan.tt > 0)
+    return p->a_dtype == HDMOE_W_F16 ? launch_few<HdmoeF16, true>(args, plan, what, s) : launch_few<HdmoeBf16, true>(args, plan, what, s);
+  return launch_gemm<HdmoeBf16, true, 2, 4, 4>(args, what, s);
 }

@@ -2,6 +2,7 @@
 outputs with torch (device memory and stream plumbing only) and enqueue the HIP
 kernels on torch's current stream. Nothing here computes with torch.
 """
+import contextlib
 import ctypes
 
 import torch
@@ -549,8 +550,17 @@ def moe_ffn(x2d, gate_w, experts, shared, H, Hs, weight_dtype, out=None, workspa
 
 
 # ---- e4m3fn with a scale for each block of 128 -------------------------------------------------------------------
+# (Calls on a few rows run for about as long as their checks take: attributes are read once, and the device is switched only
+# where it is another one.)
 
 BLOCK = 128
+_HERE = contextlib.nullcontext()
+_ACT_CODE = {BF16: W_BF16, F16: _lib.W_F16, FP8: W_E4M3FN}
+
+
+def _on(device):
+    """Context in which `device` is the current one."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _blocks(n):
@@ -559,7 +569,7 @@ def _blocks(n):
 
 def block_scales(rows, K, device):
     """Room for the scales of [rows, K] activations: fp32 [rows, ceil(K / 128)], the scales of one block next to each other."""
-    return torch.empty((_blocks(K), rows), dtype=torch.float32, device=device).t()
+    return torch.empty_strided((rows, _blocks(K)), (1, max(rows, 1)), dtype=torch.float32, device=device)
 
 
 def quant_block_fp8(x):
@@ -570,108 +580,133 @@ def quant_block_fp8(x):
     _need_hip(x, "quant_block_fp8 x")
     K = x.shape[-1]
     rows = x.numel() // K if K > 0 else 0
-    with torch.cuda.device(x.device):
-        q = torch.empty(x.shape, dtype=FP8, device=x.device)
-        s = block_scales(rows, K, x.device)
-        check(lib.hdmoe_quant_block_fp8(W_BF16 if dt == BF16 else _lib.W_F16, ptr(x), rows, K, ptr(q), ptr(s), rows, _stream(x)))
+    dev = x.device
+    with _on(dev):
+        q = torch.empty_like(x, dtype=FP8)
+        s = block_scales(rows, K, dev)
+        check(lib.hdmoe_quant_block_fp8(_ACT_CODE[dt], x.data_ptr(), rows, K, q.data_ptr(), s.data_ptr(), rows, _stream(x)))
     return q, s
 
 
 def _block_rows(a, scale_a, what):
-    """(e4m3fn rows, scales laid out as block_scales) of activations: e4m3fn with their scales, or 16-bit ones, which are cast."""
+    """Checks [rows, K] activations, 16-bit or e4m3fn with scales; the scales laid out as block_scales has them (or None)."""
     if a.dim() != 2:
         raise ValueError(f"{what}: expected [rows, K] activations, got {tuple(a.shape)}")
     if a.dtype != FP8:
+        _act_dtype(a, what)
         if scale_a is not None:
             raise TypeError(f"{what}: scales belong to float8_e4m3fn activations, got {a.dtype}")
-        return quant_block_fp8(a)
-    _need_hip(a, what, FP8)
+        _need_hip(a, what)
+        return None
+    _need_hip(a, what)
     if scale_a is None:
         raise TypeError(f"{what}: float8_e4m3fn activations need their scales")
     rows, K = a.shape
-    if scale_a.device != a.device or scale_a.dtype != torch.float32 or tuple(scale_a.shape) != (rows, _blocks(K)):
+    if scale_a.device != a.device or scale_a.dtype != torch.float32 or scale_a.shape != (rows, _blocks(K)):
         raise ValueError(f"{what}: scales must be float32 [{rows}, {_blocks(K)}] on {a.device}, got {scale_a.dtype} "
                          f"{tuple(scale_a.shape)} on {scale_a.device}")
     if not scale_a.t().is_contiguous():
         scale_a = scale_a.t().contiguous().t()
-    return a, scale_a
+    return scale_a
 
 
 def _block_matrix(weight, scale, K, device, what):
     """N of a weight [N, K] with scales [ceil(N / 128), ceil(K / 128)]."""
-    if weight.dtype != FP8 or weight.device != device or weight.dim() != 2 or weight.shape[1] != K or not weight.is_contiguous():
+    shape = weight.shape
+    if weight.dtype != FP8 or len(shape) != 2 or shape[1] != K or weight.device != device or not weight.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous float8_e4m3fn weight [N, {K}] on {device}, got {weight.dtype} "
-                         f"{tuple(weight.shape)} on {weight.device}")
-    N = weight.shape[0]
-    if (scale.dtype != torch.float32 or scale.device != device or tuple(scale.shape) != (_blocks(N), _blocks(K))
+                         f"{tuple(shape)} on {weight.device}")
+    N = shape[0]
+    if (scale.dtype != torch.float32 or scale.shape != (-(-N // BLOCK), -(-K // BLOCK)) or scale.device != device
             or not scale.is_contiguous()):
         raise ValueError(f"{what}: expected contiguous float32 scales [{_blocks(N)}, {_blocks(K)}] on {device}, got "
                          f"{scale.dtype} {tuple(scale.shape)} on {scale.device}")
     return N
 
 
-def _block_bias(bias, N, dtype, device, what):
-    if bias is not None and (bias.dtype != dtype or bias.device != device or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
-        raise ValueError(f"{what}: expected a contiguous {dtype} bias [{N}] on {device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
-    return bias
-
-
 def _block_weights(entry, K, dtype, device, what):
-    """BlockWeights and N of (weight, scale, bias or None) or, for gate/up (dtype None), (w1, scale1, w3, scale3)."""
+    """(BlockWeights, N) of (weight, scale, bias or None) or, for gate/up (dtype None), (w1, scale1, w3, scale3)."""
     if dtype is None:
         w1, s1, w3, s3 = entry
-        N = _block_matrix(w1, s1, K, device, what + " w1")
-        if _block_matrix(w3, s3, K, device, what + " w3") != N:
+        N = _block_matrix(w1, s1, K, device, what)
+        if _block_matrix(w3, s3, K, device, what) != N:
             raise ValueError(f"{what}: w1 {tuple(w1.shape)} and w3 {tuple(w3.shape)} differ")
-        return _lib.BlockWeights(ptr(w1), ptr(s1), ptr(w3), ptr(s3), None), N
-    w, s, b = entry
+        return _lib.BlockWeights(w1.data_ptr(), s1.data_ptr(), w3.data_ptr(), s3.data_ptr()), N
+    w, s, bias = entry
     N = _block_matrix(w, s, K, device, what)
-    return _lib.BlockWeights(ptr(w), ptr(s), None, None, ptr(_block_bias(b, N, dtype, device, what))), N
+    if bias is None:
+        return _lib.BlockWeights(w.data_ptr(), s.data_ptr()), N
+    if bias.dtype != dtype or bias.device != device or bias.shape != (N,) or not bias.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous {dtype} bias [{N}] on {device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
+    return _lib.BlockWeights(w.data_ptr(), s.data_ptr(), None, None, bias.data_ptr()), N
 
 
 def _block_out_dtype(a, out_dtype, what):
     if out_dtype is None:
         out_dtype = BF16 if a.dtype == FP8 else a.dtype
-    if out_dtype not in ACT_DTYPES:
-        raise TypeError(f"{what}: out_dtype must be bfloat16 or float16, got {out_dtype}")
+    if out_dtype not in ACT_DTYPES or (a.dtype != FP8 and a.dtype != out_dtype):
+        raise TypeError(f"{what}: out_dtype must be bfloat16 or float16, and that of 16-bit activations, got {out_dtype}")
     return out_dtype
 
 
-def _block_segments(a, offsets, experts, perm, what):
-    """Rows of the experts' segments; checks offsets and perm."""
+def _block_experts(a, offsets, experts, perm, dtype, what):
+    """(array of BlockWeights, rows of the segments, N); checks offsets and perm."""
     E = len(experts)
+    T, K = a.shape
+    dev = a.device
     if not 1 <= E <= _lib.BLOCK_MAX_EXPERTS:
         raise ValueError(f"{what}: {E} experts (1 to {_lib.BLOCK_MAX_EXPERTS})")
-    if offsets.dtype != torch.int32 or offsets.device != a.device or tuple(offsets.shape) != (E + 1,) or not offsets.is_contiguous():
-        raise ValueError(f"{what}: offsets must be contiguous int32 [{E + 1}] on {a.device}")
-    if perm is None:
-        return a.shape[0]
-    rows = a.shape[0] * _lib.TOPK
-    if perm.dtype != torch.int32 or perm.device != a.device or tuple(perm.shape) != (rows,) or not perm.is_contiguous():
-        raise ValueError(f"{what}: perm must be contiguous int32 [{rows}] on {a.device}")
-    return rows
+    if offsets.dtype != torch.int32 or offsets.shape != (E + 1,) or offsets.device != dev or not offsets.is_contiguous():
+        raise ValueError(f"{what}: offsets must be contiguous int32 [{E + 1}] on {dev}")
+    rows = T
+    if perm is not None:
+        rows = T * _lib.TOPK
+        if perm.dtype != torch.int32 or perm.shape != (rows,) or perm.device != dev or not perm.is_contiguous():
+            raise ValueError(f"{what}: perm must be contiguous int32 [{rows}] on {dev}")
+    arr = (_lib.BlockWeights * E)()
+    N = None
+    for i, entry in enumerate(experts):
+        arr[i], n = _block_weights(entry, K, dtype, dev, what)
+        if N is None:
+            N = n
+        elif n != N:
+            raise ValueError(f"{what}: the experts' weights differ in size")
+    return arr, rows, N
+
+
+def _block_call(fn, swiglu, args, a):
+    """fn(args) with room for the cast of 16-bit rows where it is needed."""
+    if args.rows == 0 and args.rows_static == 0:
+        return
+    if a.dtype != FP8:
+        nbytes = lib.hdmoe_block_workspace_bytes(swiglu, args.rows, args.E, args.T, args.rows_static, a.shape[1])
+        if nbytes > 0:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    check(fn(ctypes.byref(args), _stream(a)))
 
 
 def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype=None):
     """x [rows, K] times weight [N, K]^T (+ bias [N]): weight float8_e4m3fn with fp32 scales scale_weight
     [ceil(N / 128), ceil(K / 128)]; x bf16 or fp16 (cast as quant_block_fp8 does), or float8_e4m3fn with its scales scale_x
-    [rows, ceil(K / 128)]. -> [rows, N] of x's type (out_dtype, bf16 unless given, for float8_e4m3fn x). K and N are multiples
-    of 16. The sums are fp32; bias joins them before the one rounding."""
+    [rows, ceil(K / 128)] (laid out anew unless they are as quant_block_fp8 returns them). -> [rows, N] of x's type (out_dtype, bf16
+    unless given, for float8_e4m3fn x). K and N are multiples of 16. The sums are fp32; bias joins them before the one rounding."""
     what = "linear_block_fp8"
     dt = _block_out_dtype(x, out_dtype, what)
-    q, s = _block_rows(x, scale_x, what + " x")
-    rows, K = q.shape
-    w, N = _block_weights((weight, scale_weight, bias), K, dt, q.device, what)
-    with torch.cuda.device(q.device):
-        out = torch.empty((rows, N), dtype=dt, device=q.device)
-        if rows == 0:
-            return out
-        args = _lib.BlockArgs()
-        args.out_dtype = W_BF16 if dt == BF16 else _lib.W_F16
-        args.rows_static, args.K_static, args.N_static = rows, K, N
-        args.shared = ctypes.pointer(w)
-        args.fixed = _lib.BlockRows(ptr(q), ptr(s), rows, ptr(out), None, 0)
-        check(lib.hdmoe_block_linear(ctypes.byref(args), _stream(q)))
+    s = _block_rows(x, scale_x, what + " x")
+    rows, K = x.shape
+    dev = x.device
+    w, N = _block_weights((weight, scale_weight, bias), K, dt, dev, what)
+    with _on(dev):
+        out = torch.empty((rows, N), dtype=dt, device=dev)
+        if rows > 0:
+            args = _lib.BlockArgs()
+            args.a_dtype, args.out_dtype = _ACT_CODE[x.dtype], _ACT_CODE[dt]
+            args.rows_static, args.K_static, args.N_static = rows, K, N
+            args.shared = ctypes.pointer(w)
+            fixed = args.fixed
+            fixed.a, fixed.scale_a, fixed.scale_a_stride, fixed.out = x.data_ptr(), ptr(s), rows, out.data_ptr()
+            _block_call(lib.hdmoe_block_linear, 0, args, x)
     return out
 
 
@@ -685,40 +720,41 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
     -> (out, out_static)."""
     what = "grouped_linear_block_fp8"
     dt = _block_out_dtype(a, out_dtype, what)
-    a, sa = _block_rows(a, scale_a, what + " a")
+    if shared is not None and a.dtype != FP8:
+        a, scale_a = quant_block_fp8(a)
+    sa = _block_rows(a, scale_a, what + " a")
     dev = a.device
-    rows = _block_segments(a, offsets, experts, perm, what)
-    K = a.shape[1]
-    packed = [_block_weights(e, K, dt, dev, what) for e in experts]
-    N = packed[0][1]
-    if any(n != N for _, n in packed):
-        raise ValueError(f"{what}: the experts' weights differ in size")
-    with torch.cuda.device(dev):
+    arr, rows, N = _block_experts(a, offsets, experts, perm, dt, what)
+    T, K = a.shape
+    with _on(dev):
         args = _lib.BlockArgs()
-        args.out_dtype = W_BF16 if dt == BF16 else _lib.W_F16
+        args.a_dtype, args.out_dtype = _ACT_CODE[a.dtype], _ACT_CODE[dt]
         out = torch.empty((rows, N), dtype=dt, device=dev)
         if rows > 0:
             args.E, args.rows, args.K, args.N = len(experts), rows, K, N
             if perm is not None:
-                args.perm, args.T = ptr(perm), a.shape[0]
-            args.offsets = ptr(offsets)
-            args.experts = (_lib.BlockWeights * len(experts))(*(w for w, _ in packed))
-            args.routed = _lib.BlockRows(ptr(a), ptr(sa), a.shape[0], ptr(out), None, 0)
+                args.perm, args.T = perm.data_ptr(), T
+            args.offsets = offsets.data_ptr()
+            args.experts = arr
+            r = args.routed
+            r.a, r.scale_a, r.scale_a_stride, r.out = a.data_ptr(), ptr(sa), T, out.data_ptr()
         out_static = None
         if shared is not None:
-            if a_static is None:
-                raise ValueError(f"{what}: shared needs a_static")
-            q, s = _block_rows(a_static, scale_static, what + " a_static")
-            if q.device != dev:
-                raise ValueError(f"{what}: a_static is on {q.device}")
-            n, Ks = q.shape
+            if a_static is None or a_static.device != dev:
+                raise ValueError(f"{what}: shared needs a_static on {dev}")
+            if a_static.dtype != FP8 and scale_static is None:
+                _block_out_dtype(a_static, dt, what + " a_static")
+                a_static, scale_static = quant_block_fp8(a_static)
+            s = _block_rows(a_static, scale_static, what + " a_static")
+            n, Ks = a_static.shape
             w, Ns = _block_weights(shared, Ks, dt, dev, what + " shared")
             out_static = torch.empty((n, Ns), dtype=dt, device=dev)
             if n > 0:
                 args.rows_static, args.K_static, args.N_static = n, Ks, Ns
                 args.shared = ctypes.pointer(w)
-                args.fixed = _lib.BlockRows(ptr(q), ptr(s), n, ptr(out_static), None, 0)
-        check(lib.hdmoe_block_linear(ctypes.byref(args), _stream(a)))
+                f = args.fixed
+                f.a, f.scale_a, f.scale_a_stride, f.out = a_static.data_ptr(), s.data_ptr(), n, out_static.data_ptr()
+        _block_call(lib.hdmoe_block_linear, 0, args, a)
     return out if shared is None else (out, out_static)
 
 
@@ -726,37 +762,36 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
     """First half of every expert's SwiGLU feed-forward, silu(a w1^T) * (a w3^T), cast as quant_block_fp8 does:
     experts: list of (w1 [H, K], scale1, w3 [H, K], scale3); a, scale_a, offsets, perm as in grouped_linear_block_fp8.
     -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]); everything before the cast is fp32.
-    shared: one more (w1, scale1, w3, scale3) over all rows of a, with a width of its own, in the same launch;
+    shared: one more (w1, scale1, w3, scale3) over all rows of a, with a width of its own, in the same launch (with perm);
     -> (h, scales, h_shared, scales_shared)."""
     what = "grouped_swiglu_block_fp8"
-    a, sa = _block_rows(a, scale_a, what + " a")
+    sa = _block_rows(a, scale_a, what + " a")
     dev = a.device
-    rows = _block_segments(a, offsets, experts, perm, what)
-    n, K = a.shape
-    packed = [_block_weights(e, K, None, dev, what) for e in experts]
-    H = packed[0][1]
-    if any(h != H for _, h in packed):
-        raise ValueError(f"{what}: the experts' weights differ in size")
-    with torch.cuda.device(dev):
+    arr, rows, H = _block_experts(a, offsets, experts, perm, None, what)
+    T, K = a.shape
+    with _on(dev):
         args = _lib.BlockArgs()
-        args.out_dtype = W_BF16
+        args.a_dtype, args.out_dtype = _ACT_CODE[a.dtype], W_BF16
         h = torch.empty((rows, H), dtype=FP8, device=dev)
         sh = block_scales(rows, H, dev)
-        h_shared = sh_shared = None
         if rows > 0:
             args.E, args.rows, args.K, args.N = len(experts), rows, K, H
             if perm is not None:
-                args.perm, args.T = ptr(perm), n
-            args.offsets = ptr(offsets)
-            args.experts = (_lib.BlockWeights * len(experts))(*(w for w, _ in packed))
-            args.routed = _lib.BlockRows(ptr(a), ptr(sa), n, ptr(h), ptr(sh), rows)
+                args.perm, args.T = perm.data_ptr(), T
+            args.offsets = offsets.data_ptr()
+            args.experts = arr
+            r = args.routed
+            r.a, r.scale_a, r.scale_a_stride, r.out = a.data_ptr(), ptr(sa), T, h.data_ptr()
+            r.scale_out, r.scale_out_stride = sh.data_ptr(), rows
         if shared is not None:
             w, Hs = _block_weights(shared, K, None, dev, what + " shared")
-            h_shared = torch.empty((n, Hs), dtype=FP8, device=dev)
-            sh_shared = block_scales(n, Hs, dev)
-            if n > 0:
-                args.rows_static, args.K_static, args.N_static = n, K, Hs
+            h_shared = torch.empty((T, Hs), dtype=FP8, device=dev)
+            sh_shared = block_scales(T, Hs, dev)
+            if T > 0:
+                args.rows_static, args.K_static, args.N_static = T, K, Hs
                 args.shared = ctypes.pointer(w)
-                args.fixed = _lib.BlockRows(ptr(a), ptr(sa), n, ptr(h_shared), ptr(sh_shared), n)
-        check(lib.hdmoe_block_swiglu(ctypes.byref(args), _stream(a)))
+                f = args.fixed
+                f.a, f.scale_a, f.scale_a_stride, f.out = a.data_ptr(), ptr(sa), T, h_shared.data_ptr()
+                f.scale_out, f.scale_out_stride = sh_shared.data_ptr(), T
+        _block_call(lib.hdmoe_block_swiglu, 1, args, a)
     return (h, sh) if shared is None else (h, sh, h_shared, sh_shared)

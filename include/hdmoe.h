@@ -390,8 +390,8 @@ typedef struct hdmoe_block_weights {
   const void* bias;     /* [N] of out_dtype or NULL (not read by gate/up) */
 } hdmoe_block_weights;
 typedef struct hdmoe_block_rows {
-  const void* a;            /* e4m3fn [rows,K] */
-  const float* scale_a;     /* of block b of row r at scale_a[b * scale_a_stride + r] */
+  const void* a;            /* [rows,K] of a_dtype */
+  const float* scale_a;     /* e4m3fn a: the scale of block b of row r at scale_a[b * scale_a_stride + r] */
   int64_t scale_a_stride;
   void* out;                /* [rows,N] of out_dtype; gate/up: e4m3fn [rows,N] */
   float* scale_out;         /* gate/up: of block b of row r at scale_out[b * scale_out_stride + r] */
@@ -402,7 +402,8 @@ typedef struct hdmoe_block_rows {
  * 0 .. rows are cut off); rows in no segment are left as they were. perm (NULL = the rows are in segment order): sorted row r is
  * row perm[r] / 2 of routed.a [T,K] and its scales. All matrices start on 16 bytes; K % 16 == 0, N % 16 == 0. */
 typedef struct hdmoe_block_args {
-  int out_dtype;      /* HDMOE_W_BF16 or HDMOE_W_F16 (hdmoe_block_linear: output and bias) */
+  int a_dtype;        /* HDMOE_W_E4M3FN with scales, or HDMOE_W_BF16 / HDMOE_W_F16: the call casts the rows first */
+  int out_dtype;      /* HDMOE_W_BF16 or HDMOE_W_F16 (hdmoe_block_linear: output and bias; 16-bit a: its type) */
   int E;              /* experts, 0 = none, at most HDMOE_BLOCK_MAX_EXPERTS */
   int rows;           /* rows of the segments together (rows of routed.out) */
   int T;              /* rows of routed.a when perm is set (rows == 2 T) */
@@ -413,8 +414,13 @@ typedef struct hdmoe_block_args {
   const int32_t* offsets;             /* [E+1], device */
   const hdmoe_block_weights* experts; /* host array [E] */
   const hdmoe_block_weights* shared;  /* of the static group */
-  hdmoe_block_rows routed, fixed;     /* the experts' rows, the static group's */
+  hdmoe_block_rows routed, fixed;     /* the experts' rows, the static group's (16-bit a: the same rows where both are there) */
+  void* workspace;    /* 16-bit a: hdmoe_block_workspace_bytes(...) bytes, 256-byte aligned (NULL where that is 0) */
+  size_t workspace_bytes;
 } hdmoe_block_args;
+/* Room for the cast rows of 16-bit activations; 0 where the contraction casts them itself (few rows). T: as in the arguments, 0
+ * without a permutation; K: of the rows to be cast. */
+size_t hdmoe_block_workspace_bytes(int swiglu, int rows, int E, int T, int rows_static, int K);
 
 /* out[r, n] = round( sum_b scale_a[r, b] * scale[n / 128, b] * sum_{k in block b} a[r, k] * weight[n, k]  + bias[n] ); the sums over
  * a block are the matrix cores', the one over blocks is fp32, and there is one rounding to out_dtype. */

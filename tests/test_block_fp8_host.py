@@ -37,7 +37,7 @@ def arguments(p, **changes):
     L = lib()
     a = L.BlockArgs()
     w = (L.BlockWeights * 2)(*(L.BlockWeights(p, p, p, p, None) for _ in range(2)))
-    a.out_dtype, a.E, a.rows, a.K, a.N = L.W_BF16, 2, 4, 128, 128
+    a.a_dtype, a.out_dtype, a.E, a.rows, a.K, a.N = L.W_E4M3FN, L.W_BF16, 2, 4, 128, 128
     a.offsets, a.experts = p, w
     a.routed = L.BlockRows(p, p, 4, p, p, 4)
     for k, v in changes.items():
@@ -46,7 +46,7 @@ def arguments(p, **changes):
     return a
 
 
-REFUSED = [dict(out_dtype=1), dict(E=33), dict(E=-1), dict(rows=-1), dict(K=0), dict(K=136), dict(N=0), dict(N=24), dict(E=0),
+REFUSED = [dict(out_dtype=1), dict(a_dtype=3), dict(E=33), dict(E=-1), dict(rows=-1), dict(K=0), dict(K=136), dict(N=0), dict(N=24), dict(E=0),
            dict(rows_static=-1), dict(rows_static=3, K_static=128, N_static=100), dict(perm=4096, T=3), dict(K=2 ** 20, N=2 ** 12),
            dict(N=2 ** 30, K=16)]
 
@@ -90,8 +90,23 @@ def test_contraction_refuses_pointers(which):
         a = arguments(p)
         a.experts[0].weight3 = None
         assert f(ctypes.byref(a), None) == L.E_NULL
+    # 16-bit rows: room for their cast where the contraction does not make it, and the same rows for both groups
+    assert L.lib.hdmoe_block_workspace_bytes(which == "swiglu", 600, 2, 0, 0, 128) == 600 * 128 + 600 * 4
+    many = dict(a_dtype=L.W_BF16, rows=600, routed=L.BlockRows(p, None, 0, p, p, 600))
+    assert f(ctypes.byref(arguments(p, **many)), None) == L.E_WORKSPACE
+    assert f(ctypes.byref(arguments(p, **many, workspace=p + 1, workspace_bytes=1 << 20)), None) == L.E_WORKSPACE
+    a = arguments(p, a_dtype=L.W_BF16, rows_static=4, K_static=128, N_static=128, fixed=L.BlockRows(p + 256, None, 0, p, p, 4))
+    a.shared = ctypes.pointer(a.keep[0])
+    assert f(ctypes.byref(a), None) == L.E_SHAPE
     empty = L.BlockArgs()
+    empty.a_dtype = L.W_E4M3FN
     assert f(ctypes.byref(empty), None) == 0        # nothing to do
+
+
+def test_a_linear_of_16_bit_rows_returns_their_type():
+    L = lib()
+    keep, p = buffers()
+    assert L.lib.hdmoe_block_linear(ctypes.byref(arguments(p, a_dtype=L.W_F16)), None) == L.E_SHAPE
 
 
 def test_struct_layouts_match_what_a_c_compiler_sees(tmp_path):

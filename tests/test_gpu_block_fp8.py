@@ -278,7 +278,8 @@ def test_rows_in_no_segment_are_left_alone():
             off = torch.tensor(bounds, dtype=torch.int32, device="cuda")
             out = torch.full((rows, N), 7.0, dtype=torch.bfloat16, device="cuda")
             args = _lib.BlockArgs()
-            args.out_dtype, args.E, args.rows, args.K, args.N = _lib.W_BF16, E, rows, K, N
+            args.a_dtype, args.out_dtype = _lib.W_E4M3FN, _lib.W_BF16
+            args.E, args.rows, args.K, args.N = E, rows, K, N
             args.offsets = off.data_ptr()
             args.experts = (_lib.BlockWeights * E)(*(_lib.BlockWeights(w.data_ptr(), sw.data_ptr(), None, None, None) for w, sw in ws))
             args.routed = _lib.BlockRows(q.data_ptr(), s.data_ptr(), rows, out.data_ptr(), None, 0)
