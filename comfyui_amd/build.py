@@ -28,7 +28,7 @@ HIPCC_FLAGS = [
 
 def build(verbose=True, extra_flags=()):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    for script in ("gen_gemm4w.py", "gen_swiglu224.py"):   # -> *_asm.inc
+    for script in ("gen_gemm4w.py", "gen_swiglu224.py", "gen_block_fp8.py"):   # -> *_asm.inc
         subprocess.check_call([sys.executable, os.path.join(CSRC, script)])
     objs = []
     procs = []

@@ -1,0 +1,167 @@
+#!/usr/bin/env python3
+"""Writes block_fp8_asm.inc: the K loop of the block-scaled e4m3fn contraction on 256 x 256 tiles (blockscale.hip). Run by the build.
+
+    python comfyui_amd/csrc/gen_block_fp8.py [output file]
+
+Eight waves, two per SIMD; a wave multiplies 128 weight rows (8 MFMA tiles f) with 64 tokens (4 tiles t). A K step is one scale block
+of 128: 32 MFMAs (v_mfma_f32_16x16x128_f8f6f4) that start from zero, and behind each the four v_fmac of the MFMA three places before, which
+bring its result into the accumulators with the factor of its tokens and weight block. Left to the compiler each MFMA waits for its own
+result (11 wait states) and every fragment for its read.
+
+Order: pairs of f, and in a pair token tile by token tile, so that every fragment is refilled in place 7 to 9 MFMAs before its next use:
+weights in a ring of four, tokens after the last pair has used them. One barrier a step, in front of MFMA 22: all of this stage has been read
+and all of the next one has landed. Behind it the reads turn to the next stage, the loads of the step after that go out into this one, and
+the factors of the next step are formed.
+
+Register map (per wave):
+  v[128:255]  accumulators, tile (f, t) at 128 + 4 (4 f + t)
+  v[96:127]   token fragments, v[64:95] weight fragments (ring of four)
+  v[48:63]    results of the last four MFMAs
+  v[32:47]    factors: 32 + 8 (step & 1) + 4 (w3) + t
+  v[26:29]    token scales of the next step, v[30:31] its weight scales
+  v[8:25]     addresses (below)
+  v[0:7]      left to the compiler
+"""
+import os
+import sys
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+OUT = os.path.join(HERE, "block_fp8_asm.inc")
+ACC, B, A, P, M, SX, SW = 128, 96, 64, 48, 32, 26, 30
+TAIL, ADDR_T, ADDR_W, TOK, VA, VB = 8, 10, 12, 14, 18, 22
+NF, NT = 8, 4
+STAGE = 32768          # of one operand; tokens at 0, weights at 2 STAGE
+READY = 22             # MFMA in front of which the barrier stands
+BEHIND = 3             # MFMAs between one and its v_fmac
+
+
+def order():
+    return [(2 * p + r % 2, r // 2) for p in range(NF // 2) for r in range(2 * NT)]
+
+
+def quad(r):
+    return f"v[{r}:{r + 3}]"
+
+
+def oct_(r):
+    return f"v[{r}:{r + 7}]"
+
+
+def read_a(f, stage):
+    s = A + 8 * (f % 4)
+    return [f"ds_read_b128 {quad(s + 4 * h)}, v{ADDR_W + h} offset:{stage * STAGE + 2048 * f}" for h in range(2)]
+
+
+def read_b(t, stage):
+    s = B + 8 * t
+    return [f"ds_read_b128 {quad(s + 4 * h)}, v{ADDR_T + h} offset:{stage * STAGE + 2048 * t}" for h in range(2)]
+
+
+# reads at the end of a step, in order: what they fetch of the next stage, behind which MFMA
+NEXT = [(22, "a", 0), (23, "a", 1), (25, "b", 0), (27, "b", 1), (29, "b", 2), (30, "a", 2), (31, "a", 3), (31, "b", 3)]
+OWN = [(6, "a", 4), (7, "a", 5), (14, "a", 6), (15, "a", 7)]
+
+
+def reads_at(q, stage):
+    out = []
+    for at, kind, i in OWN:
+        if at == q:
+            out.append((kind, i, read_a(i, stage)))
+    for at, kind, i in NEXT:
+        if at == q:
+            out.append((kind, i, (read_a if kind == "a" else read_b)(i, stage ^ 1)))
+    return out
+
+
+def fmac(q, parity, swiglu):
+    """Of the MFMA at place q of a step with this parity of the factors."""
+    f, t = order()[q]
+    m = M + 8 * parity + (4 if swiglu and f >= 4 else 0) + t
+    p, a = P + 4 * (q % 4), ACC + 4 * (NT * f + t)
+    return [f"v_fmac_f32 v{a + i}, v{p + i}, v{m}" for i in range(4)]
+
+
+def step(stage, swiglu):
+    """One K step out of `stage`; its number has the stage's parity."""
+    L = []
+    # reads in flight at the start, oldest first
+    flight = [(k, i) for _, k, i in NEXT]
+    loads = []
+    for j in range(4):
+        loads.append((f"s_add_u32 m0, %[ldsw], {stage * STAGE + 8192 * j}", f"buffer_load_dwordx4 v{VA + j}, %[ra], %[so] offen lds"))
+        rb = "%[rb1]" if swiglu and j & 1 else "%[rb0]"
+        loads.append((f"s_add_u32 m0, %[ldsw], {2 * STAGE + stage * STAGE + 8192 * j}", f"buffer_load_dwordx4 v{VB + j}, {rb}, %[so] offen lds"))
+    load_at = dict(zip(range(READY + 1, READY + 9), loads))
+    muls = [f"v_mul_f32 v{M + 8 * (stage ^ 1) + 4 * w + t}, v{SX + t}, v{SW + w}" for w in range(2 if swiglu else 1) for t in range(NT)]
+    scale = [f"buffer_load_dword v{SX + t}, v{TOK + t}, %[rs], %[ss] offen" for t in range(NT)]
+    scale += [f"buffer_load_dword v{SW + w}, off, %[rw{w}], %[sw]" for w in range(2 if swiglu else 1)]
+    for q, (f, t) in enumerate(order()):
+        need = [("a", f), ("b", t)]
+        if q == READY:
+            L += ["s_waitcnt vmcnt(0) lgkmcnt(0)", "s_barrier"]
+            flight = []
+            # K offsets of the step after the next; past the last one the scales are read again and the rows are none
+            L += ["s_add_u32 %[so], %[so], 128", "s_sub_u32 %[left], %[left], 1", "s_cmp_gt_i32 %[left], 0", "s_cbranch_scc1 %=f".replace("%=", str(50 + stage))]
+            L += [f"v_or_b32 v{r}, v{TAIL}, v{r}" for r in list(range(VA, VA + 4)) + list(range(VB, VB + 4))]
+            L += [f"v_bfrev_b32 v{TAIL}, 1", f"{50 + stage}:", "s_cmp_ge_i32 %[left], 0",
+                  "s_cselect_b32 s60, %[ssi], 0", "s_cselect_b32 s61, 4, 0", "s_add_u32 %[ss], %[ss], s60", "s_add_u32 %[sw], %[sw], s61"]
+        pending = [k for k, x in enumerate(flight) if x in need]
+        if pending:
+            behind = len(flight) - 1 - max(pending)
+            L.append(f"s_waitcnt lgkmcnt({2 * behind})")
+            flight = flight[max(pending) + 1:]
+        if q in load_at:
+            L.append(load_at[q][0])
+        L.append(f"v_mfma_f32_16x16x128_f8f6f4 {quad(P + 4 * (q % 4))}, {oct_(A + 8 * (f % 4))}, {oct_(B + 8 * t)}, 0")
+        if q in load_at:
+            L.append(load_at[q][1])
+        for kind, i, text in reads_at(q, stage):
+            L += text
+            flight.append((kind, i))
+        L += fmac(q - BEHIND, stage, swiglu) if q >= BEHIND else fmac(q - BEHIND + 32, stage ^ 1, swiglu)
+        if q > READY:
+            k = 2 if swiglu else 1
+            L += muls[(q - READY - 1) * k:(q - READY) * k]
+            if q >= READY + 5:
+                L += scale[(q - READY - 5) * 2:(q - READY - 4) * 2]
+    assert len(flight) == len(NEXT) and [(k, i) for k, i in flight] == [(k, i) for _, k, i in NEXT]
+    return L
+
+
+def flush(stage, swiglu):
+    """What the last step has left, behind the wait states between an MFMA and a read of its result."""
+    L = ["s_nop 15"]
+    for q in range(32 - BEHIND, 32):
+        L += fmac(q, stage, swiglu)
+    return L
+
+
+def loop(swiglu):
+    L = ["11:"] + step(0, swiglu) + ["s_sub_u32 %[n], %[n], 1", "s_cmp_eq_u32 %[n], 0", "s_cbranch_scc1 12f"]
+    L += step(1, swiglu) + ["s_sub_u32 %[n], %[n], 1", "s_cmp_lg_u32 %[n], 0", "s_cbranch_scc1 11b"]
+    L += flush(1, swiglu) + ["s_branch 13f", "12:"] + flush(0, swiglu) + ["13:", "s_waitcnt vmcnt(0) lgkmcnt(0)", "s_barrier"]
+    return L
+
+
+def fill():
+    L = []
+    for _, kind, i in NEXT:
+        L += (read_a if kind == "a" else read_b)(i, 0)
+    return L
+
+
+def generate():
+    out = ["// Generated by gen_block_fp8.py; do not edit. See that script for the register map and the schedule.", ""]
+    for name, lines in (("HDMOE_BLOCK_PLAIN", fill() + loop(False)), ("HDMOE_BLOCK_SWIGLU", fill() + loop(True))):
+        out.append(f"#define {name} \\")
+        out.append(" \\\n".join('  "' + ln + '\\n"' for ln in lines))
+        out.append("")
+    return "\n".join(out)
+
+
+if __name__ == "__main__":
+    path = sys.argv[1] if len(sys.argv) > 1 else OUT
+    text = generate()
+    if not os.path.exists(path) or open(path).read() != text:
+        with open(path, "w") as f:
+            f.write(text)
