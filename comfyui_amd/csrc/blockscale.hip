@@ -147,46 +147,35 @@ struct Tiles {
   }
 };
 
+__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
+
 // The end of a tile, for a wave that holds acc(f, tt, i) as laid out below: bias, rounding and stores, or SiLU * mul and the cast.
 template <class Act, bool SWIGLU, int BM, int TT, class Acc>
-__device__ __forceinline__ void store_tile(const Operand& op, const Group& grp, const Tile& t, uint8_t* smem, int wf, int wt, int lane, Acc acc) {
-  const int N = op.N;
-  const int quad = lane >> 4;
+__device__ __forceinline__ void store_tile(const Operand& op, const Group& grp, const Tile& t, uint8_t* exchange, int wf, int wt, int lane, Acc acc) {
+  const int N = op.N, quad = lane >> 4;
+  constexpr int OUTSIDE = (int)0x80000000u;
   if constexpr (!SWIGLU) {
-    const int f0 = t.n0 + wf * BLK + quad * 32;       // the lane's 32 features
-    float bias[32];
+    const int f0 = t.n0 + wf * BLK + quad * 8;        // eight features from f0 + 32 c on
+    // rows of the tile; what lies past its rows or features gets an offset past the buffer and is not written
+    const __amdgpu_buffer_rsrc_t out = make_rsrc(static_cast<uint16_t*>(op.out) + (size_t)t.row0 * N, (uint32_t)t.rows_here * (uint32_t)N * 2u);
+    const __amdgpu_buffer_rsrc_t rbias = make_rsrc(grp.bias, grp.bias != nullptr ? (uint32_t)N * 2u : 0u);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) bias[i] = 0.0f;
-    if (grp.bias != nullptr) {
+    for (int c = 0; c < 4; ++c) {
+      const int f = f0 + c * 32;
+      const u32x4 b = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rbias, f < N ? f * 2 : OUTSIDE, 0, 0));
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (f0 + c * 8 < N) {
-          const u32x4 v = *reinterpret_cast<const u32x4*>(grp.bias + f0 + c * 8);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) { bias[c * 8 + 2 * i] = Act::lo(v[i]); bias[c * 8 + 2 * i + 1] = Act::hi(v[i]); }
-        }
-    }
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-      const int r = wt * TT * 16 + tt * 16 + (lane & 15);
-      if (r >= t.rows_here) continue;
-      uint16_t* out = static_cast<uint16_t*>(op.out) + (size_t)(t.row0 + r) * N + f0;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (f0 + c * 8 >= N) continue;                // N is a multiple of 16
+      for (int tt = 0; tt < TT; ++tt) {
+        const int r = wt * TT * 16 + tt * 16 + (lane & 15);
         u32x4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int f = 2 * c + i / 2, j = i % 2 * 2;
-          v[i] = Act::pack(acc(f, tt, j) + bias[c * 8 + 2 * i], acc(f, tt, j + 1) + bias[c * 8 + 2 * i + 1]);
-        }
-        *reinterpret_cast<u32x4*>(out + c * 8) = v;
+        for (int i = 0; i < 4; ++i) v[i] = Act::pack(acc(2 * c + i / 2, tt, i % 2 * 2) + Act::lo(b[i]), acc(2 * c + i / 2, tt, i % 2 * 2 + 1) + Act::hi(b[i]));
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, v), out, r < t.rows_here && f < N ? (r * N + f) * 2 : OUTSIDE, 0, 0);
       }
     }
   } else {
-    // silu(g) * u in place of g, then the cast of the 128 features: 16 in a lane, 64 in the four lanes of a token, two waves
-    __syncthreads();                                  // LDS is read no more
-    uint32_t* const tops = reinterpret_cast<uint32_t*>(smem);   // [WF][BM]
+    // silu(g) * u, then the cast of the 128 features: 16 in a lane, 64 in the four lanes of a token, two waves. The exponential and
+    // the reciprocal are the hardware's, 1 ulp each beside half an e4m3 step of 2^-4.
+    uint32_t* const tops = reinterpret_cast<uint32_t*>(exchange);   // [WF][BM]
     float h[TT][16];
     uint32_t top[TT];
 #pragma unroll
@@ -196,8 +185,7 @@ __device__ __forceinline__ void store_tile(const Operand& op, const Group& grp, 
       for (int f = 0; f < 4; ++f)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float g = acc(f, tt, i), u = acc(f + 4, tt, i);
-          const float v = g / (1.0f + __expf(-g)) * u;
+          const float v = silu(acc(f, tt, i)) * acc(f + 4, tt, i);
           h[tt][f * 4 + i] = v;
           top[tt] = max(top[tt], __float_as_uint(v) & 0x7fffffffu);
         }
@@ -205,29 +193,30 @@ __device__ __forceinline__ void store_tile(const Operand& op, const Group& grp, 
       top[tt] = max(top[tt], (uint32_t)__shfl_xor((int)top[tt], 32, 64));
       if (quad == 0) tops[wf * BM + wt * TT * 16 + tt * 16 + lane] = top[tt];
     }
-    __syncthreads();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
     const int f0 = t.n0 + wf * 64 + quad * 16;
+    const __amdgpu_buffer_rsrc_t out = make_rsrc(static_cast<uint8_t*>(op.out) + (size_t)t.row0 * N, (uint32_t)t.rows_here * (uint32_t)N);
+    const __amdgpu_buffer_rsrc_t outs = make_rsrc(op.s_out + (size_t)(t.n0 / BLK) * op.ld_out + t.row0, (uint32_t)t.rows_here * 4u);
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
       const int r = wt * TT * 16 + tt * 16 + (lane & 15);
       const float both = __uint_as_float(max(top[tt], tops[(1 - wf) * BM + r]));
       const float tp = both < TOP_FLOOR ? TOP_FLOOR : both;
       const float m = 448.0f / tp;
-      if (r >= t.rows_here) continue;
-      if (wf == 0 && quad == 0) op.s_out[(size_t)(t.n0 / BLK) * op.ld_out + t.row0 + r] = tp / 448.0f;
-      if (f0 >= N) continue;
-      u32x4 v;
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(tp / 448.0f), outs, r < t.rows_here && wf == 0 && quad == 0 ? r * 4 : OUTSIDE, 0, 0);
+      v4i v;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        v[i] = hdmoe_dev_pack4_e4m3fn(h[tt][4 * i] * m, h[tt][4 * i + 1] * m, h[tt][4 * i + 2] * m, h[tt][4 * i + 3] * m);
-      *reinterpret_cast<u32x4*>(static_cast<uint8_t*>(op.out) + (size_t)(t.row0 + r) * N + f0) = v;
+        v[i] = (int)hdmoe_dev_pack4_e4m3fn(h[tt][4 * i] * m, h[tt][4 * i + 1] * m, h[tt][4 * i + 2] * m, h[tt][4 * i + 3] * m);
+      __builtin_amdgcn_raw_buffer_store_b128(v, out, r < t.rows_here && f0 < N ? r * N + f0 : OUTSIDE, 0, 0);
     }
   }
 }
 
 // WF x WT waves, each FT * 16 = 128 weight rows x TT * 16 tokens in MFMA tiles of 16 x 16 x 128. Weight rows of a wave are features
 // of one weight block (gate/up: 64 of w1 and the same 64 of w3). LDS row 16 ft + r of a wave's weights holds the feature that puts
-// 4 FT consecutive ones (gate/up: 2 FT) in a lane's accumulators: stores of 16 bytes without a transposition.
+// 8 consecutive ones (gate/up: 16) in a lane's accumulators and 32 (64) in the four lanes of a token: stores of 16 bytes, 64 of them
+// next to each other, without a transposition.
 template <class Act, bool SWIGLU, int WF, int WT, int TT>
 __global__ __launch_bounds__(64 * WF * WT) void block_gemm_kernel(const BlockArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)   // (the host pass leaves out stubs of kernels whose lambdas hold arrays of dependent size)
@@ -282,7 +271,7 @@ __global__ __launch_bounds__(64 * WF * WT) void block_gemm_kernel(const BlockArg
   for (int j = 0; j < LB; ++j) {
     const int p = j * ROWS_PER_LOAD + ld_row;         // LDS row of the weight tile
     const int w = p >> 7, ft = (p >> 4) & 7, r = p & 15;
-    const int f = SWIGLU ? w * 64 + (r >> 2) * 16 + (ft & 3) * 4 + (r & 3) : w * 128 + (r >> 2) * 32 + ft * 4 + (r & 3);
+    const int f = SWIGLU ? w * 64 + (r >> 2) * 16 + (ft & 3) * 4 + (r & 3) : w * 128 + (ft >> 1) * 32 + (r >> 2) * 8 + (ft & 1) * 4 + (r & 3);
     vb[j] = f < feats ? f * K + ld_chunk * 16 : OUTSIDE;
   }
   auto issue = [&](int stage, int kb) {
@@ -363,12 +352,20 @@ __global__ __launch_bounds__(64 * WF * WT) void block_gemm_kernel(const BlockArg
     }
   }
 
+  __syncthreads();   // LDS is read no more
   store_tile<Act, SWIGLU, BM, TT>(op, grp, t, smem, wf, wt, lane, [&](int f, int tt, int i) -> float { return acc[f][tt][i]; });
 #endif
 }
 
-// The same tile of 256 x 256 with the K loop of gen_block_fp8.py, for segments that fill it.
+// The same tile of 256 x 256 with the K loop of gen_block_fp8.py, for segments that fill it; one block of 160 KiB of LDS per CU. The first
+// loads of a block's next tile go out before the end of this one.
 #include "block_fp8_asm.inc"
+// The lane, formed anew: nothing that depends on it has to live across the K loop, which takes nearly all registers.
+__device__ __forceinline__ int lane_now() {
+  int v;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(v));
+  return v;
+}
 #define HDMOE_BLOCK_ACC \
   "+{v[128:143]}"(acc[0]), "+{v[144:159]}"(acc[1]), "+{v[160:175]}"(acc[2]), "+{v[176:191]}"(acc[3]), "+{v[192:207]}"(acc[4]), \
       "+{v[208:223]}"(acc[5]), "+{v[224:239]}"(acc[6]), "+{v[240:255]}"(acc[7])
@@ -377,24 +374,23 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int BM = 256, FEAT = SWIGLU ? 128 : 256, TT = 4;
   constexpr int OUTSIDE = (int)0x80000000u;
-  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // tokens of two stages, weights of two stages, 32 KiB each
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // tokens of two stages, weights of three, 32 KiB each
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wf = wave & 1, wt = wave >> 1;
 
   const Tiles<BM, FEAT> tiles(args, lane);
+  // persistent blocks: those of an XCD take its eighth of the list in turn
   const int per_xcd = (tiles.total + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD;
-  const int slot = blockIdx.x / HDMOE_NUM_XCD;
-  const int L = (int)(blockIdx.x % HDMOE_NUM_XCD) * per_xcd + slot;
-  if (slot >= per_xcd || L >= tiles.total) return;
-  const Tile t = tiles.get(L);
-  const Group& grp = args.g[t.g];
-  const Operand& op = args.op[t.g == args.E ? 1 : 0];
-  const int K = op.K, N = op.N;
-  const int KB = (K + BLK - 1) / BLK;
-  const bool gathers = op.gather != nullptr;
+  const int first = (int)(blockIdx.x % HDMOE_NUM_XCD) * per_xcd, end = min(first + per_xcd, tiles.total);
+  const int nslots = gridDim.x / HDMOE_NUM_XCD;
+  int L = first + blockIdx.x / HDMOE_NUM_XCD;
+  if (L >= end) return;
 
+  typedef int v16i __attribute__((ext_vector_type(16)));
+  typedef int v32i __attribute__((ext_vector_type(32)));
+  typedef float v16f __attribute__((ext_vector_type(16)));
   auto sgpr = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   auto rsrc = [&](const void* p, uint32_t bytes) -> v4i {
     const uint64_t a = reinterpret_cast<uint64_t>(p);
@@ -403,98 +399,126 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
   auto buffer = [](const v4i& r) {
     return make_rsrc(reinterpret_cast<const void*>((uint64_t)(uint32_t)r.y << 32 | (uint32_t)r.x), (uint32_t)r.z);
   };
-  const int feats = min(N - t.n0, FEAT);
-  const int nblk = SWIGLU ? t.n0 / BLK : min(t.n0 / BLK + wf, (N - 1) / BLK);
-  const v4i ra = gathers ? rsrc(op.a, (uint32_t)op.a_rows * (uint32_t)K) : rsrc(op.a + (size_t)t.row0 * K, (uint32_t)t.rows_here * (uint32_t)K);
-  const v4i rb0 = rsrc(grp.w0 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K);
-  const v4i rb1 = SWIGLU ? rsrc(grp.w1 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K) : rb0;
-  const int ld_s = sgpr((int)op.ld_sa * 4);   // bytes between the scales of two blocks of a row
-  const v4i rs = rsrc(op.sa, (uint32_t)(KB - 1) * (uint32_t)ld_s + (uint32_t)op.a_rows * 4u);
-  const v4i rw0 = rsrc(grp.s0 + (size_t)nblk * KB, (uint32_t)KB * 4u);
-  const v4i rw1 = SWIGLU ? rsrc(grp.s1 + (size_t)nblk * KB, (uint32_t)KB * 4u) : rw0;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
 
-  // ctx: v[8:31] of the loop's register map
+  // What the loop is given for a tile, and its first two steps on their way into LDS. ctx0, ctx1: v[8:31] of the register map.
+  struct Source { v4i ra, rb0, rb1, rs, rw0, rw1; int KB, ld_s; };
   v8i c0 = {};
-  typedef int v16i __attribute__((ext_vector_type(16)));
-  typedef int v32i __attribute__((ext_vector_type(32)));
-  typedef float v16f __attribute__((ext_vector_type(16)));
   v16i c1 = {};
-  const int ld_row = wave * 8 + (lane >> 3);
-  const int ld_chunk = (lane & 7) ^ swz(ld_row);
-  const int tail = (KB - 1) * BLK + ld_chunk * 16 < K ? 0 : OUTSIDE;   // of the last block this lane fetches nothing
-  int va[4], vb[4], tok[TT];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = j * 64 + ld_row;
-    va[j] = OUTSIDE;
-    if (r < t.rows_here) {
-      const int from = gathers ? op.gather[t.row0 + r] >> 1 : r;   // a bad index of the permutation reads as a row of zeros
-      if (!gathers || (unsigned)from < (unsigned)op.a_rows) va[j] = from * K + ld_chunk * 16;
-    }
-    const int w = r >> 7, ft = (r >> 4) & 7, i = r & 15;
-    const int f = SWIGLU ? w * 64 + (i >> 2) * 16 + (ft & 3) * 4 + (i & 3) : w * 128 + (i >> 2) * 32 + ft * 4 + (i & 3);
-    vb[j] = f < feats ? f * K + ld_chunk * 16 : OUTSIDE;
-  }
-#pragma unroll
-  for (int tt = 0; tt < TT; ++tt) {
-    const int r = wt * 64 + tt * 16 + (lane & 15);
-    const int from = r < t.rows_here ? (gathers ? op.gather[t.row0 + r] >> 1 : t.row0 + r) : -1;
-    tok[tt] = (unsigned)from < (unsigned)op.a_rows ? from * 4 : OUTSIDE;
-  }
-  // the first two steps
-  const int second = min(1, KB - 1);
-#pragma unroll
-  for (int st = 0; st < 2; ++st) {
-    const int mask = st >= KB ? OUTSIDE : st == KB - 1 ? tail : 0;
-    uint8_t* const sa = smem + st * 32768 + wave * 1024;
+  v16f m = {};
+  auto start = [&](const Tile& t, int lane) -> Source {
+    const Group& grp = args.g[t.g];
+    const Operand& op = args.op[t.g == args.E ? 1 : 0];
+    const int K = op.K, N = op.N;
+    const int32_t* const gather = op.gather;
+    const int a_rows = op.a_rows;
+    const int KB = (K + BLK - 1) / BLK;
+    const int feats = min(N - t.n0, FEAT);
+    const int nblk = SWIGLU ? t.n0 / BLK : min(t.n0 / BLK + wf, (N - 1) / BLK);
+    Source s;
+    s.KB = KB;
+    s.ra = gather != nullptr ? rsrc(op.a, (uint32_t)a_rows * (uint32_t)K) : rsrc(op.a + (size_t)t.row0 * K, (uint32_t)t.rows_here * (uint32_t)K);
+    s.rb0 = rsrc(grp.w0 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K);
+    s.rb1 = SWIGLU ? rsrc(grp.w1 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K) : s.rb0;
+    s.ld_s = sgpr((int)op.ld_sa * 4);   // bytes between the scales of two blocks of a row
+    s.rs = rsrc(op.sa, (uint32_t)(KB - 1) * (uint32_t)s.ld_s + (uint32_t)a_rows * 4u);
+    s.rw0 = rsrc(grp.s0 + (size_t)nblk * KB, (uint32_t)KB * 4u);
+    s.rw1 = SWIGLU ? rsrc(grp.s1 + (size_t)nblk * KB, (uint32_t)KB * 4u) : s.rw0;
+
+    const int ld_row = wave * 8 + (lane >> 3);
+    const int ld_chunk = (lane & 7) ^ swz(ld_row);
+    const int tail = (KB - 1) * BLK + ld_chunk * 16 < K ? 0 : OUTSIDE;   // of the last block this lane fetches nothing
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(ra), (lds_ptr_t)(sa + j * 8192), 16, va[j] | mask, st * BLK, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(SWIGLU && (j & 1) ? rb1 : rb0), (lds_ptr_t)(sa + 65536 + j * 8192), 16, vb[j] | mask, st * BLK, 0, 0);
+      const int r = j * 64 + ld_row;
+      int va = OUTSIDE, tok = OUTSIDE;
+      if (r < t.rows_here) {
+        const int from = gather != nullptr ? gather[t.row0 + r] >> 1 : r;   // a bad index of the permutation reads as a row of zeros
+        if (gather == nullptr || (unsigned)from < (unsigned)a_rows) va = from * K + ld_chunk * 16;
+      }
+      const int w = r >> 7, ft = (r >> 4) & 7, i = r & 15;
+      const int f = SWIGLU ? w * 64 + (i >> 2) * 16 + (ft & 3) * 4 + (i & 3) : w * 128 + (ft >> 1) * 32 + (i >> 2) * 8 + (ft & 1) * 4 + (i & 3);
+      c1[2 + j] = va;
+      c1[6 + j] = f < feats ? f * K + ld_chunk * 16 : OUTSIDE;
+      const int x = wt * 64 + j * 16 + (lane & 15);
+      if (x < t.rows_here) {
+        const int from = gather != nullptr ? gather[t.row0 + x] >> 1 : t.row0 + x;
+        if ((unsigned)from < (unsigned)a_rows) tok = from * 4;
+      }
+      if (j < 2) c0[6 + j] = tok;
+      else c1[j - 2] = tok;
     }
-  }
-  v16f m = {}, p = {};
-  {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const int mask = st >= KB ? OUTSIDE : st == KB - 1 ? tail : 0;
+      uint8_t* const sa = smem + st * 32768 + wave * 1024;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(s.ra), (lds_ptr_t)(sa + j * 8192), 16, c1[2 + j] | mask, st * BLK, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(SWIGLU && (j & 1) ? s.rb1 : s.rb0), (lds_ptr_t)(sa + 65536 + j * 8192), 16, c1[6 + j] | mask, st * BLK, 0, 0);
+      }
+    }
     auto word = [&](const v4i& r, int off, int so) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buffer(r), off, so, 0)); };
-    const float s0 = word(rw0, 0, 0), s1 = SWIGLU ? word(rw1, 0, 0) : 0.0f;
+    const int second = min(1, KB - 1);
+    const float s0 = word(s.rw0, 0, 0), s1 = SWIGLU ? word(s.rw1, 0, 0) : 0.0f;
+    m = v16f{};
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
-      const float sx = word(rs, tok[tt], 0);
+      const int tok = tt < 2 ? c0[6 + tt] : c1[tt - 2];
+      const float sx = word(s.rs, tok, 0);
       m[tt] = sx * s0;
       if (SWIGLU) m[4 + tt] = sx * s1;
-      c1[10 + tt] = __float_as_int(word(rs, tok[tt], second * ld_s));
-      c1[tt + 2] = va[tt];
-      c1[tt + 6] = vb[tt];
+      c1[10 + tt] = __float_as_int(word(s.rs, tok, second * s.ld_s));
     }
-    c1[14] = __float_as_int(word(rw0, 0, second * 4));
-    if (SWIGLU) c1[15] = __float_as_int(word(rw1, 0, second * 4));
-  }
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
-  const int fr = lane & 15, quad = lane >> 4, fs = swz(fr);
-  c0[0] = KB <= 2 ? OUTSIDE : tail;
+    c1[14] = __float_as_int(word(s.rw0, 0, second * 4));
+    c1[15] = SWIGLU ? __float_as_int(word(s.rw1, 0, second * 4)) : 0;
+    const int fr = lane & 15, quad = lane >> 4, fs = swz(fr);
+    c0[0] = KB <= 2 ? OUTSIDE : tail;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int c = ((quad + 4 * h) ^ fs) * 16;
-    c0[2 + h] = (int)lds0 + (wt * 64 + fr) * BLK + c;
-    c0[4 + h] = (int)lds0 + 65536 + (wf * 128 + fr) * BLK + c;
-  }
-  c0[6] = tok[0]; c0[7] = tok[1]; c1[0] = tok[2]; c1[1] = tok[3];
-  v16f acc[8];
-#pragma unroll
-  for (int f = 0; f < 8; ++f) acc[f] = v16f{};
-  int n = sgpr(KB), left = sgpr(KB - 2), so = sgpr(BLK), ss = sgpr(second * ld_s), sw = sgpr(second * 4);
-  const int ldsw = sgpr((int)lds0 + wave * 1024);
-  v32i fa, fb;
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
-#define HDMOE_BLOCK_LOOP(TEXT) \
-  asm volatile(TEXT : HDMOE_BLOCK_ACC, "={v[96:127]}"(fb), "={v[64:95]}"(fa), "+{v[48:63]}"(p), "+{v[32:47]}"(m), "+{v[16:31]}"(c1), "+{v[8:15]}"(c0), \
-                      [n] "+s"(n), [left] "+s"(left), [so] "+s"(so), [ss] "+s"(ss), [sw] "+s"(sw) \
-                    : [ra] "s"(ra), [rb0] "s"(rb0), [rb1] "s"(rb1), [rs] "s"(rs), [rw0] "s"(rw0), [rw1] "s"(rw1), [ssi] "s"(ld_s), [ldsw] "s"(ldsw) \
-                    : "memory", "scc", "s60", "s61")
-  if constexpr (SWIGLU) HDMOE_BLOCK_LOOP(HDMOE_BLOCK_SWIGLU);
-  else HDMOE_BLOCK_LOOP(HDMOE_BLOCK_PLAIN);
+    for (int h = 0; h < 2; ++h) {
+      const int c = ((quad + 4 * h) ^ fs) * 16;
+      c0[2 + h] = (int)lds0 + (wt * 64 + fr) * BLK + c;
+      c0[4 + h] = (int)lds0 + 65536 + (wf * 128 + fr) * BLK + c;
+    }
+    return s;
+  };
 
-  store_tile<Act, SWIGLU, BM, TT>(op, grp, t, smem, wf, wt, lane, [&](int f, int tt, int i) -> float { return acc[f][tt * 4 + i]; });
+  Tile cur = tiles.get(L);
+  Source src = start(cur, lane);
+  const int ldsw = sgpr((int)lds0 + wave * 1024);
+  // between a tile's first loads and its loop: nothing, or the stores of the tile before, which need not have arrived
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
+  for (;;) {
+    v16f acc[8], p = {};
+#pragma unroll
+    for (int f = 0; f < 8; ++f) acc[f] = v16f{};
+    const int second = min(1, src.KB - 1);
+    int n = sgpr(src.KB), left = sgpr(src.KB - 2), so = sgpr(BLK), ss = sgpr(second * src.ld_s), sw = sgpr(second * 4), ws = sgpr(0);
+    v32i fa, fb;
+#define HDMOE_BLOCK_LOOP(TEXT) \
+    asm volatile(TEXT : HDMOE_BLOCK_ACC, "={v[96:127]}"(fb), "={v[64:95]}"(fa), "+{v[48:63]}"(p), "+{v[32:47]}"(m), "+{v[16:31]}"(c1), "+{v[8:15]}"(c0), \
+                        [n] "+s"(n), [left] "+s"(left), [so] "+s"(so), [ss] "+s"(ss), [sw] "+s"(sw), [ws] "+s"(ws) \
+                      : [ra] "s"(src.ra), [rb0] "s"(src.rb0), [rb1] "s"(src.rb1), [rs] "s"(src.rs), [rw0] "s"(src.rw0), [rw1] "s"(src.rw1), \
+                        [ssi] "s"(src.ld_s), [ldsw] "s"(ldsw) \
+                      : "memory", "scc", "s60", "s61", "s62")
+    if constexpr (SWIGLU) HDMOE_BLOCK_LOOP(HDMOE_BLOCK_SWIGLU);
+    else HDMOE_BLOCK_LOOP(HDMOE_BLOCK_PLAIN);
+
+    const Tile done = cur;
+    L += nslots;
+    const bool more = L < end;
+    if (more) {
+      cur = tiles.get(L);
+      src = start(cur, lane_now());
+    }
+    asm volatile("" : : : "memory");
+    store_tile<Act, SWIGLU, BM, TT>(args.op[done.g == args.E ? 1 : 0], args.g[done.g], done, smem + 131072, wf, wt, lane_now(),
+                                    [&](int f, int tt, int i) -> float { return acc[f][tt * 4 + i]; });
+    if (!more) return;
+    // a tile ends in 16 stores (gate/up: 8); the loads in front of them have come back
+    if constexpr (SWIGLU) asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" : : : "memory");
+    else asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" : : : "memory");
+  }
 #endif
 }
 
@@ -689,7 +713,7 @@ __global__ __launch_bounds__(SWIGLU ? 1024 : 512) void block_stream_kernel(const
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float g = acc[tt][i];
-          acc[tt][i] = g / (1.0f + __expf(-g)) * u[i];
+          acc[tt][i] = silu(g) * u[i];
           top = max(top, __float_as_uint(acc[tt][i]) & 0x7fffffffu);
         }
         top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
@@ -758,10 +782,10 @@ int launch_gemm(const BlockArgs& args, const char* what, hipStream_t stream) {
 template <class Act, bool SWIGLU>
 int launch_gemm8(const BlockArgs& args, const char* what, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  if (int rc = allow_lds(block_gemm8_kernel<Act, SWIGLU>, 131072, done, what)) return rc;
+  if (int rc = allow_lds(block_gemm8_kernel<Act, SWIGLU>, 163840, done, what)) return rc;
   const long long grid = grid_of(args, 256, SWIGLU ? 128 : 256);
   if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
-  block_gemm8_kernel<Act, SWIGLU><<<(unsigned)grid, 512, 131072, stream>>>(args);
+  block_gemm8_kernel<Act, SWIGLU><<<(unsigned)(grid < HDMOE_NUM_CU ? grid : HDMOE_NUM_CU), 512, 163840, stream>>>(args);
   return hdmoe_check_launch(what);
 }
 

@@ -9,9 +9,10 @@ bring its result into the accumulators with the factor of its tokens and weight 
 result (11 wait states) and every fragment for its read.
 
 Order: pairs of f, and in a pair token tile by token tile, so that every fragment is refilled in place 7 to 9 MFMAs before its next use:
-weights in a ring of four, tokens after the last pair has used them. One barrier a step, in front of MFMA 22: all of this stage has been read
-and all of the next one has landed. Behind it the reads turn to the next stage, the loads of the step after that go out into this one, and
-the factors of the next step are formed.
+weights in a ring of four, tokens after the last pair has used them. LDS holds two stages of tokens and three of weights. One barrier a
+step, in front of MFMA 22: all of this stage has been read and all of the next one has landed. Behind it the reads turn to the next stage
+and the token loads of the step after that go out into this one; the weight loads of that step have gone out since MFMA 2, into the stage
+that the step before has left. Loads are spread over the step: a burst of them keeps both waves of a SIMD waiting at the memory queue.
 
 Register map (per wave):
   v[128:255]  accumulators, tile (f, t) at 128 + 4 (4 f + t)
@@ -30,7 +31,9 @@ OUT = os.path.join(HERE, "block_fp8_asm.inc")
 ACC, B, A, P, M, SX, SW = 128, 96, 64, 48, 32, 26, 30
 TAIL, ADDR_T, ADDR_W, TOK, VA, VB = 8, 10, 12, 14, 18, 22
 NF, NT = 8, 4
-STAGE = 32768          # of one operand; tokens at 0, weights at 2 STAGE
+STAGE = 32768          # of one operand; two of tokens at 0, three of weights at 2 STAGE
+LOAD_W = (2, 6, 10, 14)
+LOAD_T = (23, 25, 27, 29)
 READY = 22             # MFMA in front of which the barrier stands
 BEHIND = 3             # MFMAs between one and its v_fmac
 
@@ -49,7 +52,7 @@ def oct_(r):
 
 def read_a(f, stage):
     s = A + 8 * (f % 4)
-    return [f"ds_read_b128 {quad(s + 4 * h)}, v{ADDR_W + h} offset:{stage * STAGE + 2048 * f}" for h in range(2)]
+    return [f"ds_read_b128 {quad(s + 4 * h)}, v{ADDR_W + h} offset:{2048 * f}" for h in range(2)]
 
 
 def read_b(t, stage):
@@ -86,25 +89,31 @@ def step(stage, swiglu):
     L = []
     # reads in flight at the start, oldest first
     flight = [(k, i) for _, k, i in NEXT]
-    loads = []
+    load_at = {}
     for j in range(4):
-        loads.append((f"s_add_u32 m0, %[ldsw], {stage * STAGE + 8192 * j}", f"buffer_load_dwordx4 v{VA + j}, %[ra], %[so] offen lds"))
+        load_at[LOAD_T[j]] = (f"s_add_u32 m0, %[ldsw], {stage * STAGE + 8192 * j}", f"buffer_load_dwordx4 v{VA + j}, %[ra], %[so] offen lds")
         rb = "%[rb1]" if swiglu and j & 1 else "%[rb0]"
-        loads.append((f"s_add_u32 m0, %[ldsw], {2 * STAGE + stage * STAGE + 8192 * j}", f"buffer_load_dwordx4 v{VB + j}, {rb}, %[so] offen lds"))
-    load_at = dict(zip(range(READY + 1, READY + 9), loads))
+        load_at[LOAD_W[j]] = (f"s_add_u32 m0, s62, {8192 * j}", f"buffer_load_dwordx4 v{VB + j}, {rb}, %[so] offen lds")
     muls = [f"v_mul_f32 v{M + 8 * (stage ^ 1) + 4 * w + t}, v{SX + t}, v{SW + w}" for w in range(2 if swiglu else 1) for t in range(NT)]
     scale = [f"buffer_load_dword v{SX + t}, v{TOK + t}, %[rs], %[ss] offen" for t in range(NT)]
     scale += [f"buffer_load_dword v{SW + w}, off, %[rw{w}], %[sw]" for w in range(2 if swiglu else 1)]
     for q, (f, t) in enumerate(order()):
         need = [("a", f), ("b", t)]
-        if q == READY:
-            L += ["s_waitcnt vmcnt(0) lgkmcnt(0)", "s_barrier"]
-            flight = []
+        if q == 0:
             # K offsets of the step after the next; past the last one the scales are read again and the rows are none
-            L += ["s_add_u32 %[so], %[so], 128", "s_sub_u32 %[left], %[left], 1", "s_cmp_gt_i32 %[left], 0", "s_cbranch_scc1 %=f".replace("%=", str(50 + stage))]
+            L += ["s_add_u32 %[so], %[so], 128", "s_sub_u32 %[left], %[left], 1", "s_cmp_gt_i32 %[left], 0", f"s_cbranch_scc1 {50 + stage}f"]
             L += [f"v_or_b32 v{r}, v{TAIL}, v{r}" for r in list(range(VA, VA + 4)) + list(range(VB, VB + 4))]
             L += [f"v_bfrev_b32 v{TAIL}, 1", f"{50 + stage}:", "s_cmp_ge_i32 %[left], 0",
                   "s_cselect_b32 s60, %[ssi], 0", "s_cselect_b32 s61, 4, 0", "s_add_u32 %[ss], %[ss], s60", "s_add_u32 %[sw], %[sw], s61"]
+            # the weights' stage of that step: the one in front of this step's
+            L += [f"s_add_u32 s62, %[ws], {-STAGE}", "s_cmp_eq_u32 %[ws], 0", f"s_cselect_b32 s62, {2 * STAGE}, s62", "s_add_u32 s62, s62, %[ldsw]",
+                  f"s_add_u32 s62, s62, {2 * STAGE}"]
+        if q == READY - 2:
+            L += [f"s_mov_b32 s60, {STAGE}", f"s_cmp_eq_u32 %[ws], {2 * STAGE}", f"s_cselect_b32 s60, {-2 * STAGE}, s60", "s_add_u32 %[ws], %[ws], s60"]
+            L += [f"v_add_u32 v{ADDR_W + h}, s60, v{ADDR_W + h}" for h in range(2)]
+        if q == READY:
+            L += ["s_waitcnt vmcnt(4) lgkmcnt(0)", "s_barrier"]   # (the weights of the step after the next are on their way)
+            flight = []
         pending = [k for k, x in enumerate(flight) if x in need]
         if pending:
             behind = len(flight) - 1 - max(pending)
