@@ -150,19 +150,33 @@ struct Tiles {
 __device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
 // The end of a tile, for a wave that holds acc(f, tt, i) as laid out below: bias, rounding and stores, or SiLU * mul and the cast.
+struct BiasWords { u32x4 w[4]; };   // of the lane's 32 features
+__device__ __forceinline__ BiasWords load_bias(const Operand& op, const Group& grp, const Tile& t, int wf, int lane) {
+  BiasWords b = {};
+  const uint16_t* const p = grp.bias;
+  if (p != nullptr) {
+    const int f0 = t.n0 + wf * BLK + (lane >> 4) * 8;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (f0 + c * 32 < op.N) b.w[c] = *reinterpret_cast<const u32x4*>(p + f0 + c * 32);   // N is a multiple of 16
+#pragma unroll
+    for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(b.w[c]));   // what waits for them does so here, not where there is no bias
+  }
+  return b;
+}
+
 template <class Act, bool SWIGLU, int BM, int TT, class Acc>
-__device__ __forceinline__ void store_tile(const Operand& op, const Group& grp, const Tile& t, uint8_t* exchange, int wf, int wt, int lane, Acc acc) {
+__device__ __forceinline__ void store_tile(const Operand& op, const BiasWords& bias, const Tile& t, uint8_t* exchange, int wf, int wt, int lane, Acc acc) {
   const int N = op.N, quad = lane >> 4;
   constexpr int OUTSIDE = (int)0x80000000u;
   if constexpr (!SWIGLU) {
     const int f0 = t.n0 + wf * BLK + quad * 8;        // eight features from f0 + 32 c on
     // rows of the tile; what lies past its rows or features gets an offset past the buffer and is not written
     const __amdgpu_buffer_rsrc_t out = make_rsrc(static_cast<uint16_t*>(op.out) + (size_t)t.row0 * N, (uint32_t)t.rows_here * (uint32_t)N * 2u);
-    const __amdgpu_buffer_rsrc_t rbias = make_rsrc(grp.bias, grp.bias != nullptr ? (uint32_t)N * 2u : 0u);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int f = f0 + c * 32;
-      const u32x4 b = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rbias, f < N ? f * 2 : OUTSIDE, 0, 0));
+      const u32x4 b = bias.w[c];
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt) {
         const int r = wt * TT * 16 + tt * 16 + (lane & 15);
@@ -353,7 +367,7 @@ __global__ __launch_bounds__(64 * WF * WT) void block_gemm_kernel(const BlockArg
   }
 
   __syncthreads();   // LDS is read no more
-  store_tile<Act, SWIGLU, BM, TT>(op, grp, t, smem, wf, wt, lane, [&](int f, int tt, int i) -> float { return acc[f][tt][i]; });
+  store_tile<Act, SWIGLU, BM, TT>(op, SWIGLU ? BiasWords{} : load_bias(op, grp, t, wf, lane), t, smem, wf, wt, lane, [&](int f, int tt, int i) -> float { return acc[f][tt][i]; });
 #endif
 }
 
@@ -367,8 +381,8 @@ __device__ __forceinline__ int lane_now() {
   return v;
 }
 #define HDMOE_BLOCK_ACC \
-  "+{v[128:143]}"(acc[0]), "+{v[144:159]}"(acc[1]), "+{v[160:175]}"(acc[2]), "+{v[176:191]}"(acc[3]), "+{v[192:207]}"(acc[4]), \
-      "+{v[208:223]}"(acc[5]), "+{v[224:239]}"(acc[6]), "+{v[240:255]}"(acc[7])
+  "={v[128:143]}"(acc[0]), "={v[144:159]}"(acc[1]), "={v[160:175]}"(acc[2]), "={v[176:191]}"(acc[3]), "={v[192:207]}"(acc[4]), \
+      "={v[208:223]}"(acc[5]), "={v[224:239]}"(acc[6]), "={v[240:255]}"(acc[7])
 template <class Act, bool SWIGLU>
 __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -388,9 +402,9 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
   int L = first + blockIdx.x / HDMOE_NUM_XCD;
   if (L >= end) return;
 
-  typedef int v16i __attribute__((ext_vector_type(16)));
   typedef int v32i __attribute__((ext_vector_type(32)));
   typedef float v16f __attribute__((ext_vector_type(16)));
+  typedef float v8f __attribute__((ext_vector_type(8)));
   auto sgpr = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   auto rsrc = [&](const void* p, uint32_t bytes) -> v4i {
     const uint64_t a = reinterpret_cast<uint64_t>(p);
@@ -401,11 +415,12 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
   };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
 
-  // What the loop is given for a tile, and its first two steps on their way into LDS. ctx0, ctx1: v[8:31] of the register map.
+  // What the loop is given for a tile, and its first two steps on their way into LDS; the registers' names are those of gen_block_fp8.py.
   struct Source { v4i ra, rb0, rb1, rs, rw0, rw1; int KB, ld_s; };
-  v8i c0 = {};
-  v16i c1 = {};
-  v16f m = {};
+  int tail = 0;
+  v4i addr, tok, va, vb;
+  v4f x0, sx;
+  float s0, s1 = 0.0f, sw[2] = {0.0f, 0.0f};
   auto start = [&](const Tile& t, int lane) -> Source {
     const Group& grp = args.g[t.g];
     const Operand& op = args.op[t.g == args.E ? 1 : 0];
@@ -427,58 +442,54 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
 
     const int ld_row = wave * 8 + (lane >> 3);
     const int ld_chunk = (lane & 7) ^ swz(ld_row);
-    const int tail = (KB - 1) * BLK + ld_chunk * 16 < K ? 0 : OUTSIDE;   // of the last block this lane fetches nothing
+    tail = (KB - 1) * BLK + ld_chunk * 16 < K ? 0 : OUTSIDE;   // of the last block this lane fetches nothing
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int r = j * 64 + ld_row;
-      int va = OUTSIDE, tok = OUTSIDE;
+      va[j] = tok[j] = OUTSIDE;
       if (r < t.rows_here) {
         const int from = gather != nullptr ? gather[t.row0 + r] >> 1 : r;   // a bad index of the permutation reads as a row of zeros
-        if (gather == nullptr || (unsigned)from < (unsigned)a_rows) va = from * K + ld_chunk * 16;
+        if (gather == nullptr || (unsigned)from < (unsigned)a_rows) va[j] = from * K + ld_chunk * 16;
       }
       const int w = r >> 7, ft = (r >> 4) & 7, i = r & 15;
       const int f = SWIGLU ? w * 64 + (i >> 2) * 16 + (ft & 3) * 4 + (i & 3) : w * 128 + (ft >> 1) * 32 + (i >> 2) * 8 + (ft & 1) * 4 + (i & 3);
-      c1[2 + j] = va;
-      c1[6 + j] = f < feats ? f * K + ld_chunk * 16 : OUTSIDE;
+      vb[j] = f < feats ? f * K + ld_chunk * 16 : OUTSIDE;
       const int x = wt * 64 + j * 16 + (lane & 15);
       if (x < t.rows_here) {
         const int from = gather != nullptr ? gather[t.row0 + x] >> 1 : t.row0 + x;
-        if ((unsigned)from < (unsigned)a_rows) tok = from * 4;
+        if ((unsigned)from < (unsigned)a_rows) tok[j] = from * 4;
       }
-      if (j < 2) c0[6 + j] = tok;
-      else c1[j - 2] = tok;
     }
+    // the scales first: requests come back in order
+    auto word = [&](const v4i& r, int off, int so) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buffer(r), off, so, 0)); };
+    const int second = min(1, KB - 1);
+    s0 = word(s.rw0, 0, 0);
+    if (SWIGLU) s1 = word(s.rw1, 0, 0);
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      x0[tt] = word(s.rs, tok[tt], 0);
+      sx[tt] = word(s.rs, tok[tt], second * s.ld_s);
+    }
+    sw[0] = word(s.rw0, 0, second * 4);
+    if (SWIGLU) sw[1] = word(s.rw1, 0, second * 4);
+    asm volatile("" : : : "memory");
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const int mask = st >= KB ? OUTSIDE : st == KB - 1 ? tail : 0;
       uint8_t* const sa = smem + st * 32768 + wave * 1024;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(s.ra), (lds_ptr_t)(sa + j * 8192), 16, c1[2 + j] | mask, st * BLK, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(SWIGLU && (j & 1) ? s.rb1 : s.rb0), (lds_ptr_t)(sa + 65536 + j * 8192), 16, c1[6 + j] | mask, st * BLK, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(s.ra), (lds_ptr_t)(sa + j * 8192), 16, va[j] | mask, st * BLK, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(SWIGLU && (j & 1) ? s.rb1 : s.rb0), (lds_ptr_t)(sa + 65536 + j * 8192), 16, vb[j] | mask, st * BLK, 0, 0);
       }
     }
-    auto word = [&](const v4i& r, int off, int so) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(buffer(r), off, so, 0)); };
-    const int second = min(1, KB - 1);
-    const float s0 = word(s.rw0, 0, 0), s1 = SWIGLU ? word(s.rw1, 0, 0) : 0.0f;
-    m = v16f{};
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-      const int tok = tt < 2 ? c0[6 + tt] : c1[tt - 2];
-      const float sx = word(s.rs, tok, 0);
-      m[tt] = sx * s0;
-      if (SWIGLU) m[4 + tt] = sx * s1;
-      c1[10 + tt] = __float_as_int(word(s.rs, tok, second * s.ld_s));
-    }
-    c1[14] = __float_as_int(word(s.rw0, 0, second * 4));
-    c1[15] = SWIGLU ? __float_as_int(word(s.rw1, 0, second * 4)) : 0;
     const int fr = lane & 15, quad = lane >> 4, fs = swz(fr);
-    c0[0] = KB <= 2 ? OUTSIDE : tail;
+    if (KB <= 2) tail = OUTSIDE;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = ((quad + 4 * h) ^ fs) * 16;
-      c0[2 + h] = (int)lds0 + (wt * 64 + fr) * BLK + c;
-      c0[4 + h] = (int)lds0 + 65536 + (wf * 128 + fr) * BLK + c;
+      addr[h] = (int)lds0 + (wt * 64 + fr) * BLK + c;
+      addr[2 + h] = (int)lds0 + 65536 + (wf * 128 + fr) * BLK + c;
     }
     return s;
   };
@@ -489,17 +500,26 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
   // between a tile's first loads and its loop: nothing, or the stores of the tile before, which need not have arrived
   asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
   for (;;) {
-    v16f acc[8], p = {};
+    // the first step's factors; not before the end of the tile before, which would wait for all of the loads above
+    asm volatile("" : "+v"(x0), "+v"(s0), "+v"(s1));
+    v4f m0, m1 = {};
 #pragma unroll
-    for (int f = 0; f < 8; ++f) acc[f] = v16f{};
+    for (int tt = 0; tt < TT; ++tt) {
+      m0[tt] = x0[tt] * s0;
+      if (SWIGLU) m1[tt] = x0[tt] * s1;
+    }
+    v16f acc[8];
     const int second = min(1, src.KB - 1);
-    int n = sgpr(src.KB), left = sgpr(src.KB - 2), so = sgpr(BLK), ss = sgpr(second * src.ld_s), sw = sgpr(second * 4), ws = sgpr(0);
+    int n = sgpr(src.KB), left = sgpr(src.KB - 2), so = sgpr(BLK), ss = sgpr(second * src.ld_s), so_w = sgpr(second * 4), ws = sgpr(0);
     v32i fa, fb;
+    v8f last;
+    v16f p;
 #define HDMOE_BLOCK_LOOP(TEXT) \
-    asm volatile(TEXT : HDMOE_BLOCK_ACC, "={v[96:127]}"(fb), "={v[64:95]}"(fa), "+{v[48:63]}"(p), "+{v[32:47]}"(m), "+{v[16:31]}"(c1), "+{v[8:15]}"(c0), \
-                        [n] "+s"(n), [left] "+s"(left), [so] "+s"(so), [ss] "+s"(ss), [sw] "+s"(sw), [ws] "+s"(ws) \
-                      : [ra] "s"(src.ra), [rb0] "s"(src.rb0), [rb1] "s"(src.rb1), [rs] "s"(src.rs), [rw0] "s"(src.rw0), [rw1] "s"(src.rw1), \
-                        [ssi] "s"(src.ld_s), [ldsw] "s"(ldsw) \
+    asm volatile(TEXT : HDMOE_BLOCK_ACC, "={v[96:127]}"(fb), "={v[64:95]}"(fa), "={v[48:63]}"(p), "={v[40:47]}"(last), "+{v[32:35]}"(m0), "+{v[36:39]}"(m1), \
+                        "+{v[26:29]}"(sx), "+{v30}"(sw[0]), "+{v31}"(sw[1]), "+{v8}"(tail), "+{v[10:13]}"(addr), "+{v[18:21]}"(va), "+{v[22:25]}"(vb), \
+                        [n] "+s"(n), [left] "+s"(left), [so] "+s"(so), [ss] "+s"(ss), [sw] "+s"(so_w), [ws] "+s"(ws) \
+                      : "{v[14:17]}"(tok), [ra] "s"(src.ra), [rb0] "s"(src.rb0), [rb1] "s"(src.rb1), [rs] "s"(src.rs), [rw0] "s"(src.rw0), [rw1] "s"(src.rw1), \
+                        [ssi] "s"(src.ld_s), [ldsw] "s"(ldsw), [steps] "s"(src.KB) \
                       : "memory", "scc", "s60", "s61", "s62")
     if constexpr (SWIGLU) HDMOE_BLOCK_LOOP(HDMOE_BLOCK_SWIGLU);
     else HDMOE_BLOCK_LOOP(HDMOE_BLOCK_PLAIN);
@@ -512,7 +532,9 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
       src = start(cur, lane_now());
     }
     asm volatile("" : : : "memory");
-    store_tile<Act, SWIGLU, BM, TT>(args.op[done.g == args.E ? 1 : 0], args.g[done.g], done, smem + 131072, wf, wt, lane_now(),
+    const Operand& op = args.op[done.g == args.E ? 1 : 0];
+    const BiasWords bias = SWIGLU ? BiasWords{} : load_bias(op, args.g[done.g], done, wf, lane_now());
+    store_tile<Act, SWIGLU, BM, TT>(op, bias, done, smem + 131072, wf, wt, lane_now(),
                                     [&](int f, int tt, int i) -> float { return acc[f][tt * 4 + i]; });
     if (!more) return;
     // a tile ends in 16 stores (gate/up: 8); the loads in front of them have come back

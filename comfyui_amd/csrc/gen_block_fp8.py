@@ -112,7 +112,11 @@ def step(stage, swiglu):
             L += [f"s_mov_b32 s60, {STAGE}", f"s_cmp_eq_u32 %[ws], {2 * STAGE}", f"s_cselect_b32 s60, {-2 * STAGE}, s60", "s_add_u32 %[ws], %[ws], s60"]
             L += [f"v_add_u32 v{ADDR_W + h}, s60, v{ADDR_W + h}" for h in range(2)]
         if q == READY:
-            L += ["s_waitcnt vmcnt(4) lgkmcnt(0)", "s_barrier"]   # (the weights of the step after the next are on their way)
+            # the weights of the step after the next are on their way; a tile's first two steps have landed before it begins, and behind
+            # their loads the stores of the tile before may be
+            if stage == 0:
+                L += ["s_cmp_eq_u32 %[n], %[steps]", "s_cbranch_scc1 52f"]
+            L += ["s_waitcnt vmcnt(4)"] + (["52:"] if stage == 0 else []) + ["s_waitcnt lgkmcnt(0)", "s_barrier"]
             flight = []
         pending = [k for k, x in enumerate(flight) if x in need]
         if pending:
@@ -146,7 +150,9 @@ def flush(stage, swiglu):
 
 
 def loop(swiglu):
-    L = ["11:"] + step(0, swiglu) + ["s_sub_u32 %[n], %[n], 1", "s_cmp_eq_u32 %[n], 0", "s_cbranch_scc1 12f"]
+    # the results of the last step's MFMAs that the first step takes for joined, and their factors, are zero
+    L = [f"v_mov_b32 v{r}, 0" for r in list(range(M + 8, M + 16)) + list(range(P, P + 16)) + list(range(ACC, 256))]
+    L += ["11:"] + step(0, swiglu) + ["s_sub_u32 %[n], %[n], 1", "s_cmp_eq_u32 %[n], 0", "s_cbranch_scc1 12f"]
     L += step(1, swiglu) + ["s_sub_u32 %[n], %[n], 1", "s_cmp_lg_u32 %[n], 0", "s_cbranch_scc1 11b"]
     L += flush(1, swiglu) + ["s_branch 13f", "12:"] + flush(0, swiglu) + ["13:", "s_waitcnt vmcnt(0) lgkmcnt(0)", "s_barrier"]
     return L
