@@ -9,6 +9,7 @@
 // fp32 once. 2^-96 keeps both quotients normal numbers. The maximum is taken on the bit patterns, where NaN orders above every
 // number: a block that holds NaN becomes NaN, as does one that holds an infinity (0 * inf).
 #include <atomic>
+#include <type_traits>
 
 #include "common.h"
 #include "numfmt.h"
@@ -546,9 +547,11 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
 
 // ---- few rows -----------------------------------------------------------------------------------------------------
 // Segments of up to a few dozen rows: the weights are read once from memory into registers, no tile of them passes through LDS, and
-// many 16-byte loads are on their way at once. A wave multiplies 16 weight rows (a strip) with TT * 16 tokens.
-//   Linear:  the NW waves of a block share one strip and deal its K blocks out; their sums meet in LDS.
-//   gate/up: 16 waves hold the 8 + 8 strips of w1 and w3 behind one block of the cast output, each over all of K.
+// many 16-byte loads are on their way at once. A wave multiplies FT strips of 16 weight rows with TT * 16 tokens; KW waves deal the K
+// blocks of the same strips out and their sums meet in LDS.
+//   Linear:  8 waves, all of them along K, on FT strips. More strips read the activations less often (they come out of L2, 16 TT rows
+//            for every 16 FT of the weights), fewer make more blocks.
+//   gate/up: 4 pairs of waves, each pair on 2 strips of w1 and the same 2 of w3, together one block of the cast output.
 // CAST: the activations are 16-bit rows; the block casts its own into LDS (rows of K + 16 bytes: 16 rows then hit all banks) while the
 // first weights are on their way, instead of a launch of its own in front.
 template <class Act>
@@ -569,18 +572,24 @@ __device__ __forceinline__ void cast_unit(const uint16_t* x, int k, bool in, uin
   s = top / 448.0f;
 }
 
-template <class Act, bool SWIGLU, int TT, bool CAST>
-__global__ __launch_bounds__(SWIGLU ? 1024 : 512) void block_stream_kernel(const BlockArgs args) {
+template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
+__global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int NW = SWIGLU ? 16 : 8;
+  constexpr int NW = 8;
+  constexpr int KW = SWIGLU ? 2 : 8, SG = NW / KW;
+  static_assert(!SWIGLU || FT == 4, "a pair of waves: two strips of w1, two of w3");
   constexpr int BM = TT * 16;
-  constexpr int FEAT = SWIGLU ? BLK : 16;
-  constexpr int DEPTH = SWIGLU ? (TT == 1 || CAST ? 4 : 2) : (TT == 1 ? 6 : 4);   // K blocks on their way (in registers: 16 waves have 128 each)
+  constexpr int FEAT = SWIGLU ? BLK : 16 * FT;
+  // K blocks on their way: as many as the registers hold
+  constexpr int PER = FT * 8 + (CAST ? 0 : TT * 9) + 2, DEPTH_MAX = (220 - 4 * FT * TT) / PER;
+  constexpr int DEPTH = DEPTH_MAX > 6 ? 6 : DEPTH_MAX;
+  static_assert(DEPTH >= 2, "two K blocks at least");
   constexpr int OUTSIDE = (int)0x80000000u;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, quad = lane >> 4;
+  const int kw = wave % KW, sg = wave / KW;
 
   const Tiles<BM, FEAT> tiles(args, lane);
   const int per_xcd = (tiles.total + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD;
@@ -592,16 +601,17 @@ __global__ __launch_bounds__(SWIGLU ? 1024 : 512) void block_stream_kernel(const
   const Operand& op = args.op[t.g == args.E ? 1 : 0];
   const int K = op.K, N = op.N;
   const int KB = (K + BLK - 1) / BLK;
-  const bool gathers = op.gather != nullptr;
+  const int32_t* const gather = op.gather;
+  const int a_rows = op.a_rows;
 
-  // weights: lane = row fr of the strip, 16-byte chunks quad and quad + 4 of a K block
-  const int strip = SWIGLU ? wave & 7 : 0;
-  const bool third = SWIGLU && wave >= 8;
-  const uint8_t* const wp = (third ? grp.w1 : grp.w0) + (size_t)(t.n0 + strip * 16) * K;
-  const bool has_strip = t.n0 + strip * 16 < N;            // N is a multiple of 16
-  const __amdgpu_buffer_rsrc_t rw = make_rsrc(has_strip ? wp : nullptr, has_strip ? 16u * (uint32_t)K : 0u);
-  const float* const sw = (third ? grp.s1 : grp.s0) + (size_t)(t.n0 / BLK) * KB;
-  const int kb_first = SWIGLU ? 0 : wave, kb_step = SWIGLU ? 1 : NW;
+  // weights: lane = row fr of a strip, 16-byte chunks quad and quad + 4 of a K block. Strips past N read as zeros.
+  const int strips = SWIGLU ? 2 : FT;                        // of one matrix
+  const int s0 = t.n0 + sg * strips * 16;
+  const int feats = min(max(N - s0, 0), strips * 16);
+  const __amdgpu_buffer_rsrc_t rw0 = make_rsrc(grp.w0 + (size_t)s0 * K, (uint32_t)feats * (uint32_t)K);
+  const __amdgpu_buffer_rsrc_t rw1 = SWIGLU ? make_rsrc(grp.w1 + (size_t)s0 * K, (uint32_t)feats * (uint32_t)K) : rw0;
+  const __amdgpu_buffer_rsrc_t rs0 = make_rsrc(grp.s0 + (size_t)(t.n0 / BLK) * KB, (uint32_t)KB * 4u);
+  const __amdgpu_buffer_rsrc_t rs1 = SWIGLU ? make_rsrc(grp.s1 + (size_t)(t.n0 / BLK) * KB, (uint32_t)KB * 4u) : rs0;
 
   // tokens: column fr of each tile
   int row[TT];
@@ -609,32 +619,40 @@ __global__ __launch_bounds__(SWIGLU ? 1024 : 512) void block_stream_kernel(const
   for (int tt = 0; tt < TT; ++tt) {
     const int r = tt * 16 + fr;
     row[tt] = -1;
-    if (r < t.rows_here) {
-      row[tt] = gathers ? op.gather[t.row0 + r] >> 1 : t.row0 + r;
-      if ((unsigned)row[tt] >= (unsigned)op.a_rows) row[tt] = -1;
-    }
+    if (r < t.rows_here) row[tt] = gather != nullptr ? gather[t.row0 + r] >> 1 : t.row0 + r;
+    if ((unsigned)row[tt] >= (unsigned)a_rows) row[tt] = -1;
   }
 
-  struct Step { v4i w[2]; v4i x[TT][2]; float sw, sx[TT]; };
+  struct Step { v4i w[FT][2]; v4i x[CAST ? 1 : TT][2]; float s0, s1, sx[TT]; };
+  const int wbase = fr * K + quad * 16;
   auto load = [&](Step& st, int kb) {
     const int k = kb * BLK + quad * 16;
-    st.w[0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, k < K ? fr * K + k : OUTSIDE, 0, 0));
-    st.w[1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, k + 64 < K ? fr * K + k + 64 : OUTSIDE, 0, 0));
-    st.sw = kb < KB ? sw[kb] : 0.0f;
+    const bool lo = k < K, hi = k + 64 < K;
+#pragma unroll
+    for (int f = 0; f < FT; ++f) {
+      const __amdgpu_buffer_rsrc_t r = SWIGLU && f >= 2 ? rw1 : rw0;
+      const int off = wbase + (SWIGLU ? f & 1 : f) * 16 * K + kb * BLK;
+      st.w[f][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, lo ? off : OUTSIDE, 0, 0));
+      st.w[f][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, hi ? off + 64 : OUTSIDE, 0, 0));
+    }
+    const int so = kb < KB ? kb * 4 : OUTSIDE;
+    st.s0 = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs0, so, 0, 0));
+    if (SWIGLU) st.s1 = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs1, so, 0, 0));
     if constexpr (!CAST) {
+      // (64-bit addresses: the rows of all segments together may pass 4 GiB)
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt) {
-        const uint8_t* const xr = op.a + (size_t)max(row[tt], 0) * K + k;
-        st.x[tt][0] = st.x[tt][1] = v4i{0, 0, 0, 0};
-        if (row[tt] >= 0 && k < K) st.x[tt][0] = *reinterpret_cast<const v4i*>(xr);
-        if (row[tt] >= 0 && k + 64 < K) st.x[tt][1] = *reinterpret_cast<const v4i*>(xr + 64);
-        st.sx[tt] = row[tt] >= 0 && kb < KB ? op.sa[(size_t)kb * op.ld_sa + row[tt]] : 0.0f;
+        const int r = max(row[tt], 0), kk = min(k, K - 16), kk2 = min(k + 64, K - 16);   // what lies past K meets weights of zero
+        const uint8_t* const xr = op.a + (size_t)r * K;
+        st.x[tt][0] = *reinterpret_cast<const v4i*>(xr + kk);
+        st.x[tt][1] = *reinterpret_cast<const v4i*>(xr + kk2);
+        st.sx[tt] = op.sa[(size_t)min(kb, KB - 1) * op.ld_sa + r];
       }
     }
   };
   Step st[DEPTH];
 #pragma unroll
-  for (int i = 0; i < DEPTH; ++i) load(st[i], kb_first + i * kb_step);
+  for (int i = 0; i < DEPTH; ++i) load(st[i], kw + i * KW);
 
   // [rows][ld_x] cast rows, [KB][rows] scales; a column without a row reads the last one's and is never stored
   const int ld_x = KB * BLK + 16, R = args.lds_rows;
@@ -647,8 +665,8 @@ __global__ __launch_bounds__(SWIGLU ? 1024 : 512) void block_stream_kernel(const
       const int r = u / KB, b = u - r * KB;
       int from = -1;
       if (r < t.rows_here) {
-        from = gathers ? op.gather[t.row0 + r] >> 1 : t.row0 + r;
-        if ((unsigned)from >= (unsigned)op.a_rows) from = -1;
+        from = gather != nullptr ? gather[t.row0 + r] >> 1 : t.row0 + r;
+        if ((unsigned)from >= (unsigned)a_rows) from = -1;
       }
       const int k = b * BLK + (tid & 15) * 8;
       uint32_t o[2];
@@ -657,14 +675,17 @@ __global__ __launch_bounds__(SWIGLU ? 1024 : 512) void block_stream_kernel(const
       *reinterpret_cast<u32x2*>(lx + r * ld_x + k) = u32x2{o[0], o[1]};
       if ((tid & 15) == 0) ls[b * R + r] = from >= 0 ? s : 0.0f;
     }
-    __syncthreads();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");   // (the weights need not have come)
   }
 
-  v4f acc[TT];
+  v4f acc[FT][TT];
 #pragma unroll
-  for (int tt = 0; tt < TT; ++tt) acc[tt] = v4f{0, 0, 0, 0};
+  for (int f = 0; f < FT; ++f)
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) acc[f][tt] = v4f{0, 0, 0, 0};
   auto multiply = [&](const Step& st, int kb) {
-    const v8i fa = {st.w[0].x, st.w[0].y, st.w[0].z, st.w[0].w, st.w[1].x, st.w[1].y, st.w[1].z, st.w[1].w};
+    v8i fb[TT];
+    float m0[TT], m1[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
       v4i x0, x1;
@@ -678,76 +699,92 @@ __global__ __launch_bounds__(SWIGLU ? 1024 : 512) void block_stream_kernel(const
       } else {
         x0 = st.x[tt][0];
         x1 = st.x[tt][1];
-        sx = st.sx[tt];
+        sx = row[tt] >= 0 ? st.sx[tt] : 0.0f;
       }
-      const v8i fb = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-      const v4f p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb, v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-      const float m = sx * st.sw;
+      fb[tt] = v8i{x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+      m0[tt] = sx * st.s0;
+      m1[tt] = SWIGLU ? sx * st.s1 : 0.0f;
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[tt][i] = __builtin_fmaf(p[i], m, acc[tt][i]);
+    for (int f = 0; f < FT; ++f) {
+      const v8i fa = {st.w[f][0].x, st.w[f][0].y, st.w[f][0].z, st.w[f][0].w, st.w[f][1].x, st.w[f][1].y, st.w[f][1].z, st.w[f][1].w};
+      v4f p[TT];
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) p[tt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb[tt], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[f][tt][i] = __builtin_fmaf(p[tt][i], SWIGLU && f >= 2 ? m1[tt] : m0[tt], acc[f][tt][i]);
     }
   };
-  for (int kb0 = kb_first; kb0 < KB; kb0 += DEPTH * kb_step) {
+  for (int kb0 = kw; kb0 < KB; kb0 += DEPTH * KW) {
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) {
-      const int kb = kb0 + i * kb_step;
-      if (kb < KB) multiply(st[i], kb);
-      load(st[i], kb + DEPTH * kb_step);
+      const int kb = kb0 + i * KW;
+      if (kb < KB) {
+        multiply(st[i], kb);
+        if (kb + DEPTH * KW < KB) load(st[i], kb + DEPTH * KW);
+      }
     }
   }
-  __syncthreads();   // the cast rows are read no more
 
-  if constexpr (!SWIGLU) {
-    // the waves' sums, [NW][TT][64] of 16 bytes; then wave w forms token tile w
-    v4f* const parts = reinterpret_cast<v4f*>(smem);
+  // the waves' sums, [KW][strip][token tile][lane] of 16 bytes
+  constexpr int CELLS = SG * FT * TT;
+  v4f* const parts = reinterpret_cast<v4f*>(smem);
+  if (CAST) __syncthreads();   // the cast rows are read no more
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) parts[(wave * TT + tt) * 64 + lane] = acc[tt];
-    __syncthreads();
-    if (wave >= TT) return;
-    v4f y = parts[wave * 64 + lane];
+  for (int f = 0; f < FT; ++f)
 #pragma unroll
-    for (int w = 1; w < NW; ++w) {
-      const v4f v = parts[(w * TT + wave) * 64 + lane];
+    for (int tt = 0; tt < TT; ++tt) parts[((kw * SG + sg) * FT * TT + f * TT + tt) * 64 + lane] = acc[f][tt];
+  __syncthreads();
+  auto total = [&](int cell) {
+    v4f y = parts[cell * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) {
+      const v4f v = parts[(w * CELLS + cell) * 64 + lane];
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] += v[i];
     }
-    const int r = wave * 16 + fr, f = t.n0 + quad * 4;
-    if (r >= t.rows_here) return;
-    if (grp.bias != nullptr) {
-      const u32x2 b = *reinterpret_cast<const u32x2*>(grp.bias + f);
-      y[0] += Act::lo(b.x); y[1] += Act::hi(b.x); y[2] += Act::lo(b.y); y[3] += Act::hi(b.y);
-    }
-    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(op.out) + (size_t)(t.row0 + r) * N + f) = u32x2{Act::pack(y[0], y[1]), Act::pack(y[2], y[3])};
-  } else {
-    // u from the upper eight waves to the lower ones, which form silu(g) * u, its largest value of a token and the cast
-    v4f* const us = reinterpret_cast<v4f*>(smem);                                   // [8][TT][64]
-    uint32_t* const tops = reinterpret_cast<uint32_t*>(smem + 8 * TT * 64 * 16);    // [8][BM]
-    if (third) {
+    return y;
+  };
+
+  if constexpr (!SWIGLU) {
 #pragma unroll
-      for (int tt = 0; tt < TT; ++tt) us[(strip * TT + tt) * 64 + lane] = acc[tt];
-    }
-    __syncthreads();
-    if (!third) {
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt) {
-        const v4f u = us[(strip * TT + tt) * 64 + lane];
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float g = acc[tt][i];
-          acc[tt][i] = silu(g) * u[i];
-          top = max(top, __float_as_uint(acc[tt][i]) & 0x7fffffffu);
-        }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-        if (quad == 0) tops[strip * BM + tt * 16 + fr] = top;
+    for (int c0 = 0; c0 < CELLS; c0 += NW) {
+      const int cell = c0 + wave, f = cell / TT, tt = cell - f * TT;
+      if (cell >= CELLS) break;
+      v4f y = total(cell);
+      const int r = tt * 16 + fr, n = t.n0 + f * 16 + quad * 4;
+      if (r >= t.rows_here || n >= N) continue;
+      if (grp.bias != nullptr) {
+        const u32x2 b = *reinterpret_cast<const u32x2*>(grp.bias + n);
+        y[0] += Act::lo(b.x); y[1] += Act::hi(b.x); y[2] += Act::lo(b.y); y[3] += Act::hi(b.y);
       }
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(op.out) + (size_t)(t.row0 + r) * N + n) = u32x2{Act::pack(y[0], y[1]), Act::pack(y[2], y[3])};
     }
-    __syncthreads();
-    if (third) return;
+  } else {
+    // wave w: strip w of w1 and of w3; silu(g) * u, the largest value of a token over the eight strips, the cast
+    uint32_t* const tops = reinterpret_cast<uint32_t*>(smem + (size_t)KW * CELLS * 1024);   // [8][BM]
+    const int g = (wave >> 1) * FT + (wave & 1);
+    v4f h[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
-      const int r = tt * 16 + fr;
+      h[tt] = total(g * TT + tt);
+      const v4f u = total((g + 2) * TT + tt);
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        h[tt][i] = silu(h[tt][i]) * u[i];
+        top = max(top, __float_as_uint(h[tt][i]) & 0x7fffffffu);
+      }
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+      if (quad == 0) tops[wave * BM + tt * 16 + fr] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+      const int r = tt * 16 + fr, n = t.n0 + wave * 16 + quad * 4;
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = max(top, tops[j * BM + r]);
@@ -756,9 +793,9 @@ __global__ __launch_bounds__(SWIGLU ? 1024 : 512) void block_stream_kernel(const
       const float m = 448.0f / tp;
       if (r >= t.rows_here) continue;
       if (wave == 0 && quad == 0) op.s_out[(size_t)(t.n0 / BLK) * op.ld_out + t.row0 + r] = tp / 448.0f;
-      if (!has_strip) continue;
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(op.out) + (size_t)(t.row0 + r) * N + t.n0 + strip * 16 + quad * 4) =
-          hdmoe_dev_pack4_e4m3fn(acc[tt][0] * m, acc[tt][1] * m, acc[tt][2] * m, acc[tt][3] * m);
+      if (n >= N) continue;
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(op.out) + (size_t)(t.row0 + r) * N + n) =
+          hdmoe_dev_pack4_e4m3fn(h[tt][0] * m, h[tt][1] * m, h[tt][2] * m, h[tt][3] * m);
     }
   }
 #endif
@@ -811,20 +848,20 @@ int launch_gemm8(const BlockArgs& args, const char* what, hipStream_t stream) {
   return hdmoe_check_launch(what);
 }
 
-// LDS of a few-row block: cast rows and their scales, later the exchange between waves
-size_t stream_lds(bool swiglu, int tt, int lds_rows, int K) {
-  const size_t exchange = (size_t)tt * 64 * 16 * 8 + (swiglu ? (size_t)8 * tt * 16 * 4 : 0);
-  const size_t KB = (K + BLK - 1) / BLK;
-  const size_t rows = (size_t)lds_rows * (KB * BLK + 16 + KB * 4);
-  return rows > exchange ? rows : exchange;
-}
+// LDS of a few-row block: cast rows and their scales, then the sums of its waves
+constexpr size_t stream_sums(bool swiglu, int ft, int tt) { return (size_t)8 * ft * tt * 1024 + (swiglu ? (size_t)8 * tt * 16 * 4 : 0); }
 
-template <class Act, bool SWIGLU, int TT, bool CAST>
+template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
 int launch_stream(const BlockArgs& args, const char* what, hipStream_t stream) {
+  constexpr size_t sums = stream_sums(SWIGLU, FT, TT);
+  static std::atomic<uint64_t> done{0};
+  if (sums > 65536)
+    if (int rc = allow_lds(block_stream_kernel<Act, SWIGLU, FT, TT, CAST>, sums, done, what)) return rc;
   const int K = args.op[0].K > args.op[1].K ? args.op[0].K : args.op[1].K;
-  const long long grid = grid_of(args, TT * 16, SWIGLU ? BLK : 16);
+  const size_t KB = (K + BLK - 1) / BLK, rows = CAST ? (size_t)args.lds_rows * (KB * BLK + 16 + KB * 4) : 0;
+  const long long grid = grid_of(args, TT * 16, SWIGLU ? BLK : 16 * FT);
   if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
-  block_stream_kernel<Act, SWIGLU, TT, CAST><<<(unsigned)grid, SWIGLU ? 1024 : 512, stream_lds(SWIGLU, TT, CAST ? args.lds_rows : 0, K), stream>>>(args);
+  block_stream_kernel<Act, SWIGLU, FT, TT, CAST><<<(unsigned)grid, 512, rows > sums ? rows : sums, stream>>>(args);
   return hdmoe_check_launch(what);
 }
 
@@ -866,20 +903,28 @@ extern "C" int hdmoe_quant_block_fp8(int src_dtype, const void* x, int64_t rows,
 
 namespace {
 
-// How a call runs: the few-row kernels on tiles of 16 * tt rows (tt > 0; with the cast inside or not), or the tiles of
-// block_gemm_kernel.
-struct Plan { int tt; bool cast_inside; int lds_rows; };
+// How a call runs: the few-row kernels on tiles of 16 * tt rows and 16 * ft features (tt > 0; with the cast inside or not), or the tiles
+// of block_gemm8_kernel.
+struct Plan { int tt, ft; bool cast_inside; int lds_rows; };
 
-Plan plan_of(bool swiglu, bool x16, int rows, int E, int rows_static, int K) {
-  Plan p = {0, false, 0};
+Plan plan_of(bool swiglu, bool x16, int rows, int E, int rows_static, int K, int N) {
+  Plan p = {0, 0, false, 0};
   const int per = E > 0 ? (rows + E - 1) / E : 0, most = per > rows_static ? per : rows_static;   // rows of a segment, if they are even
   if (most <= 16) p.tt = 1;
   else if (most <= 32) p.tt = 2;
-  if (p.tt > 0 && x16) {
+  else if (most <= 64) p.tt = 4;
+  if (p.tt == 0) return p;
+  if (x16) {
     // a block casts for itself where that takes its threads a few trips at most
     const int whole = rows > rows_static ? rows : rows_static;
-    p.lds_rows = whole < 16 * p.tt ? whole : 16 * p.tt;
-    p.cast_inside = (long long)p.lds_rows * ((K + BLK - 1) / BLK) * 16 <= 4 * (swiglu ? 1024 : 512);
+    p.lds_rows = whole < 16 ? whole : 16;
+    p.cast_inside = p.tt == 1 && (long long)p.lds_rows * ((K + BLK - 1) / BLK) * 16 <= 4 * 512;
+  }
+  p.ft = 4;
+  if (!swiglu) {
+    // as many features as leave every CU a block
+    const long long strips = (long long)((E > 0 ? (E < rows ? E : rows) : 0) + (rows_static > 0 ? 1 : 0)) * (N / 16);
+    while (p.ft > 1 && strips < (long long)HDMOE_NUM_CU * p.ft) p.ft >>= 1;
   }
   return p;
 }
@@ -955,7 +1000,7 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
   const int a_rows = routed ? args.op[0].a_rows : p->rows_static, K = routed ? p->K : p->K_static;
   if (x16 && routed && p->rows_static > 0 && (p->fixed.a != p->routed.a || p->rows_static != a_rows || p->K_static != K))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: 16-bit activations of the experts and of the static group must be the same rows", what);
-  plan = plan_of(swiglu, x16, routed ? p->rows : 0, routed ? p->E : 0, p->rows_static, K);
+  plan = plan_of(swiglu, x16, routed ? p->rows : 0, routed ? p->E : 0, p->rows_static, K, routed ? p->N : p->N_static);
   args.lds_rows = plan.lds_rows;
   if (a_rows > 0 && x16 && !plan.cast_inside) {
     if (p->workspace == nullptr || p->workspace_bytes < cast_bytes(a_rows, K) || (reinterpret_cast<uintptr_t>(p->workspace) & 255))
@@ -972,17 +1017,28 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
   return HDMOE_OK;
 }
 
+template <class Act, bool SWIGLU, int FT>
+int launch_strips(const BlockArgs& args, const Plan& plan, const char* what, hipStream_t s) {
+  if (plan.cast_inside) return launch_stream<Act, SWIGLU, FT, 1, true>(args, what, s);
+  using Out = std::conditional_t<SWIGLU, HdmoeBf16, Act>;   // (gate/up: the type of what is cast, not looked at here)
+  if (plan.tt == 1) return launch_stream<Out, SWIGLU, FT, 1, false>(args, what, s);
+  return plan.tt == 2 ? launch_stream<Out, SWIGLU, FT, 2, false>(args, what, s) : launch_stream<Out, SWIGLU, FT, 4, false>(args, what, s);
+}
+
 template <class Act, bool SWIGLU>
 int launch_few(const BlockArgs& args, const Plan& plan, const char* what, hipStream_t s) {
-  if (plan.cast_inside) return plan.tt == 1 ? launch_stream<Act, SWIGLU, 1, true>(args, what, s) : launch_stream<Act, SWIGLU, 2, true>(args, what, s);
-  return plan.tt == 1 ? launch_stream<Act, SWIGLU, 1, false>(args, what, s) : launch_stream<Act, SWIGLU, 2, false>(args, what, s);
+  if constexpr (!SWIGLU) {
+    if (plan.ft == 1) return launch_strips<Act, false, 1>(args, plan, what, s);
+    if (plan.ft == 2) return launch_strips<Act, false, 2>(args, plan, what, s);
+  }
+  return launch_strips<Act, SWIGLU, 4>(args, plan, what, s);
 }
 
 }  // namespace
 
 extern "C" size_t hdmoe_block_workspace_bytes(int swiglu, int rows, int E, int T, int rows_static, int K) {
   if (rows < 0 || E < 0 || T < 0 || rows_static < 0 || K <= 0) return 0;
-  return plan_of(swiglu != 0, true, rows, E, rows_static, K).cast_inside ? 0 : cast_bytes(rows > 0 ? (T > 0 ? T : rows) : rows_static, K);
+  return plan_of(swiglu != 0, true, rows, E, rows_static, K, 16).cast_inside ? 0 : cast_bytes(rows > 0 ? (T > 0 ? T : rows) : rows_static, K);
 }
 
 extern "C" int hdmoe_block_linear(const hdmoe_block_args* p, hdmoe_stream_t stream) {
