@@ -175,7 +175,7 @@ SIGNATURES = {
     "hdmoe_ffn_swiglu": (c_int, [c_int, c_void_p, c_int, c_int, c_int, ctypes.POINTER(FfnWeights), c_void_p, c_void_p,
                                  c_size_t, c_void_p]),
     "hdmoe_quant_block_fp8": (c_int, [c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
-    "hdmoe_block_workspace_bytes": (c_size_t, [c_int] * 6),
+    "hdmoe_block_workspace_bytes": (c_size_t, [ctypes.POINTER(BlockArgs), c_int]),
     "hdmoe_block_linear": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
     "hdmoe_block_swiglu": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
     "hdmoe_layer_layout_get": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(LayerLayout)]),

@@ -27,38 +27,73 @@ constexpr int MAX_E = HDMOE_BLOCK_MAX_EXPERTS;
 constexpr float TOP_FLOOR = 0x1p-96f;
 
 // ---- cast ---------------------------------------------------------------------------------------------------------
-// 16 lanes hold a block of a row, 8 values each; a wave takes 4 neighbouring blocks. Bound by memory: 3.03 bytes per value.
+// Sources of a cast: eight values of a lane and the largest magnitude among them as a bit pattern.
 template <class Act>
-__global__ __launch_bounds__(256) void block_cast_kernel(const uint16_t* __restrict__ x, int rows, int K, int KB,
-                                                         uint8_t* __restrict__ q, float* __restrict__ s, long long ld_s) {
+struct Half {   // bf16 or fp16
+  u32x4 v;
+  __device__ __forceinline__ void load(const void* x, size_t i) { v = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + i); }
+  __device__ __forceinline__ void clear() { v = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, max(v[i] & 0x7fffu, (v[i] >> 16) & 0x7fffu));
+    return m;
+  }
+  static __device__ __forceinline__ float value(uint32_t m) { return Act::lo(m); }
+  __device__ __forceinline__ float get(int i) const { return i & 1 ? Act::hi(v[i >> 1]) : Act::lo(v[i >> 1]); }
+};
+struct Full {   // fp32
+  v4f v[2];
+  __device__ __forceinline__ void load(const void* x, size_t i) {
+    const v4f* const p = reinterpret_cast<const v4f*>(static_cast<const float*>(x) + i);
+    v[0] = p[0];
+    v[1] = p[1];
+  }
+  __device__ __forceinline__ void clear() { v[0] = v[1] = v4f{0, 0, 0, 0}; }
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(get(i)) & 0x7fffffffu);
+    return m;
+  }
+  static __device__ __forceinline__ float value(uint32_t m) { return __uint_as_float(m); }
+  __device__ __forceinline__ float get(int i) const { return v[i >> 2][i & 3]; }
+};
+
+// Eight values of a block that 16 lanes hold -> their bytes and the block's scale.
+template <class Src>
+__device__ __forceinline__ void cast_unit(const Src& x, uint32_t (&o)[2], float& s) {
+  uint32_t m = x.largest();
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 16));
+  const float top_in = Src::value(m);
+  const float top = top_in < TOP_FLOOR ? TOP_FLOOR : top_in;
+  const float r = 448.0f / top;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) o[i] = hdmoe_dev_pack4_e4m3fn(x.get(4 * i) * r, x.get(4 * i + 1) * r, x.get(4 * i + 2) * r, x.get(4 * i + 3) * r);
+  s = top / 448.0f;
+}
+
+// 16 lanes hold a block of a row, 8 values each; a wave takes 4 neighbouring blocks. Bound by memory: 3.03 bytes per value of 16 bits.
+// bounds: NULL, or only the rows from bounds[0] to bounds[nbounds - 1] are cast.
+template <class Src>
+__global__ __launch_bounds__(256) void block_cast_kernel(const void* __restrict__ x, int rows, int K, int KB, uint8_t* __restrict__ q,
+                                                         float* __restrict__ s, long long ld_s, const int32_t* __restrict__ bounds, int nbounds) {
   const long long n = (long long)rows * KB;
   const long long u = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
   if (u >= n) return;
   const int row = (int)(u / KB), b = (int)(u - (long long)row * KB);
+  if (bounds != nullptr && (row < bounds[0] || row >= bounds[nbounds - 1])) return;
   const int k = b * BLK + (threadIdx.x & 15) * 8;
   const bool in = k < K;   // K is a multiple of 16: eight values lie inside or outside together
-  u32x4 v = {0, 0, 0, 0};
-  if (in) v = *reinterpret_cast<const u32x4*>(x + (size_t)row * K + k);
-  // the largest magnitude as an integer of 16 bits
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = v[i] & 0x7fffu, hi = (v[i] >> 16) & 0x7fffu;
-    m = max(m, max(lo, hi));
-  }
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 16));
-  const float top_in = Act::lo(m);
-  const float top = top_in < TOP_FLOOR ? TOP_FLOOR : top_in;
-  const float r = 448.0f / top;
-  if (in) {
-    u32x2 o;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      o[i] = hdmoe_dev_pack4_e4m3fn(Act::lo(v[2 * i]) * r, Act::hi(v[2 * i]) * r, Act::lo(v[2 * i + 1]) * r, Act::hi(v[2 * i + 1]) * r);
-    *reinterpret_cast<u32x2*>(q + (size_t)row * K + k) = o;
-  }
-  if ((threadIdx.x & 15) == 0) s[(size_t)b * ld_s + row] = top / 448.0f;
+  Src v;
+  v.clear();
+  if (in) v.load(x, (size_t)row * K + k);
+  uint32_t o[2];
+  float scale;
+  cast_unit(v, o, scale);
+  if (in) *reinterpret_cast<u32x2*>(q + (size_t)row * K + k) = u32x2{o[0], o[1]};
+  if ((threadIdx.x & 15) == 0) s[(size_t)b * ld_s + row] = scale;
 }
 
 // ---- contraction --------------------------------------------------------------------------------------------------
@@ -80,6 +115,7 @@ struct Operand {
   int rows;             // rows of the segments (or of the static group)
   int K, N;
   void* out;            // 16-bit [rows,N]; gate/up: e4m3fn [rows,N]
+  float* h;             // gate/up of few rows: fp32 [rows,N] in front of the cast
   float* s_out;         // gate/up: scale of block b of row r at s_out[b * ld_out + r]
   long long ld_out;
 };
@@ -549,37 +585,20 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
 // Segments of up to a few dozen rows: the weights are read once from memory into registers, no tile of them passes through LDS, and
 // many 16-byte loads are on their way at once. A wave multiplies FT strips of 16 weight rows with TT * 16 tokens; KW waves deal the K
 // blocks of the same strips out and their sums meet in LDS.
-//   Linear:  8 waves, all of them along K, on FT strips. More strips read the activations less often (they come out of L2, 16 TT rows
-//            for every 16 FT of the weights), fewer make more blocks.
-//   gate/up: 4 pairs of waves, each pair on 2 strips of w1 and the same 2 of w3, together one block of the cast output.
+// More strips a wave read the activations less often (they come out of L2, 16 TT rows for every 16 FT of the weights), fewer make more
+// blocks: a CU has only so many requests on their way, so all 256 have to take part.
+//   gate/up: half of the strips are w1's, half the same features of w3; silu(g) * u leaves in fp32, and a second launch casts it. (One
+//            launch needs the 128 features of a cast block in one thread block, 54 blocks an expert at 6912.)
 // CAST: the activations are 16-bit rows; the block casts its own into LDS (rows of K + 16 bytes: 16 rows then hit all banks) while the
 // first weights are on their way, instead of a launch of its own in front.
-template <class Act>
-__device__ __forceinline__ void cast_unit(const uint16_t* x, int k, bool in, uint32_t (&o)[2], float& s) {
-  u32x4 v = {0, 0, 0, 0};
-  if (in) v = *reinterpret_cast<const u32x4*>(x + k);
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = max(m, max(v[i] & 0x7fffu, (v[i] >> 16) & 0x7fffu));
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 16));
-  const float top_in = Act::lo(m);
-  const float top = top_in < TOP_FLOOR ? TOP_FLOOR : top_in;
-  const float r = 448.0f / top;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    o[i] = hdmoe_dev_pack4_e4m3fn(Act::lo(v[2 * i]) * r, Act::hi(v[2 * i]) * r, Act::lo(v[2 * i + 1]) * r, Act::hi(v[2 * i + 1]) * r);
-  s = top / 448.0f;
-}
-
 template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
 __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int NW = 8;
-  constexpr int KW = SWIGLU ? 2 : 8, SG = NW / KW;
-  static_assert(!SWIGLU || FT == 4, "a pair of waves: two strips of w1, two of w3");
+  constexpr int KW = 8;
+  static_assert(!SWIGLU || FT % 2 == 0, "w1 and w3 by halves");
   constexpr int BM = TT * 16;
-  constexpr int FEAT = SWIGLU ? BLK : 16 * FT;
+  constexpr int STRIPS = SWIGLU ? FT / 2 : FT;   // of one matrix
+  constexpr int FEAT = 16 * STRIPS;
   // K blocks on their way: as many as the registers hold
   constexpr int PER = FT * 8 + (CAST ? 0 : TT * 9) + 2, DEPTH_MAX = (220 - 4 * FT * TT) / PER;
   constexpr int DEPTH = DEPTH_MAX > 6 ? 6 : DEPTH_MAX;
@@ -589,7 +608,7 @@ __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, quad = lane >> 4;
-  const int kw = wave % KW, sg = wave / KW;
+  const int kw = wave;
 
   const Tiles<BM, FEAT> tiles(args, lane);
   const int per_xcd = (tiles.total + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD;
@@ -605,11 +624,9 @@ __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args)
   const int a_rows = op.a_rows;
 
   // weights: lane = row fr of a strip, 16-byte chunks quad and quad + 4 of a K block. Strips past N read as zeros.
-  const int strips = SWIGLU ? 2 : FT;                        // of one matrix
-  const int s0 = t.n0 + sg * strips * 16;
-  const int feats = min(max(N - s0, 0), strips * 16);
-  const __amdgpu_buffer_rsrc_t rw0 = make_rsrc(grp.w0 + (size_t)s0 * K, (uint32_t)feats * (uint32_t)K);
-  const __amdgpu_buffer_rsrc_t rw1 = SWIGLU ? make_rsrc(grp.w1 + (size_t)s0 * K, (uint32_t)feats * (uint32_t)K) : rw0;
+  const int feats = min(N - t.n0, FEAT);
+  const __amdgpu_buffer_rsrc_t rw0 = make_rsrc(grp.w0 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K);
+  const __amdgpu_buffer_rsrc_t rw1 = SWIGLU ? make_rsrc(grp.w1 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K) : rw0;
   const __amdgpu_buffer_rsrc_t rs0 = make_rsrc(grp.s0 + (size_t)(t.n0 / BLK) * KB, (uint32_t)KB * 4u);
   const __amdgpu_buffer_rsrc_t rs1 = SWIGLU ? make_rsrc(grp.s1 + (size_t)(t.n0 / BLK) * KB, (uint32_t)KB * 4u) : rs0;
 
@@ -630,8 +647,8 @@ __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args)
     const bool lo = k < K, hi = k + 64 < K;
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
-      const __amdgpu_buffer_rsrc_t r = SWIGLU && f >= 2 ? rw1 : rw0;
-      const int off = wbase + (SWIGLU ? f & 1 : f) * 16 * K + kb * BLK;
+      const __amdgpu_buffer_rsrc_t r = f >= STRIPS ? rw1 : rw0;
+      const int off = wbase + f % STRIPS * 16 * K + kb * BLK;
       st.w[f][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, lo ? off : OUTSIDE, 0, 0));
       st.w[f][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, hi ? off + 64 : OUTSIDE, 0, 0));
     }
@@ -659,9 +676,8 @@ __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args)
   uint8_t* const lx = smem;
   float* const ls = reinterpret_cast<float*>(smem + (size_t)R * ld_x);
   if constexpr (CAST) {
-    const uint16_t* const x16 = reinterpret_cast<const uint16_t*>(op.a);
     const int units = R * KB;
-    for (int u = tid >> 4; u < units; u += NW * 4) {
+    for (int u = tid >> 4; u < units; u += 32) {
       const int r = u / KB, b = u - r * KB;
       int from = -1;
       if (r < t.rows_here) {
@@ -669,9 +685,12 @@ __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args)
         if ((unsigned)from >= (unsigned)a_rows) from = -1;
       }
       const int k = b * BLK + (tid & 15) * 8;
+      Half<Act> v;
+      v.clear();
+      if (from >= 0 && k < K) v.load(op.a, (size_t)from * K + k);
       uint32_t o[2];
       float s;
-      cast_unit<Act>(x16 + (size_t)max(from, 0) * K, k, from >= 0 && k < K, o, s);
+      cast_unit(v, o, s);
       *reinterpret_cast<u32x2*>(lx + r * ld_x + k) = u32x2{o[0], o[1]};
       if ((tid & 15) == 0) ls[b * R + r] = from >= 0 ? s : 0.0f;
     }
@@ -714,7 +733,7 @@ __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args)
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[f][tt][i] = __builtin_fmaf(p[tt][i], SWIGLU && f >= 2 ? m1[tt] : m0[tt], acc[f][tt][i]);
+        for (int i = 0; i < 4; ++i) acc[f][tt][i] = __builtin_fmaf(p[tt][i], SWIGLU && f >= STRIPS ? m1[tt] : m0[tt], acc[f][tt][i]);
     }
   };
   for (int kb0 = kw; kb0 < KB; kb0 += DEPTH * KW) {
@@ -729,13 +748,13 @@ __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args)
   }
 
   // the waves' sums, [KW][strip][token tile][lane] of 16 bytes
-  constexpr int CELLS = SG * FT * TT;
+  constexpr int CELLS = FT * TT;
   v4f* const parts = reinterpret_cast<v4f*>(smem);
   if (CAST) __syncthreads();   // the cast rows are read no more
 #pragma unroll
   for (int f = 0; f < FT; ++f)
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) parts[((kw * SG + sg) * FT * TT + f * TT + tt) * 64 + lane] = acc[f][tt];
+    for (int tt = 0; tt < TT; ++tt) parts[(kw * CELLS + f * TT + tt) * 64 + lane] = acc[f][tt];
   __syncthreads();
   auto total = [&](int cell) {
     v4f y = parts[cell * 64 + lane];
@@ -747,55 +766,27 @@ __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args)
     }
     return y;
   };
-
-  if constexpr (!SWIGLU) {
 #pragma unroll
-    for (int c0 = 0; c0 < CELLS; c0 += NW) {
-      const int cell = c0 + wave, f = cell / TT, tt = cell - f * TT;
-      if (cell >= CELLS) break;
-      v4f y = total(cell);
-      const int r = tt * 16 + fr, n = t.n0 + f * 16 + quad * 4;
-      if (r >= t.rows_here || n >= N) continue;
+  for (int c0 = 0; c0 < STRIPS * TT; c0 += KW) {
+    const int cell = c0 + wave, f = cell / TT, tt = cell - f * TT;
+    if (cell >= STRIPS * TT) break;
+    v4f y = total(cell);
+    const int r = tt * 16 + fr, n = t.n0 + f * 16 + quad * 4;
+    if constexpr (SWIGLU) {
+      const v4f u = total(cell + STRIPS * TT);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = silu(y[i]) * u[i];
+    }
+    if (r >= t.rows_here || n >= N) continue;
+    const size_t at = (size_t)(t.row0 + r) * N + n;
+    if constexpr (SWIGLU) {
+      *reinterpret_cast<v4f*>(op.h + at) = y;
+    } else {
       if (grp.bias != nullptr) {
         const u32x2 b = *reinterpret_cast<const u32x2*>(grp.bias + n);
         y[0] += Act::lo(b.x); y[1] += Act::hi(b.x); y[2] += Act::lo(b.y); y[3] += Act::hi(b.y);
       }
-      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(op.out) + (size_t)(t.row0 + r) * N + n) = u32x2{Act::pack(y[0], y[1]), Act::pack(y[2], y[3])};
-    }
-  } else {
-    // wave w: strip w of w1 and of w3; silu(g) * u, the largest value of a token over the eight strips, the cast
-    uint32_t* const tops = reinterpret_cast<uint32_t*>(smem + (size_t)KW * CELLS * 1024);   // [8][BM]
-    const int g = (wave >> 1) * FT + (wave & 1);
-    v4f h[TT];
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-      h[tt] = total(g * TT + tt);
-      const v4f u = total((g + 2) * TT + tt);
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        h[tt][i] = silu(h[tt][i]) * u[i];
-        top = max(top, __float_as_uint(h[tt][i]) & 0x7fffffffu);
-      }
-      top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-      top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-      if (quad == 0) tops[wave * BM + tt * 16 + fr] = top;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-      const int r = tt * 16 + fr, n = t.n0 + wave * 16 + quad * 4;
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, tops[j * BM + r]);
-      const float both = __uint_as_float(top);
-      const float tp = both < TOP_FLOOR ? TOP_FLOOR : both;
-      const float m = 448.0f / tp;
-      if (r >= t.rows_here) continue;
-      if (wave == 0 && quad == 0) op.s_out[(size_t)(t.n0 / BLK) * op.ld_out + t.row0 + r] = tp / 448.0f;
-      if (n >= N) continue;
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(op.out) + (size_t)(t.row0 + r) * N + n) =
-          hdmoe_dev_pack4_e4m3fn(h[tt][0] * m, h[tt][1] * m, h[tt][2] * m, h[tt][3] * m);
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(op.out) + at) = u32x2{Act::pack(y[0], y[1]), Act::pack(y[2], y[3])};
     }
   }
 #endif
@@ -849,17 +840,16 @@ int launch_gemm8(const BlockArgs& args, const char* what, hipStream_t stream) {
 }
 
 // LDS of a few-row block: cast rows and their scales, then the sums of its waves
-constexpr size_t stream_sums(bool swiglu, int ft, int tt) { return (size_t)8 * ft * tt * 1024 + (swiglu ? (size_t)8 * tt * 16 * 4 : 0); }
 
 template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
 int launch_stream(const BlockArgs& args, const char* what, hipStream_t stream) {
-  constexpr size_t sums = stream_sums(SWIGLU, FT, TT);
+  constexpr size_t sums = (size_t)8 * FT * TT * 1024;
   static std::atomic<uint64_t> done{0};
   if (sums > 65536)
     if (int rc = allow_lds(block_stream_kernel<Act, SWIGLU, FT, TT, CAST>, sums, done, what)) return rc;
   const int K = args.op[0].K > args.op[1].K ? args.op[0].K : args.op[1].K;
   const size_t KB = (K + BLK - 1) / BLK, rows = CAST ? (size_t)args.lds_rows * (KB * BLK + 16 + KB * 4) : 0;
-  const long long grid = grid_of(args, TT * 16, SWIGLU ? BLK : 16 * FT);
+  const long long grid = grid_of(args, TT * 16, SWIGLU ? 8 * FT : 16 * FT);
   if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
   block_stream_kernel<Act, SWIGLU, FT, TT, CAST><<<(unsigned)grid, 512, rows > sums ? rows : sums, stream>>>(args);
   return hdmoe_check_launch(what);
@@ -895,9 +885,9 @@ extern "C" int hdmoe_quant_block_fp8(int src_dtype, const void* x, int64_t rows,
   if (blocks > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%lld K=%d", what, (long long)rows, K);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (src_dtype == HDMOE_W_BF16)
-    block_cast_kernel<HdmoeBf16><<<(unsigned)blocks, 256, 0, s>>>(static_cast<const uint16_t*>(x), (int)rows, K, KB, static_cast<uint8_t*>(out_e4m3fn), scale, scale_stride);
+    block_cast_kernel<Half<HdmoeBf16>><<<(unsigned)blocks, 256, 0, s>>>(x, (int)rows, K, KB, static_cast<uint8_t*>(out_e4m3fn), scale, scale_stride, nullptr, 0);
   else
-    block_cast_kernel<HdmoeF16><<<(unsigned)blocks, 256, 0, s>>>(static_cast<const uint16_t*>(x), (int)rows, K, KB, static_cast<uint8_t*>(out_e4m3fn), scale, scale_stride);
+    block_cast_kernel<Half<HdmoeF16>><<<(unsigned)blocks, 256, 0, s>>>(x, (int)rows, K, KB, static_cast<uint8_t*>(out_e4m3fn), scale, scale_stride, nullptr, 0);
   return hdmoe_check_launch(what);
 }
 
@@ -906,6 +896,7 @@ namespace {
 // How a call runs: the few-row kernels on tiles of 16 * tt rows and 16 * ft features (tt > 0; with the cast inside or not), or the tiles
 // of block_gemm8_kernel.
 struct Plan { int tt, ft; bool cast_inside; int lds_rows; };
+constexpr int FEW_BLOCKS = 160;
 
 Plan plan_of(bool swiglu, bool x16, int rows, int E, int rows_static, int K, int N) {
   Plan p = {0, 0, false, 0};
@@ -920,16 +911,21 @@ Plan plan_of(bool swiglu, bool x16, int rows, int E, int rows_static, int K, int
     p.lds_rows = whole < 16 ? whole : 16;
     p.cast_inside = p.tt == 1 && (long long)p.lds_rows * ((K + BLK - 1) / BLK) * 16 <= 4 * 512;
   }
-  p.ft = 4;
-  if (!swiglu) {
-    // as many features as leave every CU a block
-    const long long strips = (long long)((E > 0 ? (E < rows ? E : rows) : 0) + (rows_static > 0 ? 1 : 0)) * (N / 16);
-    while (p.ft > 1 && strips < (long long)HDMOE_NUM_CU * p.ft) p.ft >>= 1;
-  }
+  // as many features a block as leave most CUs one
+  const long long strips = (long long)((E > 0 ? (E < rows ? E : rows) : 0) + (rows_static > 0 ? 1 : 0)) * (N / 16) * (swiglu ? 2 : 1);
+  p.ft = p.tt == 4 ? 2 : 4;
+  while (p.ft > (swiglu ? 2 : 1) && strips < (long long)FEW_BLOCKS * p.ft) p.ft >>= 1;
   return p;
 }
 
-size_t cast_bytes(long long rows, int K) { return hdmoe_align_up((size_t)rows * K, 256) + (size_t)rows * ((K + BLK - 1) / BLK) * 4; }
+size_t cast_bytes(long long rows, int K) { return hdmoe_align_up((size_t)rows * K, 256) + hdmoe_align_up((size_t)rows * ((K + BLK - 1) / BLK) * 4, 256); }
+
+// Working memory: the cast rows of 16-bit activations, unless the contraction casts them itself; gate/up of few rows: silu(g) * u in fp32.
+size_t work_bytes(bool swiglu, bool x16, const Plan& plan, int rows, int T, int rows_static, int K, int N, int N_static) {
+  size_t n = x16 && !plan.cast_inside ? cast_bytes(rows > 0 ? (T > 0 ? T : rows) : rows_static, K) : 0;
+  if (swiglu && plan.tt > 0) n += hdmoe_align_up((size_t)rows * N * 4, 256) + hdmoe_align_up((size_t)rows_static * N_static * 4, 256);
+  return n;
+}
 
 // Arguments of both contractions -> those of the kernels; checks everything but what only the device knows. 16-bit activations are
 // cast into the workspace here unless the contraction does that itself.
@@ -1002,17 +998,25 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: 16-bit activations of the experts and of the static group must be the same rows", what);
   plan = plan_of(swiglu, x16, routed ? p->rows : 0, routed ? p->E : 0, p->rows_static, K, routed ? p->N : p->N_static);
   args.lds_rows = plan.lds_rows;
+  const size_t need = work_bytes(swiglu, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K,
+                                 routed ? p->N : 0, p->rows_static > 0 ? p->N_static : 0);
+  if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255)))
+    return hdmoe_fail(HDMOE_E_WORKSPACE, "%s: workspace %zu bytes, need %zu (256-byte aligned)", what, p->workspace_bytes, need);
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   if (a_rows > 0 && x16 && !plan.cast_inside) {
-    if (p->workspace == nullptr || p->workspace_bytes < cast_bytes(a_rows, K) || (reinterpret_cast<uintptr_t>(p->workspace) & 255))
-      return hdmoe_fail(HDMOE_E_WORKSPACE, "%s: workspace %zu bytes, need %zu (256-byte aligned)", what, p->workspace_bytes, cast_bytes(a_rows, K));
-    uint8_t* const q = static_cast<uint8_t*>(p->workspace);
-    float* const s = reinterpret_cast<float*>(q + hdmoe_align_up((size_t)a_rows * K, 256));
-    if (int rc = hdmoe_quant_block_fp8(p->a_dtype, routed ? p->routed.a : p->fixed.a, a_rows, K, q, s, a_rows, stream)) return rc;
+    float* const s = reinterpret_cast<float*>(ws + hdmoe_align_up((size_t)a_rows * K, 256));
+    if (int rc = hdmoe_quant_block_fp8(p->a_dtype, routed ? p->routed.a : p->fixed.a, a_rows, K, ws, s, a_rows, stream)) return rc;
     for (Operand& op : args.op) {
-      op.a = q;
+      op.a = ws;
       op.sa = s;
       op.ld_sa = a_rows;
     }
+    ws += cast_bytes(a_rows, K);
+  }
+  if (swiglu && plan.tt > 0) {
+    args.op[0].h = reinterpret_cast<float*>(ws);
+    if (routed) ws += hdmoe_align_up((size_t)p->rows * p->N * 4, 256);
+    args.op[1].h = reinterpret_cast<float*>(ws);
   }
   return HDMOE_OK;
 }
@@ -1027,18 +1031,36 @@ int launch_strips(const BlockArgs& args, const Plan& plan, const char* what, hip
 
 template <class Act, bool SWIGLU>
 int launch_few(const BlockArgs& args, const Plan& plan, const char* what, hipStream_t s) {
-  if constexpr (!SWIGLU) {
+  if (plan.ft == 4) return launch_strips<Act, SWIGLU, 4>(args, plan, what, s);
+  if constexpr (!SWIGLU)
     if (plan.ft == 1) return launch_strips<Act, false, 1>(args, plan, what, s);
-    if (plan.ft == 2) return launch_strips<Act, false, 2>(args, plan, what, s);
+  return launch_strips<Act, SWIGLU, 2>(args, plan, what, s);
+}
+
+// The cast behind the gate/up of few rows.
+int launch_cast(const BlockArgs& args, const char* what, hipStream_t s) {
+  for (int i = 0; i < 2; ++i) {
+    const Operand& op = args.op[i];
+    if (op.rows == 0) continue;
+    const int HB = (op.N + BLK - 1) / BLK;
+    const long long blocks = ((long long)op.rows * HB * 16 + 255) / 256;
+    block_cast_kernel<Full><<<(unsigned)blocks, 256, 0, s>>>(op.h, op.rows, op.N, HB, static_cast<uint8_t*>(op.out), op.s_out, op.ld_out,
+                                                             i == 0 ? args.offsets : nullptr, args.E + 1);
+    if (int rc = hdmoe_check_launch(what)) return rc;
   }
-  return launch_strips<Act, SWIGLU, 4>(args, plan, what, s);
+  return HDMOE_OK;
 }
 
 }  // namespace
 
-extern "C" size_t hdmoe_block_workspace_bytes(int swiglu, int rows, int E, int T, int rows_static, int K) {
-  if (rows < 0 || E < 0 || T < 0 || rows_static < 0 || K <= 0) return 0;
-  return plan_of(swiglu != 0, true, rows, E, rows_static, K, 16).cast_inside ? 0 : cast_bytes(rows > 0 ? (T > 0 ? T : rows) : rows_static, K);
+extern "C" size_t hdmoe_block_workspace_bytes(const hdmoe_block_args* p, int swiglu) {
+  if (p == nullptr || p->rows < 0 || p->E < 0 || p->T < 0 || p->rows_static < 0) return 0;
+  const bool x16 = p->a_dtype != HDMOE_W_E4M3FN, routed = p->E > 0 && p->rows > 0;
+  if (!routed && p->rows_static == 0) return 0;
+  const int K = routed ? p->K : p->K_static, N = routed ? p->N : 0, Ns = p->rows_static > 0 ? p->N_static : 0;
+  if (K <= 0 || N < 0 || Ns < 0) return 0;
+  const Plan plan = plan_of(swiglu != 0, x16, routed ? p->rows : 0, routed ? p->E : 0, p->rows_static, K, routed ? N : Ns);
+  return work_bytes(swiglu != 0, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K, N, Ns);
 }
 
 extern "C" int hdmoe_block_linear(const hdmoe_block_args* p, hdmoe_stream_t stream) {
@@ -1060,7 +1082,9 @@ extern "C" int hdmoe_block_swiglu(const hdmoe_block_args* p, hdmoe_stream_t stre
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (int rc = fill(what, p, true, args, plan, s)) return rc;
   if (args.op[0].rows + (long long)args.op[1].rows == 0) return HDMOE_OK;
-  if (plan.tt > 0)
-    return p->a_dtype == HDMOE_W_F16 ? launch_few<HdmoeF16, true>(args, plan, what, s) : launch_few<HdmoeBf16, true>(args, plan, what, s);
+  if (plan.tt > 0) {
+    if (int rc = p->a_dtype == HDMOE_W_F16 ? launch_few<HdmoeF16, true>(args, plan, what, s) : launch_few<HdmoeBf16, true>(args, plan, what, s)) return rc;
+    return launch_cast(args, what, s);
+  }
   return launch_gemm8<HdmoeBf16, true>(args, what, s);
 }

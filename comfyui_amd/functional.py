@@ -558,6 +558,11 @@ _HERE = contextlib.nullcontext()
 _ACT_CODE = {BF16: W_BF16, F16: _lib.W_F16, FP8: W_E4M3FN}
 
 
+def _raw_stream(t):
+    """_stream without the object around the handle."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def _on(device):
     """Context in which `device` is the current one."""
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
@@ -584,7 +589,7 @@ def quant_block_fp8(x):
     with _on(dev):
         q = torch.empty_like(x, dtype=FP8)
         s = block_scales(rows, K, dev)
-        check(lib.hdmoe_quant_block_fp8(_ACT_CODE[dt], x.data_ptr(), rows, K, q.data_ptr(), s.data_ptr(), rows, _stream(x)))
+        check(lib.hdmoe_quant_block_fp8(_ACT_CODE[dt], x.data_ptr(), rows, K, q.data_ptr(), s.data_ptr(), rows, _raw_stream(x)))
     return q, s
 
 
@@ -610,35 +615,38 @@ def _block_rows(a, scale_a, what):
     return scale_a
 
 
-def _block_matrix(weight, scale, K, device, what):
-    """N of a weight [N, K] with scales [ceil(N / 128), ceil(K / 128)]."""
-    shape = weight.shape
-    if weight.dtype != FP8 or len(shape) != 2 or shape[1] != K or weight.device != device or not weight.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous float8_e4m3fn weight [N, {K}] on {device}, got {weight.dtype} "
-                         f"{tuple(shape)} on {weight.device}")
-    N = shape[0]
-    if (scale.dtype != torch.float32 or scale.shape != (-(-N // BLOCK), -(-K // BLOCK)) or scale.device != device
-            or not scale.is_contiguous()):
-        raise ValueError(f"{what}: expected contiguous float32 scales [{_blocks(N)}, {_blocks(K)}] on {device}, got "
-                         f"{scale.dtype} {tuple(scale.shape)} on {scale.device}")
-    return N
+def _block_matrix(weight, scale, K, index, what, shapes=None):
+    """Checks a weight [N, K] and its scales [ceil(N / 128), ceil(K / 128)] on device `index`; shapes: what they have to be (that of the
+    experts before), else formed from the weight's. Returns the shapes."""
+    if shapes is None:
+        N = weight.shape[0] if weight.dim() == 2 else -1
+        shapes = ((N, K), (-(-N // BLOCK), -(-K // BLOCK)))
+    if weight.dtype is not FP8 or weight.shape != shapes[0] or weight.get_device() != index or not weight.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous float8_e4m3fn weight {list(shapes[0])} on device {index}, got {weight.dtype} "
+                         f"{tuple(weight.shape)} on {weight.device}")
+    if scale.dtype is not torch.float32 or scale.shape != shapes[1] or scale.get_device() != index or not scale.is_contiguous():
+        raise ValueError(f"{what}: expected contiguous float32 scales {list(shapes[1])} on device {index}, got {scale.dtype} "
+                         f"{tuple(scale.shape)} on {scale.device}")
+    return shapes
 
 
-def _block_weights(entry, K, dtype, device, what):
-    """(BlockWeights, N) of (weight, scale, bias or None) or, for gate/up (dtype None), (w1, scale1, w3, scale3)."""
+def _block_weights(w, entry, K, dtype, index, what, shapes=None):
+    """Fills a BlockWeights from (weight, scale, bias or None) or, for gate/up (dtype None), (w1, scale1, w3, scale3)."""
     if dtype is None:
         w1, s1, w3, s3 = entry
-        N = _block_matrix(w1, s1, K, device, what)
-        if _block_matrix(w3, s3, K, device, what) != N:
-            raise ValueError(f"{what}: w1 {tuple(w1.shape)} and w3 {tuple(w3.shape)} differ")
-        return _lib.BlockWeights(w1.data_ptr(), s1.data_ptr(), w3.data_ptr(), s3.data_ptr()), N
-    w, s, bias = entry
-    N = _block_matrix(w, s, K, device, what)
-    if bias is None:
-        return _lib.BlockWeights(w.data_ptr(), s.data_ptr()), N
-    if bias.dtype != dtype or bias.device != device or bias.shape != (N,) or not bias.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous {dtype} bias [{N}] on {device}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
-    return _lib.BlockWeights(w.data_ptr(), s.data_ptr(), None, None, bias.data_ptr()), N
+        shapes = _block_matrix(w1, s1, K, index, what, shapes)
+        _block_matrix(w3, s3, K, index, what, shapes)
+        w.weight3, w.scale3 = w3.data_ptr(), s3.data_ptr()
+    else:
+        w1, s1, bias = entry
+        shapes = _block_matrix(w1, s1, K, index, what, shapes)
+        if bias is not None:
+            if bias.dtype is not dtype or bias.shape != (shapes[0][0],) or bias.get_device() != index or not bias.is_contiguous():
+                raise ValueError(f"{what}: expected a contiguous {dtype} bias [{shapes[0][0]}] on device {index}, got {bias.dtype} "
+                                 f"{tuple(bias.shape)} on {bias.device}")
+            w.bias = bias.data_ptr()
+    w.weight, w.scale = w1.data_ptr(), s1.data_ptr()
+    return shapes
 
 
 def _block_out_dtype(a, out_dtype, what):
@@ -664,26 +672,23 @@ def _block_experts(a, offsets, experts, perm, dtype, what):
         if perm.dtype != torch.int32 or perm.shape != (rows,) or perm.device != dev or not perm.is_contiguous():
             raise ValueError(f"{what}: perm must be contiguous int32 [{rows}] on {dev}")
     arr = (_lib.BlockWeights * E)()
-    N = None
-    for i, entry in enumerate(experts):
-        arr[i], n = _block_weights(entry, K, dtype, dev, what)
-        if N is None:
-            N = n
-        elif n != N:
-            raise ValueError(f"{what}: the experts' weights differ in size")
-    return arr, rows, N
+    shapes, index = None, a.get_device()
+    for w, entry in zip(arr, experts):
+        shapes = _block_weights(w, entry, K, dtype, index, what, shapes)
+    return arr, rows, shapes[0][0]
 
 
 def _block_call(fn, swiglu, args, a):
-    """fn(args) with room for the cast of 16-bit rows where it is needed."""
+    """fn(args) with the working memory that it asks for."""
     if args.rows == 0 and args.rows_static == 0:
         return
-    if a.dtype != FP8:
-        nbytes = lib.hdmoe_block_workspace_bytes(swiglu, args.rows, args.E, args.T, args.rows_static, a.shape[1])
+    ref = ctypes.byref(args)
+    if swiglu or a.dtype is not FP8:
+        nbytes = lib.hdmoe_block_workspace_bytes(ref, swiglu)
         if nbytes > 0:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
             args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-    check(fn(ctypes.byref(args), _stream(a)))
+    check(fn(ref, _raw_stream(a)))
 
 
 def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype=None):
@@ -696,7 +701,8 @@ def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype
     s = _block_rows(x, scale_x, what + " x")
     rows, K = x.shape
     dev = x.device
-    w, N = _block_weights((weight, scale_weight, bias), K, dt, dev, what)
+    w = _lib.BlockWeights()
+    N = _block_weights(w, (weight, scale_weight, bias), K, dt, x.get_device(), what)[0][0]
     with _on(dev):
         out = torch.empty((rows, N), dtype=dt, device=dev)
         if rows > 0:
@@ -747,7 +753,8 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
                 a_static, scale_static = quant_block_fp8(a_static)
             s = _block_rows(a_static, scale_static, what + " a_static")
             n, Ks = a_static.shape
-            w, Ns = _block_weights(shared, Ks, dt, dev, what + " shared")
+            w = _lib.BlockWeights()
+            Ns = _block_weights(w, shared, Ks, dt, a.get_device(), what + " shared")[0][0]
             out_static = torch.empty((n, Ns), dtype=dt, device=dev)
             if n > 0:
                 args.rows_static, args.K_static, args.N_static = n, Ks, Ns
@@ -784,7 +791,8 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
             r.a, r.scale_a, r.scale_a_stride, r.out = a.data_ptr(), ptr(sa), T, h.data_ptr()
             r.scale_out, r.scale_out_stride = sh.data_ptr(), rows
         if shared is not None:
-            w, Hs = _block_weights(shared, K, None, dev, what + " shared")
+            w = _lib.BlockWeights()
+            Hs = _block_weights(w, shared, K, None, a.get_device(), what + " shared")[0][0]
             h_shared = torch.empty((T, Hs), dtype=FP8, device=dev)
             sh_shared = block_scales(T, Hs, dev)
             if T > 0:

@@ -415,12 +415,12 @@ typedef struct hdmoe_block_args {
   const hdmoe_block_weights* experts; /* host array [E] */
   const hdmoe_block_weights* shared;  /* of the static group */
   hdmoe_block_rows routed, fixed;     /* the experts' rows, the static group's (16-bit a: the same rows where both are there) */
-  void* workspace;    /* 16-bit a: hdmoe_block_workspace_bytes(...) bytes, 256-byte aligned (NULL where that is 0) */
+  void* workspace;    /* hdmoe_block_workspace_bytes(...) bytes, 256-byte aligned (NULL where that is 0) */
   size_t workspace_bytes;
 } hdmoe_block_args;
-/* Room for the cast rows of 16-bit activations; 0 where the contraction casts them itself (few rows). T: as in the arguments, 0
- * without a permutation; K: of the rows to be cast. */
-size_t hdmoe_block_workspace_bytes(int swiglu, int rows, int E, int T, int rows_static, int K);
+/* Working memory of a call: the cast rows of 16-bit activations, unless the contraction casts them itself (few rows), and for
+ * hdmoe_block_swiglu (swiglu nonzero) on few rows the fp32 values in front of the cast. Looks at the sizes, a_dtype and perm. */
+size_t hdmoe_block_workspace_bytes(const hdmoe_block_args* args, int swiglu);
 
 /* out[r, n] = round( sum_b scale_a[r, b] * scale[n / 128, b] * sum_{k in block b} a[r, k] * weight[n, k]  + bias[n] ); the sums over
  * a block are the matrix cores', the one over blocks is fp32, and there is one rounding to out_dtype. */
