@@ -187,31 +187,32 @@ struct Tiles {
 __device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
 // The end of a tile, for a wave that holds acc(f, tt, i) as laid out below: bias, rounding and stores, or SiLU * mul and the cast.
-struct BiasWords { u32x4 w[4]; };   // of the lane's 32 features
+struct BiasWords { u32x4 w[4]; };   // of the lane's 4 FT features
+template <int FT>
 __device__ __forceinline__ BiasWords load_bias(const Operand& op, const Group& grp, const Tile& t, int wf, int lane) {
   BiasWords b = {};
   const uint16_t* const p = grp.bias;
   if (p != nullptr) {
-    const int f0 = t.n0 + wf * BLK + (lane >> 4) * 8;
+    const int f0 = t.n0 + wf * FT * 16 + (lane >> 4) * 8;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < FT / 2; ++c)
       if (f0 + c * 32 < op.N) b.w[c] = *reinterpret_cast<const u32x4*>(p + f0 + c * 32);   // N is a multiple of 16
 #pragma unroll
-    for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(b.w[c]));   // what waits for them does so here, not where there is no bias
+    for (int c = 0; c < FT / 2; ++c) asm volatile("" : "+v"(b.w[c]));   // what waits for them does so here, not where there is no bias
   }
   return b;
 }
 
-template <class Act, bool SWIGLU, int BM, int TT, class Acc>
+template <class Act, bool SWIGLU, int BM, int WF, int FT, int TT, class Acc>
 __device__ __forceinline__ void store_tile(const Operand& op, const BiasWords& bias, const Tile& t, uint8_t* exchange, int wf, int wt, int lane, Acc acc) {
   const int N = op.N, quad = lane >> 4;
   constexpr int OUTSIDE = (int)0x80000000u;
   if constexpr (!SWIGLU) {
-    const int f0 = t.n0 + wf * BLK + quad * 8;        // eight features from f0 + 32 c on
+    const int f0 = t.n0 + wf * FT * 16 + quad * 8;    // eight features from f0 + 32 c on
     // rows of the tile; what lies past its rows or features gets an offset past the buffer and is not written
     const __amdgpu_buffer_rsrc_t out = make_rsrc(static_cast<uint16_t*>(op.out) + (size_t)t.row0 * N, (uint32_t)t.rows_here * (uint32_t)N * 2u);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < FT / 2; ++c) {
       const int f = f0 + c * 32;
       const u32x4 b = bias.w[c];
 #pragma unroll
@@ -224,19 +225,19 @@ __device__ __forceinline__ void store_tile(const Operand& op, const BiasWords& b
       }
     }
   } else {
-    // silu(g) * u, then the cast of the 128 features: 16 in a lane, 64 in the four lanes of a token, two waves. The exponential and
+    // silu(g) * u, then the cast of the 128 features: 2 FT in a lane, 8 FT in the four lanes of a token, WF waves. The exponential and
     // the reciprocal are the hardware's, 1 ulp each beside half an e4m3 step of 2^-4.
     uint32_t* const tops = reinterpret_cast<uint32_t*>(exchange);   // [WF][BM]
-    float h[TT][16];
+    float h[TT][FT * 2];
     uint32_t top[TT];
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
       top[tt] = 0;
 #pragma unroll
-      for (int f = 0; f < 4; ++f)
+      for (int f = 0; f < FT / 2; ++f)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float v = silu(acc(f, tt, i)) * acc(f + 4, tt, i);
+          const float v = silu(acc(f, tt, i)) * acc(f + FT / 2, tt, i);
           h[tt][f * 4 + i] = v;
           top[tt] = max(top[tt], __float_as_uint(v) & 0x7fffffffu);
         }
@@ -245,38 +246,50 @@ __device__ __forceinline__ void store_tile(const Operand& op, const BiasWords& b
       if (quad == 0) tops[wf * BM + wt * TT * 16 + tt * 16 + lane] = top[tt];
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    const int f0 = t.n0 + wf * 64 + quad * 16;
+    const int f0 = t.n0 + wf * FT * 8 + quad * FT * 2;
     const __amdgpu_buffer_rsrc_t out = make_rsrc(static_cast<uint8_t*>(op.out) + (size_t)t.row0 * N, (uint32_t)t.rows_here * (uint32_t)N);
     const __amdgpu_buffer_rsrc_t outs = make_rsrc(op.s_out + (size_t)(t.n0 / BLK) * op.ld_out + t.row0, (uint32_t)t.rows_here * 4u);
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
       const int r = wt * TT * 16 + tt * 16 + (lane & 15);
-      const float both = __uint_as_float(max(top[tt], tops[(1 - wf) * BM + r]));
+#pragma unroll
+      for (int w = 1; w < WF; ++w) top[tt] = max(top[tt], tops[(wf + w) % WF * BM + r]);
+      const float both = __uint_as_float(top[tt]);
       const float tp = both < TOP_FLOOR ? TOP_FLOOR : both;
       const float m = 448.0f / tp;
       __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(tp / 448.0f), outs, r < t.rows_here && wf == 0 && quad == 0 ? r * 4 : OUTSIDE, 0, 0);
-      v4i v;
+      const int at = r < t.rows_here && f0 < N ? r * N + f0 : OUTSIDE;
+      int v[FT / 2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < FT / 2; ++i)
         v[i] = (int)hdmoe_dev_pack4_e4m3fn(h[tt][4 * i] * m, h[tt][4 * i + 1] * m, h[tt][4 * i + 2] * m, h[tt][4 * i + 3] * m);
-      __builtin_amdgcn_raw_buffer_store_b128(v, out, r < t.rows_here && f0 < N ? r * N + f0 : OUTSIDE, 0, 0);
+      if constexpr (FT == 8) __builtin_amdgcn_raw_buffer_store_b128(v4i{v[0], v[1], v[2], v[3]}, out, at, 0, 0);
+      else __builtin_amdgcn_raw_buffer_store_b64(u32x2{(uint32_t)v[0], (uint32_t)v[1]}, out, at, 0, 0);
     }
   }
 }
 
-// WF x WT waves, each FT * 16 = 128 weight rows x TT * 16 tokens in MFMA tiles of 16 x 16 x 128. Weight rows of a wave are features
-// of one weight block (gate/up: 64 of w1 and the same 64 of w3). LDS row 16 ft + r of a wave's weights holds the feature that puts
-// 8 consecutive ones (gate/up: 16) in a lane's accumulators and 32 (64) in the four lanes of a token: stores of 16 bytes, 64 of them
-// next to each other, without a transposition.
-template <class Act, bool SWIGLU, int WF, int WT, int TT>
-__global__ __launch_bounds__(64 * WF * WT) void block_gemm_kernel(const BlockArgs args) {
+// The feature (of its wave's) that row r of MFMA tile f holds: one that puts 8 consecutive features (gate/up: 2 FT) in a lane's
+// accumulators and 32 (8 FT) in the four lanes of a token, so that stores are 16 bytes each and 64 of them lie next to each other. Gate/up:
+// tiles below FT / 2 are w1, the others the same features of w3.
+template <bool SWIGLU, int FT>
+__device__ __forceinline__ int tile_feature(int f, int r) {
+  return SWIGLU ? (r >> 2) * FT * 2 + f % (FT / 2) * 4 + (r & 3) : (f >> 1) * 32 + (r >> 2) * 8 + (f & 1) * 4 + (r & 3);
+}
+
+// Tiles of 128 tokens x 128 features (gate/up: 64 tokens x 128 of w1 and of w3), for launches whose 256-row tiles would leave CUs idle.
+// WF x WT waves, each FT * 16 weight rows x TT * 16 tokens in MFMA tiles of 16 x 16 x 128; the results of a weight tile join the
+// accumulators behind the MFMAs of the next one. STAGES K steps in LDS, STAGES - 1 of them asked for ahead: with two, two blocks share
+// a CU and one fills the other's waits; with more, for launches that have at most a block for every CU, a step does not last as long as
+// its loads are on their way (128 x 6912 x 2560: X us with two).
+template <class Act, bool SWIGLU, int WF, int WT, int FT, int TT, int STAGES>
+__global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_kernel(const BlockArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)   // (the host pass leaves out stubs of kernels whose lambdas hold arrays of dependent size)
-  constexpr int FT = 8;
   constexpr int NT = 64 * WF * WT;
-  constexpr int BM = WT * TT * 16, BN = WF * BLK;
+  constexpr int BM = WT * TT * 16, BN = WF * FT * 16;
   constexpr int FEAT = SWIGLU ? BN / 2 : BN;
-  static_assert(!SWIGLU || WF == 2, "a block of the cast output is 128 features");
-  constexpr int STAGE = (BM + BN) * BLK;
+  static_assert(FEAT == BLK, "one block of weight scales, one of the cast output");
+  constexpr int STAGE = (BM + BN) * BLK + 2048;      // and the scales of the tokens
   constexpr int ROWS_PER_LOAD = NT / 8;               // rows that one load of every wave moves
   constexpr int LA = BM / ROWS_PER_LOAD, LB = BN / ROWS_PER_LOAD;
   static_assert(LA * ROWS_PER_LOAD == BM && LB * ROWS_PER_LOAD == BN && ROWS_PER_LOAD % 16 == 0, "whole loads");
@@ -296,6 +309,8 @@ __global__ __launch_bounds__(64 * WF * WT) void block_gemm_kernel(const BlockArg
   const Operand& op = args.op[t.g == args.E ? 1 : 0];
   const int K = op.K, N = op.N;
   const int KB = (K + BLK - 1) / BLK;
+  const int32_t* const gather = op.gather;
+  const int a_rows = op.a_rows;
 
   // ---- global -> LDS: lane i of a load lands in 16-byte chunk i & 7 of row i >> 3 and fetches the chunk that the swizzle puts there.
   // Rows and chunks that do not exist get an offset past the buffer and read as zero.
@@ -303,63 +318,64 @@ __global__ __launch_bounds__(64 * WF * WT) void block_gemm_kernel(const BlockArg
   const int ld_chunk = (lane & 7) ^ swz(ld_row);
   constexpr int OUTSIDE = (int)0x80000000u;
   int va[LA], vb[LB];
-  const bool gathers = op.gather != nullptr;
-  const __amdgpu_buffer_rsrc_t ra = gathers ? make_rsrc(op.a, (uint32_t)op.a_rows * (uint32_t)K)
-                                            : make_rsrc(op.a + (size_t)t.row0 * K, (uint32_t)t.rows_here * (uint32_t)K);
+  const __amdgpu_buffer_rsrc_t ra = gather != nullptr ? make_rsrc(op.a, (uint32_t)a_rows * (uint32_t)K)
+                                                      : make_rsrc(op.a + (size_t)t.row0 * K, (uint32_t)t.rows_here * (uint32_t)K);
 #pragma unroll
   for (int j = 0; j < LA; ++j) {
     const int r = j * ROWS_PER_LOAD + ld_row;
     va[j] = OUTSIDE;
     if (r < t.rows_here) {
-      const int from = gathers ? op.gather[t.row0 + r] >> 1 : r;   // a bad index of the permutation reads as a row of zeros
-      if (!gathers || (unsigned)from < (unsigned)op.a_rows) va[j] = from * K + ld_chunk * 16;
+      const int from = gather != nullptr ? gather[t.row0 + r] >> 1 : r;   // a bad index of the permutation reads as a row of zeros
+      if (gather == nullptr || (unsigned)from < (unsigned)a_rows) va[j] = from * K + ld_chunk * 16;
     }
   }
   const int feats = min(N - t.n0, FEAT);
   const __amdgpu_buffer_rsrc_t rb0 = make_rsrc(grp.w0 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K);
   const __amdgpu_buffer_rsrc_t rb1 = SWIGLU ? make_rsrc(grp.w1 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K) : rb0;
+  // gate/up: whether load j of this wave fetches rows of w3 (one answer for its 8 rows)
+  auto upper = [&](int j) { return SWIGLU && ((j * ROWS_PER_LOAD + wave * 8) / 16) % FT >= FT / 2; };
 #pragma unroll
   for (int j = 0; j < LB; ++j) {
     const int p = j * ROWS_PER_LOAD + ld_row;         // LDS row of the weight tile
-    const int w = p >> 7, ft = (p >> 4) & 7, r = p & 15;
-    const int f = SWIGLU ? w * 64 + (r >> 2) * 16 + (ft & 3) * 4 + (r & 3) : w * 128 + (ft >> 1) * 32 + (r >> 2) * 8 + (ft & 1) * 4 + (r & 3);
+    const int w = p / (FT * 16), f = w * (SWIGLU ? FT * 8 : FT * 16) + tile_feature<SWIGLU, FT>(p / 16 % FT, p & 15);
     vb[j] = f < feats ? f * K + ld_chunk * 16 : OUTSIDE;
   }
+  // scales of the tile's tokens: one word a lane, 64 tokens a wave (the waves past them ask for none); they go through LDS as well
+  const int ld_s = __builtin_amdgcn_readfirstlane((int)op.ld_sa * 4);
+  const __amdgpu_buffer_rsrc_t rs = make_rsrc(op.sa, (uint32_t)(KB - 1) * (uint32_t)ld_s + (uint32_t)a_rows * 4u);
+  int tok = OUTSIDE;
+  {
+    const int r = wave * 64 + lane;
+    if (r < t.rows_here && r < BM) {
+      const int from = gather != nullptr ? gather[t.row0 + r] >> 1 : t.row0 + r;
+      if ((unsigned)from < (unsigned)a_rows) tok = from * 4;
+    }
+  }
+  // The loads are written by hand so that the compiler, which takes any of them for one that a later LDS read may want, does not wait.
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
+  auto to_lds = [](const __amdgpu_buffer_rsrc_t& r, uint32_t lds, int voff, int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
+  };
   auto issue = [&](int stage, int kb) {
-    uint8_t* sa = smem + stage * STAGE + wave * 8 * BLK;
-    uint8_t* sb = sa + BM * BLK;
+    const uint32_t sa = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + wave * 8 * BLK), sb = sa + BM * BLK;
     const int k0 = kb * BLK;
-    const bool ok = k0 + ld_chunk * 16 < K;
+    const int mask = k0 + ld_chunk * 16 < K ? 0 : OUTSIDE;   // (none past the last step)
 #pragma unroll
-    for (int j = 0; j < LA; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(sa + j * ROWS_PER_LOAD * BLK), 16, ok ? va[j] : OUTSIDE, k0, 0, 0);
+    for (int j = 0; j < LA; ++j) to_lds(ra, sa + j * ROWS_PER_LOAD * BLK, va[j] | mask, k0);
 #pragma unroll
     for (int j = 0; j < LB; ++j) {
-      // gate/up: the w3 rows are the upper 64 of every wave's 128; a load's rows lie on one side for a given wave
-      const bool up = SWIGLU && (((j * ROWS_PER_LOAD + wave * 8) >> 6) & 1);
-      if (up) __builtin_amdgcn_raw_ptr_buffer_load_lds(rb1, (lds_ptr_t)(sb + j * ROWS_PER_LOAD * BLK), 16, ok ? vb[j] : OUTSIDE, k0, 0, 0);
-      else __builtin_amdgcn_raw_ptr_buffer_load_lds(rb0, (lds_ptr_t)(sb + j * ROWS_PER_LOAD * BLK), 16, ok ? vb[j] : OUTSIDE, k0, 0, 0);
+      if (upper(j)) to_lds(rb1, sb + j * ROWS_PER_LOAD * BLK, vb[j] | mask, k0);
+      else to_lds(rb0, sb + j * ROWS_PER_LOAD * BLK, vb[j] | mask, k0);
     }
+    const uint32_t ss = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + (BM + BN) * BLK + wave * 256);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(ss), "v"(tok), "s"(rs), "s"(min(kb, KB - 1) * ld_s) : "memory");
   };
+  constexpr int LOADS = LA + LB + 1;
 
-  // ---- scales: of the lane's token in every token tile, of the wave's weight block
-  int tok[TT];   // row of sa, -1: none
-#pragma unroll
-  for (int tt = 0; tt < TT; ++tt) {
-    const int r = wt * TT * 16 + tt * 16 + (lane & 15);
-    tok[tt] = r < t.rows_here ? (gathers ? op.gather[t.row0 + r] >> 1 : t.row0 + r) : -1;
-    if (tok[tt] >= op.a_rows) tok[tt] = -1;
-  }
-  const int nblk = SWIGLU ? t.n0 / BLK : min(t.n0 / BLK + wf, (N - 1) / BLK);
-  const float* sw0 = grp.s0 + (size_t)nblk * KB;
-  const float* sw1 = SWIGLU ? grp.s1 + (size_t)nblk * KB : sw0;
-  float sx[TT], s0 = 0.0f, s1 = 0.0f;
-  auto load_scales = [&](int kb) {
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) sx[tt] = tok[tt] >= 0 ? op.sa[(size_t)kb * op.ld_sa + tok[tt]] : 0.0f;
-    s0 = sw0[kb];
-    if (SWIGLU) s1 = sw1[kb];
-  };
+  // the weight block's scales come by scalar loads, a step ahead
+  typedef const __attribute__((address_space(4))) float* const_float_ptr;
+  const const_float_ptr sw0 = (const_float_ptr)(uintptr_t)(grp.s0 + (size_t)(t.n0 / BLK) * KB);
+  const const_float_ptr sw1 = SWIGLU ? (const_float_ptr)(uintptr_t)(grp.s1 + (size_t)(t.n0 / BLK) * KB) : sw0;
 
   const int fr = lane & 15, fs = swz(fr), c0 = lane >> 4;
   v4f acc[FT][TT];
@@ -367,44 +383,82 @@ __global__ __launch_bounds__(64 * WF * WT) void block_gemm_kernel(const BlockArg
   for (int f = 0; f < FT; ++f)
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) acc[f][tt] = v4f{0, 0, 0, 0};
-
   auto frag = [&](const uint8_t* row) -> v8i {
     const v4i lo = *reinterpret_cast<const v4i*>(row + ((c0 ^ fs) << 4)), hi = *reinterpret_cast<const v4i*>(row + (((c0 + 4) ^ fs) << 4));
     return v8i{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   };
-
-  issue(0, 0);
-  load_scales(0);
-  for (int kb = 0; kb < KB; ++kb) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
-    __syncthreads();
+  // what a wave reads of a step
+  struct Step { v8i a[FT], b[TT]; float x[TT], s0, s1; };
+  auto read = [&](Step& st, int stage, int kb) {
+    const uint8_t* const base = smem + stage * STAGE;
+    const float* const sx = reinterpret_cast<const float*>(base + (BM + BN) * BLK) + wt * TT * 16 + fr;
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) st.x[tt] = sx[tt * 16];
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) st.b[tt] = frag(base + (wt * TT * 16 + tt * 16 + fr) * BLK);
+#pragma unroll
+    for (int f = 0; f < FT; ++f) st.a[f] = frag(base + (BM + wf * FT * 16 + f * 16 + fr) * BLK);
+    st.s0 = sw0[kb];
+    st.s1 = SWIGLU ? sw1[kb] : 0.0f;
+  };
+  auto multiply = [&](const Step& st) {
+    v4f p[2][TT];
     float m0[TT], m1[TT];
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) { m0[tt] = sx[tt] * s0; m1[tt] = SWIGLU ? sx[tt] * s1 : m0[tt]; }
-    if (kb + 1 < KB) {
-      issue((kb + 1) & 1, kb + 1);
-      load_scales(kb + 1);
-    }
-    const uint8_t* sa = smem + (kb & 1) * STAGE + (wt * TT * 16 + fr) * BLK;
-    const uint8_t* sb = smem + (kb & 1) * STAGE + (BM + wf * BLK + fr) * BLK;
-    v8i fb[TT];
+    for (int tt = 0; tt < TT; ++tt) { m0[tt] = st.x[tt] * st.s0; m1[tt] = st.x[tt] * st.s1; }
+    auto join = [&](int f) {
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) fb[tt] = frag(sa + tt * 16 * BLK);
+      for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[f][tt][i] = __builtin_fmaf(p[f & 1][tt][i], SWIGLU && f >= FT / 2 ? m1[tt] : m0[tt], acc[f][tt][i]);
+    };
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
-      const v8i fa = frag(sb + f * 16 * BLK);
 #pragma unroll
-      for (int tt = 0; tt < TT; ++tt) {
-        const v4f p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb[tt], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-        const float m = SWIGLU && f >= FT / 2 ? m1[tt] : m0[tt];
+      for (int tt = 0; tt < TT; ++tt) p[f & 1][tt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(st.a[f], st.b[tt], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (f > 0) join(f - 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    join(FT - 1);
+  };
+  auto ring = [](int stage) { return stage + 1 == STAGES ? 0 : stage + 1; };
+
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[f][tt][i] = __builtin_fmaf(p[i], m, acc[f][tt][i]);
+  for (int st = 0; st < STAGES - 1; ++st) issue(st, st);
+  int next = STAGES - 1, stage = 0;
+  if constexpr (STAGES == 2) {
+    for (int kb = 0; kb < KB; ++kb) {
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
+      Step st;
+      read(st, stage, kb);
+      issue(next, kb + 1);
+      stage = next;
+      next = ring(next);
+      multiply(st);
+    }
+  } else {
+    // a step's operands are read while the one before is multiplied
+    Step st[2];
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((STAGES - 2) * LOADS) : "memory");
+    read(st[0], 0, 0);
+    for (int kb = 0; kb < KB; kb += 2) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (kb + i < KB) {
+          asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((STAGES - 3) * LOADS) : "memory");
+          stage = ring(stage);
+          read(st[1 - i], stage, min(kb + i + 1, KB - 1));
+          issue(next, kb + i + STAGES - 1);
+          next = ring(next);
+          multiply(st[i]);
+        }
       }
     }
   }
-
-  __syncthreads();   // LDS is read no more
-  store_tile<Act, SWIGLU, BM, TT>(op, SWIGLU ? BiasWords{} : load_bias(op, grp, t, wf, lane), t, smem, wf, wt, lane, [&](int f, int tt, int i) -> float { return acc[f][tt][i]; });
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");   // LDS is read and written no more
+  store_tile<Act, SWIGLU, BM, WF, FT, TT>(op, SWIGLU ? BiasWords{} : load_bias<FT>(op, grp, t, wf, lane), t, smem, wf, wt, lane,
+                                          [&](int f, int tt, int i) -> float { return acc[f][tt][i]; });
 #endif
 }
 
@@ -488,8 +542,7 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
         const int from = gather != nullptr ? gather[t.row0 + r] >> 1 : r;   // a bad index of the permutation reads as a row of zeros
         if (gather == nullptr || (unsigned)from < (unsigned)a_rows) va[j] = from * K + ld_chunk * 16;
       }
-      const int w = r >> 7, ft = (r >> 4) & 7, i = r & 15;
-      const int f = SWIGLU ? w * 64 + (i >> 2) * 16 + (ft & 3) * 4 + (i & 3) : w * 128 + (ft >> 1) * 32 + (i >> 2) * 8 + (ft & 1) * 4 + (i & 3);
+      const int f = (r >> 7) * (SWIGLU ? 64 : 128) + tile_feature<SWIGLU, 8>(r / 16 % 8, r & 15);
       vb[j] = f < feats ? f * K + ld_chunk * 16 : OUTSIDE;
       const int x = wt * 64 + j * 16 + (lane & 15);
       if (x < t.rows_here) {
@@ -570,8 +623,8 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
     }
     asm volatile("" : : : "memory");
     const Operand& op = args.op[done.g == args.E ? 1 : 0];
-    const BiasWords bias = SWIGLU ? BiasWords{} : load_bias(op, args.g[done.g], done, wf, lane_now());
-    store_tile<Act, SWIGLU, BM, TT>(op, bias, done, smem + 131072, wf, wt, lane_now(),
+    const BiasWords bias = SWIGLU ? BiasWords{} : load_bias<8>(op, args.g[done.g], done, wf, lane_now());
+    store_tile<Act, SWIGLU, BM, 2, 8, TT>(op, bias, done, smem + 131072, wf, wt, lane_now(),
                                     [&](int f, int tt, int i) -> float { return acc[f][tt * 4 + i]; });
     if (!more) return;
     // a tile ends in 16 stores (gate/up: 8); the loads in front of them have come back
@@ -817,15 +870,16 @@ long long grid_of(const BlockArgs& args, int bm, int feat) {
   return (tiles + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD * HDMOE_NUM_XCD;
 }
 
-template <class Act, bool SWIGLU, int WF, int WT, int TT>
+template <class Act, bool SWIGLU, int STAGES>
 int launch_gemm(const BlockArgs& args, const char* what, hipStream_t stream) {
-  constexpr int BM = WT * TT * 16, FEAT = SWIGLU ? WF * BLK / 2 : WF * BLK;
-  constexpr size_t SMEM = 2 * (size_t)(BM + WF * BLK) * BLK;
+  constexpr int BM = SWIGLU ? 64 : 128, BN = SWIGLU ? 256 : 128;
+  constexpr size_t SMEM = STAGES * ((size_t)(BM + BN) * BLK + 2048);
+  const auto kernel = block_gemm_kernel<Act, SWIGLU, SWIGLU ? 4 : 2, SWIGLU ? 2 : 4, 4, 2, STAGES>;
   static std::atomic<uint64_t> done{0};
-  if (int rc = allow_lds(block_gemm_kernel<Act, SWIGLU, WF, WT, TT>, SMEM, done, what)) return rc;
-  const long long grid = grid_of(args, BM, FEAT);
+  if (int rc = allow_lds(kernel, SMEM, done, what)) return rc;
+  const long long grid = grid_of(args, BM, BLK);
   if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
-  block_gemm_kernel<Act, SWIGLU, WF, WT, TT><<<(unsigned)grid, 64 * WF * WT, SMEM, stream>>>(args);
+  kernel<<<(unsigned)grid, 512, SMEM, stream>>>(args);
   return hdmoe_check_launch(what);
 }
 
@@ -895,11 +949,11 @@ namespace {
 
 // How a call runs: the few-row kernels on tiles of 16 * tt rows and 16 * ft features (tt > 0; with the cast inside or not), or the tiles
 // of block_gemm8_kernel.
-struct Plan { int tt, ft; bool cast_inside; int lds_rows; };
+struct Plan { int tt, ft; bool cast_inside; int lds_rows; int stages; };
 constexpr int FEW_BLOCKS = 160;
 
 Plan plan_of(bool swiglu, bool x16, int rows, int E, int rows_static, int K, int N) {
-  Plan p = {0, 0, false, 0};
+  Plan p = {0, 0, false, 0, 0};
   const int per = E > 0 ? (rows + E - 1) / E : 0, most = per > rows_static ? per : rows_static;   // rows of a segment, if they are even
   if (most <= 16) p.tt = 1;
   else if (most <= 32) p.tt = 2;
@@ -1072,6 +1126,8 @@ extern "C" int hdmoe_block_linear(const hdmoe_block_args* p, hdmoe_stream_t stre
   if (args.op[0].rows + (long long)args.op[1].rows == 0) return HDMOE_OK;
   const bool bf16 = p->out_dtype == HDMOE_W_BF16;
   if (plan.tt > 0) return bf16 ? launch_few<HdmoeBf16, false>(args, plan, what, s) : launch_few<HdmoeF16, false>(args, plan, what, s);
+  if (plan.stages == 2) return bf16 ? launch_gemm<HdmoeBf16, false, 2>(args, what, s) : launch_gemm<HdmoeF16, false, 2>(args, what, s);
+  if (plan.stages == 4) return bf16 ? launch_gemm<HdmoeBf16, false, 4>(args, what, s) : launch_gemm<HdmoeF16, false, 4>(args, what, s);
   return bf16 ? launch_gemm8<HdmoeBf16, false>(args, what, s) : launch_gemm8<HdmoeF16, false>(args, what, s);
 }
 
@@ -1086,5 +1142,6 @@ extern "C" int hdmoe_block_swiglu(const hdmoe_block_args* p, hdmoe_stream_t stre
     if (int rc = p->a_dtype == HDMOE_W_F16 ? launch_few<HdmoeF16, true>(args, plan, what, s) : launch_few<HdmoeBf16, true>(args, plan, what, s)) return rc;
     return launch_cast(args, what, s);
   }
+  if (plan.stages > 0) return launch_gemm<HdmoeBf16, true, 3>(args, what, s);
   return launch_gemm8<HdmoeBf16, true>(args, what, s);
 }
