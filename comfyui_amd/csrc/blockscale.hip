@@ -9,6 +9,7 @@
 // fp32 once. 2^-96 keeps both quotients normal numbers. The maximum is taken on the bit patterns, where NaN orders above every
 // number: a block that holds NaN becomes NaN, as does one that holds an infinity (0 * inf).
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -206,7 +207,7 @@ __device__ __forceinline__ BiasWords load_bias(const Operand& op, const Group& g
 template <class Act, bool SWIGLU, int BM, int WF, int FT, int TT, class Acc>
 __device__ __forceinline__ void store_tile(const Operand& op, const BiasWords& bias, const Tile& t, uint8_t* exchange, int wf, int wt, int lane, Acc acc) {
   const int N = op.N, quad = lane >> 4;
-  constexpr int OUTSIDE = (int)0x80000000u;
+  constexpr int OUTSIDE = (int)0x80000000u, WT = BM / (TT * 16);
   if constexpr (!SWIGLU) {
     const int f0 = t.n0 + wf * FT * 16 + quad * 8;    // eight features from f0 + 32 c on
     // rows of the tile; what lies past its rows or features gets an offset past the buffer and is not written
@@ -217,7 +218,7 @@ __device__ __forceinline__ void store_tile(const Operand& op, const BiasWords& b
       const u32x4 b = bias.w[c];
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt) {
-        const int r = wt * TT * 16 + tt * 16 + (lane & 15);
+        const int r = (tt * WT + wt) * 16 + (lane & 15);
         u32x4 v;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = Act::pack(acc(2 * c + i / 2, tt, i % 2 * 2) + Act::lo(b[i]), acc(2 * c + i / 2, tt, i % 2 * 2 + 1) + Act::hi(b[i]));
@@ -243,7 +244,7 @@ __device__ __forceinline__ void store_tile(const Operand& op, const BiasWords& b
         }
       top[tt] = max(top[tt], (uint32_t)__shfl_xor((int)top[tt], 16, 64));
       top[tt] = max(top[tt], (uint32_t)__shfl_xor((int)top[tt], 32, 64));
-      if (quad == 0) tops[wf * BM + wt * TT * 16 + tt * 16 + lane] = top[tt];
+      if (quad == 0) tops[wf * BM + (tt * WT + wt) * 16 + lane] = top[tt];
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
     const int f0 = t.n0 + wf * FT * 8 + quad * FT * 2;
@@ -251,7 +252,7 @@ __device__ __forceinline__ void store_tile(const Operand& op, const BiasWords& b
     const __amdgpu_buffer_rsrc_t outs = make_rsrc(op.s_out + (size_t)(t.n0 / BLK) * op.ld_out + t.row0, (uint32_t)t.rows_here * 4u);
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
-      const int r = wt * TT * 16 + tt * 16 + (lane & 15);
+      const int r = (tt * WT + wt) * 16 + (lane & 15);
 #pragma unroll
       for (int w = 1; w < WF; ++w) top[tt] = max(top[tt], tops[(wf + w) % WF * BM + r]);
       const float both = __uint_as_float(top[tt]);
@@ -340,10 +341,15 @@ __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_
     const int w = p / (FT * 16), f = w * (SWIGLU ? FT * 8 : FT * 16) + tile_feature<SWIGLU, FT>(p / 16 % FT, p & 15);
     vb[j] = f < feats ? f * K + ld_chunk * 16 : OUTSIDE;
   }
-  // scales of the tile's tokens: one word a lane, 64 tokens a wave (the waves past them ask for none); they go through LDS as well
+  // Scales go through LDS as well, 64 words a wave: of the tile's tokens, and (one value for all lanes) of the weight block by wave 7,
+  // gate/up: of w3's by wave 6. The other waves ask for none. (Scalar loads return out of order with LDS reads, and a wait for one is a
+  // wait for all.)
   const int ld_s = __builtin_amdgcn_readfirstlane((int)op.ld_sa * 4);
-  const __amdgpu_buffer_rsrc_t rs = make_rsrc(op.sa, (uint32_t)(KB - 1) * (uint32_t)ld_s + (uint32_t)a_rows * 4u);
-  int tok = OUTSIDE;
+  const bool of_w = wave == 7 || (SWIGLU && wave == 6);
+  const float* const sw = (SWIGLU && wave == 6 ? grp.s1 : grp.s0) + (size_t)(t.n0 / BLK) * KB;
+  const __amdgpu_buffer_rsrc_t rs = of_w ? make_rsrc(sw, (uint32_t)KB * 4u) : make_rsrc(op.sa, (uint32_t)(KB - 1) * (uint32_t)ld_s + (uint32_t)a_rows * 4u);
+  const int s_step = __builtin_amdgcn_readfirstlane(of_w ? 4 : ld_s);
+  int tok = of_w ? 0 : OUTSIDE;
   {
     const int r = wave * 64 + lane;
     if (r < t.rows_here && r < BM) {
@@ -351,31 +357,33 @@ __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_
       if ((unsigned)from < (unsigned)a_rows) tok = from * 4;
     }
   }
+  static_assert(BM <= 6 * 64, "waves 6 and 7 load the weights' scales");
   // The loads are written by hand so that the compiler, which takes any of them for one that a later LDS read may want, does not wait.
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
   auto to_lds = [](const __amdgpu_buffer_rsrc_t& r, uint32_t lds, int voff, int soff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
   };
-  auto issue = [&](int stage, int kb) {
-    const uint32_t sa = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + wave * 8 * BLK), sb = sa + BM * BLK;
+  // load i of the step kb into `stage`
+  auto load = [&](int i, int stage, int kb) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + wave * 8 * BLK);
     const int k0 = kb * BLK;
     const int mask = k0 + ld_chunk * 16 < K ? 0 : OUTSIDE;   // (none past the last step)
-#pragma unroll
-    for (int j = 0; j < LA; ++j) to_lds(ra, sa + j * ROWS_PER_LOAD * BLK, va[j] | mask, k0);
-#pragma unroll
-    for (int j = 0; j < LB; ++j) {
-      if (upper(j)) to_lds(rb1, sb + j * ROWS_PER_LOAD * BLK, vb[j] | mask, k0);
-      else to_lds(rb0, sb + j * ROWS_PER_LOAD * BLK, vb[j] | mask, k0);
+    if (i < LA) {
+      to_lds(ra, at + i * ROWS_PER_LOAD * BLK, va[i] | mask, k0);
+    } else if (i < LA + LB) {
+      const int j = i - LA;
+      if (upper(j)) to_lds(rb1, at + (BM + j * ROWS_PER_LOAD) * BLK, vb[j] | mask, k0);
+      else to_lds(rb0, at + (BM + j * ROWS_PER_LOAD) * BLK, vb[j] | mask, k0);
+    } else {
+      const uint32_t ss = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + (BM + BN) * BLK + wave * 256);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(ss), "v"(tok), "s"(rs), "s"(min(kb, KB - 1) * s_step) : "memory");
     }
-    const uint32_t ss = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + (BM + BN) * BLK + wave * 256);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(ss), "v"(tok), "s"(rs), "s"(min(kb, KB - 1) * ld_s) : "memory");
   };
   constexpr int LOADS = LA + LB + 1;
-
-  // the weight block's scales come by scalar loads, a step ahead
-  typedef const __attribute__((address_space(4))) float* const_float_ptr;
-  const const_float_ptr sw0 = (const_float_ptr)(uintptr_t)(grp.s0 + (size_t)(t.n0 / BLK) * KB);
-  const const_float_ptr sw1 = SWIGLU ? (const_float_ptr)(uintptr_t)(grp.s1 + (size_t)(t.n0 / BLK) * KB) : sw0;
+  auto issue = [&](int stage, int kb) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(i, stage, kb);
+  };
 
   const int fr = lane & 15, fs = swz(fr), c0 = lane >> 4;
   v4f acc[FT][TT];
@@ -383,25 +391,41 @@ __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_
   for (int f = 0; f < FT; ++f)
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) acc[f][tt] = v4f{0, 0, 0, 0};
-  auto frag = [&](const uint8_t* row) -> v8i {
-    const v4i lo = *reinterpret_cast<const v4i*>(row + ((c0 ^ fs) << 4)), hi = *reinterpret_cast<const v4i*>(row + (((c0 + 4) ^ fs) << 4));
-    return v8i{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-  };
-  // what a wave reads of a step
+  // What a wave reads of a step. The addresses are those of the step's stage and move on in place: formed anew for every read they take
+  // registers that reads on their way are still to fill, and each of those is waited for.
   struct Step { v8i a[FT], b[TT]; float x[TT], s0, s1; };
-  auto read = [&](Step& st, int stage, int kb) {
-    const uint8_t* const base = smem + stage * STAGE;
-    const float* const sx = reinterpret_cast<const float*>(base + (BM + BN) * BLK) + wt * TT * 16 + fr;
+  typedef const __attribute__((address_space(3))) v4i* lds_v4i;
+  typedef const __attribute__((address_space(3))) float* lds_float;
+  uint32_t at_a[2], at_b[2], at_x = lds0 + (BM + BN) * BLK + (wt * 16 + fr) * 4, at_s = lds0 + (BM + BN) * BLK + lane * 4;
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) st.x[tt] = sx[tt * 16];
+  for (int h = 0; h < 2; ++h) {
+    const int c = ((c0 + 4 * h) ^ fs) << 4;
+    at_b[h] = lds0 + (wt * 16 + fr) * BLK + c;
+    at_a[h] = lds0 + (BM + wf * FT * 16 + fr) * BLK + c;
+  }
+  int stage = 0;
+  auto read = [&](Step& st) {
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) st.b[tt] = frag(base + (wt * TT * 16 + tt * 16 + fr) * BLK);
+    for (int tt = 0; tt < TT; ++tt) st.x[tt] = *(lds_float)(at_x + tt * WT * 64);
+    st.s0 = *(lds_float)(at_s + 7 * 256);
+    st.s1 = SWIGLU ? *(lds_float)(at_s + 6 * 256) : 0.0f;
+    auto frag = [&](const uint32_t (&at)[2], int off) -> v8i {
+      const v4i lo = *(lds_v4i)(at[0] + off), hi = *(lds_v4i)(at[1] + off);
+      return v8i{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    };
 #pragma unroll
-    for (int f = 0; f < FT; ++f) st.a[f] = frag(base + (BM + wf * FT * 16 + f * 16 + fr) * BLK);
-    st.s0 = sw0[kb];
-    st.s1 = SWIGLU ? sw1[kb] : 0.0f;
+    for (int tt = 0; tt < TT; ++tt) st.b[tt] = frag(at_b, tt * WT * 16 * BLK);
+#pragma unroll
+    for (int f = 0; f < FT; ++f) st.a[f] = frag(at_a, f * 16 * BLK);
+    const int on = stage + 1 == STAGES ? -(STAGES - 1) * STAGE : STAGE;
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    at_x += on;
+    at_s += on;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) { at_a[h] += on; at_b[h] += on; }
   };
-  auto multiply = [&](const Step& st) {
+  // (with one block on a CU the loads go between the MFMAs: a burst of them in front keeps the waves at the memory queue)
+  auto multiply = [&](const Step& st, int next, int kb) {
     v4f p[2][TT];
     float m0[TT], m1[TT];
 #pragma unroll
@@ -417,6 +441,9 @@ __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_
 #pragma unroll
       for (int tt = 0; tt < TT; ++tt) p[f & 1][tt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(st.a[f], st.b[tt], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = f * LOADS / FT; i < (f + 1) * LOADS / FT; ++i)
+        if (STAGES > 2) load(i, next, kb);
       if (f > 0) join(f - 1);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -426,35 +453,34 @@ __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_
 
 #pragma unroll
   for (int st = 0; st < STAGES - 1; ++st) issue(st, st);
-  int next = STAGES - 1, stage = 0;
+  int next = STAGES - 1;
   if constexpr (STAGES == 2) {
     for (int kb = 0; kb < KB; ++kb) {
       asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
       Step st;
-      read(st, stage, kb);
+      read(st);
       issue(next, kb + 1);
-      stage = next;
       next = ring(next);
-      multiply(st);
+      multiply(st, 0, KB);
     }
   } else {
     // a step's operands are read while the one before is multiplied
     Step st[2];
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((STAGES - 2) * LOADS) : "memory");
-    read(st[0], 0, 0);
-    for (int kb = 0; kb < KB; kb += 2) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (kb + i < KB) {
-          asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((STAGES - 3) * LOADS) : "memory");
-          stage = ring(stage);
-          read(st[1 - i], stage, min(kb + i + 1, KB - 1));
-          issue(next, kb + i + STAGES - 1);
-          next = ring(next);
-          multiply(st[i]);
-        }
-      }
+    read(st[0]);
+    auto step = [&](Step& here, Step& there, int kb) {
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"((STAGES - 3) * LOADS) : "memory");
+      read(there);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(here, next, kb + STAGES - 1);
+      next = ring(next);
+    };
+    int kb = 0;
+    for (; kb + 2 <= KB; kb += 2) {
+      step(st[0], st[1], kb);
+      step(st[1], st[0], kb + 1);
     }
+    if (kb < KB) step(st[0], st[1], kb);
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");   // LDS is read and written no more
   store_tile<Act, SWIGLU, BM, WF, FT, TT>(op, SWIGLU ? BiasWords{} : load_bias<FT>(op, grp, t, wf, lane), t, smem, wf, wt, lane,
@@ -544,7 +570,7 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
       }
       const int f = (r >> 7) * (SWIGLU ? 64 : 128) + tile_feature<SWIGLU, 8>(r / 16 % 8, r & 15);
       vb[j] = f < feats ? f * K + ld_chunk * 16 : OUTSIDE;
-      const int x = wt * 64 + j * 16 + (lane & 15);
+      const int x = (j * 4 + wt) * 16 + (lane & 15);
       if (x < t.rows_here) {
         const int from = gather != nullptr ? gather[t.row0 + x] >> 1 : t.row0 + x;
         if ((unsigned)from < (unsigned)a_rows) tok[j] = from * 4;
@@ -578,7 +604,7 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = ((quad + 4 * h) ^ fs) * 16;
-      addr[h] = (int)lds0 + (wt * 64 + fr) * BLK + c;
+      addr[h] = (int)lds0 + (wt * 16 + fr) * BLK + c;
       addr[2 + h] = (int)lds0 + 65536 + (wf * 128 + fr) * BLK + c;
     }
     return s;
@@ -609,7 +635,7 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
                         "+{v[26:29]}"(sx), "+{v30}"(sw[0]), "+{v31}"(sw[1]), "+{v8}"(tail), "+{v[10:13]}"(addr), "+{v[18:21]}"(va), "+{v[22:25]}"(vb), \
                         [n] "+s"(n), [left] "+s"(left), [so] "+s"(so), [ss] "+s"(ss), [sw] "+s"(so_w), [ws] "+s"(ws) \
                       : "{v[14:17]}"(tok), [ra] "s"(src.ra), [rb0] "s"(src.rb0), [rb1] "s"(src.rb1), [rs] "s"(src.rs), [rw0] "s"(src.rw0), [rw1] "s"(src.rw1), \
-                        [ssi] "s"(src.ld_s), [ldsw] "s"(ldsw), [steps] "s"(src.KB) \
+                        [ssi] "s"(src.ld_s), [ldsw] "s"(ldsw), [steps] "s"(src.KB), [nt] "s"((cur.rows_here + 63) / 64) \
                       : "memory", "scc", "s60", "s61", "s62")
     if constexpr (SWIGLU) HDMOE_BLOCK_LOOP(HDMOE_BLOCK_SWIGLU);
     else HDMOE_BLOCK_LOOP(HDMOE_BLOCK_PLAIN);
@@ -947,29 +973,80 @@ extern "C" int hdmoe_quant_block_fp8(int src_dtype, const void* x, int64_t rows,
 
 namespace {
 
-// How a call runs: the few-row kernels on tiles of 16 * tt rows and 16 * ft features (tt > 0; with the cast inside or not), or the tiles
-// of block_gemm8_kernel.
+// How a call runs: the few-row kernels on tiles of 16 * tt rows and ft strips (tt > 0; with the cast inside or not), block_gemm_kernel with
+// `stages` K steps in LDS (stages > 0), or block_gemm8_kernel.
 struct Plan { int tt, ft; bool cast_inside; int lds_rows; int stages; };
-constexpr int FEW_BLOCKS = 160;
 
-Plan plan_of(bool swiglu, bool x16, int rows, int E, int rows_static, int K, int N) {
-  Plan p = {0, 0, false, 0, 0};
-  const int per = E > 0 ? (rows + E - 1) / E : 0, most = per > rows_static ? per : rows_static;   // rows of a segment, if they are even
-  if (most <= 16) p.tt = 1;
-  else if (most <= 32) p.tt = 2;
-  else if (most <= 64) p.tt = 4;
-  if (p.tt == 0) return p;
-  if (x16) {
-    // a block casts for itself where that takes its threads a few trips at most
-    const int whole = rows > rows_static ? rows : rows_static;
-    p.lds_rows = whole < 16 ? whole : 16;
-    p.cast_inside = p.tt == 1 && (long long)p.lds_rows * ((K + BLK - 1) / BLK) * 16 <= 4 * 512;
+// What a launch is likely to take in microseconds, by what the kernels measured over 1 to 16384 rows of 2560 and 6912 wide Linears. Where the
+// segments end is not known here; on average half a tile of each is empty.
+struct Sizes { int rows, E, rows_static, K, N, K_static, N_static; };
+double tiles_of(const Sizes& z, int bm, int feat) {   // in tiles of the experts' K
+  double t = 0;
+  if (z.rows > 0) {
+    const int n = z.E < z.rows ? z.E : z.rows;
+    const double m = z.E == 1 ? (double)((z.rows + bm - 1) / bm) : (double)z.rows / bm + 0.5 * n;
+    t += (m > n ? m : n) * ((z.N + feat - 1) / feat);
   }
-  // as many features a block as leave most CUs one
-  const long long strips = (long long)((E > 0 ? (E < rows ? E : rows) : 0) + (rows_static > 0 ? 1 : 0)) * (N / 16) * (swiglu ? 2 : 1);
-  p.ft = p.tt == 4 ? 2 : 4;
-  while (p.ft > (swiglu ? 2 : 1) && strips < (long long)FEW_BLOCKS * p.ft) p.ft >>= 1;
-  return p;
+  if (z.rows_static > 0) {
+    const double share = z.rows > 0 ? (double)z.K_static / z.K : 1.0;
+    t += (double)((z.rows_static + bm - 1) / bm) * ((z.N_static + feat - 1) / feat) * share;
+  }
+  return t;
+}
+// Few rows. A CU runs one block at a time, 2.5 us to its first operands and then 39 KB/us of weights and activations (1 x 6912 x 2560: 8.2, 11.1
+// and 17.5 us with 1, 2 and 4 strips a block; 16 rows 10.4, 13.3, 19.6).
+double few_us(const Sizes& z, bool swiglu, int tt, int ft) {
+  const double blocks = tiles_of(z, 16 * tt, swiglu ? 8 * ft : 16 * ft);
+  const int per = z.rows > 0 ? (z.rows + z.E - 1) / z.E : 0, most = per > z.rows_static ? per : z.rows_static;
+  const int rows = most < 16 * tt ? most : 16 * tt, K = z.rows > 0 ? z.K : z.K_static;
+  const double rounds = ceil(blocks / HDMOE_NUM_CU);
+  return 2.7 + rounds * (2.5 + (16.0 * ft + rows) * K / 39e3) + (swiglu ? 3.5 : 0.0);
+}
+// Low tiles. 128 x 6912 x 2560: 32.7 us with four stages (two 41.6), where a step lasts half as long as memory's answer; from a block for every CU on
+// two blocks share one (1024 x 2560 x 6912: 32.6 against 25.8).
+double low_us(const Sizes& z, bool swiglu, int stages) {
+  const double t = tiles_of(z, swiglu ? 64 : 128, BLK), kb = ((z.rows > 0 ? z.K : z.K_static) + BLK - 1) / BLK;
+  if (stages > 2) return 5.0 + ceil(t / HDMOE_NUM_CU) * (2.0 + kb * (swiglu ? 0.82 : 0.5));
+  const double over = t <= HDMOE_NUM_CU ? 0.0 : t >= 2 * HDMOE_NUM_CU ? 1.0 : t / HDMOE_NUM_CU - 1.0;
+  return 5.0 + (t > 2 * HDMOE_NUM_CU ? 1.1 * t / (2 * HDMOE_NUM_CU) : 1.0) * kb * (0.63 + 0.45 * over);
+}
+// Tiles of 256 x 256: a step lasts 1.05 us with few blocks and 1.5 with one on every CU, where the clock falls.
+double high_us(const Sizes& z, bool swiglu) {
+  const double t = tiles_of(z, 256, swiglu ? 128 : 256), kb = ((z.rows > 0 ? z.K : z.K_static) + BLK - 1) / BLK;
+  const double rounds = ceil(t / HDMOE_NUM_CU), full = t < HDMOE_NUM_CU ? t / HDMOE_NUM_CU : 1.0;
+  return 4.0 + rounds * (5.0 + kb * (1.05 + 0.4 * full));
+}
+
+Plan plan_of(bool swiglu, bool x16, const Sizes& z) {
+  Plan best = {0, 0, false, 0, 0};
+  double us = high_us(z, swiglu);
+  auto offer = [&](double t, const Plan& p) {
+    if (t < us) {
+      us = t;
+      best = p;
+    }
+  };
+  if (swiglu) {
+    offer(low_us(z, true, 3), Plan{0, 0, false, 0, 3});
+  } else {
+    offer(low_us(z, false, 4), Plan{0, 0, false, 0, 4});
+    offer(low_us(z, false, 2), Plan{0, 0, false, 0, 2});
+  }
+  const int K = z.rows > 0 ? z.K : z.K_static;
+  for (int tt = 1; tt <= 4; tt *= 2)
+    for (int ft = swiglu ? 2 : 1; ft <= (tt == 4 ? 2 : 4); ft *= 2) {
+      Plan p = {tt, ft, false, 0, 0};
+      double t = few_us(z, swiglu, tt, ft);
+      if (x16 && tt == 1) {
+        // a block casts for itself where that takes its threads a few trips at most: a launch (4 us) less
+        const int whole = z.rows > z.rows_static ? z.rows : z.rows_static;
+        p.lds_rows = whole < 16 ? whole : 16;
+        p.cast_inside = (long long)p.lds_rows * ((K + BLK - 1) / BLK) * 16 <= 4 * 512;
+        if (p.cast_inside) t -= 4.0;
+      }
+      offer(t, p);
+    }
+  return best;
 }
 
 size_t cast_bytes(long long rows, int K) { return hdmoe_align_up((size_t)rows * K, 256) + hdmoe_align_up((size_t)rows * ((K + BLK - 1) / BLK) * 4, 256); }
@@ -1050,7 +1127,7 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
   const int a_rows = routed ? args.op[0].a_rows : p->rows_static, K = routed ? p->K : p->K_static;
   if (x16 && routed && p->rows_static > 0 && (p->fixed.a != p->routed.a || p->rows_static != a_rows || p->K_static != K))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: 16-bit activations of the experts and of the static group must be the same rows", what);
-  plan = plan_of(swiglu, x16, routed ? p->rows : 0, routed ? p->E : 0, p->rows_static, K, routed ? p->N : p->N_static);
+  plan = plan_of(swiglu, x16, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, p->N, p->K_static, p->N_static});
   args.lds_rows = plan.lds_rows;
   const size_t need = work_bytes(swiglu, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K,
                                  routed ? p->N : 0, p->rows_static > 0 ? p->N_static : 0);
@@ -1113,7 +1190,7 @@ extern "C" size_t hdmoe_block_workspace_bytes(const hdmoe_block_args* p, int swi
   if (!routed && p->rows_static == 0) return 0;
   const int K = routed ? p->K : p->K_static, N = routed ? p->N : 0, Ns = p->rows_static > 0 ? p->N_static : 0;
   if (K <= 0 || N < 0 || Ns < 0) return 0;
-  const Plan plan = plan_of(swiglu != 0, x16, routed ? p->rows : 0, routed ? p->E : 0, p->rows_static, K, routed ? N : Ns);
+  const Plan plan = plan_of(swiglu != 0, x16, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, N, p->K_static, Ns});
   return work_bytes(swiglu != 0, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K, N, Ns);
 }
 

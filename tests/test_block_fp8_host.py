@@ -91,8 +91,8 @@ def test_contraction_refuses_pointers(which):
         a.experts[0].weight3 = None
         assert f(ctypes.byref(a), None) == L.E_NULL
     # 16-bit rows: room for their cast where the contraction does not make it, and the same rows for both groups
-    many = dict(a_dtype=L.W_BF16, rows=640, routed=L.BlockRows(p, None, 0, p, p, 640))
-    assert L.lib.hdmoe_block_workspace_bytes(ctypes.byref(arguments(p, **many)), which == "swiglu") == 640 * 128 + 640 * 4
+    many = dict(a_dtype=L.W_BF16, rows=25600, routed=L.BlockRows(p, None, 0, p, p, 25600))
+    assert L.lib.hdmoe_block_workspace_bytes(ctypes.byref(arguments(p, **many)), which == "swiglu") == 25600 * 128 + 25600 * 4
     assert f(ctypes.byref(arguments(p, **many)), None) == L.E_WORKSPACE
     assert f(ctypes.byref(arguments(p, **many, workspace=p + 1, workspace_bytes=1 << 20)), None) == L.E_WORKSPACE
     a = arguments(p, a_dtype=L.W_BF16, rows_static=4, K_static=128, N_static=128, fixed=L.BlockRows(p + 256, None, 0, p, p, 4))
