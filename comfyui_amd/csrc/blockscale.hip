@@ -1010,11 +1010,13 @@ double low_us(const Sizes& z, bool swiglu, int stages) {
   const double over = t <= HDMOE_NUM_CU ? 0.0 : t >= 2 * HDMOE_NUM_CU ? 1.0 : t / HDMOE_NUM_CU - 1.0;
   return 5.0 + (t > 2 * HDMOE_NUM_CU ? 1.1 * t / (2 * HDMOE_NUM_CU) : 1.0) * kb * (0.63 + 0.45 * over);
 }
-// Tiles of 256 x 256: a step lasts 1.05 us with few blocks and 1.5 with one on every CU, where the clock falls.
+// Tiles of 256 x 256: a step lasts 0.49, 0.63, 0.85 or 1.07 us with 1 to 4 parts of 64 rows, and 1.5 where every CU multiplies a full one: the clock
+// falls.
 double high_us(const Sizes& z, bool swiglu) {
-  const double t = tiles_of(z, 256, swiglu ? 128 : 256), kb = ((z.rows > 0 ? z.K : z.K_static) + BLK - 1) / BLK;
+  const int feat = swiglu ? 128 : 256;
+  const double t = tiles_of(z, 256, feat), parts = tiles_of(z, 64, feat), kb = ((z.rows > 0 ? z.K : z.K_static) + BLK - 1) / BLK;
   const double rounds = ceil(t / HDMOE_NUM_CU), full = t < HDMOE_NUM_CU ? t / HDMOE_NUM_CU : 1.0;
-  return 4.0 + rounds * (5.0 + kb * (1.05 + 0.4 * full));
+  return 4.0 + rounds * (5.0 + kb * (0.3 + (0.19 + 0.1 * full) * parts / t));
 }
 
 Plan plan_of(bool swiglu, bool x16, const Sizes& z) {
