@@ -9,6 +9,8 @@ Follows the reference's conventions:
   * on saving, a scaled model carries an empty marker of its storage dtype (comfy/model_base.py:326-327).
   * Linear keys `<layer>.{shared_experts,experts.N}.{w1,w2,w3}.{weight,scale_weight,scale_input}` and
     `<layer>.gate.weight` (comfy/ldm/hidream/model.py:233-235, 255, 297-304).
+  * weights with a scale for each 128 x 128 block (not in the reference): `scale_weight` is a matrix instead of a scalar; the
+    operations class is then ops.block_fp8_ops, whatever the marker says of `scale_input`.
   * files are opened with safetensors' own reader, tensor by tensor, onto the target device
     (comfy/utils.py:53-66); nothing is unpickled.
 """
@@ -138,9 +140,13 @@ def load_moe_layers(source, prefix="", device=None, compute_dtype=torch.bfloat16
         if weight_dtype is None and shapes:
             first = next(iter(shapes))
             weight_dtype = get(f"{first}.experts.0.w1.weight").dtype
+        block_scales = False
+        if shapes and weight_dtype == FP8:
+            scale = f"{next(iter(shapes))}.experts.0.w1.scale_weight"
+            block_scales = scale in available and get(scale).dim() == 2
         operations = amd_ops.pick_operations(weight_dtype, compute_dtype, load_device=device if device.type == "cuda" else None,
                                              fp8_optimizations=fp8_opt, scaled_fp8=scaled_fp8,
-                                             fast_fp8_matrix_mult=fast_fp8_matrix_mult)
+                                             fast_fp8_matrix_mult=fast_fp8_matrix_mult, block_scales=block_scales)
         modules = {}
         for layer, shp in shapes.items():
             if layers is not None and layer not in layers:

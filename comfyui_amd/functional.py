@@ -803,3 +803,27 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
                 f.scale_out, f.scale_out_stride = sh_shared.data_ptr(), T
         _block_call(lib.hdmoe_block_swiglu, 1, args, a)
     return (h, sh) if shared is None else (h, sh, h_shared, sh_shared)
+
+
+def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None):
+    """First half of one dense SwiGLU feed-forward, silu(x w1^T) * (x w3^T), cast as quant_block_fp8 does: x and scale_x as in
+    linear_block_fp8 -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]), what linear_block_fp8 takes for w2."""
+    what = "swiglu_block_fp8"
+    s = _block_rows(x, scale_x, what + " x")
+    rows, K = x.shape
+    dev = x.device
+    w = _lib.BlockWeights()
+    H = _block_weights(w, (w1, scale_w1, w3, scale_w3), K, None, x.get_device(), what)[0][0]
+    with _on(dev):
+        h = torch.empty((rows, H), dtype=FP8, device=dev)
+        sh = block_scales(rows, H, dev)
+        if rows > 0:
+            args = _lib.BlockArgs()
+            args.a_dtype, args.out_dtype = _ACT_CODE[x.dtype], W_BF16
+            args.rows_static, args.K_static, args.N_static = rows, K, H
+            args.shared = ctypes.pointer(w)
+            f = args.fixed
+            f.a, f.scale_a, f.scale_a_stride, f.out = x.data_ptr(), ptr(s), rows, h.data_ptr()
+            f.scale_out, f.scale_out_stride = sh.data_ptr(), rows
+            _block_call(lib.hdmoe_block_swiglu, 1, args, x)
+    return h, sh

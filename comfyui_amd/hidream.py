@@ -12,7 +12,8 @@ key maps and checkpoints address.
 
 MOEFeedForwardSwiGLU.forward enqueues the whole layer through ONE library call when all
 Linears share a supported storage dtype (bf16, or float8_e4m3fn with fp8 matrix multiply or multiplied
-in bf16); otherwise it composes the same HIP stages per expert through the Linear modules, which
+in bf16). Linears with a scale for each block of 128 (ops.block_fp8_ops) run as two launches for all experts
+and the shared one between gate, dispatch and combine. Otherwise it composes the same HIP stages per expert through the Linear modules, which
 needs the per-expert row counts on the host (one sync, as the reference's mask indexing).
 Inputs must be bf16 HIP tensors: there is no CPU path.
 """
@@ -189,6 +190,18 @@ def _gate_weight(gate, hidden_states):
     return amd_ops.cast_to(gate.weight, dtype=hidden_states.dtype, device=hidden_states.device).contiguous()
 
 
+def _block_parts(ffns, x):
+    """([gate/up entries], [down entries]) of feed-forwards whose Linears all carry a scale for each block of 128
+    (functional.grouped_swiglu_block_fp8 and grouped_linear_block_fp8), or None."""
+    if not isinstance(ffns[0].w1, amd_ops.block_fp8_ops.Linear) or any(type(f).forward is not FeedForwardSwiGLU.forward or _observed(f) for f in ffns):
+        return None
+    parts = amd_ops.block_fp8_parts([l for f in ffns for l in (f.w1, f.w3, f.w2)], x)
+    if parts is None or any(b is not None for i, (_, _, b) in enumerate(parts) if i % 3 != 2):
+        return None   # gate/up has no bias
+    one, three, two = parts[0::3], parts[1::3], parts[2::3]
+    return [(w1, s1, w3, s3) for (w1, s1, _), (w3, s3, _) in zip(one, three)], two
+
+
 class FeedForwardSwiGLU(nn.Module):
     def __init__(self, dim: int, hidden_dim: int, multiple_of: int = 256,
                  ffn_dim_multiplier: Optional[float] = None, dtype=None, device=None, operations=None):
@@ -217,7 +230,23 @@ class FeedForwardSwiGLU(nn.Module):
         del keep
         return y.view(*x.shape[:-1], self.w2.weight.shape[0])
 
+    def _block(self, x):
+        """The feed-forward of Linears with block scales, or None."""
+        if not isinstance(self.w1, amd_ops.block_fp8_ops.Linear):
+            return None
+        got = _block_parts([self], x)
+        if got is None:
+            return None
+        x2 = x.reshape(-1, x.shape[-1]).contiguous()
+        h, sh = HF.swiglu_block_fp8(x2, *got[0][0])
+        w, s, b = got[1][0]
+        return HF.linear_block_fp8(h, w, s, bias=b, scale_x=sh, out_dtype=x.dtype).view(*x.shape[:-1], w.shape[0])
+
     def forward(self, x):
+        if x.is_cuda and x.dtype in HF.ACT_DTYPES:
+            y = self._block(x)
+            if y is not None:
+                return y
         if x.is_cuda and x.dtype == BF16:
             y = self._fused(x, HF.ffn_swiglu)
             if y is not None:
@@ -356,6 +385,9 @@ class MOEFeedForwardSwiGLU(nn.Module):
         orig_shape = x.shape
         x2 = x.reshape(-1, orig_shape[-1]).contiguous()
         gate_w = _gate_weight(self.gate, x2)
+        parts = _block_parts([*self.experts, self.shared_experts], x2)
+        if parts is not None:
+            return self._forward_block(x2, gate_w, *parts).view(*orig_shape)
         got = self._one_call(x2)
         if got is not None:
             wdt, experts, shared, keep, H, Hs = got
@@ -379,6 +411,10 @@ class MOEFeedForwardSwiGLU(nn.Module):
         x2 = x.reshape(-1, D).contiguous()
         mods = tuple(m.reshape(B, D).contiguous() for m in (shift, scale, gate))
         gate_w = _gate_weight(self.gate, x2)
+        parts = _block_parts([*self.experts, self.shared_experts], x2)
+        if parts is not None:
+            n = HF.ln_modulate(x2, mods[1], mods[0], S, eps)
+            return self._forward_block(n, gate_w, *parts, gated_residual=(mods[2], x2, S)).view(B, S, D)
         got = self._one_call(x2)
         if got is not None:
             wdt, experts, shared, keep, H, Hs = got
@@ -390,6 +426,22 @@ class MOEFeedForwardSwiGLU(nn.Module):
             return y.view(B, S, D)
         n = HF.ln_modulate(x2, mods[1], mods[0], S, eps)
         return self._forward_composed(n, gate_w, gated_residual=(mods[2], x2, S)).view(B, S, D)
+
+    # ---- Linears with block scales -----------------------------------------------------
+
+    def _forward_block(self, x2, gate_w, gate_up, down, gated_residual=None):
+        """Gate, dispatch, the products of every expert and the shared one in two launches (with the cast in front, and on a few tokens
+        the one between them), combine: no host sync."""
+        idx, w = HF.gate_top2(x2, gate_w)
+        if getattr(self.gate, "norm_topk_prob", False):
+            w = HF.renorm_top2(w)
+        _, offsets, perm, inv_perm = HF.dispatch(idx, len(self.experts))
+        h, sh, hs, shs = HF.grouped_swiglu_block_fp8(x2, offsets, gate_up[:-1], perm=perm, shared=gate_up[-1])
+        y, ys = HF.grouped_linear_block_fp8(h, offsets, down[:-1], scale_a=sh, shared=down[-1], a_static=hs, scale_static=shs)
+        if gated_residual is not None:
+            g, res, per_batch = gated_residual
+            return HF.combine_gated_residual(y, inv_perm, w, ys, g, res, per_batch)
+        return HF.combine(y, inv_perm, w, ys)
 
     # ---- composed path -----------------------------------------------------------------
 

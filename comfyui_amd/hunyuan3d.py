@@ -14,9 +14,11 @@ HiDream combine forms. Inputs must be bf16 or fp16 HIP tensors (fp16 is what mod
 this model family on a device with fp16 support, supported_models_base.py:46): there is no CPU path. With fp16
 every tensor and every rounding point of the block is fp16; scaled-fp8 Linears take bf16 activations only.
 
-Two ways through the experts:
+Three ways through the experts:
   * every Linear a plain one of the activation dtype resident on the device (no weight function, no scale_weight):
     two grouped launches for all experts and the shared expert;
+  * every Linear one with a scale for each block of 128 (ops.block_fp8_ops): the same two products with casts in front
+    of them and the GELU between;
   * anything else the `operations` argument brings (scaled-fp8 Linears with or without the fp8 matrix multiply,
     manual-cast or offloaded weights, weight functions): one expert at a time through the Linear modules' own
     forward, the GELU as an elementwise kernel, with the same gate, dispatch and combine kernels around them.
@@ -136,6 +138,18 @@ def _stages(ff, x):
     return ff.stage_weights() if ff.fusable(x) else None
 
 
+def _block_parts(ffs, x):
+    """([first Linears], [second Linears]) of feed-forwards whose Linears carry a scale for each block of 128, as
+    functional.grouped_linear_block_fp8 takes them, or None."""
+    if any(type(f) is not FeedForward or type(f.net[0]) is not GELU for f in ffs):
+        return None
+    watched = [m for f in ffs for m in (f, f.net[0])]
+    if any(m.__dict__["_forward_hooks"] or m.__dict__["_forward_pre_hooks"] or "forward" in m.__dict__ for m in watched):
+        return None
+    parts = amd_ops.block_fp8_parts([l for f in ffs for l in (f.net[0].proj, f.net[2])], x)
+    return None if parts is None else (parts[0::2], parts[1::2])
+
+
 class MoEGate(nn.Module):
     def __init__(self, embed_dim, num_experts=16, num_experts_per_tok=2, aux_loss_alpha=0.01, device=None, dtype=None):
         super().__init__()
@@ -185,6 +199,12 @@ class MoEBlock(nn.Module):
         idx, w = HF.gate_top2(x2, gate_w)
         _, offsets, perm, inv_perm = HF.dispatch(idx, self.num_experts)
         stages = [_stages(f, x2) for f in (*self.experts, self.shared_experts)]
+        parts = _block_parts([*self.experts, self.shared_experts], x2) if stages[0] is None else None
+        if parts is not None:
+            first, second = parts
+            h, h_sh = HF.grouped_linear_block_fp8(x2, offsets, first[:-1], perm=perm, shared=first[-1], a_static=x2)
+            y, y_sh = HF.grouped_linear_block_fp8(HF.gelu(h), offsets, second[:-1], shared=second[-1], a_static=HF.gelu(h_sh))
+            return HF.combine(y, inv_perm, w, y_sh).view(*orig_shape)
         if any(v is None for v in stages):
             xs = HF.permute_bf16(x2, perm)
             y = torch.empty_like(xs)

@@ -376,6 +376,82 @@ def scaled_fp8_ops(fp8_matrix_mult=False, scale_input=False, override_dtype=None
     return scaled_fp8_op
 
 
+class block_fp8_ops(manual_cast):
+    """Operations class whose Linear weights are float8_e4m3fn with one fp32 scale for every 128 x 128 block
+    (`scale_weight` [ceil(out / 128), ceil(in / 128)]) and whose activations are cast with one for every 128 values of a row, as they
+    are. bf16 and fp16 activations; in_features and out_features multiples of 16. The reference's scaled-fp8 Linear has one scale for
+    a tensor (ops.py:379-428); hooks and attributes are those of that one."""
+    class Linear(manual_cast.Linear):
+        def __init__(self, *args, **kwargs):
+            dtype = kwargs.get("dtype")
+            kwargs["dtype"] = FP8
+            super().__init__(*args, **kwargs)
+            if self.bias is not None:   # stored in the model's type
+                self.bias = torch.nn.Parameter(torch.empty(self.out_features, dtype=BF16 if dtype in (None, FP8) else dtype,
+                                                           device=self.weight.device))
+
+        def reset_parameters(self):
+            if not hasattr(self, "scale_weight"):
+                n, k = self.weight.shape
+                self.scale_weight = torch.nn.parameter.Parameter(
+                    data=torch.ones((HF._blocks(n), HF._blocks(k)), device=self.weight.device, dtype=torch.float32), requires_grad=False)
+            return None
+
+        def parts(self, input):
+            """(weight, scales, bias) on the input's device, weight functions (LowVramPatch objects) applied to the stored weight."""
+            dev = input.device
+            if len(self.weight_function) == 0 and len(self.bias_function) == 0 and self.weight.device == dev and self.bias is None:
+                weight, bias = self.weight, None
+            else:
+                weight, bias = cast_bias_weight(self, input, dtype=FP8, bias_dtype=input.dtype)
+            return weight.contiguous(), self.scale_weight.to(dev).contiguous(), None if bias is None else bias.contiguous()
+
+        def forward_comfy_cast_weights(self, input):
+            weight, scale, bias = self.parts(input)
+            x2 = input.reshape(-1, input.shape[-1]).contiguous()
+            return HF.linear_block_fp8(x2, weight, scale, bias=bias).reshape(*input.shape[:-1], weight.shape[0])
+
+        def _spread(self, weight):
+            """scale_weight as one value per element, in the weight's dtype on its device."""
+            s = self.scale_weight.to(device=weight.device, dtype=weight.dtype)
+            n, k = weight.shape
+            return s.repeat_interleave(HF.BLOCK, 0)[:n].repeat_interleave(HF.BLOCK, 1)[:, :k]
+
+        def convert_weight(self, weight, inplace=False, **kwargs):
+            s = self._spread(weight)
+            if inplace:
+                weight *= s
+                return weight
+            return weight * s
+
+        def set_weight(self, weight, inplace_update=False, seed=None, return_weight=False, **kwargs):
+            from .float_round import stochastic_rounding
+            weight = weight / self._spread(weight)
+            if weight.is_cuda and weight.dtype in (torch.float32, BF16):
+                weight = HF.stochastic_round_e4m3fn(weight.contiguous(), None, seed or 0)
+            else:
+                weight = stochastic_rounding(weight, FP8, seed=seed)
+            if return_weight:
+                return weight
+            if inplace_update:
+                self.weight.data.copy_(weight)
+            else:
+                self.weight = torch.nn.Parameter(weight, requires_grad=False)
+
+
+def block_fp8_parts(linears, input):
+    """[(weight, scales, bias)] if every one of these is a block_fp8_ops.Linear whose call does nothing more than its class says (no hooks,
+    no forward of its own), so that their products can join others' launches; else None."""
+    for l in linears:
+        if not isinstance(l, block_fp8_ops.Linear):
+            return None
+        d, cls = l.__dict__, type(l)
+        if (d["_forward_hooks"] or d["_forward_pre_hooks"] or "forward" in d or cls.forward is not disable_weight_init.Linear.forward
+                or cls.forward_comfy_cast_weights is not block_fp8_ops.Linear.forward_comfy_cast_weights or l.weight.dtype != FP8):
+            return None
+    return [l.parts(input) for l in linears]
+
+
 def supports_fp8_compute(device=None):
     """model_management.supports_fp8_compute narrowed to this build's only target: true on a
     gfx950 HIP device (the reference enables fp8 ops for gfx950 with torch >= 2.7 and ROCm >= 6.4,
@@ -390,9 +466,12 @@ def supports_fp8_compute(device=None):
 
 
 def pick_operations(weight_dtype, compute_dtype, load_device=None, disable_fast_fp8=False, fp8_optimizations=False,
-                    scaled_fp8=None, fast_fp8_matrix_mult=False):
+                    scaled_fp8=None, fast_fp8_matrix_mult=False, block_scales=False):
     """ops.pick_operations policy. `fast_fp8_matrix_mult` stands for the reference's
-    `--fast fp8_matrix_mult` command-line switch (cli_args.py:142-148), which has no global here."""
+    `--fast fp8_matrix_mult` command-line switch (cli_args.py:142-148), which has no global here. `block_scales`: the
+    weights carry a scale for each 128 x 128 block (not in the reference)."""
+    if block_scales:
+        return block_fp8_ops
     fp8_compute = supports_fp8_compute(load_device)
     if scaled_fp8 is not None:
         return scaled_fp8_ops(fp8_matrix_mult=fp8_compute and fp8_optimizations, scale_input=fp8_optimizations,

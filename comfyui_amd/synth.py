@@ -35,6 +35,15 @@ def quantize_per_tensor(w_fp32):
     return (w_fp32 / s).to(FP8), s
 
 
+def quantize_per_block(w_fp32):
+    """One scale for each 128 x 128 block, amax/448 (fp32); W8 = (W / scale) -> float8_e4m3fn. Returns (W8, scales)."""
+    n, k = w_fp32.shape
+    pad = torch.nn.functional.pad(w_fp32, (0, -k % 128, 0, -n % 128))
+    blocks = pad.view(pad.shape[0] // 128, 128, pad.shape[1] // 128, 128)
+    s = (blocks.abs().amax((1, 3), keepdim=True).clamp_min(2.0 ** -96) / 448.0).to(torch.float32)
+    return (blocks / s).view(pad.shape)[:n, :k].to(FP8).contiguous(), s[:, 0, :, 0].contiguous()
+
+
 def make_weights(seed=0, dim=DIM, hidden_arg=None, num_experts=NUM_EXPERTS, sigma=0.02, generator=None, device=None):
     """fp32 master weights as a flat dict keyed like the module's state dict. `device` draws them there (its own
     generator stream: not the same numbers as on the CPU, the same distribution)."""
@@ -57,17 +66,17 @@ def make_weights(seed=0, dim=DIM, hidden_arg=None, num_experts=NUM_EXPERTS, sigm
 
 def to_state_dict(master, weights="fp8", scale_input=True):
     """Cast the fp32 master weights into a loadable state dict.
-    weights="bf16": all bf16. weights="fp8": Linear weights e4m3fn + scale_weight (+ scale_input = 1.0),
+    weights="bf16": all bf16. weights="fp8_block": Linear weights e4m3fn + scale_weight of each 128 x 128 block. weights="fp8": Linear weights e4m3fn + scale_weight (+ scale_input = 1.0),
     gate.weight bf16."""
     out = {}
     for k, v in master.items():
         if k == "gate.weight" or weights == "bf16":
             out[k] = v.to(torch.bfloat16)
             continue
-        w8, s = quantize_per_tensor(v)
+        w8, s = quantize_per_block(v) if weights == "fp8_block" else quantize_per_tensor(v)
         out[k] = w8
         out[k.replace(".weight", ".scale_weight")] = s
-        if scale_input:
+        if scale_input and weights != "fp8_block":
             out[k.replace(".weight", ".scale_input")] = torch.ones((), dtype=torch.float32, device=v.device)
     return out
 
@@ -123,6 +132,8 @@ def build_module(state_dict, weights, device, dim=DIM, hidden_arg=None, num_expe
     hidden_arg = hidden_arg if hidden_arg is not None else 4 * dim
     if weights == "bf16":
         operations, dtype = ops.disable_weight_init, torch.bfloat16
+    elif weights == "fp8_block":
+        operations, dtype = ops.block_fp8_ops, torch.bfloat16
     else:
         operations = ops.scaled_fp8_ops(fp8_matrix_mult=fp8_matrix_mult, scale_input=scale_input, override_dtype=FP8)
         dtype = torch.bfloat16
