@@ -127,6 +127,7 @@ struct BlockArgs {
   const int32_t* offsets;
   int E;
   int lds_rows;         // few rows, cast inside: rows that a tile can have (the tile's height at most)
+  int parts;            // tiles of 256 rows: 64-row parts that a tile can have (4 at most)
 };
 
 __device__ __forceinline__ int swz(int row) { return ((row >> 1) & 7) ^ ((row & 1) << 2); }
@@ -180,6 +181,87 @@ struct Tiles {
     t.g = g;
     t.row0 = rb + (band * GROUP_M + within - n * gm) * BM;
     t.rows_here = min(re - t.row0, BM);
+    t.n0 = n * FEAT;
+    return t;
+  }
+};
+
+// The lane, formed anew: nothing that depends on it has to live across the K loop, which takes nearly all registers.
+__device__ __forceinline__ int lane_now() {
+  int v;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(v));
+  return v;
+}
+
+// The tiles of block_gemm8_kernel: a group's rows are cut into as few tiles of up to `parts` parts of 64 rows as they fill. Blocks are persistent.
+// Up to two rounds of them: a group's tiles are as even as parts allow, the groups with the highest ones come first, and the second round is
+// dealt backwards, so that who had a high tile gets a low one, over all XCDs by fours (the row tiles of a feature tile): one XCD alone reads
+// 0.6 MB/us. More rounds, or tiles of one height: full tiles, an eighth of the list to each XCD, which keeps its rows in L2.
+// Four segments of 1021 rows, 2560 x 6912 x 2560: 111-113 us (full tiles by eighths 116); seven of 3001, 2048 x 8192: 72.5 (75.4; the second round to whole
+// XCDs 74); 7656 x 3728 x 2752 in tiles of 3 parts 106 (of 4: 137); 16384 rows in four, 6912 x 2560, three rounds: by eighths 322, in turn 336.
+template <int FEAT>
+struct Deal {
+  int begin, end, start, cut, wide;   // per lane: rows of group `lane`, its first tile in the list, its row tiles << 3 | the parts of the lowest, its feature tiles
+  int next, then, step, stop;   // this block's next tile, if it is below `stop`, the one after it, and the way to others
+  __device__ __forceinline__ Deal(const BlockArgs& args, int lane) {
+    begin = end = 0;
+    if (lane < args.E) {
+      const int rows = args.op[0].rows;
+      begin = min(max(args.offsets[lane], 0), rows);
+      end = min(max(args.offsets[lane + 1], begin), rows);
+    } else if (lane == args.E) {
+      end = args.op[1].rows;
+    }
+    wide = (args.op[lane == args.E ? 1 : 0].N + FEAT - 1) / FEAT;
+    const int p = (end - begin + 63) / 64, mt = (p + args.parts - 1) / args.parts, count = mt * wide;
+    int total = 0;
+    for (int o = 0; o <= args.E; ++o) total += __builtin_amdgcn_readlane(count, o);
+    const bool even = total <= 2 * HDMOE_NUM_CU && mt > 0;
+    const int low = even ? p / mt : args.parts, high = even ? (p + mt - 1) / mt : min(p, low);
+    cut = mt << 3 | low;
+    start = 0;
+    int top = 0, least = 8;
+    for (int o = 0; o <= args.E; ++o) {
+      const int n = __builtin_amdgcn_readlane(count, o), h = __builtin_amdgcn_readlane(high, o);
+      if (h > high || (h == high && o < lane)) start += n;
+      top = max(top, h);
+      if (n > 0) least = min(least, h);
+    }
+    const int slots = (int)(gridDim.x / HDMOE_NUM_XCD), xcd = (int)(blockIdx.x % HDMOE_NUM_XCD), slot = (int)(blockIdx.x / HDMOE_NUM_XCD);
+    if (gridDim.x == HDMOE_NUM_CU && total > HDMOE_NUM_CU && total <= 2 * HDMOE_NUM_CU && top > least) {
+      auto at = [&](int t) { return (t / 4 * HDMOE_NUM_XCD + xcd) * 4 + t % 4; };
+      next = at(slot);
+      then = at(2 * slots - 1 - slot);
+      step = stop = total;   // no third one
+    } else {
+      const int each = (total + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD;
+      next = xcd * each + slot;
+      then = next + slots;
+      step = slots;
+      stop = min((xcd + 1) * each, total);
+    }
+  }
+  __device__ __forceinline__ bool more() const { return next < stop; }
+  // The block's next tile
+  __device__ __forceinline__ Tile take() {
+    constexpr int GROUP_M = 4;
+    int L = next;
+    next = then;
+    then += step;
+    const int g = __ffsll((long long)__ballot(L >= start && L < start + (cut >> 3) * wide)) - 1;
+    const int rb = __builtin_amdgcn_readlane(begin, g), re = __builtin_amdgcn_readlane(end, g), nt = __builtin_amdgcn_readlane(wide, g);
+    const int mt = __builtin_amdgcn_readlane(cut, g) >> 3, low = __builtin_amdgcn_readlane(cut, g) & 7;
+    const int more = max((re - rb + 63) / 64 - mt * low, 0);   // row tiles with a part more
+    L -= __builtin_amdgcn_readlane(start, g);
+    const int nbands = max(1, (mt + GROUP_M / 2) / GROUP_M);
+    const int band = min(L / (GROUP_M * nt), nbands - 1);
+    const int gm = band == nbands - 1 ? mt - band * GROUP_M : GROUP_M;
+    const int within = L - band * GROUP_M * nt;
+    const int n = within / gm, m = band * GROUP_M + within - n * gm;
+    Tile t;
+    t.g = g;
+    t.row0 = rb + 64 * (m * low + min(m, more));
+    t.rows_here = min(re - t.row0, 64 * (m < more ? low + 1 : low));
     t.n0 = n * FEAT;
     return t;
   }
@@ -491,12 +573,6 @@ __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_
 // The same tile of 256 x 256 with the K loop of gen_block_fp8.py, for segments that fill it; one block of 160 KiB of LDS per CU. The first
 // loads of a block's next tile go out before the end of this one.
 #include "block_fp8_asm.inc"
-// The lane, formed anew: nothing that depends on it has to live across the K loop, which takes nearly all registers.
-__device__ __forceinline__ int lane_now() {
-  int v;
-  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(v));
-  return v;
-}
 #define HDMOE_BLOCK_ACC \
   "={v[128:143]}"(acc[0]), "={v[144:159]}"(acc[1]), "={v[160:175]}"(acc[2]), "={v[176:191]}"(acc[3]), "={v[192:207]}"(acc[4]), \
       "={v[208:223]}"(acc[5]), "={v[224:239]}"(acc[6]), "={v[240:255]}"(acc[7])
@@ -511,13 +587,8 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wf = wave & 1, wt = wave >> 1;
 
-  const Tiles<BM, FEAT> tiles(args, lane);
-  // persistent blocks: those of an XCD take its eighth of the list in turn
-  const int per_xcd = (tiles.total + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD;
-  const int first = (int)(blockIdx.x % HDMOE_NUM_XCD) * per_xcd, end = min(first + per_xcd, tiles.total);
-  const int nslots = gridDim.x / HDMOE_NUM_XCD;
-  int L = first + blockIdx.x / HDMOE_NUM_XCD;
-  if (L >= end) return;
+  Deal<FEAT> tiles(args, lane);
+  if (!tiles.more()) return;
 
   typedef int v32i __attribute__((ext_vector_type(32)));
   typedef float v16f __attribute__((ext_vector_type(16)));
@@ -610,7 +681,7 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
     return s;
   };
 
-  Tile cur = tiles.get(L);
+  Tile cur = tiles.take();
   Source src = start(cur, lane);
   const int ldsw = sgpr((int)lds0 + wave * 1024);
   // between a tile's first loads and its loop: nothing, or the stores of the tile before, which need not have arrived
@@ -641,10 +712,9 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
     else HDMOE_BLOCK_LOOP(HDMOE_BLOCK_PLAIN);
 
     const Tile done = cur;
-    L += nslots;
-    const bool more = L < end;
+    const bool more = tiles.more();
     if (more) {
-      cur = tiles.get(L);
+      cur = tiles.take();
       src = start(cur, lane_now());
     }
     asm volatile("" : : : "memory");
@@ -913,7 +983,7 @@ template <class Act, bool SWIGLU>
 int launch_gemm8(const BlockArgs& args, const char* what, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   if (int rc = allow_lds(block_gemm8_kernel<Act, SWIGLU>, 163840, done, what)) return rc;
-  const long long grid = grid_of(args, 256, SWIGLU ? 128 : 256);
+  const long long grid = grid_of(args, 64 * args.parts, SWIGLU ? 128 : 256);
   if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
   block_gemm8_kernel<Act, SWIGLU><<<(unsigned)(grid < HDMOE_NUM_CU ? grid : HDMOE_NUM_CU), 512, 163840, stream>>>(args);
   return hdmoe_check_launch(what);
@@ -975,7 +1045,7 @@ namespace {
 
 // How a call runs: the few-row kernels on tiles of 16 * tt rows and ft strips (tt > 0; with the cast inside or not), block_gemm_kernel with
 // `stages` K steps in LDS (stages > 0), or block_gemm8_kernel.
-struct Plan { int tt, ft; bool cast_inside; int lds_rows; int stages; };
+struct Plan { int tt, ft; bool cast_inside; int lds_rows; int stages, parts; };
 
 // What a launch is likely to take in microseconds, by what the kernels measured over 1 to 16384 rows of 2560 and 6912 wide Linears. Where the
 // segments end is not known here; on average half a tile of each is empty.
@@ -1010,34 +1080,40 @@ double low_us(const Sizes& z, bool swiglu, int stages) {
   const double over = t <= HDMOE_NUM_CU ? 0.0 : t >= 2 * HDMOE_NUM_CU ? 1.0 : t / HDMOE_NUM_CU - 1.0;
   return 5.0 + (t > 2 * HDMOE_NUM_CU ? 1.1 * t / (2 * HDMOE_NUM_CU) : 1.0) * kb * (0.63 + 0.45 * over);
 }
-// Tiles of 256 x 256: a step lasts 0.49, 0.63, 0.85 or 1.07 us with 1 to 4 parts of 64 rows, and 1.5 where every CU multiplies a full one: the clock
-// falls.
-double high_us(const Sizes& z, bool swiglu) {
+// Tiles of 64 * cap x 256: a step lasts 0.49, 0.63, 0.85 or 1.07 us with 1 to 4 parts of 64 rows, and 1.5 where every CU multiplies a full one: the
+// clock falls. A CU with a tile more than others has lower ones.
+double high_us(const Sizes& z, bool swiglu, int cap) {
   const int feat = swiglu ? 128 : 256;
-  const double t = tiles_of(z, 256, feat), parts = tiles_of(z, 64, feat), kb = ((z.rows > 0 ? z.K : z.K_static) + BLK - 1) / BLK;
-  const double rounds = ceil(t / HDMOE_NUM_CU), full = t < HDMOE_NUM_CU ? t / HDMOE_NUM_CU : 1.0;
-  return 4.0 + rounds * (5.0 + kb * (0.3 + (0.19 + 0.1 * full) * parts / t));
+  const double t = tiles_of(z, 64 * cap, feat), parts = tiles_of(z, 64, feat), kb = ((z.rows > 0 ? z.K : z.K_static) + BLK - 1) / BLK;
+  const double rounds = ceil(t / HDMOE_NUM_CU), full = t < HDMOE_NUM_CU ? t / HDMOE_NUM_CU : 1.0, mean = parts / t;
+  const int segments = (z.rows > 0 ? z.E : 0) + (z.rows_static > 0 ? 1 : 0);
+  const double top = segments == 1 ? ceil(mean) : 1.5 * mean < cap ? 1.5 * mean : (double)cap;
+  const double low = segments == 1 || rounds < 2 ? mean : mean - (top - mean) * (rounds - t / HDMOE_NUM_CU) / (rounds - 1);
+  auto tile = [&](double p) { return 5.0 + kb * (0.3 + (0.19 + 0.1 * full) * p); };
+  const double one = tile(top), most = rounds * tile(low);
+  return 4.0 + (one > most ? one : most);
 }
 
 Plan plan_of(bool swiglu, bool x16, const Sizes& z) {
-  Plan best = {0, 0, false, 0, 0};
-  double us = high_us(z, swiglu);
+  Plan best = {0, 0, false, 0, 0, 4};
+  double us = high_us(z, swiglu, 4);
   auto offer = [&](double t, const Plan& p) {
     if (t < us) {
       us = t;
       best = p;
     }
   };
+  for (int cap = 3; cap >= 2; --cap) offer(high_us(z, swiglu, cap), Plan{0, 0, false, 0, 0, cap});
   if (swiglu) {
-    offer(low_us(z, true, 3), Plan{0, 0, false, 0, 3});
+    offer(low_us(z, true, 3), Plan{0, 0, false, 0, 3, 0});
   } else {
-    offer(low_us(z, false, 4), Plan{0, 0, false, 0, 4});
-    offer(low_us(z, false, 2), Plan{0, 0, false, 0, 2});
+    offer(low_us(z, false, 4), Plan{0, 0, false, 0, 4, 0});
+    offer(low_us(z, false, 2), Plan{0, 0, false, 0, 2, 0});
   }
   const int K = z.rows > 0 ? z.K : z.K_static;
   for (int tt = 1; tt <= 4; tt *= 2)
     for (int ft = swiglu ? 2 : 1; ft <= (tt == 4 ? 2 : 4); ft *= 2) {
-      Plan p = {tt, ft, false, 0, 0};
+      Plan p = {tt, ft, false, 0, 0, 0};
       double t = few_us(z, swiglu, tt, ft);
       if (x16 && tt == 1) {
         // a block casts for itself where that takes its threads a few trips at most: a launch (4 us) less
@@ -1131,6 +1207,7 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: 16-bit activations of the experts and of the static group must be the same rows", what);
   plan = plan_of(swiglu, x16, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, p->N, p->K_static, p->N_static});
   args.lds_rows = plan.lds_rows;
+  args.parts = plan.parts;
   const size_t need = work_bytes(swiglu, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K,
                                  routed ? p->N : 0, p->rows_static > 0 ? p->N_static : 0);
   if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255)))
