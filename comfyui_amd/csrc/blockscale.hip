@@ -740,8 +740,13 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
 //            launch needs the 128 features of a cast block in one thread block, 54 blocks an expert at 6912.)
 // CAST: the activations are 16-bit rows; the block casts its own into LDS (rows of K + 16 bytes: 16 rows then hit all banks) while the
 // first weights are on their way, instead of a launch of its own in front.
+// Blocks of a CU at once: two where 128 registers a thread hold two K blocks and what else a block needs, so that one starts while the other
+// streams (gate/up of 2 tokens, 2560 x 6912 x 2560 with both casts: 33.2 us, 42.4 with one block); more strips are better off with one that has three
+// K blocks on their way (8 rows of 4 experts, 6912 x 2560, four strips: 23.5 us with one, 27.7 with two).
+constexpr int stream_blocks(int ft, int tt, bool cast) { return cast || ft * tt <= 2 ? 2 : 1; }
+
 template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
-__global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args) {
+__global__ __launch_bounds__(512, stream_blocks(FT, TT, CAST) * 2) void block_stream_kernel(const BlockArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int KW = 8;
   static_assert(!SWIGLU || FT % 2 == 0, "w1 and w3 by halves");
@@ -749,7 +754,7 @@ __global__ __launch_bounds__(512) void block_stream_kernel(const BlockArgs args)
   constexpr int STRIPS = SWIGLU ? FT / 2 : FT;   // of one matrix
   constexpr int FEAT = 16 * STRIPS;
   // K blocks on their way: as many as the registers hold
-  constexpr int PER = FT * 8 + (CAST ? 0 : TT * 9) + 2, DEPTH_MAX = (220 - 4 * FT * TT) / PER;
+  constexpr int PER = FT * 8 + (CAST ? 0 : TT * 9) + 2, DEPTH_MAX = ((stream_blocks(FT, TT, CAST) == 2 ? 84 : 220) - 4 * FT * TT) / PER;
   constexpr int DEPTH = DEPTH_MAX > 6 ? 6 : DEPTH_MAX;
   static_assert(DEPTH >= 2, "two K blocks at least");
   constexpr int OUTSIDE = (int)0x80000000u;
@@ -1063,14 +1068,13 @@ double tiles_of(const Sizes& z, int bm, int feat) {   // in tiles of the experts
   }
   return t;
 }
-// Few rows. A CU runs one block at a time, 2.5 us to its first operands and then 39 KB/us of weights and activations (1 x 6912 x 2560: 8.2, 11.1
-// and 17.5 us with 1, 2 and 4 strips a block; 16 rows 10.4, 13.3, 19.6).
-double few_us(const Sizes& z, bool swiglu, int tt, int ft) {
+// Few rows. 2.5 us to a block's first operands, then 39 KB/us of weights and activations for a CU (1 x 6912 x 2560: 8.5, 11.4 and 17.2 us with 1, 2
+// and 4 strips a block).
+double few_us(const Sizes& z, bool swiglu, int tt, int ft, bool cast) {
   const double blocks = tiles_of(z, 16 * tt, swiglu ? 8 * ft : 16 * ft);
   const int per = z.rows > 0 ? (z.rows + z.E - 1) / z.E : 0, most = per > z.rows_static ? per : z.rows_static;
   const int rows = most < 16 * tt ? most : 16 * tt, K = z.rows > 0 ? z.K : z.K_static;
-  const double rounds = ceil(blocks / HDMOE_NUM_CU);
-  return 2.7 + rounds * (2.5 + (16.0 * ft + rows) * K / 39e3) + (swiglu ? 3.5 : 0.0);
+  return 2.7 + ceil(blocks / (HDMOE_NUM_CU * stream_blocks(ft, tt, cast))) * 2.5 + ceil(blocks / HDMOE_NUM_CU) * (16.0 * ft + rows) * K / 39e3 + (swiglu ? 3.5 : 0.0);
 }
 // Low tiles. 128 x 6912 x 2560: 32.7 us with four stages (two 41.6), where a step lasts half as long as memory's answer; from a block for every CU on
 // two blocks share one (1024 x 2560 x 6912: 32.6 against 25.8).
@@ -1114,14 +1118,14 @@ Plan plan_of(bool swiglu, bool x16, const Sizes& z) {
   for (int tt = 1; tt <= 4; tt *= 2)
     for (int ft = swiglu ? 2 : 1; ft <= (tt == 4 ? 2 : 4); ft *= 2) {
       Plan p = {tt, ft, false, 0, 0, 0};
-      double t = few_us(z, swiglu, tt, ft);
       if (x16 && tt == 1) {
         // a block casts for itself where that takes its threads a few trips at most: a launch (4 us) less
         const int whole = z.rows > z.rows_static ? z.rows : z.rows_static;
         p.lds_rows = whole < 16 ? whole : 16;
         p.cast_inside = (long long)p.lds_rows * ((K + BLK - 1) / BLK) * 16 <= 4 * 512;
-        if (p.cast_inside) t -= 4.0;
       }
+      double t = few_us(z, swiglu, tt, ft, p.cast_inside);
+      if (p.cast_inside) t -= 4.0;
       offer(t, p);
     }
   return best;
