@@ -2,6 +2,7 @@
 outputs with torch (device memory and stream plumbing only) and enqueue the HIP
 kernels on torch's current stream. Nothing here computes with torch.
 """
+import array
 import contextlib
 import ctypes
 
@@ -565,7 +566,7 @@ def _raw_stream(t):
 
 def _on(device):
     """Context in which `device` is the current one."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _blocks(n):
@@ -671,11 +672,30 @@ def _block_experts(a, offsets, experts, perm, dtype, what):
         rows = T * _lib.TOPK
         if perm.dtype != torch.int32 or perm.shape != (rows,) or perm.device != dev or not perm.is_contiguous():
             raise ValueError(f"{what}: perm must be contiguous int32 [{rows}] on {dev}")
-    arr = (_lib.BlockWeights * E)()
-    shapes, index = None, a.get_device()
-    for w, entry in zip(arr, experts):
-        shapes = _block_weights(w, entry, K, dtype, index, what, shapes)
-    return arr, rows, shapes[0][0]
+    # (_block_matrix and _block_weights for all experts, without a call each: it takes the few that fail)
+    index, words = a.get_device(), array.array("Q")
+    first = experts[0][0]
+    N = first.shape[0] if first.dim() == 2 else -1
+    of_w, of_s, of_b, f32 = (N, K), (-(-N // BLOCK), -(-K // BLOCK)), (N,), torch.float32
+    for entry in experts:
+        if dtype is None:
+            w1, s1, w3, s3 = entry
+            if (w3.dtype is not FP8 or w3.shape != of_w or w3.get_device() != index or not w3.is_contiguous()
+                    or s3.dtype is not f32 or s3.shape != of_s or s3.get_device() != index or not s3.is_contiguous()):
+                _block_matrix(w3, s3, K, index, what, (of_w, of_s))
+            more = (w3.data_ptr(), s3.data_ptr(), 0)
+        else:
+            w1, s1, bias = entry
+            more = (0, 0, 0)
+            if bias is not None:
+                if bias.dtype is not dtype or bias.shape != of_b or bias.get_device() != index or not bias.is_contiguous():
+                    _block_weights(_lib.BlockWeights(), entry, K, dtype, index, what, (of_w, of_s))
+                more = (0, 0, bias.data_ptr())
+        if (w1.dtype is not FP8 or w1.shape != of_w or w1.get_device() != index or not w1.is_contiguous()
+                or s1.dtype is not f32 or s1.shape != of_s or s1.get_device() != index or not s1.is_contiguous()):
+            _block_matrix(w1, s1, K, index, what, (of_w, of_s))
+        words.extend((w1.data_ptr(), s1.data_ptr(), *more))
+    return (_lib.BlockWeights * E).from_buffer(words), rows, N
 
 
 def _block_call(fn, swiglu, args, a):
