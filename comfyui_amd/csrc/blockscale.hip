@@ -364,7 +364,7 @@ __device__ __forceinline__ int tile_feature(int f, int r) {
 // WF x WT waves, each FT * 16 weight rows x TT * 16 tokens in MFMA tiles of 16 x 16 x 128; the results of a weight tile join the
 // accumulators behind the MFMAs of the next one. STAGES K steps in LDS, STAGES - 1 of them asked for ahead: with two, two blocks share
 // a CU and one fills the other's waits; with more, for launches that have at most a block for every CU, a step does not last as long as
-// its loads are on their way (128 x 6912 x 2560: X us with two).
+// its loads are on their way (128 x 6912 x 2560: 32 us, 41.5 with two stages).
 template <class Act, bool SWIGLU, int WF, int WT, int FT, int TT, int STAGES>
 __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_kernel(const BlockArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)   // (the host pass leaves out stubs of kernels whose lambdas hold arrays of dependent size)
@@ -731,32 +731,44 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------
-// Segments of up to a few dozen rows: the weights are read once from memory into registers, no tile of them passes through LDS, and
-// many 16-byte loads are on their way at once. A wave multiplies FT strips of 16 weight rows with TT * 16 tokens; KW waves deal the K
-// blocks of the same strips out and their sums meet in LDS.
+// Segments of up to a few dozen rows: the weights are read once from memory. A wave multiplies FT strips of 16 weight rows with TT * 16
+// tokens; KW waves deal the K blocks of the same strips out, each through a ring of its own in LDS, so none waits for another before
+// the end, where their sums meet.
+// What a CU fetches in a microsecond is the bound. Lanes that hold a row each would ask for 16 bytes of a cache line 4 at a time, one line a
+// cycle: 39 KB/us. Through LDS 8 neighbouring lanes ask for 128 bytes of a row: 80 KB/us (48 x 6912 x 2560
+// with the cast 10.7 us, 15.7 the other way; 128 rows in four segments 25.6 and 30.0, the weights at 3.6 TB/s).
 // More strips a wave read the activations less often (they come out of L2, 16 TT rows for every 16 FT of the weights), fewer make more
 // blocks: a CU has only so many requests on their way, so all 256 have to take part.
 //   gate/up: half of the strips are w1's, half the same features of w3; silu(g) * u leaves in fp32, and a second launch casts it. (One
 //            launch needs the 128 features of a cast block in one thread block, 54 blocks an expert at 6912.)
 // CAST: the activations are 16-bit rows; the block casts its own into LDS (rows of K + 16 bytes: 16 rows then hit all banks) while the
 // first weights are on their way, instead of a launch of its own in front.
-// Blocks of a CU at once: two where 128 registers a thread hold two K blocks and what else a block needs, so that one starts while the other
-// streams (gate/up of 2 tokens, 2560 x 6912 x 2560 with both casts: 33.2 us, 42.4 with one block); more strips are better off with one that has three
-// K blocks on their way (8 rows of 4 experts, 6912 x 2560, four strips: 23.5 us with one, 27.7 with two).
+constexpr int STREAM_WAVES = 4, CAST_UNITS = 128;   // CAST: blocks of 128 values that a thread block can cast
+// Blocks of a CU at once: two where half of the LDS holds enough on its way, so that one starts while the other streams.
 constexpr int stream_blocks(int ft, int tt, bool cast) { return cast || ft * tt <= 2 ? 2 : 1; }
+// Of a wave: a K block of weights and activations with their scales, and how many of them its ring has
+constexpr int stream_slot(int ft, int tt, bool swiglu, bool cast) { return 2048 * (ft + (cast ? 0 : tt)) + 256 * (1 + (swiglu ? 1 : 0) + (cast ? 0 : 1)); }
+constexpr int stream_depth(int ft, int tt, bool swiglu, bool cast) {
+  const int budget = stream_blocks(ft, tt, cast) == 1 ? 159744 : cast ? 73728 : 81920, n = budget / (STREAM_WAVES * stream_slot(ft, tt, swiglu, cast));
+  return n > 8 ? 8 : n;
+}
+
+// CAST: cast rows and scales, and in front of the 16-bit ones
+__host__ __device__ constexpr int stream_cast_bytes(int rows, int KB) { return (rows * (KB * BLK + 16 + KB * 4) + 255) / 256 * 256; }
+constexpr int stream_raw_bytes(int rows, int KB) { return (rows * KB + 4 * STREAM_WAVES - 1) / (4 * STREAM_WAVES) * STREAM_WAVES * 1024; }
 
 template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
-__global__ __launch_bounds__(512, stream_blocks(FT, TT, CAST) * 2) void block_stream_kernel(const BlockArgs args) {
+__global__ __launch_bounds__(64 * STREAM_WAVES) void block_stream_kernel(const BlockArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int KW = 8;
+  constexpr int KW = STREAM_WAVES;
   static_assert(!SWIGLU || FT % 2 == 0, "w1 and w3 by halves");
   constexpr int BM = TT * 16;
   constexpr int STRIPS = SWIGLU ? FT / 2 : FT;   // of one matrix
   constexpr int FEAT = 16 * STRIPS;
-  // K blocks on their way: as many as the registers hold
-  constexpr int PER = FT * 8 + (CAST ? 0 : TT * 9) + 2, DEPTH_MAX = ((stream_blocks(FT, TT, CAST) == 2 ? 84 : 220) - 4 * FT * TT) / PER;
-  constexpr int DEPTH = DEPTH_MAX > 6 ? 6 : DEPTH_MAX;
-  static_assert(DEPTH >= 2, "two K blocks at least");
+  constexpr int XT = CAST ? 0 : TT;              // strips of activations in a slot
+  constexpr int SLOT = stream_slot(FT, TT, SWIGLU, CAST), DEPTH = stream_depth(FT, TT, SWIGLU, CAST), RING = DEPTH * SLOT;
+  constexpr int LOADS = 2 * (FT + XT) + 1 + (SWIGLU ? 1 : 0) + (CAST ? 0 : 1);   // of a step
+  static_assert(DEPTH >= 2 && (DEPTH - 1) * LOADS < 64, "two K blocks at least, and their loads counted in 6 bits");
   constexpr int OUTSIDE = (int)0x80000000u;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -766,9 +778,9 @@ __global__ __launch_bounds__(512, stream_blocks(FT, TT, CAST) * 2) void block_st
 
   const Tiles<BM, FEAT> tiles(args, lane);
   const int per_xcd = (tiles.total + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD;
-  const int slot = blockIdx.x / HDMOE_NUM_XCD;
-  const int L = (int)(blockIdx.x % HDMOE_NUM_XCD) * per_xcd + slot;
-  if (slot >= per_xcd || L >= tiles.total) return;
+  const int slot_x = blockIdx.x / HDMOE_NUM_XCD;
+  const int L = (int)(blockIdx.x % HDMOE_NUM_XCD) * per_xcd + slot_x;
+  if (slot_x >= per_xcd || L >= tiles.total) return;
   const Tile t = tiles.get(L);
   const Group& grp = args.g[t.g];
   const Operand& op = args.op[t.g == args.E ? 1 : 0];
@@ -777,78 +789,104 @@ __global__ __launch_bounds__(512, stream_blocks(FT, TT, CAST) * 2) void block_st
   const int32_t* const gather = op.gather;
   const int a_rows = op.a_rows;
 
-  // weights: lane = row fr of a strip, 16-byte chunks quad and quad + 4 of a K block. Strips past N read as zeros.
+  // global -> LDS: lane i of a load lands in 16-byte chunk i & 7 of row i >> 3 of a strip's half and fetches the chunk that the swizzle puts
+  // there. Rows and chunks that do not exist read as zero.
   const int feats = min(N - t.n0, FEAT);
   const __amdgpu_buffer_rsrc_t rw0 = make_rsrc(grp.w0 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K);
   const __amdgpu_buffer_rsrc_t rw1 = SWIGLU ? make_rsrc(grp.w1 + (size_t)t.n0 * K, (uint32_t)feats * (uint32_t)K) : rw0;
   const __amdgpu_buffer_rsrc_t rs0 = make_rsrc(grp.s0 + (size_t)(t.n0 / BLK) * KB, (uint32_t)KB * 4u);
   const __amdgpu_buffer_rsrc_t rs1 = SWIGLU ? make_rsrc(grp.s1 + (size_t)(t.n0 / BLK) * KB, (uint32_t)KB * 4u) : rs0;
-
-  // tokens: column fr of each tile
-  int row[TT];
+  const __amdgpu_buffer_rsrc_t ra = gather != nullptr ? make_rsrc(op.a, (uint32_t)a_rows * (uint32_t)K)
+                                                      : make_rsrc(op.a + (size_t)t.row0 * K, (uint32_t)t.rows_here * (uint32_t)K);
+  const int ld_s = __builtin_amdgcn_readfirstlane((int)op.ld_sa * 4);
+  const __amdgpu_buffer_rsrc_t rs = make_rsrc(op.sa, (uint32_t)(KB - 1) * (uint32_t)ld_s + (uint32_t)a_rows * 4u);
+  int vw[2], last[2], vx[CAST ? 1 : TT][2], tok = OUTSIDE;
 #pragma unroll
-  for (int tt = 0; tt < TT; ++tt) {
-    const int r = tt * 16 + fr;
-    row[tt] = -1;
-    if (r < t.rows_here) row[tt] = gather != nullptr ? gather[t.row0 + r] >> 1 : t.row0 + r;
-    if ((unsigned)row[tt] >= (unsigned)a_rows) row[tt] = -1;
+  for (int j = 0; j < 2; ++j) {
+    const int r = j * 8 + (lane >> 3), c = (lane & 7) ^ swz(r);
+    vw[j] = r * K + c * 16;
+    last[j] = (KB - 1) * BLK + c * 16 < K ? 0 : OUTSIDE;
+#pragma unroll
+    for (int tt = 0; tt < XT; ++tt) {
+      const int x = tt * 16 + r;
+      vx[tt][j] = OUTSIDE;
+      if (x < t.rows_here) {
+        const int from = gather != nullptr ? gather[t.row0 + x] >> 1 : x;   // a bad index of the permutation reads as a row of zeros
+        if (gather == nullptr || (unsigned)from < (unsigned)a_rows) vx[tt][j] = from * K + c * 16;
+      }
+    }
   }
-
-  struct Step { v4i w[FT][2]; v4i x[CAST ? 1 : TT][2]; float s0, s1, sx[TT]; };
-  const int wbase = fr * K + quad * 16;
-  auto load = [&](Step& st, int kb) {
-    const int k = kb * BLK + quad * 16;
-    const bool lo = k < K, hi = k + 64 < K;
-#pragma unroll
-    for (int f = 0; f < FT; ++f) {
-      const __amdgpu_buffer_rsrc_t r = f >= STRIPS ? rw1 : rw0;
-      const int off = wbase + f % STRIPS * 16 * K + kb * BLK;
-      st.w[f][0] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, lo ? off : OUTSIDE, 0, 0));
-      st.w[f][1] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, hi ? off + 64 : OUTSIDE, 0, 0));
-    }
-    const int so = kb < KB ? kb * 4 : OUTSIDE;
-    st.s0 = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs0, so, 0, 0));
-    if (SWIGLU) st.s1 = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs1, so, 0, 0));
-    if constexpr (!CAST) {
-      // (64-bit addresses: the rows of all segments together may pass 4 GiB)
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt) {
-        const int r = max(row[tt], 0), kk = min(k, K - 16), kk2 = min(k + 64, K - 16);   // what lies past K meets weights of zero
-        const uint8_t* const xr = op.a + (size_t)r * K;
-        st.x[tt][0] = *reinterpret_cast<const v4i*>(xr + kk);
-        st.x[tt][1] = *reinterpret_cast<const v4i*>(xr + kk2);
-        st.sx[tt] = op.sa[(size_t)min(kb, KB - 1) * op.ld_sa + r];
-      }
-    }
+  if (!CAST && lane < BM && lane < t.rows_here) {
+    const int from = gather != nullptr ? gather[t.row0 + lane] >> 1 : t.row0 + lane;
+    if ((unsigned)from < (unsigned)a_rows) tok = from * 4;
+  }
+  const uint32_t ring = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr_t)smem + wave * RING);
+  // (by hand: the compiler takes any of them for one that a later LDS read may want)
+  auto to_lds = [](const __amdgpu_buffer_rsrc_t& r, uint32_t lds, int voff, int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
   };
-  Step st[DEPTH];
+  auto word_to_lds = [](const __amdgpu_buffer_rsrc_t& r, uint32_t lds, int voff, int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
+  };
+  constexpr int SCALES = 2048 * (FT + XT);   // of a slot: w1's, w3's, the tokens', 64 words each
+  auto issue = [&](int slot, int kb) {   // (past the last K block as well, asking for nothing: the loads on their way are counted)
+    const uint32_t at = ring + slot * SLOT;
+    const int kc = min(kb, KB - 1);
+    int mask[2];
 #pragma unroll
-  for (int i = 0; i < DEPTH; ++i) load(st[i], kw + i * KW);
+    for (int j = 0; j < 2; ++j) mask[j] = kb >= KB ? OUTSIDE : kb == KB - 1 ? last[j] : 0;
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) to_lds(f >= STRIPS ? rw1 : rw0, at + f * 2048 + j * 1024, (vw[j] + f % STRIPS * 16 * K) | mask[j], kc * BLK);
+#pragma unroll
+    for (int tt = 0; tt < XT; ++tt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) to_lds(ra, at + (FT + tt) * 2048 + j * 1024, vx[tt][j] | mask[j], kc * BLK);
+    word_to_lds(rs0, at + SCALES, 0, kc * 4);
+    if (SWIGLU) word_to_lds(rs1, at + SCALES + 256, 0, kc * 4);
+    if (!CAST) word_to_lds(rs, at + SCALES + (SWIGLU ? 512 : 256), tok, kc * ld_s);
+  };
 
-  // [rows][ld_x] cast rows, [KB][rows] scales; a column without a row reads the last one's and is never stored
+  // CAST: the 16-bit rows first, 16 lanes for each block of 128; [rows][ld_x] cast rows, [KB][rows] scales. A column without a row reads the
+  // last one's and is never stored.
   const int ld_x = KB * BLK + 16, R = args.lds_rows;
-  uint8_t* const lx = smem;
-  float* const ls = reinterpret_cast<float*>(smem + (size_t)R * ld_x);
+  uint8_t* const lx = smem + KW * RING;
+  float* const ls = reinterpret_cast<float*>(lx + (size_t)R * ld_x);
+  uint8_t* const raw = lx + stream_cast_bytes(R, KB);
   if constexpr (CAST) {
-    const int units = R * KB;
-    for (int u = tid >> 4; u < units; u += 32) {
-      const int r = u / KB, b = u - r * KB;
-      int from = -1;
-      if (r < t.rows_here) {
-        from = gather != nullptr ? gather[t.row0 + r] >> 1 : t.row0 + r;
-        if ((unsigned)from >= (unsigned)a_rows) from = -1;
+    const __amdgpu_buffer_rsrc_t rx = gather != nullptr ? make_rsrc(op.a, (uint32_t)a_rows * (uint32_t)K * 2u)
+                                                        : make_rsrc(op.a + (size_t)t.row0 * K * 2, (uint32_t)t.rows_here * (uint32_t)K * 2u);
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr_t)raw + wave * 1024);
+    for (int i = 0; i * 4 * KW < R * KB; ++i) {
+      const int u = i * 4 * KW + (tid >> 4), r = u / KB, k = (u - r * KB) * BLK + (tid & 15) * 8;
+      int off = OUTSIDE;
+      if (r < t.rows_here && k < K) {
+        const int from = gather != nullptr ? gather[t.row0 + r] >> 1 : r;
+        if (gather == nullptr || (unsigned)from < (unsigned)a_rows) off = (from * K + k) * 2;
       }
-      const int k = b * BLK + (tid & 15) * 8;
+      to_lds(rx, at + i * KW * 1024, off, 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i) issue(i, kw + i * KW);
+
+  if constexpr (CAST) {
+    static_assert(DEPTH * LOADS < 64, "counted in 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(DEPTH * LOADS) : "memory");   // a thread casts what it asked for itself
+    for (int i = 0; i * 4 * KW < R * KB; ++i) {
+      const int u = i * 4 * KW + (tid >> 4), r = u / KB, b = u - r * KB;
       Half<Act> v;
-      v.clear();
-      if (from >= 0 && k < K) v.load(op.a, (size_t)from * K + k);
+      v.load(raw, (size_t)(i * 64 * KW + tid) * 8);
       uint32_t o[2];
       float s;
       cast_unit(v, o, s);
-      *reinterpret_cast<u32x2*>(lx + r * ld_x + k) = u32x2{o[0], o[1]};
-      if ((tid & 15) == 0) ls[b * R + r] = from >= 0 ? s : 0.0f;
+      if (r < R) {
+        *reinterpret_cast<u32x2*>(lx + r * ld_x + b * BLK + (tid & 15) * 8) = u32x2{o[0], o[1]};
+        if ((tid & 15) == 0) ls[b * R + r] = s;
+      }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");   // (the weights need not have come)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
   }
 
   v4f acc[FT][TT];
@@ -856,65 +894,72 @@ __global__ __launch_bounds__(512, stream_blocks(FT, TT, CAST) * 2) void block_st
   for (int f = 0; f < FT; ++f)
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) acc[f][tt] = v4f{0, 0, 0, 0};
-  auto multiply = [&](const Step& st, int kb) {
-    v8i fb[TT];
-    float m0[TT], m1[TT];
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-      v4i x0, x1;
-      float sx;
-      if constexpr (CAST) {
-        const int r = min(tt * 16 + fr, R - 1);
-        const uint8_t* const xr = lx + r * ld_x + kb * BLK + quad * 16;
-        x0 = *reinterpret_cast<const v4i*>(xr);
-        x1 = *reinterpret_cast<const v4i*>(xr + 64);
-        sx = ls[kb * R + r];
-      } else {
-        x0 = st.x[tt][0];
-        x1 = st.x[tt][1];
-        sx = row[tt] >= 0 ? st.sx[tt] : 0.0f;
-      }
-      fb[tt] = v8i{x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-      m0[tt] = sx * st.s0;
-      m1[tt] = SWIGLU ? sx * st.s1 : 0.0f;
-    }
-#pragma unroll
-    for (int f = 0; f < FT; ++f) {
-      const v8i fa = {st.w[f][0].x, st.w[f][0].y, st.w[f][0].z, st.w[f][0].w, st.w[f][1].x, st.w[f][1].y, st.w[f][1].z, st.w[f][1].w};
-      v4f p[TT];
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt) p[tt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb[tt], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[f][tt][i] = __builtin_fmaf(p[tt][i], SWIGLU && f >= STRIPS ? m1[tt] : m0[tt], acc[f][tt][i]);
-    }
+  typedef const __attribute__((address_space(3))) v4i* lds_v4i;
+  typedef const __attribute__((address_space(3))) float* lds_float;
+  const int c0 = (quad ^ swz(fr)) * 16, c1 = ((quad + 4) ^ swz(fr)) * 16;
+  auto strip = [&](uint32_t at) -> v8i {
+    const v4i lo = *(lds_v4i)(at + fr * BLK + c0), hi = *(lds_v4i)(at + fr * BLK + c1);
+    return v8i{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
   };
-  for (int kb0 = kw; kb0 < KB; kb0 += DEPTH * KW) {
+  const int steps = kw < KB ? (KB - kw + KW - 1) / KW : 0;
+  for (int j0 = 0; j0 < steps; j0 += DEPTH) {
 #pragma unroll
     for (int i = 0; i < DEPTH; ++i) {
-      const int kb = kb0 + i * KW;
-      if (kb < KB) {
-        multiply(st[i], kb);
-        if (kb + DEPTH * KW < KB) load(st[i], kb + DEPTH * KW);
+      if (j0 + i >= steps) break;
+      const int kb = kw + (j0 + i) * KW;
+      const uint32_t at = ring + i * SLOT;
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"((DEPTH - 1) * LOADS) : "memory");
+      v8i fa[FT], fb[TT];
+      float m0[TT], m1[TT];
+#pragma unroll
+      for (int f = 0; f < FT; ++f) fa[f] = strip(at + f * 2048);
+      const float s0 = *(lds_float)(at + SCALES + lane * 4), s1 = SWIGLU ? *(lds_float)(at + SCALES + 256 + lane * 4) : 0.0f;
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) {
+        float sx;
+        if constexpr (CAST) {
+          const int r = min(tt * 16 + fr, R - 1);
+          const uint8_t* const row = lx + r * ld_x + kb * BLK + quad * 16;
+          const v4i lo = *reinterpret_cast<const v4i*>(row), hi = *reinterpret_cast<const v4i*>(row + 64);
+          fb[tt] = v8i{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          sx = ls[kb * R + r];
+        } else {
+          fb[tt] = strip(at + (FT + tt) * 2048);
+          sx = *(lds_float)(at + SCALES + (SWIGLU ? 512 : 256) + (tt * 16 + fr) * 4);
+        }
+        m0[tt] = sx * s0;
+        m1[tt] = SWIGLU ? sx * s1 : 0.0f;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");   // the slot is read: its next K block may come
+      issue(i, kb + DEPTH * KW);
+#pragma unroll
+      for (int f = 0; f < FT; ++f) {
+        v4f p[TT];
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) p[tt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa[f], fb[tt], v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[f][tt][c] = __builtin_fmaf(p[tt][c], SWIGLU && f >= STRIPS ? m1[tt] : m0[tt], acc[f][tt][c]);
       }
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // of the loads that asked for nothing: their zeros land in the ring too
 
-  // the waves' sums, [KW][strip][token tile][lane] of 16 bytes
+  // the waves' sums, each in its own ring: [strip][token tile][lane] of 16 bytes
   constexpr int CELLS = FT * TT;
-  v4f* const parts = reinterpret_cast<v4f*>(smem);
-  if (CAST) __syncthreads();   // the cast rows are read no more
+  static_assert(CELLS * 1024 <= RING, "a wave's sums take its ring's place");
+  auto parts = [&](int w, int cell) -> v4f& { return reinterpret_cast<v4f*>(smem + w * RING)[cell * 64 + lane]; };
 #pragma unroll
   for (int f = 0; f < FT; ++f)
 #pragma unroll
-    for (int tt = 0; tt < TT; ++tt) parts[(kw * CELLS + f * TT + tt) * 64 + lane] = acc[f][tt];
+    for (int tt = 0; tt < TT; ++tt) parts(kw, f * TT + tt) = acc[f][tt];
   __syncthreads();
   auto total = [&](int cell) {
-    v4f y = parts[cell * 64 + lane];
+    v4f y = parts(0, cell);
 #pragma unroll
     for (int w = 1; w < KW; ++w) {
-      const v4f v = parts[(w * CELLS + cell) * 64 + lane];
+      const v4f v = parts(w, cell);
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] += v[i];
     }
@@ -998,15 +1043,15 @@ int launch_gemm8(const BlockArgs& args, const char* what, hipStream_t stream) {
 
 template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
 int launch_stream(const BlockArgs& args, const char* what, hipStream_t stream) {
-  constexpr size_t sums = (size_t)8 * FT * TT * 1024;
+  constexpr size_t rings = (size_t)STREAM_WAVES * stream_depth(FT, TT, SWIGLU, CAST) * stream_slot(FT, TT, SWIGLU, CAST);
   static std::atomic<uint64_t> done{0};
-  if (sums > 65536)
-    if (int rc = allow_lds(block_stream_kernel<Act, SWIGLU, FT, TT, CAST>, sums, done, what)) return rc;
+  if (int rc = allow_lds(block_stream_kernel<Act, SWIGLU, FT, TT, CAST>, rings + (CAST ? stream_cast_bytes(16, CAST_UNITS / 16) + stream_raw_bytes(16, CAST_UNITS / 16) : 0), done, what)) return rc;
   const int K = args.op[0].K > args.op[1].K ? args.op[0].K : args.op[1].K;
-  const size_t KB = (K + BLK - 1) / BLK, rows = CAST ? (size_t)args.lds_rows * (KB * BLK + 16 + KB * 4) : 0;
+  const int KB = (K + BLK - 1) / BLK;
+  const size_t rows = CAST ? stream_cast_bytes(args.lds_rows, KB) + stream_raw_bytes(args.lds_rows, KB) : 0;
   const long long grid = grid_of(args, TT * 16, SWIGLU ? 8 * FT : 16 * FT);
   if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
-  block_stream_kernel<Act, SWIGLU, FT, TT, CAST><<<(unsigned)grid, 512, rows > sums ? rows : sums, stream>>>(args);
+  block_stream_kernel<Act, SWIGLU, FT, TT, CAST><<<(unsigned)grid, 64 * STREAM_WAVES, rings + rows, stream>>>(args);
   return hdmoe_check_launch(what);
 }
 
@@ -1068,13 +1113,14 @@ double tiles_of(const Sizes& z, int bm, int feat) {   // in tiles of the experts
   }
   return t;
 }
-// Few rows. 2.5 us to a block's first operands, then 39 KB/us of weights and activations for a CU (1 x 6912 x 2560: 8.5, 11.4 and 17.2 us with 1, 2
-// and 4 strips a block).
+// Few rows. 3.5 us to a block's first operands and behind its last, 80 KB/us of weights and activations for a CU (32 x 6912 x 2560 with its cast, 1, 2 and 4 strips a
+// block: 12.1, 10.6, 13.1 us); 55 KB/us where a wave multiplies 16 tiles of each K block and has only one more on its way (100 x 2560 x 6912: 13.9, 17.9 in
+// two rounds of 8 tiles).
 double few_us(const Sizes& z, bool swiglu, int tt, int ft, bool cast) {
   const double blocks = tiles_of(z, 16 * tt, swiglu ? 8 * ft : 16 * ft);
   const int per = z.rows > 0 ? (z.rows + z.E - 1) / z.E : 0, most = per > z.rows_static ? per : z.rows_static;
   const int rows = most < 16 * tt ? most : 16 * tt, K = z.rows > 0 ? z.K : z.K_static;
-  return 2.7 + ceil(blocks / (HDMOE_NUM_CU * stream_blocks(ft, tt, cast))) * 2.5 + ceil(blocks / HDMOE_NUM_CU) * (16.0 * ft + rows) * K / 39e3 + (swiglu ? 3.5 : 0.0);
+  return 1.7 + ceil(blocks / (HDMOE_NUM_CU * stream_blocks(ft, tt, cast))) * 3.5 + ceil(blocks / HDMOE_NUM_CU) * (16.0 * ft + rows) * K / (ft * tt == 16 ? 55e3 : 80e3) + (swiglu ? 3.5 : 0.0);
 }
 // Low tiles. 128 x 6912 x 2560: 32.7 us with four stages (two 41.6), where a step lasts half as long as memory's answer; from a block for every CU on
 // two blocks share one (1024 x 2560 x 6912: 32.6 against 25.8).
@@ -1116,13 +1162,13 @@ Plan plan_of(bool swiglu, bool x16, const Sizes& z) {
   }
   const int K = z.rows > 0 ? z.K : z.K_static;
   for (int tt = 1; tt <= 4; tt *= 2)
-    for (int ft = swiglu ? 2 : 1; ft <= (tt == 4 ? 2 : 4); ft *= 2) {
+    for (int ft = swiglu ? 2 : 1; ft <= 4; ft *= 2) {
       Plan p = {tt, ft, false, 0, 0, 0};
       if (x16 && tt == 1) {
-        // a block casts for itself where that takes its threads a few trips at most: a launch (4 us) less
+        // a block casts for itself where its threads hold all of it at once: a launch (4 us) less
         const int whole = z.rows > z.rows_static ? z.rows : z.rows_static;
         p.lds_rows = whole < 16 ? whole : 16;
-        p.cast_inside = (long long)p.lds_rows * ((K + BLK - 1) / BLK) * 16 <= 4 * 512;
+        p.cast_inside = (long long)p.lds_rows * ((K + BLK - 1) / BLK) <= CAST_UNITS && (long long)whole * K * 2 <= 0x7fffffff;
       }
       double t = few_us(z, swiglu, tt, ft, p.cast_inside);
       if (p.cast_inside) t -= 4.0;
