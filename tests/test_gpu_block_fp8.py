@@ -372,3 +372,73 @@ def test_no_rows():
     assert HF.grouped_linear_block_fp8(x, segments([0, 0]), [(w, sw, None)] * 2).shape == (0, 256)
     h, sh = HF.grouped_swiglu_block_fp8(x, segments([0]), [(w, sw, w, sw)])
     assert h.shape == (0, 256) and sh.shape == (0, 2)
+
+
+def uneven(rows, n):
+    """Sizes of n segments, the first about half of the rows, the second empty where there are more than three."""
+    if n == 0:
+        return []
+    left, sizes = rows, []
+    for i in range(n):
+        take = left if i == n - 1 else 0 if i == 1 and n > 3 else -(-left // 2)
+        sizes.append(take)
+        left -= take
+    return sizes
+
+
+# Sizes at which each way to run a contraction is taken: few rows with 1, 2 and 4 tiles of 16 rows by 1, 2 and 4 strips of weights, with and
+# without the cast inside; 128-row tiles with 2 and 4 steps on their way; 256-row ones of up to 2, 3 and 4 parts
+EVERY = [(5, 0, 608, 64), (30, 3, 320, 64), (12, 0, 704, 64), (42, 3, 208, 64), (558, 0, 176, 160), (1285, 3, 240, 80), (292, 0, 144, 224),
+         (495, 3, 144, 144), (77, 0, 144, 3136), (544, 3, 304, 448), (1494, 0, 176, 96), (3774, 3, 144, 64), (1584, 0, 400, 80), (852, 3, 352, 144),
+         (1621, 0, 144, 112), (2544, 6, 160, 64), (1695, 0, 144, 192), (1717, 6, 144, 224), (33, 0, 144, 3056), (119, 3, 160, 1104),
+         (916, 0, 240, 544), (165, 3, 160, 1392), (1017, 0, 144, 528), (2134, 3, 160, 288), (3807, 3, 2128, 4080), (3440, 0, 880, 3552),
+         (3356, 3, 1040, 3312), (3980, 0, 832, 3888), (3888, 3, 736, 3808), (2908, 0, 208, 336), (3413, 3, 192, 320), (3666, 0, 1936, 304),
+         (2959, 3, 2000, 336), (100, 0, 6912, 272), (3, 0, 5360, 400), (20, 4, 16400, 96), (1, 0, 16400, 144)]
+EVERY_GATE_UP = [(5, 0, 592, 64), (36, 3, 272, 80), (5, 0, 480, 64), (62, 3, 192, 80), (202, 0, 288, 608), (193, 3, 416, 576), (290, 0, 144, 224),
+                 (1224, 3, 400, 64), (854, 0, 272, 96), (230, 3, 352, 272), (1214, 0, 272, 144), (843, 3, 288, 176), (46, 0, 288, 2256),
+                 (1608, 3, 304, 144), (1143, 0, 304, 240), (1760, 6, 288, 144), (3128, 0, 144, 688), (3498, 3, 144, 592), (3117, 0, 160, 1312),
+                 (1969, 3, 144, 1984), (1997, 0, 160, 2976), (3374, 3, 144, 1680), (10, 0, 176, 80), (69, 3, 224, 64), (3, 0, 5360, 272), (20, 4, 8208, 96)]
+
+
+@pytest.mark.parametrize("rows,E,K,N", EVERY)
+def test_linear_every_way(rows, E, K, N):
+    from comfyui_amd import functional as HF
+    g = gen(rows + K + N)
+    x = tokens(g, rows, K)
+    q, s = HF.quant_block_fp8(x)
+    sizes = uneven(rows, E) or [rows]
+    experts = [(*weight(g, N, K), None) for _ in sizes]
+    off = segments(sizes)
+    b = off.tolist()
+    for a, scale in ((x, None), (q, s)):
+        y = HF.grouped_linear_block_fp8(a, off, experts, scale_a=scale) if E else HF.linear_block_fp8(a, *experts[0][:2], scale_x=scale)
+        for e, (w, sw, _) in enumerate(experts):
+            lo, hi = b[e], b[e + 1]
+            if hi > lo:
+                close(y[lo:hi], *product64(q[lo:hi], s[lo:hi], w, sw, None))
+
+
+@pytest.mark.parametrize("rows,E,K,N", EVERY_GATE_UP)
+def test_swiglu_every_way(rows, E, K, N):
+    from comfyui_amd import functional as HF
+    g = gen(rows + K + N)
+    x = tokens(g, rows, K)
+    q, s = HF.quant_block_fp8(x)
+    sizes = uneven(rows, E) or [rows]
+    experts = [(*weight(g, N, K), *weight(g, N, K)) for _ in sizes]
+    off = segments(sizes)
+    b = off.tolist()
+    for a, scale in ((x, None), (q, s)):
+        h, sh = HF.grouped_swiglu_block_fp8(a, off, experts, scale_a=scale) if E else HF.swiglu_block_fp8(a, *experts[0], scale_x=scale)
+        for e, ws in enumerate(experts):
+            lo, hi = b[e], b[e + 1]
+            if hi > lo:
+                close_cast(h[lo:hi], sh[lo:hi], q[lo:hi], s[lo:hi], *ws)
+
+
+@pytest.mark.parametrize("sizes,K,N", [([700, 130, 0, 300, 65, 500], 1552, 7696), ([900, 64, 330], 1040, 6800), ([257] * 5, 1040, 7952),
+                                       ([1500, 1100, 700], 656, 5264), ([200, 520, 90, 700], 656, 5264), ([1300, 40, 40], 528, 4624), ([480, 0, 700, 350, 420, 600, 250, 201], 2064, 8176)])
+def test_more_tiles_than_cus(sizes, K, N):
+    """Tiles of different heights, up to two for every CU and a few more."""
+    test_grouped_linear(sizes, K, N, torch.bfloat16)
+    test_grouped_swiglu(sizes, K, N // 2 // 16 * 16)
