@@ -58,13 +58,15 @@ def matrix64(w, s):
     return w.double() * s.double().repeat_interleave(BLOCK, 0)[:w.shape[0]].repeat_interleave(BLOCK, 1)[:, :w.shape[1]]
 
 
-def product64(q, s, w, sw, bias=None):
-    """The product in 64 bits and how far the device's sums may be from it."""
+def product64(q, s, w, sw, bias=None, exact=False):
+    """The product in 64 bits and how far the device's sums may be from it (exact: with products that are not cut)."""
     a, m = rows64(q, s), matrix64(w, sw)
     y = a @ m.t()
     err = (a.abs() @ m.abs().t()) * 2.0 ** -15.8
     if bias is not None:
         y, err = y + bias.double(), err + bias.double().abs() * 2.0 ** -23
+    if exact:
+        return y, err
     a8, m8 = a.abs().float(), m.abs().float()
     largest = torch.zeros_like(y, dtype=torch.float32)
     for k in range(0, a.shape[1], 8):
@@ -85,9 +87,9 @@ def silu64(v):
     return v * torch.sigmoid(v)
 
 
-def close_cast(h, sh, q, s, w1, s1, w3, s3):
+def close_cast(h, sh, q, s, w1, s1, w3, s3, exact=False):
     """h, sh against the unrounded 64-bit silu(g) * u of the same cast rows."""
-    (gt, gm), (u, um) = product64(q, s, w1, s1), product64(q, s, w3, s3)
+    (gt, gm), (u, um) = product64(q, s, w1, s1, exact=exact), product64(q, s, w3, s3, exact=exact)
     want = silu64(gt) * u
     # |silu'| <= 1.1; the fp32 exp, quotient and product add a few 2^-23 of the value, and |g| 2^-22 of it the exponent's rounding
     err = 1.1 * gm * (u.abs() + um) + silu64(gt).abs() * um + (2.0 ** -20 + gt.abs() * 2.0 ** -22) * want.abs()
@@ -442,3 +444,21 @@ def test_more_tiles_than_cus(sizes, K, N):
     """Tiles of different heights, up to two for every CU and a few more."""
     test_grouped_linear(sizes, K, N, torch.bfloat16)
     test_grouped_swiglu(sizes, K, N // 2 // 16 * 16)
+
+
+@pytest.mark.parametrize("rows,E,K,N", EVERY_GATE_UP)
+def test_swiglu_of_fp16_has_exact_products(rows, E, K, N):
+    """Products and sums of fp16 activations' gate/up are fp32: within 2^-15.8 of the sum of magnitudes, without what the e4m3fn instruction cuts."""
+    from comfyui_amd import functional as HF
+    g = gen(rows + K + N)
+    x = tokens(g, rows, K, torch.float16)
+    q, s = HF.quant_block_fp8(x)
+    sizes = uneven(rows, E) or [rows]
+    experts = [(*weight(g, N, K), *weight(g, N, K)) for _ in sizes]
+    off = segments(sizes)
+    b = off.tolist()
+    h, sh = HF.grouped_swiglu_block_fp8(x, off, experts) if E else HF.swiglu_block_fp8(x, *experts[0])
+    for e, ws in enumerate(experts):
+        lo, hi = b[e], b[e + 1]
+        if hi > lo:
+            close_cast(h[lo:hi], sh[lo:hi], q[lo:hi], s[lo:hi], *ws, exact=True)
