@@ -747,7 +747,10 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
     what = "grouped_linear_block_fp8"
     dt = _block_out_dtype(a, out_dtype, what)
     if shared is not None and a.dtype != FP8:
+        same = a_static is a and scale_static is None
         a, scale_a = quant_block_fp8(a)
+        if same:
+            a_static, scale_static = a, scale_a
     sa = _block_rows(a, scale_a, what + " a")
     dev = a.device
     arr, rows, N = _block_experts(a, offsets, experts, perm, dt, what)
@@ -788,7 +791,8 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
 def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, shared=None):
     """First half of every expert's SwiGLU feed-forward, silu(a w1^T) * (a w3^T), cast as quant_block_fp8 does:
     experts: list of (w1 [H, K], scale1, w3 [H, K], scale3); a, scale_a, offsets, perm as in grouped_linear_block_fp8.
-    -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]); everything before the cast is fp32.
+    -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]); everything before the cast is fp32, with fp16 a (not yet cast) its
+    products are exact as well (hdmoe_block_swiglu).
     shared: one more (w1, scale1, w3, scale3) over all rows of a, with a width of its own, in the same launch (with perm);
     -> (h, scales, h_shared, scales_shared)."""
     what = "grouped_swiglu_block_fp8"
