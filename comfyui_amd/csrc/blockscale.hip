@@ -75,7 +75,8 @@ __device__ __forceinline__ void cast_unit(const Src& x, uint32_t (&o)[2], float&
   s = top / 448.0f;
 }
 
-// 16 lanes hold a block of a row, 8 values each; a wave takes 4 neighbouring blocks. Bound by memory: 3.03 bytes per value of 16 bits.
+// 16 lanes hold a block of a row, 8 values each; a wave takes 4 neighbouring blocks. Bound by memory: 3.03 bytes per value of 16 bits
+// (32768 x 6912: 126 us, 5.4 TB/s).
 // bounds: NULL, or only the rows from bounds[0] to bounds[nbounds - 1] are cast.
 template <class Src>
 __global__ __launch_bounds__(256) void block_cast_kernel(const void* __restrict__ x, int rows, int K, int KB, uint8_t* __restrict__ q,
@@ -599,8 +600,11 @@ __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_
 #endif
 }
 
-// The same tile of 256 x 256 with the K loop of gen_block_fp8.py, for segments that fill it; one block of 160 KiB of LDS per CU. The first
-// loads of a block's next tile go out before the end of this one.
+// Tiles of 256 x 256 (gate/up: 256 x 128 of w1 and of w3) with the K loop of gen_block_fp8.py, for segments that fill them; one block of 160 KiB of
+// LDS per CU. The first loads of a block's next tile go out before the end of this one. Bound by MFMA issue at the clock that the power limit
+// leaves: a K step is 2470 cycles of which the MFMAs take 2048, at 1.6 GHz, and a tile's start and stores 6 us (16384 x 4096 x 8192 454-480 us,
+// 2.3-2.4 PFLOP/s; the 8-wave loop left to the compiler 650). Two waves a SIMD on 128 x 64 each: 4 x 8 tiles' accumulators and a step's fragments
+// are all of the 256 registers.
 #include "block_fp8_asm.inc"
 #define HDMOE_BLOCK_ACC \
   "={v[128:143]}"(acc[0]), "={v[144:159]}"(acc[1]), "={v[160:175]}"(acc[2]), "={v[176:191]}"(acc[3]), "={v[192:207]}"(acc[4]), \
@@ -773,7 +777,8 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
 // CAST: the activations are 16-bit rows; the block casts its own into LDS (rows of K + 16 bytes: 16 rows then hit all banks) while the
 // first weights are on their way, instead of a launch of its own in front.
 constexpr int STREAM_WAVES = 4, CAST_UNITS = 128;   // CAST: blocks of 128 values that a thread block can cast
-// Blocks of a CU at once: two where half of the LDS holds enough on its way, so that one starts while the other streams.
+// Blocks of a CU at once: two where half of the LDS holds enough on its way, so that one starts while the other streams (gate/up and down of 2 tokens,
+// 2560 x 6912 x 2560, 33.2 us, 42.4 with one).
 constexpr int stream_blocks(int ft, int tt, bool cast) { return cast || ft * tt <= 2 ? 2 : 1; }
 // Of a wave: a K block of weights and activations with their scales, and how many of them its ring has
 constexpr int stream_slot(int ft, int tt, bool swiglu, bool cast) { return 2048 * (ft + (cast ? 0 : tt)) + 256 * (1 + (swiglu ? 1 : 0) + (cast ? 0 : 1)); }
@@ -1195,7 +1200,7 @@ Plan plan_of(bool swiglu, int a_dtype, const Sizes& z) {
     for (int ft = swiglu ? 2 : 1; ft <= 4; ft *= 2) {
       Plan p = {tt, ft, false, 0, 0, 0};
       if (x16 && tt == 1) {
-        // a block casts for itself where its threads hold all of it at once: a launch (4 us) less
+        // a block casts for itself what takes its threads 8 trips at most: a launch (4 us) less
         const int whole = z.rows > z.rows_static ? z.rows : z.rows_static;
         p.lds_rows = whole < 16 ? whole : 16;
         p.cast_inside = (long long)p.lds_rows * ((K + BLK - 1) / BLK) <= CAST_UNITS && (long long)whole * K * 2 <= 0x7fffffff;
