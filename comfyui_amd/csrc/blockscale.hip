@@ -1094,6 +1094,7 @@ int check_sizes(const char* what, const char* which, long long rows, int K, int 
     return hdmoe_fail(HDMOE_E_SHAPE, "%s%s: rows=%lld K=%d N=%d (K and N must be multiples of 16)", what, which, rows, K, N);
   if ((long long)N * K > 0x7fffffffll || (long long)256 * K > 0x7fffffffll)
     return hdmoe_fail(HDMOE_E_SHAPE, "%s%s: K=%d N=%d: a weight must be smaller than 2 GiB", what, which, K, N);
+  if ((long long)256 * N * 2 > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s%s: N=%d: at most 4194288", what, which, N);   // a tile's rows of the output
   return HDMOE_OK;
 }
 

@@ -400,7 +400,8 @@ typedef struct hdmoe_block_rows {
 /* Experts over the row segments of a dispatched batch, and optionally one more group over all rows of another input (a shared
  * expert, or the one weight of a dense Linear). Expert e takes rows [offsets[e], offsets[e + 1]) (ascending, device; bounds beyond
  * 0 .. rows are cut off); rows in no segment are left as they were. perm (NULL = the rows are in segment order): sorted row r is
- * row perm[r] / 2 of routed.a [T,K] and its scales. All matrices start on 16 bytes; K % 16 == 0, N % 16 == 0. */
+ * row perm[r] / 2 of routed.a [T,K] and its scales. All matrices start on 16 bytes; K % 16 == 0, N % 16 == 0,
+ * K < 2^23, N < 2^22, and a weight is smaller than 2 GiB. */
 typedef struct hdmoe_block_args {
   int a_dtype;        /* HDMOE_W_E4M3FN with scales, or HDMOE_W_BF16 / HDMOE_W_F16: the call casts the rows first */
   int out_dtype;      /* HDMOE_W_BF16 or HDMOE_W_F16 (hdmoe_block_linear: output and bias; 16-bit a: its type) */

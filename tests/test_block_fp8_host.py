@@ -48,7 +48,7 @@ def arguments(p, **changes):
 
 REFUSED = [dict(out_dtype=1), dict(a_dtype=3), dict(E=33), dict(E=-1), dict(rows=-1), dict(K=0), dict(K=136), dict(N=0), dict(N=24), dict(E=0),
            dict(rows_static=-1), dict(rows_static=3, K_static=128, N_static=100), dict(perm=4096, T=3), dict(K=2 ** 20, N=2 ** 12),
-           dict(N=2 ** 30, K=16)]
+           dict(N=2 ** 30, K=16), dict(N=2 ** 22, K=16), dict(N=16, K=2 ** 23)]
 
 
 @pytest.mark.parametrize("changes", REFUSED)
