@@ -11,6 +11,11 @@ import torch
 from . import _lib
 from ._lib import FfnWeights, LayerArgs, LayerLayout, W_BF16, W_E4M3FN, check, lib, ptr
 
+try:
+    from . import _block_calls
+except ImportError as e:
+    raise RuntimeError("comfyui_amd/_block_calls.so is missing or was built for another torch. Build it with `python -m comfyui_amd.build`.") from e
+
 FP8 = torch.float8_e4m3fn
 BF16 = torch.bfloat16
 F16 = torch.float16
@@ -551,17 +556,31 @@ def moe_ffn(x2d, gate_w, experts, shared, H, Hs, weight_dtype, out=None, workspa
 
 
 # ---- e4m3fn with a scale for each block of 128 -------------------------------------------------------------------
-# (Calls on a few rows run for about as long as their checks take: attributes are read once, and the device is switched only
-# where it is another one.)
+# (Calls on a few rows run for about as long as their checks take. _block_calls makes the ordinary ones, with the same checks, and answers
+# None where something is to be done first, to be switched or to be refused: that happens here.)
 
 BLOCK = 128
 _HERE = contextlib.nullcontext()
 _ACT_CODE = {BF16: W_BF16, F16: _lib.W_F16, FP8: W_E4M3FN}
+_OUT_CODE = {None: -1, BF16: W_BF16, F16: _lib.W_F16}
+_block_calls.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.hdmoe_quant_block_fp8, lib.hdmoe_block_workspace_bytes,
+                                                                    lib.hdmoe_block_linear, lib.hdmoe_block_swiglu)))
 
 
 def _raw_stream(t):
     """_stream without the object around the handle."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _stream_here(t):
+    """The current stream's handle where the tensor is on the current device, else None."""
+    d = t.get_device()
+    return torch._C._cuda_getCurrentRawStream(d) if d >= 0 and d == torch._C._cuda_getDevice() else None
+
+
+def _done(r):
+    """What a function of _block_calls returned, or the library's error."""
+    return check(r) if r.__class__ is int else r
 
 
 def _on(device):
@@ -582,6 +601,11 @@ def quant_block_fp8(x):
     """Cast of 16-bit rows with a scale for every 128 values: x [..., K] bf16 or fp16, K a multiple of 16 ->
     (float8_e4m3fn of x's shape, fp32 scales [rows, ceil(K / 128)] as block_scales lays them out).
     scale = max(max|x|, 2^-96) / 448, value = e4m3fn(x * (448 / max(max|x|, 2^-96)))."""
+    st = _stream_here(x)
+    if st is not None:
+        r = _block_calls.cast(x, st)
+        if r is not None:
+            return _done(r)
     dt = _act_dtype(x, "quant_block_fp8 x")
     _need_hip(x, "quant_block_fp8 x")
     K = x.shape[-1]
@@ -716,6 +740,11 @@ def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype
     [ceil(N / 128), ceil(K / 128)]; x bf16 or fp16 (cast as quant_block_fp8 does), or float8_e4m3fn with its scales scale_x
     [rows, ceil(K / 128)] (laid out anew unless they are as quant_block_fp8 returns them). -> [rows, N] of x's type (out_dtype, bf16
     unless given, for float8_e4m3fn x). K and N are multiples of 16. The sums are fp32; bias joins them before the one rounding."""
+    st = _stream_here(x)
+    if st is not None:
+        r = _block_calls.linear(x, weight, scale_weight, bias, scale_x, _OUT_CODE.get(out_dtype, -2), st)
+        if r is not None:
+            return _done(r)
     what = "linear_block_fp8"
     dt = _block_out_dtype(x, out_dtype, what)
     s = _block_rows(x, scale_x, what + " x")
@@ -744,6 +773,11 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
     segment holds are not written. -> out [rows, N].
     shared: one more (weight, scale, bias) over all rows of a_static (with scale_static), of sizes of its own, in the same launch;
     -> (out, out_static)."""
+    st = _stream_here(a) if shared is None else None
+    if st is not None:
+        r = _block_calls.grouped_linear(a, offsets, experts, scale_a, _OUT_CODE.get(out_dtype, -2), perm, st)
+        if r is not None:
+            return _done(r)
     what = "grouped_linear_block_fp8"
     dt = _block_out_dtype(a, out_dtype, what)
     if shared is not None and a.dtype != FP8:
@@ -795,6 +829,11 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
     products are exact as well (hdmoe_block_swiglu).
     shared: one more (w1, scale1, w3, scale3) over all rows of a, with a width of its own, in the same launch (with perm);
     -> (h, scales, h_shared, scales_shared)."""
+    st = _stream_here(a) if shared is None else None
+    if st is not None:
+        r = _block_calls.grouped_swiglu(a, offsets, experts, scale_a, perm, st)
+        if r is not None:
+            return _done(r)
     what = "grouped_swiglu_block_fp8"
     sa = _block_rows(a, scale_a, what + " a")
     dev = a.device
@@ -832,6 +871,11 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
 def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None):
     """First half of one dense SwiGLU feed-forward, silu(x w1^T) * (x w3^T), cast as quant_block_fp8 does: x and scale_x as in
     linear_block_fp8 -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]), what linear_block_fp8 takes for w2."""
+    st = _stream_here(x)
+    if st is not None:
+        r = _block_calls.swiglu(x, w1, scale_w1, w3, scale_w3, scale_x, st)
+        if r is not None:
+            return _done(r)
     what = "swiglu_block_fp8"
     s = _block_rows(x, scale_x, what + " x")
     rows, K = x.shape

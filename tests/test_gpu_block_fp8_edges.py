@@ -170,3 +170,53 @@ def test_a_row_that_is_not_finite_spoils_no_other(rows, N, dtype):
     h, sh = HF.swiglu_block_fp8(x, wn, w[1], *w3)
     values = h.float() * sh.repeat_interleave(128, 1)[:, :N]
     assert torch.isnan(values[:, 128:256]).all() and torch.isfinite(values[fine][:, :128]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 20, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_both_ways_to_make_a_call_are_one(rows, dtype, monkeypatch):
+    """The compiled calls against the ones made here: the same bytes, shapes, strides and refusals."""
+    from comfyui_amd import functional as HF
+    g = gen(rows)
+    K, N, E = 656, 272, 3
+    x = tokens(g, rows, K, dtype)
+    q, s = HF.quant_block_fp8(x)
+    bias = torch.randn(N, generator=g, device="cuda").to(dtype)
+    experts = [(*weight(g, N, K), bias if e else None) for e in range(E)]
+    up = [(*weight(g, N, K), *weight(g, N, K)) for _ in range(E)]
+    off, off2 = segments([rows - rows // 2, 0, rows // 2]), segments([rows, 0, rows])
+    perm = torch.randperm(2 * rows, generator=torch.Generator().manual_seed(rows)).to(torch.int32).cuda()
+    w, sw, _ = experts[0]
+    calls = [lambda: HF.quant_block_fp8(x), lambda: HF.quant_block_fp8(x.view(1, rows, K)), lambda: HF.linear_block_fp8(x, w, sw, bias=bias),
+             lambda: HF.linear_block_fp8(q, w, sw, scale_x=s), lambda: HF.linear_block_fp8(q, w, sw, scale_x=s.contiguous(), out_dtype=dtype),
+             lambda: HF.linear_block_fp8(x, w, sw, out_dtype=dtype), lambda: HF.grouped_linear_block_fp8(x, off, experts),
+             lambda: HF.grouped_linear_block_fp8(q, off2, tuple(map(list, experts)), scale_a=s, perm=perm, out_dtype=dtype),
+             lambda: HF.swiglu_block_fp8(x, *up[0]), lambda: HF.swiglu_block_fp8(q, *up[0], scale_x=s),
+             lambda: HF.grouped_swiglu_block_fp8(x, off, up), lambda: HF.grouped_swiglu_block_fp8(q, off2, up, scale_a=s, perm=perm)]
+    other = torch.float16 if dtype == torch.bfloat16 else torch.bfloat16
+    refused = [lambda: HF.linear_block_fp8(x, w, sw, bias=bias.to(other)), lambda: HF.linear_block_fp8(x, w, sw, out_dtype=other),
+               lambda: HF.linear_block_fp8(x, w, sw, scale_x=s), lambda: HF.linear_block_fp8(q, w, sw), lambda: HF.linear_block_fp8(x, w.cpu(), sw),
+               lambda: HF.linear_block_fp8(x, w, sw[:1]), lambda: HF.linear_block_fp8(x[:, :K - 16], w, sw), lambda: HF.linear_block_fp8(x.float(), w, sw),
+               lambda: HF.linear_block_fp8(x, w.float(), sw), lambda: HF.linear_block_fp8(x, w, sw.double()), lambda: HF.linear_block_fp8(x, w[:-8], sw),
+               lambda: HF.grouped_linear_block_fp8(x, off.long(), experts), lambda: HF.grouped_linear_block_fp8(x, off[:-1], experts),
+               lambda: HF.grouped_linear_block_fp8(x, off, []), lambda: HF.grouped_linear_block_fp8(x, off2, experts, perm=perm[:-1]),
+               lambda: HF.grouped_linear_block_fp8(x, off, experts[:2] + [(experts[2][0][:-16], experts[2][1], None)]),
+               lambda: HF.grouped_swiglu_block_fp8(x, off, up[:2] + [(*up[2][:2], up[2][2][:, :-16], up[2][3])]),
+               lambda: HF.swiglu_block_fp8(x[None], *up[0]), lambda: HF.quant_block_fp8(x.t()), lambda: HF.quant_block_fp8(x[:, :24].contiguous())]
+
+    def outcome(f):
+        try:
+            f()
+        except Exception as e:  # noqa: BLE001
+            return type(e), str(e)
+        return None
+
+    made, no = [f() for f in calls], [outcome(f) for f in refused]
+    with monkeypatch.context() as m:
+        m.setattr(HF, "_stream_here", lambda t: None)
+        slow, slow_no = [f() for f in calls], [outcome(f) for f in refused]
+    for a, b in zip(made, slow):
+        for t, u in zip(*((v if isinstance(v, tuple) else (v,)) for v in (a, b))):
+            assert t.dtype == u.dtype and t.shape == u.shape and t.stride() == u.stride()
+            assert torch.equal(t.contiguous().view(torch.uint8), u.contiguous().view(torch.uint8))
+    assert no == slow_no and all(n is not None for n in no)
