@@ -9,6 +9,7 @@
 #include <ATen/ops/empty_strided.h>
 
 #include <exception>
+#include <initializer_list>
 
 #include "../../include/hdmoe.h"
 
@@ -122,6 +123,15 @@ struct Call {
     activations(a.fixed);
     return rows;
   }
+  // The static group of another call of one group
+  void with(const Call& d) {
+    need(d.act == act && d.x.device() == x.device());
+    a.rows_static = d.a.rows_static;
+    a.K_static = d.a.K_static;
+    a.N_static = d.a.N_static;
+    a.shared = d.a.shared;
+    a.fixed = d.a.fixed;
+  }
   void activations(hdmoe_block_rows& r) {
     r.a = x.const_data_ptr();
     if (scale.defined()) {
@@ -154,12 +164,16 @@ struct Call {
   }
 };
 
-PyObject* pair(const at::Tensor& q, const at::Tensor& s) {
-  PyObject* const r = PyTuple_New(2);
+PyObject* tuple(std::initializer_list<at::Tensor> tensors) {
+  PyObject* const r = PyTuple_New(tensors.size());
   if (r == nullptr) return nullptr;
-  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(q));
-  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(s));
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : tensors) PyTuple_SET_ITEM(r, i++, THPVariable_Wrap(t));
   return r;
+}
+PyObject* const* items(PyObject* o, Py_ssize_t n) {
+  need((PyList_Check(o) || PyTuple_Check(o)) && PySequence_Fast_GET_SIZE(o) == n);
+  return PySequence_Fast_ITEMS(o);
 }
 
 // f's answer; None where f threw
@@ -190,7 +204,7 @@ PyObject* do_cast(PyObject*, PyObject* const* o, Py_ssize_t count) {
     const at::Tensor q = at::empty(x.sizes(), at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(x.device()));
     const at::Tensor s = at::empty_strided({rows, blocks(K)}, {1, rows}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
     const int rc = cast_rows(act, x.const_data_ptr(), rows, static_cast<int>(K), q.mutable_data_ptr(), static_cast<float*>(s.mutable_data_ptr()), rows, stream_of(o[1]));
-    return rc != 0 ? PyLong_FromLong(rc) : pair(q, s);
+    return rc != 0 ? PyLong_FromLong(rc) : tuple({q, s});
   });
 }
 
@@ -208,28 +222,40 @@ PyObject* do_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
   });
 }
 
-// (a, offsets, experts, scale_a, out_dtype, perm, stream)
+// (a, offsets, experts, scale_a, out_dtype, perm, shared, a_static, scale_static, stream)
 PyObject* do_grouped_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(7)
+  HDMOE_ARGUMENTS(10)
   return answer([&]() -> PyObject* {
     Call c(o[0], o[3]);
     c.a.out_dtype = c.type(o[4]);
+    const at::ScalarType type = c.a.out_dtype == HDMOE_W_BF16 ? at::kBFloat16 : at::kHalf;
     const int64_t n = c.routed(o[1], o[2], o[5], false, c.a.out_dtype);
-    const at::Tensor y = c.make(n, c.N, c.a.out_dtype == HDMOE_W_BF16 ? at::kBFloat16 : at::kHalf);
+    const at::Tensor y = c.make(n, c.N, type);
     c.a.routed.out = y.mutable_data_ptr();
-    const int rc = c.run(false, stream_of(o[6]));
-    return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(y);
+    if (o[6] == Py_None) {
+      const int rc = c.run(false, stream_of(o[9]));
+      return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(y);
+    }
+    need(c.act == HDMOE_W_E4M3FN);   // (16-bit rows of two groups: cast before)
+    Call d(o[7], o[8]);
+    const int64_t m = d.dense(items(o[6], 3), false, c.a.out_dtype);
+    const at::Tensor z = d.make(m, d.N, type);
+    d.a.fixed.out = z.mutable_data_ptr();
+    c.with(d);
+    const int rc = c.run(false, stream_of(o[9]));
+    return rc != 0 ? PyLong_FromLong(rc) : tuple({y, z});
   });
 }
 
-PyObject* gate_up(Call& c, hdmoe_block_rows& r, int64_t n, PyObject* stream) {
-  const at::Tensor h = c.make(n, c.N, at::kFloat8_e4m3fn), s = c.scales(n, c.N);
-  r.out = h.mutable_data_ptr();
-  r.scale_out = static_cast<float*>(s.mutable_data_ptr());
-  r.scale_out_stride = n;
-  const int rc = c.run(true, stream_of(stream));
-  return rc != 0 ? PyLong_FromLong(rc) : pair(h, s);
-}
+// What a gate/up writes for n rows
+struct Cast {
+  at::Tensor h, s;
+  Cast(const Call& c, hdmoe_block_rows& r, int64_t n) : h(c.make(n, c.N, at::kFloat8_e4m3fn)), s(c.scales(n, c.N)) {
+    r.out = h.mutable_data_ptr();
+    r.scale_out = static_cast<float*>(s.mutable_data_ptr());
+    r.scale_out_stride = n;
+  }
+};
 
 // (x, w1, scale1, w3, scale3, scale_x, stream)
 PyObject* do_swiglu(PyObject*, PyObject* const* o, Py_ssize_t count) {
@@ -238,18 +264,30 @@ PyObject* do_swiglu(PyObject*, PyObject* const* o, Py_ssize_t count) {
     Call c(o[0], o[5]);
     c.a.out_dtype = HDMOE_W_BF16;
     const int64_t n = c.dense(o + 1, true, HDMOE_W_BF16);
-    return gate_up(c, c.a.fixed, n, o[6]);
+    const Cast out(c, c.a.fixed, n);
+    const int rc = c.run(true, stream_of(o[6]));
+    return rc != 0 ? PyLong_FromLong(rc) : tuple({out.h, out.s});
   });
 }
 
-// (a, offsets, experts, scale_a, perm, stream)
+// (a, offsets, experts, scale_a, perm, shared, stream)
 PyObject* do_grouped_swiglu(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(6)
+  HDMOE_ARGUMENTS(7)
   return answer([&]() -> PyObject* {
     Call c(o[0], o[3]);
     c.a.out_dtype = HDMOE_W_BF16;
     const int64_t n = c.routed(o[1], o[2], o[4], true, HDMOE_W_BF16);
-    return gate_up(c, c.a.routed, n, o[5]);
+    const Cast out(c, c.a.routed, n);
+    if (o[5] == Py_None) {
+      const int rc = c.run(true, stream_of(o[6]));
+      return rc != 0 ? PyLong_FromLong(rc) : tuple({out.h, out.s});
+    }
+    Call d(o[0], o[3]);
+    const int64_t m = d.dense(items(o[5], 4), true, HDMOE_W_BF16);
+    const Cast shared(d, d.a.fixed, m);
+    c.with(d);
+    const int rc = c.run(true, stream_of(o[6]));
+    return rc != 0 ? PyLong_FromLong(rc) : tuple({out.h, out.s, shared.h, shared.s});
   });
 }
 

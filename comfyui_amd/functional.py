@@ -2,7 +2,6 @@
 outputs with torch (device memory and stream plumbing only) and enqueue the HIP
 kernels on torch's current stream. Nothing here computes with torch.
 """
-import array
 import contextlib
 import ctypes
 
@@ -696,30 +695,11 @@ def _block_experts(a, offsets, experts, perm, dtype, what):
         rows = T * _lib.TOPK
         if perm.dtype != torch.int32 or perm.shape != (rows,) or perm.device != dev or not perm.is_contiguous():
             raise ValueError(f"{what}: perm must be contiguous int32 [{rows}] on {dev}")
-    # (_block_matrix and _block_weights for all experts, without a call each: it takes the few that fail)
-    index, words = a.get_device(), array.array("Q")
-    first = experts[0][0]
-    N = first.shape[0] if first.dim() == 2 else -1
-    of_w, of_s, of_b, f32 = (N, K), (-(-N // BLOCK), -(-K // BLOCK)), (N,), torch.float32
-    for entry in experts:
-        if dtype is None:
-            w1, s1, w3, s3 = entry
-            if (w3.dtype is not FP8 or w3.shape != of_w or w3.get_device() != index or not w3.is_contiguous()
-                    or s3.dtype is not f32 or s3.shape != of_s or s3.get_device() != index or not s3.is_contiguous()):
-                _block_matrix(w3, s3, K, index, what, (of_w, of_s))
-            more = (w3.data_ptr(), s3.data_ptr(), 0)
-        else:
-            w1, s1, bias = entry
-            more = (0, 0, 0)
-            if bias is not None:
-                if bias.dtype is not dtype or bias.shape != of_b or bias.get_device() != index or not bias.is_contiguous():
-                    _block_weights(_lib.BlockWeights(), entry, K, dtype, index, what, (of_w, of_s))
-                more = (0, 0, bias.data_ptr())
-        if (w1.dtype is not FP8 or w1.shape != of_w or w1.get_device() != index or not w1.is_contiguous()
-                or s1.dtype is not f32 or s1.shape != of_s or s1.get_device() != index or not s1.is_contiguous()):
-            _block_matrix(w1, s1, K, index, what, (of_w, of_s))
-        words.extend((w1.data_ptr(), s1.data_ptr(), *more))
-    return (_lib.BlockWeights * E).from_buffer(words), rows, N
+    arr = (_lib.BlockWeights * E)()
+    shapes, index = None, a.get_device()
+    for w, entry in zip(arr, experts):
+        shapes = _block_weights(w, entry, K, dtype, index, what, shapes)
+    return arr, rows, shapes[0][0]
 
 
 def _block_call(fn, swiglu, args, a):
@@ -773,18 +753,19 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
     segment holds are not written. -> out [rows, N].
     shared: one more (weight, scale, bias) over all rows of a_static (with scale_static), of sizes of its own, in the same launch;
     -> (out, out_static)."""
-    st = _stream_here(a) if shared is None else None
-    if st is not None:
-        r = _block_calls.grouped_linear(a, offsets, experts, scale_a, _OUT_CODE.get(out_dtype, -2), perm, st)
-        if r is not None:
-            return _done(r)
     what = "grouped_linear_block_fp8"
-    dt = _block_out_dtype(a, out_dtype, what)
     if shared is not None and a.dtype != FP8:
+        out_dtype = _block_out_dtype(a, out_dtype, what)
         same = a_static is a and scale_static is None
         a, scale_a = quant_block_fp8(a)
         if same:
             a_static, scale_static = a, scale_a
+    st = _stream_here(a)
+    if st is not None:
+        r = _block_calls.grouped_linear(a, offsets, experts, scale_a, _OUT_CODE.get(out_dtype, -2), perm, shared, a_static, scale_static, st)
+        if r is not None:
+            return _done(r)
+    dt = _block_out_dtype(a, out_dtype, what)
     sa = _block_rows(a, scale_a, what + " a")
     dev = a.device
     arr, rows, N = _block_experts(a, offsets, experts, perm, dt, what)
@@ -829,9 +810,9 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
     products are exact as well (hdmoe_block_swiglu).
     shared: one more (w1, scale1, w3, scale3) over all rows of a, with a width of its own, in the same launch (with perm);
     -> (h, scales, h_shared, scales_shared)."""
-    st = _stream_here(a) if shared is None else None
+    st = _stream_here(a)
     if st is not None:
-        r = _block_calls.grouped_swiglu(a, offsets, experts, scale_a, perm, st)
+        r = _block_calls.grouped_swiglu(a, offsets, experts, scale_a, perm, shared, st)
         if r is not None:
             return _done(r)
     what = "grouped_swiglu_block_fp8"

@@ -187,12 +187,16 @@ def test_both_ways_to_make_a_call_are_one(rows, dtype, monkeypatch):
     off, off2 = segments([rows - rows // 2, 0, rows // 2]), segments([rows, 0, rows])
     perm = torch.randperm(2 * rows, generator=torch.Generator().manual_seed(rows)).to(torch.int32).cuda()
     w, sw, _ = experts[0]
+    wide = (*weight(g, 400, K), *weight(g, 400, K))
     calls = [lambda: HF.quant_block_fp8(x), lambda: HF.quant_block_fp8(x.view(1, rows, K)), lambda: HF.linear_block_fp8(x, w, sw, bias=bias),
              lambda: HF.linear_block_fp8(q, w, sw, scale_x=s), lambda: HF.linear_block_fp8(q, w, sw, scale_x=s.contiguous(), out_dtype=dtype),
              lambda: HF.linear_block_fp8(x, w, sw, out_dtype=dtype), lambda: HF.grouped_linear_block_fp8(x, off, experts),
              lambda: HF.grouped_linear_block_fp8(q, off2, tuple(map(list, experts)), scale_a=s, perm=perm, out_dtype=dtype),
              lambda: HF.swiglu_block_fp8(x, *up[0]), lambda: HF.swiglu_block_fp8(q, *up[0], scale_x=s),
-             lambda: HF.grouped_swiglu_block_fp8(x, off, up), lambda: HF.grouped_swiglu_block_fp8(q, off2, up, scale_a=s, perm=perm)]
+             lambda: HF.grouped_swiglu_block_fp8(x, off, up), lambda: HF.grouped_swiglu_block_fp8(q, off2, up, scale_a=s, perm=perm),
+             lambda: HF.grouped_swiglu_block_fp8(x, off2, up, perm=perm, shared=wide), lambda: HF.grouped_swiglu_block_fp8(q, off, up, scale_a=s, shared=wide),
+             lambda: HF.grouped_linear_block_fp8(x, off2, experts, perm=perm, shared=experts[1], a_static=x),
+             lambda: HF.grouped_linear_block_fp8(q, off, experts, scale_a=s, shared=(*weight(gen(9), 400, 144), None), a_static=x[:, :144].contiguous(), out_dtype=dtype)]
     other = torch.float16 if dtype == torch.bfloat16 else torch.bfloat16
     refused = [lambda: HF.linear_block_fp8(x, w, sw, bias=bias.to(other)), lambda: HF.linear_block_fp8(x, w, sw, out_dtype=other),
                lambda: HF.linear_block_fp8(x, w, sw, scale_x=s), lambda: HF.linear_block_fp8(q, w, sw), lambda: HF.linear_block_fp8(x, w.cpu(), sw),
@@ -211,6 +215,9 @@ def test_both_ways_to_make_a_call_are_one(rows, dtype, monkeypatch):
             return type(e), str(e)
         return None
 
+    refused += [lambda: HF.grouped_swiglu_block_fp8(x, off, up, shared=up[0][:3]), lambda: HF.grouped_linear_block_fp8(x, off, experts, shared=experts[0]),
+                lambda: HF.grouped_linear_block_fp8(q, off, experts, scale_a=s, shared=experts[0], a_static=q),
+                lambda: HF.grouped_swiglu_block_fp8(x, off, up, shared=(*up[0][:2], up[0][2][:-16], up[0][3]))]
     made, no = [f() for f in calls], [outcome(f) for f in refused]
     with monkeypatch.context() as m:
         m.setattr(HF, "_stream_here", lambda t: None)
