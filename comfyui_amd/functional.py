@@ -806,8 +806,8 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
 def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, shared=None):
     """First half of every expert's SwiGLU feed-forward, silu(a w1^T) * (a w3^T), cast as quant_block_fp8 does:
     experts: list of (w1 [H, K], scale1, w3 [H, K], scale3); a, scale_a, offsets, perm as in grouped_linear_block_fp8.
-    -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]); everything before the cast is fp32, with fp16 a (not yet cast) its
-    products are exact as well (hdmoe_block_swiglu).
+    -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]); everything before the cast is fp32; its products are exact as
+    well on few rows and with fp16 a (not yet cast).
     shared: one more (w1, scale1, w3, scale3) over all rows of a, with a width of its own, in the same launch (with perm);
     -> (h, scales, h_shared, scales_shared)."""
     st = _stream_here(a)

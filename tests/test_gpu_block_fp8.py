@@ -462,3 +462,22 @@ def test_swiglu_of_fp16_has_exact_products(rows, E, K, N):
         lo, hi = b[e], b[e + 1]
         if hi > lo:
             close_cast(h[lo:hi], sh[lo:hi], q[lo:hi], s[lo:hi], *ws, exact=True)
+
+
+@pytest.mark.parametrize("rows,E,K,N", [(1, 0, 2560, 6912), (2, 4, 2560, 1040), (5, 0, 592, 64), (36, 3, 272, 80), (48, 3, 656, 400), (16, 0, 6912, 272)])
+def test_swiglu_of_few_rows_has_exact_products(rows, E, K, N):
+    """So it is in bf16 where the few-row kernels run."""
+    from comfyui_amd import functional as HF
+    g = gen(rows + K + N)
+    x = tokens(g, rows, K)
+    q, s = HF.quant_block_fp8(x)
+    sizes = uneven(rows, E) or [rows]
+    experts = [(*weight(g, N, K), *weight(g, N, K)) for _ in sizes]
+    off = segments(sizes)
+    b = off.tolist()
+    for a, scale in ((x, None), (q, s)):
+        h, sh = HF.grouped_swiglu_block_fp8(a, off, experts, scale_a=scale) if E else HF.swiglu_block_fp8(a, *experts[0], scale_x=scale)
+        for e, ws in enumerate(experts):
+            lo, hi = b[e], b[e + 1]
+            if hi > lo:
+                close_cast(h[lo:hi], sh[lo:hi], q[lo:hi], s[lo:hi], *ws, exact=True)
