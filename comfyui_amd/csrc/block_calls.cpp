@@ -20,6 +20,12 @@ void need(bool ok) {
   if (!ok) throw Otherwise();
 }
 
+// Other Python threads may run while this one allocates or enqueues
+struct Unlocked {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 decltype(&hdmoe_quant_block_fp8) cast_rows;
 decltype(&hdmoe_block_workspace_bytes) workspace_bytes;
 decltype(&hdmoe_block_linear) linear;
@@ -139,11 +145,16 @@ struct Call {
       r.scale_a_stride = rows;
     }
   }
-  at::Tensor make(int64_t n, int64_t m, at::ScalarType type) const { return at::empty({n, m}, at::TensorOptions().dtype(type).device(x.device())); }
+  at::Tensor make(int64_t n, int64_t m, at::ScalarType type) const {
+    Unlocked u;
+    return at::empty({n, m}, at::TensorOptions().dtype(type).device(x.device()));
+  }
   at::Tensor scales(int64_t n, int64_t m) const {
+    Unlocked u;
     return at::empty_strided({n, blocks(m)}, {1, n}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
   }
   int run(bool gate_up, void* stream) {
+    Unlocked u;
     at::Tensor room;
     if (gate_up || act != HDMOE_W_E4M3FN) {
       const size_t n = workspace_bytes(&a, gate_up);
@@ -201,9 +212,15 @@ PyObject* do_cast(PyObject*, PyObject* const* o, Py_ssize_t count) {
     const int64_t K = x.size(-1);
     need(K > 0 && K < (1ll << 30) && x.numel() > 0);
     const int64_t rows = x.numel() / K;
-    const at::Tensor q = at::empty(x.sizes(), at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(x.device()));
-    const at::Tensor s = at::empty_strided({rows, blocks(K)}, {1, rows}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
-    const int rc = cast_rows(act, x.const_data_ptr(), rows, static_cast<int>(K), q.mutable_data_ptr(), static_cast<float*>(s.mutable_data_ptr()), rows, stream_of(o[1]));
+    void* const stream = stream_of(o[1]);
+    at::Tensor q, s;
+    int rc;
+    {
+      Unlocked u;
+      q = at::empty(x.sizes(), at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(x.device()));
+      s = at::empty_strided({rows, blocks(K)}, {1, rows}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
+      rc = cast_rows(act, x.const_data_ptr(), rows, static_cast<int>(K), q.mutable_data_ptr(), static_cast<float*>(s.mutable_data_ptr()), rows, stream);
+    }
     return rc != 0 ? PyLong_FromLong(rc) : tuple({q, s});
   });
 }

@@ -227,3 +227,38 @@ def test_both_ways_to_make_a_call_are_one(rows, dtype, monkeypatch):
             assert t.dtype == u.dtype and t.shape == u.shape and t.stride() == u.stride()
             assert torch.equal(t.contiguous().view(torch.uint8), u.contiguous().view(torch.uint8))
     assert no == slow_no and all(n is not None for n in no)
+
+
+def test_threads():
+    """Calls from several Python threads on streams of their own."""
+    import threading
+
+    from comfyui_amd import functional as HF
+    g = gen(4)
+    xs = [tokens(g, rows, 656) for rows in (2, 50, 300, 7)]
+    up = [(*weight(g, 272, 656), *weight(g, 272, 656)) for _ in range(2)]
+    w, sw = weight(g, 400, 272)
+
+    def run(x):
+        n = x.shape[0]
+        h, sh = HF.grouped_swiglu_block_fp8(x, off[n], up)
+        return HF.linear_block_fp8(h, w, sw, scale_x=sh)
+
+    off = {x.shape[0]: segments([x.shape[0] // 2, x.shape[0] - x.shape[0] // 2]) for x in xs}
+    want = [run(x) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [run(xs[i]) for _ in range(30)]
+            torch.cuda.current_stream().synchronize()
+        if not all(torch.equal(y, want[i]) for y in got):
+            bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
