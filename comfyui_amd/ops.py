@@ -412,8 +412,8 @@ class block_fp8_ops(manual_cast):
             return HF.linear_block_fp8(x2, weight, scale, bias=bias).reshape(*input.shape[:-1], weight.shape[0])
 
         def _spread(self, weight):
-            """scale_weight as one value per element, in the weight's dtype on its device."""
-            s = self.scale_weight.to(device=weight.device, dtype=weight.dtype)
+            """scale_weight as one fp32 value per element, on the weight's device (fp16 would lose scales below 2^-25)."""
+            s = self.scale_weight.to(device=weight.device, dtype=torch.float32)
             n, k = weight.shape
             return s.repeat_interleave(HF.BLOCK, 0)[:n].repeat_interleave(HF.BLOCK, 1)[:, :k]
 
@@ -422,12 +422,15 @@ class block_fp8_ops(manual_cast):
             if inplace:
                 weight *= s
                 return weight
-            return weight * s
+            return (weight * s).to(weight.dtype)
 
         def set_weight(self, weight, inplace_update=False, seed=None, return_weight=False, **kwargs):
+            """The stored scales stay: a value past 448 of its block's scale becomes 448 of it, and a block whose scale is 0 stays zero
+            whatever a patch adds to it."""
             from .float_round import stochastic_rounding
-            weight = weight / self._spread(weight)
-            if weight.is_cuda and weight.dtype in (torch.float32, BF16):
+            s = self._spread(weight)
+            weight = torch.where(s != 0, weight / s, torch.zeros_like(s))
+            if weight.is_cuda and weight.dtype == torch.float32:
                 weight = HF.stochastic_round_e4m3fn(weight.contiguous(), None, seed or 0)
             else:
                 weight = stochastic_rounding(weight, FP8, seed=seed)
