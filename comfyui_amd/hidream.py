@@ -97,6 +97,8 @@ def _fusable_dtype(ffns):
         # any Linear that follows the operations contract (this package's or ComfyUI's own classes)
         if not isinstance(l, torch.nn.Linear) or l.bias is not None or len(getattr(l, "bias_function", ())) > 0:
             return None
+        if isinstance(l, amd_ops.block_fp8_ops.Linear):   # its scales are a matrix, whatever its weight has become (module.to(bfloat16))
+            return None
     wdt = lins[0].weight.dtype
     if wdt not in (BF16, FP8) or any(l.weight.dtype != wdt for l in lins):
         return None
