@@ -195,7 +195,9 @@ def _gate_weight(gate, hidden_states):
 def _block_parts(ffns, x):
     """([gate/up entries], [down entries]) of feed-forwards whose Linears all carry a scale for each block of 128
     (functional.grouped_swiglu_block_fp8 and grouped_linear_block_fp8), or None."""
-    if not isinstance(ffns[0].w1, amd_ops.block_fp8_ops.Linear) or any(type(f).forward is not FeedForwardSwiGLU.forward or _observed(f) for f in ffns):
+    if any(type(f).forward is not FeedForwardSwiGLU.forward or _observed(f) for f in ffns):   # (experts of another class may have no w1)
+        return None
+    if not isinstance(ffns[0].w1, amd_ops.block_fp8_ops.Linear):
         return None
     parts = amd_ops.block_fp8_parts([l for f in ffns for l in (f.w1, f.w3, f.w2)], x)
     if parts is None or any(b is not None for i, (_, _, b) in enumerate(parts) if i % 3 != 2):

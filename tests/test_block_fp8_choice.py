@@ -19,3 +19,21 @@ def test_weights_turned_into_16_bits_do_not_lose_their_scales():
     plain = hidream.FeedForwardSwiGLU(64, 96, multiple_of=16, dtype=torch.bfloat16)
     assert hidream._fusable_dtype([plain]) == torch.bfloat16
     assert hidream._fusable_dtype([plain, f]) is None
+
+
+class Other(torch.nn.Module):
+    """An expert of somebody else's."""
+
+    def __init__(self):
+        super().__init__()
+        self.up = torch.nn.Linear(64, 64, bias=False)
+
+    def forward(self, x):
+        return self.up(x)
+
+
+def test_experts_of_another_class_are_asked_for_no_linears():
+    """They are called as they are, with renormalised gate weights for one."""
+    x = torch.zeros((1, 64), dtype=torch.bfloat16)
+    assert hidream._block_parts([Other(), Other(), feed_forward()], x) is None
+    assert hidream._block_parts([feed_forward(), Other()], x) is None
