@@ -199,9 +199,11 @@ def _block_parts(ffns, x):
         return None
     if not isinstance(ffns[0].w1, amd_ops.block_fp8_ops.Linear):
         return None
+    if any(l.bias is not None for f in ffns for l in (f.w1, f.w3)):   # gate/up has none
+        return None
     parts = amd_ops.block_fp8_parts([l for f in ffns for l in (f.w1, f.w3, f.w2)], x)
-    if parts is None or any(b is not None for i, (_, _, b) in enumerate(parts) if i % 3 != 2):
-        return None   # gate/up has no bias
+    if parts is None:
+        return None
     one, three, two = parts[0::3], parts[1::3], parts[2::3]
     return [(w1, s1, w3, s3) for (w1, s1, _), (w3, s3, _) in zip(one, three)], two
 

@@ -37,3 +37,21 @@ def test_experts_of_another_class_are_asked_for_no_linears():
     x = torch.zeros((1, 64), dtype=torch.bfloat16)
     assert hidream._block_parts([Other(), Other(), feed_forward()], x) is None
     assert hidream._block_parts([feed_forward(), Other()], x) is None
+
+
+def test_weights_are_brought_over_only_where_they_are_used(monkeypatch):
+    """Offloaded weights of feed-forwards whose gate/up has a bias, or that hold a Linear of another kind, are not moved or cast in vain."""
+    moved = []
+    parts = ops.block_fp8_ops.Linear.parts
+    monkeypatch.setattr(ops.block_fp8_ops.Linear, "parts", lambda self, x: moved.append(self) or parts(self, x))
+    x = torch.zeros((1, 64), dtype=torch.bfloat16)
+    plain, biased, mixed = feed_forward(), feed_forward(), feed_forward()
+    assert hidream._block_parts([plain, plain], x) is not None and len(moved) == 6
+    del moved[:]
+    biased.w3.bias = torch.nn.Parameter(torch.zeros(96, dtype=torch.bfloat16))
+    mixed.w2 = ops.manual_cast.Linear(96, 64, bias=False)
+    assert hidream._block_parts([plain, biased], x) is None and hidream._block_parts([plain, mixed], x) is None
+    assert moved == []
+    down = feed_forward()
+    down.w2.bias = torch.nn.Parameter(torch.zeros(64, dtype=torch.bfloat16))
+    assert hidream._block_parts([plain, down], x)[1][1][2] is not None
