@@ -756,6 +756,7 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
     what = "grouped_linear_block_fp8"
     if shared is not None and a.dtype != FP8:
         out_dtype = _block_out_dtype(a, out_dtype, what)
+        _block_rows(a, scale_a, what + " a")
         same = a_static is a and scale_static is None
         a, scale_a = quant_block_fp8(a)
         if same:
