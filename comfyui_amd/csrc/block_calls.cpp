@@ -247,16 +247,18 @@ PyObject* do_grouped_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
     c.a.out_dtype = c.type(o[4]);
     const at::ScalarType type = c.a.out_dtype == HDMOE_W_BF16 ? at::kBFloat16 : at::kHalf;
     const int64_t n = c.routed(o[1], o[2], o[5], false, c.a.out_dtype);
-    const at::Tensor y = c.make(n, c.N, type);
-    c.a.routed.out = y.mutable_data_ptr();
     if (o[6] == Py_None) {
+      const at::Tensor y = c.make(n, c.N, type);
+      c.a.routed.out = y.mutable_data_ptr();
       const int rc = c.run(false, stream_of(o[9]));
       return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(y);
     }
     need(c.act == HDMOE_W_E4M3FN);   // (16-bit rows of two groups: cast before)
     Call d(o[7], o[8]);
+    need(d.act == c.act && d.x.device() == c.x.device());   // before anything is allocated
     const int64_t m = d.dense(items(o[6], 3), false, c.a.out_dtype);
-    const at::Tensor z = d.make(m, d.N, type);
+    const at::Tensor y = c.make(n, c.N, type), z = d.make(m, d.N, type);
+    c.a.routed.out = y.mutable_data_ptr();
     d.a.fixed.out = z.mutable_data_ptr();
     c.with(d);
     const int rc = c.run(false, stream_of(o[9]));

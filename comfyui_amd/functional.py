@@ -761,6 +761,12 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
         a, scale_a = quant_block_fp8(a)
         if same:
             a_static, scale_static = a, scale_a
+    if shared is not None:
+        if a_static is None or a_static.device != a.device:
+            raise ValueError(f"{what}: shared needs a_static on {a.device}")
+        if a_static.dtype is not FP8 and scale_static is None:
+            _block_out_dtype(a_static, _block_out_dtype(a, out_dtype, what), what + " a_static")
+            a_static, scale_static = quant_block_fp8(a_static)
     st = _stream_here(a)
     if st is not None:
         r = _block_calls.grouped_linear(a, offsets, experts, scale_a, _OUT_CODE.get(out_dtype, -2), perm, shared, a_static, scale_static, st)
@@ -785,11 +791,6 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
             r.a, r.scale_a, r.scale_a_stride, r.out = a.data_ptr(), ptr(sa), T, out.data_ptr()
         out_static = None
         if shared is not None:
-            if a_static is None or a_static.device != dev:
-                raise ValueError(f"{what}: shared needs a_static on {dev}")
-            if a_static.dtype != FP8 and scale_static is None:
-                _block_out_dtype(a_static, dt, what + " a_static")
-                a_static, scale_static = quant_block_fp8(a_static)
             s = _block_rows(a_static, scale_static, what + " a_static")
             n, Ks = a_static.shape
             w = _lib.BlockWeights()
