@@ -34,6 +34,7 @@ def calls_command():
     import torch
     t = os.path.dirname(torch.__file__)
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f'-DHDMOE_TORCH_VERSION="{torch.__version__}"',
             "-I" + os.path.join(t, "include"), "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"),
             "-I" + sysconfig.get_paths()["include"], os.path.join(CSRC, "block_calls.cpp"), "-o", CALLS_LIB,
             "-L" + os.path.join(t, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]

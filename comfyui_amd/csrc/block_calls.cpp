@@ -331,4 +331,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_block_calls", nullptr, -1, method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__block_calls() { return PyModule_Create(&module); }
+// torch_version: whose headers this was compiled with; the caller compares it with the torch that is there
+PyMODINIT_FUNC PyInit__block_calls() {
+  PyObject* const m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", HDMOE_TORCH_VERSION) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

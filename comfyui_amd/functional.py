@@ -4,6 +4,7 @@ kernels on torch's current stream. Nothing here computes with torch.
 """
 import contextlib
 import ctypes
+import logging
 
 import torch
 
@@ -12,8 +13,11 @@ from ._lib import FfnWeights, LayerArgs, LayerLayout, W_BF16, W_E4M3FN, check, l
 
 try:
     from . import _block_calls
-except ImportError as e:
-    raise RuntimeError("comfyui_amd/_block_calls.so is missing or was built for another torch. Build it with `python -m comfyui_amd.build`.") from e
+    if getattr(_block_calls, "torch_version", None) != torch.__version__:
+        raise ImportError(f"not built for torch {torch.__version__}")
+except ImportError as e:   # host code only: every call it makes is made below as well, at a few times the host's time
+    logging.warning("comfyui_amd: no compiled calls of the block-scaled operators (%s). `python -m comfyui_amd.build` builds them.", e)
+    _block_calls = None
 
 FP8 = torch.float8_e4m3fn
 BF16 = torch.bfloat16
@@ -562,8 +566,9 @@ BLOCK = 128
 _HERE = contextlib.nullcontext()
 _ACT_CODE = {BF16: W_BF16, F16: _lib.W_F16, FP8: W_E4M3FN}
 _OUT_CODE = {None: -1, BF16: W_BF16, F16: _lib.W_F16}
-_block_calls.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.hdmoe_quant_block_fp8, lib.hdmoe_block_workspace_bytes,
-                                                                    lib.hdmoe_block_linear, lib.hdmoe_block_swiglu)))
+if _block_calls is not None:
+    _block_calls.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.hdmoe_quant_block_fp8, lib.hdmoe_block_workspace_bytes,
+                                                                        lib.hdmoe_block_linear, lib.hdmoe_block_swiglu)))
 
 
 def _raw_stream(t):
@@ -572,7 +577,10 @@ def _raw_stream(t):
 
 
 def _stream_here(t):
-    """The current stream's handle where the tensor is on the current device, else None."""
+    """The current stream's handle where the compiled functions can make the call: they are there, and the tensor is on the current device.
+    Else None."""
+    if _block_calls is None:
+        return None
     d = t.get_device()
     return torch._C._cuda_getCurrentRawStream(d) if d >= 0 and d == torch._C._cuda_getDevice() else None
 
