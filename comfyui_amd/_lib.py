@@ -112,6 +112,11 @@ class BlockArgs(ctypes.Structure):
     ]
 
 
+class BlockPlan(ctypes.Structure):
+    """hdmoe_block_plan"""
+    _fields_ = [(n, c_int) for n in ("kernel", "tile_rows", "strips", "cast_inside", "stages", "blocks_per_cu", "lds_bytes")]
+
+
 # name -> (restype, argtypes); every symbol include/hdmoe.h declares
 SIGNATURES = {
     "hdmoe_version": (c_int, []),
@@ -176,6 +181,7 @@ SIGNATURES = {
                                  c_size_t, c_void_p]),
     "hdmoe_quant_block_fp8": (c_int, [c_int, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
     "hdmoe_block_workspace_bytes": (c_size_t, [ctypes.POINTER(BlockArgs), c_int]),
+    "hdmoe_block_plan_get": (c_int, [ctypes.POINTER(BlockArgs), c_int, ctypes.POINTER(BlockPlan)]),
     "hdmoe_block_linear": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
     "hdmoe_block_swiglu": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
     "hdmoe_layer_layout_get": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(LayerLayout)]),

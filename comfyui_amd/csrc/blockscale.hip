@@ -788,6 +788,10 @@ constexpr int stream_depth(int ft, int tt, bool swiglu, bool cast) {
 // CAST: cast rows and scales, and in front of the 16-bit ones
 __host__ __device__ constexpr int stream_cast_bytes(int rows, int KB) { return (rows * (KB * BLK + 16 + KB * 4) + 255) / 256 * 256; }
 constexpr int stream_raw_bytes(int rows, int KB) { return (rows * KB + 4 * STREAM_WAVES - 1) / (4 * STREAM_WAVES) * STREAM_WAVES * 1024; }
+// LDS of a block: its waves' rings, whose place their sums take at the end, and where it casts `rows` rows (at most) of KB blocks for itself, these
+constexpr int stream_lds(int ft, int tt, bool swiglu, bool cast, int rows, int KB) {
+  return STREAM_WAVES * stream_depth(ft, tt, swiglu, cast) * stream_slot(ft, tt, swiglu, cast) + (cast ? stream_cast_bytes(rows, KB) + stream_raw_bytes(rows, KB) : 0);
+}
 
 template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
 __global__ __launch_bounds__(64 * STREAM_WAVES) void block_stream_kernel(const BlockArgs args) {
@@ -1048,10 +1052,13 @@ long long grid_of(const BlockArgs& args, int bm, int feat) {
   return (tiles + HDMOE_NUM_XCD - 1) / HDMOE_NUM_XCD * HDMOE_NUM_XCD;
 }
 
+constexpr int low_stage(bool swiglu) { return (swiglu ? 64 + 256 : 128 + 128) * BLK + 2048; }   // LDS of a K step of block_gemm_kernel
+
 template <class Act, bool SWIGLU, int STAGES>
 int launch_gemm(const BlockArgs& args, const char* what, hipStream_t stream) {
   constexpr int BM = SWIGLU ? 64 : 128, BN = SWIGLU ? 256 : 128;
-  constexpr size_t SMEM = STAGES * ((size_t)(BM + BN) * BLK + 2048);
+  constexpr size_t SMEM = STAGES * low_stage(SWIGLU);
+  static_assert(low_stage(SWIGLU) == (BM + BN) * BLK + 2048, "a stage of the kernel's");
   const auto kernel = block_gemm_kernel<Act, SWIGLU, SWIGLU ? 4 : 2, SWIGLU ? 2 : 4, 4, 2, STAGES>;
   static std::atomic<uint64_t> done{0};
   if (int rc = allow_lds(kernel, SMEM, done, what)) return rc;
@@ -1061,29 +1068,27 @@ int launch_gemm(const BlockArgs& args, const char* what, hipStream_t stream) {
   return hdmoe_check_launch(what);
 }
 
+constexpr int HIGH_LDS = 5 * 32768;   // tokens of two K steps, weights of three
+
 template <class Act, bool SWIGLU>
 int launch_gemm8(const BlockArgs& args, const char* what, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  if (int rc = allow_lds(block_gemm8_kernel<Act, SWIGLU>, 163840, done, what)) return rc;
+  if (int rc = allow_lds(block_gemm8_kernel<Act, SWIGLU>, HIGH_LDS, done, what)) return rc;
   const long long grid = grid_of(args, 64 * args.parts, SWIGLU ? 128 : 256);
   if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
-  block_gemm8_kernel<Act, SWIGLU><<<(unsigned)(grid < HDMOE_NUM_CU ? grid : HDMOE_NUM_CU), 512, 163840, stream>>>(args);
+  block_gemm8_kernel<Act, SWIGLU><<<(unsigned)(grid < HDMOE_NUM_CU ? grid : HDMOE_NUM_CU), 512, HIGH_LDS, stream>>>(args);
   return hdmoe_check_launch(what);
 }
 
-// LDS of a few-row block: cast rows and their scales, then the sums of its waves
-
 template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
 int launch_stream(const BlockArgs& args, const char* what, hipStream_t stream) {
-  constexpr size_t rings = (size_t)STREAM_WAVES * stream_depth(FT, TT, SWIGLU, CAST) * stream_slot(FT, TT, SWIGLU, CAST);
   static std::atomic<uint64_t> done{0};
-  if (int rc = allow_lds(block_stream_kernel<Act, SWIGLU, FT, TT, CAST>, rings + (CAST ? stream_cast_bytes(16, CAST_UNITS / 16) + stream_raw_bytes(16, CAST_UNITS / 16) : 0), done, what)) return rc;
+  if (int rc = allow_lds(block_stream_kernel<Act, SWIGLU, FT, TT, CAST>, stream_lds(FT, TT, SWIGLU, CAST, 16, CAST_UNITS / 16), done, what)) return rc;
   const int K = args.op[0].K > args.op[1].K ? args.op[0].K : args.op[1].K;
-  const int KB = (K + BLK - 1) / BLK;
-  const size_t rows = CAST ? stream_cast_bytes(args.lds_rows, KB) + stream_raw_bytes(args.lds_rows, KB) : 0;
+  const size_t bytes = stream_lds(FT, TT, SWIGLU, CAST, args.lds_rows, (K + BLK - 1) / BLK);
   const long long grid = grid_of(args, TT * 16, SWIGLU ? 8 * FT : 16 * FT);
   if (grid > 0x7fffffffll) return hdmoe_fail(HDMOE_E_SHAPE, "%s: %lld tiles", what, grid);
-  block_stream_kernel<Act, SWIGLU, FT, TT, CAST><<<(unsigned)grid, 64 * STREAM_WAVES, rings + rows, stream>>>(args);
+  block_stream_kernel<Act, SWIGLU, FT, TT, CAST><<<(unsigned)grid, 64 * STREAM_WAVES, bytes, stream>>>(args);
   return hdmoe_check_launch(what);
 }
 
@@ -1359,6 +1364,43 @@ extern "C" size_t hdmoe_block_workspace_bytes(const hdmoe_block_args* p, int swi
   if (K <= 0 || N < 0 || Ns < 0) return 0;
   const Plan plan = plan_of(swiglu != 0, p->a_dtype, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, N, p->K_static, Ns});
   return work_bytes(swiglu != 0, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K, N, Ns);
+}
+
+extern "C" int hdmoe_block_plan_get(const hdmoe_block_args* p, int swiglu, hdmoe_block_plan* out) {
+  const char* what = "hdmoe_block_plan_get";
+  HDMOE_REQUIRE_PTR(p);
+  HDMOE_REQUIRE_PTR(out);
+  const bool routed = p->E > 0 && p->rows > 0, fixed = p->rows_static > 0;
+  if (p->E < 0 || p->E > MAX_E || p->rows < 0 || p->rows_static < 0 || !(routed || fixed))
+    return hdmoe_fail(HDMOE_E_SHAPE, "%s: E=%d rows=%d rows_static=%d", what, p->E, p->rows, p->rows_static);
+  if (routed)
+    if (int rc = check_sizes(what, "", p->rows, p->K, p->N)) return rc;
+  if (fixed)
+    if (int rc = check_sizes(what, " (static)", p->rows_static, p->K_static, p->N_static)) return rc;
+  const Sizes z = {routed ? p->rows : 0, p->E, p->rows_static, p->K, p->N, p->K_static, p->N_static};
+  const Plan plan = plan_of(swiglu != 0, p->a_dtype, z);
+  const int Kr = routed ? p->K : 0, Ks = fixed ? p->K_static : 0, K = Kr > Ks ? Kr : Ks;
+  *out = hdmoe_block_plan{};
+  if (plan.tt > 0) {
+    out->kernel = HDMOE_BLOCK_FEW_ROWS;
+    out->tile_rows = 16 * plan.tt;
+    out->strips = plan.ft;
+    out->cast_inside = plan.cast_inside;
+    out->lds_bytes = stream_lds(plan.ft, plan.tt, swiglu != 0, plan.cast_inside, plan.lds_rows, (K + BLK - 1) / BLK);
+    out->blocks_per_cu = stream_blocks(plan.ft, plan.tt, plan.cast_inside);
+  } else if (plan.stages > 0) {
+    out->kernel = HDMOE_BLOCK_LOW_TILES;
+    out->tile_rows = swiglu ? 64 : 128;
+    out->stages = plan.stages;
+    out->lds_bytes = plan.stages * low_stage(swiglu != 0);
+    out->blocks_per_cu = plan.stages == 2 ? 2 : 1;
+  } else {
+    out->kernel = HDMOE_BLOCK_HIGH_TILES;
+    out->tile_rows = 64 * plan.parts;
+    out->lds_bytes = HIGH_LDS;
+    out->blocks_per_cu = 1;
+  }
+  return HDMOE_OK;
 }
 
 extern "C" int hdmoe_block_linear(const hdmoe_block_args* p, hdmoe_stream_t stream) {

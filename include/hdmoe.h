@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define HDMOE_VERSION 117
+#define HDMOE_VERSION 118
 
 #define HDMOE_OK 0
 #define HDMOE_E_NULL (-1)      /* required pointer is NULL */
@@ -422,6 +422,22 @@ typedef struct hdmoe_block_args {
 /* Working memory of a call: the cast rows of 16-bit activations, unless the contraction casts them itself (few rows), and for
  * hdmoe_block_swiglu (swiglu nonzero) on few rows the fp32 values in front of the cast. Looks at the sizes, a_dtype and perm. */
 size_t hdmoe_block_workspace_bytes(const hdmoe_block_args* args, int swiglu);
+
+/* How a call of these sizes, a_dtype and perm runs (no device, and no pointer but args and plan, is looked at): which kernel, on tiles of how many
+ * rows. For tests and for tuning; the choice is a cost model's and may change. */
+#define HDMOE_BLOCK_FEW_ROWS 0    /* tiles of 16, 32 or 64 rows by strips of 16 weight rows; K dealt to four waves */
+#define HDMOE_BLOCK_LOW_TILES 1   /* 128 rows (gate/up 64) x 128 features */
+#define HDMOE_BLOCK_HIGH_TILES 2  /* 128, 192 or 256 rows x 256 features (gate/up 128 of w1 and of w3) */
+typedef struct hdmoe_block_plan {
+  int kernel;
+  int tile_rows;      /* at most */
+  int strips;         /* few rows: of weights, a wave (gate/up: half of them w1's) */
+  int cast_inside;    /* few rows: 16-bit activations are cast by the contraction */
+  int stages;         /* low tiles: K steps in LDS */
+  int blocks_per_cu;  /* that the choice counts on */
+  int lds_bytes;      /* of a block */
+} hdmoe_block_plan;
+int hdmoe_block_plan_get(const hdmoe_block_args* args, int swiglu, hdmoe_block_plan* plan);
 
 /* out[r, n] = round( sum_b scale_a[r, b] * scale[n / 128, b] * sum_{k in block b} a[r, k] * weight[n, k]  + bias[n] ); the sums over
  * a block are the matrix cores' (each of eight neighbouring products is cut at 2^-13 of the largest: about 6e-5 of a sum), the one over
