@@ -108,7 +108,7 @@ class BlockArgs(ctypes.Structure):
         ("perm", c_void_p), ("offsets", c_void_p),
         ("experts", ctypes.POINTER(BlockWeights)), ("shared", ctypes.POINTER(BlockWeights)),
         ("routed", BlockRows), ("fixed", BlockRows),
-        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("fixed_k_cut", c_int),
     ]
 
 

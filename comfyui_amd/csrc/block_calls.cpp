@@ -201,6 +201,11 @@ PyObject* answer(F&& f) {
   if (count != (n)) { PyErr_SetString(PyExc_TypeError, "wrong number of arguments"); return nullptr; }
 
 void* stream_of(PyObject* o) { return PyLong_AsVoidPtr(o); }
+int truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  need(v >= 0);
+  return v;
+}
 
 // (x, stream)
 PyObject* do_cast(PyObject*, PyObject* const* o, Py_ssize_t count) {
@@ -225,32 +230,34 @@ PyObject* do_cast(PyObject*, PyObject* const* o, Py_ssize_t count) {
   });
 }
 
-// (x, weight, scale, bias, scale_x, out_dtype, stream)
+// (x, weight, scale, bias, scale_x, out_dtype, fixed_k_cut, stream)
 PyObject* do_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(7)
+  HDMOE_ARGUMENTS(8)
   return answer([&]() -> PyObject* {
     Call c(o[0], o[4]);
     c.a.out_dtype = c.type(o[5]);
+    c.a.fixed_k_cut = truth(o[6]);
     const int64_t n = c.dense(o + 1, false, c.a.out_dtype);
     const at::Tensor y = c.make(n, c.N, c.a.out_dtype == HDMOE_W_BF16 ? at::kBFloat16 : at::kHalf);
     c.a.fixed.out = y.mutable_data_ptr();
-    const int rc = c.run(false, stream_of(o[6]));
+    const int rc = c.run(false, stream_of(o[7]));
     return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(y);
   });
 }
 
-// (a, offsets, experts, scale_a, out_dtype, perm, shared, a_static, scale_static, stream)
+// (a, offsets, experts, scale_a, out_dtype, perm, shared, a_static, scale_static, fixed_k_cut, stream)
 PyObject* do_grouped_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(10)
+  HDMOE_ARGUMENTS(11)
   return answer([&]() -> PyObject* {
     Call c(o[0], o[3]);
     c.a.out_dtype = c.type(o[4]);
+    c.a.fixed_k_cut = truth(o[9]);
     const at::ScalarType type = c.a.out_dtype == HDMOE_W_BF16 ? at::kBFloat16 : at::kHalf;
     const int64_t n = c.routed(o[1], o[2], o[5], false, c.a.out_dtype);
     if (o[6] == Py_None) {
       const at::Tensor y = c.make(n, c.N, type);
       c.a.routed.out = y.mutable_data_ptr();
-      const int rc = c.run(false, stream_of(o[9]));
+      const int rc = c.run(false, stream_of(o[10]));
       return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(y);
     }
     need(c.act == HDMOE_W_E4M3FN);   // (16-bit rows of two groups: cast before)
@@ -261,7 +268,7 @@ PyObject* do_grouped_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
     c.a.routed.out = y.mutable_data_ptr();
     d.a.fixed.out = z.mutable_data_ptr();
     c.with(d);
-    const int rc = c.run(false, stream_of(o[9]));
+    const int rc = c.run(false, stream_of(o[10]));
     return rc != 0 ? PyLong_FromLong(rc) : tuple({y, z});
   });
 }
@@ -276,36 +283,38 @@ struct Cast {
   }
 };
 
-// (x, w1, scale1, w3, scale3, scale_x, stream)
+// (x, w1, scale1, w3, scale3, scale_x, fixed_k_cut, stream)
 PyObject* do_swiglu(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(7)
+  HDMOE_ARGUMENTS(8)
   return answer([&]() -> PyObject* {
     Call c(o[0], o[5]);
     c.a.out_dtype = HDMOE_W_BF16;
+    c.a.fixed_k_cut = truth(o[6]);
     const int64_t n = c.dense(o + 1, true, HDMOE_W_BF16);
     const Cast out(c, c.a.fixed, n);
-    const int rc = c.run(true, stream_of(o[6]));
+    const int rc = c.run(true, stream_of(o[7]));
     return rc != 0 ? PyLong_FromLong(rc) : tuple({out.h, out.s});
   });
 }
 
-// (a, offsets, experts, scale_a, perm, shared, stream)
+// (a, offsets, experts, scale_a, perm, shared, fixed_k_cut, stream)
 PyObject* do_grouped_swiglu(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(7)
+  HDMOE_ARGUMENTS(8)
   return answer([&]() -> PyObject* {
     Call c(o[0], o[3]);
     c.a.out_dtype = HDMOE_W_BF16;
+    c.a.fixed_k_cut = truth(o[6]);
     const int64_t n = c.routed(o[1], o[2], o[4], true, HDMOE_W_BF16);
     const Cast out(c, c.a.routed, n);
     if (o[5] == Py_None) {
-      const int rc = c.run(true, stream_of(o[6]));
+      const int rc = c.run(true, stream_of(o[7]));
       return rc != 0 ? PyLong_FromLong(rc) : tuple({out.h, out.s});
     }
     Call d(o[0], o[3]);
     const int64_t m = d.dense(items(o[5], 4), true, HDMOE_W_BF16);
     const Cast shared(d, d.a.fixed, m);
     c.with(d);
-    const int rc = c.run(true, stream_of(o[6]));
+    const int rc = c.run(true, stream_of(o[7]));
     return rc != 0 ? PyLong_FromLong(rc) : tuple({out.h, out.s, shared.h, shared.s});
   });
 }

@@ -1186,7 +1186,9 @@ double high_us(const Sizes& z, bool swiglu, int cap) {
   return 4.0 + (one > most ? one : most);
 }
 
-Plan plan_of(bool swiglu, int a_dtype, const Sizes& z) {
+// fixed: the kernels whose sums go block after block of K, in fp32 on the matrix instruction's result for each (the tile kernels: low and high ones
+// give a row the same bytes), whatever the sizes.
+Plan plan_of(bool swiglu, int a_dtype, const Sizes& z, bool fixed) {
   const bool x16 = a_dtype != HDMOE_W_E4M3FN, exact = swiglu && a_dtype == HDMOE_W_F16;
   Plan best = {0, 0, false, 0, 0, 4};
   double us = exact ? 1e30 : high_us(z, swiglu, 4);   // (that kernel's loop has no exact products)
@@ -1204,7 +1206,7 @@ Plan plan_of(bool swiglu, int a_dtype, const Sizes& z) {
     offer(low_us(z, false, 2), Plan{0, 0, false, 0, 2, 0});
   }
   const int K = z.rows > 0 ? z.K : z.K_static;
-  for (int tt = 1; tt <= 4; tt *= 2)
+  for (int tt = 1; !fixed && tt <= 4; tt *= 2)
     for (int ft = swiglu ? 2 : 1; ft <= 4; ft *= 2) {
       Plan p = {tt, ft, false, 0, 0, 0};
       if (x16 && tt == 1) {
@@ -1298,7 +1300,7 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
   const int a_rows = routed ? args.op[0].a_rows : p->rows_static, K = routed ? p->K : p->K_static;
   if (x16 && routed && p->rows_static > 0 && (p->fixed.a != p->routed.a || p->rows_static != a_rows || p->K_static != K))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: 16-bit activations of the experts and of the static group must be the same rows", what);
-  plan = plan_of(swiglu, p->a_dtype, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, p->N, p->K_static, p->N_static});
+  plan = plan_of(swiglu, p->a_dtype, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, p->N, p->K_static, p->N_static}, p->fixed_k_cut != 0);
   args.lds_rows = plan.lds_rows;
   args.parts = plan.parts;
   const size_t need = work_bytes(swiglu, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K,
@@ -1362,7 +1364,7 @@ extern "C" size_t hdmoe_block_workspace_bytes(const hdmoe_block_args* p, int swi
   if (!routed && p->rows_static == 0) return 0;
   const int K = routed ? p->K : p->K_static, N = routed ? p->N : 0, Ns = p->rows_static > 0 ? p->N_static : 0;
   if (K <= 0 || N < 0 || Ns < 0) return 0;
-  const Plan plan = plan_of(swiglu != 0, p->a_dtype, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, N, p->K_static, Ns});
+  const Plan plan = plan_of(swiglu != 0, p->a_dtype, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, N, p->K_static, Ns}, p->fixed_k_cut != 0);
   return work_bytes(swiglu != 0, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K, N, Ns);
 }
 
@@ -1378,7 +1380,7 @@ extern "C" int hdmoe_block_plan_get(const hdmoe_block_args* p, int swiglu, hdmoe
   if (fixed)
     if (int rc = check_sizes(what, " (static)", p->rows_static, p->K_static, p->N_static)) return rc;
   const Sizes z = {routed ? p->rows : 0, p->E, p->rows_static, p->K, p->N, p->K_static, p->N_static};
-  const Plan plan = plan_of(swiglu != 0, p->a_dtype, z);
+  const Plan plan = plan_of(swiglu != 0, p->a_dtype, z, p->fixed_k_cut != 0);
   const int Kr = routed ? p->K : 0, Ks = fixed ? p->K_static : 0, K = Kr > Ks ? Kr : Ks;
   *out = hdmoe_block_plan{};
   if (plan.tt > 0) {

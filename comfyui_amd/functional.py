@@ -723,14 +723,16 @@ def _block_call(fn, swiglu, args, a):
     check(fn(ref, _raw_stream(a)))
 
 
-def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype=None):
+def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype=None, fixed_k_cut=False):
     """x [rows, K] times weight [N, K]^T (+ bias [N]): weight float8_e4m3fn with fp32 scales scale_weight
     [ceil(N / 128), ceil(K / 128)]; x bf16 or fp16 (cast as quant_block_fp8 does), or float8_e4m3fn with its scales scale_x
     [rows, ceil(K / 128)] (laid out anew unless they are as quant_block_fp8 returns them). -> [rows, N] of x's type (out_dtype, bf16
-    unless given, for float8_e4m3fn x). K and N are multiples of 16. The sums are fp32; bias joins them before the one rounding."""
+    unless given, for float8_e4m3fn x). K and N are multiples of 16. The sums are fp32; bias joins them before the one rounding.
+    fixed_k_cut: the sums go in one order whatever the number of rows: a row's bytes do not depend on which rows come with it (few rows are
+    otherwise dealt along K, up to three times as fast)."""
     st = _stream_here(x)
     if st is not None:
-        r = _block_calls.linear(x, weight, scale_weight, bias, scale_x, _OUT_CODE.get(out_dtype, -2), st)
+        r = _block_calls.linear(x, weight, scale_weight, bias, scale_x, _OUT_CODE.get(out_dtype, -2), fixed_k_cut, st)
         if r is not None:
             return _done(r)
     what = "linear_block_fp8"
@@ -745,6 +747,7 @@ def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype
         if rows > 0:
             args = _lib.BlockArgs()
             args.a_dtype, args.out_dtype = _ACT_CODE[x.dtype], _ACT_CODE[dt]
+            args.fixed_k_cut = 1 if fixed_k_cut else 0
             args.rows_static, args.K_static, args.N_static = rows, K, N
             args.shared = ctypes.pointer(w)
             fixed = args.fixed
@@ -754,13 +757,13 @@ def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype
 
 
 def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, perm=None, shared=None, a_static=None,
-                             scale_static=None):
+                             scale_static=None, fixed_k_cut=False):
     """linear_block_fp8 of every expert over its row segment [offsets[e], offsets[e + 1]) of a [rows, K]. experts: list of
     (weight [N, K], scale, bias [N] or None), at most 32; offsets: int32 [E + 1] on the device, ascending. a as in linear_block_fp8.
     perm: the dispatch's permutation, sorted row r being row perm[r] // 2 of a [T, K]; the output then has 2T rows. Rows that no
     segment holds are not written. -> out [rows, N].
     shared: one more (weight, scale, bias) over all rows of a_static (with scale_static), of sizes of its own, in the same launch;
-    -> (out, out_static)."""
+    -> (out, out_static). fixed_k_cut: see linear_block_fp8."""
     what = "grouped_linear_block_fp8"
     if shared is not None and a.dtype != FP8:
         out_dtype = _block_out_dtype(a, out_dtype, what)
@@ -777,7 +780,7 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
             a_static, scale_static = quant_block_fp8(a_static)
     st = _stream_here(a)
     if st is not None:
-        r = _block_calls.grouped_linear(a, offsets, experts, scale_a, _OUT_CODE.get(out_dtype, -2), perm, shared, a_static, scale_static, st)
+        r = _block_calls.grouped_linear(a, offsets, experts, scale_a, _OUT_CODE.get(out_dtype, -2), perm, shared, a_static, scale_static, fixed_k_cut, st)
         if r is not None:
             return _done(r)
     dt = _block_out_dtype(a, out_dtype, what)
@@ -788,6 +791,7 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
     with _on(dev):
         args = _lib.BlockArgs()
         args.a_dtype, args.out_dtype = _ACT_CODE[a.dtype], _ACT_CODE[dt]
+        args.fixed_k_cut = 1 if fixed_k_cut else 0
         out = torch.empty((rows, N), dtype=dt, device=dev)
         if rows > 0:
             args.E, args.rows, args.K, args.N = len(experts), rows, K, N
@@ -813,16 +817,17 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
     return out if shared is None else (out, out_static)
 
 
-def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, shared=None):
+def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, shared=None, fixed_k_cut=False):
     """First half of every expert's SwiGLU feed-forward, silu(a w1^T) * (a w3^T), cast as quant_block_fp8 does:
     experts: list of (w1 [H, K], scale1, w3 [H, K], scale3); a, scale_a, offsets, perm as in grouped_linear_block_fp8.
     -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]); everything before the cast is fp32; its products are exact as
     well on few rows and with fp16 a (not yet cast).
     shared: one more (w1, scale1, w3, scale3) over all rows of a, with a width of its own, in the same launch (with perm);
-    -> (h, scales, h_shared, scales_shared)."""
+    -> (h, scales, h_shared, scales_shared). fixed_k_cut: see linear_block_fp8; the products are then the same kind on any number of rows as
+    well."""
     st = _stream_here(a)
     if st is not None:
-        r = _block_calls.grouped_swiglu(a, offsets, experts, scale_a, perm, shared, st)
+        r = _block_calls.grouped_swiglu(a, offsets, experts, scale_a, perm, shared, fixed_k_cut, st)
         if r is not None:
             return _done(r)
     what = "grouped_swiglu_block_fp8"
@@ -833,6 +838,7 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
     with _on(dev):
         args = _lib.BlockArgs()
         args.a_dtype, args.out_dtype = _ACT_CODE[a.dtype], W_BF16
+        args.fixed_k_cut = 1 if fixed_k_cut else 0
         h = torch.empty((rows, H), dtype=FP8, device=dev)
         sh = block_scales(rows, H, dev)
         if rows > 0:
@@ -859,12 +865,12 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
     return (h, sh) if shared is None else (h, sh, h_shared, sh_shared)
 
 
-def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None):
+def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None, fixed_k_cut=False):
     """First half of one dense SwiGLU feed-forward, silu(x w1^T) * (x w3^T), cast as quant_block_fp8 does: x and scale_x as in
-    linear_block_fp8 -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]), what linear_block_fp8 takes for w2."""
+    linear_block_fp8, fixed_k_cut as in grouped_swiglu_block_fp8 -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]), what linear_block_fp8 takes for w2."""
     st = _stream_here(x)
     if st is not None:
-        r = _block_calls.swiglu(x, w1, scale_w1, w3, scale_w3, scale_x, st)
+        r = _block_calls.swiglu(x, w1, scale_w1, w3, scale_w3, scale_x, fixed_k_cut, st)
         if r is not None:
             return _done(r)
     what = "swiglu_block_fp8"
@@ -879,6 +885,7 @@ def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None):
         if rows > 0:
             args = _lib.BlockArgs()
             args.a_dtype, args.out_dtype = _ACT_CODE[x.dtype], W_BF16
+            args.fixed_k_cut = 1 if fixed_k_cut else 0
             args.rows_static, args.K_static, args.N_static = rows, K, H
             args.shared = ctypes.pointer(w)
             f = args.fixed

@@ -208,6 +208,11 @@ def _block_parts(ffns, x):
     return [(w1, s1, w3, s3) for (w1, s1, _), (w3, s3, _) in zip(one, three)], two
 
 
+def _same_sums(ffns, *names):
+    """Whether one of these Linears asks for a row's bytes not to depend on the others (`batch_invariant`): the launch that they share then does."""
+    return any(amd_ops._batch_invariant(getattr(f, n)) for f in ffns for n in names)
+
+
 class FeedForwardSwiGLU(nn.Module):
     def __init__(self, dim: int, hidden_dim: int, multiple_of: int = 256,
                  ffn_dim_multiplier: Optional[float] = None, dtype=None, device=None, operations=None):
@@ -244,9 +249,9 @@ class FeedForwardSwiGLU(nn.Module):
         if got is None:
             return None
         x2 = x.reshape(-1, x.shape[-1]).contiguous()
-        h, sh = HF.swiglu_block_fp8(x2, *got[0][0])
+        h, sh = HF.swiglu_block_fp8(x2, *got[0][0], fixed_k_cut=_same_sums([self], "w1", "w3"))
         w, s, b = got[1][0]
-        return HF.linear_block_fp8(h, w, s, bias=b, scale_x=sh, out_dtype=x.dtype).view(*x.shape[:-1], w.shape[0])
+        return HF.linear_block_fp8(h, w, s, bias=b, scale_x=sh, out_dtype=x.dtype, fixed_k_cut=_same_sums([self], "w2")).view(*x.shape[:-1], w.shape[0])
 
     def forward(self, x):
         if x.is_cuda and x.dtype in HF.ACT_DTYPES:
@@ -442,8 +447,10 @@ class MOEFeedForwardSwiGLU(nn.Module):
         if getattr(self.gate, "norm_topk_prob", False):
             w = HF.renorm_top2(w)
         _, offsets, perm, inv_perm = HF.dispatch(idx, len(self.experts))
-        h, sh, hs, shs = HF.grouped_swiglu_block_fp8(x2, offsets, gate_up[:-1], perm=perm, shared=gate_up[-1])
-        y, ys = HF.grouped_linear_block_fp8(h, offsets, down[:-1], scale_a=sh, shared=down[-1], a_static=hs, scale_static=shs)
+        ffns = [*self.experts, self.shared_experts]
+        h, sh, hs, shs = HF.grouped_swiglu_block_fp8(x2, offsets, gate_up[:-1], perm=perm, shared=gate_up[-1], fixed_k_cut=_same_sums(ffns, "w1", "w3"))
+        y, ys = HF.grouped_linear_block_fp8(h, offsets, down[:-1], scale_a=sh, shared=down[-1], a_static=hs, scale_static=shs,
+                                            fixed_k_cut=_same_sums(ffns, "w2"))
         if gated_residual is not None:
             g, res, per_batch = gated_residual
             return HF.combine_gated_residual(y, inv_perm, w, ys, g, res, per_batch)

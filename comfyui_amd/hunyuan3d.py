@@ -202,8 +202,10 @@ class MoEBlock(nn.Module):
         parts = _block_parts([*self.experts, self.shared_experts], x2) if stages[0] is None else None
         if parts is not None:
             first, second = parts
-            h, h_sh = HF.grouped_linear_block_fp8(x2, offsets, first[:-1], perm=perm, shared=first[-1], a_static=x2)
-            y, y_sh = HF.grouped_linear_block_fp8(HF.gelu(h), offsets, second[:-1], shared=second[-1], a_static=HF.gelu(h_sh))
+            ffs = (*self.experts, self.shared_experts)   # one that asks for it has the launch that it shares
+            fixed = [any(amd_ops._batch_invariant(l) for l in ls) for ls in ([f.net[0].proj for f in ffs], [f.net[2] for f in ffs])]
+            h, h_sh = HF.grouped_linear_block_fp8(x2, offsets, first[:-1], perm=perm, shared=first[-1], a_static=x2, fixed_k_cut=fixed[0])
+            y, y_sh = HF.grouped_linear_block_fp8(HF.gelu(h), offsets, second[:-1], shared=second[-1], a_static=HF.gelu(h_sh), fixed_k_cut=fixed[1])
             return HF.combine(y, inv_perm, w, y_sh).view(*orig_shape)
         if any(v is None for v in stages):
             xs = HF.permute_bf16(x2, perm)

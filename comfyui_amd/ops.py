@@ -409,7 +409,7 @@ class block_fp8_ops(manual_cast):
         def forward_comfy_cast_weights(self, input):
             weight, scale, bias = self.parts(input)
             x2 = input.reshape(-1, input.shape[-1]).contiguous()
-            return HF.linear_block_fp8(x2, weight, scale, bias=bias).reshape(*input.shape[:-1], weight.shape[0])
+            return HF.linear_block_fp8(x2, weight, scale, bias=bias, fixed_k_cut=_batch_invariant(self)).reshape(*input.shape[:-1], weight.shape[0])
 
         def _spread(self, weight):
             """scale_weight as one fp32 value per element, on the weight's device (fp16 would lose scales below 2^-25)."""

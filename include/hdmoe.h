@@ -418,12 +418,14 @@ typedef struct hdmoe_block_args {
   hdmoe_block_rows routed, fixed;     /* the experts' rows, the static group's (16-bit a: the same rows where both are there) */
   void* workspace;    /* hdmoe_block_workspace_bytes(...) bytes, 256-byte aligned (NULL where that is 0) */
   size_t workspace_bytes;
+  int fixed_k_cut;    /* nonzero: the sums of a row go in one order whatever the number of rows, so that its bytes do not depend on which rows come
+                       * with it (few rows are otherwise dealt along K: up to three times as fast there) */
 } hdmoe_block_args;
 /* Working memory of a call: the cast rows of 16-bit activations, unless the contraction casts them itself (few rows), and for
- * hdmoe_block_swiglu (swiglu nonzero) on few rows the fp32 values in front of the cast. Looks at the sizes, a_dtype and perm. */
+ * hdmoe_block_swiglu (swiglu nonzero) on few rows the fp32 values in front of the cast. Looks at the sizes, a_dtype, perm and fixed_k_cut. */
 size_t hdmoe_block_workspace_bytes(const hdmoe_block_args* args, int swiglu);
 
-/* How a call of these sizes, a_dtype and perm runs (no device, and no pointer but args and plan, is looked at): which kernel, on tiles of how many
+/* How a call of these sizes, a_dtype, perm and fixed_k_cut runs (no device, and no pointer but args and plan, is looked at): which kernel, on tiles of how many
  * rows. For tests and for tuning; the choice is a cost model's and may change. */
 #define HDMOE_BLOCK_FEW_ROWS 0    /* tiles of 16, 32 or 64 rows by strips of 16 weight rows; K dealt to four waves */
 #define HDMOE_BLOCK_LOW_TILES 1   /* 128 rows (gate/up 64) x 128 features */
