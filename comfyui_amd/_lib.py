@@ -108,13 +108,13 @@ class BlockArgs(ctypes.Structure):
         ("perm", c_void_p), ("offsets", c_void_p),
         ("experts", ctypes.POINTER(BlockWeights)), ("shared", ctypes.POINTER(BlockWeights)),
         ("routed", BlockRows), ("fixed", BlockRows),
-        ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("fixed_k_cut", c_int),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("fixed_k_cut", c_int), ("exact", c_int),
     ]
 
 
 class BlockPlan(ctypes.Structure):
     """hdmoe_block_plan"""
-    _fields_ = [(n, c_int) for n in ("kernel", "tile_rows", "strips", "cast_inside", "stages", "blocks_per_cu", "lds_bytes")]
+    _fields_ = [(n, c_int) for n in ("kernel", "tile_rows", "strips", "cast_inside", "stages", "blocks_per_cu", "lds_bytes", "exact")]
 
 
 # name -> (restype, argtypes); every symbol include/hdmoe.h declares

@@ -283,38 +283,40 @@ struct Cast {
   }
 };
 
-// (x, w1, scale1, w3, scale3, scale_x, fixed_k_cut, stream)
+// (x, w1, scale1, w3, scale3, scale_x, fixed_k_cut, exact, stream)
 PyObject* do_swiglu(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(8)
+  HDMOE_ARGUMENTS(9)
   return answer([&]() -> PyObject* {
     Call c(o[0], o[5]);
     c.a.out_dtype = HDMOE_W_BF16;
     c.a.fixed_k_cut = truth(o[6]);
+    c.a.exact = truth(o[7]);
     const int64_t n = c.dense(o + 1, true, HDMOE_W_BF16);
     const Cast out(c, c.a.fixed, n);
-    const int rc = c.run(true, stream_of(o[7]));
+    const int rc = c.run(true, stream_of(o[8]));
     return rc != 0 ? PyLong_FromLong(rc) : tuple({out.h, out.s});
   });
 }
 
-// (a, offsets, experts, scale_a, perm, shared, fixed_k_cut, stream)
+// (a, offsets, experts, scale_a, perm, shared, fixed_k_cut, exact, stream)
 PyObject* do_grouped_swiglu(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(8)
+  HDMOE_ARGUMENTS(9)
   return answer([&]() -> PyObject* {
     Call c(o[0], o[3]);
     c.a.out_dtype = HDMOE_W_BF16;
     c.a.fixed_k_cut = truth(o[6]);
+    c.a.exact = truth(o[7]);
     const int64_t n = c.routed(o[1], o[2], o[4], true, HDMOE_W_BF16);
     const Cast out(c, c.a.routed, n);
     if (o[5] == Py_None) {
-      const int rc = c.run(true, stream_of(o[7]));
+      const int rc = c.run(true, stream_of(o[8]));
       return rc != 0 ? PyLong_FromLong(rc) : tuple({out.h, out.s});
     }
     Call d(o[0], o[3]);
     const int64_t m = d.dense(items(o[5], 4), true, HDMOE_W_BF16);
     const Cast shared(d, d.a.fixed, m);
     c.with(d);
-    const int rc = c.run(true, stream_of(o[7]));
+    const int rc = c.run(true, stream_of(o[8]));
     return rc != 0 ? PyLong_FromLong(rc) : tuple({out.h, out.s, shared.h, shared.s});
   });
 }

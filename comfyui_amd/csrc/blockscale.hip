@@ -271,10 +271,10 @@ struct Deal {
 // One block of 128: p = A B^T of 16 x 16. The e4m3fn instruction cuts each product at 2^-13 of the largest of its eight neighbours, which leaves a
 // sum off by 6e-5 of itself. That drowns in the rounding of a 16-bit output, but not where the sum is cast again: 0.23 % of an intermediate's
 // codes then are a step off (0.003 % with exact products), and the feed-forward's output by 0.0013 of itself: below bf16's rounding, six times fp16's.
-// EXACT: the values as fp16, which holds them, at half the rate and behind a conversion; products and sums are fp32. Gate/up has it on few rows, where
-// it waits for memory anyway and a handful of codes can be much of an output (2 rows of 2560 x 6912 x 2560 34.4 us, 33.7 without), and
-// on any number of rows where the activations are fp16 (600 rows in eight segments, 1024 x 1024 x 1024, 30.7 and 27.1; 16384 in four, 2560 x 4096 x
-// 2560, 1258 us, 521 on the 256-row tiles, whose loop has none).
+// EXACT: the values as fp16, which holds them, at half the rate and behind a conversion; products and sums are fp32. Gate/up has it up to EXACT_ROWS
+// rows, where a handful of codes can be much of an output (2560 x 6912, four experts: 2 rows 34.4 us, 33.7 without, gate/up and down; gate/up of 8 to
+// 64 rows 45 us, 40 without), and on any number where the caller asks for it or the activations are fp16 (600 rows in eight segments, 1024 x 1024 x
+// 1024, 30.7 and 27.1; 16384 in four, 2560 x 4096 x 2560, 1258 us, 521 on the 256-row tiles, whose loop has none).
 template <bool EXACT>
 __device__ __forceinline__ v4f block_product(const v8i& a, const v8i& b) {
   v4f c = {0, 0, 0, 0};
@@ -393,6 +393,7 @@ __device__ __forceinline__ int tile_feature(int f, int r) {
 // accumulators behind the MFMAs of the next one. STAGES K steps in LDS, STAGES - 1 of them asked for ahead: with two, two blocks share
 // a CU and one fills the other's waits; with more, for launches that have at most a block for every CU, a step does not last as long as
 // its loads are on their way (128 x 6912 x 2560: 32 us, 41.5 with two stages).
+// Gate/up: Act says whether products are exact (HdmoeF16) or not; nothing of its type is read or written.
 template <class Act, bool SWIGLU, int WF, int WT, int FT, int TT, int STAGES>
 __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_kernel(const BlockArgs args) {
 #if defined(__HIP_DEVICE_COMPILE__)   // (the host pass leaves out stubs of kernels whose lambdas hold arrays of dependent size)
@@ -1133,7 +1134,7 @@ namespace {
 
 // How a call runs: the few-row kernels on tiles of 16 * tt rows and ft strips (tt > 0; with the cast inside or not), block_gemm_kernel with
 // `stages` K steps in LDS (stages > 0), or block_gemm8_kernel.
-struct Plan { int tt, ft; bool cast_inside; int lds_rows; int stages, parts; };
+struct Plan { int tt, ft; bool cast_inside; int lds_rows; int stages, parts; bool exact; };
 
 // What a launch is likely to take in microseconds, by what the kernels measured over 1 to 16384 rows of 2560 and 6912 wide Linears. Where the
 // segments end is not known here; on average half a tile of each is empty.
@@ -1186,11 +1187,14 @@ double high_us(const Sizes& z, bool swiglu, int cap) {
   return 4.0 + (one > most ? one : most);
 }
 
+// Gate/up: rows of either group up to which its products are exact in every type
+constexpr int EXACT_ROWS = 64;
 // fixed: the kernels whose sums go block after block of K, in fp32 on the matrix instruction's result for each (the tile kernels: low and high ones
-// give a row the same bytes), whatever the sizes.
-Plan plan_of(bool swiglu, int a_dtype, const Sizes& z, bool fixed) {
-  const bool x16 = a_dtype != HDMOE_W_E4M3FN, exact = swiglu && a_dtype == HDMOE_W_F16;
-  Plan best = {0, 0, false, 0, 0, 4};
+// give a row the same bytes), and products of one kind, whatever the sizes. exact: gate/up's products are.
+Plan plan_of(bool swiglu, int a_dtype, const Sizes& z, bool fixed, bool exact) {
+  const bool x16 = a_dtype != HDMOE_W_E4M3FN;
+  exact = swiglu && (exact || a_dtype == HDMOE_W_F16 || (!fixed && z.rows <= EXACT_ROWS && z.rows_static <= EXACT_ROWS));
+  Plan best = {0, 0, false, 0, 0, 4, false};
   double us = exact ? 1e30 : high_us(z, swiglu, 4);   // (that kernel's loop has no exact products)
   auto offer = [&](double t, const Plan& p) {
     if (t < us) {
@@ -1198,17 +1202,17 @@ Plan plan_of(bool swiglu, int a_dtype, const Sizes& z, bool fixed) {
       best = p;
     }
   };
-  for (int cap = 3; !exact && cap >= 2; --cap) offer(high_us(z, swiglu, cap), Plan{0, 0, false, 0, 0, cap});
+  for (int cap = 3; !exact && cap >= 2; --cap) offer(high_us(z, swiglu, cap), Plan{0, 0, false, 0, 0, cap, exact});
   if (swiglu) {
-    offer(low_us(z, true, 3), Plan{0, 0, false, 0, 3, 0});
+    offer(low_us(z, true, 3), Plan{0, 0, false, 0, 3, 0, exact});
   } else {
-    offer(low_us(z, false, 4), Plan{0, 0, false, 0, 4, 0});
-    offer(low_us(z, false, 2), Plan{0, 0, false, 0, 2, 0});
+    offer(low_us(z, false, 4), Plan{0, 0, false, 0, 4, 0, exact});
+    offer(low_us(z, false, 2), Plan{0, 0, false, 0, 2, 0, exact});
   }
   const int K = z.rows > 0 ? z.K : z.K_static;
   for (int tt = 1; !fixed && tt <= 4; tt *= 2)
     for (int ft = swiglu ? 2 : 1; ft <= 4; ft *= 2) {
-      Plan p = {tt, ft, false, 0, 0, 0};
+      Plan p = {tt, ft, false, 0, 0, 0, swiglu};
       if (x16 && tt == 1) {
         // a block casts for itself what takes its threads 8 trips at most: a launch (4 us) less
         const int whole = z.rows > z.rows_static ? z.rows : z.rows_static;
@@ -1300,7 +1304,7 @@ int fill(const char* what, const hdmoe_block_args* p, bool swiglu, BlockArgs& ar
   const int a_rows = routed ? args.op[0].a_rows : p->rows_static, K = routed ? p->K : p->K_static;
   if (x16 && routed && p->rows_static > 0 && (p->fixed.a != p->routed.a || p->rows_static != a_rows || p->K_static != K))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: 16-bit activations of the experts and of the static group must be the same rows", what);
-  plan = plan_of(swiglu, p->a_dtype, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, p->N, p->K_static, p->N_static}, p->fixed_k_cut != 0);
+  plan = plan_of(swiglu, p->a_dtype, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, p->N, p->K_static, p->N_static}, p->fixed_k_cut != 0, p->exact != 0);
   args.lds_rows = plan.lds_rows;
   args.parts = plan.parts;
   const size_t need = work_bytes(swiglu, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K,
@@ -1364,7 +1368,7 @@ extern "C" size_t hdmoe_block_workspace_bytes(const hdmoe_block_args* p, int swi
   if (!routed && p->rows_static == 0) return 0;
   const int K = routed ? p->K : p->K_static, N = routed ? p->N : 0, Ns = p->rows_static > 0 ? p->N_static : 0;
   if (K <= 0 || N < 0 || Ns < 0) return 0;
-  const Plan plan = plan_of(swiglu != 0, p->a_dtype, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, N, p->K_static, Ns}, p->fixed_k_cut != 0);
+  const Plan plan = plan_of(swiglu != 0, p->a_dtype, Sizes{routed ? p->rows : 0, p->E, p->rows_static, p->K, N, p->K_static, Ns}, p->fixed_k_cut != 0, p->exact != 0);
   return work_bytes(swiglu != 0, x16, plan, routed ? p->rows : 0, routed && p->perm != nullptr ? p->T : 0, p->rows_static, K, N, Ns);
 }
 
@@ -1380,7 +1384,7 @@ extern "C" int hdmoe_block_plan_get(const hdmoe_block_args* p, int swiglu, hdmoe
   if (fixed)
     if (int rc = check_sizes(what, " (static)", p->rows_static, p->K_static, p->N_static)) return rc;
   const Sizes z = {routed ? p->rows : 0, p->E, p->rows_static, p->K, p->N, p->K_static, p->N_static};
-  const Plan plan = plan_of(swiglu != 0, p->a_dtype, z, p->fixed_k_cut != 0);
+  const Plan plan = plan_of(swiglu != 0, p->a_dtype, z, p->fixed_k_cut != 0, p->exact != 0);
   const int Kr = routed ? p->K : 0, Ks = fixed ? p->K_static : 0, K = Kr > Ks ? Kr : Ks;
   *out = hdmoe_block_plan{};
   if (plan.tt > 0) {
@@ -1402,6 +1406,7 @@ extern "C" int hdmoe_block_plan_get(const hdmoe_block_args* p, int swiglu, hdmoe
     out->lds_bytes = HIGH_LDS;
     out->blocks_per_cu = 1;
   }
+  out->exact = plan.exact;
   return HDMOE_OK;
 }
 
@@ -1430,6 +1435,6 @@ extern "C" int hdmoe_block_swiglu(const hdmoe_block_args* p, hdmoe_stream_t stre
     if (int rc = p->a_dtype == HDMOE_W_F16 ? launch_few<HdmoeF16, true>(args, plan, what, s) : launch_few<HdmoeBf16, true>(args, plan, what, s)) return rc;
     return launch_cast(args, what, s);
   }
-  if (plan.stages > 0) return p->a_dtype == HDMOE_W_F16 ? launch_gemm<HdmoeF16, true, 3>(args, what, s) : launch_gemm<HdmoeBf16, true, 3>(args, what, s);
+  if (plan.stages > 0) return plan.exact ? launch_gemm<HdmoeF16, true, 3>(args, what, s) : launch_gemm<HdmoeBf16, true, 3>(args, what, s);
   return launch_gemm8<HdmoeBf16, true>(args, what, s);
 }

@@ -817,17 +817,18 @@ def grouped_linear_block_fp8(a, offsets, experts, scale_a=None, out_dtype=None, 
     return out if shared is None else (out, out_static)
 
 
-def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, shared=None, fixed_k_cut=False):
+def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, shared=None, fixed_k_cut=False, exact=False):
     """First half of every expert's SwiGLU feed-forward, silu(a w1^T) * (a w3^T), cast as quant_block_fp8 does:
     experts: list of (w1 [H, K], scale1, w3 [H, K], scale3); a, scale_a, offsets, perm as in grouped_linear_block_fp8.
-    -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]); everything before the cast is fp32; its products are exact as
-    well on few rows and with fp16 a (not yet cast).
+    -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]); everything before the cast is fp32. Its products are
+    exact with `exact`, for fp16 a (not yet cast), and where neither group has more than 64 rows (unless fixed_k_cut); elsewhere the matrix
+    cores cut them, which moves 0.23 % of the cast values by a step. exact costs 15 % on few rows, at most 2.4 times on many.
     shared: one more (w1, scale1, w3, scale3) over all rows of a, with a width of its own, in the same launch (with perm);
     -> (h, scales, h_shared, scales_shared). fixed_k_cut: see linear_block_fp8; the products are then the same kind on any number of rows as
     well."""
     st = _stream_here(a)
     if st is not None:
-        r = _block_calls.grouped_swiglu(a, offsets, experts, scale_a, perm, shared, fixed_k_cut, st)
+        r = _block_calls.grouped_swiglu(a, offsets, experts, scale_a, perm, shared, fixed_k_cut, exact, st)
         if r is not None:
             return _done(r)
     what = "grouped_swiglu_block_fp8"
@@ -838,7 +839,7 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
     with _on(dev):
         args = _lib.BlockArgs()
         args.a_dtype, args.out_dtype = _ACT_CODE[a.dtype], W_BF16
-        args.fixed_k_cut = 1 if fixed_k_cut else 0
+        args.fixed_k_cut, args.exact = 1 if fixed_k_cut else 0, 1 if exact else 0
         h = torch.empty((rows, H), dtype=FP8, device=dev)
         sh = block_scales(rows, H, dev)
         if rows > 0:
@@ -865,12 +866,13 @@ def grouped_swiglu_block_fp8(a, offsets, experts, scale_a=None, perm=None, share
     return (h, sh) if shared is None else (h, sh, h_shared, sh_shared)
 
 
-def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None, fixed_k_cut=False):
+def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None, fixed_k_cut=False, exact=False):
     """First half of one dense SwiGLU feed-forward, silu(x w1^T) * (x w3^T), cast as quant_block_fp8 does: x and scale_x as in
-    linear_block_fp8, fixed_k_cut as in grouped_swiglu_block_fp8 -> (h float8_e4m3fn [rows, H], its scales [rows, ceil(H / 128)]), what linear_block_fp8 takes for w2."""
+    linear_block_fp8, fixed_k_cut and exact as in grouped_swiglu_block_fp8 -> (h float8_e4m3fn [rows, H], its scales
+    [rows, ceil(H / 128)]), what linear_block_fp8 takes for w2."""
     st = _stream_here(x)
     if st is not None:
-        r = _block_calls.swiglu(x, w1, scale_w1, w3, scale_w3, scale_x, fixed_k_cut, st)
+        r = _block_calls.swiglu(x, w1, scale_w1, w3, scale_w3, scale_x, fixed_k_cut, exact, st)
         if r is not None:
             return _done(r)
     what = "swiglu_block_fp8"
@@ -885,7 +887,7 @@ def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None, fixed_k_cut=Fa
         if rows > 0:
             args = _lib.BlockArgs()
             args.a_dtype, args.out_dtype = _ACT_CODE[x.dtype], W_BF16
-            args.fixed_k_cut = 1 if fixed_k_cut else 0
+            args.fixed_k_cut, args.exact = 1 if fixed_k_cut else 0, 1 if exact else 0
             args.rows_static, args.K_static, args.N_static = rows, K, H
             args.shared = ctypes.pointer(w)
             f = args.fixed

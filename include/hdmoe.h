@@ -420,12 +420,13 @@ typedef struct hdmoe_block_args {
   size_t workspace_bytes;
   int fixed_k_cut;    /* nonzero: the sums of a row go in one order whatever the number of rows, so that its bytes do not depend on which rows come
                        * with it (few rows are otherwise dealt along K: up to three times as fast there) */
+  int exact;          /* hdmoe_block_swiglu, nonzero: exact products at any size */
 } hdmoe_block_args;
 /* Working memory of a call: the cast rows of 16-bit activations, unless the contraction casts them itself (few rows), and for
- * hdmoe_block_swiglu (swiglu nonzero) on few rows the fp32 values in front of the cast. Looks at the sizes, a_dtype, perm and fixed_k_cut. */
+ * hdmoe_block_swiglu (swiglu nonzero) on few rows the fp32 values in front of the cast. Looks at the sizes, a_dtype, perm, fixed_k_cut and exact. */
 size_t hdmoe_block_workspace_bytes(const hdmoe_block_args* args, int swiglu);
 
-/* How a call of these sizes, a_dtype, perm and fixed_k_cut runs (no device, and no pointer but args and plan, is looked at): which kernel, on tiles of how many
+/* How a call of these sizes, a_dtype, perm, fixed_k_cut and exact runs (no device, and no pointer but args and plan, is looked at): which kernel, on tiles of how many
  * rows. For tests and for tuning; the choice is a cost model's and may change. */
 #define HDMOE_BLOCK_FEW_ROWS 0    /* tiles of 16, 32 or 64 rows by strips of 16 weight rows; K dealt to four waves */
 #define HDMOE_BLOCK_LOW_TILES 1   /* 128 rows (gate/up 64) x 128 features */
@@ -438,6 +439,7 @@ typedef struct hdmoe_block_plan {
   int stages;         /* low tiles: K steps in LDS */
   int blocks_per_cu;  /* that the choice counts on */
   int lds_bytes;      /* of a block */
+  int exact;          /* gate/up: its products are */
 } hdmoe_block_plan;
 int hdmoe_block_plan_get(const hdmoe_block_args* args, int swiglu, hdmoe_block_plan* plan);
 
@@ -447,8 +449,8 @@ int hdmoe_block_plan_get(const hdmoe_block_args* args, int swiglu, hdmoe_block_p
 int hdmoe_block_linear(const hdmoe_block_args* args, hdmoe_stream_t stream);
 /* The first half of a SwiGLU feed-forward: h = silu(g) * u with g and u such sums over w1 and w3, all in fp32, and the cast of h's rows
  * as hdmoe_quant_block_fp8 makes it (out, scale_out). What the matrix cores' e4m3fn sums lose moves a few of the
- * cast values by a step (0.23 %; the output of the second half by 0.0013 of itself). It is lost on many rows of bf16
- * or e4m3fn activations only: on few rows, and for fp16 on any number, the products are exact and the sums fp32. */
+ * cast values by a step (0.23 %; the output of the second half by 0.0013 of itself). Products are exact, and the sums fp32,
+ * where neither group has more than 64 rows (unless fixed_k_cut), for fp16 activations, and with `exact`; elsewhere they may be cut. */
 int hdmoe_block_swiglu(const hdmoe_block_args* args, hdmoe_stream_t stream);
 
 /* ---- whole layer -------------------------------------------------------------- */

@@ -87,3 +87,35 @@ def test_a_block_fits_its_cu():
         rows, K, N = sample(rng, 16384)
         p = plan(rng.choice((0, 1)), rng.choice((L.W_BF16, L.W_E4M3FN)), rows, rng.choice((0, 1, 4, 8)), K, N)
         assert 0 < p.lds_bytes <= 163840
+
+
+@pytest.mark.parametrize("a_dtype", [L.W_BF16, L.W_F16, L.W_E4M3FN])
+def test_gate_up_has_exact_products_where_the_header_says(a_dtype):
+    """Up to 64 rows in each group, with fp16 activations, and when asked. (A Linear has none, and no flag.)"""
+    rng, p = random.Random(10), L.BlockPlan()
+    few = many = 0
+    for _ in range(4000):
+        rows, K, N = sample(rng, 8192)
+        a = L.BlockArgs()
+        a.a_dtype, a.out_dtype = a_dtype, L.W_BF16
+        form = rng.choice(("dense", "experts", "layer"))
+        if form != "dense":
+            a.E, a.rows, a.K, a.N = rng.choice((1, 2, 4, 32)), rows, K, N
+        if form != "experts":
+            a.rows_static, a.K_static, a.N_static = rows if form == "dense" else -(-rows // 2), K, 16 * rng.randint(1, 400)
+        for exact in (0, 1):
+            for fixed in (0, 1):
+                a.exact, a.fixed_k_cut = exact, fixed
+                L.check(L.lib.hdmoe_block_plan_get(ctypes.byref(a), 1, ctypes.byref(p)))
+                if exact or a_dtype == L.W_F16 or (rows <= 64 and not fixed):
+                    assert p.exact, (form, rows, K, N)
+                    few += 1
+                elif fixed:
+                    assert not p.exact    # one kind at any size
+                else:
+                    many += not p.exact
+                assert not (p.exact and p.kernel == 2)
+        a.exact = a.fixed_k_cut = 0
+        L.check(L.lib.hdmoe_block_plan_get(ctypes.byref(a), 0, ctypes.byref(p)))
+        assert not p.exact
+    assert few > 100 and (many > 100 or a_dtype == L.W_F16)
