@@ -472,7 +472,7 @@ __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_
   // The loads are written by hand so that the compiler, which takes any of them for one that a later LDS read may want, does not wait.
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
   auto to_lds = [](const __amdgpu_buffer_rsrc_t& r, uint32_t lds, int voff, int soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
   };
   // load i of the step kb into `stage`
   auto load = [&](int i, int stage, int kb) {
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(64 * WF * WT, STAGES == 2 ? 4 : 2) void block_gemm_
       else to_lds(rb0, at + (BM + j * ROWS_PER_LOAD) * BLK, vb[j] | mask, k0);
     } else {
       const uint32_t ss = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + (BM + BN) * BLK + wave * 256);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(ss), "v"(tok), "s"(rs), "s"(min(kb, KB - 1) * s_step) : "memory");
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(ss), "v"(tok), "s"(rs), "s"(min(kb, KB - 1) * s_step) : "memory", "m0");
     }
   };
   constexpr int LOADS = LA + LB + 1;
@@ -739,7 +739,7 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
                         [n] "+s"(n), [left] "+s"(left), [so] "+s"(so), [ss] "+s"(ss), [sw] "+s"(so_w), [ws] "+s"(ws) \
                       : "{v[14:17]}"(tok), [ra] "s"(src.ra), [rb0] "s"(src.rb0), [rb1] "s"(src.rb1), [rs] "s"(src.rs), [rw0] "s"(src.rw0), [rw1] "s"(src.rw1), \
                         [ssi] "s"(src.ld_s), [ldsw] "s"(ldsw), [steps] "s"(src.KB), [nt] "s"((cur.rows_here + 63) / 64) \
-                      : "memory", "scc", "s60", "s61", "s62")
+                      : "memory", "m0", "scc", "s60", "s61", "s62")
     if constexpr (SWIGLU) HDMOE_BLOCK_LOOP(HDMOE_BLOCK_SWIGLU);
     else HDMOE_BLOCK_LOOP(HDMOE_BLOCK_PLAIN);
 
@@ -860,10 +860,10 @@ __global__ __launch_bounds__(64 * STREAM_WAVES) void block_stream_kernel(const B
   const uint32_t ring = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr_t)smem + wave * RING);
   // (by hand: the compiler takes any of them for one that a later LDS read may want)
   auto to_lds = [](const __amdgpu_buffer_rsrc_t& r, uint32_t lds, int voff, int soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
   };
   auto word_to_lds = [](const __amdgpu_buffer_rsrc_t& r, uint32_t lds, int voff, int soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(lds), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
   };
   constexpr int SCALES = 2048 * (FT + XT);   // of a slot: w1's, w3's, the tokens', 64 words each
   auto issue = [&](int slot, int kb) {   // (past the last K block as well, asking for nothing: the loads on their way are counted)
