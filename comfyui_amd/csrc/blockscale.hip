@@ -776,13 +776,13 @@ __global__ __launch_bounds__(512) void block_gemm8_kernel(const BlockArgs args) 
 // CAST: the activations are 16-bit rows; the block casts its own into LDS (rows of K + 16 bytes: 16 rows then hit all banks) while the
 // first weights are on their way, instead of a launch of its own in front.
 constexpr int STREAM_WAVES = 4, CAST_UNITS = 128;   // CAST: blocks of 128 values that a thread block can cast
-// Blocks of a CU at once: two where half of the LDS holds enough on its way, so that one starts while the other streams (gate/up and down of 2 tokens,
-// 2560 x 6912 x 2560, 33.2 us, 42.4 with one).
-constexpr int stream_blocks(int ft, int tt, bool cast) { return cast || ft * tt <= 2 ? 2 : 1; }
+// Blocks that rings are sized for on a CU: two where half of the LDS holds enough on its way, so that one starts while the other streams. What the
+// blocks cast for themselves comes on top (stream_blocks).
+constexpr int stream_rings(int ft, int tt, bool cast) { return cast || ft * tt <= 2 ? 2 : 1; }
 // Of a wave: a K block of weights and activations with their scales, and how many of them its ring has
 constexpr int stream_slot(int ft, int tt, bool swiglu, bool cast) { return 2048 * (ft + (cast ? 0 : tt)) + 256 * (1 + (swiglu ? 1 : 0) + (cast ? 0 : 1)); }
 constexpr int stream_depth(int ft, int tt, bool swiglu, bool cast) {
-  const int budget = stream_blocks(ft, tt, cast) == 1 ? 159744 : cast ? 73728 : 81920, n = budget / (STREAM_WAVES * stream_slot(ft, tt, swiglu, cast));
+  const int budget = stream_rings(ft, tt, cast) == 1 ? 159744 : cast ? 73728 : 81920, n = budget / (STREAM_WAVES * stream_slot(ft, tt, swiglu, cast));
   return n > 8 ? 8 : n;
 }
 
@@ -793,6 +793,8 @@ constexpr int stream_raw_bytes(int rows, int KB) { return (rows * KB + 4 * STREA
 constexpr int stream_lds(int ft, int tt, bool swiglu, bool cast, int rows, int KB) {
   return STREAM_WAVES * stream_depth(ft, tt, swiglu, cast) * stream_slot(ft, tt, swiglu, cast) + (cast ? stream_cast_bytes(rows, KB) + stream_raw_bytes(rows, KB) : 0);
 }
+// Blocks that a CU holds at once. Casting, two of gate/up only for one row (2560 values: 80640 bytes; two rows 87296).
+constexpr int stream_blocks(int ft, int tt, bool swiglu, bool cast, int rows, int KB) { return 163840 / stream_lds(ft, tt, swiglu, cast, rows, KB) >= 2 ? 2 : 1; }
 
 template <class Act, bool SWIGLU, int FT, int TT, bool CAST>
 __global__ __launch_bounds__(64 * STREAM_WAVES) void block_stream_kernel(const BlockArgs args) {
@@ -1155,11 +1157,11 @@ double tiles_of(const Sizes& z, int bm, int feat) {   // in tiles of the experts
 // Few rows. 3.5 us to a block's first operands and behind its last, 80 KB/us of weights and activations for a CU (32 x 6912 x 2560 with its cast, 1, 2 and 4 strips a
 // block: 12.1, 10.6, 13.1 us); 55 KB/us where a wave multiplies 16 tiles of each K block and has only one more on its way (100 x 2560 x 6912: 13.9, 17.9 in
 // two rounds of 8 tiles).
-double few_us(const Sizes& z, bool swiglu, int tt, int ft, bool cast) {
+double few_us(const Sizes& z, bool swiglu, int tt, int ft, bool cast, int lds_rows) {
   const double blocks = tiles_of(z, 16 * tt, swiglu ? 8 * ft : 16 * ft);
   const int per = z.rows > 0 ? (z.rows + z.E - 1) / z.E : 0, most = per > z.rows_static ? per : z.rows_static;
   const int rows = most < 16 * tt ? most : 16 * tt, K = z.rows > 0 ? z.K : z.K_static;
-  return 1.7 + ceil(blocks / (HDMOE_NUM_CU * stream_blocks(ft, tt, cast))) * 3.5 + ceil(blocks / HDMOE_NUM_CU) * (16.0 * ft + rows) * K / (ft * tt == 16 ? 55e3 : 80e3) + (swiglu ? 3.5 : 0.0);
+  return 1.7 + ceil(blocks / (HDMOE_NUM_CU * stream_blocks(ft, tt, swiglu, cast, lds_rows, (K + BLK - 1) / BLK))) * 3.5 + ceil(blocks / HDMOE_NUM_CU) * (16.0 * ft + rows) * K / (ft * tt == 16 ? 55e3 : 80e3) + (swiglu ? 3.5 : 0.0);
 }
 // Low tiles. 128 x 6912 x 2560: 32.7 us with four stages (two 41.6), where a step lasts half as long as memory's answer; from a block for every CU on
 // two blocks share one (1024 x 2560 x 6912: 32.6 against 25.8).
@@ -1219,7 +1221,7 @@ Plan plan_of(bool swiglu, int a_dtype, const Sizes& z, bool fixed, bool exact) {
         p.lds_rows = whole < 16 ? whole : 16;
         p.cast_inside = (long long)p.lds_rows * ((K + BLK - 1) / BLK) <= CAST_UNITS && (long long)whole * K * 2 <= 0x7fffffff;
       }
-      double t = few_us(z, swiglu, tt, ft, p.cast_inside);
+      double t = few_us(z, swiglu, tt, ft, p.cast_inside, p.lds_rows);
       if (p.cast_inside) t -= 4.0;
       offer(t, p);
     }
@@ -1393,7 +1395,7 @@ extern "C" int hdmoe_block_plan_get(const hdmoe_block_args* p, int swiglu, hdmoe
     out->strips = plan.ft;
     out->cast_inside = plan.cast_inside;
     out->lds_bytes = stream_lds(plan.ft, plan.tt, swiglu != 0, plan.cast_inside, plan.lds_rows, (K + BLK - 1) / BLK);
-    out->blocks_per_cu = stream_blocks(plan.ft, plan.tt, plan.cast_inside);
+    out->blocks_per_cu = stream_blocks(plan.ft, plan.tt, swiglu != 0, plan.cast_inside, plan.lds_rows, (K + BLK - 1) / BLK);
   } else if (plan.stages > 0) {
     out->kernel = HDMOE_BLOCK_LOW_TILES;
     out->tile_rows = swiglu ? 64 : 128;

@@ -89,6 +89,19 @@ def test_a_block_fits_its_cu():
         assert 0 < p.lds_bytes <= 163840
 
 
+def test_blocks_fit_their_cu_together():
+    """As many as the choice counts on: rings, and the rows that a block casts for itself, in 160 KiB."""
+    rng, casting = random.Random(9), 0
+    for _ in range(20000):
+        rows, K, N = sample(rng, 16384)
+        p = plan(rng.choice((0, 1)), rng.choice((L.W_BF16, L.W_E4M3FN)), rows, rng.choice((0, 1, 4, 8)), K, N)
+        assert p.blocks_per_cu * p.lds_bytes <= 163840, (rows, K, N)
+        casting += p.cast_inside
+    assert casting > 1000
+    two, one = plan(1, L.W_BF16, 2, 4, 2560, 6912), plan(1, L.W_BF16, 1, 4, 2560, 6912)
+    assert (two.cast_inside, two.lds_bytes, two.blocks_per_cu) == (1, 87296, 1) and (one.lds_bytes, one.blocks_per_cu) == (80640, 2)
+
+
 @pytest.mark.parametrize("a_dtype", [L.W_BF16, L.W_F16, L.W_E4M3FN])
 def test_gate_up_has_exact_products_where_the_header_says(a_dtype):
     """Up to 64 rows in each group, with fp16 activations, and when asked. (A Linear has none, and no flag.)"""
