@@ -248,8 +248,7 @@ class FeedForwardSwiGLU(nn.Module):
         got = _block_parts([self], x)
         if got is None:
             return None
-        x2 = x.reshape(-1, x.shape[-1]).contiguous()
-        h, sh = HF.swiglu_block_fp8(x2, *got[0][0], fixed_k_cut=_same_sums([self], "w1", "w3"))
+        h, sh = HF.swiglu_block_fp8(amd_ops.block_fp8_rows(x), *got[0][0], fixed_k_cut=_same_sums([self], "w1", "w3"))
         w, s, b = got[1][0]
         return HF.linear_block_fp8(h, w, s, bias=b, scale_x=sh, out_dtype=x.dtype, fixed_k_cut=_same_sums([self], "w2")).view(*x.shape[:-1], w.shape[0])
 
@@ -398,7 +397,7 @@ class MOEFeedForwardSwiGLU(nn.Module):
         gate_w = _gate_weight(self.gate, x2)
         parts = _block_parts([*self.experts, self.shared_experts], x2)
         if parts is not None:
-            return self._forward_block(x2, gate_w, *parts).view(*orig_shape)
+            return self._forward_block(amd_ops.block_fp8_rows(x2), gate_w, *parts).view(*orig_shape)
         got = self._one_call(x2)
         if got is not None:
             wdt, experts, shared, keep, H, Hs = got

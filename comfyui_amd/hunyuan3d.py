@@ -204,6 +204,7 @@ class MoEBlock(nn.Module):
             first, second = parts
             ffs = (*self.experts, self.shared_experts)   # one that asks for it has the launch that it shares
             fixed = [any(amd_ops._batch_invariant(l) for l in ls) for ls in ([f.net[0].proj for f in ffs], [f.net[2] for f in ffs])]
+            x2 = amd_ops.block_fp8_rows(x2)
             h, h_sh = HF.grouped_linear_block_fp8(x2, offsets, first[:-1], perm=perm, shared=first[-1], a_static=x2, fixed_k_cut=fixed[0])
             y, y_sh = HF.grouped_linear_block_fp8(HF.gelu(h), offsets, second[:-1], shared=second[-1], a_static=HF.gelu(h_sh), fixed_k_cut=fixed[1])
             return HF.combine(y, inv_perm, w, y_sh).view(*orig_shape)

@@ -376,6 +376,12 @@ def scaled_fp8_ops(fp8_matrix_mult=False, scale_input=False, override_dtype=None
     return scaled_fp8_op
 
 
+def block_fp8_rows(input):
+    """input's rows as the block-scaled operators take them: [rows, K], contiguous, on 16 bytes (a view may start anywhere; it is copied)."""
+    x2 = input.reshape(-1, input.shape[-1]).contiguous()
+    return x2 if x2.data_ptr() % 16 == 0 else x2.clone()
+
+
 class block_fp8_ops(manual_cast):
     """Operations class whose Linear weights are float8_e4m3fn with one fp32 scale for every 128 x 128 block
     (`scale_weight` [ceil(out / 128), ceil(in / 128)]) and whose activations are cast with one for every 128 values of a row, as they
@@ -408,8 +414,7 @@ class block_fp8_ops(manual_cast):
 
         def forward_comfy_cast_weights(self, input):
             weight, scale, bias = self.parts(input)
-            x2 = input.reshape(-1, input.shape[-1]).contiguous()
-            return HF.linear_block_fp8(x2, weight, scale, bias=bias, fixed_k_cut=_batch_invariant(self)).reshape(*input.shape[:-1], weight.shape[0])
+            return HF.linear_block_fp8(block_fp8_rows(input), weight, scale, bias=bias, fixed_k_cut=_batch_invariant(self)).reshape(*input.shape[:-1], weight.shape[0])
 
         def _spread(self, weight):
             """scale_weight as one fp32 value per element, on the weight's device (fp16 would lose scales below 2^-25)."""
