@@ -1198,6 +1198,8 @@ Plan plan_of(bool swiglu, int a_dtype, const Sizes& z, bool fixed, bool exact) {
   exact = swiglu && (exact || a_dtype == HDMOE_W_F16 || (!fixed && z.rows <= EXACT_ROWS && z.rows_static <= EXACT_ROWS));
   Plan best = {0, 0, false, 0, 0, 4, false};
   double us = exact ? 1e30 : high_us(z, swiglu, 4);   // (that kernel's loop has no exact products)
+  Plan rows16 = best;   // of the few-row kernels on tiles of 16 rows
+  double us16 = 1e30;
   auto offer = [&](double t, const Plan& p) {
     if (t < us) {
       us = t;
@@ -1224,7 +1226,17 @@ Plan plan_of(bool swiglu, int a_dtype, const Sizes& z, bool fixed, bool exact) {
       double t = few_us(z, swiglu, tt, ft, p.cast_inside, p.lds_rows);
       if (p.cast_inside) t -= 4.0;
       offer(t, p);
+      if (tt == 1 && (p.cast_inside ? p.lds_rows <= 4 : z.rows_static == 0) && t < us16) {
+        us16 = t;
+        rows16 = p;
+      }
     }
+  // Exact products take the low tiles 0.45 us more a step (600 rows in eight segments, K 1024: 27.1 -> 30.7 us), for empty rows too: segments of up to 16
+  // rows go to tiles of 16 (8 to 32 rows of four experts, 2560 x 6912: 36 us, low tiles 42; 15 of eight, 1392 x 5456: 44 and 57; 143 of sixteen,
+  // 2304 x 1648: 4 % less). Not beside a shared expert (8 tokens, 3584 wide: 49 us, low tiles 46), not for up to 8 steps, and where blocks cast
+  // their rows over and over only up to four of them (a layer of 2 tokens: 38 us, low tiles 43; 5 rows of eight, 1600 x 5536: 10 % more).
+  const int kb = (K + BLK - 1) / BLK;
+  if (exact && best.stages > 0 && kb > 8 && z.rows <= 16 * z.E && us16 < us + 0.45 * kb) best = rows16;
   return best;
 }
 
