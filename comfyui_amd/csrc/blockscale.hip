@@ -272,9 +272,9 @@ struct Deal {
 // sum off by 6e-5 of itself. That drowns in the rounding of a 16-bit output, but not where the sum is cast again: 0.23 % of an intermediate's
 // codes then are a step off (0.003 % with exact products), and the feed-forward's output by 0.0013 of itself: below bf16's rounding, six times fp16's.
 // EXACT: the values as fp16, which holds them, at half the rate and behind a conversion; products and sums are fp32. Gate/up has it up to EXACT_ROWS
-// rows, where a handful of codes can be much of an output (2560 x 6912, four experts: 2 rows 34.4 us, 33.7 without, gate/up and down; gate/up of 8 to
-// 64 rows 45 us, 40 without), and on any number where the caller asks for it or the activations are fp16 (600 rows in eight segments, 1024 x 1024 x
-// 1024, 30.7 and 27.1; 16384 in four, 2560 x 4096 x 2560, 1258 us, 521 on the 256-row tiles, whose loop has none).
+// rows, where a handful of codes can be much of an output (2560 x 6912, four experts: 2 rows 34.4 us, 33.7 without, gate/up and down; gate/up of
+// 64 rows 45 us, 40 without, of a layer of 4 to 32 tokens with its shared expert 46 and 41.5), and on any number where the caller asks for it or the activations are
+// fp16 (600 rows in eight segments, 1024 x 1024 x 1024, 30.7 and 27.1; 16384 in four, 2560 x 4096 x 2560, 1258 us, 521 on the 256-row tiles, whose loop has none).
 template <bool EXACT>
 __device__ __forceinline__ v4f block_product(const v8i& a, const v8i& b) {
   v4f c = {0, 0, 0, 0};
