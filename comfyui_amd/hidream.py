@@ -199,7 +199,7 @@ def _block_parts(ffns, x):
         return None
     if not isinstance(ffns[0].w1, amd_ops.block_fp8_ops.Linear):
         return None
-    if any(l.bias is not None for f in ffns for l in (f.w1, f.w3)):   # gate/up has none
+    if any(getattr(l, "bias", None) is not None for f in ffns for l in (f.w1, f.w3)):   # gate/up has none
         return None
     parts = amd_ops.block_fp8_parts([l for f in ffns for l in (f.w1, f.w3, f.w2)], x)
     if parts is None:

@@ -55,3 +55,11 @@ def test_weights_are_brought_over_only_where_they_are_used(monkeypatch):
     down = feed_forward()
     down.w2.bias = torch.nn.Parameter(torch.zeros(64, dtype=torch.bfloat16))
     assert hidream._block_parts([plain, down], x)[1][1][2] is not None
+
+
+def test_a_linear_wrapped_in_another_module_is_left_to_itself():
+    """Wrappers (adapters) need not have a bias to be looked at."""
+    x = torch.zeros((1, 64), dtype=torch.bfloat16)
+    plain, wrapped = feed_forward(), feed_forward()
+    wrapped.w1 = torch.nn.Sequential(wrapped.w1)
+    assert hidream._block_parts([plain, wrapped], x) is None
