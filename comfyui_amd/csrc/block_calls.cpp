@@ -342,10 +342,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_block_calls", nullptr, -1, method
 
 }  // namespace
 
-// torch_version: whose headers this was compiled with; the caller compares it with the torch that is there
+// torch_version, hdmoe_version: whose headers this was compiled with; the caller compares them with the torch and the library that are there
 PyMODINIT_FUNC PyInit__block_calls() {
   PyObject* const m = PyModule_Create(&module);
-  if (m != nullptr && PyModule_AddStringConstant(m, "torch_version", HDMOE_TORCH_VERSION) != 0) {
+  if (m != nullptr && (PyModule_AddStringConstant(m, "torch_version", HDMOE_TORCH_VERSION) != 0 || PyModule_AddIntConstant(m, "hdmoe_version", HDMOE_VERSION) != 0)) {
     Py_DECREF(m);
     return nullptr;
   }

@@ -13,8 +13,8 @@ from ._lib import FfnWeights, LayerArgs, LayerLayout, W_BF16, W_E4M3FN, check, l
 
 try:
     from . import _block_calls
-    if getattr(_block_calls, "torch_version", None) != torch.__version__:
-        raise ImportError(f"not built for torch {torch.__version__}")
+    if (getattr(_block_calls, "torch_version", None), getattr(_block_calls, "hdmoe_version", None)) != (torch.__version__, lib.hdmoe_version()):
+        raise ImportError(f"not built for torch {torch.__version__} and this library")
 except ImportError as e:   # host code only: every call it makes is made below as well, at a few times the host's time
     logging.warning("comfyui_amd: no compiled calls of the block-scaled operators (%s). `python -m comfyui_amd.build` builds them.", e)
     _block_calls = None

@@ -1,4 +1,4 @@
-"""The package where _block_calls.so is missing or was built for another torch: it imports, with a warning, and makes the calls itself."""
+"""The package where _block_calls.so is missing or was built for another torch or another library: it imports, with a warning, and makes the calls itself."""
 import os
 import subprocess
 import sys
@@ -24,7 +24,10 @@ MISSING = "sys.modules['comfyui_amd._block_calls'] = None"
 OTHER = "m = types.ModuleType('m'); m.torch_version = '1.0'; sys.modules['comfyui_amd._block_calls'] = m"
 
 
-@pytest.mark.parametrize("block", [MISSING, OTHER], ids=["missing", "other torch"])
+OLDER = "import torch; m = types.ModuleType('m'); m.torch_version, m.hdmoe_version = torch.__version__, 117; sys.modules['comfyui_amd._block_calls'] = m"
+
+
+@pytest.mark.parametrize("block", [MISSING, OTHER, OLDER], ids=["missing", "other torch", "older library"])
 def test_import(block):
     r = subprocess.run([sys.executable, "-c", PROGRAM.format(block=block)], cwd=ROOT, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
@@ -34,4 +37,4 @@ def test_import(block):
 def test_the_built_one_is_taken():
     import torch
     from comfyui_amd import functional as HF
-    assert HF._block_calls is not None and HF._block_calls.torch_version == torch.__version__
+    assert HF._block_calls is not None and HF._block_calls.torch_version == torch.__version__ and HF._block_calls.hdmoe_version == HF.lib.hdmoe_version()
