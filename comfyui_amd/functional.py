@@ -727,7 +727,8 @@ def linear_block_fp8(x, weight, scale_weight, bias=None, scale_x=None, out_dtype
     """x [rows, K] times weight [N, K]^T (+ bias [N]): weight float8_e4m3fn with fp32 scales scale_weight
     [ceil(N / 128), ceil(K / 128)]; x bf16 or fp16 (cast as quant_block_fp8 does), or float8_e4m3fn with its scales scale_x
     [rows, ceil(K / 128)] (laid out anew unless they are as quant_block_fp8 returns them). -> [rows, N] of x's type (out_dtype, bf16
-    unless given, for float8_e4m3fn x). K and N are multiples of 16; x, weight and bias are contiguous and start on 16 bytes. The sums are fp32; bias joins them before the one rounding.
+    unless given, for float8_e4m3fn x). K and N are multiples of 16; x, weight and bias are contiguous and
+    start on 16 bytes. The sums are fp32; bias joins them before the one rounding.
     fixed_k_cut: the sums go in one order whatever the number of rows: a row's bytes do not depend on which rows come with it (few rows are
     otherwise dealt along K, up to three times as fast)."""
     st = _stream_here(x)
