@@ -17,12 +17,14 @@ W_BF16 = 0
 W_E4M3FN = 1
 W_F16 = 2
 W_E4M3FN_UPCAST = 3     # e4m3fn weights, bf16 arithmetic
+T_BF16, T_F16, T_F32 = 0, 2, 4   # element types of the layer norm and of the products with a narrow side
 SRC_BF16 = 0
 SRC_F32 = 2
 ACT_NONE = 0
 ACT_GELU = 1
 MAX_EXPERTS = 16
 BLOCK_MAX_EXPERTS = 32
+NORM_MAX_D = 16384
 E_NULL, E_SHAPE, E_WORKSPACE, E_LAUNCH = -1, -2, -3, -4
 TOPK = 2
 NUM_STAGES = 6
@@ -112,6 +114,16 @@ class BlockArgs(ctypes.Structure):
     ]
 
 
+class NormGradArgs(ctypes.Structure):
+    """hdmoe_norm_grad_args"""
+    _fields_ = [
+        ("dtype", c_int), ("gain_dtype", c_int), ("D", c_int), ("one_plus", c_int),
+        ("rows", c_int64), ("rows_per_group", c_int64), ("eps", ctypes.c_float),
+        ("dy", c_void_p), ("x", c_void_p), ("weight", c_void_p), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 class BlockPlan(ctypes.Structure):
     """hdmoe_block_plan"""
     _fields_ = [(n, c_int) for n in ("kernel", "tile_rows", "strips", "cast_inside", "stages", "blocks_per_cu", "lds_bytes", "exact")]
@@ -184,6 +196,9 @@ SIGNATURES = {
     "hdmoe_block_plan_get": (c_int, [ctypes.POINTER(BlockArgs), c_int, ctypes.POINTER(BlockPlan)]),
     "hdmoe_block_linear": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
     "hdmoe_block_swiglu": (c_int, [ctypes.POINTER(BlockArgs), c_void_p]),
+    "hdmoe_layer_norm": (c_int, [c_int, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, ctypes.c_float, c_void_p, c_void_p]),
+    "hdmoe_layer_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int64]),
+    "hdmoe_layer_norm_backward": (c_int, [ctypes.POINTER(NormGradArgs), c_void_p]),
     "hdmoe_layer_layout_get": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(LayerLayout)]),
 }
 

@@ -896,3 +896,108 @@ def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None, fixed_k_cut=Fa
             f.scale_out, f.scale_out_stride = sh.data_ptr(), rows
             _block_call(lib.hdmoe_block_swiglu, 1, args, x)
     return h, sh
+
+
+# ---- layer norm and its gradients --------------------------------------------------------------------------------
+
+_T_CODE = {BF16: _lib.T_BF16, F16: _lib.T_F16, torch.float32: _lib.T_F32}
+
+
+def _norm_rows(x, what):
+    """(dtype, rows, D) of contiguous rows of bf16, fp16 or fp32 on the device."""
+    if x.dtype not in _T_CODE:
+        raise TypeError(f"{what}: expected bfloat16, float16 or float32, got {x.dtype}")
+    _need_hip(x, what)
+    D = x.shape[-1] if x.dim() > 0 else 0
+    if not 1 <= D <= _lib.NORM_MAX_D:
+        raise ValueError(f"{what}: rows of {D} values (1 to {_lib.NORM_MAX_D})")
+    return x.dtype, x.numel() // D, D
+
+
+def _norm_gain(t, x, shape, what):
+    """Code of a gain's type: that of x or fp32."""
+    if t.dtype != x.dtype and t.dtype != torch.float32:
+        raise TypeError(f"{what}: expected {x.dtype} or float32, got {t.dtype}")
+    if t.device != x.device or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: expected contiguous {list(shape)} on {x.device}, got {tuple(t.shape)} on {t.device}")
+    return _T_CODE[t.dtype]
+
+
+def _norm_gains(x, weight, bias, D, what):
+    code = _T_CODE[x.dtype]
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            code = _norm_gain(t, x, (D,), f"{what} {name}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"{what}: weight {weight.dtype} and bias {bias.dtype} differ in type")
+    return code
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """torch.nn.functional.layer_norm over the last axis: (x - mean) / sqrt(var + eps) * weight + bias. x [..., D] bf16, fp16 or fp32,
+    contiguous, D from 1 to 16384; weight, bias [D] of x's type or fp32 (both the same). Statistics are fp32, of the values' differences from
+    their mean; the result is rounded once. ln_modulate, with a scale and a shift of each batch item, rounds between its steps."""
+    what = "layer_norm"
+    _, rows, D = _norm_rows(x, what + " x")
+    code = _norm_gains(x, weight, bias, D, what)
+    with _on(x.device):
+        out = torch.empty_like(x)
+        check(lib.hdmoe_layer_norm(_T_CODE[x.dtype], ptr(x), rows, D, code, ptr(weight), ptr(bias), eps, ptr(out), _raw_stream(x)))
+    return out
+
+
+def _norm_backward(dy, x, weight, dweight, dbias, gain_code, D, rows, per_group, one_plus, eps):
+    dx = torch.empty_like(x)
+    args = _lib.NormGradArgs()
+    args.dtype, args.gain_dtype, args.D, args.one_plus = _T_CODE[x.dtype], gain_code, D, one_plus
+    args.rows, args.rows_per_group, args.eps = rows, per_group, eps
+    args.dy, args.x, args.weight = ptr(dy), ptr(x), ptr(weight)
+    args.dx, args.dweight, args.dbias = ptr(dx), ptr(dweight), ptr(dbias)
+    if dweight is not None or dbias is not None:
+        nbytes = lib.hdmoe_layer_norm_backward_workspace_bytes(rows, D, per_group)
+        if nbytes > 0:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    check(lib.hdmoe_layer_norm_backward(ctypes.byref(args), _raw_stream(x)))
+    return dx
+
+
+def _norm_dy(dy, x, what):
+    if dy.dtype != x.dtype or dy.shape != x.shape or dy.device != x.device or not dy.is_contiguous():
+        raise ValueError(f"{what}: dy must be contiguous {x.dtype} {list(x.shape)} on {x.device}, got {dy.dtype} {tuple(dy.shape)} on {dy.device}")
+
+
+def layer_norm_backward(dy, x, weight=None, bias=None, eps=1e-5):
+    """Gradients of layer_norm(x, weight, bias, eps) from dy, that of its result: (dx, dweight, dbias), None for a weight or bias that is
+    None. Nothing is kept from the forward pass: mean and variance are taken from x again, which is read anyway. dweight and
+    dbias are summed over the rows in fp32, in an order that depends on the sizes alone, and have their gains' type."""
+    what = "layer_norm_backward"
+    _, rows, D = _norm_rows(x, what + " x")
+    _norm_dy(dy, x, what)
+    code = _norm_gains(x, weight, bias, D, what)
+    with _on(x.device):
+        dweight = None if weight is None else torch.empty_like(weight)
+        dbias = None if bias is None else torch.empty_like(bias)
+        dx = _norm_backward(dy, x, weight, dweight, dbias, code, D, rows, rows, 0, eps)
+    return dx, dweight, dbias
+
+
+def ln_modulate_backward(dy, x2d, scale, tokens_per_batch, eps=1e-6):
+    """Gradients of LayerNorm(x) * (1 + scale) + shift with one row of scale and shift for tokens_per_batch rows, from dy:
+    (dx [T, D], dscale [B, D], dshift [B, D]). bf16 as ln_modulate, whose roundings between its steps count as none here, fp16 or
+    fp32. Sums over a batch item's rows are fp32."""
+    what = "ln_modulate_backward"
+    dt, T, D = _norm_rows(x2d, what + " x")
+    if x2d.dim() != 2:
+        raise ValueError(f"{what}: expected x [T, D], got {tuple(x2d.shape)}")
+    _norm_dy(dy, x2d, what)
+    if scale.dim() == 3 and scale.shape[1] == 1:
+        scale = scale[:, 0]
+    if scale.dim() != 2 or scale.dtype != dt or scale.shape[1] != D or scale.device != x2d.device or not scale.is_contiguous():
+        raise ValueError(f"{what}: scale must be contiguous {dt} [batch, {D}] on {x2d.device}, got {scale.dtype} {tuple(scale.shape)} on {scale.device}")
+    if tokens_per_batch <= 0 or T != scale.shape[0] * tokens_per_batch:
+        raise ValueError(f"{what}: T={T} is not batch={scale.shape[0]} x tokens_per_batch={tokens_per_batch}")
+    with _on(x2d.device):
+        dscale, dshift = torch.empty_like(scale), torch.empty_like(scale)
+        dx = _norm_backward(dy, x2d, scale, dscale, dshift, _T_CODE[dt], D, T, tokens_per_batch, 1, eps)
+    return dx, dscale, dshift

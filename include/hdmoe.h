@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define HDMOE_VERSION 118
+#define HDMOE_VERSION 119
 
 #define HDMOE_OK 0
 #define HDMOE_E_NULL (-1)      /* required pointer is NULL */
@@ -366,6 +366,39 @@ int hdmoe_combine_gated_residual(const void* y_sorted_bf16, const int32_t* inv_p
  * out[t] = bf16( bf16(gate[t / tokens_per_batch] * y[t]) + residual[t] ). */
 int hdmoe_gated_residual_bf16(const void* y_bf16, const void* gate_bf16, const void* residual_bf16,
                               int tokens_per_batch, int T, int D, void* out_bf16, hdmoe_stream_t stream);
+
+/* ---- layer norm and its gradients ---------------------------------------------- */
+
+/* element types of the entry points below (fp16 and bf16 have the codes of HDMOE_W_*) */
+#define HDMOE_T_BF16 0
+#define HDMOE_T_F16 2
+#define HDMOE_T_F32 4
+#define HDMOE_NORM_MAX_D 16384
+
+/* out = (x - mean) / sqrt(var + eps) * weight + bias of every row of x [rows, D], D from 1 to HDMOE_NORM_MAX_D: torch.nn.LayerNorm over the last
+ * axis. weight, bias [D] of gain_dtype (the rows' type or fp32); either may be NULL. Statistics and products are fp32, rounded
+ * once. out may not overlap the inputs; rows start on any multiple of their element's size. */
+int hdmoe_layer_norm(int dtype, const void* x, int64_t rows, int D, int gain_dtype, const void* weight, const void* bias, float eps,
+                     void* out, hdmoe_stream_t stream);
+
+/* Gradients of y = n * (weight + one_plus) + bias, n = (x - mean) / sqrt(var + eps), where weight [rows / rows_per_group, D] has one row
+ * for rows_per_group rows of x (an affine norm: rows_per_group = rows; hdmoe_ln_modulate_bf16: tokens_per_batch and one_plus, the
+ * roundings between its steps taken as none):
+ *   dx [rows, D]; dweight [groups, D] = sum dy n; dbias [groups, D] = sum dy     (the last two NULL: not wanted)
+ * weight NULL is a gain of one_plus, or 1 where that is 0 too. Sums over rows are fp32 in one fixed order, rounded once to gain_dtype. rows = 0 with
+ * rows_per_group = 0 leaves zeros in dweight and dbias [D]. Outputs may not overlap inputs. workspace: hdmoe_layer_norm_backward_workspace_bytes, on
+ * 16 bytes, device, only if dweight or dbias is wanted. */
+typedef struct hdmoe_norm_grad_args {
+  int dtype, gain_dtype, D, one_plus;
+  int64_t rows, rows_per_group;
+  float eps;
+  const void *dy, *x, *weight;
+  void *dx, *dweight, *dbias;
+  void* workspace;
+  size_t workspace_bytes;
+} hdmoe_norm_grad_args;
+size_t hdmoe_layer_norm_backward_workspace_bytes(int64_t rows, int D, int64_t rows_per_group);
+int hdmoe_layer_norm_backward(const hdmoe_norm_grad_args* args, hdmoe_stream_t stream);
 
 /* ---- e4m3fn with a scale for each block of 128 --------------------------------- */
 
