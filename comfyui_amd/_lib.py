@@ -25,6 +25,8 @@ ACT_GELU = 1
 MAX_EXPERTS = 16
 BLOCK_MAX_EXPERTS = 32
 NORM_MAX_D = 16384
+ADAPTER_MAX = 4096
+ADAPTER_MAX_RANK = 256
 E_NULL, E_SHAPE, E_WORKSPACE, E_LAUNCH = -1, -2, -3, -4
 TOPK = 2
 NUM_STAGES = 6
@@ -124,6 +126,13 @@ class NormGradArgs(ctypes.Structure):
     ]
 
 
+class AdapterArgs(ctypes.Structure):
+    """hdmoe_adapter_args"""
+    _fields_ = [(n, c_int) for n in ("dtype", "rows", "requests", "K", "N", "n", "R")] + [
+        (n, c_void_p) for n in ("x", "a", "b", "scale", "index", "base", "out", "dy", "dx", "da", "db", "workspace")] + [
+        ("workspace_bytes", c_size_t)]
+
+
 class BlockPlan(ctypes.Structure):
     """hdmoe_block_plan"""
     _fields_ = [(n, c_int) for n in ("kernel", "tile_rows", "strips", "cast_inside", "stages", "blocks_per_cu", "lds_bytes", "exact")]
@@ -199,6 +208,9 @@ SIGNATURES = {
     "hdmoe_layer_norm": (c_int, [c_int, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, ctypes.c_float, c_void_p, c_void_p]),
     "hdmoe_layer_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int64]),
     "hdmoe_layer_norm_backward": (c_int, [ctypes.POINTER(NormGradArgs), c_void_p]),
+    "hdmoe_adapters_workspace_bytes": (c_size_t, [ctypes.POINTER(AdapterArgs), c_int]),
+    "hdmoe_add_adapters": (c_int, [ctypes.POINTER(AdapterArgs), c_void_p]),
+    "hdmoe_add_adapters_backward": (c_int, [ctypes.POINTER(AdapterArgs), c_void_p]),
     "hdmoe_layer_layout_get": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(LayerLayout)]),
 }
 

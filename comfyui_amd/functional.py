@@ -1001,3 +1001,79 @@ def ln_modulate_backward(dy, x2d, scale, tokens_per_batch, eps=1e-6):
         dscale, dshift = torch.empty_like(scale), torch.empty_like(scale)
         dx = _norm_backward(dy, x2d, scale, dscale, dshift, _T_CODE[dt], D, T, tokens_per_batch, 1, eps)
     return dx, dscale, dshift
+
+
+# ---- low-rank adapters of many requests --------------------------------------------------------------------------
+
+def _adapter_args(x, a, b, scale, index, what):
+    """AdapterArgs of x [rows, K] (or [..., K]) with the adapters' tensors, all checked."""
+    dt = _act_dtype(x, what + " x")
+    _need_hip(x, what + " x")
+    dev = x.device
+    if a.dim() != 3 or b.dim() != 3 or x.dim() < 2:
+        raise ValueError(f"{what}: expected x [..., K], a [n, R, K] and b [n, N, R], got {tuple(x.shape)}, {tuple(a.shape)} and {tuple(b.shape)}")
+    n, R, K = a.shape
+    N = b.shape[1]
+    if x.shape[-1] != K or b.shape[0] != n or b.shape[2] != R:
+        raise ValueError(f"{what}: x {tuple(x.shape)}, a {tuple(a.shape)} and b {tuple(b.shape)} do not match")
+    for name, t, dtype in (("a", a, dt), ("b", b, dt), ("scale", scale, torch.float32), ("index", index, torch.int32)):
+        if t.dtype != dtype:
+            raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+        if t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous on {dev}")
+    if scale.shape != (n,):
+        raise ValueError(f"{what}: scale must be [{n}], got {tuple(scale.shape)}")
+    rows = x.numel() // K if K > 0 else 0
+    requests = index.numel()
+    if rows > 0 and (requests == 0 or rows % requests != 0):
+        raise ValueError(f"{what}: {requests} requests do not divide {rows} rows")
+    args = _lib.AdapterArgs()
+    args.dtype, args.rows, args.requests, args.K, args.N, args.n, args.R = _T_CODE[dt], rows, requests, K, N, n, R
+    args.x, args.a, args.b, args.scale, args.index = ptr(x), ptr(a), ptr(b), ptr(scale), ptr(index)
+    return args
+
+
+def _adapter_rows(t, x, N, what):
+    if t.dtype != x.dtype or t.shape != (*x.shape[:-1], N) or t.device != x.device or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous {x.dtype} {[*x.shape[:-1], N]} on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _adapter_call(fn, args, x, backward):
+    nbytes = lib.hdmoe_adapters_workspace_bytes(ctypes.byref(args), backward)
+    if nbytes > 0:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    check(fn(ctypes.byref(args), _raw_stream(x)))
+
+
+def add_adapters(base, x, a, b, scale, index, out=None):
+    """base + scale[i] * b[i] @ (a[i] @ x) for every row, i the index of the row's request: low-rank adapters of many requests beside one
+    Linear, whose result base [..., N] is on x [..., K]. a [n, R, K] and b [n, N, R] of x's type (bf16 or fp16), R up to 256, adapters of a
+    smaller rank filled up with zeros; scale [n] fp32. index: int32, one for each request, each of as many rows of x in turn (x [B, S, K] with index [B]; an
+    index for each row: index [rows]); negative or from n on: no adapter, and the row is base's. Sums are fp32, the narrow product between the two
+    keeps 16 significant bits, the result is rounded once. `out`: takes the result, base itself if it is to be added in place."""
+    what = "add_adapters"
+    args = _adapter_args(x, a, b, scale, index, what)
+    _adapter_rows(base, x, args.N, what + " base")
+    if out is not None and out is not base:
+        _adapter_rows(out, x, args.N, what + " out")
+    with _on(x.device):
+        if out is None:
+            out = torch.empty_like(base)
+        args.base, args.out = ptr(base), ptr(out)
+        _adapter_call(lib.hdmoe_add_adapters, args, x, 0)
+    return out
+
+
+def add_adapters_backward(dy, x, a, b, scale, index):
+    """Gradients of add_adapters from dy, that of its result and of base: (dx, da, db) of the types of x, a and b. dx is the
+    adapters' part alone, 0 for rows without one; da and db are sums over each adapter's rows in fp32, in an order that depends on the sizes alone, 0 for an
+    adapter without rows."""
+    what = "add_adapters_backward"
+    args = _adapter_args(x, a, b, scale, index, what)
+    _adapter_rows(dy, x, args.N, what + " dy")
+    with _on(x.device):
+        dx, da, db = torch.empty_like(x), torch.empty_like(a), torch.empty_like(b)
+        args.dy, args.dx, args.da, args.db = ptr(dy), ptr(dx), ptr(da), ptr(db)
+        _adapter_call(lib.hdmoe_add_adapters_backward, args, x, 1)
+    return dx, da, db

@@ -400,6 +400,38 @@ typedef struct hdmoe_norm_grad_args {
 size_t hdmoe_layer_norm_backward_workspace_bytes(int64_t rows, int D, int64_t rows_per_group);
 int hdmoe_layer_norm_backward(const hdmoe_norm_grad_args* args, hdmoe_stream_t stream);
 
+/* ---- low-rank adapters of many requests beside a shared projection ------------- */
+
+/* out[t] = base[t] + scale[i] * b[i] . (a[i] . x[t]) with i = index[t / (rows / requests)]; an index outside 0 .. n - 1 is no adapter, and its
+ * rows of out are those of base. x [rows, K], base and out [rows, N] of dtype (bf16 or fp16), a [n, R, K], b [n, N, R] of the same; scale [n] fp32,
+ * index [requests] int32, requests a divisor of rows (every request has as many rows; requests = rows: an index for each). R from 1 to
+ * HDMOE_ADAPTER_MAX_RANK (adapters of a smaller rank are filled up with zeros), any K and N, n up to HDMOE_ADAPTER_MAX. a . x is held in fp32, and
+ * enters the second product with 16 significant bits; sums are fp32, out is rounded once. out may be base.
+ *
+ * The gradients, from dy [rows, N], that of out (and of base):
+ *   dx [rows, K] = scale dy b a (0 for rows without an adapter), da [n, R, K], db [n, N, R]: sums over the rows of each adapter, fp32 in one
+ * order that depends on the sizes alone. rows = 0 leaves zeros in da and db.
+ *
+ * What rows of other adapters hold, NaN among it, never reaches a row or a gradient. Outputs may not overlap inputs but for out and base. Rows start on
+ * any address of their type; workspace: hdmoe_adapters_workspace_bytes (backward 0 or 1), on 16 bytes, device. */
+#define HDMOE_ADAPTER_MAX 4096
+#define HDMOE_ADAPTER_MAX_RANK 256
+typedef struct hdmoe_adapter_args {
+  int dtype, rows, requests, K, N, n, R;
+  const void *x, *a, *b;
+  const float* scale;
+  const int32_t* index;
+  const void* base;          /* hdmoe_add_adapters */
+  void* out;
+  const void* dy;            /* hdmoe_add_adapters_backward */
+  void *dx, *da, *db;
+  void* workspace;
+  size_t workspace_bytes;
+} hdmoe_adapter_args;
+size_t hdmoe_adapters_workspace_bytes(const hdmoe_adapter_args* args, int backward);
+int hdmoe_add_adapters(const hdmoe_adapter_args* args, hdmoe_stream_t stream);
+int hdmoe_add_adapters_backward(const hdmoe_adapter_args* args, hdmoe_stream_t stream);
+
 /* ---- e4m3fn with a scale for each block of 128 --------------------------------- */
 
 /* Linears whose weights carry one fp32 scale for every 128 x 128 block and whose activations carry one for every 128
