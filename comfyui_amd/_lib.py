@@ -126,6 +126,13 @@ class NormGradArgs(ctypes.Structure):
     ]
 
 
+class BalanceArgs(ctypes.Structure):
+    """hdmoe_balance_args"""
+    _fields_ = [(n, c_int) for n in ("dtype", "T", "sequences", "D", "E", "k")] + [("alpha", ctypes.c_float)] + [
+        (n, c_void_p) for n in ("x", "gate_w", "topk_idx", "mask", "scores", "counts", "loss", "dloss", "dweight", "dx", "dgate_w", "workspace")] + [
+        ("workspace_bytes", c_size_t)]
+
+
 class AdapterArgs(ctypes.Structure):
     """hdmoe_adapter_args"""
     _fields_ = [(n, c_int) for n in ("dtype", "rows", "requests", "K", "N", "n", "R")] + [
@@ -208,6 +215,9 @@ SIGNATURES = {
     "hdmoe_layer_norm": (c_int, [c_int, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, ctypes.c_float, c_void_p, c_void_p]),
     "hdmoe_layer_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int, c_int64]),
     "hdmoe_layer_norm_backward": (c_int, [ctypes.POINTER(NormGradArgs), c_void_p]),
+    "hdmoe_gate_balance_workspace_bytes": (c_size_t, [ctypes.POINTER(BalanceArgs), c_int]),
+    "hdmoe_gate_balance": (c_int, [ctypes.POINTER(BalanceArgs), c_void_p]),
+    "hdmoe_gate_balance_backward": (c_int, [ctypes.POINTER(BalanceArgs), c_void_p]),
     "hdmoe_adapters_workspace_bytes": (c_size_t, [ctypes.POINTER(AdapterArgs), c_int]),
     "hdmoe_add_adapters": (c_int, [ctypes.POINTER(AdapterArgs), c_void_p]),
     "hdmoe_add_adapters_backward": (c_int, [ctypes.POINTER(AdapterArgs), c_void_p]),

@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhdmoe.so")
 CALLS_LIB = os.path.join(HERE, "_block_calls.so")
 PROBE_LIB = os.path.join(HERE, "libhdmoe_probe.so")
-SOURCES = ["gate.hip", "dispatch.hip", "elementwise.hip", "gemm.hip", "layer.hip", "weights.hip", "blockscale.hip", "norm.hip", "adapters.hip"]
+SOURCES = ["gate.hip", "dispatch.hip", "elementwise.hip", "gemm.hip", "layer.hip", "weights.hip", "blockscale.hip", "norm.hip", "router.hip", "adapters.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

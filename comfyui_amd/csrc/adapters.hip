@@ -386,24 +386,6 @@ __global__ __launch_bounds__(WAVES * 64, 2) void outer_kernel(OuterArgs p) {
     }
 }
 
-// Sums of `splits` parts in their order, rounded once; no parts: zeros.
-struct SumArgs {
-  const float* part[2];
-  uint16_t* out[2];
-  size_t n[2];
-  int splits;
-};
-template <class A>
-__global__ __launch_bounds__(256) void sum_parts_kernel(SumArgs p) {
-  size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const int side = i >= p.n[0];
-  if (side) i -= p.n[0];
-  if (i >= p.n[side]) return;
-  float v = 0.0f;
-  for (int s = 0; s < p.splits; ++s) v += p.part[side][s * p.n[side] + i];
-  p.out[side][i] = (uint16_t)A::pack(v, 0.0f);
-}
-
 // ---- sizes ---------------------------------------------------------------------------------------------------------
 
 struct Plan {

@@ -1003,6 +1003,79 @@ def ln_modulate_backward(dy, x2d, scale, tokens_per_batch, eps=1e-6):
     return dx, dscale, dshift
 
 
+# ---- the router's balance loss -----------------------------------------------------------------------------------
+
+def _balance_args(x2d, gate_w, topk_idx, sequences, mask, alpha, what):
+    dt = _act_dtype(x2d, what + " x")
+    _need_hip(x2d, what + " x")
+    dev = x2d.device
+    if x2d.dim() != 2 or gate_w.dim() != 2 or topk_idx.dim() != 2 or gate_w.shape[1] != x2d.shape[1] or topk_idx.shape[0] != x2d.shape[0]:
+        raise ValueError(f"{what}: expected x [T, D], gate weight [E, D] and topk_idx [T, k], got {tuple(x2d.shape)}, {tuple(gate_w.shape)} and "
+                         f"{tuple(topk_idx.shape)}")
+    T, D = x2d.shape
+    for name, t, dtype in (("gate weight", gate_w, dt), ("topk_idx", topk_idx, torch.int32), ("mask", mask, torch.bool)):
+        if t is None:
+            continue
+        if t.dtype != dtype:
+            raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+        if t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous on {dev}")
+    if mask is not None and mask.numel() != T:
+        raise ValueError(f"{what}: a mask of {mask.numel()} for {T} tokens")
+    if sequences < 1 or T % sequences != 0:
+        raise ValueError(f"{what}: {T} tokens in {sequences} sequences")
+    args = _lib.BalanceArgs()
+    args.dtype, args.T, args.sequences, args.D, args.E, args.k, args.alpha = _T_CODE[dt], T, sequences, D, gate_w.shape[0], topk_idx.shape[1], alpha
+    args.x, args.gate_w, args.topk_idx, args.mask = ptr(x2d), ptr(gate_w), ptr(topk_idx), ptr(mask)
+    return args
+
+
+def _balance_call(fn, args, x, backward):
+    nbytes = lib.hdmoe_gate_balance_workspace_bytes(ctypes.byref(args), backward)
+    if nbytes > 0:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    check(fn(ctypes.byref(args), _raw_stream(x)))
+
+
+def gate_balance(x2d, gate_w, topk_idx, alpha=0.01, sequences=1, mask=None):
+    """The router's auxiliary loss for x2d [T, D] (bf16 or fp16, D a multiple of 8), gate_w [E, D] (E up to 16) and the experts that gate_top2 (or any
+    other rule) chose, topk_idx int32 [T, k]: (loss, counts, scores) with scores = softmax(x W^T) fp32 [T, E], counts int32 [sequences, E] of the choices
+    in each sequence of T / sequences tokens (1: the whole batch, the reference's seq_aux off), and
+    loss = alpha * mean over sequences of sum_e (E counts / (k n)) * (mean score of e), an fp32 scalar. mask: bool, T values in any shape; tokens with
+    False are left out of counts, means and n, a sequence of nothing else out of the mean. Logits are fp32: gate_top2 rounds them to
+    the activations' type before it chooses. Choices outside 0 .. E - 1 are not counted."""
+    what = "gate_balance"
+    args = _balance_args(x2d, gate_w, topk_idx, sequences, mask, alpha, what)
+    with _on(x2d.device):
+        dev = x2d.device
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty((sequences, args.E), dtype=torch.int32, device=dev)
+        scores = torch.empty((args.T, args.E), dtype=torch.float32, device=dev)
+        args.loss, args.counts, args.scores = ptr(loss), ptr(counts), ptr(scores)
+        _balance_call(lib.hdmoe_gate_balance, args, x2d, 0)
+    return loss, counts, scores
+
+
+def gate_balance_backward(dloss, x2d, gate_w, topk_idx, counts, scores, alpha=0.01, mask=None, dweight=None):
+    """Gradients (dx, dgate_w) of gate_balance from dloss, an fp32 scalar on the device, and from dweight [T, k] of x's type, that of the
+    chosen scores scores[t, topk_idx[t, j]] (what gate_top2 returns beside the experts), if there is one. counts and scores are those
+    that gate_balance returned, which also say how many sequences there were; the other arguments are its own. Sums over tokens are fp32, in an order that
+    depends on the sizes alone."""
+    what = "gate_balance_backward"
+    args = _balance_args(x2d, gate_w, topk_idx, counts.shape[0] if counts.dim() == 2 else 0, mask, alpha, what)
+    dev = x2d.device
+    for name, t, dtype, shape in (("dloss", dloss, torch.float32, ()), ("counts", counts, torch.int32, (args.sequences, args.E)),
+                                  ("scores", scores, torch.float32, (args.T, args.E)), ("dweight", dweight, x2d.dtype, (args.T, args.k))):
+        if t is not None and (t.dtype != dtype or t.shape != shape or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be contiguous {dtype} {list(shape)} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    with _on(dev):
+        dx, dw = torch.empty_like(x2d), torch.empty_like(gate_w)
+        args.counts, args.scores, args.dloss, args.dweight, args.dx, args.dgate_w = ptr(counts), ptr(scores), ptr(dloss), ptr(dweight), ptr(dx), ptr(dw)
+        _balance_call(lib.hdmoe_gate_balance_backward, args, x2d, 1)
+    return dx, dw
+
+
 # ---- low-rank adapters of many requests --------------------------------------------------------------------------
 
 def _adapter_args(x, a, b, scale, index, what):

@@ -400,6 +400,39 @@ typedef struct hdmoe_norm_grad_args {
 size_t hdmoe_layer_norm_backward_workspace_bytes(int64_t rows, int D, int64_t rows_per_group);
 int hdmoe_layer_norm_backward(const hdmoe_norm_grad_args* args, hdmoe_stream_t stream);
 
+/* ---- the router's balance loss and its gradients ------------------------------- */
+
+/* What the reference's gates return for training (an auxiliary loss, comfy/ldm/hidream/model.py:242-283), from x [T, D] and gate_w [E, D] of
+ * dtype (bf16 or fp16, D a multiple of 8, E up to HDMOE_MAX_EXPERTS) and the chosen experts topk_idx [T, k] int32, k from 1 to HDMOE_MAX_EXPERTS:
+ *   scores [T, E] fp32 = softmax(x gate_w^T), logits and softmax in fp32
+ *   counts [sequences, E] int32: how often each expert is chosen by the tokens of a sequence, T / sequences in a row (1: the whole batch)
+ *   loss (one fp32) = alpha * mean over sequences of sum_e (E counts[s, e] / (k n_s)) * (sum_t scores[t, e] / n_s)
+ * mask [T] bytes or NULL: tokens with 0 are padding, left out of counts, sums, n_s and gradients whatever they hold; sequences without
+ * tokens are left out of the mean. A choice outside 0 .. E - 1 is not counted; one made twice counts twice.
+ *
+ * The gradients, from dloss (one fp32 on the device; counts carry none) and, unless NULL, dweight [T, k] of dtype, that of the chosen scores
+ * scores[t, topk_idx[t, j]]: dx [T, D] and dgate_w [E, D] of dtype. scores and counts are those of the forward call. Sums over tokens are
+ * fp32 in an order that depends on the sizes alone. Outputs may not overlap inputs; rows start on any address of their type. workspace:
+ * hdmoe_gate_balance_workspace_bytes (backward 0 or 1; it looks at mask for NULL), on 16 bytes, device. */
+typedef struct hdmoe_balance_args {
+  int dtype, T, sequences, D, E, k;
+  float alpha;
+  const void *x, *gate_w;
+  const int32_t* topk_idx;
+  const uint8_t* mask;
+  void* scores;              /* fp32; backward reads them and counts */
+  int32_t* counts;
+  float* loss;
+  const float* dloss;        /* hdmoe_gate_balance_backward */
+  const void* dweight;
+  void *dx, *dgate_w;
+  void* workspace;
+  size_t workspace_bytes;
+} hdmoe_balance_args;
+size_t hdmoe_gate_balance_workspace_bytes(const hdmoe_balance_args* args, int backward);
+int hdmoe_gate_balance(const hdmoe_balance_args* args, hdmoe_stream_t stream);
+int hdmoe_gate_balance_backward(const hdmoe_balance_args* args, hdmoe_stream_t stream);
+
 /* ---- low-rank adapters of many requests beside a shared projection ------------- */
 
 /* out[t] = base[t] + scale[i] * b[i] . (a[i] . x[t]) with i = index[t / (rows / requests)]; an index outside 0 .. n - 1 is no adapter, and its
