@@ -3,9 +3,13 @@
 //   out[t] = base[t] + s_a B_a (A_a x[t]),  a = index[t / rows_per] (outside 0 .. n - 1: none, out[t] = base[t])
 //   h = A x, g = dy B      dx = s g A      dA_a = s sum_t g[t]^T x[t]      dB_a = s sum_t dy[t]^T h[t]
 //
-// Three products with a narrow side, in as many kernels: `narrow` (rows to rank), `wide` (rank to rows) and `outer` (sums over rows). The
-// narrow results stay fp32 (lowrank.h says how they are multiplied). Rows of one tile may have different adapters: a tile is gone
-// through once for every adapter in it, and values of rows that have another one are never multiplied, not even by zero.
+// Three products with a narrow side, in as many kernels: `narrow` (rows to rank), `wide` (rank to rows) and `outer` (sums over rows). Rows of
+// one tile may have different adapters: a tile is gone through once for every adapter in it, and values of rows that have another one are
+// never multiplied, not even by zero.
+//
+// Narrow values go from one kernel to the next as fp32 parts where the contraction is cut over blocks (few rows), added up by the reader; else
+// scaled and split into bf16 hi and lo (lowrank.h) in the order in which the next product loads its operand: along the rank for `wide`, along the
+// rows for `outer`. Both then run without LDS and barriers.
 #include <type_traits>
 
 #include "lowrank.h"
@@ -14,9 +18,11 @@ using namespace lowrank;
 
 namespace {
 
-constexpr int WAVES = 4;
+constexpr int WAVES = 4;                   // of `wide`
+constexpr int NARROW_WAVES = 8;
 constexpr int K_STEP = 64;                 // along the contraction, of a wave: 128 bytes of each row
-constexpr int STAGE = 128;                 // tokens whose narrow values `outer` holds in LDS
+constexpr int RUN = 256;                   // tokens of a block of `wide_run`
+constexpr int STAGE = 128;                 // tokens that `outer` looks at the adapters of at a time
 
 struct Requests {
   const int32_t* index;
@@ -43,24 +49,56 @@ __device__ __forceinline__ void each_adapter(int mine, int z, int turns, F f) {
   }
 }
 
-// First of the eight r that lane `col` of a transposed operand holds: where they would pass R, the last eight once more (the same values
-// then come out in two places). Below 8: 0.
-__device__ __forceinline__ int across_r(int r0, int col, int R) { return max(0, min(r0 + col * 8, R - 8)); }
+// Where narrow values end up, split: planes of hi and lo.
+struct Planes {
+  uint16_t* rank;       // [2][T][stride_r]: along the rank, 0 from R to stride_r (R filled up to 8)
+  uint16_t* rows;       // [2][R][stride_t]: along the rows (T filled up to 32; what rows without an adapter or past T hold is not read)
+  int stride_r;
+  int64_t stride_t;
+};
+
+// Eight r from r0 on of row t, scaled, into the planes.
+__device__ __forceinline__ void put_planes(const Planes& to, int T, int R, int t, int r, const float (&v)[8]) {
+  u4 vh, vl;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t h, l;
+    split(v[2 * j], v[2 * j + 1], h, l);
+    vh[j] = h, vl[j] = l;
+  }
+  if (to.rank != nullptr) {
+    uint16_t* at = to.rank + (size_t)t * to.stride_r + r;
+    *reinterpret_cast<u4*>(at) = vh;
+    *reinterpret_cast<u4*>(at + (size_t)T * to.stride_r) = vl;
+  }
+  if (to.rows != nullptr) {
+    uint16_t* at = to.rows + (size_t)r * to.stride_t + t;
+    const size_t plane = (size_t)R * to.stride_t;
+#pragma unroll
+    for (int j = 0; j < 8; ++j, at += to.stride_t)
+      if (r + j < R) {
+        at[0] = (uint16_t)(vh[j / 2] >> (16 * (j & 1)));
+        at[plane] = (uint16_t)(vl[j / 2] >> (16 * (j & 1)));
+      }
+  }
+}
 
 struct NarrowArgs {
   Requests q;
   const uint16_t *x, *w;    // x [T, K]; w [n, R, K], or [n, K, R] (ACROSS)
-  float* part;              // [slices, T, R]
+  float* part;              // [slices, T, R] fp32, or NULL: to the planes (one slice)
+  Planes to;
   int K, R, slice, slices, turns;
 };
 
-// part[slice][t][r] = sum over the slice's k of x[t][k] w[a][r][k]. A tile is 16 TM tokens; the block's waves take steps of the slice in
-// turn and join their sums in LDS. ACROSS: w runs along r: eight k of eight r at a time, transposed in registers, 128 r of them (those past R are
-// not loaded) whatever R is.
+// sum over the slice's k of x[t][k] w[a][r][k]. A tile is 16 TM tokens; the block's waves take steps of the slice in turn, 1 KB of a row next to
+// each other, and join their sums in LDS. ACROSS: w runs along r: eight k of eight r at a time, transposed in registers, 128 r of them (those past
+// R are not loaded) whatever R is.
 template <class A, bool ACROSS, int RT, int TM>
-__global__ __launch_bounds__(WAVES * 64) void narrow_kernel(NarrowArgs p) {
+__global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p) {
   static_assert(!ACROSS || RT == 8, "128 r");
-  __shared__ f4 joined[2][RT * TM][64];
+  static_assert(RT * TM <= 16, "64 KB of LDS");
+  __shared__ f4 joined[4][RT * TM][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int tiles = (p.q.T + 16 * TM - 1) / (16 * TM);
   const int tile = blockIdx.x % tiles, slice = (blockIdx.x / tiles) % p.slices, z = blockIdx.x / tiles / p.slices;
@@ -97,14 +135,16 @@ __global__ __launch_bounds__(WAVES * 64) void narrow_kernel(NarrowArgs p) {
 #pragma unroll
             for (int m = 0; m < TM; ++m) acc[r][m] = A::mul(wv[r][i], xv[m][i], acc[r][m]);
       } else {
-        const int r = across_r(r0, col, p.R);
+        // r from R on: not stored (R a multiple of 8, the last eight are loaded again), or 0
+        const bool even = p.R % 8 == 0;
+        const int r = even ? min(r0 + col * 8, p.R - 8) : r0 + col * 8;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           u4 wv[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {   // past the end x is 0: the last row again
             const uint16_t* from = w + (size_t)(WHOLE ? k + 8 * i + j : min(k + 8 * i + j, p.K - 1)) * p.R + r;
-            wv[j] = p.R >= 8 ? load8(from) : load8(from, p.R);
+            wv[j] = even ? load8(from) : load8(from, p.R - r);
           }
           transpose8(wv);
 #pragma unroll
@@ -115,11 +155,11 @@ __global__ __launch_bounds__(WAVES * 64) void narrow_kernel(NarrowArgs p) {
       }
     };
     int k0 = lo + wave * K_STEP;
-    for (; k0 + K_STEP <= hi; k0 += WAVES * K_STEP) step(k0, std::true_type());
+    for (; k0 + K_STEP <= hi; k0 += NARROW_WAVES * K_STEP) step(k0, std::true_type());
     if (k0 < hi) step(k0, std::false_type());
-    // waves 2 and 3 into 0 and 1, 1 into 0
+    // the upper half of the waves into the lower one, and so on
 #pragma unroll
-    for (int half = 2; half > 0; half >>= 1) {
+    for (int half = NARROW_WAVES / 2; half > 0; half >>= 1) {
       __syncthreads();
       if (wave >= half && wave < 2 * half)
 #pragma unroll
@@ -127,58 +167,179 @@ __global__ __launch_bounds__(WAVES * 64) void narrow_kernel(NarrowArgs p) {
       __syncthreads();
       if (wave < half)
 #pragma unroll
-        for (int i = 0; i < RT * TM; ++i) acc[i / TM][i % TM] += joined[wave][i][lane];
-    }
-    if (wave != 0) return;
-#pragma unroll
-    for (int m = 0; m < TM; ++m) {
-      if (!((has >> (m * 16 + col)) & 1)) continue;
-      float* to = p.part + ((size_t)slice * p.q.T + t0 + m * 16 + col) * p.R;
-#pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = ACROSS ? across_r(r0, quad * 4 + e, p.R) + i : r0 + i * 16 + quad * 4 + e;
-          if (r < p.R) to[r] = acc[i][m][e];
+        for (int i = 0; i < RT * TM; ++i) {
+          acc[i / TM][i % TM] += joined[wave][i][lane];
+          if (half == 1) joined[0][i][lane] = acc[i / TM][i % TM];
         }
+    }
+    __syncthreads();
+    const float scale = p.part != nullptr ? 1.0f : p.q.scale[a];
+    for (int u = threadIdx.x; u < 16 * TM * RT * 2; u += NARROW_WAVES * 64) {   // eight r of a token
+      const int m = u / 16 % TM, eight = u / (16 * TM), bit = u % (16 * TM), r = r0 + eight * 8, t = t0 + bit;
+      if (r >= p.R || !((has >> bit) & 1)) continue;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // ACROSS: instruction j, row `eight`
+        const int row = ACROSS ? eight : (eight & 1) * 8 + j, tile_r = ACROSS ? j : eight >> 1;
+        v[j] = r + j < p.R ? joined[0][tile_r * TM + m][(row >> 2) * 16 + (bit & 15)][row & 3] * scale : 0.0f;
+      }
+      if (p.part == nullptr) {
+        put_planes(p.to, p.q.T, p.R, t, r, v);
+        continue;
+      }
+      float* to = p.part + ((size_t)slice * p.q.T + t) * p.R + r;
+      if (r + 8 <= p.R) __builtin_memcpy(to, v, 32);
+      else
+        for (int j = 0; j < 8; ++j)
+          if (r + j < p.R) to[j] = v[j];
     }
   });
 }
 
+// Parts to planes: sums of the slices, scaled and split. Eight r of a row a thread.
+struct JoinArgs {
+  Requests q;
+  const float* part[2];     // h, g; NULL: planes are there
+  Planes to[2];
+  int slices[2], R;
+};
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs p) {
+  const int side = blockIdx.y;
+  if (p.part[side] == nullptr) return;
+  const int eights = (p.R + 7) / 8;
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int t = (int)(u % p.q.T), r = (int)(u / p.q.T) * 8;
+  if (r >= eights * 8) return;
+  const int a = p.q.of(t);
+  if (a < 0) return;
+  float v[8] = {};
+  for (int s = 0; s < p.slices[side]; ++s) {
+    const float* from = p.part[side] + ((size_t)s * p.q.T + t) * p.R + r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (r + j < p.R) v[j] += from[j];
+  }
+  const float f = p.q.scale[a];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] *= f;
+  put_planes(p.to[side], p.q.T, p.R, t, r, v);
+}
+
 struct WideArgs {
   Requests q;
-  const float* part;                  // [slices, T, R]
+  const float* part;                  // [slices, T, R] (wide_kernel)
+  Planes from;                        // (wide_run_kernel)
   const uint16_t *w, *base;           // w [n, C, R], or [n, R, C] (ACROSS); base [T, C] or NULL
   uint16_t* out;                      // [T, C]
   int C, R, slices, turns;
 };
 
-// out[t][c] = base[t][c] + s sum_r h[t][r] w[a][c][r]. A tile is 16 TM tokens; a wave has 64 columns (ACROSS: 128), which a lane holds 16 (32) next to each
-// other of, so that it loads and stores whole 16-byte pieces and a token's 128 bytes are one wave's.
-// Bound by base and out: R of 64 takes 16 matrix instructions (256 cycles of one of four units) for 4 KB of them.
-template <class A, bool ACROSS, int TM>
+// out[t][c] = base[t][c] + s sum_r h[t][r] w[a][c][r]. A wave has 64 columns (ACROSS: 128), a lane 16 (32) of them next to each other, so that it
+// loads and stores whole 16-byte pieces and a token's 128 (256) bytes are one wave's.
+template <class A, bool ACROSS>
+struct Wide {
+  static constexpr int NT = ACROSS ? 8 : 4;    // instructions side by side
+  static constexpr int COLS = NT * 16;
+  const WideArgs& p;
+  int c0, col, quad, c, have;
+  bool whole;
+  __device__ __forceinline__ Wide(const WideArgs& args, int first, int lane) : p(args), c0(first), col(lane & 15), quad(lane >> 4) {
+    c = c0 + quad * 4 * NT;
+    have = p.C - c;
+    whole = c0 + COLS <= p.C;
+  }
+  // Weights of 32 r from r0 on, in bf16. r past R meets values of 0: the row's last ones again, so that nothing but the lane's own column enters.
+  __device__ __forceinline__ void weights(int a, int r0, u4 (&wh)[NT], u4 (&wl)[NT]) const {
+    const uint16_t* w = p.w + (size_t)a * p.R * p.C;
+    const int r = r0 + quad * 8;
+    if constexpr (ACROSS) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint16_t* from = w + (size_t)min(r + j, p.R - 1) * p.C + c0 + col * 8;
+        wh[j] = whole ? load8(from) : load8(from, p.C - c0 - col * 8);
+      }
+      transpose8(wh);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const uint16_t* from = w + (size_t)min(c0 + (col >> 2) * 16 + j * 4 + (col & 3), p.C - 1) * p.R;
+        wh[j] = p.R % 8 == 0 ? load8(from + min(r, p.R - 8)) : load8(from + r, p.R - r);
+      }
+    }
+    if constexpr (A::HALF)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) to_bf16<A>(wh[j], wh[j], wl[j]);
+  }
+  __device__ __forceinline__ void base(int t, bool want, u4 (&b)[NT / 2]) const {
+    const uint16_t* from = p.base + (size_t)t * p.C + c;
+#pragma unroll
+    for (int i = 0; i < NT / 2; ++i) {
+      b[i] = u4{0, 0, 0, 0};
+      if (want && p.base != nullptr) b[i] = whole ? load8(from + 8 * i) : load8(from + 8 * i, have - 8 * i);
+    }
+  }
+  __device__ __forceinline__ void put(int t, const f4 (&acc)[NT], const u4 (&b)[NT / 2]) const {
+    uint16_t* to = p.out + (size_t)t * p.C + c;
+#pragma unroll
+    for (int i = 0; i < NT / 2; ++i) {
+      u4 o;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        // ACROSS: instruction j, element e are column 8 e + j, else 4 j + e
+        const int u = 8 * i + 2 * w;
+        const float v0 = ACROSS ? acc[u % 8][u / 8] : acc[u / 4][u % 4], v1 = ACROSS ? acc[u % 8 + 1][u / 8] : acc[u / 4][u % 4 + 1];
+        o[w] = p.base != nullptr ? A::pack(v0 + A::lo(b[i][w]), v1 + A::hi(b[i][w])) : A::pack(v0, v1);
+      }
+      if (whole) __builtin_memcpy(to + 8 * i, &o, 16);
+      else store8(to + 8 * i, o, have - 8 * i);
+    }
+  }
+  // a row without an adapter: the base as it is, bit for bit
+  __device__ __forceinline__ void copy(int t) const {
+    if ((const void*)p.out == (const void*)p.base) return;
+#pragma unroll
+    for (int i = 0; i < NT / 2; ++i) {
+      u4 v = {0, 0, 0, 0};
+      if (p.base != nullptr) v = load8(p.base + (size_t)t * p.C + c + 8 * i, have - 8 * i);
+      store8(p.out + (size_t)t * p.C + c + 8 * i, v, have - 8 * i);
+    }
+  }
+};
+
+// Few rows: 16 tokens a tile, their narrow values added up from the parts and split in LDS; a tile's adapters are dealt to `turns` blocks.
+template <class A, bool ACROSS>
 __global__ __launch_bounds__(WAVES * 64) void wide_kernel(WideArgs p) {
-  constexpr int NT = ACROSS ? 8 : 4;           // instructions side by side
-  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];   // [2][16 TM][stride]: hi, lo of s h
+  typedef Wide<A, ACROSS> W;
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];   // [2][16][stride]: hi, lo of s h
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int steps = (p.R + 31) / 32, stride = steps * 32 + 8;
-  const int tiles = (p.q.T + 16 * TM - 1) / (16 * TM), chunks = (p.C + WAVES * NT * 16 - 1) / (WAVES * NT * 16);
+  const int tiles = (p.q.T + 15) / 16, chunks = (p.C + WAVES * W::COLS - 1) / (WAVES * W::COLS);
   const int chunk = blockIdx.x % chunks, tile = (blockIdx.x / chunks) % tiles, z = blockIdx.x / chunks / tiles;
-  const int t0 = tile * 16 * TM, c0 = (chunk * WAVES + wave) * NT * 16;
-  const int mine = lane < 16 * TM ? p.q.of(t0 + lane) : -1;
-  // the narrow values of the tile, eight a thread at a time
-  for (int u = threadIdx.x; u < 16 * TM * steps * 4; u += WAVES * 64) {
+  const int t0 = tile * 16;
+  const int mine = lane < 16 ? p.q.of(t0 + lane) : -1;
+  for (int u = threadIdx.x; u < 16 * steps * 4; u += WAVES * 64) {   // eight values a thread
     const int row = u / (steps * 4), r = (u - row * (steps * 4)) * 8, t = t0 + row;
     const int a = p.q.of(t);
     float v[8] = {};
     if (a >= 0) {
-      for (int s = 0; s < p.slices; ++s) {
-        const float* from = p.part + ((size_t)s * p.q.T + t) * p.R + r;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (r + j < p.R) v[j] += from[j];
-      }
       const float f = p.q.scale[a];
+      const float* from = p.part + (size_t)t * p.R + r;
+      const size_t next = (size_t)p.q.T * p.R;
+      if (r + 8 <= p.R) {
+#pragma unroll 8
+        for (int s = 0; s < p.slices; ++s) {
+          f4 q[2];
+          __builtin_memcpy(q, from + s * next, 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] += q[j / 4][j % 4];
+        }
+      } else {
+        for (int s = 0; s < p.slices; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (r + j < p.R) v[j] += from[s * next + j];
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= f;
     }
@@ -190,251 +351,322 @@ __global__ __launch_bounds__(WAVES * 64) void wide_kernel(WideArgs p) {
       vh[j] = h, vl[j] = l;
     }
     *reinterpret_cast<u4*>(lds + (size_t)row * stride + r) = vh;
-    *reinterpret_cast<u4*>(lds + (size_t)(16 * TM + row) * stride + r) = vl;
+    *reinterpret_cast<u4*>(lds + (size_t)(16 + row) * stride + r) = vl;
   }
   __syncthreads();
-  if (c0 >= p.C) return;
-  // the lane's columns: 4 NT next to each other
-  const int c = c0 + quad * 4 * NT, have = p.C - c;
-  const bool whole = c0 + 16 * NT <= p.C;
-  auto put = [&](int m, f4 (&acc)[NT], u4 (&b)[NT / 2]) {
-    uint16_t* to = p.out + (size_t)(t0 + m * 16 + col) * p.C + c;
-#pragma unroll
-    for (int i = 0; i < NT / 2; ++i) {
-      u4 o;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        // ACROSS: instruction j, element e are column 8 e + j, else 4 j + e
-        const int u = 8 * i + 2 * w;
-        const float v0 = ACROSS ? acc[u % 8][u / 8] : acc[u / 4][u % 4], v1 = ACROSS ? acc[u % 8 + 1][u / 8] : acc[u / 4][u % 4 + 1];
-        o[w] = p.base != nullptr ? A::pack(v0 + A::lo(b[i][w]), v1 + A::hi(b[i][w])) : A::pack(v0, v1);
-      }
-      store8(to + 8 * i, o, have - 8 * i);
-    }
-  };
-  auto bases = [&](int m, u4 (&b)[NT / 2], bool want) {
-    const uint16_t* from = p.base + (size_t)(t0 + m * 16 + col) * p.C + c;
-#pragma unroll
-    for (int i = 0; i < NT / 2; ++i) b[i] = want && p.base != nullptr ? load8(from + 8 * i, have - 8 * i) : u4{0, 0, 0, 0};
-  };
-  if (z == 0) {   // rows without an adapter
-    const uint64_t none = __ballot(lane < 16 * TM && t0 + lane < p.q.T && mine < 0);
-    if (none != 0 && (const void*)p.out != (const void*)p.base)
-#pragma unroll
-      for (int m = 0; m < TM; ++m)
-        if ((none >> (m * 16 + col)) & 1) {
-          f4 zero[NT] = {};
-          u4 b[NT / 2];
-          const uint16_t* from = p.base + (size_t)(t0 + m * 16 + col) * p.C + c;
-          if (p.base == nullptr) {
-            put(m, zero, b);
-          } else {   // as it is, bit for bit
-#pragma unroll
-            for (int i = 0; i < NT / 2; ++i)
-              store8(p.out + (size_t)(t0 + m * 16 + col) * p.C + c + 8 * i, load8(from + 8 * i, have - 8 * i), have - 8 * i);
-          }
-        }
-  }
-  each_adapter(mine, z, p.turns, [&](int a, uint64_t has) {
-    u4 b[TM][NT / 2];
-#pragma unroll
-    for (int m = 0; m < TM; ++m) bases(m, b[m], (has >> (m * 16 + col)) & 1);
-    f4 acc[TM][NT] = {};
-    const uint16_t* w = p.w + (size_t)a * p.R * p.C;
+  const W w(p, (chunk * WAVES + wave) * W::COLS, lane);
+  if (w.c0 >= p.C) return;
+  const int own = __shfl(mine, col, 64);
+  if (z == 0 && own < 0 && t0 + col < p.q.T) w.copy(t0 + col);
+  each_adapter(mine, z, p.turns, [&](int a, uint64_t) {
+    u4 b[W::NT / 2];
+    w.base(t0 + col, own == a, b);
+    f4 acc[W::NT] = {};
     for (int s = 0; s < steps; ++s) {
-      const int r = s * 32 + quad * 8;
-      u4 wh[NT], wl[NT];
-      // r past R meets h of 0: the row's last values again, so that nothing but the lane's own column enters
-      if constexpr (ACROSS) {
+      u4 wh[W::NT], wl[W::NT];
+      w.weights(a, s * 32, wh, wl);
+      const u4 qh = *reinterpret_cast<const u4*>(lds + (size_t)col * stride + s * 32 + quad * 8);
+      const u4 ql = *reinterpret_cast<const u4*>(lds + (size_t)(16 + col) * stride + s * 32 + quad * 8);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint16_t* from = w + (size_t)min(r + j, p.R - 1) * p.C + c0 + col * 8;
-          wh[j] = whole ? load8(from) : load8(from, p.C - c0 - col * 8);
-        }
-        transpose8(wh);
-      } else {
+      for (int j = 0; j < W::NT; ++j) acc[j] = mul_split<A>(wh[j], wl[j], qh, ql, acc[j]);
+    }
+    if (own == a) w.put(t0 + col, acc, b);
+  });
+}
+
+// Many rows: a block has RUN tokens, 16 at a time; a wave keeps the weights of its columns in registers for as long as the adapter stays the same (R up to
+// 32 STEPS; `parts` times that are gone through one after the other, loaded anew). Values and base of the next 16 tokens are on their way
+// while these are multiplied. Bound by base and out: R of 64 takes 16 instructions (256 cycles of one of four units) for 4 KB of them.
+template <class A, bool ACROSS, int STEPS>
+__global__ __launch_bounds__(WAVES * 64) void wide_run_kernel(WideArgs p, int parts) {
+  typedef Wide<A, ACROSS> W;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+  const int chunks = (p.C + WAVES * W::COLS - 1) / (WAVES * W::COLS);
+  const int chunk = blockIdx.x % chunks, t0 = blockIdx.x / chunks * RUN;
+  const W w(p, (chunk * WAVES + wave) * W::COLS, lane);
+  if (w.c0 >= p.C) return;
+  int of[RUN / 64];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const uint16_t* from = w + (size_t)min(c0 + (col >> 2) * 16 + j * 4 + (col & 3), p.C - 1) * p.R;
-          wh[j] = p.R % 8 == 0 ? load8(from + min(r, p.R - 8)) : load8(from + r, p.R - r);
-        }
-      }
-      if constexpr (A::HALF)
+  for (int i = 0; i < RUN / 64; ++i) of[i] = p.q.of(t0 + i * 64 + lane);
+  const int groups = min(RUN, p.q.T - t0 + 15) / 16;
+  const size_t plane = (size_t)p.q.T * p.from.stride_r;
+  struct Tokens {
+    u4 q[2][STEPS], b[W::NT / 2];
+  };
+  auto values = [&](int g, int part, u4 (&q)[2][STEPS]) {
+    const uint16_t* from = p.from.rank + (size_t)min(t0 + g * 16 + col, p.q.T - 1) * p.from.stride_r;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) to_bf16<A>(wh[j], wh[j], wl[j]);
-#pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        const u4 qh = *reinterpret_cast<const u4*>(lds + (size_t)(m * 16 + col) * stride + r);
-        const u4 ql = *reinterpret_cast<const u4*>(lds + (size_t)((TM + m) * 16 + col) * stride + r);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[m][j] = mul_split<A>(wh[j], wl[j], qh, ql, acc[m][j]);
+    for (int s = 0; s < STEPS; ++s) {
+      const int r = (part * STEPS + s) * 32 + quad * 8;
+      q[0][s] = q[1][s] = u4{0, 0, 0, 0};
+      if (r < p.from.stride_r) {
+        q[0][s] = *reinterpret_cast<const u4*>(from + r);
+        q[1][s] = *reinterpret_cast<const u4*>(from + plane + r);
       }
     }
+  };
+  auto load = [&](int g, Tokens& k) {
+    values(g, 0, k.q);
+    w.base(t0 + g * 16 + col, t0 + g * 16 + col < p.q.T, k.b);
+  };
+  u4 wh[STEPS][W::NT], wl[STEPS][W::NT];
+  int held = -1;
+  auto compute = [&](int g, Tokens& k) {
+    int mine = 0;
 #pragma unroll
-    for (int m = 0; m < TM; ++m)
-      if ((has >> (m * 16 + col)) & 1) put(m, acc[m], b[m]);
-  });
+    for (int i = 0; i < RUN / 64; ++i)
+      if (g / 4 == i) mine = of[i];
+    mine = __shfl(mine, (g & 3) * 16 + col, 64);
+    const int t = t0 + g * 16 + col;
+    if (mine < 0 && t < p.q.T) w.copy(t);
+    each_adapter(mine, 0, 1, [&](int a, uint64_t) {
+      f4 acc[W::NT] = {};
+      for (int part = 0; part < parts; ++part) {
+        if (a != held || parts > 1) {
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) w.weights(a, (part * STEPS + s) * 32, wh[s], wl[s]);
+          held = a;
+        }
+        if (parts > 1) values(g, part, k.q);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+          for (int j = 0; j < W::NT; ++j) acc[j] = mul_split<A>(wh[s][j], wl[s][j], k.q[0][s], k.q[1][s], acc[j]);
+      }
+      if (mine == a) w.put(t, acc, k.b);
+    });
+  };
+  Tokens k[2];
+  load(0, k[0]);
+  for (int g = 0; g < groups; g += 2) {
+    if (g + 1 < groups) load(g + 1, k[1]);
+    compute(g, k[0]);
+    if (g + 2 < groups) load(g + 2, k[0]);
+    if (g + 1 < groups) compute(g + 1, k[1]);
+  }
 }
 
 struct OuterSide {
   const uint16_t* v;        // [T, C]
-  const float* part;        // [slices, T, R]
+  const uint16_t* rows;     // narrow values along the rows, hi; lo behind
   void* out;                // fp32 parts [splits, n, R, C] (flip: [splits, n, C, R]), or the result itself
-  int C, slices, flip, blocks;   // blocks of 512 columns
+  int C, flip, blocks;      // blocks of 512 columns
 };
 
 struct OuterArgs {
   Requests q;
   OuterSide side[2];
-  int R, splits, per_split, direct;   // per_split: tokens, a multiple of STAGE
+  int64_t stride_t;
+  int R, splits, per_split, direct;   // per_split: tokens, a multiple of 2 STAGE
 };
 
-// out[a][r][c] = s sum over the rows t of adapter a of q[t][r] v[t][c], 16 RT of the r. A wave has 128 columns; eight rows of eight columns
-// a lane are loaded as they lie and transposed in registers.
+// out[a][r][c] = s sum over the rows t of adapter a of q[t][r] v[t][c], 16 RT of the r. A wave has 128 columns and one half of the block's rows: eight rows of
+// eight columns a lane are loaded as they lie and transposed in registers; the halves are joined in LDS.
 template <class A, int RT>
-__global__ __launch_bounds__(WAVES * 64, 2) void outer_kernel(OuterArgs p) {
-  __shared__ uint16_t lds[2][16 * RT][STAGE + 8];
+__global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
+  static_assert(RT <= 2, "64 KB of LDS; four r tiles do not fit the registers beside the rows to come either");
+  __shared__ f4 joined[4][8 * RT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const bool second = (int)blockIdx.x >= p.side[0].blocks;
   const OuterSide side = second ? p.side[1] : p.side[0];
   const int block = second ? blockIdx.x - p.side[0].blocks : blockIdx.x;
   const int a = blockIdx.y % p.q.n, r0 = blockIdx.y / p.q.n * 16 * RT, split = blockIdx.z;
-  const int c0 = (block * WAVES + wave) * 128, c = c0 + col * 8, have = side.C - c;
-  const float f = p.q.scale[a];
+  const int c0 = (block * 4 + (wave & 3)) * 128, c = c0 + col * 8, have = side.C - c;
   const bool whole = c0 + 128 <= side.C;
   f4 acc[RT][8] = {};
-  const int end = (int)min((int64_t)p.q.T, (int64_t)(split + 1) * p.per_split);
-  for (int t0 = split * p.per_split; t0 < end; t0 += STAGE) {
-    const uint64_t first = __ballot(t0 + lane < end && p.q.of(t0 + lane) == a), next = __ballot(t0 + 64 + lane < end && p.q.of(t0 + 64 + lane) == a);
-    if ((first | next) == 0) continue;
-    __syncthreads();
-    for (int u = threadIdx.x; u < STAGE * 4 * RT; u += WAVES * 64) {   // two rows of one r .. + 3 a thread, transposed
-      const int row = u % (STAGE / 2) * 2, r = u / (STAGE / 2) * 2;
-      float v[2][2] = {};
+  const int64_t begin = (int64_t)split * p.per_split + (wave >> 2) * (p.per_split / 2);
+  const int end = (int)min((int64_t)p.q.T, begin + p.per_split / 2);
+  const uint16_t* q[RT];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (!(((row + i < 64 ? first : next) >> ((row + i) & 63)) & 1)) continue;
-        for (int s = 0; s < side.slices; ++s) {
-          const float* from = side.part + ((size_t)s * p.q.T + t0 + row + i) * p.R + r0 + r;
+  for (int r = 0; r < RT; ++r) q[r] = side.rows + (size_t)min(r0 + r * 16 + col, p.R - 1) * p.stride_t + quad * 8;
+  const size_t plane = (size_t)p.R * p.stride_t;
+  if (c0 < side.C)
+    for (int t0 = (int)min(begin, (int64_t)p.q.T); t0 < end; t0 += STAGE) {
+      const uint64_t first = __ballot(t0 + lane < end && p.q.of(t0 + lane) == a), next = __ballot(t0 + 64 + lane < end && p.q.of(t0 + 64 + lane) == a);
+      if ((first | next) == 0) continue;
+      const bool all = whole && (first & next) == ~0ull;
+      auto multiply = [&](u4 (&v)[8], u4 (&qh)[RT], u4 (&ql)[RT]) {
+        transpose8(v);
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if (r0 + r + j < p.R) v[i][j] += from[j];
+        for (int j = 0; j < 8; ++j) {
+          u4 vh, vl;
+          to_bf16<A>(v[j], vh, vl);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            acc[r][j] = Bf16::mul(ql[r], vh, acc[r][j]);
+            if constexpr (A::HALF) acc[r][j] = Bf16::mul(qh[r], vl, acc[r][j]);
+            acc[r][j] = Bf16::mul(qh[r], vh, acc[r][j]);
+          }
         }
-      }
+      };
+      const uint16_t* from = side.v + (size_t)(t0 + quad * 8) * side.C + c;
+      if (all) {
+        u4 v[2][8];
+        auto load = [&](int st, u4 (&x)[8]) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t h, l;
-        lowrank::split(v[0][j] * f, v[1][j] * f, h, l);
-        *reinterpret_cast<uint32_t*>(&lds[0][r + j][row]) = h;
-        *reinterpret_cast<uint32_t*>(&lds[1][r + j][row]) = l;
-      }
-    }
-    __syncthreads();
-    if (c0 >= side.C) continue;
-#pragma unroll 2
-    for (int st = 0; st < STAGE / 32; ++st) {
-      const uint32_t has = (uint32_t)((st < 2 ? first : next) >> (32 * (st & 1)));
-      if (has == 0) continue;
-      const uint32_t eight = (has >> (quad * 8)) & 0xff;
-      u4 v[8];
-      const uint16_t* from = side.v + (size_t)(t0 + st * 32 + quad * 8) * side.C + c;
-      if (has == 0xffffffffu && whole) {
+          for (int j = 0; j < 8; ++j) x[j] = load8(from + (size_t)(st * 32 + j) * side.C);
+        };
+        load(0, v[0]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = load8(from + (size_t)j * side.C);
-      } else {   // rows of another adapter are 0, not multiplied by it
+        for (int st = 0; st < STAGE / 32; ++st) {
+          u4 qh[RT], ql[RT];
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            qh[r] = *reinterpret_cast<const u4*>(q[r] + t0 + st * 32);
+            ql[r] = *reinterpret_cast<const u4*>(q[r] + plane + t0 + st * 32);
+          }
+          if (st + 1 < STAGE / 32) load(st + 1, v[(st + 1) & 1]);
+          multiply(v[st & 1], qh, ql);
+        }
+        continue;
+      }
+      for (int st = 0; st < STAGE / 32; ++st) {
+        const uint32_t has = (uint32_t)((st < 2 ? first : next) >> (32 * (st & 1)));
+        if (has == 0) continue;
+        const uint32_t eight = (has >> (quad * 8)) & 0xff;
+        // rows of another adapter, or past the last one, are 0 on both sides
+        u4 v[8], qh[RT], ql[RT], keep;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) keep[j] = ((eight >> (2 * j)) & 1 ? 0xffffu : 0u) | ((eight >> (2 * j + 1)) & 1 ? 0xffff0000u : 0u);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           v[j] = u4{0, 0, 0, 0};
-          if ((eight >> j) & 1) v[j] = load8(from + (size_t)j * side.C, have);
+          if ((eight >> j) & 1) v[j] = load8(from + (size_t)(st * 32 + j) * side.C, have);
         }
-      }
-      transpose8(v);
-      u4 qh[RT], ql[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        qh[r] = *reinterpret_cast<const u4*>(&lds[0][r * 16 + col][st * 32 + quad * 8]);
-        ql[r] = *reinterpret_cast<const u4*>(&lds[1][r * 16 + col][st * 32 + quad * 8]);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        u4 vh, vl;
-        to_bf16<A>(v[j], vh, vl);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          acc[r][j] = Bf16::mul(ql[r], vh, acc[r][j]);
-          if constexpr (A::HALF) acc[r][j] = Bf16::mul(qh[r], vl, acc[r][j]);
-          acc[r][j] = Bf16::mul(qh[r], vh, acc[r][j]);
+          qh[r] = *reinterpret_cast<const u4*>(q[r] + t0 + st * 32) & keep;
+          ql[r] = *reinterpret_cast<const u4*>(q[r] + plane + t0 + st * 32) & keep;
+        }
+        multiply(v, qh, ql);
+      }
+    }
+  if (wave >= 4)
+#pragma unroll
+    for (int i = 0; i < 8 * RT; ++i) joined[wave - 4][i][lane] = acc[i / 8][i % 8];
+  __syncthreads();
+  if (wave >= 4 || c0 >= side.C) return;
+#pragma unroll
+  for (int i = 0; i < 8 * RT; ++i) acc[i / 8][i % 8] += joined[wave][i][lane];
+  const size_t at = ((size_t)split * p.q.n + a) * p.R * side.C;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = r0 + r * 16 + quad * 4;
+    if (side.flip) {        // a column's four r next to each other
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j >= have || row >= p.R) continue;
+        const size_t i = at + (size_t)(c + j) * p.R + row;
+        if (p.direct) {
+          uint16_t* to = static_cast<uint16_t*>(side.out) + i;
+          const uint32_t o[2] = {A::pack(acc[r][j][0], acc[r][j][1]), A::pack(acc[r][j][2], acc[r][j][3])};
+          if (row + 4 <= p.R) __builtin_memcpy(to, o, 8);
+          else
+            for (int e = 0; e < 4; ++e)
+              if (row + e < p.R) to[e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
+        } else {
+          float* to = static_cast<float*>(side.out) + i;
+          if (row + 4 <= p.R) __builtin_memcpy(to, &acc[r][j], 16);
+          else
+            for (int e = 0; e < 4; ++e)
+              if (row + e < p.R) to[e] = acc[r][j][e];
+        }
+      }
+    } else {                // a row's eight columns
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (row + e >= p.R || have <= 0) continue;
+        const size_t i = at + (size_t)(row + e) * side.C + c;
+        if (p.direct) {
+          u4 o;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[k] = A::pack(acc[r][2 * k][e], acc[r][2 * k + 1][e]);
+          store8(static_cast<uint16_t*>(side.out) + i, o, have);
+        } else {
+          float* to = static_cast<float*>(side.out) + i;
+          if (have >= 8) {
+            const f4 o[2] = {{acc[r][0][e], acc[r][1][e], acc[r][2][e], acc[r][3][e]}, {acc[r][4][e], acc[r][5][e], acc[r][6][e], acc[r][7][e]}};
+            __builtin_memcpy(to, o, 32);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (j < have) to[j] = acc[r][j][e];
+          }
         }
       }
     }
   }
-  if (c0 >= side.C) return;
-  const size_t at = ((size_t)split * p.q.n + a) * p.R * side.C;
-  auto put = [&](size_t i, float v) {
-    if (p.direct) static_cast<uint16_t*>(side.out)[at + i] = (uint16_t)A::pack(v, 0.0f);
-    else static_cast<float*>(side.out)[at + i] = v;
-  };
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = r0 + r * 16 + quad * 4 + e;
-      if (row >= p.R) continue;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < have) put(side.flip ? (size_t)(c + j) * p.R + row : (size_t)row * side.C + c + j, acc[r][j][e]);
-    }
 }
 
 // ---- sizes ---------------------------------------------------------------------------------------------------------
 
+struct Side {                 // a narrow product
+  int slices, slice;
+  size_t part, rank, rows;    // bytes of its parts and planes in the workspace
+};
+
 struct Plan {
-  int tm_narrow, slices_x, slice_x, slices_y, slice_y, turns, tm_wide, turns_wide, splits, per_split, rt;
-  size_t h_bytes, g_bytes, da_bytes, db_bytes;
+  int tm, turns, run;         // run: many rows
+  Side h, g;
+  int stride_r, splits, per_split, rt;
+  int64_t stride_t;
+  size_t da_bytes, db_bytes, total;
 };
 
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// Tokens a tile: 16 where rows of a tile have different adapters or where there are few; the contraction is cut until the card has about two
-// blocks a CU, in slices of at least one step of each wave.
-void narrow_plan(int tiles, int turns, int K, int rblocks, int& slices, int& slice) {
-  const int most = div_up(K, WAVES * K_STEP);
-  int want = div_up(2 * HDMOE_NUM_CU, (int64_t)tiles * turns * rblocks);
+size_t bytes_of(size_t n) { return hdmoe_align_up(n, 256); }
+
+constexpr int MANY_ROWS = 512;   // from here on `wide` keeps its weights over runs of tokens
+
+// The contraction is cut over blocks until the card has about one a CU, in slices of at least two steps of each wave; with `run` not at all.
+void cut(int tiles, int turns, int K, int rblocks, bool whole, Side& s) {
+  const int most = div_up(K, 2 * NARROW_WAVES * K_STEP);
+  int want = whole ? 1 : div_up(HDMOE_NUM_CU, (int64_t)tiles * turns * rblocks);
   if (want > most) want = most;
-  if (want > 16) want = 16;
-  slice = div_up(most, want) * WAVES * K_STEP;
-  slices = div_up(K, slice);
+  if (want > 8) want = 8;
+  s.slice = div_up(div_up(K, want), NARROW_WAVES * K_STEP) * NARROW_WAVES * K_STEP;
+  s.slices = div_up(K, s.slice);
 }
 
 Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   Plan p = {};
   const int rows_per = a.rows / a.requests;
-  const bool mixed = rows_per < 64;
-  p.tm_narrow = mixed || a.rows <= 512 ? 1 : a.R > 64 ? 2 : 4;
-  const int tile = 16 * p.tm_narrow;
-  const int distinct = rows_per >= tile ? 1 : div_up(tile, rows_per);
+  p.run = a.rows >= MANY_ROWS;
+  // tokens of a tile of `narrow`: 16, and more where there are tiles for every CU all the same and a tile's rows share an adapter
+  p.tm = rows_per < 64 || a.rows < 32 * HDMOE_NUM_CU ? 1 : a.rows < 64 * HDMOE_NUM_CU || a.R > 64 ? 2 : 4;
+  const int tile = 16 * p.tm, distinct = div_up(tile, rows_per);
   p.turns = distinct < a.n ? distinct : a.n;
-  if (p.turns > tile) p.turns = tile;
-  const int tiles = div_up(a.rows, tile), rblocks = a.R > 128 ? 2 : 1;
-  narrow_plan(tiles, p.turns, a.K, rblocks, p.slices_x, p.slice_x);
-  narrow_plan(tiles, p.turns, a.N, rblocks, p.slices_y, p.slice_y);
-  p.tm_wide = mixed || a.rows <= 256 ? 1 : a.R > 128 ? 2 : 4;
-  p.turns_wide = p.tm_wide == 1 ? p.turns : 1;
-  p.h_bytes = hdmoe_align_up((size_t)p.slices_x * a.rows * a.R * sizeof(float), 256);
-  if (!backward) return p;
-  p.g_bytes = hdmoe_align_up((size_t)p.slices_y * a.rows * a.R * sizeof(float), 256);
-  p.rt = a.R <= 16 ? 1 : a.R <= 32 ? 2 : 4;
-  const int blocks = (div_up(a.K, WAVES * 128) + div_up(a.N, WAVES * 128)) * a.n * div_up(a.R, 16 * p.rt);
-  int splits = div_up(2 * HDMOE_NUM_CU, blocks);
-  const int most = div_up(a.rows, 2 * STAGE);
+  const int tiles = div_up(a.rows, tile);
+  cut(tiles, p.turns, a.K, div_up(a.R, 128), p.run, p.h);
+  p.stride_r = (a.R + 7) / 8 * 8;
+  p.stride_t = (int64_t)div_up(a.rows, STAGE) * STAGE;
+  const size_t part = (size_t)a.rows * a.R * sizeof(float), rank = bytes_of((size_t)2 * a.rows * p.stride_r * 2);
+  const size_t rows = bytes_of((size_t)2 * a.R * p.stride_t * 2);
+  if (!backward) {
+    if (p.run) p.h.rank = rank;
+    else p.h.part = bytes_of(part * p.h.slices);
+    p.total = p.h.part + p.h.rank;
+    return p;
+  }
+  cut(tiles, p.turns, a.N, div_up(a.R, 128), p.run, p.g);
+  p.h.part = p.h.slices > 1 ? bytes_of(part * p.h.slices) : 0;
+  p.g.part = p.g.slices > 1 ? bytes_of(part * p.g.slices) : 0;
+  p.h.rows = p.g.rows = rows;
+  p.g.rank = rank;
+  p.rt = a.R <= 16 ? 1 : 2;
+  // rows are cut over blocks until the card has one a CU, each with a run of 1024 at least: parts are written and read again
+  const int64_t blocks = (int64_t)(div_up(a.K, 512) + div_up(a.N, 512)) * a.n * div_up(a.R, 16 * p.rt);
+  int splits = div_up(HDMOE_NUM_CU, blocks);
+  const int most = div_up(a.rows, 4 * STAGE);
   if (splits > most) splits = most;
-  if (splits > 64) splits = 64;
-  p.per_split = div_up(div_up(a.rows, splits), STAGE) * STAGE;
+  p.per_split = div_up(div_up(a.rows, splits), 2 * STAGE) * 2 * STAGE;
   p.splits = div_up(a.rows, p.per_split);
   if (p.splits > 1) {
-    p.da_bytes = hdmoe_align_up((size_t)p.splits * a.n * a.R * a.K * sizeof(float), 256);
-    p.db_bytes = hdmoe_align_up((size_t)p.splits * a.n * a.R * a.N * sizeof(float), 256);
+    p.da_bytes = bytes_of((size_t)p.splits * a.n * a.R * a.K * sizeof(float));
+    p.db_bytes = bytes_of((size_t)p.splits * a.n * a.R * a.N * sizeof(float));
   }
+  p.total = p.h.part + p.g.part + p.h.rows + p.g.rows + p.g.rank + p.da_bytes + p.db_bytes;
   return p;
 }
 
@@ -443,12 +675,13 @@ void launch_narrow(const NarrowArgs& p, int tm, hipStream_t s) {
   auto go = [&](auto rt, auto m) {
     constexpr int RT = decltype(rt)::value, TM = decltype(m)::value;
     const dim3 grid(div_up(p.q.T, 16 * TM) * p.slices * p.turns, div_up(p.R, 16 * RT));
-    hipLaunchKernelGGL((narrow_kernel<A, ACROSS, RT, TM>), grid, dim3(WAVES * 64), 0, s, p);
+    hipLaunchKernelGGL((narrow_kernel<A, ACROSS, RT, TM>), grid, dim3(NARROW_WAVES * 64), 0, s, p);
   };
   using std::integral_constant;
   auto rt = [&](auto r) {
     if (tm == 1) go(r, integral_constant<int, 1>());
     else if constexpr (decltype(r)::value == 8) go(r, integral_constant<int, 2>());
+    else if (tm == 2) go(r, integral_constant<int, 2>());
     else go(r, integral_constant<int, 4>());
   };
   if constexpr (ACROSS) {
@@ -462,18 +695,14 @@ void launch_narrow(const NarrowArgs& p, int tm, hipStream_t s) {
 }
 
 template <class A, bool ACROSS>
-void launch_wide(const WideArgs& p, int tm, hipStream_t s) {
-  auto go = [&](auto m) {
-    constexpr int TM = decltype(m)::value;
-    const int chunks = div_up(p.C, WAVES * (ACROSS ? 128 : 64)), tiles = div_up(p.q.T, 16 * TM);
-    const size_t bytes = (size_t)2 * 16 * TM * ((p.R + 31) / 32 * 32 + 8) * 2;
-    hipLaunchKernelGGL((wide_kernel<A, ACROSS, TM>), dim3((unsigned)(chunks * tiles * p.turns)), dim3(WAVES * 64), bytes, s, p);
+void launch_wide_run(const WideArgs& p, hipStream_t s) {
+  auto go = [&](auto steps) {
+    constexpr int STEPS = decltype(steps)::value;
+    const dim3 grid(div_up(p.C, WAVES * Wide<A, ACROSS>::COLS) * div_up(p.q.T, RUN));
+    hipLaunchKernelGGL((wide_run_kernel<A, ACROSS, STEPS>), grid, dim3(WAVES * 64), 0, s, p, div_up(p.R, 32 * STEPS));
   };
-  using std::integral_constant;
-  if (tm == 1) go(integral_constant<int, 1>());
-  else if constexpr (ACROSS) go(integral_constant<int, 2>());   // 128 columns: half the rows in as many registers
-  else if (tm == 2) go(integral_constant<int, 2>());
-  else go(integral_constant<int, 4>());
+  if (p.R <= 32) go(std::integral_constant<int, 1>());
+  else go(std::integral_constant<int, 2>());
 }
 
 int check_args(const hdmoe_adapter_args* a, const char* what, bool backward) {
@@ -483,7 +712,7 @@ int check_args(const hdmoe_adapter_args* a, const char* what, bool backward) {
       a->requests < 0 || (a->rows > 0 && (a->requests == 0 || a->rows % a->requests != 0)))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%d requests=%d K=%d N=%d n=%d (1 to %d) R=%d (1 to %d)", what, a->rows, a->requests, a->K, a->N,
                       a->n, HDMOE_ADAPTER_MAX, a->R, HDMOE_ADAPTER_MAX_RANK);
-  const int64_t blocks = (int64_t)div_up(a->rows, 16) * 16 * (div_up(a->N, 64) + div_up(a->K, 64));
+  const int64_t blocks = (int64_t)div_up(a->rows, 16) * 16 * (div_up(a->N, 256) + div_up(a->K, 256) + 8);
   if (blocks >= (int64_t)1 << 31) return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%d K=%d N=%d: too many tiles", what, a->rows, a->K, a->N);
   if (a->K > (1 << 24) || a->N > (1 << 24) || a->rows > (1 << 30))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%d (at most 2^30) K=%d N=%d (at most 2^24)", what, a->rows, a->K, a->N);
@@ -507,8 +736,13 @@ const uint16_t* bits(const void* p) { return static_cast<const uint16_t*>(p); }
 
 extern "C" size_t hdmoe_adapters_workspace_bytes(const hdmoe_adapter_args* a, int backward) {
   if (check_args(a, "hdmoe_adapters_workspace_bytes", backward != 0) != HDMOE_OK || a->rows == 0) return 0;
-  const Plan p = plan_of(*a, backward != 0);
-  return p.h_bytes + p.g_bytes + p.da_bytes + p.db_bytes;
+  return plan_of(*a, backward != 0).total;
+}
+
+static int check_workspace(const hdmoe_adapter_args* a, const Plan& plan, const char* what) {
+  if (a->workspace == nullptr || a->workspace_bytes < plan.total || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0)
+    return hdmoe_fail(HDMOE_E_WORKSPACE, "%s: workspace of %zu bytes on 16 needed, got %zu", what, plan.total, a->workspace_bytes);
+  return HDMOE_OK;
 }
 
 extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t stream) {
@@ -516,16 +750,22 @@ extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t st
   if (a->rows == 0) return HDMOE_OK;
   if (a->base == nullptr || a->out == nullptr) return hdmoe_fail(HDMOE_E_NULL, "hdmoe_add_adapters: base or out is NULL");
   const Plan plan = plan_of(*a, false);
-  if (a->workspace == nullptr || a->workspace_bytes < plan.h_bytes || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0)
-    return hdmoe_fail(HDMOE_E_WORKSPACE, "hdmoe_add_adapters: workspace of %zu bytes on 16 needed, got %zu", plan.h_bytes, a->workspace_bytes);
+  if (int rc = check_workspace(a, plan, "hdmoe_add_adapters")) return rc;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  float* h = static_cast<float*>(a->workspace);
-  const NarrowArgs np = {requests_of(a), bits(a->x), bits(a->a), h, a->K, a->R, plan.slice_x, plan.slices_x, plan.turns};
-  const WideArgs wp = {requests_of(a), h, bits(a->b), bits(a->base), static_cast<uint16_t*>(a->out), a->N, a->R, plan.slices_x, plan.turns_wide};
+  const Requests q = requests_of(a);
+  float* part = plan.run ? nullptr : static_cast<float*>(a->workspace);
+  const Planes planes = {plan.run ? static_cast<uint16_t*>(a->workspace) : nullptr, nullptr, plan.stride_r, 0};
+  const NarrowArgs np = {q, bits(a->x), bits(a->a), part, planes, a->K, a->R, plan.h.slice, plan.h.slices, plan.turns};
+  const WideArgs wp = {q, part, planes, bits(a->b), bits(a->base), static_cast<uint16_t*>(a->out), a->N, a->R, plan.h.slices, plan.turns};
   typed(a->dtype, [&](auto t) {
     typedef decltype(t) A;
-    launch_narrow<A, false>(np, plan.tm_narrow, s);
-    launch_wide<A, false>(wp, plan.tm_wide, s);
+    launch_narrow<A, false>(np, plan.tm, s);
+    if (plan.run) {
+      launch_wide_run<A, false>(wp, s);
+    } else {
+      const dim3 grid(div_up(a->N, WAVES * Wide<A, false>::COLS) * div_up(a->rows, 16) * plan.turns);
+      hipLaunchKernelGGL((wide_kernel<A, false>), grid, dim3(WAVES * 64), (size_t)2 * 16 * ((a->R + 31) / 32 * 32 + 8) * 2, s, wp);
+    }
   });
   return hdmoe_check_launch("hdmoe_add_adapters");
 }
@@ -537,43 +777,50 @@ extern "C" int hdmoe_add_adapters_backward(const hdmoe_adapter_args* a, hdmoe_st
   SumArgs sp = {};
   sp.out[0] = static_cast<uint16_t*>(a->da), sp.out[1] = static_cast<uint16_t*>(a->db);
   sp.n[0] = (size_t)a->n * a->R * a->K, sp.n[1] = (size_t)a->n * a->R * a->N;
-  if ((sp.n[0] + sp.n[1]) / 256 >= (1u << 31)) return hdmoe_fail(HDMOE_E_SHAPE, "hdmoe_add_adapters_backward: n=%d R=%d K=%d N=%d", a->n, a->R, a->K, a->N);
-  auto sum = [&] {
-    typed(a->dtype, [&](auto t) {
-      hipLaunchKernelGGL(sum_parts_kernel<decltype(t)>, dim3((unsigned)((sp.n[0] + sp.n[1] + 255) / 256)), dim3(256), 0, s, sp);
-    });
-  };
+  if (sp.n[0] + sp.n[1] >= (size_t)1 << 38) return hdmoe_fail(HDMOE_E_SHAPE, "hdmoe_add_adapters_backward: n=%d R=%d K=%d N=%d", a->n, a->R, a->K, a->N);
   if (a->rows == 0) {   // gradients of zero
-    sum();
+    typed(a->dtype, [&](auto t) { launch_sum_parts<decltype(t)>(sp, s); });
     return hdmoe_check_launch("hdmoe_add_adapters_backward");
   }
   if (a->dy == nullptr || a->dx == nullptr) return hdmoe_fail(HDMOE_E_NULL, "hdmoe_add_adapters_backward: dy or dx is NULL");
   const Plan plan = plan_of(*a, true);
-  const size_t need = plan.h_bytes + plan.g_bytes + plan.da_bytes + plan.db_bytes;
-  if (a->workspace == nullptr || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0)
-    return hdmoe_fail(HDMOE_E_WORKSPACE, "hdmoe_add_adapters_backward: workspace of %zu bytes on 16 needed, got %zu", need, a->workspace_bytes);
+  if (int rc = check_workspace(a, plan, "hdmoe_add_adapters_backward")) return rc;
   char* ws = static_cast<char*>(a->workspace);
-  float *h = reinterpret_cast<float*>(ws), *g = reinterpret_cast<float*>(ws + plan.h_bytes);
-  float *da = reinterpret_cast<float*>(ws + plan.h_bytes + plan.g_bytes), *db = reinterpret_cast<float*>(ws + plan.h_bytes + plan.g_bytes + plan.da_bytes);
+  auto take = [&](size_t n) {
+    void* at = n > 0 ? ws : nullptr;
+    ws += n;
+    return at;
+  };
   const Requests q = requests_of(a);
-  const NarrowArgs hp = {q, bits(a->x), bits(a->a), h, a->K, a->R, plan.slice_x, plan.slices_x, plan.turns};
-  const NarrowArgs gp = {q, bits(a->dy), bits(a->b), g, a->N, a->R, plan.slice_y, plan.slices_y, plan.turns};
-  const WideArgs wp = {q, g, bits(a->a), nullptr, static_cast<uint16_t*>(a->dx), a->K, a->R, plan.slices_y, plan.turns_wide};
+  JoinArgs jp = {};
+  jp.q = q, jp.R = a->R, jp.slices[0] = plan.h.slices, jp.slices[1] = plan.g.slices;
+  float* h = static_cast<float*>(take(plan.h.part));
+  float* g = static_cast<float*>(take(plan.g.part));
+  jp.part[0] = h, jp.part[1] = g;
+  jp.to[0] = {nullptr, static_cast<uint16_t*>(take(plan.h.rows)), plan.stride_r, plan.stride_t};
+  uint16_t* grows = static_cast<uint16_t*>(take(plan.g.rows));
+  jp.to[1] = {static_cast<uint16_t*>(take(plan.g.rank)), grows, plan.stride_r, plan.stride_t};
+  const NarrowArgs hp = {q, bits(a->x), bits(a->a), h, jp.to[0], a->K, a->R, plan.h.slice, plan.h.slices, plan.turns};
+  const NarrowArgs gp = {q, bits(a->dy), bits(a->b), g, jp.to[1], a->N, a->R, plan.g.slice, plan.g.slices, plan.turns};
+  const WideArgs wp = {q, nullptr, jp.to[1], bits(a->a), nullptr, static_cast<uint16_t*>(a->dx), a->K, a->R, 1, 1};
   OuterArgs op = {};
-  op.q = q, op.R = a->R, op.splits = plan.splits, op.per_split = plan.per_split, op.direct = plan.splits == 1;
-  op.side[0] = {bits(a->x), g, op.direct ? a->da : da, a->K, plan.slices_y, 0, div_up(a->K, WAVES * 128)};
-  op.side[1] = {bits(a->dy), h, op.direct ? a->db : db, a->N, plan.slices_x, 1, div_up(a->N, WAVES * 128)};
+  op.q = q, op.R = a->R, op.splits = plan.splits, op.per_split = plan.per_split, op.direct = plan.splits == 1, op.stride_t = plan.stride_t;
+  float* da = static_cast<float*>(take(plan.da_bytes));
+  float* db = static_cast<float*>(take(plan.db_bytes));
+  op.side[0] = {bits(a->x), jp.to[1].rows, op.direct ? a->da : da, a->K, 0, div_up(a->K, 512)};
+  op.side[1] = {bits(a->dy), jp.to[0].rows, op.direct ? a->db : db, a->N, 1, div_up(a->N, 512)};
   sp.part[0] = da, sp.part[1] = db, sp.splits = plan.splits;
   const dim3 grid(op.side[0].blocks + op.side[1].blocks, a->n * div_up(a->R, 16 * plan.rt), plan.splits);
   typed(a->dtype, [&](auto t) {
     typedef decltype(t) A;
-    launch_narrow<A, false>(hp, plan.tm_narrow, s);
-    launch_narrow<A, true>(gp, plan.tm_narrow, s);
-    launch_wide<A, true>(wp, plan.tm_wide, s);
-    if (plan.rt == 1) hipLaunchKernelGGL((outer_kernel<A, 1>), grid, dim3(WAVES * 64), 0, s, op);
-    else if (plan.rt == 2) hipLaunchKernelGGL((outer_kernel<A, 2>), grid, dim3(WAVES * 64), 0, s, op);
-    else hipLaunchKernelGGL((outer_kernel<A, 4>), grid, dim3(WAVES * 64), 0, s, op);
+    launch_narrow<A, false>(hp, plan.tm, s);
+    launch_narrow<A, true>(gp, plan.tm, s);
+    if (h != nullptr || g != nullptr)
+      hipLaunchKernelGGL(join_kernel, dim3(div_up((int64_t)a->rows * div_up(a->R, 8), 256), 2), dim3(256), 0, s, jp);
+    launch_wide_run<A, true>(wp, s);
+    if (plan.rt == 1) hipLaunchKernelGGL((outer_kernel<A, 1>), grid, dim3(512), 0, s, op);
+    else hipLaunchKernelGGL((outer_kernel<A, 2>), grid, dim3(512), 0, s, op);
+    if (plan.splits > 1) launch_sum_parts<A>(sp, s);
   });
-  if (plan.splits > 1) sum();
   return hdmoe_check_launch("hdmoe_add_adapters_backward");
 }

@@ -104,22 +104,56 @@ __device__ __forceinline__ f4 mul_split(u4 ah, u4 al, u4 qh, u4 ql, f4 c) {
   return Bf16::mul(ah, qh, c);
 }
 
-// Sums of `splits` parts in their order, rounded once; no parts: zeros.
+// Sums of `splits` parts, each group of parts in its order and the groups in theirs, rounded once; no parts: zeros. Four values a thread; GROUPS threads share
+// them where there are many parts (103 parts of 10240 values 28 us with one, 4 with 16).
 struct SumArgs {
   const float* part[2];
   uint16_t* out[2];
   size_t n[2];
   int splits;
 };
+template <class A, int GROUPS>
+static __global__ __launch_bounds__(GROUPS == 1 ? 256 : 64 * GROUPS) void sum_parts_kernel(SumArgs p) {
+  constexpr int LANES = GROUPS == 1 ? 256 : 64;
+  __shared__ f4 lds[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? 64 : 1];
+  const size_t blocks = (p.n[0] + LANES * 4 - 1) / (LANES * 4);
+  const int side = blockIdx.x >= blocks, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const size_t n = p.n[side], i = ((size_t)blockIdx.x - (side ? blocks : 0)) * LANES * 4 + lane * 4;
+  f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int each = (p.splits + GROUPS - 1) / GROUPS, hi = min(p.splits, (group + 1) * each);
+  const float* from = p.part[side] + i;
+  if (i + 4 <= n) {
+#pragma unroll 8
+    for (int s = group * each; s < hi; ++s) {
+      f4 q;
+      __builtin_memcpy(&q, from + (size_t)s * n, 16);
+      v += q;
+    }
+  } else if (i < n) {
+    for (int s = group * each; s < hi; ++s)
+      for (int j = 0; j < 4; ++j)
+        if (i + j < n) v[j] += from[(size_t)s * n + j];
+  }
+  if constexpr (GROUPS > 1) {
+    lds[group][lane] = v;
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) v += lds[g][lane];
+  }
+  uint16_t* to = p.out[side] + i;
+  const uint32_t o[2] = {A::pack(v[0], v[1]), A::pack(v[2], v[3])};
+  if (i + 4 <= n) __builtin_memcpy(to, o, 8);
+  else
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) to[j] = (uint16_t)(o[j / 2] >> (16 * (j & 1)));
+}
+
 template <class A>
-static __global__ __launch_bounds__(256) void sum_parts_kernel(SumArgs p) {
-  size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const int side = i >= p.n[0];
-  if (side) i -= p.n[0];
-  if (i >= p.n[side]) return;
-  float v = 0.0f;
-  for (int s = 0; s < p.splits; ++s) v += p.part[side][s * p.n[side] + i];
-  p.out[side][i] = (uint16_t)A::pack(v, 0.0f);
+static void launch_sum_parts(const SumArgs& p, hipStream_t s) {
+  auto blocks = [&](size_t lanes) { return dim3((unsigned)((p.n[0] + lanes * 4 - 1) / (lanes * 4) + (p.n[1] + lanes * 4 - 1) / (lanes * 4))); };
+  if (p.splits > 16) hipLaunchKernelGGL((sum_parts_kernel<A, 16>), blocks(64), dim3(1024), 0, s, p);
+  else hipLaunchKernelGGL((sum_parts_kernel<A, 1>), blocks(256), dim3(256), 0, s, p);
 }
 
 }  // namespace lowrank

@@ -463,7 +463,7 @@ extern "C" int hdmoe_gate_balance_backward(const hdmoe_balance_args* a, hdmoe_st
       if (n != nullptr) hipLaunchKernelGGL(mask_counts_kernel, dim3(a->sequences), dim3(256), 0, s, a->mask, p.length, n);
       hipLaunchKernelGGL(gate_balance_backward_kernel<A>, dim3(div_up(a->D, WAVES * 128), splits), dim3(WAVES * 64), 0, s, p);
     }
-    if (splits != 1) hipLaunchKernelGGL(sum_parts_kernel<A>, dim3((unsigned)((sp.n[0] + 255) / 256)), dim3(256), 0, s, sp);
+    if (splits != 1) launch_sum_parts<A>(sp, s);
   });
   return hdmoe_check_launch("hdmoe_gate_balance_backward");
 }

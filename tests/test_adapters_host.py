@@ -56,7 +56,7 @@ def _args(**kwargs):
     buf = (ctypes.c_char * 64)()
     p = (ctypes.addressof(buf) + 15) // 16 * 16
     a = _lib.AdapterArgs()
-    a.dtype, a.rows, a.requests, a.K, a.N, a.n, a.R = _lib.T_BF16, 64, 4, 256, 128, 2, 16
+    a.dtype, a.rows, a.requests, a.K, a.N, a.n, a.R = _lib.T_BF16, 64, 4, 4096, 2048, 2, 16
     for name in ("x", "a", "b", "scale", "index", "base", "out", "dy", "dx", "da", "db"):
         setattr(a, name, p)
     for k, v in kwargs.items():
