@@ -21,7 +21,7 @@ namespace {
 constexpr int WAVES = 4;                   // of `wide`
 constexpr int NARROW_WAVES = 8;
 constexpr int K_STEP = 64;                 // along the contraction, of a wave: 128 bytes of each row
-constexpr int RUN = 256;                   // tokens of a block of `wide_run`
+constexpr int RUN = 256;                   // tokens of a block of `wide_run` at most
 constexpr int STAGE = 128;                 // tokens that `outer` looks at the adapters of at a time
 
 struct Requests {
@@ -113,20 +113,20 @@ __global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p)
     const uint16_t* w = p.w + (size_t)a * p.R * p.K;
     auto step = [&](int k0, auto whole) {
       constexpr bool WHOLE = decltype(whole)::value;
-      // a lane's 16 values of a row: two instructions' worth
-      const int k = k0 + quad * 16, have = WHOLE ? 16 : hi - k;
+      // two instructions' worth of 32 k, of which a lane has eight each: 64 bytes of a row next to each other
+      const int k = k0 + quad * 8, have = WHOLE ? K_STEP : hi - k;
       u4 xv[TM][2];
 #pragma unroll
       for (int m = 0; m < TM; ++m)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) xv[m][i] = WHOLE ? load8(rows[m] + k + 8 * i) : load8(rows[m] + k + 8 * i, have - 8 * i);
+        for (int i = 0; i < 2; ++i) xv[m][i] = WHOLE ? load8(rows[m] + k + 32 * i) : load8(rows[m] + k + 32 * i, have - 32 * i);
       if constexpr (!ACROSS) {
         u4 wv[RT][2];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           const uint16_t* wr = w + (size_t)min(r0 + r * 16 + col, p.R - 1) * p.K + k;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) wv[r][i] = WHOLE ? load8(wr + 8 * i) : load8(wr + 8 * i, have - 8 * i);
+          for (int i = 0; i < 2; ++i) wv[r][i] = WHOLE ? load8(wr + 32 * i) : load8(wr + 32 * i, have - 32 * i);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p)
           u4 wv[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {   // past the end x is 0: the last row again
-            const uint16_t* from = w + (size_t)(WHOLE ? k + 8 * i + j : min(k + 8 * i + j, p.K - 1)) * p.R + r;
+            const uint16_t* from = w + (size_t)(WHOLE ? k + 32 * i + j : min(k + 32 * i + j, p.K - 1)) * p.R + r;
             wv[j] = even ? load8(from) : load8(from, p.R - r);
           }
           transpose8(wv);
@@ -235,8 +235,8 @@ struct WideArgs {
   int C, R, slices, turns;
 };
 
-// out[t][c] = base[t][c] + s sum_r h[t][r] w[a][c][r]. A wave has 64 columns (ACROSS: 128), a lane 16 (32) of them next to each other, so that it
-// loads and stores whole 16-byte pieces and a token's 128 (256) bytes are one wave's.
+// out[t][c] = base[t][c] + s sum_r h[t][r] w[a][c][r]. A wave has 64 columns (ACROSS: 128), a lane eight of every 32 of them: a load or store of the
+// wave takes 64 bytes next to each other of 16 rows (16 pieces with gaps between them before: 16384 rows, rank 64, 154 us).
 template <class A, bool ACROSS>
 struct Wide {
   static constexpr int NT = ACROSS ? 8 : 4;    // instructions side by side
@@ -245,7 +245,7 @@ struct Wide {
   int c0, col, quad, c, have;
   bool whole;
   __device__ __forceinline__ Wide(const WideArgs& args, int first, int lane) : p(args), c0(first), col(lane & 15), quad(lane >> 4) {
-    c = c0 + quad * 4 * NT;
+    c = c0 + quad * 8;
     have = p.C - c;
     whole = c0 + COLS <= p.C;
   }
@@ -256,14 +256,16 @@ struct Wide {
     if constexpr (ACROSS) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint16_t* from = w + (size_t)min(r + j, p.R - 1) * p.C + c0 + col * 8;
-        wh[j] = whole ? load8(from) : load8(from, p.C - c0 - col * 8);
+        const int at = c0 + ((col & 3) * 4 + (col >> 2)) * 8;     // result row 4 quad + e: the lane's eight of piece e
+        const uint16_t* from = w + (size_t)min(r + j, p.R - 1) * p.C + at;
+        wh[j] = whole ? load8(from) : load8(from, p.C - at);
       }
       transpose8(wh);
     } else {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const uint16_t* from = w + (size_t)min(c0 + (col >> 2) * 16 + j * 4 + (col & 3), p.C - 1) * p.R;
+        // result row 4 quad + e of instruction j: value 4 j + e of the lane's
+        const uint16_t* from = w + (size_t)min(c0 + (j >> 1) * 32 + (col >> 2) * 8 + (j & 1) * 4 + (col & 3), p.C - 1) * p.R;
         wh[j] = p.R % 8 == 0 ? load8(from + min(r, p.R - 8)) : load8(from + r, p.R - r);
       }
     }
@@ -276,7 +278,7 @@ struct Wide {
 #pragma unroll
     for (int i = 0; i < NT / 2; ++i) {
       b[i] = u4{0, 0, 0, 0};
-      if (want && p.base != nullptr) b[i] = whole ? load8(from + 8 * i) : load8(from + 8 * i, have - 8 * i);
+      if (want && p.base != nullptr) b[i] = whole ? load8(from + 32 * i) : load8(from + 32 * i, have - 32 * i);
     }
   }
   __device__ __forceinline__ void put(int t, const f4 (&acc)[NT], const u4 (&b)[NT / 2]) const {
@@ -286,13 +288,13 @@ struct Wide {
       u4 o;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        // ACROSS: instruction j, element e are column 8 e + j, else 4 j + e
+        // value u of the lane: ACROSS, of instruction u % 8, else u / 4
         const int u = 8 * i + 2 * w;
         const float v0 = ACROSS ? acc[u % 8][u / 8] : acc[u / 4][u % 4], v1 = ACROSS ? acc[u % 8 + 1][u / 8] : acc[u / 4][u % 4 + 1];
         o[w] = p.base != nullptr ? A::pack(v0 + A::lo(b[i][w]), v1 + A::hi(b[i][w])) : A::pack(v0, v1);
       }
-      if (whole) __builtin_memcpy(to + 8 * i, &o, 16);
-      else store8(to + 8 * i, o, have - 8 * i);
+      if (whole) __builtin_memcpy(to + 32 * i, &o, 16);
+      else store8(to + 32 * i, o, have - 32 * i);
     }
   }
   // a row without an adapter: the base as it is, bit for bit
@@ -301,8 +303,8 @@ struct Wide {
 #pragma unroll
     for (int i = 0; i < NT / 2; ++i) {
       u4 v = {0, 0, 0, 0};
-      if (p.base != nullptr) v = load8(p.base + (size_t)t * p.C + c + 8 * i, have - 8 * i);
-      store8(p.out + (size_t)t * p.C + c + 8 * i, v, have - 8 * i);
+      if (p.base != nullptr) v = load8(p.base + (size_t)t * p.C + c + 32 * i, have - 32 * i);
+      store8(p.out + (size_t)t * p.C + c + 32 * i, v, have - 32 * i);
     }
   }
 };
@@ -374,21 +376,21 @@ __global__ __launch_bounds__(WAVES * 64) void wide_kernel(WideArgs p) {
   });
 }
 
-// Many rows: a block has RUN tokens, 16 at a time; a wave keeps the weights of its columns in registers for as long as the adapter stays the same (R up to
+// Many rows: a block has up to RUN tokens, 16 at a time; a wave keeps the weights of its columns in registers for as long as the adapter stays the same (R up to
 // 32 STEPS; `parts` times that are gone through one after the other, loaded anew). Values and base of the next 16 tokens are on their way
 // while these are multiplied. Bound by base and out: R of 64 takes 16 instructions (256 cycles of one of four units) for 4 KB of them.
 template <class A, bool ACROSS, int STEPS>
-__global__ __launch_bounds__(WAVES * 64) void wide_run_kernel(WideArgs p, int parts) {
+__global__ __launch_bounds__(WAVES * 64) void wide_run_kernel(WideArgs p, int parts, int run) {
   typedef Wide<A, ACROSS> W;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int chunks = (p.C + WAVES * W::COLS - 1) / (WAVES * W::COLS);
-  const int chunk = blockIdx.x % chunks, t0 = blockIdx.x / chunks * RUN;
+  const int chunk = blockIdx.x % chunks, t0 = blockIdx.x / chunks * run;
   const W w(p, (chunk * WAVES + wave) * W::COLS, lane);
   if (w.c0 >= p.C) return;
   int of[RUN / 64];
 #pragma unroll
-  for (int i = 0; i < RUN / 64; ++i) of[i] = p.q.of(t0 + i * 64 + lane);
-  const int groups = min(RUN, p.q.T - t0 + 15) / 16;
+  for (int i = 0; i < RUN / 64; ++i) of[i] = i * 64 < run ? p.q.of(t0 + i * 64 + lane) : -1;
+  const int groups = min(run, p.q.T - t0 + 15) / 16;
   const size_t plane = (size_t)p.q.T * p.from.stride_r;
   struct Tokens {
     u4 q[2][STEPS], b[W::NT / 2];
@@ -619,7 +621,7 @@ size_t bytes_of(size_t n) { return hdmoe_align_up(n, 256); }
 
 constexpr int MANY_ROWS = 512;   // from here on `wide` keeps its weights over runs of tokens
 
-// The contraction is cut over blocks until the card has about one a CU, in slices of at least two steps of each wave; with `run` not at all.
+// The contraction is cut over blocks until the card has about one a CU, in slices of at least two steps of each wave; `whole`: not at all.
 void cut(int tiles, int turns, int K, int rblocks, bool whole, Side& s) {
   const int most = div_up(K, 2 * NARROW_WAVES * K_STEP);
   int want = whole ? 1 : div_up(HDMOE_NUM_CU, (int64_t)tiles * turns * rblocks);
@@ -638,7 +640,7 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   const int tile = 16 * p.tm, distinct = div_up(tile, rows_per);
   p.turns = distinct < a.n ? distinct : a.n;
   const int tiles = div_up(a.rows, tile);
-  cut(tiles, p.turns, a.K, div_up(a.R, 128), p.run, p.h);
+  cut(tiles, p.turns, a.K, div_up(a.R, 128), p.run && !backward, p.h);
   p.stride_r = (a.R + 7) / 8 * 8;
   p.stride_t = (int64_t)div_up(a.rows, STAGE) * STAGE;
   const size_t part = (size_t)a.rows * a.R * sizeof(float), rank = bytes_of((size_t)2 * a.rows * p.stride_r * 2);
@@ -649,7 +651,7 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
     p.total = p.h.part + p.h.rank;
     return p;
   }
-  cut(tiles, p.turns, a.N, div_up(a.R, 128), p.run, p.g);
+  cut(tiles, p.turns, a.N, div_up(a.R, 128), false, p.g);
   p.h.part = p.h.slices > 1 ? bytes_of(part * p.h.slices) : 0;
   p.g.part = p.g.slices > 1 ? bytes_of(part * p.g.slices) : 0;
   p.h.rows = p.g.rows = rows;
@@ -698,8 +700,11 @@ template <class A, bool ACROSS>
 void launch_wide_run(const WideArgs& p, hipStream_t s) {
   auto go = [&](auto steps) {
     constexpr int STEPS = decltype(steps)::value;
-    const dim3 grid(div_up(p.C, WAVES * Wide<A, ACROSS>::COLS) * div_up(p.q.T, RUN));
-    hipLaunchKernelGGL((wide_run_kernel<A, ACROSS, STEPS>), grid, dim3(WAVES * 64), 0, s, p, div_up(p.R, 32 * STEPS));
+    // runs as long as four blocks a CU allow
+    const int chunks = div_up(p.C, WAVES * Wide<A, ACROSS>::COLS);
+    int run = div_up((int64_t)p.q.T * chunks, 4 * HDMOE_NUM_CU * 16) * 16;
+    if (run > RUN) run = RUN;
+    hipLaunchKernelGGL((wide_run_kernel<A, ACROSS, STEPS>), dim3(chunks * div_up(p.q.T, run)), dim3(WAVES * 64), 0, s, p, div_up(p.R, 32 * STEPS), run);
   };
   if (p.R <= 32) go(std::integral_constant<int, 1>());
   else go(std::integral_constant<int, 2>());

@@ -50,13 +50,13 @@ __global__ __launch_bounds__(WAVES * 64) void gate_balance_kernel(BalanceArgs p)
   for (int m = 0; m < TM; ++m) rows[m] = p.x + (size_t)(seq * p.length + min(l0 + m * 16 + col, p.length - 1)) * p.D;
   auto step = [&](int k0, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
-    const int k = k0 + quad * 16;
+    const int k = k0 + quad * 8;     // 64 bytes of a row next to each other
     u4 wv[2], xv[TM][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      wv[i] = WHOLE ? load8(wr + k + 8 * i) : load8(wr + k + 8 * i, p.D - k - 8 * i);
+      wv[i] = WHOLE ? load8(wr + k + 32 * i) : load8(wr + k + 32 * i, p.D - k - 32 * i);
 #pragma unroll
-      for (int m = 0; m < TM; ++m) xv[m][i] = WHOLE ? load8(rows[m] + k + 8 * i) : load8(rows[m] + k + 8 * i, p.D - k - 8 * i);
+      for (int m = 0; m < TM; ++m) xv[m][i] = WHOLE ? load8(rows[m] + k + 32 * i) : load8(rows[m] + k + 32 * i, p.D - k - 32 * i);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -226,7 +226,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void gate_balance_backward_kernel(Ba
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int e = (quad >> 1) * 8 + j;
-    wh[j] = mine && e < p.E ? load8(p.w + (size_t)e * p.D + c) : u4{0, 0, 0, 0};
+    const int at = c0 + ((col & 3) * 4 + (col >> 2)) * 8;   // result row 4 quad + e: the lane's eight of every 32 columns
+    wh[j] = at < p.D && e < p.E ? load8(p.w + (size_t)e * p.D + at) : u4{0, 0, 0, 0};
   }
   transpose8(wh);
   if constexpr (A::HALF)
@@ -320,7 +321,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void gate_balance_backward_kernel(Ba
           if constexpr (A::HALF) y[j] = Bf16::mul(wl[j], q, y[j]);
           y[j] = Bf16::mul(wh[j], q, y[j]);
         }
-        const int d = c0 + quad * 32;
+        const int d = c0 + quad * 8;
         if (t < end) {
           uint16_t* to = p.dx + (size_t)t * p.D + d;
 #pragma unroll
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void gate_balance_backward_kernel(Ba
             u4 o;
 #pragma unroll
             for (int w = 0; w < 4; ++w) o[w] = A::pack(y[2 * w][e], y[2 * w + 1][e]);
-            if (d + 8 * e < p.D) __builtin_memcpy(to + 8 * e, &o, 16);
+            if (d + 32 * e < p.D) __builtin_memcpy(to + 32 * e, &o, 16);
           }
         }
       }
