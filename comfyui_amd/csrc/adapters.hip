@@ -18,9 +18,9 @@ using namespace lowrank;
 
 namespace {
 
-constexpr int WAVES = 4;                   // of `wide`
+constexpr int WAVES = 4;                   // of `wide_run`
+constexpr int WIDE_WAVES = 2;              // of `wide`
 constexpr int NARROW_WAVES = 8;
-constexpr int K_STEP = 64;                 // along the contraction, of a wave: 128 bytes of each row
 constexpr int RUN = 256;                   // tokens of a block of `wide_run` at most
 constexpr int STAGE = 128;                 // tokens that `outer` looks at the adapters of at a time
 
@@ -49,16 +49,17 @@ __device__ __forceinline__ void each_adapter(int mine, int z, int turns, F f) {
   }
 }
 
-// Where narrow values end up, split: planes of hi and lo.
+// Where narrow values end up, split: pieces of 1 KB, what the 64 lanes of an instruction load.
+//   rank  [T / 16][R / 32][hi, lo][64][8]: lane 16 q + c has r = 8 q .. + 7 of token c (0 from R on)
+//   rows  [T / 32][R / 16][hi, lo][64][8]: lane 16 q + c has tokens 8 q .. + 7 of r = c
+// What rows without an adapter, or past T, and r past R of `rows` hold is not written and not used.
 struct Planes {
-  uint16_t* rank;       // [2][T][stride_r]: along the rank, 0 from R to stride_r (R filled up to 8)
-  uint16_t* rows;       // [2][R][stride_t]: along the rows (T filled up to 32; what rows without an adapter or past T hold is not read)
-  int stride_r;
-  int64_t stride_t;
+  uint16_t *rank, *rows;
+  int steps, tiles;     // R / 32, R / 16, filled up
 };
 
-// Eight r from r0 on of row t, scaled, into the planes.
-__device__ __forceinline__ void put_planes(const Planes& to, int T, int R, int t, int r, const float (&v)[8]) {
+// Eight r from r on of token t, scaled, into the planes.
+__device__ __forceinline__ void put_planes(const Planes& to, int R, int t, int r, const float (&v)[8]) {
   u4 vh, vl;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -67,19 +68,17 @@ __device__ __forceinline__ void put_planes(const Planes& to, int T, int R, int t
     vh[j] = h, vl[j] = l;
   }
   if (to.rank != nullptr) {
-    uint16_t* at = to.rank + (size_t)t * to.stride_r + r;
+    uint16_t* at = to.rank + (((size_t)(t >> 4) * to.steps + (r >> 5)) * 128 + ((r >> 3) & 3) * 16 + (t & 15)) * 8;
     *reinterpret_cast<u4*>(at) = vh;
-    *reinterpret_cast<u4*>(at + (size_t)T * to.stride_r) = vl;
+    *reinterpret_cast<u4*>(at + 512) = vl;
   }
-  if (to.rows != nullptr) {
-    uint16_t* at = to.rows + (size_t)r * to.stride_t + t;
-    const size_t plane = (size_t)R * to.stride_t;
+  if (to.rows != nullptr && r < R) {
+    uint16_t* at = to.rows + (((size_t)(t >> 5) * to.tiles + (r >> 4)) * 128 + ((t >> 3) & 3) * 16 + (r & 15)) * 8 + (t & 7);
 #pragma unroll
-    for (int j = 0; j < 8; ++j, at += to.stride_t)
-      if (r + j < R) {
-        at[0] = (uint16_t)(vh[j / 2] >> (16 * (j & 1)));
-        at[plane] = (uint16_t)(vl[j / 2] >> (16 * (j & 1)));
-      }
+    for (int j = 0; j < 8; ++j) {
+      at[8 * j] = (uint16_t)(vh[j / 2] >> (16 * (j & 1)));
+      at[8 * j + 512] = (uint16_t)(vl[j / 2] >> (16 * (j & 1)));
+    }
   }
 }
 
@@ -91,71 +90,109 @@ struct NarrowArgs {
   int K, R, slice, slices, turns;
 };
 
-// sum over the slice's k of x[t][k] w[a][r][k]. A tile is 16 TM tokens; the block's waves take steps of the slice in turn, 1 KB of a row next to
-// each other, and join their sums in LDS. ACROSS: w runs along r: eight k of eight r at a time, transposed in registers, 128 r of them (those past
-// R are not loaded) whatever R is.
-template <class A, bool ACROSS, int RT, int TM>
+// sum over the slice's k of x[t][k] w[a][r][k]. A tile is 16 TM tokens; the block's waves take blocks of 128 k of the slice in turn and join their sums in
+// LDS. Where w runs along r, eight k of eight r a lane are transposed in registers: ACROSS has 128 r side by side in eight instructions, whatever R is;
+// ACROSS32 has up to 32, four k blocks side by side instead, which are then dealt to instructions of 16 r each (8192 x 6912 rows, rank 32: 48 -> 29 us).
+enum { ALONG, ACROSS, ACROSS32 };
+template <class A, int MODE, int RT, int TM>
 __global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p) {
-  static_assert(!ACROSS || RT == 8, "128 r");
+  static_assert(MODE == ALONG || RT == (MODE == ACROSS ? 8 : 2), "128 or 32 r");
   static_assert(RT * TM <= 16, "64 KB of LDS");
-  __shared__ f4 joined[4][RT * TM][64];
+  __shared__ f4 joined[NARROW_WAVES / 2][RT * TM][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int tiles = (p.q.T + 16 * TM - 1) / (16 * TM);
   const int tile = blockIdx.x % tiles, slice = (blockIdx.x / tiles) % p.slices, z = blockIdx.x / tiles / p.slices;
   const int t0 = tile * 16 * TM, r0 = blockIdx.y * 16 * RT;
   const int lo = slice * p.slice, hi = min(p.K, lo + p.slice);
-  const uint16_t* rows[TM];
-#pragma unroll
-  for (int m = 0; m < TM; ++m) rows[m] = p.x + (size_t)min(t0 + m * 16 + col, p.q.T - 1) * p.K;
+  const int lane_row = col >> 2, lane_k = (quad * 4 + (col & 3)) * 8;      // of a load
   const int mine = lane < 16 * TM ? p.q.of(t0 + lane) : -1;
   each_adapter(mine, z, p.turns, [&](int a, uint64_t has) {
     f4 acc[RT][TM] = {};
     const uint16_t* w = p.w + (size_t)a * p.R * p.K;
     auto step = [&](int k0, auto whole) {
       constexpr bool WHOLE = decltype(whole)::value;
-      // two instructions' worth of 32 k, of which a lane has eight each: 64 bytes of a row next to each other
-      const int k = k0 + quad * 8, have = WHOLE ? K_STEP : hi - k;
-      u4 xv[TM][2];
+      const int k = k0 + lane_k;
+      u4 x[TM][4];
 #pragma unroll
       for (int m = 0; m < TM; ++m)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) xv[m][i] = WHOLE ? load8(rows[m] + k + 32 * i) : load8(rows[m] + k + 32 * i, have - 32 * i);
-      if constexpr (!ACROSS) {
-        u4 wv[RT][2];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const uint16_t* wr = w + (size_t)min(r0 + r * 16 + col, p.R - 1) * p.K + k;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) wv[r][i] = WHOLE ? load8(wr + 32 * i) : load8(wr + 32 * i, have - 32 * i);
+        for (int i = 0; i < 4; ++i) {
+          const uint16_t* from = p.x + (size_t)min(t0 + m * 16 + i * 4 + lane_row, p.q.T - 1) * p.K + k;
+          x[m][i] = WHOLE ? load8(from) : load8(from, hi - k);
         }
+      if constexpr (MODE == ALONG) {
+        constexpr int RB = RT < 2 ? RT : 2;     // r tiles at a time: registers
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int rb = 0; rb < RT; rb += RB) {
+          u4 wv[RB][4];
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
+          for (int r = 0; r < RB; ++r)
 #pragma unroll
-            for (int m = 0; m < TM; ++m) acc[r][m] = A::mul(wv[r][i], xv[m][i], acc[r][m]);
+            for (int i = 0; i < 4; ++i) {
+              const uint16_t* from = w + (size_t)min(r0 + (rb + r) * 16 + i * 4 + lane_row, p.R - 1) * p.K + k;
+              wv[r][i] = WHOLE ? load8(from) : load8(from, hi - k);
+            }
+          if (rb == 0)
+#pragma unroll
+            for (int m = 0; m < TM; ++m) quad_transpose(x[m]);
+#pragma unroll
+          for (int r = 0; r < RB; ++r) quad_transpose(wv[r]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+#pragma unroll
+              for (int m = 0; m < TM; ++m) acc[rb + r][m] = A::mul(wv[r][n], x[m][n], acc[rb + r][m]);
+          if (RB < RT) __builtin_amdgcn_sched_barrier(0);
+        }
+      } else if constexpr (MODE == ACROSS32) {
+        const int r = (col & 3) * 8;
+        u4 wv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {   // past the end x is 0: the last row again
+          const int kk = k0 + quad * 32 + (col >> 2) * 8 + j;
+          const uint16_t* from = w + (size_t)(WHOLE ? kk : min(kk, p.K - 1)) * p.R;
+          wv[j] = p.R % 8 == 0 ? load8(from + min(r, p.R - 8)) : load8(from + r, p.R - r);   // r past R is not stored
+        }
+        transpose8(wv);
+        u4 (*half)[4] = reinterpret_cast<u4 (*)[4]>(wv);      // instruction 4 h + n: block n, r = 8 (l % 4) + 4 h + l / 4 % 4
+        row_transpose(half[0]);
+        row_transpose(half[1]);
+#pragma unroll
+        for (int m = 0; m < TM; ++m) quad_transpose(x[m]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int m = 0; m < TM; ++m) acc[h][m] = A::mul(wv[4 * h + n], x[m][n], acc[h][m]);
       } else {
-        // r from R on: not stored (R a multiple of 8, the last eight are loaded again), or 0
-        const bool even = p.R % 8 == 0;
-        const int r = even ? min(r0 + col * 8, p.R - 8) : r0 + col * 8;
+        const int r = r0 + col * 8;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int n = 0; n < 4; ++n) {
           u4 wv[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {   // past the end x is 0: the last row again
-            const uint16_t* from = w + (size_t)(WHOLE ? k + 32 * i + j : min(k + 32 * i + j, p.K - 1)) * p.R + r;
-            wv[j] = even ? load8(from) : load8(from, p.R - r);
+            const int kk = k0 + quad * 32 + n * 8 + j;
+            wv[j] = u4{0, 0, 0, 0};
+            if (r < p.R) {
+              const uint16_t* from = w + (size_t)(WHOLE ? kk : min(kk, p.K - 1)) * p.R + r;
+              wv[j] = p.R % 8 == 0 ? load8(from) : load8(from, p.R - r);
+            }
           }
           transpose8(wv);
+          if (n == 0)
+#pragma unroll
+            for (int m = 0; m < TM; ++m) quad_transpose(x[m]);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int m = 0; m < TM; ++m) acc[j][m] = A::mul(wv[j], xv[m][i], acc[j][m]);
+            for (int m = 0; m < TM; ++m) acc[j][m] = A::mul(wv[j], x[m][n], acc[j][m]);
         }
       }
     };
-    int k0 = lo + wave * K_STEP;
-    for (; k0 + K_STEP <= hi; k0 += NARROW_WAVES * K_STEP) step(k0, std::true_type());
+    int k0 = lo + wave * K_BLOCK;
+    for (; k0 + K_BLOCK <= hi; k0 += NARROW_WAVES * K_BLOCK) step(k0, std::true_type());
     if (k0 < hi) step(k0, std::false_type());
     // the upper half of the waves into the lower one, and so on
 #pragma unroll
@@ -174,18 +211,20 @@ __global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p)
     }
     __syncthreads();
     const float scale = p.part != nullptr ? 1.0f : p.q.scale[a];
-    for (int u = threadIdx.x; u < 16 * TM * RT * 2; u += NARROW_WAVES * 64) {   // eight r of a token
+    constexpr int EIGHTS = RT == 1 ? 4 : RT * 2;     // `rank` holds 32 r at least
+    for (int u = threadIdx.x; u < 16 * TM * EIGHTS; u += NARROW_WAVES * 64) {   // eight r of a token
       const int m = u / 16 % TM, eight = u / (16 * TM), bit = u % (16 * TM), r = r0 + eight * 8, t = t0 + bit;
-      if (r >= p.R || !((has >> bit) & 1)) continue;
+      if (!((has >> bit) & 1)) continue;
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        // ACROSS: instruction j, row `eight`
-        const int row = ACROSS ? eight : (eight & 1) * 8 + j, tile_r = ACROSS ? j : eight >> 1;
-        v[j] = r + j < p.R ? joined[0][tile_r * TM + m][(row >> 2) * 16 + (bit & 15)][row & 3] * scale : 0.0f;
+        // r of a result: ACROSS 8 row + tile, ACROSS32 8 (row % 4) + 4 tile + row / 4, else 16 tile + row_of(row) (which undoes itself, as for tokens)
+        const int row = MODE == ACROSS ? eight : MODE == ACROSS32 ? (j & 3) * 4 + (eight & 3) : row_of((eight & 1) * 8 + j);
+        const int tile_r = MODE == ACROSS ? j : MODE == ACROSS32 ? j >> 2 : min(eight >> 1, RT - 1);
+        v[j] = r + j < p.R ? joined[0][tile_r * TM + m][(row >> 2) * 16 + row_of(bit & 15)][row & 3] * scale : 0.0f;
       }
       if (p.part == nullptr) {
-        put_planes(p.to, p.q.T, p.R, t, r, v);
+        if (r < p.to.steps * 32) put_planes(p.to, p.R, t, r, v);
         continue;
       }
       float* to = p.part + ((size_t)slice * p.q.T + t) * p.R + r;
@@ -197,6 +236,24 @@ __global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p)
   });
 }
 
+// v += eight values of each of `slices` parts, `next` apart (`have` of them).
+__device__ __forceinline__ void add_parts(const float* from, int slices, size_t next, int have, float (&v)[8]) {
+  if (have >= 8) {
+#pragma unroll 4
+    for (int s = 0; s < slices; ++s) {
+      f4 q[2];
+      __builtin_memcpy(q, from + s * next, 32);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += q[j / 4][j % 4];
+    }
+  } else {
+    for (int s = 0; s < slices; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < have) v[j] += from[s * next + j];
+  }
+}
+
 // Parts to planes: sums of the slices, scaled and split. Eight r of a row a thread.
 struct JoinArgs {
   Requests q;
@@ -204,144 +261,142 @@ struct JoinArgs {
   Planes to[2];
   int slices[2], R;
 };
-__global__ __launch_bounds__(256) void join_kernel(JoinArgs p) {
+__global__ __launch_bounds__(64) void join_kernel(JoinArgs p) {
   const int side = blockIdx.y;
   if (p.part[side] == nullptr) return;
-  const int eights = (p.R + 7) / 8;
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int eights = p.to[side].steps * 4;
+  const int64_t u = (int64_t)blockIdx.x * 64 + threadIdx.x;
   const int t = (int)(u % p.q.T), r = (int)(u / p.q.T) * 8;
   if (r >= eights * 8) return;
   const int a = p.q.of(t);
   if (a < 0) return;
   float v[8] = {};
-  for (int s = 0; s < p.slices[side]; ++s) {
-    const float* from = p.part[side] + ((size_t)s * p.q.T + t) * p.R + r;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (r + j < p.R) v[j] += from[j];
-  }
+  add_parts(p.part[side] + (size_t)t * p.R + r, p.slices[side], (size_t)p.q.T * p.R, p.R - r, v);
   const float f = p.q.scale[a];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] *= f;
-  put_planes(p.to[side], p.q.T, p.R, t, r, v);
+  put_planes(p.to[side], p.R, t, r, v);
 }
 
 struct WideArgs {
   Requests q;
   const float* part;                  // [slices, T, R] (wide_kernel)
-  Planes from;                        // (wide_run_kernel)
-  const uint16_t *w, *base;           // w [n, C, R], or [n, R, C] (ACROSS); base [T, C] or NULL
+  const uint16_t* rank;               // Planes::rank (wide_run_kernel)
+  const uint16_t *w, *base;           // w [n, C, R], or [n, R, C] (TURNED); base [T, C] or NULL
   uint16_t* out;                      // [T, C]
   int C, R, slices, turns;
 };
 
-// out[t][c] = base[t][c] + s sum_r h[t][r] w[a][c][r]. A wave has 64 columns (ACROSS: 128), a lane eight of every 32 of them: a load or store of the
-// wave takes 64 bytes next to each other of 16 rows (16 pieces with gaps between them before: 16384 rows, rank 64, 154 us).
-template <class A, bool ACROSS>
+// out[t][c] = base[t][c] + s sum_r h[t][r] w[a][c][r] of 16 tokens and 128 columns, of which a lane has 32 of token l % 16 next to each other in the products. Base
+// and out are loaded and stored transposed among four lanes: piece j of lane l is 16 bytes of token 4 (l / 4 % 4) + j.
+template <class A, bool TURNED>
 struct Wide {
-  static constexpr int NT = ACROSS ? 8 : 4;    // instructions side by side
-  static constexpr int COLS = NT * 16;
+  static constexpr int COLS = 128;
   const WideArgs& p;
   int c0, col, quad, c, have;
   bool whole;
   __device__ __forceinline__ Wide(const WideArgs& args, int first, int lane) : p(args), c0(first), col(lane & 15), quad(lane >> 4) {
-    c = c0 + quad * 8;
+    c = c0 + quad * 32 + (col & 3) * 8;      // of a load or store
     have = p.C - c;
     whole = c0 + COLS <= p.C;
   }
+  __device__ __forceinline__ int token(int j) const { return (col & 12) + j; }
   // Weights of 32 r from r0 on, in bf16. r past R meets values of 0: the row's last ones again, so that nothing but the lane's own column enters.
-  __device__ __forceinline__ void weights(int a, int r0, u4 (&wh)[NT], u4 (&wl)[NT]) const {
+  __device__ __forceinline__ void weights(int a, int r0, u4 (&wh)[8], u4 (&wl)[8]) const {
     const uint16_t* w = p.w + (size_t)a * p.R * p.C;
     const int r = r0 + quad * 8;
-    if constexpr (ACROSS) {
+    if constexpr (TURNED) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int at = c0 + ((col & 3) * 4 + (col >> 2)) * 8;     // result row 4 quad + e: the lane's eight of piece e
+        const int at = c0 + col * 8;     // result row 4 quad + e of instruction j: value 8 e + j of the lane's 32
         const uint16_t* from = w + (size_t)min(r + j, p.R - 1) * p.C + at;
         wh[j] = whole ? load8(from) : load8(from, p.C - at);
       }
       transpose8(wh);
     } else {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        // result row 4 quad + e of instruction j: value 4 j + e of the lane's
-        const uint16_t* from = w + (size_t)min(c0 + (j >> 1) * 32 + (col >> 2) * 8 + (j & 1) * 4 + (col & 3), p.C - 1) * p.R;
+      for (int j = 0; j < 8; ++j) {      // value 4 j + e
+        const uint16_t* from = w + (size_t)min(c0 + (col >> 2) * 32 + j * 4 + (col & 3), p.C - 1) * p.R;
         wh[j] = p.R % 8 == 0 ? load8(from + min(r, p.R - 8)) : load8(from + r, p.R - r);
       }
     }
     if constexpr (A::HALF)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) to_bf16<A>(wh[j], wh[j], wl[j]);
+      for (int j = 0; j < 8; ++j) to_bf16<A>(wh[j], wh[j], wl[j]);
   }
-  __device__ __forceinline__ void base(int t, bool want, u4 (&b)[NT / 2]) const {
-    const uint16_t* from = p.base + (size_t)t * p.C + c;
+  // base of the tokens t + 0 .. 15 that `want` says (bits)
+  __device__ __forceinline__ void base(int t, uint32_t want, u4 (&b)[4]) const {
 #pragma unroll
-    for (int i = 0; i < NT / 2; ++i) {
-      b[i] = u4{0, 0, 0, 0};
-      if (want && p.base != nullptr) b[i] = whole ? load8(from + 32 * i) : load8(from + 32 * i, have - 32 * i);
+    for (int j = 0; j < 4; ++j) {
+      b[j] = u4{0, 0, 0, 0};
+      if (p.base != nullptr && ((want >> token(j)) & 1)) {
+        const uint16_t* from = p.base + (size_t)(t + token(j)) * p.C + c;
+        b[j] = whole ? load8(from) : load8(from, have);
+      }
     }
   }
-  __device__ __forceinline__ void put(int t, const f4 (&acc)[NT], const u4 (&b)[NT / 2]) const {
-    uint16_t* to = p.out + (size_t)t * p.C + c;
+  __device__ __forceinline__ void put(int t, uint32_t want, const f4 (&acc)[8], u4 (&b)[4]) const {
+    if (p.base != nullptr) quad_transpose(b);
+    u4 o[4];
 #pragma unroll
-    for (int i = 0; i < NT / 2; ++i) {
-      u4 o;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        // value u of the lane: ACROSS, of instruction u % 8, else u / 4
         const int u = 8 * i + 2 * w;
-        const float v0 = ACROSS ? acc[u % 8][u / 8] : acc[u / 4][u % 4], v1 = ACROSS ? acc[u % 8 + 1][u / 8] : acc[u / 4][u % 4 + 1];
-        o[w] = p.base != nullptr ? A::pack(v0 + A::lo(b[i][w]), v1 + A::hi(b[i][w])) : A::pack(v0, v1);
+        const float v0 = TURNED ? acc[u % 8][u / 8] : acc[u / 4][u % 4], v1 = TURNED ? acc[u % 8 + 1][u / 8] : acc[u / 4][u % 4 + 1];
+        o[i][w] = p.base != nullptr ? A::pack(v0 + A::lo(b[i][w]), v1 + A::hi(b[i][w])) : A::pack(v0, v1);
       }
-      if (whole) __builtin_memcpy(to + 32 * i, &o, 16);
-      else store8(to + 32 * i, o, have - 32 * i);
-    }
-  }
-  // a row without an adapter: the base as it is, bit for bit
-  __device__ __forceinline__ void copy(int t) const {
-    if ((const void*)p.out == (const void*)p.base) return;
+    quad_transpose(o);
 #pragma unroll
-    for (int i = 0; i < NT / 2; ++i) {
-      u4 v = {0, 0, 0, 0};
-      if (p.base != nullptr) v = load8(p.base + (size_t)t * p.C + c + 32 * i, have - 32 * i);
-      store8(p.out + (size_t)t * p.C + c + 32 * i, v, have - 32 * i);
-    }
+    for (int j = 0; j < 4; ++j)
+      if ((want >> token(j)) & 1) {
+        uint16_t* to = p.out + (size_t)(t + token(j)) * p.C + c;
+        if (whole) __builtin_memcpy(to, &o[j], 16);
+        else store8(to, o[j], have);
+      }
+  }
+  // rows without an adapter: the base as it is, bit for bit
+  __device__ __forceinline__ void copy(int t, uint32_t want) const {
+    if ((const void*)p.out == (const void*)p.base || want == 0) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if ((want >> token(j)) & 1) {
+        const size_t at = (size_t)(t + token(j)) * p.C + c;
+        u4 v = {0, 0, 0, 0};
+        if (p.base != nullptr) v = load8(p.base + at, have);
+        store8(p.out + at, v, have);
+      }
   }
 };
 
 // Few rows: 16 tokens a tile, their narrow values added up from the parts and split in LDS; a tile's adapters are dealt to `turns` blocks.
-template <class A, bool ACROSS>
-__global__ __launch_bounds__(WAVES * 64) void wide_kernel(WideArgs p) {
-  typedef Wide<A, ACROSS> W;
+template <class A>
+__global__ __launch_bounds__(WIDE_WAVES * 64) void wide_kernel(WideArgs p) {
+  typedef Wide<A, false> W;
   extern __shared__ __attribute__((aligned(16))) uint16_t lds[];   // [2][16][stride]: hi, lo of s h
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int steps = (p.R + 31) / 32, stride = steps * 32 + 8;
-  const int tiles = (p.q.T + 15) / 16, chunks = (p.C + WAVES * W::COLS - 1) / (WAVES * W::COLS);
+  const int tiles = (p.q.T + 15) / 16, chunks = (p.C + WIDE_WAVES * W::COLS - 1) / (WIDE_WAVES * W::COLS);
   const int chunk = blockIdx.x % chunks, tile = (blockIdx.x / chunks) % tiles, z = blockIdx.x / chunks / tiles;
   const int t0 = tile * 16;
   const int mine = lane < 16 ? p.q.of(t0 + lane) : -1;
-  for (int u = threadIdx.x; u < 16 * steps * 4; u += WAVES * 64) {   // eight values a thread
+  const W w(p, (chunk * WIDE_WAVES + wave) * W::COLS, lane);
+  // the first adapter's weights and base are on their way meanwhile
+  int early = -1;
+  u4 wh[8], wl[8], b[4];
+  each_adapter(mine, z, p.turns, [&](int a, uint64_t has) {
+    if (early >= 0 || w.c0 >= p.C) return;
+    early = a;
+    w.weights(a, 0, wh, wl);
+    w.base(t0, (uint32_t)has, b);
+  });
+  for (int u = threadIdx.x; u < 16 * steps * 4; u += WIDE_WAVES * 64) {   // eight values a thread
     const int row = u / (steps * 4), r = (u - row * (steps * 4)) * 8, t = t0 + row;
     const int a = p.q.of(t);
     float v[8] = {};
     if (a >= 0) {
       const float f = p.q.scale[a];
-      const float* from = p.part + (size_t)t * p.R + r;
-      const size_t next = (size_t)p.q.T * p.R;
-      if (r + 8 <= p.R) {
-#pragma unroll 8
-        for (int s = 0; s < p.slices; ++s) {
-          f4 q[2];
-          __builtin_memcpy(q, from + s * next, 32);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] += q[j / 4][j % 4];
-        }
-      } else {
-        for (int s = 0; s < p.slices; ++s)
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (r + j < p.R) v[j] += from[s * next + j];
-      }
+      add_parts(p.part + (size_t)t * p.R + r, p.slices, (size_t)p.q.T * p.R, p.R - r, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= f;
     }
@@ -356,101 +411,118 @@ __global__ __launch_bounds__(WAVES * 64) void wide_kernel(WideArgs p) {
     *reinterpret_cast<u4*>(lds + (size_t)(16 + row) * stride + r) = vl;
   }
   __syncthreads();
-  const W w(p, (chunk * WAVES + wave) * W::COLS, lane);
   if (w.c0 >= p.C) return;
-  const int own = __shfl(mine, col, 64);
-  if (z == 0 && own < 0 && t0 + col < p.q.T) w.copy(t0 + col);
-  each_adapter(mine, z, p.turns, [&](int a, uint64_t) {
-    u4 b[W::NT / 2];
-    w.base(t0 + col, own == a, b);
-    f4 acc[W::NT] = {};
+  if (z == 0) w.copy(t0, (uint32_t)__ballot(lane < 16 && mine < 0 && t0 + lane < p.q.T));
+  each_adapter(mine, z, p.turns, [&](int a, uint64_t has) {
+    if (a != early) w.base(t0, (uint32_t)has, b);
+    f4 acc[8] = {};
     for (int s = 0; s < steps; ++s) {
-      u4 wh[W::NT], wl[W::NT];
-      w.weights(a, s * 32, wh, wl);
+      if (a != early || s > 0) w.weights(a, s * 32, wh, wl);
       const u4 qh = *reinterpret_cast<const u4*>(lds + (size_t)col * stride + s * 32 + quad * 8);
       const u4 ql = *reinterpret_cast<const u4*>(lds + (size_t)(16 + col) * stride + s * 32 + quad * 8);
 #pragma unroll
-      for (int j = 0; j < W::NT; ++j) acc[j] = mul_split<A>(wh[j], wl[j], qh, ql, acc[j]);
+      for (int j = 0; j < 8; ++j) acc[j] = mul_split<A>(wh[j], wl[j], qh, ql, acc[j]);
     }
-    if (own == a) w.put(t0 + col, acc, b);
+    w.put(t0, (uint32_t)has, acc, b);
   });
 }
 
 // Many rows: a block has up to RUN tokens, 16 at a time; a wave keeps the weights of its columns in registers for as long as the adapter stays the same (R up to
-// 32 STEPS; `parts` times that are gone through one after the other, loaded anew). Values and base of the next 16 tokens are on their way
-// while these are multiplied. Bound by base and out: R of 64 takes 16 instructions (256 cycles of one of four units) for 4 KB of them.
-template <class A, bool ACROSS, int STEPS>
+// 32 STEPS; `parts` times that are gone through one after the other, loaded anew). Bound by base and out: R of 64 takes 32 instructions
+// (512 cycles of one of four units) for 8 KB of them. Where the whole run has one adapter, values and base of the AHEAD 16 tokens to come are on
+// their way while some are multiplied.
+template <class A, bool TURNED, int STEPS>
 __global__ __launch_bounds__(WAVES * 64) void wide_run_kernel(WideArgs p, int parts, int run) {
-  typedef Wide<A, ACROSS> W;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-  const int chunks = (p.C + WAVES * W::COLS - 1) / (WAVES * W::COLS);
+  typedef Wide<A, TURNED> W;
+  constexpr int AHEAD = 2;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int chunks = (p.C + WAVES * W::COLS - 1) / (WAVES * W::COLS), steps = (p.R + 31) / 32;
   const int chunk = blockIdx.x % chunks, t0 = blockIdx.x / chunks * run;
   const W w(p, (chunk * WAVES + wave) * W::COLS, lane);
   if (w.c0 >= p.C) return;
+  const int end = min(p.q.T, t0 + run);
   int of[RUN / 64];
+  const int first = p.q.of(t0);
+  bool same = first >= 0;
 #pragma unroll
-  for (int i = 0; i < RUN / 64; ++i) of[i] = i * 64 < run ? p.q.of(t0 + i * 64 + lane) : -1;
-  const int groups = min(run, p.q.T - t0 + 15) / 16;
-  const size_t plane = (size_t)p.q.T * p.from.stride_r;
+  for (int i = 0; i < RUN / 64; ++i) {
+    const int t = t0 + i * 64 + lane;
+    of[i] = t < end ? p.q.of(t) : -1;
+    same = same && (t >= end || of[i] == first);
+  }
+  const int groups = (end - t0 + 15) / 16;
+  auto in = [&](int g) { return end - t0 - g * 16 >= 16 ? 0xffffu : (1u << (end - t0 - g * 16)) - 1; };   // tokens of the group that there are
   struct Tokens {
-    u4 q[2][STEPS], b[W::NT / 2];
+    u4 q[2][STEPS], b[4];
   };
   auto values = [&](int g, int part, u4 (&q)[2][STEPS]) {
-    const uint16_t* from = p.from.rank + (size_t)min(t0 + g * 16 + col, p.q.T - 1) * p.from.stride_r;
+    const uint16_t* from = p.rank + ((size_t)(t0 / 16 + g) * steps * 128 + lane) * 8;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const int r = (part * STEPS + s) * 32 + quad * 8;
-      q[0][s] = q[1][s] = u4{0, 0, 0, 0};
-      if (r < p.from.stride_r) {
-        q[0][s] = *reinterpret_cast<const u4*>(from + r);
-        q[1][s] = *reinterpret_cast<const u4*>(from + plane + r);
-      }
+      const int at = min(part * STEPS + s, steps - 1);     // past the last step the weights are
+      q[0][s] = *reinterpret_cast<const u4*>(from + (size_t)at * 1024);
+      q[1][s] = *reinterpret_cast<const u4*>(from + (size_t)at * 1024 + 512);
+      if (part * STEPS + s >= steps) q[0][s] = q[1][s] = u4{0, 0, 0, 0};
     }
   };
-  auto load = [&](int g, Tokens& k) {
-    values(g, 0, k.q);
-    w.base(t0 + g * 16 + col, t0 + g * 16 + col < p.q.T, k.b);
+  u4 wh[STEPS][8], wl[STEPS][8];
+  auto multiply = [&](const u4 (&q)[2][STEPS], f4 (&acc)[8]) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = mul_split<A>(wh[s][j], wl[s][j], q[0][s], q[1][s], acc[j]);
   };
-  u4 wh[STEPS][W::NT], wl[STEPS][W::NT];
+  if (__all(same) && parts == 1) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) w.weights(first, s * 32, wh[s], wl[s]);
+    Tokens k[AHEAD];
+    auto load = [&](int g, Tokens& v) {
+      values(g, 0, v.q);
+      w.base(t0 + g * 16, in(g), v.b);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i < groups) load(i, k[i]);
+    for (int g = 0; g < groups; g += AHEAD)
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (g + i < groups) {
+          f4 acc[8] = {};
+          multiply(k[i].q, acc);
+          w.put(t0 + (g + i) * 16, in(g + i), acc, k[i].b);
+          if (g + i + AHEAD < groups) load(g + i + AHEAD, k[i]);
+        }
+    return;
+  }
   int held = -1;
-  auto compute = [&](int g, Tokens& k) {
+  for (int g = 0; g < groups; ++g) {
     int mine = 0;
 #pragma unroll
     for (int i = 0; i < RUN / 64; ++i)
       if (g / 4 == i) mine = of[i];
-    mine = __shfl(mine, (g & 3) * 16 + col, 64);
-    const int t = t0 + g * 16 + col;
-    if (mine < 0 && t < p.q.T) w.copy(t);
-    each_adapter(mine, 0, 1, [&](int a, uint64_t) {
-      f4 acc[W::NT] = {};
+    mine = __shfl(mine, (g & 3) * 16 + (lane & 15), 64);
+    w.copy(t0 + g * 16, (uint32_t)__ballot(mine < 0) & in(g));
+    each_adapter(mine, 0, 1, [&](int a, uint64_t has) {
+      Tokens k;
+      w.base(t0 + g * 16, (uint32_t)has & 0xffff, k.b);
+      f4 acc[8] = {};
       for (int part = 0; part < parts; ++part) {
+        values(g, part, k.q);
         if (a != held || parts > 1) {
 #pragma unroll
           for (int s = 0; s < STEPS; ++s) w.weights(a, (part * STEPS + s) * 32, wh[s], wl[s]);
           held = a;
         }
-        if (parts > 1) values(g, part, k.q);
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-          for (int j = 0; j < W::NT; ++j) acc[j] = mul_split<A>(wh[s][j], wl[s][j], k.q[0][s], k.q[1][s], acc[j]);
+        multiply(k.q, acc);
       }
-      if (mine == a) w.put(t, acc, k.b);
+      w.put(t0 + g * 16, (uint32_t)has & 0xffff, acc, k.b);
     });
-  };
-  Tokens k[2];
-  load(0, k[0]);
-  for (int g = 0; g < groups; g += 2) {
-    if (g + 1 < groups) load(g + 1, k[1]);
-    compute(g, k[0]);
-    if (g + 2 < groups) load(g + 2, k[0]);
-    if (g + 1 < groups) compute(g + 1, k[1]);
   }
 }
 
 struct OuterSide {
   const uint16_t* v;        // [T, C]
-  const uint16_t* rows;     // narrow values along the rows, hi; lo behind
+  const uint16_t* rows;     // Planes::rows
   void* out;                // fp32 parts [splits, n, R, C] (flip: [splits, n, C, R]), or the result itself
   int C, flip, blocks;      // blocks of 512 columns
 };
@@ -458,8 +530,7 @@ struct OuterSide {
 struct OuterArgs {
   Requests q;
   OuterSide side[2];
-  int64_t stride_t;
-  int R, splits, per_split, direct;   // per_split: tokens, a multiple of 2 STAGE
+  int R, splits, per_split, direct, tiles;   // per_split: tokens, a multiple of 2 STAGE
 };
 
 // out[a][r][c] = s sum over the rows t of adapter a of q[t][r] v[t][c], 16 RT of the r. A wave has 128 columns and one half of the block's rows: eight rows of
@@ -478,10 +549,10 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
   f4 acc[RT][8] = {};
   const int64_t begin = (int64_t)split * p.per_split + (wave >> 2) * (p.per_split / 2);
   const int end = (int)min((int64_t)p.q.T, begin + p.per_split / 2);
-  const uint16_t* q[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) q[r] = side.rows + (size_t)min(r0 + r * 16 + col, p.R - 1) * p.stride_t + quad * 8;
-  const size_t plane = (size_t)p.R * p.stride_t;
+  // values of 32 rows, r tile r
+  auto value = [&](int t, int r, int lo) {
+    return *reinterpret_cast<const u4*>(side.rows + (((size_t)(t >> 5) * p.tiles + min((r0 >> 4) + r, p.tiles - 1)) * 128 + 64 * lo + lane) * 8);
+  };
   if (c0 < side.C)
     for (int t0 = (int)min(begin, (int64_t)p.q.T); t0 < end; t0 += STAGE) {
       const uint64_t first = __ballot(t0 + lane < end && p.q.of(t0 + lane) == a), next = __ballot(t0 + 64 + lane < end && p.q.of(t0 + 64 + lane) == a);
@@ -514,8 +585,8 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
           u4 qh[RT], ql[RT];
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
-            qh[r] = *reinterpret_cast<const u4*>(q[r] + t0 + st * 32);
-            ql[r] = *reinterpret_cast<const u4*>(q[r] + plane + t0 + st * 32);
+            qh[r] = value(t0 + st * 32, r, 0);
+            ql[r] = value(t0 + st * 32, r, 1);
           }
           if (st + 1 < STAGE / 32) load(st + 1, v[(st + 1) & 1]);
           multiply(v[st & 1], qh, ql);
@@ -537,8 +608,8 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          qh[r] = *reinterpret_cast<const u4*>(q[r] + t0 + st * 32) & keep;
-          ql[r] = *reinterpret_cast<const u4*>(q[r] + plane + t0 + st * 32) & keep;
+          qh[r] = value(t0 + st * 32, r, 0) & keep;
+          ql[r] = value(t0 + st * 32, r, 1) & keep;
         }
         multiply(v, qh, ql);
       }
@@ -610,8 +681,7 @@ struct Side {                 // a narrow product
 struct Plan {
   int tm, turns, run;         // run: many rows
   Side h, g;
-  int stride_r, splits, per_split, rt;
-  int64_t stride_t;
+  int steps, tiles, splits, per_split, rt;
   size_t da_bytes, db_bytes, total;
 };
 
@@ -621,13 +691,13 @@ size_t bytes_of(size_t n) { return hdmoe_align_up(n, 256); }
 
 constexpr int MANY_ROWS = 512;   // from here on `wide` keeps its weights over runs of tokens
 
-// The contraction is cut over blocks until the card has about one a CU, in slices of at least two steps of each wave; `whole`: not at all.
+// The contraction is cut over blocks until the card has about one a CU, in slices of a block of each wave at least; `whole`: not at all.
 void cut(int tiles, int turns, int K, int rblocks, bool whole, Side& s) {
-  const int most = div_up(K, 2 * NARROW_WAVES * K_STEP);
+  const int most = div_up(K, NARROW_WAVES * K_BLOCK);
   int want = whole ? 1 : div_up(HDMOE_NUM_CU, (int64_t)tiles * turns * rblocks);
   if (want > most) want = most;
   if (want > 8) want = 8;
-  s.slice = div_up(div_up(K, want), NARROW_WAVES * K_STEP) * NARROW_WAVES * K_STEP;
+  s.slice = div_up(div_up(K, want), NARROW_WAVES * K_BLOCK) * NARROW_WAVES * K_BLOCK;
   s.slices = div_up(K, s.slice);
 }
 
@@ -636,15 +706,16 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   const int rows_per = a.rows / a.requests;
   p.run = a.rows >= MANY_ROWS;
   // tokens of a tile of `narrow`: 16, and more where there are tiles for every CU all the same and a tile's rows share an adapter
-  p.tm = rows_per < 64 || a.rows < 32 * HDMOE_NUM_CU ? 1 : a.rows < 64 * HDMOE_NUM_CU || a.R > 64 ? 2 : 4;
-  const int tile = 16 * p.tm, distinct = div_up(tile, rows_per);
-  p.turns = distinct < a.n ? distinct : a.n;
+  p.tm = rows_per < 64 || a.rows < 32 * HDMOE_NUM_CU ? 1 : a.rows < 64 * HDMOE_NUM_CU || a.R > 32 ? 2 : 4;
+  const int tile = 16 * p.tm;
+  p.turns = div_up(tile, rows_per);          // adapters of a tile at most, as tiles go
+  if (p.turns > a.n) p.turns = a.n;
+  if (p.turns > a.requests) p.turns = a.requests;
   const int tiles = div_up(a.rows, tile);
   cut(tiles, p.turns, a.K, div_up(a.R, 128), p.run && !backward, p.h);
-  p.stride_r = (a.R + 7) / 8 * 8;
-  p.stride_t = (int64_t)div_up(a.rows, STAGE) * STAGE;
-  const size_t part = (size_t)a.rows * a.R * sizeof(float), rank = bytes_of((size_t)2 * a.rows * p.stride_r * 2);
-  const size_t rows = bytes_of((size_t)2 * a.R * p.stride_t * 2);
+  p.steps = div_up(a.R, 32), p.tiles = div_up(a.R, 16);
+  const size_t part = (size_t)a.rows * a.R * sizeof(float), rank = (size_t)div_up(a.rows, 16) * p.steps * 2048;
+  const size_t rows = (size_t)div_up(a.rows, STAGE) * (STAGE / 32) * p.tiles * 2048;
   if (!backward) {
     if (p.run) p.h.rank = rank;
     else p.h.part = bytes_of(part * p.h.slices);
@@ -657,10 +728,10 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   p.h.rows = p.g.rows = rows;
   p.g.rank = rank;
   p.rt = a.R <= 16 ? 1 : 2;
-  // rows are cut over blocks until the card has one a CU, each with a run of 1024 at least: parts are written and read again
+  // rows are cut over blocks until the card has one a CU, each with 256 of them at least: parts are written and read again
   const int64_t blocks = (int64_t)(div_up(a.K, 512) + div_up(a.N, 512)) * a.n * div_up(a.R, 16 * p.rt);
   int splits = div_up(HDMOE_NUM_CU, blocks);
-  const int most = div_up(a.rows, 4 * STAGE);
+  const int most = div_up(a.rows, 2 * STAGE);
   if (splits > most) splits = most;
   p.per_split = div_up(div_up(a.rows, splits), 2 * STAGE) * 2 * STAGE;
   p.splits = div_up(a.rows, p.per_split);
@@ -672,39 +743,41 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   return p;
 }
 
-template <class A, bool ACROSS>
+template <class A, bool TURNED>
 void launch_narrow(const NarrowArgs& p, int tm, hipStream_t s) {
-  auto go = [&](auto rt, auto m) {
-    constexpr int RT = decltype(rt)::value, TM = decltype(m)::value;
-    const dim3 grid(div_up(p.q.T, 16 * TM) * p.slices * p.turns, div_up(p.R, 16 * RT));
-    hipLaunchKernelGGL((narrow_kernel<A, ACROSS, RT, TM>), grid, dim3(NARROW_WAVES * 64), 0, s, p);
-  };
   using std::integral_constant;
-  auto rt = [&](auto r) {
-    if (tm == 1) go(r, integral_constant<int, 1>());
-    else if constexpr (decltype(r)::value == 8) go(r, integral_constant<int, 2>());
-    else if (tm == 2) go(r, integral_constant<int, 2>());
-    else go(r, integral_constant<int, 4>());
+  auto go = [&](auto mode, auto rt) {
+    constexpr int MODE = decltype(mode)::value, RT = decltype(rt)::value;
+    auto tiles = [&](auto m) {
+      constexpr int TM = decltype(m)::value;
+      const dim3 grid(div_up(p.q.T, 16 * TM) * p.slices * p.turns, div_up(p.R, 16 * RT));
+      hipLaunchKernelGGL((narrow_kernel<A, MODE, RT, TM>), grid, dim3(NARROW_WAVES * 64), 0, s, p);
+    };
+    if (tm == 1) tiles(integral_constant<int, 1>());
+    else if constexpr (RT > 2) tiles(integral_constant<int, 2>());
+    else if (tm == 2) tiles(integral_constant<int, 2>());
+    else tiles(integral_constant<int, 4>());
   };
-  if constexpr (ACROSS) {
-    rt(integral_constant<int, 8>());
+  if constexpr (TURNED) {
+    if (p.R <= 32) go(integral_constant<int, ACROSS32>(), integral_constant<int, 2>());
+    else go(integral_constant<int, ACROSS>(), integral_constant<int, 8>());
   } else {
-    if (p.R <= 16) rt(integral_constant<int, 1>());
-    else if (p.R <= 32) rt(integral_constant<int, 2>());
-    else if (p.R <= 64) rt(integral_constant<int, 4>());
-    else rt(integral_constant<int, 8>());
+    if (p.R <= 16) go(integral_constant<int, ALONG>(), integral_constant<int, 1>());
+    else if (p.R <= 32) go(integral_constant<int, ALONG>(), integral_constant<int, 2>());
+    else if (p.R <= 64) go(integral_constant<int, ALONG>(), integral_constant<int, 4>());
+    else go(integral_constant<int, ALONG>(), integral_constant<int, 8>());
   }
 }
 
-template <class A, bool ACROSS>
+template <class A, bool TURNED>
 void launch_wide_run(const WideArgs& p, hipStream_t s) {
   auto go = [&](auto steps) {
     constexpr int STEPS = decltype(steps)::value;
     // runs as long as four blocks a CU allow
-    const int chunks = div_up(p.C, WAVES * Wide<A, ACROSS>::COLS);
+    const int chunks = div_up(p.C, WAVES * Wide<A, TURNED>::COLS);
     int run = div_up((int64_t)p.q.T * chunks, 4 * HDMOE_NUM_CU * 16) * 16;
     if (run > RUN) run = RUN;
-    hipLaunchKernelGGL((wide_run_kernel<A, ACROSS, STEPS>), dim3(chunks * div_up(p.q.T, run)), dim3(WAVES * 64), 0, s, p, div_up(p.R, 32 * STEPS), run);
+    hipLaunchKernelGGL((wide_run_kernel<A, TURNED, STEPS>), dim3(chunks * div_up(p.q.T, run)), dim3(WAVES * 64), 0, s, p, div_up(p.R, 32 * STEPS), run);
   };
   if (p.R <= 32) go(std::integral_constant<int, 1>());
   else go(std::integral_constant<int, 2>());
@@ -759,17 +832,17 @@ extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t st
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Requests q = requests_of(a);
   float* part = plan.run ? nullptr : static_cast<float*>(a->workspace);
-  const Planes planes = {plan.run ? static_cast<uint16_t*>(a->workspace) : nullptr, nullptr, plan.stride_r, 0};
+  const Planes planes = {plan.run ? static_cast<uint16_t*>(a->workspace) : nullptr, nullptr, plan.steps, plan.tiles};
   const NarrowArgs np = {q, bits(a->x), bits(a->a), part, planes, a->K, a->R, plan.h.slice, plan.h.slices, plan.turns};
-  const WideArgs wp = {q, part, planes, bits(a->b), bits(a->base), static_cast<uint16_t*>(a->out), a->N, a->R, plan.h.slices, plan.turns};
+  const WideArgs wp = {q, part, planes.rank, bits(a->b), bits(a->base), static_cast<uint16_t*>(a->out), a->N, a->R, plan.h.slices, plan.turns};
   typed(a->dtype, [&](auto t) {
     typedef decltype(t) A;
     launch_narrow<A, false>(np, plan.tm, s);
     if (plan.run) {
       launch_wide_run<A, false>(wp, s);
     } else {
-      const dim3 grid(div_up(a->N, WAVES * Wide<A, false>::COLS) * div_up(a->rows, 16) * plan.turns);
-      hipLaunchKernelGGL((wide_kernel<A, false>), grid, dim3(WAVES * 64), (size_t)2 * 16 * ((a->R + 31) / 32 * 32 + 8) * 2, s, wp);
+      const dim3 grid(div_up(a->N, WIDE_WAVES * Wide<A, false>::COLS) * div_up(a->rows, 16) * plan.turns);
+      hipLaunchKernelGGL(wide_kernel<A>, grid, dim3(WIDE_WAVES * 64), (size_t)2 * 16 * ((a->R + 31) / 32 * 32 + 8) * 2, s, wp);
     }
   });
   return hdmoe_check_launch("hdmoe_add_adapters");
@@ -802,14 +875,14 @@ extern "C" int hdmoe_add_adapters_backward(const hdmoe_adapter_args* a, hdmoe_st
   float* h = static_cast<float*>(take(plan.h.part));
   float* g = static_cast<float*>(take(plan.g.part));
   jp.part[0] = h, jp.part[1] = g;
-  jp.to[0] = {nullptr, static_cast<uint16_t*>(take(plan.h.rows)), plan.stride_r, plan.stride_t};
+  jp.to[0] = {nullptr, static_cast<uint16_t*>(take(plan.h.rows)), plan.steps, plan.tiles};
   uint16_t* grows = static_cast<uint16_t*>(take(plan.g.rows));
-  jp.to[1] = {static_cast<uint16_t*>(take(plan.g.rank)), grows, plan.stride_r, plan.stride_t};
+  jp.to[1] = {static_cast<uint16_t*>(take(plan.g.rank)), grows, plan.steps, plan.tiles};
   const NarrowArgs hp = {q, bits(a->x), bits(a->a), h, jp.to[0], a->K, a->R, plan.h.slice, plan.h.slices, plan.turns};
   const NarrowArgs gp = {q, bits(a->dy), bits(a->b), g, jp.to[1], a->N, a->R, plan.g.slice, plan.g.slices, plan.turns};
-  const WideArgs wp = {q, nullptr, jp.to[1], bits(a->a), nullptr, static_cast<uint16_t*>(a->dx), a->K, a->R, 1, 1};
+  const WideArgs wp = {q, nullptr, jp.to[1].rank, bits(a->a), nullptr, static_cast<uint16_t*>(a->dx), a->K, a->R, 1, 1};
   OuterArgs op = {};
-  op.q = q, op.R = a->R, op.splits = plan.splits, op.per_split = plan.per_split, op.direct = plan.splits == 1, op.stride_t = plan.stride_t;
+  op.q = q, op.R = a->R, op.splits = plan.splits, op.per_split = plan.per_split, op.direct = plan.splits == 1, op.tiles = plan.tiles;
   float* da = static_cast<float*>(take(plan.da_bytes));
   float* db = static_cast<float*>(take(plan.db_bytes));
   op.side[0] = {bits(a->x), jp.to[1].rows, op.direct ? a->da : da, a->K, 0, div_up(a->K, 512)};
@@ -821,7 +894,7 @@ extern "C" int hdmoe_add_adapters_backward(const hdmoe_adapter_args* a, hdmoe_st
     launch_narrow<A, false>(hp, plan.tm, s);
     launch_narrow<A, true>(gp, plan.tm, s);
     if (h != nullptr || g != nullptr)
-      hipLaunchKernelGGL(join_kernel, dim3(div_up((int64_t)a->rows * div_up(a->R, 8), 256), 2), dim3(256), 0, s, jp);
+      hipLaunchKernelGGL(join_kernel, dim3(div_up((int64_t)a->rows * plan.steps * 4, 64), 2), dim3(64), 0, s, jp);
     launch_wide_run<A, true>(wp, s);
     if (plan.rt == 1) hipLaunchKernelGGL((outer_kernel<A, 1>), grid, dim3(512), 0, s, op);
     else hipLaunchKernelGGL((outer_kernel<A, 2>), grid, dim3(512), 0, s, op);

@@ -75,6 +75,59 @@ __device__ __forceinline__ void transpose8(u4 (&v)[8]) {
   for (int j = 0; j < 8; ++j) v[j] = o[j];
 }
 
+// v[i] of lane c <-> v[c] of lane i among four neighbouring lanes: 32 instructions. The matrix instructions want one row a lane and its neighbour's
+// next to it, memory wants neighbouring lanes on neighbouring addresses: a load or store whose four neighbours take 64 bytes of one row goes through
+// the address unit four times as fast as one where every lane has a row of its own (62 accesses each, counted; 16384 x 6912 in and out, rank 64: 147 us).
+__device__ __forceinline__ void quad_transpose(u4 (&v)[4]) {
+  const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int a = (int)v[i][w], b = (int)v[i + 1][w];
+      const int a1 = __builtin_amdgcn_mov_dpp(a, 0xb1, 0xf, 0xf, true), b1 = __builtin_amdgcn_mov_dpp(b, 0xb1, 0xf, 0xf, true);   // the lane's neighbour in its pair
+      v[i][w] = (uint32_t)(odd ? b1 : a);
+      v[i + 1][w] = (uint32_t)(odd ? b : a1);
+    }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int a = (int)v[i][w], b = (int)v[i + 2][w];
+      const int a2 = __builtin_amdgcn_mov_dpp(a, 0x4e, 0xf, 0xf, true), b2 = __builtin_amdgcn_mov_dpp(b, 0x4e, 0xf, 0xf, true);   // in the other pair
+      v[i][w] = (uint32_t)(high ? b2 : a);
+      v[i + 2][w] = (uint32_t)(high ? b : a2);
+    }
+}
+
+// v[i] of lane l <-> v[c] of lane l - 4 c + 4 i, c = l / 4 % 4: the same among lanes four apart.
+__device__ __forceinline__ void row_transpose(u4 (&v)[4]) {
+  const bool odd = threadIdx.x & 4, high = threadIdx.x & 8;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int a = (int)v[i][w], b = (int)v[i + 1][w];
+      const int a1 = __builtin_amdgcn_mov_dpp(a, 0x104, 0xf, 0xf, true), b1 = __builtin_amdgcn_mov_dpp(b, 0x114, 0xf, 0xf, true);   // of lane l + 4, l - 4
+      v[i][w] = (uint32_t)(odd ? b1 : a);
+      v[i + 1][w] = (uint32_t)(odd ? b : a1);
+    }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int a = (int)v[i][w], b = (int)v[i + 2][w];
+      const int a2 = __builtin_amdgcn_mov_dpp(a, 0x128, 0xf, 0xf, true), b2 = __builtin_amdgcn_mov_dpp(b, 0x128, 0xf, 0xf, true);   // l + 8 or l - 8
+      v[i][w] = (uint32_t)(high ? b2 : a);
+      v[i + 2][w] = (uint32_t)(high ? b : a2);
+    }
+}
+
+// Operands of 16 rows and 128 k: lane l loads 16 bytes of row 4 i + l / 4 % 4, k = 8 (4 (l / 16) + l % 4), i = 0 .. 3; transposed, instruction n has
+// k = 32 (l / 16) + 8 n .. + 7 of row 4 (l % 4) + l / 4 % 4 in lane l. row_of(l % 16) is that row.
+constexpr int K_BLOCK = 128;
+__device__ __forceinline__ int row_of(int col) { return (col & 3) * 4 + (col >> 2); }
+
 // Two fp32 values as packed bf16 pairs, hi + lo.
 __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = HdmoeBf16::pack(a, b);

@@ -15,8 +15,8 @@ using namespace lowrank;
 
 namespace {
 
-constexpr int WAVES = 4;
-constexpr int K_STEP = 64;
+constexpr int WAVES = 4;         // of the backward kernel
+constexpr int SCORE_WAVES = 8;
 constexpr int STAGE = 64;       // tokens whose dz a block of the backward kernel holds
 constexpr int LANES_E = 16;     // experts, filled up
 
@@ -37,34 +37,39 @@ struct BalanceArgs {
 
 // Scores of 16 TM tokens of one sequence and their sums. The block's waves take steps along D in turn; subtile m of the sums is wave m's.
 template <class A, int TM>
-__global__ __launch_bounds__(WAVES * 64) void gate_balance_kernel(BalanceArgs p) {
-  __shared__ f4 joined[WAVES][TM][64];
+__global__ __launch_bounds__(SCORE_WAVES * 64) void gate_balance_kernel(BalanceArgs p) {
+  __shared__ f4 joined[SCORE_WAVES][TM][64];
   __shared__ TileSums part[TM];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int seq = blockIdx.x / p.tiles_per_seq, l0 = (blockIdx.x - seq * p.tiles_per_seq) * 16 * TM;
   const int t0 = seq * p.length + l0;
   f4 acc[TM] = {};
-  const uint16_t* wr = p.w + (size_t)min(col, p.E - 1) * p.D;
-  const uint16_t* rows[TM];
-#pragma unroll
-  for (int m = 0; m < TM; ++m) rows[m] = p.x + (size_t)(seq * p.length + min(l0 + m * 16 + col, p.length - 1)) * p.D;
+  const int lane_row = col >> 2, lane_k = (quad * 4 + (col & 3)) * 8;      // of a load
   auto step = [&](int k0, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
-    const int k = k0 + quad * 8;     // 64 bytes of a row next to each other
-    u4 wv[2], xv[TM][2];
+    const int k = k0 + lane_k;
+    const bool on = WHOLE || k < p.D;             // D is a multiple of 8
+    u4 wv[4], xv[TM][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      wv[i] = WHOLE ? load8(wr + k + 32 * i) : load8(wr + k + 32 * i, p.D - k - 32 * i);
+    for (int i = 0; i < 4; ++i) {
+      wv[i] = u4{0, 0, 0, 0};
+      if (on) wv[i] = load8(p.w + (size_t)min(i * 4 + lane_row, p.E - 1) * p.D + k);
 #pragma unroll
-      for (int m = 0; m < TM; ++m) xv[m][i] = WHOLE ? load8(rows[m] + k + 32 * i) : load8(rows[m] + k + 32 * i, p.D - k - 32 * i);
+      for (int m = 0; m < TM; ++m) {
+        xv[m][i] = u4{0, 0, 0, 0};
+        if (on) xv[m][i] = load8(p.x + (size_t)(seq * p.length + min(l0 + m * 16 + i * 4 + lane_row, p.length - 1)) * p.D + k);
+      }
     }
+    quad_transpose(wv);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int m = 0; m < TM; ++m) quad_transpose(xv[m]);
 #pragma unroll
-      for (int m = 0; m < TM; ++m) acc[m] = A::mul(wv[i], xv[m][i], acc[m]);
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int m = 0; m < TM; ++m) acc[m] = A::mul(wv[n], xv[m][n], acc[m]);
   };
-  int k0 = wave * K_STEP;
-  for (; k0 + K_STEP <= p.D; k0 += WAVES * K_STEP) step(k0, std::true_type());
+  int k0 = wave * K_BLOCK;
+  for (; k0 + K_BLOCK <= p.D; k0 += SCORE_WAVES * K_BLOCK) step(k0, std::true_type());
   if (k0 < p.D) step(k0, std::false_type());
 #pragma unroll
   for (int m = 0; m < TM; ++m) joined[wave][m][lane] = acc[m];
@@ -72,20 +77,20 @@ __global__ __launch_bounds__(WAVES * 64) void gate_balance_kernel(BalanceArgs p)
   if (wave < TM) {
     f4 z = {};
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) z += joined[w][wave][lane];
-    // the lane's token has its 16 logits in four lanes, 16 apart
-    const int t = t0 + wave * 16 + col;
-    const bool in = l0 + wave * 16 + col < p.length;
+    for (int w = 0; w < SCORE_WAVES; ++w) z += joined[w][wave][lane];
+    // token row_of(col), experts row_of(4 quad + i) = 4 i + quad: a token has its 16 logits in four lanes, 16 apart
+    const int t = t0 + wave * 16 + row_of(col);
+    const bool in = l0 + wave * 16 + row_of(col) < p.length;
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (quad * 4 + i < p.E) top = fmaxf(top, z[i]);
+      if (i * 4 + quad < p.E) top = fmaxf(top, z[i]);
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     float sum = 0.0f, s[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s[i] = quad * 4 + i < p.E ? expf(z[i] - top) : 0.0f;
+      s[i] = i * 4 + quad < p.E ? expf(z[i] - top) : 0.0f;
       sum += s[i];
     }
     sum += __shfl_xor(sum, 16, 64);
@@ -95,15 +100,15 @@ __global__ __launch_bounds__(WAVES * 64) void gate_balance_kernel(BalanceArgs p)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       s[i] /= sum;
-      const int e = quad * 4 + i;
+      const int e = i * 4 + quad;
       if (in && e < p.E) p.scores[(size_t)t * p.E + e] = s[i];
       if (!counts) s[i] = 0.0f;
     }
     if (counts)
       for (int j = 0; j < p.k; ++j) {
-        const int e = p.idx[(size_t)t * p.k + j] - quad * 4;
+        const int e = p.idx[(size_t)t * p.k + j];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] += e == i;
+        for (int i = 0; i < 4; ++i) c[i] += e == i * 4 + quad;
       }
     int n = counts;
 #pragma unroll
@@ -117,7 +122,7 @@ __global__ __launch_bounds__(WAVES * 64) void gate_balance_kernel(BalanceArgs p)
     }
     if (col == 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[wave].p[quad * 4 + i] = s[i], part[wave].c[quad * 4 + i] = c[i];
+      for (int i = 0; i < 4; ++i) part[wave].p[i * 4 + quad] = s[i], part[wave].c[i * 4 + quad] = c[i];
       if (quad == 0) part[wave].n = n;
     }
   }
@@ -226,8 +231,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void gate_balance_backward_kernel(Ba
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int e = (quad >> 1) * 8 + j;
-    const int at = c0 + ((col & 3) * 4 + (col >> 2)) * 8;   // result row 4 quad + e: the lane's eight of every 32 columns
-    wh[j] = at < p.D && e < p.E ? load8(p.w + (size_t)e * p.D + at) : u4{0, 0, 0, 0};
+    wh[j] = mine && e < p.E ? load8(p.w + (size_t)e * p.D + c) : u4{0, 0, 0, 0};
   }
   transpose8(wh);
   if constexpr (A::HALF)
@@ -312,7 +316,6 @@ __global__ __launch_bounds__(WAVES * 64, 2) void gate_balance_backward_kernel(Ba
       // dx of 16 tokens at a time
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const int t = t0 + st * 32 + m * 16 + col;
         const u4 q = *reinterpret_cast<const u4*>(&along_e[st * 32 + m * 16 + col][quad * 8]);
         f4 y[8];
 #pragma unroll
@@ -321,16 +324,17 @@ __global__ __launch_bounds__(WAVES * 64, 2) void gate_balance_backward_kernel(Ba
           if constexpr (A::HALF) y[j] = Bf16::mul(wl[j], q, y[j]);
           y[j] = Bf16::mul(wh[j], q, y[j]);
         }
-        const int d = c0 + quad * 8;
-        if (t < end) {
-          uint16_t* to = p.dx + (size_t)t * p.D + d;
+        u4 o[4];      // 32 columns of a token next to each other
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            u4 o;
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) o[w] = A::pack(y[2 * w][e], y[2 * w + 1][e]);
-            if (d + 32 * e < p.D) __builtin_memcpy(to + 32 * e, &o, 16);
-          }
+          for (int w = 0; w < 4; ++w) o[e][w] = A::pack(y[2 * w][e], y[2 * w + 1][e]);
+        quad_transpose(o);
+        const int d = c0 + quad * 32 + (col & 3) * 8;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = t0 + st * 32 + m * 16 + (col & 12) + e;
+          if (t < end && d < p.D) __builtin_memcpy(p.dx + (size_t)t * p.D + d, &o[e], 16);
         }
       }
       // dW
@@ -433,8 +437,8 @@ extern "C" int hdmoe_gate_balance(const hdmoe_balance_args* a, hdmoe_stream_t st
     typed(a->dtype, [&](auto t) {
       typedef decltype(t) A;
       const dim3 grid((unsigned)(p.tiles_per_seq * a->sequences));
-      if (tile == 16) hipLaunchKernelGGL((gate_balance_kernel<A, 1>), grid, dim3(WAVES * 64), 0, s, p);
-      else hipLaunchKernelGGL((gate_balance_kernel<A, 4>), grid, dim3(WAVES * 64), 0, s, p);
+      if (tile == 16) hipLaunchKernelGGL((gate_balance_kernel<A, 1>), grid, dim3(SCORE_WAVES * 64), 0, s, p);
+      else hipLaunchKernelGGL((gate_balance_kernel<A, 4>), grid, dim3(SCORE_WAVES * 64), 0, s, p);
     });
   }
   hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(1024), 0, s, p.tiles, a->sequences, p.tiles_per_seq, a->E, a->k, a->alpha, a->loss, a->counts);
