@@ -1,5 +1,5 @@
-"""Compile comfyui_amd/csrc/*.hip into comfyui_amd/libhdmoe.so for gfx950 with hipcc, and block_calls.cpp (host code against torch's
-headers) into comfyui_amd/_block_calls.so.
+"""Compile comfyui_amd/csrc/*.hip into comfyui_amd/libhdmoe.so for gfx950 with hipcc, and block_calls.cpp and row_calls.cpp (host code
+against torch's headers) into comfyui_amd/_block_calls.so and _row_calls.so.
 
 hipcc cross-compiles without a GPU present. Run as `python -m comfyui_amd.build`
 (or through __graft_entry__.build()). The library is built in-tree so that the
@@ -12,7 +12,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhdmoe.so")
-CALLS_LIB = os.path.join(HERE, "_block_calls.so")
+CALLS = ("block_calls", "row_calls")     # csrc/<name>.cpp -> _<name>.so
 PROBE_LIB = os.path.join(HERE, "libhdmoe_probe.so")
 SOURCES = ["gate.hip", "dispatch.hip", "elementwise.hip", "gemm.hip", "layer.hip", "weights.hip", "blockscale.hip", "norm.hip", "router.hip", "adapters.hip"]
 
@@ -28,7 +28,7 @@ HIPCC_FLAGS = [
 ]
 
 
-def calls_command():
+def calls_command(name):
     import sysconfig
 
     import torch
@@ -36,7 +36,7 @@ def calls_command():
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
             f'-DHDMOE_TORCH_VERSION="{torch.__version__}"',
             "-I" + os.path.join(t, "include"), "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"),
-            "-I" + sysconfig.get_paths()["include"], os.path.join(CSRC, "block_calls.cpp"), "-o", CALLS_LIB,
+            "-I" + sysconfig.get_paths()["include"], os.path.join(CSRC, name + ".cpp"), "-o", os.path.join(HERE, f"_{name}.so"),
             "-L" + os.path.join(t, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
 
 
@@ -66,13 +66,14 @@ def build(verbose=True, extra_flags=()):
                 print(out, file=sys.stderr)
     if failed:
         raise RuntimeError("hipcc failed")
-    cmd = calls_command()
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    out = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if out.returncode != 0:
-        print(out.stdout, file=sys.stderr)
-        raise RuntimeError("g++ failed: block_calls.cpp")
+    for name in CALLS:
+        cmd = calls_command(name)
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        out = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        if out.returncode != 0:
+            print(out.stdout, file=sys.stderr)
+            raise RuntimeError(f"g++ failed: {name}.cpp")
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -109,10 +109,9 @@ __global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p)
   each_adapter(mine, z, p.turns, [&](int a, uint64_t has) {
     f4 acc[RT][TM] = {};
     const uint16_t* w = p.w + (size_t)a * p.R * p.K;
-    auto step = [&](int k0, auto whole) {
+    auto load = [&](int k0, u4 (&x)[TM][4], auto whole) {
       constexpr bool WHOLE = decltype(whole)::value;
       const int k = k0 + lane_k;
-      u4 x[TM][4];
 #pragma unroll
       for (int m = 0; m < TM; ++m)
 #pragma unroll
@@ -120,8 +119,12 @@ __global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p)
           const uint16_t* from = p.x + (size_t)min(t0 + m * 16 + i * 4 + lane_row, p.q.T - 1) * p.K + k;
           x[m][i] = WHOLE ? load8(from) : load8(from, hi - k);
         }
+    };
+    auto multiply = [&](int k0, u4 (&x)[TM][4], auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      const int k = k0 + lane_k;
       if constexpr (MODE == ALONG) {
-        constexpr int RB = RT < 2 ? RT : 2;     // r tiles at a time: registers
+        constexpr int RB = RT < 2 || TM == 4 ? 1 : 2;     // r tiles at a time: registers
 #pragma unroll
         for (int rb = 0; rb < RT; rb += RB) {
           u4 wv[RB][4];
@@ -191,9 +194,26 @@ __global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p)
         }
       }
     };
+    // the rows of the next block are on their way while one is multiplied
+    constexpr int EACH = NARROW_WAVES * K_BLOCK;
+    constexpr int AHEAD = TM < 4;
+    u4 x[1 + AHEAD][TM][4];
     int k0 = lo + wave * K_BLOCK;
-    for (; k0 + K_BLOCK <= hi; k0 += NARROW_WAVES * K_BLOCK) step(k0, std::true_type());
-    if (k0 < hi) step(k0, std::false_type());
+    if (AHEAD && k0 + K_BLOCK <= hi) load(k0, x[0], std::true_type());
+    while (k0 + K_BLOCK <= hi) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (k0 + K_BLOCK <= hi) {
+          if (!AHEAD) load(k0, x[0], std::true_type());
+          if (AHEAD && k0 + EACH + K_BLOCK <= hi) load(k0 + EACH, x[(1 - i) * AHEAD], std::true_type());
+          multiply(k0, x[i * AHEAD], std::true_type());
+          k0 += EACH;
+        }
+    }
+    if (k0 < hi) {
+      load(k0, x[0], std::false_type());
+      multiply(k0, x[0], std::false_type());
+    }
     // the upper half of the waves into the lower one, and so on
 #pragma unroll
     for (int half = NARROW_WAVES / 2; half > 0; half >>= 1) {
@@ -706,7 +726,7 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   const int rows_per = a.rows / a.requests;
   p.run = a.rows >= MANY_ROWS;
   // tokens of a tile of `narrow`: 16, and more where there are tiles for every CU all the same and a tile's rows share an adapter
-  p.tm = rows_per < 64 || a.rows < 32 * HDMOE_NUM_CU ? 1 : a.rows < 64 * HDMOE_NUM_CU || a.R > 32 ? 2 : 4;
+  p.tm = rows_per < 64 || a.rows < 32 * HDMOE_NUM_CU ? 1 : a.rows < 64 * HDMOE_NUM_CU || a.R > 64 ? 2 : 4;
   const int tile = 16 * p.tm;
   p.turns = div_up(tile, rows_per);          // adapters of a tile at most, as tiles go
   if (p.turns > a.n) p.turns = a.n;
@@ -754,7 +774,7 @@ void launch_narrow(const NarrowArgs& p, int tm, hipStream_t s) {
       hipLaunchKernelGGL((narrow_kernel<A, MODE, RT, TM>), grid, dim3(NARROW_WAVES * 64), 0, s, p);
     };
     if (tm == 1) tiles(integral_constant<int, 1>());
-    else if constexpr (RT > 2) tiles(integral_constant<int, 2>());
+    else if constexpr (RT > 4) tiles(integral_constant<int, 2>());
     else if (tm == 2) tiles(integral_constant<int, 2>());
     else tiles(integral_constant<int, 4>());
   };

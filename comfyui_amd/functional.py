@@ -19,6 +19,14 @@ except ImportError as e:   # host code only: every call it makes is made below a
     logging.warning("comfyui_amd: no compiled calls of the block-scaled operators (%s). `python -m comfyui_amd.build` builds them.", e)
     _block_calls = None
 
+try:
+    from . import _row_calls
+    if (getattr(_row_calls, "torch_version", None), getattr(_row_calls, "hdmoe_version", None)) != (torch.__version__, lib.hdmoe_version()):
+        raise ImportError(f"not built for torch {torch.__version__} and this library")
+except ImportError as e:   # as above
+    logging.warning("comfyui_amd: no compiled calls of the layer norm, the balance loss and the adapters (%s). `python -m comfyui_amd.build` builds them.", e)
+    _row_calls = None
+
 FP8 = torch.float8_e4m3fn
 BF16 = torch.bfloat16
 F16 = torch.float16
@@ -901,6 +909,21 @@ def swiglu_block_fp8(x, w1, scale_w1, w3, scale_w3, scale_x=None, fixed_k_cut=Fa
 # ---- layer norm and its gradients --------------------------------------------------------------------------------
 
 _T_CODE = {BF16: _lib.T_BF16, F16: _lib.T_F16, torch.float32: _lib.T_F32}
+if _row_calls is not None:
+    _row_calls.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+        lib.hdmoe_layer_norm, lib.hdmoe_layer_norm_backward_workspace_bytes, lib.hdmoe_layer_norm_backward, lib.hdmoe_gate_balance_workspace_bytes,
+        lib.hdmoe_gate_balance, lib.hdmoe_gate_balance_backward, lib.hdmoe_adapters_workspace_bytes, lib.hdmoe_add_adapters, lib.hdmoe_add_adapters_backward)))
+
+
+def _row_call(name, x, *args):
+    """The compiled call of that name on `args` and x's current stream, or None: it is not there, x is on another device than the current one, or it
+    leaves this call to Python."""
+    if _row_calls is None:
+        return None
+    d = x.get_device()
+    if d < 0 or d != torch._C._cuda_getDevice():
+        return None
+    return _done(getattr(_row_calls, name)(*args, torch._C._cuda_getCurrentRawStream(d)))
 
 
 def _norm_rows(x, what):
@@ -937,6 +960,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """torch.nn.functional.layer_norm over the last axis: (x - mean) / sqrt(var + eps) * weight + bias. x [..., D] bf16, fp16 or fp32,
     contiguous, D from 1 to 16384; weight, bias [D] of x's type or fp32 (both the same). Statistics are fp32, of the values' differences from
     their mean; the result is rounded once. ln_modulate, with a scale and a shift of each batch item, rounds between its steps."""
+    r = _row_call("layer_norm", x, x, weight, bias, eps)
+    if r is not None:
+        return r
     what = "layer_norm"
     _, rows, D = _norm_rows(x, what + " x")
     code = _norm_gains(x, weight, bias, D, what)
@@ -971,6 +997,9 @@ def layer_norm_backward(dy, x, weight=None, bias=None, eps=1e-5):
     """Gradients of layer_norm(x, weight, bias, eps) from dy, that of its result: (dx, dweight, dbias), None for a weight or bias that is
     None. Nothing is kept from the forward pass: mean and variance are taken from x again, which is read anyway. dweight and
     dbias are summed over the rows in fp32, in an order that depends on the sizes alone, and have their gains' type."""
+    r = _row_call("layer_norm_backward", x, dy, x, weight, bias, eps)
+    if r is not None:
+        return r
     what = "layer_norm_backward"
     _, rows, D = _norm_rows(x, what + " x")
     _norm_dy(dy, x, what)
@@ -986,6 +1015,9 @@ def ln_modulate_backward(dy, x2d, scale, tokens_per_batch, eps=1e-6):
     """Gradients of LayerNorm(x) * (1 + scale) + shift with one row of scale and shift for tokens_per_batch rows, from dy:
     (dx [T, D], dscale [B, D], dshift [B, D]). bf16 as ln_modulate, whose roundings between its steps count as none here, fp16 or
     fp32. Sums over a batch item's rows are fp32."""
+    r = _row_call("ln_modulate_backward", x2d, dy, x2d, scale, tokens_per_batch, eps)
+    if r is not None:
+        return r
     what = "ln_modulate_backward"
     dt, T, D = _norm_rows(x2d, what + " x")
     if x2d.dim() != 2:
@@ -1045,6 +1077,9 @@ def gate_balance(x2d, gate_w, topk_idx, alpha=0.01, sequences=1, mask=None):
     loss = alpha * mean over sequences of sum_e (E counts / (k n)) * (mean score of e), an fp32 scalar. mask: bool, T values in any shape; tokens with
     False are left out of counts, means and n, a sequence of nothing else out of the mean. Logits are fp32: gate_top2 rounds them to
     the activations' type before it chooses. Choices outside 0 .. E - 1 are not counted."""
+    r = _row_call("gate_balance", x2d, x2d, gate_w, topk_idx, alpha, sequences, mask)
+    if r is not None:
+        return r
     what = "gate_balance"
     args = _balance_args(x2d, gate_w, topk_idx, sequences, mask, alpha, what)
     with _on(x2d.device):
@@ -1062,6 +1097,9 @@ def gate_balance_backward(dloss, x2d, gate_w, topk_idx, counts, scores, alpha=0.
     chosen scores scores[t, topk_idx[t, j]] (what gate_top2 returns beside the experts), if there is one. counts and scores are those
     that gate_balance returned, which also say how many sequences there were; the other arguments are its own. Sums over tokens are fp32, in an order that
     depends on the sizes alone."""
+    r = _row_call("gate_balance_backward", x2d, dloss, x2d, gate_w, topk_idx, counts, scores, alpha, mask, dweight)
+    if r is not None:
+        return r
     what = "gate_balance_backward"
     args = _balance_args(x2d, gate_w, topk_idx, counts.shape[0] if counts.dim() == 2 else 0, mask, alpha, what)
     dev = x2d.device
@@ -1125,6 +1163,9 @@ def add_adapters(base, x, a, b, scale, index, out=None):
     smaller rank filled up with zeros; scale [n] fp32. index: int32, one for each request, each of as many rows of x in turn (x [B, S, K] with index [B]; an
     index for each row: index [rows]); negative or from n on: no adapter, and the row is base's. Sums are fp32, the narrow product between the two
     keeps 16 significant bits, the result is rounded once. `out`: takes the result, base itself if it is to be added in place."""
+    r = _row_call("add_adapters", x, base, x, a, b, scale, index, out)
+    if r is not None:
+        return r
     what = "add_adapters"
     args = _adapter_args(x, a, b, scale, index, what)
     _adapter_rows(base, x, args.N, what + " base")
@@ -1142,6 +1183,9 @@ def add_adapters_backward(dy, x, a, b, scale, index):
     """Gradients of add_adapters from dy, that of its result and of base: (dx, da, db) of the types of x, a and b. dx is the
     adapters' part alone, 0 for rows without one; da and db are sums over each adapter's rows in fp32, in an order that depends on the sizes alone, 0 for an
     adapter without rows."""
+    r = _row_call("add_adapters_backward", x, dy, x, a, b, scale, index)
+    if r is not None:
+        return r
     what = "add_adapters_backward"
     args = _adapter_args(x, a, b, scale, index, what)
     _adapter_rows(dy, x, args.N, what + " dy")
