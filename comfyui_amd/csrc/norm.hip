@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) void layer_norm_backward_kernel(NormGrad p) {
   constexpr int TEAMS = 4 / W;
   constexpr int WIDTH = W * 64 * V * C;
   __shared__ float lds[2][W][2];
-  __shared__ float joined[TEAMS > 1 ? 2 : 1][TEAMS > 1 ? WIDTH : 1];
+  __shared__ __attribute__((aligned(16))) float joined[TEAMS][TEAMS > 1 ? WIDTH : 1];
   int turn = 0;
   const int lane = threadIdx.x & (W * 64 - 1), team = threadIdx.x / (W * 64), D = p.D;
   const float inv = 1.0f / (float)D;
@@ -257,39 +257,47 @@ __global__ __launch_bounds__(256) void layer_norm_backward_kernel(NormGrad p) {
     }
   }
   if (!sums) return;
-  if constexpr (TEAMS > 1) {   // the teams' sums, added up in turn
-    for (int w = 0; w < TEAMS; ++w) {
-      if (team == w)
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int i = (c * V + j) * 64 + lane;   // a lane's own places, next to its neighbours'
-            joined[0][i] = w == 0 ? aw[c][j] : joined[0][i] + aw[c][j];
-            joined[1][i] = w == 0 ? ab[c][j] : joined[1][i] + ab[c][j];
-          }
-      __syncthreads();
-    }
-    if (team != 0) return;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < V; ++j) aw[c][j] = joined[0][(c * V + j) * 64 + lane], ab[c][j] = joined[1][(c * V + j) * 64 + lane];
-  }
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int col = (c * W * 64 + lane) * V;
+  // the teams' sums, dw and then db: each thread adds up columns of its own
+  auto put = [&](int which, int col, float v) {
     if (p.part != nullptr) {
-      float* q = p.part + (size_t)blockIdx.x * 2 * D + col;
-      store<NormF32>(q, aw[c], have[c]);
-      store<NormF32>(q + D, ab[c], have[c]);
+      p.part[((size_t)blockIdx.x * 2 + which) * D + col] = v;
     } else {
+      void* to = which == 0 ? p.dw : p.db;
+      if (to != nullptr) put_grad<A>(to, p.g_f32, (size_t)group * D + col, v);
+    }
+  };
+  if constexpr (TEAMS > 1) {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < have[c]) {
-          if (p.dw != nullptr) put_grad<A>(p.dw, p.g_f32, (size_t)group * D + col + j, aw[c][j]);
-          if (p.db != nullptr) put_grad<A>(p.db, p.g_f32, (size_t)group * D + col + j, ab[c][j]);
-        }
+    for (int which = 0; which < 2; ++which) {
+      if (which == 1) __syncthreads();
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j) joined[team][(c * V + j) * 64 + lane] = which == 0 ? aw[c][j] : ab[c][j];   // next to the neighbours'
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < WIDTH / 256; ++i) {
+        // column 8 l + j of chunk c lies at (8 c + j) 64 + l
+        const int col = i * 256 + threadIdx.x, at = ((col >> 9) * V + (col & 7)) * 64 + ((col >> 3) & 63);
+        float v = joined[0][at];
+#pragma unroll
+        for (int w = 1; w < TEAMS; ++w) v += joined[w][at];
+        if (col < D) put(which, col, v);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * W * 64 + lane) * V;
+      if (p.part != nullptr) {
+        float* q = p.part + (size_t)blockIdx.x * 2 * D + col;
+        store<NormF32>(q, aw[c], have[c]);
+        store<NormF32>(q + D, ab[c], have[c]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < have[c]) put(0, col + j, aw[c][j]), put(1, col + j, ab[c][j]);
+      }
     }
   }
 }
@@ -347,6 +355,7 @@ template <class F>
 void norm_shape(int D, F f) {
   if (D <= 512) f(std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
   else if (D <= 1024) f(std::integral_constant<int, 1>(), std::integral_constant<int, 2>());
+  else if (D <= 1536) f(std::integral_constant<int, 1>(), std::integral_constant<int, 3>());
   else if (D <= 2048) f(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
   else if (D <= 2560) f(std::integral_constant<int, 1>(), std::integral_constant<int, 5>());
   else if (D <= 4096) f(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());

@@ -139,14 +139,12 @@ __global__ __launch_bounds__(SCORE_WAVES * 64) void gate_balance_kernel(BalanceA
   }
 }
 
-// The loss and the counts from the tiles' sums: 64 groups of 16 lanes, as many of them a sequence as there are sequences few.
+// The loss and the counts from the tiles' sums: 64 groups of 16 lanes, as many of them a sequence as there are sequences few, four in a wave.
 __global__ __launch_bounds__(1024) void balance_finish_kernel(const TileSums* tiles, int seqs, int tiles_per_seq, int E, int k, float alpha,
                                                               float* loss, int32_t* counts) {
-  __shared__ float sp[64][LANES_E];
-  __shared__ int32_t sc[64][LANES_E], sn[64];
-  __shared__ float total[64];
-  __shared__ int32_t held[64];
-  const int e = threadIdx.x & 15, group = threadIdx.x >> 4;
+  __shared__ float sp[16][LANES_E], total[64];
+  __shared__ int32_t sc[16][LANES_E], sn[16], held[64];
+  const int e = threadIdx.x & 15, group = threadIdx.x >> 4, wave = threadIdx.x >> 6;
   int share = 64;   // groups of a sequence
   while (share > 1 && share * seqs > 64) share >>= 1;
   const int member = group & (share - 1), teams = 64 / share;
@@ -161,13 +159,24 @@ __global__ __launch_bounds__(1024) void balance_finish_kernel(const TileSums* ti
 #pragma unroll 8
       for (int i = member; i < tiles_per_seq; i += share) p += from[i].p[e], c += from[i].c[e], n += from[i].n;
     }
-    __syncthreads();
-    sp[group][e] = p;
-    sc[group][e] = c;
-    if (e == 0) sn[group] = n;
-    __syncthreads();
+    for (int off = 16; off < 64 && off < 16 * share; off <<= 1) {   // within the wave
+      p += __shfl_xor(p, off, 64);
+      c += __shfl_xor(c, off, 64);
+      n += __shfl_xor(n, off, 64);
+    }
+    if (share > 4) {                                                // over the waves
+      __syncthreads();
+      if ((group & 3) == 0) {
+        sp[wave][e] = p;
+        sc[wave][e] = c;
+        if (e == 0) sn[wave] = n;
+      }
+      __syncthreads();
+      if (member == 0)
+#pragma unroll 4
+        for (int i = 1; i < share / 4; ++i) p += sp[wave + i][e], c += sc[wave + i][e], n += sn[wave + i];
+    }
     if (member == 0 && s < seqs) {
-      for (int i = 1; i < share; ++i) p += sp[group + i][e], c += sc[group + i][e], n += sn[group + i];
       if (e < E) counts[(size_t)s * E + e] = c;
       if (n > 0) {
         const float f = 1.0f / (float)n;
@@ -181,12 +190,12 @@ __global__ __launch_bounds__(1024) void balance_finish_kernel(const TileSums* ti
   }
   if (e == 0) total[group] = mine, held[group] = mine_held;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    float v = 0.0f;
-    int32_t h = 0;
-    for (int g = 0; g < 64; ++g) v += total[g], h += held[g];
-    *loss = h > 0 ? alpha * (v / (float)h) : 0.0f;
-  }
+  if (threadIdx.x >= 64) return;
+  float v = total[threadIdx.x];
+  int32_t h = held[threadIdx.x];
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off, 64), h += __shfl_xor(h, off, 64);
+  if (threadIdx.x == 0) *loss = h > 0 ? alpha * (v / (float)h) : 0.0f;
 }
 
 // Tokens that the mask leaves of each sequence.
