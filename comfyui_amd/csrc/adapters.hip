@@ -95,18 +95,15 @@ struct NarrowArgs {
 // ACROSS32 has up to 32, four k blocks side by side instead, which are then dealt to instructions of 16 r each (8192 x 6912 rows, rank 32: 48 -> 29 us).
 enum { ALONG, ACROSS, ACROSS32 };
 template <class A, int MODE, int RT, int TM>
-__global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p) {
+struct NarrowTile {
   static_assert(MODE == ALONG || RT == (MODE == ACROSS ? 8 : 2), "128 or 32 r");
   static_assert(RT * TM <= 16, "64 KB of LDS");
-  __shared__ f4 joined[NARROW_WAVES / 2][RT * TM][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-  const int tiles = (p.q.T + 16 * TM - 1) / (16 * TM);
-  const int tile = blockIdx.x % tiles, slice = (blockIdx.x / tiles) % p.slices, z = blockIdx.x / tiles / p.slices;
-  const int t0 = tile * 16 * TM, r0 = blockIdx.y * 16 * RT;
-  const int lo = slice * p.slice, hi = min(p.K, lo + p.slice);
-  const int lane_row = col >> 2, lane_k = (quad * 4 + (col & 3)) * 8;      // of a load
-  const int mine = lane < 16 * TM ? p.q.of(t0 + lane) : -1;
-  each_adapter(mine, z, p.turns, [&](int a, uint64_t has) {
+  static constexpr int EIGHTS = RT == 1 ? 4 : RT * 2;     // of r; `rank` holds 32 r at least
+  typedef f4 Joined[NARROW_WAVES / 2][RT * TM][64];
+  // Sums of tokens t0 .. for adapter a, r0 .. and k from lo to hi into joined[0], for every wave to read.
+  static __device__ __forceinline__ void sums(const NarrowArgs& p, int a, int t0, int r0, int lo, int hi, Joined& joined) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+    const int lane_row = col >> 2, lane_k = (quad * 4 + (col & 3)) * 8;      // of a load
     f4 acc[RT][TM] = {};
     const uint16_t* w = p.w + (size_t)a * p.R * p.K;
     auto load = [&](int k0, u4 (&x)[TM][4], auto whole) {
@@ -230,30 +227,64 @@ __global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p)
         }
     }
     __syncthreads();
-    const float scale = p.part != nullptr ? 1.0f : p.q.scale[a];
-    constexpr int EIGHTS = RT == 1 ? 4 : RT * 2;     // `rank` holds 32 r at least
-    for (int u = threadIdx.x; u < 16 * TM * EIGHTS; u += NARROW_WAVES * 64) {   // eight r of a token
-      const int m = u / 16 % TM, eight = u / (16 * TM), bit = u % (16 * TM), r = r0 + eight * 8, t = t0 + bit;
-      if (!((has >> bit) & 1)) continue;
-      float v[8];
+  }
+  // Eight r of token `bit` of the tile, 0 from R on
+  static __device__ __forceinline__ void eight(const Joined& joined, int R, int r0, int bit, int eight, float scale, float (&v)[8]) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // r of a result: ACROSS 8 row + tile, ACROSS32 8 (row % 4) + 4 tile + row / 4, else 16 tile + row_of(row) (which undoes itself, as for tokens)
-        const int row = MODE == ACROSS ? eight : MODE == ACROSS32 ? (j & 3) * 4 + (eight & 3) : row_of((eight & 1) * 8 + j);
-        const int tile_r = MODE == ACROSS ? j : MODE == ACROSS32 ? j >> 2 : min(eight >> 1, RT - 1);
-        v[j] = r + j < p.R ? joined[0][tile_r * TM + m][(row >> 2) * 16 + row_of(bit & 15)][row & 3] * scale : 0.0f;
-      }
-      if (p.part == nullptr) {
-        if (r < p.to.steps * 32) put_planes(p.to, p.R, t, r, v);
-        continue;
-      }
-      float* to = p.part + ((size_t)slice * p.q.T + t) * p.R + r;
-      if (r + 8 <= p.R) __builtin_memcpy(to, v, 32);
-      else
-        for (int j = 0; j < 8; ++j)
-          if (r + j < p.R) to[j] = v[j];
+    for (int j = 0; j < 8; ++j) {
+      // r of a result: ACROSS 8 row + tile, ACROSS32 8 (row % 4) + 4 tile + row / 4, else 16 tile + row_of(row) (which undoes itself, as for tokens)
+      const int row = MODE == ACROSS ? eight : MODE == ACROSS32 ? (j & 3) * 4 + (eight & 3) : row_of((eight & 1) * 8 + j);
+      const int tile_r = MODE == ACROSS ? j : MODE == ACROSS32 ? j >> 2 : min(eight >> 1, RT - 1);
+      v[j] = r0 + eight * 8 + j < R ? joined[0][tile_r * TM + (bit >> 4)][(row >> 2) * 16 + row_of(bit & 15)][row & 3] * scale : 0.0f;
     }
-  });
+  }
+  // One block's share of the whole product: tile, slice and turn from `block`.
+  static __device__ __forceinline__ void run(const NarrowArgs& p, int block, int r0, Joined& joined) {
+    const int lane = threadIdx.x & 63;
+    const int tiles = (p.q.T + 16 * TM - 1) / (16 * TM);
+    const int tile = block % tiles, slice = (block / tiles) % p.slices, z = block / tiles / p.slices;
+    const int t0 = tile * 16 * TM, lo = slice * p.slice, hi = min(p.K, lo + p.slice);
+    const int mine = lane < 16 * TM ? p.q.of(t0 + lane) : -1;
+    each_adapter(mine, z, p.turns, [&](int a, uint64_t has) {
+      sums(p, a, t0, r0, lo, hi, joined);
+      const float scale = p.part != nullptr ? 1.0f : p.q.scale[a];
+      for (int u = threadIdx.x; u < 16 * TM * EIGHTS; u += NARROW_WAVES * 64) {
+        const int e = u / (16 * TM), bit = u % (16 * TM), r = r0 + e * 8, t = t0 + bit;
+        if (!((has >> bit) & 1)) continue;
+        float v[8];
+        eight(joined, p.R, r0, bit, e, scale, v);
+        if (p.part == nullptr) {
+          if (r < p.to.steps * 32) put_planes(p.to, p.R, t, r, v);
+          continue;
+        }
+        float* to = p.part + ((size_t)slice * p.q.T + t) * p.R + r;
+        if (r + 8 <= p.R) __builtin_memcpy(to, v, 32);
+        else
+          for (int j = 0; j < 8; ++j)
+            if (r + j < p.R) to[j] = v[j];
+      }
+    });
+  }
+};
+
+template <class A, int RT, int TM>
+__global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_kernel(NarrowArgs p) {
+  typedef NarrowTile<A, ALONG, RT, TM> Tile;
+  __shared__ typename Tile::Joined joined;
+  Tile::run(p, blockIdx.x, blockIdx.y * 16 * RT, joined);
+}
+
+// h and g of the backward pass in one launch: the shorter one's blocks fill what the longer one's leave.
+template <class A, int MODE, int RT, int RTG, int TM>
+__global__ __launch_bounds__(NARROW_WAVES * 64) void narrow_pair_kernel(NarrowArgs h, NarrowArgs g, int blocks_g) {
+  typedef NarrowTile<A, ALONG, RT, TM> H;
+  typedef NarrowTile<A, MODE, RTG, TM> G;
+  __shared__ union {
+    typename H::Joined h;
+    typename G::Joined g;
+  } joined;
+  if ((int)blockIdx.x < blocks_g) G::run(g, blockIdx.x, blockIdx.y * 16 * RTG, joined.g);
+  else H::run(h, blockIdx.x - blocks_g, blockIdx.y * 16 * RT, joined.h);
 }
 
 // v += eight values of each of `slices` parts, `next` apart (`have` of them).
@@ -440,6 +471,54 @@ __global__ __launch_bounds__(WIDE_WAVES * 64) void wide_kernel(WideArgs p) {
       if (a != early || s > 0) w.weights(a, s * 32, wh, wl);
       const u4 qh = *reinterpret_cast<const u4*>(lds + (size_t)col * stride + s * 32 + quad * 8);
       const u4 ql = *reinterpret_cast<const u4*>(lds + (size_t)(16 + col) * stride + s * 32 + quad * 8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = mul_split<A>(wh[j], wl[j], qh, ql, acc[j]);
+    }
+    w.put(t0, (uint32_t)has, acc, b);
+  });
+}
+
+// Very few rows: both products in one launch. Every block goes through the whole contraction for its tile and turn, whose weights come out of the
+// caches, and two of its waves have 128 columns each; one launch fewer is worth 3 us.
+template <class A, int RT>
+__global__ __launch_bounds__(NARROW_WAVES * 64) void few_kernel(NarrowArgs np, WideArgs p) {
+  typedef NarrowTile<A, ALONG, RT, 1> Tile;
+  typedef Wide<A, false> W;
+  __shared__ typename Tile::Joined joined;
+  __shared__ __attribute__((aligned(16))) uint16_t values[2][RT < 2 ? 1 : RT / 2][64][8];     // as Planes::rank of one tile
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tiles = (p.q.T + 15) / 16, chunks = (p.C + WIDE_WAVES * W::COLS - 1) / (WIDE_WAVES * W::COLS), steps = (p.R + 31) / 32;
+  const int chunk = blockIdx.x % chunks, tile = (blockIdx.x / chunks) % tiles, z = blockIdx.x / chunks / tiles;
+  const int t0 = tile * 16;
+  const int mine = lane < 16 ? p.q.of(t0 + lane) : -1;
+  const W w(p, (chunk * WIDE_WAVES + wave) * W::COLS, lane);
+  const bool writes = wave < WIDE_WAVES && w.c0 < p.C;
+  if (writes && z == 0) w.copy(t0, (uint32_t)__ballot(lane < 16 && mine < 0 && t0 + lane < p.q.T));
+  each_adapter(mine, z, p.turns, [&](int a, uint64_t has) {
+    u4 wh[8], wl[8], b[4];
+    if (writes) {      // on their way meanwhile
+      w.weights(a, 0, wh, wl);
+      w.base(t0, (uint32_t)has, b);
+    }
+    Tile::sums(np, a, t0, 0, 0, np.K, joined);
+    const float scale = p.q.scale[a];
+    for (int u = threadIdx.x; u < 16 * steps * 4; u += NARROW_WAVES * 64) {
+      float v[8];
+      Tile::eight(joined, p.R, 0, u & 15, u >> 4, scale, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t h, l;
+        split(v[2 * j], v[2 * j + 1], h, l);
+        *reinterpret_cast<uint32_t*>(&values[0][u >> 6][u & 63][2 * j]) = h;
+        *reinterpret_cast<uint32_t*>(&values[1][u >> 6][u & 63][2 * j]) = l;
+      }
+    }
+    __syncthreads();
+    if (!writes) return;
+    f4 acc[8] = {};
+    for (int s = 0; s < steps; ++s) {
+      if (s > 0) w.weights(a, s * 32, wh, wl);
+      const u4 qh = *reinterpret_cast<const u4*>(values[0][s][lane]), ql = *reinterpret_cast<const u4*>(values[1][s][lane]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] = mul_split<A>(wh[j], wl[j], qh, ql, acc[j]);
     }
@@ -699,7 +778,7 @@ struct Side {                 // a narrow product
 };
 
 struct Plan {
-  int tm, turns, run;         // run: many rows
+  int tm, turns, run, few;    // run: many rows; few: one launch
   Side h, g;
   int steps, tiles, splits, per_split, rt;
   size_t da_bytes, db_bytes, total;
@@ -709,6 +788,7 @@ int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 size_t bytes_of(size_t n) { return hdmoe_align_up(n, 256); }
 
+constexpr int64_t FEW_BYTES = 64 << 20;
 constexpr int MANY_ROWS = 512;   // from here on `wide` keeps its weights over runs of tokens
 
 // The contraction is cut over blocks until the card has about one a CU, in slices of a block of each wave at least; `whole`: not at all.
@@ -737,6 +817,11 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   const size_t part = (size_t)a.rows * a.R * sizeof(float), rank = (size_t)div_up(a.rows, 16) * p.steps * 2048;
   const size_t rows = (size_t)div_up(a.rows, STAGE) * (STAGE / 32) * p.tiles * 2048;
   if (!backward) {
+    // One launch, whose blocks each read x and w for themselves, while all of them run at once and that is little for the caches: 1 row of 2560 x 6912, rank 16,
+    // 9.4 -> 6.5 us, 8 rows of 8 adapters (34 MB) 10.7 -> 6.9, 64 rows of one 10.0 -> 6.6; 16 rows of 16 adapters, 432 blocks, 12.4 -> 12.3.
+    const int64_t blocks = (int64_t)div_up(a.N, 128 * WIDE_WAVES) * tiles * p.turns;
+    p.few = a.R <= 64 && !p.run && blocks <= HDMOE_NUM_CU && blocks * (a.R + 16) * a.K * 2 <= FEW_BYTES;
+    if (p.few) return p;
     if (p.run) p.h.rank = rank;
     else p.h.part = bytes_of(part * p.h.slices);
     p.total = p.h.part + p.h.rank;
@@ -763,39 +848,35 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   return p;
 }
 
-template <class A, bool TURNED>
-void launch_narrow(const NarrowArgs& p, int tm, hipStream_t s) {
+// f(r tiles of 16, mode and r tiles of the turned product, tokens of a tile in 16) as constants; PAIR: both products run
+template <bool PAIR, class F>
+void narrow_shape(int R, int tm, F f) {
   using std::integral_constant;
-  auto go = [&](auto mode, auto rt) {
-    constexpr int MODE = decltype(mode)::value, RT = decltype(rt)::value;
-    auto tiles = [&](auto m) {
-      constexpr int TM = decltype(m)::value;
-      const dim3 grid(div_up(p.q.T, 16 * TM) * p.slices * p.turns, div_up(p.R, 16 * RT));
-      hipLaunchKernelGGL((narrow_kernel<A, MODE, RT, TM>), grid, dim3(NARROW_WAVES * 64), 0, s, p);
-    };
-    if (tm == 1) tiles(integral_constant<int, 1>());
-    else if constexpr (RT > 4) tiles(integral_constant<int, 2>());
-    else if (tm == 2) tiles(integral_constant<int, 2>());
-    else tiles(integral_constant<int, 4>());
+  auto tokens = [&](auto rt, auto mode, auto rtg) {
+    constexpr int most = decltype(rt)::value > 4 || (PAIR && decltype(rtg)::value > 4) ? 2 : 4;
+    if (tm == 1) f(rt, mode, rtg, integral_constant<int, 1>());
+    else if (tm == 2 || most == 2) f(rt, mode, rtg, integral_constant<int, 2>());
+    else f(rt, mode, rtg, integral_constant<int, most>());
   };
-  if constexpr (TURNED) {
-    if (p.R <= 32) go(integral_constant<int, ACROSS32>(), integral_constant<int, 2>());
-    else go(integral_constant<int, ACROSS>(), integral_constant<int, 8>());
-  } else {
-    if (p.R <= 16) go(integral_constant<int, ALONG>(), integral_constant<int, 1>());
-    else if (p.R <= 32) go(integral_constant<int, ALONG>(), integral_constant<int, 2>());
-    else if (p.R <= 64) go(integral_constant<int, ALONG>(), integral_constant<int, 4>());
-    else go(integral_constant<int, ALONG>(), integral_constant<int, 8>());
-  }
+  const integral_constant<int, ACROSS32> narrow;
+  const integral_constant<int, ACROSS> wide;
+  const integral_constant<int, 2> two;
+  const integral_constant<int, 8> eight;
+  if (R <= 16) tokens(integral_constant<int, 1>(), narrow, two);
+  else if (R <= 32) tokens(two, narrow, two);
+  else if (R <= 64) tokens(integral_constant<int, 4>(), wide, eight);
+  else tokens(eight, wide, eight);
 }
+
+int narrow_blocks(const NarrowArgs& p, int tm) { return div_up(p.q.T, 16 * tm) * p.slices * p.turns; }
 
 template <class A, bool TURNED>
 void launch_wide_run(const WideArgs& p, hipStream_t s) {
   auto go = [&](auto steps) {
     constexpr int STEPS = decltype(steps)::value;
-    // runs as long as four blocks a CU allow
-    const int chunks = div_up(p.C, WAVES * Wide<A, TURNED>::COLS);
-    int run = div_up((int64_t)p.q.T * chunks, 4 * HDMOE_NUM_CU * 16) * 16;
+    // the shortest runs that leave no more blocks than the card holds at once, two a CU
+    const int chunks = div_up(p.C, WAVES * Wide<A, TURNED>::COLS), most = chunks < 2 * HDMOE_NUM_CU ? 2 * HDMOE_NUM_CU / chunks : 1;
+    int run = div_up(p.q.T, (int64_t)16 * most) * 16;
     if (run > RUN) run = RUN;
     hipLaunchKernelGGL((wide_run_kernel<A, TURNED, STEPS>), dim3(chunks * div_up(p.q.T, run)), dim3(WAVES * 64), 0, s, p, div_up(p.R, 32 * STEPS), run);
   };
@@ -838,6 +919,7 @@ extern "C" size_t hdmoe_adapters_workspace_bytes(const hdmoe_adapter_args* a, in
 }
 
 static int check_workspace(const hdmoe_adapter_args* a, const Plan& plan, const char* what) {
+  if (plan.total == 0) return HDMOE_OK;
   if (a->workspace == nullptr || a->workspace_bytes < plan.total || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0)
     return hdmoe_fail(HDMOE_E_WORKSPACE, "%s: workspace of %zu bytes on 16 needed, got %zu", what, plan.total, a->workspace_bytes);
   return HDMOE_OK;
@@ -857,7 +939,17 @@ extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t st
   const WideArgs wp = {q, part, planes.rank, bits(a->b), bits(a->base), static_cast<uint16_t*>(a->out), a->N, a->R, plan.h.slices, plan.turns};
   typed(a->dtype, [&](auto t) {
     typedef decltype(t) A;
-    launch_narrow<A, false>(np, plan.tm, s);
+    if (plan.few) {
+      const dim3 grid(div_up(a->N, WIDE_WAVES * Wide<A, false>::COLS) * div_up(a->rows, 16) * plan.turns);
+      if (a->R <= 16) hipLaunchKernelGGL((few_kernel<A, 1>), grid, dim3(NARROW_WAVES * 64), 0, s, np, wp);
+      else if (a->R <= 32) hipLaunchKernelGGL((few_kernel<A, 2>), grid, dim3(NARROW_WAVES * 64), 0, s, np, wp);
+      else hipLaunchKernelGGL((few_kernel<A, 4>), grid, dim3(NARROW_WAVES * 64), 0, s, np, wp);
+      return;
+    }
+    narrow_shape<false>(a->R, plan.tm, [&](auto rt, auto, auto, auto tm) {
+      constexpr int RT = decltype(rt)::value, TM = decltype(tm)::value;
+      hipLaunchKernelGGL((narrow_kernel<A, RT, TM>), dim3(narrow_blocks(np, TM), div_up(a->R, 16 * RT)), dim3(NARROW_WAVES * 64), 0, s, np);
+    });
     if (plan.run) {
       launch_wide_run<A, false>(wp, s);
     } else {
@@ -911,8 +1003,11 @@ extern "C" int hdmoe_add_adapters_backward(const hdmoe_adapter_args* a, hdmoe_st
   const dim3 grid(op.side[0].blocks + op.side[1].blocks, a->n * div_up(a->R, 16 * plan.rt), plan.splits);
   typed(a->dtype, [&](auto t) {
     typedef decltype(t) A;
-    launch_narrow<A, false>(hp, plan.tm, s);
-    launch_narrow<A, true>(gp, plan.tm, s);
+    narrow_shape<true>(a->R, plan.tm, [&](auto rt, auto mode, auto rtg, auto tm) {
+      constexpr int RT = decltype(rt)::value, MODE = decltype(mode)::value, RTG = decltype(rtg)::value, TM = decltype(tm)::value;
+      const int nh = narrow_blocks(hp, TM), ng = narrow_blocks(gp, TM);
+      hipLaunchKernelGGL((narrow_pair_kernel<A, MODE, RT, RTG, TM>), dim3(nh + ng, div_up(a->R, 128)), dim3(NARROW_WAVES * 64), 0, s, hp, gp, ng);
+    });
     if (h != nullptr || g != nullptr)
       hipLaunchKernelGGL(join_kernel, dim3(div_up((int64_t)a->rows * plan.steps * 4, 64), 2), dim3(64), 0, s, jp);
     launch_wide_run<A, true>(wp, s);

@@ -123,24 +123,6 @@ __device__ __forceinline__ void row_transpose(u4 (&v)[4]) {
     }
 }
 
-// v[i] of the lanes 16 g .. + 15 <-> v[g] of the lanes 16 i .. + 15.
-__device__ __forceinline__ void half_transpose(u4 (&v)[4]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const auto r = __builtin_amdgcn_permlane32_swap(v[i][w], v[i + 2][w], false, false);
-      v[i][w] = r[0], v[i + 2][w] = r[1];
-    }
-#pragma unroll
-  for (int i = 0; i < 4; i += 2)
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const auto r = __builtin_amdgcn_permlane16_swap(v[i][w], v[i + 1][w], false, false);
-      v[i][w] = r[0], v[i + 1][w] = r[1];
-    }
-}
-
 // Operands of 16 rows and 128 k: lane l loads 16 bytes of row 4 i + l / 4 % 4, k = 8 (4 (l / 16) + l % 4), i = 0 .. 3; transposed, instruction n has
 // k = 32 (l / 16) + 8 n .. + 7 of row 4 (l % 4) + l / 4 % 4 in lane l. row_of(l % 16) is that row.
 constexpr int K_BLOCK = 128;
