@@ -160,21 +160,23 @@ int norm_backward(hdmoe_norm_grad_args& a, const at::Tensor& dy, const at::Tenso
   return layer_norm_backward(&a, stream);
 }
 
-// (dy, x, weight, bias, eps, stream)
+// (dy, x, weight, bias, eps, gains, stream)
 PyObject* do_layer_norm_backward(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(6)
+  HDMOE_ARGUMENTS(7)
   return answer([&]() -> PyObject* {
     const Norm n(o[1], o[2], o[3]);
     const at::Tensor& dy = tensor(o[0]);
     like(dy, n.x, n.x.scalar_type(), n.x.sizes());
     hdmoe_norm_grad_args a = {};
     a.gain_dtype = n.gain, a.D = static_cast<int>(n.D), a.rows = a.rows_per_group = n.rows, a.eps = number(o[4]);
-    void* const stream = stream_of(o[5]);
+    const int gains = PyObject_IsTrue(o[5]);
+    need(gains >= 0);
+    void* const stream = stream_of(o[6]);
     at::Tensor dx, dw, db;
     int rc;
     {
       Unlocked u;
-      dw = make_like(n.w), db = make_like(n.b);
+      if (gains) dw = make_like(n.w), db = make_like(n.b);
       rc = norm_backward(a, dy, n.x, n.w, dx, dw, db, stream);
     }
     return rc != 0 ? PyLong_FromLong(rc) : tuple({dx, dw, db});

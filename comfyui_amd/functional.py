@@ -31,6 +31,7 @@ FP8 = torch.float8_e4m3fn
 BF16 = torch.bfloat16
 F16 = torch.float16
 FP8_UPCAST = "float8_e4m3fn multiplied in bfloat16"   # a "weight dtype" of moe_ffn / ffn_swiglu: no activation is cast
+TOPK = _lib.TOPK
 ACT_DTYPES = (BF16, F16)   # 16-bit activation formats; fp16 is served by the *_f16 entry points (Hunyuan3D block)
 
 
@@ -993,11 +994,11 @@ def _norm_dy(dy, x, what):
         raise ValueError(f"{what}: dy must be contiguous {x.dtype} {list(x.shape)} on {x.device}, got {dy.dtype} {tuple(dy.shape)} on {dy.device}")
 
 
-def layer_norm_backward(dy, x, weight=None, bias=None, eps=1e-5):
+def layer_norm_backward(dy, x, weight=None, bias=None, eps=1e-5, gains=True):
     """Gradients of layer_norm(x, weight, bias, eps) from dy, that of its result: (dx, dweight, dbias), None for a weight or bias that is
-    None. Nothing is kept from the forward pass: mean and variance are taken from x again, which is read anyway. dweight and
+    None; without `gains` dx alone. Nothing is kept from the forward pass: mean and variance are taken from x again, which is read anyway. dweight and
     dbias are summed over the rows in fp32, in an order that depends on the sizes alone, and have their gains' type."""
-    r = _row_call("layer_norm_backward", x, dy, x, weight, bias, eps)
+    r = _row_call("layer_norm_backward", x, dy, x, weight, bias, eps, gains)
     if r is not None:
         return r
     what = "layer_norm_backward"
@@ -1005,8 +1006,8 @@ def layer_norm_backward(dy, x, weight=None, bias=None, eps=1e-5):
     _norm_dy(dy, x, what)
     code = _norm_gains(x, weight, bias, D, what)
     with _on(x.device):
-        dweight = None if weight is None else torch.empty_like(weight)
-        dbias = None if bias is None else torch.empty_like(bias)
+        dweight = None if weight is None or not gains else torch.empty_like(weight)
+        dbias = None if bias is None or not gains else torch.empty_like(bias)
         dx = _norm_backward(dy, x, weight, dweight, dbias, code, D, rows, rows, 0, eps)
     return dx, dweight, dbias
 

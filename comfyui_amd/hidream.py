@@ -99,6 +99,8 @@ def _fusable_dtype(ffns):
             return None
         if isinstance(l, amd_ops.block_fp8_ops.Linear):   # its scales are a matrix, whatever its weight has become (module.to(bfloat16))
             return None
+        if amd_ops.adapters_of(l) is not None:
+            return None
     wdt = lins[0].weight.dtype
     if wdt not in (BF16, FP8) or any(l.weight.dtype != wdt for l in lins):
         return None
@@ -159,6 +161,8 @@ def _pack_key(ffns, dev):
         mods = f.__dict__["_modules"]
         for l in (mods["w1"], mods["w2"], mods["w3"]):
             w, b, sw, si = _lin_tensors(l)
+            if amd_ops.adapters_of(l) is not None:
+                return None
             if w.device != dev or getattr(l, "weight_function", None) or getattr(l, "bias_function", None):
                 return None
             if (sw is not None and sw.device != dev) or (si is not None and si.device != dev):
@@ -306,6 +310,19 @@ class MoEGate(nn.Module):
 
     def device_weight(self, hidden_states):
         return _gate_weight(self, hidden_states)
+
+    def route(self, hidden_states, mask=None):
+        """forward for training: (topk_idx, topk_weight, aux_loss) with gradients of topk_weight and aux_loss for the input and the gate weight. aux_loss is
+        `alpha` times the balance loss, over each sequence of its own with `seq_aux`; mask [B, S] bool: False is padding. Not a method of the reference
+        class, whose forward returns None for the loss."""
+        from . import autograd
+        self._check()
+        if self.norm_topk_prob:
+            raise NotImplementedError("renormalised gate weights have no gradient here")
+        bsz, seq_len, h = hidden_states.shape
+        x2 = hidden_states.reshape(-1, h).contiguous()
+        idx, w, loss, _ = autograd.gate(x2, self.device_weight(x2), self.alpha, bsz if self.seq_aux else 1, None if mask is None else mask.contiguous())
+        return idx.to(torch.int64), w, loss
 
     def forward(self, hidden_states):
         self._check()
@@ -471,7 +488,8 @@ class MOEFeedForwardSwiGLU(nn.Module):
         for i, expert in enumerate(self.experts):
             lo, hi = bounds[i], bounds[i + 1]
             if hi > lo:
-                y[lo:hi] = expert(xs[lo:hi])
+                with amd_ops.routed_adapters(expert, x2.shape[0], perm[lo:hi]):
+                    y[lo:hi] = expert(xs[lo:hi])
         shared = self.shared_experts(x2)
         if gated_residual is not None:
             g, res, per_batch = gated_residual

@@ -77,7 +77,7 @@ def _plain_pair(lin, x):
     device, nothing to apply to them first. None otherwise. (Looking a parameter up in its module takes the host as long as the rest.)"""
     if getattr(lin, "weight_function", None) or getattr(lin, "bias_function", None):
         return None
-    if getattr(lin, "scale_weight", None) is not None:
+    if getattr(lin, "scale_weight", None) is not None or amd_ops.adapters_of(lin) is not None:
         return None
     weight, bias = lin.weight, lin.bias
     if weight.dtype != x.dtype or weight.device != x.device:
@@ -159,6 +159,17 @@ class MoEGate(nn.Module):
         self.gating_dim = embed_dim
         self.weight = nn.Parameter(torch.empty((self.n_routed_experts, self.gating_dim), device=device, dtype=dtype))
 
+    def route(self, hidden_states, mask=None):
+        """forward for training: (topk_idx, topk_weight, aux_loss) with gradients of topk_weight and aux_loss for the input and the gate weight; the balance
+        loss is over the whole batch. mask: bool, one value a token, False is padding. Not a method of the reference class."""
+        from . import autograd
+        if self.top_k != 2:
+            raise NotImplementedError("the HIP gate kernel selects the top 2 experts")
+        x2 = hidden_states.reshape(-1, hidden_states.size(-1)).contiguous()
+        gate_w = amd_ops.cast_to(self.weight, dtype=x2.dtype, device=x2.device).contiguous()
+        idx, w, loss, _ = autograd.gate(x2, gate_w, self.alpha, 1, None if mask is None else mask.contiguous())
+        return idx.to(torch.int64), w, loss
+
     def forward(self, hidden_states: torch.Tensor):
         if self.top_k != 2:
             raise NotImplementedError("the HIP gate kernel selects the top 2 experts")
@@ -215,7 +226,8 @@ class MoEBlock(nn.Module):
             for i, expert in enumerate(self.experts):
                 lo, hi = bounds[i], bounds[i + 1]
                 if hi > lo:
-                    y[lo:hi] = expert(xs[lo:hi])
+                    with amd_ops.routed_adapters(expert, x2.shape[0], perm[lo:hi]):
+                        y[lo:hi] = expert(xs[lo:hi])
             return HF.combine(y, inv_perm, w, self.shared_experts(x2)).view(*orig_shape)
         (*stage1, sh1), (*stage2, sh2) = zip(*stages)
         fixed = amd_ops._batch_invariant(self)

@@ -207,10 +207,102 @@ def _linear_upcast(lin, input, scale):
     return out.reshape(*shape[:-1], lin.weight.shape[0])
 
 
+class Adapters(torch.nn.Module):
+    """Low-rank adapters of many requests beside a Linear: set as `linear.adapters`, they join each result of its forward. a [n, R, in], b [n, out, R] in the
+    activations' type, scale [n] fp32 (the usual alpha / rank times the strength). `index`, set before a forward, is int32 on the device with the
+    adapter of each request in the batch (-1: none), each request having as many rows as the others. Not in the reference, which patches a
+    LoRA into the weights: these differ between the requests of one batch, and the weights stay as they are. Inference only, as the Linear is; autograd.add_adapters
+    has the gradients."""
+
+    def __init__(self, a, b, scale):
+        super().__init__()
+        self.a, self.b = (torch.nn.Parameter(t, requires_grad=False) for t in (a, b))
+        self.register_buffer("scale", scale)
+        self.index = None
+        self._rows = None      # an index for each row, while a routed expert is called (functional.dispatch's order)
+
+    @classmethod
+    def stack(cls, adapters, dtype=None, device=None):
+        """Of [(a [r, in], b [out, r], scale)], whose ranks may differ: those below the largest are filled up with zeros."""
+        rank = max(a.shape[0] for a, _, _ in adapters)
+        pad = torch.nn.functional.pad
+        a = torch.stack([pad(a, (0, 0, 0, rank - a.shape[0])) for a, _, _ in adapters])
+        b = torch.stack([pad(b, (0, rank - b.shape[1])) for _, b, _ in adapters])
+        scale = torch.tensor([float(s) for _, _, s in adapters], dtype=torch.float32)
+        return cls(a.to(device=device, dtype=dtype).contiguous(), b.to(device=device, dtype=dtype).contiguous(), scale.to(device))
+
+    def forward(self, base, x):
+        if torch.is_grad_enabled() and (self.a.requires_grad or self.b.requires_grad):
+            raise RuntimeError("comfyui_amd.ops.Adapters: a Linear with adapters is inference only; autograd.add_adapters has the gradients")
+        index = self.index if self._rows is None else self._rows
+        if index is None:
+            raise RuntimeError("comfyui_amd.ops.Adapters: set `index`, the adapter of each request, before the forward")
+        x = x.contiguous()
+        base = base.contiguous()
+        return HF.add_adapters(base, x, self.a, self.b, self.scale, index, out=base)
+
+
+def adapters_of(lin):
+    """The adapters beside a Linear, or None."""
+    return lin.__dict__["_modules"].get("adapters")
+
+
+class routed_adapters:
+    """Context in which the adapters of a module's Linears take T tokens' rows in functional.dispatch's order: row r of the module's input is token
+    perm[r] // 2."""
+
+    def __init__(self, module, T, perm):
+        self.on = [ad for ad in (adapters_of(l) for l in module.modules() if isinstance(l, torch.nn.Linear)) if ad is not None]
+        self.T, self.perm = T, perm
+
+    def __enter__(self):
+        for ad in self.on:
+            if ad.index is None or ad.index.numel() == 0 or self.T % ad.index.numel() != 0:
+                raise RuntimeError(f"comfyui_amd.ops.Adapters: `index` must be set and divide the {self.T} tokens of the layer")
+            ad._rows = ad.index.reshape(-1)[self.perm // (HF.TOPK * (self.T // ad.index.numel()))]
+
+    def __exit__(self, *exc):
+        for ad in self.on:
+            ad._rows = None
+
+
+def _with_adapters(lin, input, out):
+    ad = adapters_of(lin)
+    return out if ad is None else ad(out, input)
+
+
 class disable_weight_init:
+    class LayerNorm(torch.nn.LayerNorm, CastWeightBiasOp):
+        """Over the last axis, with gradients (autograd.layer_norm) for input, weight and bias."""
+
+        def reset_parameters(self):
+            return None
+
+        def _norm(self, input, weight, bias):
+            from . import autograd
+            if len(self.normalized_shape) != 1:
+                raise NotImplementedError("the HIP layer norm is over the last axis")
+            if input.shape[-1:] != torch.Size(self.normalized_shape):
+                raise ValueError(f"LayerNorm over {tuple(self.normalized_shape)} for an input {tuple(input.shape)}")
+            return autograd.layer_norm(input.contiguous(), weight, bias, self.eps)
+
+        def forward_comfy_cast_weights(self, input):
+            if self.weight is None:
+                return self._norm(input, None, None)
+            weight, bias = cast_bias_weight(self, input)
+            return self._norm(input, weight, bias)
+
+        def forward(self, *args, **kwargs):
+            if self.comfy_cast_weights or len(self.weight_function) > 0 or len(self.bias_function) > 0:
+                return self.forward_comfy_cast_weights(*args, **kwargs)
+            return self._norm(args[0], self.weight, self.bias)
+
     class Linear(torch.nn.Linear, CastWeightBiasOp):
         def reset_parameters(self):
             return None
+
+        def __call__(self, input, *args, **kwargs):
+            return _with_adapters(self, input, super().__call__(input, *args, **kwargs))
 
         def _load_from_state_dict(self, *args, **kwargs):
             invalidate_scale_cache()   # load_state_dict copies into the Parameters in place
@@ -230,6 +322,9 @@ class disable_weight_init:
 
 class manual_cast(disable_weight_init):
     class Linear(disable_weight_init.Linear):
+        comfy_cast_weights = True
+
+    class LayerNorm(disable_weight_init.LayerNorm):
         comfy_cast_weights = True
 
 
@@ -454,7 +549,7 @@ def block_fp8_parts(linears, input):
         if not isinstance(l, block_fp8_ops.Linear):
             return None
         d, cls = l.__dict__, type(l)
-        if (d["_forward_hooks"] or d["_forward_pre_hooks"] or "forward" in d or cls.forward is not disable_weight_init.Linear.forward
+        if (d["_forward_hooks"] or d["_forward_pre_hooks"] or "forward" in d or adapters_of(l) is not None or cls.forward is not disable_weight_init.Linear.forward
                 or cls.forward_comfy_cast_weights is not block_fp8_ops.Linear.forward_comfy_cast_weights or l.weight.dtype != FP8):
             return None
     return [l.parts(input) for l in linears]
