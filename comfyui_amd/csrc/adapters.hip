@@ -14,6 +14,7 @@
 
 #include "lowrank.h"
 
+
 using namespace lowrank;
 
 namespace {
@@ -22,6 +23,7 @@ constexpr int WAVES = 4;                   // of `wide_run`
 constexpr int WIDE_WAVES = 2;              // of `wide`
 constexpr int NARROW_WAVES = 8;
 constexpr int RUN = 256;                   // tokens of a block of `wide_run` at most
+constexpr int OUTER_BLOCKS = 160;          // of `outer`, about
 constexpr int STAGE = 128;                 // tokens that `outer` looks at the adapters of at a time
 
 struct Requests {
@@ -420,10 +422,11 @@ struct Wide {
   }
 };
 
-// Few rows: 16 tokens a tile, their narrow values added up from the parts and split in LDS; a tile's adapters are dealt to `turns` blocks.
-template <class A>
+// Few rows, or rows of many adapters: 16 tokens a tile, whose adapters are dealt to `turns` blocks. Their narrow values are added up from the parts and
+// split in LDS, or loaded as `rank` has them (p.part NULL).
+template <class A, bool TURNED>
 __global__ __launch_bounds__(WIDE_WAVES * 64) void wide_kernel(WideArgs p) {
-  typedef Wide<A, false> W;
+  typedef Wide<A, TURNED> W;
   extern __shared__ __attribute__((aligned(16))) uint16_t lds[];   // [2][16][stride]: hi, lo of s h
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int steps = (p.R + 31) / 32, stride = steps * 32 + 8;
@@ -441,7 +444,7 @@ __global__ __launch_bounds__(WIDE_WAVES * 64) void wide_kernel(WideArgs p) {
     w.weights(a, 0, wh, wl);
     w.base(t0, (uint32_t)has, b);
   });
-  for (int u = threadIdx.x; u < 16 * steps * 4; u += WIDE_WAVES * 64) {   // eight values a thread
+  for (int u = threadIdx.x; p.part != nullptr && u < 16 * steps * 4; u += WIDE_WAVES * 64) {   // eight values a thread
     const int row = u / (steps * 4), r = (u - row * (steps * 4)) * 8, t = t0 + row;
     const int a = p.q.of(t);
     float v[8] = {};
@@ -469,8 +472,15 @@ __global__ __launch_bounds__(WIDE_WAVES * 64) void wide_kernel(WideArgs p) {
     f4 acc[8] = {};
     for (int s = 0; s < steps; ++s) {
       if (a != early || s > 0) w.weights(a, s * 32, wh, wl);
-      const u4 qh = *reinterpret_cast<const u4*>(lds + (size_t)col * stride + s * 32 + quad * 8);
-      const u4 ql = *reinterpret_cast<const u4*>(lds + (size_t)(16 + col) * stride + s * 32 + quad * 8);
+      u4 qh, ql;
+      if (p.part != nullptr) {
+        qh = *reinterpret_cast<const u4*>(lds + (size_t)col * stride + s * 32 + quad * 8);
+        ql = *reinterpret_cast<const u4*>(lds + (size_t)(16 + col) * stride + s * 32 + quad * 8);
+      } else {
+        const uint16_t* from = p.rank + (((size_t)tile * steps + s) * 128 + lane) * 8;
+        qh = *reinterpret_cast<const u4*>(from);
+        ql = *reinterpret_cast<const u4*>(from + 512);
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] = mul_split<A>(wh[j], wl[j], qh, ql, acc[j]);
     }
@@ -527,10 +537,10 @@ __global__ __launch_bounds__(NARROW_WAVES * 64) void few_kernel(NarrowArgs np, W
 }
 
 // Many rows: a block has up to RUN tokens, 16 at a time; a wave keeps the weights of its columns in registers for as long as the adapter stays the same (R up to
-// 32 STEPS; `parts` times that are gone through one after the other, loaded anew). Bound by base and out: R of 64 takes 32 instructions
+// 32 STEPS; `parts` times that are gone through one after the other, for GROUPS times 16 tokens at a time). Bound by base and out: R of 64 takes 32 instructions
 // (512 cycles of one of four units) for 8 KB of them. Where the whole run has one adapter, values and base of the AHEAD 16 tokens to come are on
 // their way while some are multiplied.
-template <class A, bool TURNED, int STEPS>
+template <class A, bool TURNED, int STEPS, int GROUPS>
 __global__ __launch_bounds__(WAVES * 64) void wide_run_kernel(WideArgs p, int parts, int run) {
   typedef Wide<A, TURNED> W;
   constexpr int AHEAD = 2;
@@ -571,7 +581,31 @@ __global__ __launch_bounds__(WAVES * 64) void wide_run_kernel(WideArgs p, int pa
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] = mul_split<A>(wh[s][j], wl[s][j], q[0][s], q[1][s], acc[j]);
   };
-  if (__all(same) && parts == 1) {
+  if constexpr (GROUPS > 1) {
+    if (__all(same)) {
+      for (int g = 0; g < groups; g += GROUPS) {
+        f4 acc[GROUPS][8] = {};
+        for (int part = 0; part < parts; ++part) {
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) w.weights(first, (part * STEPS + s) * 32, wh[s], wl[s]);
+#pragma unroll
+          for (int i = 0; i < GROUPS; ++i) {
+            u4 q[2][STEPS];
+            values(min(g + i, groups - 1), part, q);
+            multiply(q, acc[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i)
+          if (g + i < groups) {
+            u4 b[4];
+            w.base(t0 + (g + i) * 16, in(g + i), b);
+            w.put(t0 + (g + i) * 16, in(g + i), acc[i], b);
+          }
+      }
+      return;
+    }
+  } else if (__all(same)) {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) w.weights(first, s * 32, wh[s], wl[s]);
     Tokens k[AHEAD];
@@ -629,29 +663,78 @@ struct OuterSide {
 struct OuterArgs {
   Requests q;
   OuterSide side[2];
-  int R, splits, per_split, direct, tiles;   // per_split: tokens, a multiple of 2 STAGE
+  int32_t* there;           // [splits, n]: whether a part was written; NULL with one split
+  int R, splits, per_split, tiles, turns;   // per_split: tokens, a multiple of STAGE
 };
 
-// out[a][r][c] = s sum over the rows t of adapter a of q[t][r] v[t][c], 16 RT of the r. A wave has 128 columns and one half of the block's rows: eight rows of
-// eight columns a lane are loaded as they lie and transposed in registers; the halves are joined in LDS.
+// out[a][r][c] = s sum over the rows t of adapter a of q[t][r] v[t][c], 16 RT of the r. A block has one run of rows and the adapters that it finds there, one
+// after the other (or every turns-th): what rows share an adapter, and how many adapters have none, changes nothing in how the rows are dealt to blocks. A
+// wave has 128 columns and one half of the rows: eight rows of eight columns a lane are loaded as they lie and transposed in registers; the halves are joined in LDS.
 template <class A, int RT>
 __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
   static_assert(RT <= 2, "64 KB of LDS; four r tiles do not fit the registers beside the rows to come either");
-  __shared__ f4 joined[4][8 * RT][64];
+  constexpr int WORDS = HDMOE_ADAPTER_MAX / 32;
+  static_assert(WORDS == 128, "two words a lane");
+  __shared__ union {
+    uint32_t seen[WORDS];
+    f4 joined[4][8 * RT][64];
+  } lds;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const bool second = (int)blockIdx.x >= p.side[0].blocks;
   const OuterSide side = second ? p.side[1] : p.side[0];
   const int block = second ? blockIdx.x - p.side[0].blocks : blockIdx.x;
-  const int a = blockIdx.y % p.q.n, r0 = blockIdx.y / p.q.n * 16 * RT, split = blockIdx.z;
+  const int turn = blockIdx.y % p.turns, r0 = blockIdx.y / p.turns * 16 * RT, split = blockIdx.z;
   const int c0 = (block * 4 + (wave & 3)) * 128, c = c0 + col * 8, have = side.C - c;
   const bool whole = c0 + 128 <= side.C;
-  f4 acc[RT][8] = {};
-  const int64_t begin = (int64_t)split * p.per_split + (wave >> 2) * (p.per_split / 2);
+  const int64_t start = (int64_t)split * p.per_split;
+  const int64_t begin = start + (wave >> 2) * (p.per_split / 2);
   const int end = (int)min((int64_t)p.q.T, begin + p.per_split / 2);
+  // the adapters of the run, a bit each: word l and l + 64 in lane l
+  uint32_t seen[2] = {0, 0};
+  const int64_t stop = min((int64_t)p.q.T, start + p.per_split);
+  const int head = (int)(start / p.q.rows_per), last = start < p.q.T ? (int)((stop - 1) / p.q.rows_per) : head - 1;
+  if (head == last) {       // one request
+    const int a = p.q.index[head];
+    if (a >= 0 && a < p.q.n) {
+      if ((a >> 5) == lane) seen[0] = 1u << (a & 31);
+      if ((a >> 5) == lane + 64) seen[1] = 1u << (a & 31);
+    }
+  } else {
+    if (threadIdx.x < WORDS) lds.seen[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = head + threadIdx.x; i <= last; i += 512) {
+      const int a = p.q.index[i];
+      if (a >= 0 && a < p.q.n) atomicOr(&lds.seen[a >> 5], 1u << (a & 31));
+    }
+    __syncthreads();
+    seen[0] = lds.seen[lane];
+    seen[1] = lds.seen[lane + 64];
+    __syncthreads();
+  }
+  if (p.there != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && wave == 0)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      for (int j = 0; j < 32; ++j) {
+        const int a = (lane + 64 * h) * 32 + j;
+        if (a < p.q.n) p.there[(size_t)split * p.q.n + a] = (seen[h] >> j) & 1;
+      }
+  // f of every adapter whose bit is `bit`, those of the block's turn
+  auto each = [&](uint32_t flip, auto f) {
+    int at = 0;
+    for (int w = 0; w * 32 < p.q.n; ++w) {
+      uint32_t word = (uint32_t)__builtin_amdgcn_readlane((int)(w < 64 ? seen[0] : seen[1]), w & 63) ^ flip;
+      if (p.q.n - w * 32 < 32) word &= (1u << (p.q.n - w * 32)) - 1;
+      for (; word != 0; word &= word - 1) {
+        if (at == turn) f(w * 32 + __builtin_ctz(word));
+        at = at + 1 == p.turns ? 0 : at + 1;
+      }
+    }
+  };
   // values of 32 rows, r tile r
   auto value = [&](int t, int r, int lo) {
     return *reinterpret_cast<const u4*>(side.rows + (((size_t)(t >> 5) * p.tiles + min((r0 >> 4) + r, p.tiles - 1)) * 128 + 64 * lo + lane) * 8);
   };
+  auto accumulate = [&](int a, f4 (&acc)[RT][8]) {
   if (c0 < side.C)
     for (int t0 = (int)min(begin, (int64_t)p.q.T); t0 < end; t0 += STAGE) {
       const uint64_t first = __ballot(t0 + lane < end && p.q.of(t0 + lane) == a), next = __ballot(t0 + 64 + lane < end && p.q.of(t0 + 64 + lane) == a);
@@ -700,10 +783,15 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
         u4 v[8], qh[RT], ql[RT], keep;
 #pragma unroll
         for (int j = 0; j < 4; ++j) keep[j] = ((eight >> (2 * j)) & 1 ? 0xffffu : 0u) | ((eight >> (2 * j + 1)) & 1 ? 0xffff0000u : 0u);
+        if (whole && has == ~0u) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j] = u4{0, 0, 0, 0};
-          if ((eight >> j) & 1) v[j] = load8(from + (size_t)(st * 32 + j) * side.C, have);
+          for (int j = 0; j < 8; ++j) v[j] = load8(from + (size_t)(st * 32 + j) * side.C);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[j] = u4{0, 0, 0, 0};
+            if ((eight >> j) & 1) v[j] = load8(from + (size_t)(st * 32 + j) * side.C, have);
+          }
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -713,14 +801,11 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
         multiply(v, qh, ql);
       }
     }
-  if (wave >= 4)
-#pragma unroll
-    for (int i = 0; i < 8 * RT; ++i) joined[wave - 4][i][lane] = acc[i / 8][i % 8];
-  __syncthreads();
-  if (wave >= 4 || c0 >= side.C) return;
-#pragma unroll
-  for (int i = 0; i < 8 * RT; ++i) acc[i / 8][i % 8] += joined[wave][i][lane];
-  const size_t at = ((size_t)split * p.q.n + a) * p.R * side.C;
+  };
+  // One adapter's result, 4 r and 8 columns a lane
+  auto store = [&](int a, const f4 (&acc)[RT][8]) {
+    const size_t at = ((size_t)split * p.q.n + a) * p.R * side.C;
+    const bool direct = p.there == nullptr;
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int row = r0 + r * 16 + quad * 4;
@@ -729,7 +814,7 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
       for (int j = 0; j < 8; ++j) {
         if (j >= have || row >= p.R) continue;
         const size_t i = at + (size_t)(c + j) * p.R + row;
-        if (p.direct) {
+        if (direct) {
           uint16_t* to = static_cast<uint16_t*>(side.out) + i;
           const uint32_t o[2] = {A::pack(acc[r][j][0], acc[r][j][1]), A::pack(acc[r][j][2], acc[r][j][3])};
           if (row + 4 <= p.R) __builtin_memcpy(to, o, 8);
@@ -749,7 +834,7 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
       for (int e = 0; e < 4; ++e) {
         if (row + e >= p.R || have <= 0) continue;
         const size_t i = at + (size_t)(row + e) * side.C + c;
-        if (p.direct) {
+        if (direct) {
           u4 o;
 #pragma unroll
           for (int k = 0; k < 4; ++k) o[k] = A::pack(acc[r][2 * k][e], acc[r][2 * k + 1][e]);
@@ -768,6 +853,24 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
       }
     }
   }
+  };
+  each(0, [&](int a) {
+    f4 acc[RT][8] = {};
+    accumulate(a, acc);
+    if (wave >= 4)
+#pragma unroll
+      for (int j = 0; j < 8 * RT; ++j) lds.joined[wave - 4][j][lane] = acc[j / 8][j % 8];
+    __syncthreads();
+    if (wave < 4 && c0 < side.C) {
+#pragma unroll
+      for (int j = 0; j < 8 * RT; ++j) acc[j / 8][j % 8] += lds.joined[wave][j][lane];
+      store(a, acc);
+    }
+    __syncthreads();
+  });
+  if (p.there != nullptr || wave >= 4 || c0 >= side.C) return;
+  const f4 zero[RT][8] = {};
+  each(~0u, [&](int a) { store(a, zero); });      // adapters without rows
 }
 
 // ---- sizes ---------------------------------------------------------------------------------------------------------
@@ -778,10 +881,10 @@ struct Side {                 // a narrow product
 };
 
 struct Plan {
-  int tm, turns, run, few;    // run: many rows; few: one launch
+  int tm, turns, run, few, mixed;   // run: many rows; few: one launch; mixed: rows of several adapters to a tile
   Side h, g;
-  int steps, tiles, splits, per_split, rt;
-  size_t da_bytes, db_bytes, total;
+  int steps, tiles, splits, per_split, rt, outer_turns;
+  size_t da_bytes, db_bytes, there_bytes, total;
 };
 
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -804,7 +907,8 @@ void cut(int tiles, int turns, int K, int rblocks, bool whole, Side& s) {
 Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   Plan p = {};
   const int rows_per = a.rows / a.requests;
-  p.run = a.rows >= MANY_ROWS;
+  p.mixed = rows_per < 16 && a.n > 1 && a.requests > 1;
+  p.run = a.rows >= MANY_ROWS && !p.mixed;
   // tokens of a tile of `narrow`: 16, and more where there are tiles for every CU all the same and a tile's rows share an adapter
   p.tm = rows_per < 64 || a.rows < 32 * HDMOE_NUM_CU ? 1 : a.rows < 64 * HDMOE_NUM_CU || a.R > 64 ? 2 : 4;
   const int tile = 16 * p.tm;
@@ -833,18 +937,27 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   p.h.rows = p.g.rows = rows;
   p.g.rank = rank;
   p.rt = a.R <= 16 ? 1 : 2;
-  // rows are cut over blocks until the card has one a CU, each with 256 of them at least: parts are written and read again
-  const int64_t blocks = (int64_t)(div_up(a.K, 512) + div_up(a.N, 512)) * a.n * div_up(a.R, 16 * p.rt);
-  int splits = div_up(HDMOE_NUM_CU, blocks);
-  const int most = div_up(a.rows, 2 * STAGE);
-  if (splits > most) splits = most;
-  p.per_split = div_up(div_up(a.rows, splits), 2 * STAGE) * 2 * STAGE;
+  // Rows are cut over blocks, 128 each at least, until there are 160 of these: parts are written and read again, and a run is whole stages of both halves (two
+  // adapters of 4096 rows, 2560 and 6912 columns, rank 32: 152 blocks 33 us, 247 39, 133 46); a run's adapters over as many blocks as there
+  // can be adapters in it, if there are CUs for them.
+  const int64_t blocks = (int64_t)(div_up(a.K, 512) + div_up(a.N, 512)) * div_up(a.R, 16 * p.rt);
+  const int cus = div_up(OUTER_BLOCKS, blocks), most = div_up(a.rows, STAGE);
+  const int all = a.n < a.requests ? a.n : a.requests;      // adapters of all rows at most
+  int splits = cus < most ? cus : most;
+  for (int i = 0; i < 2; ++i) {
+    const int each = div_up(a.rows, splits), unit = each > 2 * STAGE ? 2 * STAGE : STAGE;
+    p.per_split = div_up(each, unit) * unit;
+    p.outer_turns = div_up(p.per_split, rows_per);
+    if (p.outer_turns > all) p.outer_turns = all;
+    if (i == 0 && p.outer_turns > 1) splits = div_up(splits, p.outer_turns);
+  }
   p.splits = div_up(a.rows, p.per_split);
   if (p.splits > 1) {
     p.da_bytes = bytes_of((size_t)p.splits * a.n * a.R * a.K * sizeof(float));
     p.db_bytes = bytes_of((size_t)p.splits * a.n * a.R * a.N * sizeof(float));
+    p.there_bytes = bytes_of((size_t)p.splits * a.n * sizeof(int32_t));
   }
-  p.total = p.h.part + p.g.part + p.h.rows + p.g.rows + p.g.rank + p.da_bytes + p.db_bytes;
+  p.total = p.there_bytes + p.h.part + p.g.part + p.h.rows + p.g.rows + p.g.rank + p.da_bytes + p.db_bytes;
   return p;
 }
 
@@ -872,16 +985,27 @@ int narrow_blocks(const NarrowArgs& p, int tm) { return div_up(p.q.T, 16 * tm) *
 
 template <class A, bool TURNED>
 void launch_wide_run(const WideArgs& p, hipStream_t s) {
-  auto go = [&](auto steps) {
-    constexpr int STEPS = decltype(steps)::value;
+  auto go = [&](auto steps, auto groups) {
+    constexpr int STEPS = decltype(steps)::value, GROUPS = decltype(groups)::value;
     // the shortest runs that leave no more blocks than the card holds at once, two a CU
     const int chunks = div_up(p.C, WAVES * Wide<A, TURNED>::COLS), most = chunks < 2 * HDMOE_NUM_CU ? 2 * HDMOE_NUM_CU / chunks : 1;
     int run = div_up(p.q.T, (int64_t)16 * most) * 16;
     if (run > RUN) run = RUN;
-    hipLaunchKernelGGL((wide_run_kernel<A, TURNED, STEPS>), dim3(chunks * div_up(p.q.T, run)), dim3(WAVES * 64), 0, s, p, div_up(p.R, 32 * STEPS), run);
+    hipLaunchKernelGGL((wide_run_kernel<A, TURNED, STEPS, GROUPS>), dim3(chunks * div_up(p.q.T, run)), dim3(WAVES * 64), 0, s, p, div_up(p.R, 32 * STEPS), run);
   };
-  if (p.R <= 32) go(std::integral_constant<int, 1>());
-  else go(std::integral_constant<int, 2>());
+  using std::integral_constant;
+  const integral_constant<int, 1> one;
+  const integral_constant<int, 2> two;
+  if (p.R <= 32) go(one, one);
+  else if (p.R <= 64) go(two, one);
+  else go(one, integral_constant<int, A::HALF ? 3 : 4>());
+}
+
+template <class A, bool TURNED>
+void launch_wide(const WideArgs& p, hipStream_t s) {
+  const dim3 grid(div_up(p.C, WIDE_WAVES * Wide<A, TURNED>::COLS) * div_up(p.q.T, 16) * p.turns);
+  const size_t bytes = p.part != nullptr ? (size_t)2 * 16 * ((p.R + 31) / 32 * 32 + 8) * 2 : 0;
+  hipLaunchKernelGGL((wide_kernel<A, TURNED>), grid, dim3(WIDE_WAVES * 64), bytes, s, p);
 }
 
 int check_args(const hdmoe_adapter_args* a, const char* what, bool backward) {
@@ -953,8 +1077,7 @@ extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t st
     if (plan.run) {
       launch_wide_run<A, false>(wp, s);
     } else {
-      const dim3 grid(div_up(a->N, WIDE_WAVES * Wide<A, false>::COLS) * div_up(a->rows, 16) * plan.turns);
-      hipLaunchKernelGGL(wide_kernel<A>, grid, dim3(WIDE_WAVES * 64), (size_t)2 * 16 * ((a->R + 31) / 32 * 32 + 8) * 2, s, wp);
+      launch_wide<A, false>(wp, s);
     }
   });
   return hdmoe_check_launch("hdmoe_add_adapters");
@@ -992,15 +1115,17 @@ extern "C" int hdmoe_add_adapters_backward(const hdmoe_adapter_args* a, hdmoe_st
   jp.to[1] = {static_cast<uint16_t*>(take(plan.g.rank)), grows, plan.steps, plan.tiles};
   const NarrowArgs hp = {q, bits(a->x), bits(a->a), h, jp.to[0], a->K, a->R, plan.h.slice, plan.h.slices, plan.turns};
   const NarrowArgs gp = {q, bits(a->dy), bits(a->b), g, jp.to[1], a->N, a->R, plan.g.slice, plan.g.slices, plan.turns};
-  const WideArgs wp = {q, nullptr, jp.to[1].rank, bits(a->a), nullptr, static_cast<uint16_t*>(a->dx), a->K, a->R, 1, 1};
+  const WideArgs wp = {q, nullptr, jp.to[1].rank, bits(a->a), nullptr, static_cast<uint16_t*>(a->dx), a->K, a->R, 1, plan.turns};
   OuterArgs op = {};
-  op.q = q, op.R = a->R, op.splits = plan.splits, op.per_split = plan.per_split, op.direct = plan.splits == 1, op.tiles = plan.tiles;
+  op.q = q, op.R = a->R, op.splits = plan.splits, op.per_split = plan.per_split, op.tiles = plan.tiles, op.turns = plan.outer_turns;
+  op.there = static_cast<int32_t*>(take(plan.there_bytes));
   float* da = static_cast<float*>(take(plan.da_bytes));
   float* db = static_cast<float*>(take(plan.db_bytes));
-  op.side[0] = {bits(a->x), jp.to[1].rows, op.direct ? a->da : da, a->K, 0, div_up(a->K, 512)};
-  op.side[1] = {bits(a->dy), jp.to[0].rows, op.direct ? a->db : db, a->N, 1, div_up(a->N, 512)};
+  op.side[0] = {bits(a->x), jp.to[1].rows, plan.splits == 1 ? a->da : da, a->K, 0, div_up(a->K, 512)};
+  op.side[1] = {bits(a->dy), jp.to[0].rows, plan.splits == 1 ? a->db : db, a->N, 1, div_up(a->N, 512)};
   sp.part[0] = da, sp.part[1] = db, sp.splits = plan.splits;
-  const dim3 grid(op.side[0].blocks + op.side[1].blocks, a->n * div_up(a->R, 16 * plan.rt), plan.splits);
+  sp.there = op.there, sp.groups = a->n;
+  const dim3 grid(op.side[0].blocks + op.side[1].blocks, plan.outer_turns * div_up(a->R, 16 * plan.rt), plan.splits);
   typed(a->dtype, [&](auto t) {
     typedef decltype(t) A;
     narrow_shape<true>(a->R, plan.tm, [&](auto rt, auto mode, auto rtg, auto tm) {
@@ -1010,7 +1135,8 @@ extern "C" int hdmoe_add_adapters_backward(const hdmoe_adapter_args* a, hdmoe_st
     });
     if (h != nullptr || g != nullptr)
       hipLaunchKernelGGL(join_kernel, dim3(div_up((int64_t)a->rows * plan.steps * 4, 64), 2), dim3(64), 0, s, jp);
-    launch_wide_run<A, true>(wp, s);
+    if (plan.mixed) launch_wide<A, true>(wp, s);
+    else launch_wide_run<A, true>(wp, s);
     if (plan.rt == 1) hipLaunchKernelGGL((outer_kernel<A, 1>), grid, dim3(512), 0, s, op);
     else hipLaunchKernelGGL((outer_kernel<A, 2>), grid, dim3(512), 0, s, op);
     if (plan.splits > 1) launch_sum_parts<A>(sp, s);

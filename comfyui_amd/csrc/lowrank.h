@@ -164,6 +164,8 @@ struct SumArgs {
   uint16_t* out[2];
   size_t n[2];
   int splits;
+  const int32_t* there;     // [splits, groups]: parts that were written, of equal shares of n; NULL: all
+  int groups;
 };
 template <class A, int GROUPS>
 static __global__ __launch_bounds__(GROUPS == 1 ? 256 : 64 * GROUPS) void sum_parts_kernel(SumArgs p) {
@@ -175,7 +177,34 @@ static __global__ __launch_bounds__(GROUPS == 1 ? 256 : 64 * GROUPS) void sum_pa
   f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
   const int each = (p.splits + GROUPS - 1) / GROUPS, hi = min(p.splits, (group + 1) * each);
   const float* from = p.part[side] + i;
-  if (i + 4 <= n) {
+  if (p.there != nullptr) {
+    const size_t share = n / p.groups;
+    const size_t end = i + 3 < n ? i + 3 : n - 1;
+    const int first = i >= n ? -1 : n < ((size_t)1 << 32) ? (int)((uint32_t)i / (uint32_t)share) : (int)(i / share);
+    const int one = __builtin_amdgcn_readfirstlane(first);
+    const bool simple = i >= n || (first == one && end < ((size_t)one + 1) * share && i + 4 <= n);
+    if (one >= 0 && __all(simple)) {          // the wave's values are of one group: its parts, four at a time
+      for (int s0 = group * each; s0 < hi; s0 += 64) {
+        const int s = s0 + (threadIdx.x & 63);
+        uint64_t left = __ballot(s < hi && p.there[(size_t)s * p.groups + one] != 0);
+        while (left != 0) {
+          f4 q[4] = {};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (left != 0) {
+              if (i < n) __builtin_memcpy(&q[j], from + (size_t)(s0 + __builtin_ctzll(left)) * n, 16);
+              left &= left - 1;
+            }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v += q[j];
+        }
+      }
+    } else if (i < n) {
+      for (int s = group * each; s < hi; ++s)
+        for (int j = 0; j < 4; ++j)
+          if (i + j < n && p.there[(size_t)s * p.groups + (i + j) / share] != 0) v[j] += from[(size_t)s * n + j];
+    }
+  } else if (i + 4 <= n) {
 #pragma unroll 8
     for (int s = group * each; s < hi; ++s) {
       f4 q;

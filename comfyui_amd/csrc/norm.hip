@@ -3,7 +3,7 @@
 //   n = (x - mean) r,  r = 1 / sqrt(mean((x - mean)^2) + eps)      y = n w + b
 //   g = dy w           dx = r (g - mean(g) - n mean(g n))          dw = sum_rows dy n,  db = sum_rows dy
 //
-// A row stays in the registers of one wave (up to 4096 values) or of the four waves of a block (up to 16384), so it is read once, its
+// A row stays in the registers of one wave, or of four or eight of a block where it is long or rows are few, so it is read once, its
 // variance is that of the differences from its mean (nothing cancels), and the backward pass takes mean and r from x again instead of
 // reading what a forward pass would have stored. All sums are fp32; every output is rounded once.
 //
@@ -18,6 +18,7 @@ namespace {
 
 constexpr int V = 8;                 // values a lane takes at a time
 constexpr int NORM_BLOCKS = 512;     // partial sums at most: two blocks a CU
+constexpr int FEW_ROWS = HDMOE_NUM_CU * 8;
 
 struct NormBf16 {
   typedef uint16_t type;
@@ -124,12 +125,14 @@ __device__ __forceinline__ void gains(float (&f)[V], const void* w, int f32, siz
 
 // W waves a row (1: every wave of the block takes rows of its own), C chunks of W * 64 * V values of it.
 // FULL: D is all of them.
+constexpr int threads(int W) { return W > 4 ? W * 64 : 256; }
+
 template <class A, int W, int C, bool FULL>
-__global__ __launch_bounds__(256) void layer_norm_kernel(const typename A::type* __restrict__ x, Gain gain, int64_t rows, int D, float eps,
+__global__ __launch_bounds__(threads(W)) void layer_norm_kernel(const typename A::type* __restrict__ x, Gain gain, int64_t rows, int D, float eps,
                                                          typename A::type* __restrict__ out) {
   __shared__ float lds[2][W][1];
   int turn = 0;
-  constexpr int TEAMS = 4 / W;
+  constexpr int TEAMS = W > 4 ? 1 : 4 / W;
   const int lane = threadIdx.x & (W * 64 - 1);
   const float inv = 1.0f / (float)D;
   int have[C];
@@ -191,8 +194,8 @@ __device__ __forceinline__ void put_grad(void* p, int f32, size_t i, float v) {
 }
 
 template <class A, int W, int C, bool FULL>
-__global__ __launch_bounds__(256) void layer_norm_backward_kernel(NormGrad p) {
-  constexpr int TEAMS = 4 / W;
+__global__ __launch_bounds__(threads(W)) void layer_norm_backward_kernel(NormGrad p) {
+  constexpr int TEAMS = W > 4 ? 1 : 4 / W;
   constexpr int WIDTH = W * 64 * V * C;
   __shared__ float lds[2][W][2];
   __shared__ __attribute__((aligned(16))) float joined[TEAMS][TEAMS > 1 ? WIDTH : 1];
@@ -328,11 +331,11 @@ __global__ __launch_bounds__(1024) void norm_sums_kernel(NormGrad p) {
 
 // One block a group where a second launch (2 us) costs more than the rows that its waves then take one after the other.
 int norm_blocks(int64_t per_group, int64_t groups, int D) {
-  const int teams = D <= 4096 ? 4 : 1;
+  const int teams = D <= 512 || (per_group * groups >= FEW_ROWS && D <= 2560) ? 4 : 1;
   int64_t most = NORM_BLOCKS / (groups > 0 ? groups : 1);
   if (most < 1) most = 1;
-  const int64_t fill = (per_group + teams - 1) / teams;
-  if (fill <= 4) return 1;
+  const int64_t each = D > 8192 ? 2 : teams, fill = (per_group + each - 1) / each;     // 300 rows of 16384: one a block 29 us, two 21
+  if (per_group <= 4 * teams) return 1;
   return (int)(fill < most ? fill : most);
 }
 
@@ -340,27 +343,36 @@ template <class A, int W, int C>
 void launch_norm(bool full, int grid, hipStream_t s, const void* x, const Gain& gain, int64_t rows, int D, float eps, void* out) {
   const typename A::type* xp = static_cast<const typename A::type*>(x);
   typename A::type* op = static_cast<typename A::type*>(out);
-  if (full) hipLaunchKernelGGL((layer_norm_kernel<A, W, C, true>), dim3(grid), dim3(256), 0, s, xp, gain, rows, D, eps, op);
-  else hipLaunchKernelGGL((layer_norm_kernel<A, W, C, false>), dim3(grid), dim3(256), 0, s, xp, gain, rows, D, eps, op);
+  if (full) hipLaunchKernelGGL((layer_norm_kernel<A, W, C, true>), dim3(grid), dim3(threads(W)), 0, s, xp, gain, rows, D, eps, op);
+  else hipLaunchKernelGGL((layer_norm_kernel<A, W, C, false>), dim3(grid), dim3(threads(W)), 0, s, xp, gain, rows, D, eps, op);
 }
 
 template <class A, int W, int C>
 void launch_grad(bool full, int grid, hipStream_t s, const NormGrad& p) {
-  if (full) hipLaunchKernelGGL((layer_norm_backward_kernel<A, W, C, true>), dim3(grid), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((layer_norm_backward_kernel<A, W, C, false>), dim3(grid), dim3(256), 0, s, p);
+  if (full) hipLaunchKernelGGL((layer_norm_backward_kernel<A, W, C, true>), dim3(grid), dim3(threads(W)), 0, s, p);
+  else hipLaunchKernelGGL((layer_norm_backward_kernel<A, W, C, false>), dim3(grid), dim3(threads(W)), 0, s, p);
 }
 
-// f(W, C) with the smallest shape that holds a row
+// f(W, C) with the shape that a row of D values is held in: one wave where there are rows for eight waves of every CU, four where there are fewer (forward
+// of 1021 x 1153 5.5 -> 4.5 us, gradients of 77 x 2560 10.3 -> 9.2) or where the row would take more than five chunks of a wave (12 x 2817 15 -> 9).
 template <class F>
-void norm_shape(int D, F f) {
-  if (D <= 512) f(std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
-  else if (D <= 1024) f(std::integral_constant<int, 1>(), std::integral_constant<int, 2>());
-  else if (D <= 1536) f(std::integral_constant<int, 1>(), std::integral_constant<int, 3>());
-  else if (D <= 2048) f(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
-  else if (D <= 2560) f(std::integral_constant<int, 1>(), std::integral_constant<int, 5>());
-  else if (D <= 4096) f(std::integral_constant<int, 1>(), std::integral_constant<int, 8>());
-  else if (D <= 8192) f(std::integral_constant<int, 4>(), std::integral_constant<int, 4>());
-  else f(std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
+void norm_shape(int D, int64_t rows, F f) {
+  using std::integral_constant;
+  const integral_constant<int, 1> one;
+  const integral_constant<int, 2> two;
+  const integral_constant<int, 3> three;
+  const integral_constant<int, 4> four;
+  if (D <= 512) f(one, one);
+  else if (rows >= FEW_ROWS && D <= 2560) {
+    if (D <= 1024) f(one, two);
+    else if (D <= 1536) f(one, three);
+    else if (D <= 2048) f(one, four);
+    else f(one, integral_constant<int, 5>());
+  } else if (D <= 2048) f(four, one);
+  else if (D <= 4096) f(four, two);
+  else if (D <= 6144) f(four, three);
+  else if (D <= 8192) f(four, four);
+  else f(integral_constant<int, 8>(), four);
 }
 
 bool norm_dtype(int dtype) { return dtype == HDMOE_T_BF16 || dtype == HDMOE_T_F16 || dtype == HDMOE_T_F32; }
@@ -385,9 +397,10 @@ extern "C" int hdmoe_layer_norm(int dtype, const void* x, int64_t rows, int D, i
   HDMOE_REQUIRE_PTR(out);
   const Gain gain = {weight, bias, gain_dtype == HDMOE_T_F32, 0.0f};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  norm_shape(D, [&](auto w, auto c) {
+  norm_shape(D, rows, [&](auto w, auto c) {
     constexpr int W = decltype(w)::value, C = decltype(c)::value;
-    int64_t grid = (rows + 4 / W - 1) / (4 / W);
+    constexpr int TEAMS = W > 4 ? 1 : 4 / W;
+    int64_t grid = (rows + TEAMS - 1) / TEAMS;
     if (grid > HDMOE_NUM_CU * 8) grid = HDMOE_NUM_CU * 8;
     norm_type(dtype, [&](auto a) { launch_norm<decltype(a), W, C>(D == W * 64 * V * C, (int)grid, s, x, gain, rows, D, eps, out); });
   });
@@ -436,7 +449,7 @@ extern "C" int hdmoe_layer_norm_backward(const hdmoe_norm_grad_args* a, hdmoe_st
       return hdmoe_fail(HDMOE_E_WORKSPACE, "hdmoe_layer_norm_backward: workspace of %zu bytes on 16 needed, got %zu", need, a->workspace_bytes);
     p.part = static_cast<float*>(a->workspace);
   }
-  norm_shape(a->D, [&](auto w, auto c) {
+  norm_shape(a->D, a->rows, [&](auto w, auto c) {
     constexpr int W = decltype(w)::value, C = decltype(c)::value;
     norm_type(a->dtype, [&](auto t) { launch_grad<decltype(t), W, C>(a->D == W * 64 * V * C, (int)(groups * p.blocks), s, p); });
   });

@@ -215,3 +215,21 @@ def test_captured_replayed_and_on_another_stream(requests, per):
         for s, out in zip(sets, outs):
             assert all(torch.equal(a, c) for a, c in zip(call(s), out)), turn
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("requests,per,K,N,n,R,used", [(3, 700, 264, 520, 40, 16, (7, 39)), (2, 3000, 136, 648, 300, 24, (299,)), (600, 1, 328, 264, 30, 72, None),
+                                                       (70, 15, 264, 776, 9, 100, None), (70, 16, 264, 776, 9, 33, None), (5, 1, 96, 72, 4096, 8, (0, 31, 32, 4095)),
+                                                       (900, 2, 72, 1032, 700, 8, None), (2, 1500, 1032, 72, 33, 96, (32, 1))])
+def test_many_adapters_of_which_few_are_used(dtype, requests, per, K, N, n, R, used):
+    """Rows dealt to blocks by runs, each with whatever adapters it has: all rows of one, a run with hundreds, most without any rows."""
+    index = None
+    if used is not None:
+        index = torch.tensor(used)[torch.randint(0, len(used), (requests,), generator=torch.Generator().manual_seed(n))]
+    check(problem(n + R, requests, per, K, N, n, R, dtype, index))
+
+
+@pytest.mark.parametrize("R", [65, 96, 128, 200])
+def test_long_ranks_over_runs_of_every_length(R):
+    for rows in (511, 513, 560, 1000):
+        check(problem(R + rows, 1, rows, 200, 392, 1, R, torch.bfloat16 if R % 2 else torch.float16, torch.tensor([0])))
