@@ -381,15 +381,16 @@ struct Wide {
   __device__ __forceinline__ void base(int t, uint32_t want, u4 (&b)[4]) const {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      if constexpr (TURNED) continue;
       b[j] = u4{0, 0, 0, 0};
-      if (p.base != nullptr && ((want >> token(j)) & 1)) {
+      if ((want >> token(j)) & 1) {
         const uint16_t* from = p.base + (size_t)(t + token(j)) * p.C + c;
         b[j] = whole ? load8(from) : load8(from, have);
       }
     }
   }
   __device__ __forceinline__ void put(int t, uint32_t want, const f4 (&acc)[8], u4 (&b)[4]) const {
-    if (p.base != nullptr) quad_transpose(b);
+    if constexpr (!TURNED) quad_transpose(b);
     u4 o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -397,7 +398,8 @@ struct Wide {
       for (int w = 0; w < 4; ++w) {
         const int u = 8 * i + 2 * w;
         const float v0 = TURNED ? acc[u % 8][u / 8] : acc[u / 4][u % 4], v1 = TURNED ? acc[u % 8 + 1][u / 8] : acc[u / 4][u % 4 + 1];
-        o[i][w] = p.base != nullptr ? A::pack(v0 + A::lo(b[i][w]), v1 + A::hi(b[i][w])) : A::pack(v0, v1);
+        if constexpr (TURNED) o[i][w] = A::pack(v0, v1);
+        else o[i][w] = A::pack(v0 + A::lo(b[i][w]), v1 + A::hi(b[i][w]));
       }
     quad_transpose(o);
 #pragma unroll
@@ -416,7 +418,7 @@ struct Wide {
       if ((want >> token(j)) & 1) {
         const size_t at = (size_t)(t + token(j)) * p.C + c;
         u4 v = {0, 0, 0, 0};
-        if (p.base != nullptr) v = load8(p.base + at, have);
+        if constexpr (!TURNED) v = load8(p.base + at, have);
         store8(p.out + at, v, have);
       }
   }
@@ -987,8 +989,10 @@ template <class A, bool TURNED>
 void launch_wide_run(const WideArgs& p, hipStream_t s) {
   auto go = [&](auto steps, auto groups) {
     constexpr int STEPS = decltype(steps)::value, GROUPS = decltype(groups)::value;
-    // the shortest runs that leave no more blocks than the card holds at once, two a CU
-    const int chunks = div_up(p.C, WAVES * Wide<A, TURNED>::COLS), most = chunks < 2 * HDMOE_NUM_CU ? 2 * HDMOE_NUM_CU / chunks : 1;
+    // The shortest runs that leave no more blocks than the card holds at once: two a CU, or three without a base (8192 x 2560, rank 32: 235 blocks 20.8 us, 430
+    // 15.1, 640 12.8, 855 14.2).
+    constexpr int HELD = (TURNED ? 3 : 2) * HDMOE_NUM_CU;
+    const int chunks = div_up(p.C, WAVES * Wide<A, TURNED>::COLS), most = chunks < HELD ? HELD / chunks : 1;
     int run = div_up(p.q.T, (int64_t)16 * most) * 16;
     if (run > RUN) run = RUN;
     hipLaunchKernelGGL((wide_run_kernel<A, TURNED, STEPS, GROUPS>), dim3(chunks * div_up(p.q.T, run)), dim3(WAVES * 64), 0, s, p, div_up(p.R, 32 * STEPS), run);
