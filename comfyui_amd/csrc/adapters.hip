@@ -14,7 +14,6 @@
 
 #include "lowrank.h"
 
-
 using namespace lowrank;
 
 namespace {
@@ -86,7 +85,7 @@ __device__ __forceinline__ void put_planes(const Planes& to, int R, int t, int r
 
 struct NarrowArgs {
   Requests q;
-  const uint16_t *x, *w;    // x [T, K]; w [n, R, K], or [n, K, R] (ACROSS)
+  const uint16_t *x, *w;    // x [T, K]; w [n, R, K], or [n, K, R] (ACROSS, ACROSS32)
   float* part;              // [slices, T, R] fp32, or NULL: to the planes (one slice)
   Planes to;
   int K, R, slice, slices, turns;
@@ -94,7 +93,8 @@ struct NarrowArgs {
 
 // sum over the slice's k of x[t][k] w[a][r][k]. A tile is 16 TM tokens; the block's waves take blocks of 128 k of the slice in turn and join their sums in
 // LDS. Where w runs along r, eight k of eight r a lane are transposed in registers: ACROSS has 128 r side by side in eight instructions, whatever R is;
-// ACROSS32 has up to 32, four k blocks side by side instead, which are then dealt to instructions of 16 r each (8192 x 6912 rows, rank 32: 48 -> 29 us).
+// ACROSS32 has up to 32, four k blocks side by side instead, which are then dealt to instructions of 16 r each: a quarter
+// of the loads and instructions (8192 x 6912 rows, rank 32: 49 -> 44 us, 36 with the rows of the next block on their way).
 enum { ALONG, ACROSS, ACROSS32 };
 template <class A, int MODE, int RT, int TM>
 struct NarrowTile {
@@ -334,8 +334,8 @@ __global__ __launch_bounds__(64) void join_kernel(JoinArgs p) {
 struct WideArgs {
   Requests q;
   const float* part;                  // [slices, T, R] (wide_kernel)
-  const uint16_t* rank;               // Planes::rank (wide_run_kernel)
-  const uint16_t *w, *base;           // w [n, C, R], or [n, R, C] (TURNED); base [T, C] or NULL
+  const uint16_t* rank;               // Planes::rank (wide_run_kernel; wide_kernel without parts)
+  const uint16_t *w, *base;           // w [n, C, R] and base [T, C], or w [n, R, C] and no base (TURNED)
   uint16_t* out;                      // [T, C]
   int C, R, slices, turns;
 };
@@ -737,124 +737,124 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
     return *reinterpret_cast<const u4*>(side.rows + (((size_t)(t >> 5) * p.tiles + min((r0 >> 4) + r, p.tiles - 1)) * 128 + 64 * lo + lane) * 8);
   };
   auto accumulate = [&](int a, f4 (&acc)[RT][8]) {
-  if (c0 < side.C)
-    for (int t0 = (int)min(begin, (int64_t)p.q.T); t0 < end; t0 += STAGE) {
-      const uint64_t first = __ballot(t0 + lane < end && p.q.of(t0 + lane) == a), next = __ballot(t0 + 64 + lane < end && p.q.of(t0 + 64 + lane) == a);
-      if ((first | next) == 0) continue;
-      const bool all = whole && (first & next) == ~0ull;
-      auto multiply = [&](u4 (&v)[8], u4 (&qh)[RT], u4 (&ql)[RT]) {
-        transpose8(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          u4 vh, vl;
-          to_bf16<A>(v[j], vh, vl);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            acc[r][j] = Bf16::mul(ql[r], vh, acc[r][j]);
-            if constexpr (A::HALF) acc[r][j] = Bf16::mul(qh[r], vl, acc[r][j]);
-            acc[r][j] = Bf16::mul(qh[r], vh, acc[r][j]);
-          }
-        }
-      };
-      const uint16_t* from = side.v + (size_t)(t0 + quad * 8) * side.C + c;
-      if (all) {
-        u4 v[2][8];
-        auto load = [&](int st, u4 (&x)[8]) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = load8(from + (size_t)(st * 32 + j) * side.C);
-        };
-        load(0, v[0]);
-#pragma unroll
-        for (int st = 0; st < STAGE / 32; ++st) {
-          u4 qh[RT], ql[RT];
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            qh[r] = value(t0 + st * 32, r, 0);
-            ql[r] = value(t0 + st * 32, r, 1);
-          }
-          if (st + 1 < STAGE / 32) load(st + 1, v[(st + 1) & 1]);
-          multiply(v[st & 1], qh, ql);
-        }
-        continue;
-      }
-      for (int st = 0; st < STAGE / 32; ++st) {
-        const uint32_t has = (uint32_t)((st < 2 ? first : next) >> (32 * (st & 1)));
-        if (has == 0) continue;
-        const uint32_t eight = (has >> (quad * 8)) & 0xff;
-        // rows of another adapter, or past the last one, are 0 on both sides
-        u4 v[8], qh[RT], ql[RT], keep;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) keep[j] = ((eight >> (2 * j)) & 1 ? 0xffffu : 0u) | ((eight >> (2 * j + 1)) & 1 ? 0xffff0000u : 0u);
-        if (whole && has == ~0u) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = load8(from + (size_t)(st * 32 + j) * side.C);
-        } else {
+    if (c0 < side.C)
+      for (int t0 = (int)min(begin, (int64_t)p.q.T); t0 < end; t0 += STAGE) {
+        const uint64_t first = __ballot(t0 + lane < end && p.q.of(t0 + lane) == a), next = __ballot(t0 + 64 + lane < end && p.q.of(t0 + 64 + lane) == a);
+        if ((first | next) == 0) continue;
+        const bool all = whole && (first & next) == ~0ull;
+        auto multiply = [&](u4 (&v)[8], u4 (&qh)[RT], u4 (&ql)[RT]) {
+          transpose8(v);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            v[j] = u4{0, 0, 0, 0};
-            if ((eight >> j) & 1) v[j] = load8(from + (size_t)(st * 32 + j) * side.C, have);
-          }
-        }
+            u4 vh, vl;
+            to_bf16<A>(v[j], vh, vl);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          qh[r] = value(t0 + st * 32, r, 0) & keep;
-          ql[r] = value(t0 + st * 32, r, 1) & keep;
+            for (int r = 0; r < RT; ++r) {
+              acc[r][j] = Bf16::mul(ql[r], vh, acc[r][j]);
+              if constexpr (A::HALF) acc[r][j] = Bf16::mul(qh[r], vl, acc[r][j]);
+              acc[r][j] = Bf16::mul(qh[r], vh, acc[r][j]);
+            }
+          }
+        };
+        const uint16_t* from = side.v + (size_t)(t0 + quad * 8) * side.C + c;
+        if (all) {
+          u4 v[2][8];
+          auto load = [&](int st, u4 (&x)[8]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = load8(from + (size_t)(st * 32 + j) * side.C);
+          };
+          load(0, v[0]);
+#pragma unroll
+          for (int st = 0; st < STAGE / 32; ++st) {
+            u4 qh[RT], ql[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              qh[r] = value(t0 + st * 32, r, 0);
+              ql[r] = value(t0 + st * 32, r, 1);
+            }
+            if (st + 1 < STAGE / 32) load(st + 1, v[(st + 1) & 1]);
+            multiply(v[st & 1], qh, ql);
+          }
+          continue;
         }
-        multiply(v, qh, ql);
+        for (int st = 0; st < STAGE / 32; ++st) {
+          const uint32_t has = (uint32_t)((st < 2 ? first : next) >> (32 * (st & 1)));
+          if (has == 0) continue;
+          const uint32_t eight = (has >> (quad * 8)) & 0xff;
+          // rows of another adapter, or past the last one, are 0 on both sides
+          u4 v[8], qh[RT], ql[RT], keep;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) keep[j] = ((eight >> (2 * j)) & 1 ? 0xffffu : 0u) | ((eight >> (2 * j + 1)) & 1 ? 0xffff0000u : 0u);
+          if (whole && has == ~0u) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = load8(from + (size_t)(st * 32 + j) * side.C);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              v[j] = u4{0, 0, 0, 0};
+              if ((eight >> j) & 1) v[j] = load8(from + (size_t)(st * 32 + j) * side.C, have);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            qh[r] = value(t0 + st * 32, r, 0) & keep;
+            ql[r] = value(t0 + st * 32, r, 1) & keep;
+          }
+          multiply(v, qh, ql);
+        }
       }
-    }
   };
   // One adapter's result, 4 r and 8 columns a lane
   auto store = [&](int a, const f4 (&acc)[RT][8]) {
     const size_t at = ((size_t)split * p.q.n + a) * p.R * side.C;
     const bool direct = p.there == nullptr;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = r0 + r * 16 + quad * 4;
-    if (side.flip) {        // a column's four r next to each other
+    for (int r = 0; r < RT; ++r) {
+      const int row = r0 + r * 16 + quad * 4;
+      if (side.flip) {        // a column's four r next to each other
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j >= have || row >= p.R) continue;
-        const size_t i = at + (size_t)(c + j) * p.R + row;
-        if (direct) {
-          uint16_t* to = static_cast<uint16_t*>(side.out) + i;
-          const uint32_t o[2] = {A::pack(acc[r][j][0], acc[r][j][1]), A::pack(acc[r][j][2], acc[r][j][3])};
-          if (row + 4 <= p.R) __builtin_memcpy(to, o, 8);
-          else
-            for (int e = 0; e < 4; ++e)
-              if (row + e < p.R) to[e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
-        } else {
-          float* to = static_cast<float*>(side.out) + i;
-          if (row + 4 <= p.R) __builtin_memcpy(to, &acc[r][j], 16);
-          else
-            for (int e = 0; e < 4; ++e)
-              if (row + e < p.R) to[e] = acc[r][j][e];
-        }
-      }
-    } else {                // a row's eight columns
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (row + e >= p.R || have <= 0) continue;
-        const size_t i = at + (size_t)(row + e) * side.C + c;
-        if (direct) {
-          u4 o;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) o[k] = A::pack(acc[r][2 * k][e], acc[r][2 * k + 1][e]);
-          store8(static_cast<uint16_t*>(side.out) + i, o, have);
-        } else {
-          float* to = static_cast<float*>(side.out) + i;
-          if (have >= 8) {
-            const f4 o[2] = {{acc[r][0][e], acc[r][1][e], acc[r][2][e], acc[r][3][e]}, {acc[r][4][e], acc[r][5][e], acc[r][6][e], acc[r][7][e]}};
-            __builtin_memcpy(to, o, 32);
+        for (int j = 0; j < 8; ++j) {
+          if (j >= have || row >= p.R) continue;
+          const size_t i = at + (size_t)(c + j) * p.R + row;
+          if (direct) {
+            uint16_t* to = static_cast<uint16_t*>(side.out) + i;
+            const uint32_t o[2] = {A::pack(acc[r][j][0], acc[r][j][1]), A::pack(acc[r][j][2], acc[r][j][3])};
+            if (row + 4 <= p.R) __builtin_memcpy(to, o, 8);
+            else
+              for (int e = 0; e < 4; ++e)
+                if (row + e < p.R) to[e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
           } else {
+            float* to = static_cast<float*>(side.out) + i;
+            if (row + 4 <= p.R) __builtin_memcpy(to, &acc[r][j], 16);
+            else
+              for (int e = 0; e < 4; ++e)
+                if (row + e < p.R) to[e] = acc[r][j][e];
+          }
+        }
+      } else {                // a row's eight columns
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (j < have) to[j] = acc[r][j][e];
+        for (int e = 0; e < 4; ++e) {
+          if (row + e >= p.R || have <= 0) continue;
+          const size_t i = at + (size_t)(row + e) * side.C + c;
+          if (direct) {
+            u4 o;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = A::pack(acc[r][2 * k][e], acc[r][2 * k + 1][e]);
+            store8(static_cast<uint16_t*>(side.out) + i, o, have);
+          } else {
+            float* to = static_cast<float*>(side.out) + i;
+            if (have >= 8) {
+              const f4 o[2] = {{acc[r][0][e], acc[r][1][e], acc[r][2][e], acc[r][3][e]}, {acc[r][4][e], acc[r][5][e], acc[r][6][e], acc[r][7][e]}};
+              __builtin_memcpy(to, o, 32);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (j < have) to[j] = acc[r][j][e];
+            }
           }
         }
       }
     }
-  }
   };
   each(0, [&](int a) {
     f4 acc[RT][8] = {};
@@ -893,8 +893,8 @@ int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 size_t bytes_of(size_t n) { return hdmoe_align_up(n, 256); }
 
-constexpr int64_t FEW_BYTES = 64 << 20;
-constexpr int MANY_ROWS = 512;   // from here on `wide` keeps its weights over runs of tokens
+constexpr int64_t FEW_BYTES = 64 << 20;   // that the blocks of `few` may read
+constexpr int MANY_ROWS = 512;            // from here on `wide` keeps its weights over runs of tokens
 
 // The contraction is cut over blocks until the card has about one a CU, in slices of a block of each wave at least; `whole`: not at all.
 void cut(int tiles, int turns, int K, int rblocks, bool whole, Side& s) {
@@ -1012,7 +1012,7 @@ void launch_wide(const WideArgs& p, hipStream_t s) {
   hipLaunchKernelGGL((wide_kernel<A, TURNED>), grid, dim3(WIDE_WAVES * 64), bytes, s, p);
 }
 
-int check_args(const hdmoe_adapter_args* a, const char* what, bool backward) {
+int check_args(const hdmoe_adapter_args* a, const char* what) {
   if (a == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: args is NULL", what);
   if (a->dtype != HDMOE_T_BF16 && a->dtype != HDMOE_T_F16) return hdmoe_fail(HDMOE_E_SHAPE, "%s: dtype=%d", what, a->dtype);
   if (a->rows < 0 || a->K < 1 || a->N < 1 || a->n < 1 || a->n > HDMOE_ADAPTER_MAX || a->R < 1 || a->R > HDMOE_ADAPTER_MAX_RANK ||
@@ -1042,7 +1042,7 @@ const uint16_t* bits(const void* p) { return static_cast<const uint16_t*>(p); }
 }  // namespace
 
 extern "C" size_t hdmoe_adapters_workspace_bytes(const hdmoe_adapter_args* a, int backward) {
-  if (check_args(a, "hdmoe_adapters_workspace_bytes", backward != 0) != HDMOE_OK || a->rows == 0) return 0;
+  if (check_args(a, "hdmoe_adapters_workspace_bytes") != HDMOE_OK || a->rows == 0) return 0;
   return plan_of(*a, backward != 0).total;
 }
 
@@ -1054,7 +1054,7 @@ static int check_workspace(const hdmoe_adapter_args* a, const Plan& plan, const 
 }
 
 extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t stream) {
-  if (int rc = check_args(a, "hdmoe_add_adapters", false)) return rc;
+  if (int rc = check_args(a, "hdmoe_add_adapters")) return rc;
   if (a->rows == 0) return HDMOE_OK;
   if (a->base == nullptr || a->out == nullptr) return hdmoe_fail(HDMOE_E_NULL, "hdmoe_add_adapters: base or out is NULL");
   const Plan plan = plan_of(*a, false);
@@ -1078,17 +1078,14 @@ extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t st
       constexpr int RT = decltype(rt)::value, TM = decltype(tm)::value;
       hipLaunchKernelGGL((narrow_kernel<A, RT, TM>), dim3(narrow_blocks(np, TM), div_up(a->R, 16 * RT)), dim3(NARROW_WAVES * 64), 0, s, np);
     });
-    if (plan.run) {
-      launch_wide_run<A, false>(wp, s);
-    } else {
-      launch_wide<A, false>(wp, s);
-    }
+    if (plan.run) launch_wide_run<A, false>(wp, s);
+    else launch_wide<A, false>(wp, s);
   });
   return hdmoe_check_launch("hdmoe_add_adapters");
 }
 
 extern "C" int hdmoe_add_adapters_backward(const hdmoe_adapter_args* a, hdmoe_stream_t stream) {
-  if (int rc = check_args(a, "hdmoe_add_adapters_backward", true)) return rc;
+  if (int rc = check_args(a, "hdmoe_add_adapters_backward")) return rc;
   if (a->da == nullptr || a->db == nullptr) return hdmoe_fail(HDMOE_E_NULL, "hdmoe_add_adapters_backward: da or db is NULL");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   SumArgs sp = {};

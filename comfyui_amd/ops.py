@@ -237,9 +237,7 @@ class Adapters(torch.nn.Module):
         index = self.index if self._rows is None else self._rows
         if index is None:
             raise RuntimeError("comfyui_amd.ops.Adapters: set `index`, the adapter of each request, before the forward")
-        x = x.contiguous()
-        base = base.contiguous()
-        return HF.add_adapters(base, x, self.a, self.b, self.scale, index, out=base)
+        return HF.add_adapters(base.contiguous(), x.contiguous(), self.a, self.b, self.scale, index)
 
 
 def adapters_of(lin):
