@@ -23,6 +23,7 @@ constexpr int WIDE_WAVES = 2;              // of `wide`
 constexpr int NARROW_WAVES = 8;
 constexpr int RUN = 256;                   // tokens of a block of `wide_run` at most
 constexpr int OUTER_BLOCKS = 160;          // of `outer`, about
+constexpr size_t OUTER_BYTES = (size_t)1 << 30;   // of its parts at most
 constexpr int STAGE = 128;                 // tokens that `outer` looks at the adapters of at a time
 
 struct Requests {
@@ -945,7 +946,10 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   const int64_t blocks = (int64_t)(div_up(a.K, 512) + div_up(a.N, 512)) * div_up(a.R, 16 * p.rt);
   const int cus = div_up(OUTER_BLOCKS, blocks), most = div_up(a.rows, STAGE);
   const int all = a.n < a.requests ? a.n : a.requests;      // adapters of all rows at most
+  // Parts are of all adapters, those of other rows too: with many of them, fewer runs and in the end none.
+  const size_t one = (size_t)a.n * a.R * ((size_t)a.K + a.N) * sizeof(float);
   int splits = cus < most ? cus : most;
+  if (one * splits > OUTER_BYTES) splits = one < OUTER_BYTES ? (int)(OUTER_BYTES / one) : 1;
   for (int i = 0; i < 2; ++i) {
     const int each = div_up(a.rows, splits), unit = each > 2 * STAGE ? 2 * STAGE : STAGE;
     p.per_split = div_up(each, unit) * unit;

@@ -101,6 +101,14 @@ def test_workspace_stays_within_reason(backward):
         assert (0 if rows == 1 and not backward else 1) <= nb <= 2 * 16 * (rows * R * 4 + 256) + (64 * n * R * (K + N) * 4 if backward and n < 4 else 2 * 4 * n * R * (K + N) * 4) + 1024
 
 
+def test_parts_of_many_adapters_stay_bounded():
+    """Parts of the gradients hold every adapter: with thousands of them the rows are not cut into as many runs."""
+    from comfyui_amd import _lib
+    for rows, requests, n, R in ((16384, 4, 4096, 64), (65536, 8, 1024, 128), (512, 4, 4096, 256), (8192, 8192, 30, 32)):
+        nb = _lib.lib.hdmoe_adapters_workspace_bytes(ctypes.byref(_args(rows=rows, requests=requests, K=2560, N=6912, n=n, R=R)), 1)
+        assert 0 < nb <= (1 << 30) + 2 * 16 * (rows * R * 4 + 256) + 160 * n * 4 + 4096, (rows, n, R, nb)
+
+
 def test_struct_layouts_match_what_a_c_compiler_sees(tmp_path):
     from comfyui_amd import _lib
     structs = {"hdmoe_norm_grad_args": _lib.NormGradArgs, "hdmoe_adapter_args": _lib.AdapterArgs}

@@ -233,3 +233,9 @@ def test_many_adapters_of_which_few_are_used(dtype, requests, per, K, N, n, R, u
 def test_long_ranks_over_runs_of_every_length(R):
     for rows in (511, 513, 560, 1000):
         check(problem(R + rows, 1, rows, 200, 392, 1, R, torch.bfloat16 if R % 2 else torch.float16, torch.tensor([0])))
+
+
+@pytest.mark.parametrize("n,R", [(2048, 16), (2048, 40)])
+def test_parts_that_are_too_many_to_be_cut_as_finely(n, R):
+    """Adapters whose gradients, times the runs that the rows alone would be cut into, pass what the parts may take."""
+    check(problem(n + R, 2, 1500, 72, 1032, n, R, torch.bfloat16, torch.tensor([5, n - 1])))
