@@ -895,6 +895,7 @@ int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 size_t bytes_of(size_t n) { return hdmoe_align_up(n, 256); }
 
 constexpr int64_t FEW_BYTES = 64 << 20;   // that the blocks of `few` may read
+constexpr int64_t LANES_MAX = (int64_t)1 << 32;
 constexpr int MANY_ROWS = 512;            // from here on `wide` keeps its weights over runs of tokens
 
 // The contraction is cut over blocks until the card has about one a CU, in slices of a block of each wave at least; `whole`: not at all.
@@ -1023,13 +1024,18 @@ int check_args(const hdmoe_adapter_args* a, const char* what) {
       a->requests < 0 || (a->rows > 0 && (a->requests == 0 || a->rows % a->requests != 0)))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%d requests=%d K=%d N=%d n=%d (1 to %d) R=%d (1 to %d)", what, a->rows, a->requests, a->K, a->N,
                       a->n, HDMOE_ADAPTER_MAX, a->R, HDMOE_ADAPTER_MAX_RANK);
-  const int64_t blocks = (int64_t)div_up(a->rows, 16) * 16 * (div_up(a->N, 256) + div_up(a->K, 256) + 8);
-  if (blocks >= (int64_t)1 << 31) return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%d K=%d N=%d: too many tiles", what, a->rows, a->K, a->N);
   if (a->K > (1 << 24) || a->N > (1 << 24) || a->rows > (1 << 30))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%d (at most 2^30) K=%d N=%d (at most 2^24)", what, a->rows, a->K, a->N);
   if (a->a == nullptr || a->b == nullptr || a->scale == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: a, b or scale is NULL", what);
   if (a->rows == 0) return HDMOE_OK;
   if (a->x == nullptr || a->index == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: x or index is NULL", what);
+  // A launch has fewer than 2^32 threads, along each of its dimensions: both narrow products of a pair, the planes' groups, and the products back where
+  // tiles have a block for each adapter that they can hold.
+  const int64_t rows_per = a->rows / a->requests, tiles = div_up(a->rows, 16), most = rows_per < 16 ? 16 : 1;
+  const int64_t turns = most < a->n ? most : a->n, narrow = tiles * turns * 2 * NARROW_WAVES * 64 + 16 * NARROW_WAVES * 64 * HDMOE_NUM_CU;
+  const int64_t wide = tiles * turns * div_up(a->K > a->N ? a->K : a->N, 128 * WIDE_WAVES) * WIDE_WAVES * 64, join = (int64_t)a->rows * div_up(a->R, 32) * 4 + 64;
+  if (narrow >= LANES_MAX || join >= LANES_MAX || ((rows_per < 16 || a->rows < MANY_ROWS) && wide >= LANES_MAX))
+    return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%d requests=%d K=%d N=%d: more threads than a launch has", what, a->rows, a->requests, a->K, a->N);
   return HDMOE_OK;
 }
 
@@ -1095,7 +1101,7 @@ extern "C" int hdmoe_add_adapters_backward(const hdmoe_adapter_args* a, hdmoe_st
   SumArgs sp = {};
   sp.out[0] = static_cast<uint16_t*>(a->da), sp.out[1] = static_cast<uint16_t*>(a->db);
   sp.n[0] = (size_t)a->n * a->R * a->K, sp.n[1] = (size_t)a->n * a->R * a->N;
-  if (sp.n[0] + sp.n[1] >= (size_t)1 << 38) return hdmoe_fail(HDMOE_E_SHAPE, "hdmoe_add_adapters_backward: n=%d R=%d K=%d N=%d", a->n, a->R, a->K, a->N);
+  if (sp.n[0] + sp.n[1] >= (size_t)1 << 33) return hdmoe_fail(HDMOE_E_SHAPE, "hdmoe_add_adapters_backward: n=%d R=%d K=%d N=%d", a->n, a->R, a->K, a->N);
   if (a->rows == 0) {   // gradients of zero
     typed(a->dtype, [&](auto t) { launch_sum_parts<decltype(t)>(sp, s); });
     return hdmoe_check_launch("hdmoe_add_adapters_backward");

@@ -99,13 +99,7 @@ struct Gain {
   const void* w;      // NULL: 1
   const void* b;      // NULL: 0
   int f32;            // w and b are fp32, else of the rows' type
-  float plus;         // added to w
 };
-
-template <class A>
-__device__ __forceinline__ float gain_at(const void* w, int f32, size_t i) {
-  return f32 ? static_cast<const float*>(w)[i] : A::one(static_cast<const typename A::type*>(w)[i]);
-}
 
 // Gains of the lane's V columns (16-byte loads where the columns are all there), 0 beyond the row.
 template <class A>
@@ -395,7 +389,7 @@ extern "C" int hdmoe_layer_norm(int dtype, const void* x, int64_t rows, int D, i
   if (rows == 0) return HDMOE_OK;
   HDMOE_REQUIRE_PTR(x);
   HDMOE_REQUIRE_PTR(out);
-  const Gain gain = {weight, bias, gain_dtype == HDMOE_T_F32, 0.0f};
+  const Gain gain = {weight, bias, gain_dtype == HDMOE_T_F32};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   norm_shape(D, rows, [&](auto w, auto c) {
     constexpr int W = decltype(w)::value, C = decltype(c)::value;
@@ -425,7 +419,7 @@ extern "C" int hdmoe_layer_norm_backward(const hdmoe_norm_grad_args* a, hdmoe_st
     return hdmoe_fail(HDMOE_E_SHAPE, "hdmoe_layer_norm_backward: rows=%lld rows_per_group=%lld D=%d (1 to %d) eps=%g", (long long)a->rows,
                       (long long)a->rows_per_group, a->D, HDMOE_NORM_MAX_D, (double)a->eps);
   const int64_t groups = a->rows > 0 ? a->rows / a->rows_per_group : (a->rows_per_group == 0 ? 1 : 0);
-  if (groups > 65535 * (int64_t)NORM_BLOCKS)
+  if (groups >= (int64_t)1 << 23)     // of 512 threads at least: a launch has fewer than 2^32
     return hdmoe_fail(HDMOE_E_SHAPE, "hdmoe_layer_norm_backward: %lld groups", (long long)groups);
   NormGrad p = {};
   p.dy = a->dy, p.x = a->x, p.w = a->weight, p.dx = a->dx, p.dw = a->dweight, p.db = a->dbias;

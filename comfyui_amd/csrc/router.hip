@@ -380,7 +380,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void gate_balance_backward_kernel(Ba
 int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // 16 tokens a tile while that makes at most two blocks a CU, else 64: a quarter of the reads of W
-int balance_tile(int T, int length, int seqs) { return (int64_t)div_up(length, 16) * seqs <= 2 * HDMOE_NUM_CU ? 16 : 64; }
+int balance_tile(int length, int seqs) { return (int64_t)div_up(length, 16) * seqs <= 2 * HDMOE_NUM_CU ? 16 : 64; }
 
 // tokens of a block of the backward kernel
 int balance_split(int T, int D) {
@@ -397,6 +397,9 @@ int check_balance(const hdmoe_balance_args* a, const char* what) {
       a->sequences < 1 || a->T % a->sequences != 0)
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: T=%d sequences=%d D=%d (a multiple of 8) E=%d k=%d (1 to %d)", what, a->T, a->sequences, a->D, a->E, a->k,
                       HDMOE_MAX_EXPERTS);
+  const int length = a->T / a->sequences;
+  if ((int64_t)a->sequences * (div_up(length, balance_tile(length, a->sequences)) + 1) * SCORE_WAVES * 64 >= (int64_t)1 << 32)      // threads of a launch
+    return hdmoe_fail(HDMOE_E_SHAPE, "%s: T=%d sequences=%d: too many", what, a->T, a->sequences);
   if (a->gate_w == nullptr || a->counts == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: gate_w or counts is NULL", what);
   if (a->T > 0 && (a->x == nullptr || a->topk_idx == nullptr || a->scores == nullptr))
     return hdmoe_fail(HDMOE_E_NULL, "%s: x, topk_idx or scores is NULL", what);
@@ -406,7 +409,7 @@ int check_balance(const hdmoe_balance_args* a, const char* what) {
 size_t balance_bytes(const hdmoe_balance_args* a, bool backward) {
   if (!backward) {
     const int length = a->T / a->sequences;
-    return a->T == 0 ? 0 : (size_t)a->sequences * div_up(length, balance_tile(a->T, length, a->sequences)) * sizeof(TileSums);
+    return a->T == 0 ? 0 : (size_t)a->sequences * div_up(length, balance_tile(length, a->sequences)) * sizeof(TileSums);
   }
   const int each = a->T > 0 ? balance_split(a->T, a->D) : 1, splits = div_up(a->T, each);
   return hdmoe_align_up(a->mask != nullptr ? (size_t)a->sequences * sizeof(int32_t) : 0, 256) + (splits > 1 ? (size_t)splits * a->E * a->D * sizeof(float) : 0);
@@ -441,7 +444,7 @@ extern "C" int hdmoe_gate_balance(const hdmoe_balance_args* a, hdmoe_stream_t st
   p.scores = static_cast<float*>(a->scores), p.tiles = static_cast<TileSums*>(a->workspace);
   p.T = a->T, p.length = a->T / a->sequences, p.D = a->D, p.E = a->E, p.k = a->k;
   if (a->T > 0) {
-    const int tile = balance_tile(a->T, p.length, a->sequences);
+    const int tile = balance_tile(p.length, a->sequences);
     p.tiles_per_seq = div_up(p.length, tile);
     typed(a->dtype, [&](auto t) {
       typedef decltype(t) A;

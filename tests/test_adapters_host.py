@@ -109,6 +109,19 @@ def test_parts_of_many_adapters_stay_bounded():
         assert 0 < nb <= (1 << 30) + 2 * 16 * (rows * R * 4 + 256) + 160 * n * 4 + 4096, (rows, n, R, nb)
 
 
+def test_launches_that_are_too_large_are_refused():
+    from comfyui_amd import _lib
+    L = _lib.lib
+    for fn in (L.hdmoe_add_adapters, L.hdmoe_add_adapters_backward):
+        for bad in (dict(rows=1 << 23, requests=1 << 23, K=16, N=16, n=64), dict(rows=1 << 22, requests=1 << 21, K=16, N=16384, n=64),
+                    dict(rows=1 << 28, requests=1, K=16, N=16, R=256), dict(rows=1 << 30, requests=1, K=16, N=16)):
+            assert fn(ctypes.byref(_args(**bad)), None) == _lib.E_SHAPE, bad
+            assert L.hdmoe_adapters_workspace_bytes(ctypes.byref(_args(**bad)), 1) == 0
+        for good in (dict(rows=1 << 20, requests=1 << 20, K=2560, N=2560, n=64), dict(rows=1 << 24, requests=4, K=64, N=64, R=256)):
+            assert fn(ctypes.byref(_args(**good)), None) == _lib.E_WORKSPACE, good
+    assert L.hdmoe_add_adapters_backward(ctypes.byref(_args(n=4096, R=256, K=4096, N=4096)), None) == _lib.E_SHAPE
+
+
 def test_struct_layouts_match_what_a_c_compiler_sees(tmp_path):
     from comfyui_amd import _lib
     structs = {"hdmoe_norm_grad_args": _lib.NormGradArgs, "hdmoe_adapter_args": _lib.AdapterArgs}

@@ -70,6 +70,7 @@ def test_library_refusals_without_a_device():
     assert backward(rows_per_group=300) == _lib.E_SHAPE
     assert backward(rows_per_group=0) == _lib.E_SHAPE
     assert backward(rows=-1) == _lib.E_SHAPE
+    assert backward(rows=1 << 23, rows_per_group=1) == _lib.E_SHAPE        # more threads than a launch has
     assert backward(eps=-1.0) == _lib.E_SHAPE
     assert backward(dy=None) == _lib.E_NULL
     assert backward() == _lib.E_WORKSPACE

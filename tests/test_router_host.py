@@ -85,6 +85,9 @@ def test_library_refusals_without_a_device():
         assert need > 0
         for ws, size in ((None, 0), (ptr, need - 1), (ptr + 4, need)):
             assert fn(ctypes.byref(args(workspace=ws, workspace_bytes=size)), None) == _lib.E_WORKSPACE
+        for bad in (dict(T=1 << 23, sequences=1 << 23), dict(T=1 << 30, sequences=1 << 22)):      # more threads than a launch has
+            assert fn(ctypes.byref(args(**bad)), None) == _lib.E_SHAPE, bad
+        assert fn(ctypes.byref(args(T=1 << 20, sequences=1 << 20)), None) == _lib.E_WORKSPACE
     masked = L.hdmoe_gate_balance_workspace_bytes(ctypes.byref(args(mask=ptr)), 1)
     assert masked > L.hdmoe_gate_balance_workspace_bytes(ctypes.byref(args()), 1)
 
