@@ -1038,6 +1038,12 @@ def ln_modulate_backward(dy, x2d, scale, tokens_per_batch, eps=1e-6):
 
 # ---- the router's balance loss -----------------------------------------------------------------------------------
 
+def _fit_int32(what, **sizes):
+    """ctypes would cut a size that a C int does not hold."""
+    if any(v >= 1 << 31 for v in sizes.values()):
+        raise ValueError(f"{what}: {', '.join(f'{k}={v}' for k, v in sizes.items())} (each below 2^31)")
+
+
 def _balance_args(x2d, gate_w, topk_idx, sequences, mask, alpha, what):
     dt = _act_dtype(x2d, what + " x")
     _need_hip(x2d, what + " x")
@@ -1057,6 +1063,7 @@ def _balance_args(x2d, gate_w, topk_idx, sequences, mask, alpha, what):
         raise ValueError(f"{what}: a mask of {mask.numel()} for {T} tokens")
     if sequences < 1 or T % sequences != 0:
         raise ValueError(f"{what}: {T} tokens in {sequences} sequences")
+    _fit_int32(what, T=T, D=D, sequences=sequences, E=gate_w.shape[0], k=topk_idx.shape[1])
     args = _lib.BalanceArgs()
     args.dtype, args.T, args.sequences, args.D, args.E, args.k, args.alpha = _T_CODE[dt], T, sequences, D, gate_w.shape[0], topk_idx.shape[1], alpha
     args.x, args.gate_w, args.topk_idx, args.mask = ptr(x2d), ptr(gate_w), ptr(topk_idx), ptr(mask)
@@ -1139,6 +1146,7 @@ def _adapter_args(x, a, b, scale, index, what):
     requests = index.numel()
     if rows > 0 and (requests == 0 or rows % requests != 0):
         raise ValueError(f"{what}: {requests} requests do not divide {rows} rows")
+    _fit_int32(what, rows=rows, requests=requests, K=K, N=N, n=n, R=R)
     args = _lib.AdapterArgs()
     args.dtype, args.rows, args.requests, args.K, args.N, args.n, args.R = _T_CODE[dt], rows, requests, K, N, n, R
     args.x, args.a, args.b, args.scale, args.index = ptr(x), ptr(a), ptr(b), ptr(scale), ptr(index)

@@ -138,3 +138,14 @@ def test_struct_layouts_match_what_a_c_compiler_sees(tmp_path):
         assert int(got[cname]) == ctypes.sizeof(cls), cname
         for f, _ in cls._fields_:
             assert int(got[f"{cname}.{f}"]) == getattr(cls, f).offset, f"{cname}.{f}"
+
+
+def test_sizes_that_a_c_int_does_not_hold(monkeypatch):
+    from comfyui_amd import functional as HF
+    monkeypatch.setattr(HF, "_need_hip", lambda *a: None)
+    make = lambda *s, dtype=torch.bfloat16: torch.empty(s, dtype=dtype, device="meta")  # noqa: E731
+    scale, index = make(2, dtype=torch.float32), make(4, dtype=torch.int32)
+    for rows, N in (((1 << 32) + 4, 8), (4, (1 << 32) + 8)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            HF._adapter_args(make(rows, 1), make(2, 8, 1), make(2, N, 8), scale, index, "add_adapters")
+    assert HF._adapter_args(make(8, 1), make(2, 8, 1), make(2, 8, 8), scale, index, "add_adapters").rows == 8

@@ -104,3 +104,13 @@ def test_struct_layout_matches_what_a_c_compiler_sees(tmp_path):
     assert int(got[cname]) == ctypes.sizeof(cls)
     for f, _ in cls._fields_:
         assert int(got[f]) == getattr(cls, f).offset, f
+
+
+def test_sizes_that_a_c_int_does_not_hold(monkeypatch):
+    from comfyui_amd import functional as HF
+    monkeypatch.setattr(HF, "_need_hip", lambda *a: None)
+    make = lambda *s, dtype=torch.bfloat16: torch.empty(s, dtype=dtype, device="meta")  # noqa: E731
+    for T, sequences in (((1 << 32) + 4, 1), ((1 << 32) + 4, (1 << 32) + 4)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            HF._balance_args(make(T, 8), make(4, 8), make(T, 2, dtype=torch.int32), sequences, None, 0.01, "gate_balance")
+    assert HF._balance_args(make(64, 8), make(4, 8), make(64, 2, dtype=torch.int32), 2, None, 0.01, "gate_balance").T == 64
