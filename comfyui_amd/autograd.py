@@ -6,7 +6,8 @@ contiguous first. There is no second derivative.
 
 Captured graphs: torch keeps a gradient accumulator for a leaf for as long as any eager graph of it lives, with the stream of that graph; a backward pass
 that is captured meanwhile would make this stream part of the capture and end the process. These functions cannot see whether one lives and refuse
-inputs with gradients while a graph is captured: there the *_backward functions are called as they are, which is what they are tested for."""
+inputs with gradients while a graph is captured, and a captured backward pass of an eager one: there the *_backward functions are called as they are, which
+is what they are tested for."""
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -19,6 +20,11 @@ def _check(what, *tensors):
         raise RuntimeError(f"autograd.{what}: inputs with gradients while a graph is captured; call functional's {what} and its backward instead")
 
 
+def _check_backward(what):
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"autograd.{what}: a backward pass while a graph is captured; call functional's {what}_backward instead")
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -29,6 +35,7 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _check_backward("layer_norm")
         x, weight, bias = ctx.saved_tensors
         sums = any(ctx.needs_input_grad[1:3])
         dx, dw, db = HF.layer_norm_backward(dy.contiguous(), x, weight, bias, ctx.eps, gains=sums)
@@ -52,6 +59,7 @@ class _Modulate(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _check_backward("ln_modulate")
         x2d, scale = ctx.saved_tensors
         dx, ds, dsh = HF.ln_modulate_backward(dy.contiguous(), x2d, scale, *ctx.args)
         return dx, ds.view(ctx.shapes[0]), dsh.view(ctx.shapes[1]), None, None
@@ -77,6 +85,7 @@ class _Gate(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, _, dweight, dloss, __):
+        _check_backward("gate_balance")
         x2d, gate_w, idx, counts, scores, mask = ctx.saved_tensors
         if dweight is None and dloss is None:
             return None, None, None, None, None
@@ -104,6 +113,7 @@ class _Adapters(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _check_backward("add_adapters")
         dx = da = db = None
         if any(ctx.needs_input_grad[1:4]):
             dx, da, db = HF.add_adapters_backward(dy.contiguous(), *ctx.saved_tensors)

@@ -20,6 +20,26 @@ def test_inputs_with_gradients_are_refused_while_a_graph_is_captured(monkeypatch
             call()
 
 
+def test_a_captured_backward_pass_of_an_eager_call_is_refused(monkeypatch):
+    from comfyui_amd import autograd as A
+    from comfyui_amd import functional as HF
+    like = lambda x, *a: x.clone()  # noqa: E731
+    monkeypatch.setattr(HF, "layer_norm", like)
+    monkeypatch.setattr(HF, "ln_modulate", like)
+    monkeypatch.setattr(HF, "add_adapters", like)
+    monkeypatch.setattr(HF, "gate_top2", lambda x, w: (torch.zeros((4, 2), dtype=torch.int32), x[:, :2].clone()))
+    monkeypatch.setattr(HF, "gate_balance", lambda *a: (torch.zeros(()), torch.zeros((1, 3), dtype=torch.int32), torch.zeros((4, 3))))
+    x = torch.zeros((4, 16), dtype=BF16, requires_grad=True)
+    a, b = torch.zeros((1, 8, 16), dtype=BF16), torch.zeros((1, 16, 8), dtype=BF16)
+    results = [A.layer_norm(x), A.ln_modulate(x, x[:1], x[:1], 4), A.gate(x, torch.zeros((3, 16), dtype=BF16))[2],
+               A.add_adapters(x, x, a, b, torch.ones(1), torch.zeros(1, dtype=torch.int32))]
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for y in results:
+        with pytest.raises(RuntimeError, match="while a graph is captured"):
+            y.sum().backward()
+
+
 def test_scales_have_no_gradient():
     from comfyui_amd import autograd as A
     x = torch.zeros((4, 16), dtype=BF16)
