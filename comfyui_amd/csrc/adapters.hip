@@ -1069,6 +1069,15 @@ extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t st
   if (a->base == nullptr || a->out == nullptr) return hdmoe_fail(HDMOE_E_NULL, "hdmoe_add_adapters: base or out is NULL");
   const Plan plan = plan_of(*a, false);
   if (int rc = check_workspace(a, plan, "hdmoe_add_adapters")) return rc;
+  // `out` may be `base`: a value is read once, by the wave that writes it afterwards. All else is read by several blocks.
+  const size_t value = sizeof(uint16_t), rows = a->rows, out_bytes = rows * a->N * value;
+  auto meets = [&](const void* p, size_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), out = reinterpret_cast<uintptr_t>(a->out);
+    return at < out + out_bytes && out < at + bytes;
+  };
+  if (meets(a->x, rows * a->K * value) || meets(a->a, (size_t)a->n * a->R * a->K * value) || meets(a->b, (size_t)a->n * a->R * a->N * value) ||
+      (a->base != a->out && meets(a->base, out_bytes)))
+    return hdmoe_fail(HDMOE_E_SHAPE, "hdmoe_add_adapters: out overlaps an input (it may be base, as a whole)");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Requests q = requests_of(a);
   float* part = plan.run ? nullptr : static_cast<float*>(a->workspace);

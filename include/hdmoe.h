@@ -445,9 +445,9 @@ int hdmoe_gate_balance_backward(const hdmoe_balance_args* args, hdmoe_stream_t s
  *   dx [rows, K] = scale dy b a (0 for rows without an adapter), da [n, R, K], db [n, N, R]: sums over the rows of each adapter, fp32 in one
  * order that depends on the sizes alone. rows = 0 leaves zeros in da and db.
  *
- * What rows of other adapters hold, NaN among it, never reaches a row or a gradient. (Infinities in a row's own values or adapter can come out as NaN.) Rows
- * of one adapter next to each other are fastest; the gradients look through all rows once for each adapter among them. Outputs may not overlap inputs but for out and base. Rows start on
- * any address of their type; workspace: hdmoe_adapters_workspace_bytes (backward 0 or 1), on 16 bytes, device. */
+ * What rows of other adapters hold, NaN among it, never reaches a row or a gradient. (Infinities in a row's own values or adapter can come out as NaN.)
+ * Rows of one adapter next to each other are fastest; the gradients look through all rows once for each adapter among them. Outputs may not overlap
+ * inputs but for out and base. Rows start on any address of their type; workspace: hdmoe_adapters_workspace_bytes (backward 0 or 1), on 16 bytes, device. */
 #define HDMOE_ADAPTER_MAX 4096
 #define HDMOE_ADAPTER_MAX_RANK 256
 typedef struct hdmoe_adapter_args {

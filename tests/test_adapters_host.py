@@ -122,6 +122,21 @@ def test_launches_that_are_too_large_are_refused():
     assert L.hdmoe_add_adapters_backward(ctypes.byref(_args(n=4096, R=256, K=4096, N=4096)), None) == _lib.E_SHAPE
 
 
+def test_results_over_inputs_are_refused():
+    """base itself takes the result; x, an adapter or a part of base does not, x that is base neither."""
+    from comfyui_amd import _lib
+    L = _lib.lib
+    sizes = dict(rows=64, requests=64, K=256, N=256, n=2, R=16)
+    buf = (ctypes.c_char * (1 << 20))()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    at = {name: p + i * (1 << 16) for i, name in enumerate(("x", "a", "b", "base", "workspace"))}      # 32 KB each at most, but for the workspace
+    for name, shift in (("x", 0), ("x", 32766), ("a", 2), ("b", -32766), ("base", 2), ("base", -2)):
+        args = _args(**sizes, **at, out=at[name] + shift, workspace_bytes=1 << 19)
+        assert L.hdmoe_add_adapters(ctypes.byref(args), None) == _lib.E_SHAPE and b"overlaps" in L.hdmoe_last_error(), (name, shift)
+    args = _args(**sizes, **{**at, "base": at["x"]}, out=at["x"], workspace_bytes=1 << 19)
+    assert L.hdmoe_add_adapters(ctypes.byref(args), None) == _lib.E_SHAPE
+
+
 def test_struct_layouts_match_what_a_c_compiler_sees(tmp_path):
     from comfyui_amd import _lib
     structs = {"hdmoe_norm_grad_args": _lib.NormGradArgs, "hdmoe_adapter_args": _lib.AdapterArgs}
