@@ -693,14 +693,14 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
   const int64_t begin = start + (wave >> 2) * (p.per_split / 2);
   const int end = (int)min((int64_t)p.q.T, begin + p.per_split / 2);
   // the adapters of the run, a bit each: word l and l + 64 in lane l
-  uint32_t seen[2] = {0, 0};
+  uint32_t seen_low = 0, seen_high = 0;
   const int64_t stop = min((int64_t)p.q.T, start + p.per_split);
   const int head = (int)(start / p.q.rows_per), last = start < p.q.T ? (int)((stop - 1) / p.q.rows_per) : head - 1;
   if (head == last) {       // one request
     const int a = p.q.index[head];
     if (a >= 0 && a < p.q.n) {
-      if ((a >> 5) == lane) seen[0] = 1u << (a & 31);
-      if ((a >> 5) == lane + 64) seen[1] = 1u << (a & 31);
+      if ((a >> 5) == lane) seen_low = 1u << (a & 31);
+      if ((a >> 5) == lane + 64) seen_high = 1u << (a & 31);
     }
   } else {
     if (threadIdx.x < WORDS) lds.seen[threadIdx.x] = 0;
@@ -710,8 +710,8 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
       if (a >= 0 && a < p.q.n) atomicOr(&lds.seen[a >> 5], 1u << (a & 31));
     }
     __syncthreads();
-    seen[0] = lds.seen[lane];
-    seen[1] = lds.seen[lane + 64];
+    seen_low = lds.seen[lane];
+    seen_high = lds.seen[lane + 64];
     __syncthreads();
   }
   if (p.there != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && wave == 0)
@@ -719,13 +719,14 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
     for (int h = 0; h < 2; ++h)
       for (int j = 0; j < 32; ++j) {
         const int a = (lane + 64 * h) * 32 + j;
-        if (a < p.q.n) p.there[(size_t)split * p.q.n + a] = (seen[h] >> j) & 1;
+        if (a < p.q.n) p.there[(size_t)split * p.q.n + a] = ((h == 0 ? seen_low : seen_high) >> j) & 1;
       }
   // f of every adapter whose bit is `bit`, those of the block's turn
   auto each = [&](uint32_t flip, auto f) {
     int at = 0;
     for (int w = 0; w * 32 < p.q.n; ++w) {
-      uint32_t word = (uint32_t)__builtin_amdgcn_readlane((int)(w < 64 ? seen[0] : seen[1]), w & 63) ^ flip;
+      const int there = w < 64 ? __builtin_amdgcn_readlane(seen_low, w) : __builtin_amdgcn_readlane(seen_high, w - 64);
+      uint32_t word = (uint32_t)there ^ flip;
       if (p.q.n - w * 32 < 32) word &= (1u << (p.q.n - w * 32)) - 1;
       for (; word != 0; word &= word - 1) {
         if (at == turn) f(w * 32 + __builtin_ctz(word));
