@@ -45,22 +45,26 @@ __device__ __forceinline__ u4 load8(const uint16_t* p) {
   __builtin_memcpy(&v, p, 16);
   return v;
 }
+// Nobody has a part of eight where rows are multiples of eight long: the wave then passes over those loads
 __device__ __forceinline__ u4 load8(const uint16_t* p, int have) {
-  if (have >= 8) return load8(p);
   u4 v = {0, 0, 0, 0};
+  if (have >= 8) {
+    v = load8(p);
+  } else if (have > 0) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < have) v[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
+    for (int j = 0; j < 7; ++j)
+      if (j < have) v[j / 2] |= (uint32_t)p[j] << (16 * (j & 1));
+  }
   return v;
 }
 __device__ __forceinline__ void store8(uint16_t* p, u4 v, int have) {
   if (have >= 8) {
     __builtin_memcpy(p, &v, 16);
-    return;
-  }
+  } else if (have > 0) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < have) p[j] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+    for (int j = 0; j < 7; ++j)
+      if (j < have) p[j] = (uint16_t)(v[j / 2] >> (16 * (j & 1)));
+  }
 }
 
 // v[j] value q <-> v[q] value j: eight rows of eight values become eight columns.
@@ -199,10 +203,26 @@ static __global__ __launch_bounds__(GROUPS == 1 ? 256 : 64 * GROUPS) void sum_pa
           for (int j = 0; j < 4; ++j) v += q[j];
         }
       }
-    } else if (i < n) {
-      for (int s = group * each; s < hi; ++s)
+    } else if (i < n) {                       // of several: flags and values of four parts at a time, whatever the flags say
+      int of[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const size_t at = i + j < n ? i + j : n - 1;
+        of[j] = n < ((size_t)1 << 32) ? (int)((uint32_t)at / (uint32_t)share) : (int)(at / share);
+      }
+#pragma unroll 4
+      for (int s = group * each; s < hi; ++s) {
+        f4 q = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (i + 4 <= n) {
+          __builtin_memcpy(&q, from + (size_t)s * n, 16);
+        } else {
+          for (int j = 0; j < 4; ++j)
+            if (i + j < n) q[j] = from[(size_t)s * n + j];
+        }
+#pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (i + j < n && p.there[(size_t)s * p.groups + (i + j) / share] != 0) v[j] += from[(size_t)s * n + j];
+          if (p.there[(size_t)s * p.groups + of[j]] != 0) v[j] += q[j];
+      }
     }
   } else if (i + 4 <= n) {
 #pragma unroll 8
