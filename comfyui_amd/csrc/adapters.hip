@@ -94,7 +94,7 @@ struct NarrowArgs {
 
 // sum over the slice's k of x[t][k] w[a][r][k]. A tile is 16 TM tokens; the block's waves take blocks of 128 k of the slice in turn and join their sums in
 // LDS. Where w runs along r, eight k of eight r a lane are transposed in registers: ACROSS has 128 r side by side in eight instructions, whatever R is;
-// ACROSS32 has up to 32, four k blocks side by side instead, which are then dealt to instructions of 16 r each: a quarter
+// ACROSS32 has 32, four k blocks side by side instead, which are then dealt to instructions of 16 r each: a quarter
 // of the loads and instructions (8192 x 6912 rows, rank 32: 49 -> 44 us, 36 with the rows of the next block on their way).
 enum { ALONG, ACROSS, ACROSS32 };
 template <class A, int MODE, int RT, int TM>
@@ -149,7 +149,7 @@ struct NarrowTile {
           if (RB < RT) __builtin_amdgcn_sched_barrier(0);
         }
       } else if constexpr (MODE == ACROSS32) {
-        const int r = (col & 3) * 8;
+        const int r = r0 + (col & 3) * 8;
         u4 wv[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {   // past the end x is 0: the last row again
@@ -687,7 +687,11 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
   const OuterSide side = second ? p.side[1] : p.side[0];
   const int block = second ? blockIdx.x - p.side[0].blocks : blockIdx.x;
   const int turn = blockIdx.y % p.turns, r0 = blockIdx.y / p.turns * 16 * RT, split = blockIdx.z;
-  const int c0 = (block * 4 + (wave & 3)) * 128, c = c0 + col * 8, have = side.C - c;
+  // The last 128 columns for a wave that would have fewer: the same loads for all (10220 rows of 1120 and 488 columns, rank 104, 70 -> 36 us). What two waves
+  // have of them is the same sum twice.
+  const int own = (block * 4 + (wave & 3)) * 128;
+  const bool on = own < side.C;
+  const int c0 = on && side.C >= 128 ? min(own, side.C - 128) : own, c = c0 + col * 8, have = side.C - c;
   const bool whole = c0 + 128 <= side.C;
   const int64_t start = (int64_t)split * p.per_split;
   const int64_t begin = start + (wave >> 2) * (p.per_split / 2);
@@ -739,7 +743,7 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
     return *reinterpret_cast<const u4*>(side.rows + (((size_t)(t >> 5) * p.tiles + min((r0 >> 4) + r, p.tiles - 1)) * 128 + 64 * lo + lane) * 8);
   };
   auto accumulate = [&](int a, f4 (&acc)[RT][8]) {
-    if (c0 < side.C)
+    if (on)
       for (int t0 = (int)min(begin, (int64_t)p.q.T); t0 < end; t0 += STAGE) {
         const uint64_t first = __ballot(t0 + lane < end && p.q.of(t0 + lane) == a), next = __ballot(t0 + 64 + lane < end && p.q.of(t0 + 64 + lane) == a);
         if ((first | next) == 0) continue;
@@ -865,14 +869,14 @@ __global__ __launch_bounds__(512, 2) void outer_kernel(OuterArgs p) {
 #pragma unroll
       for (int j = 0; j < 8 * RT; ++j) lds.joined[wave - 4][j][lane] = acc[j / 8][j % 8];
     __syncthreads();
-    if (wave < 4 && c0 < side.C) {
+    if (wave < 4 && on) {
 #pragma unroll
       for (int j = 0; j < 8 * RT; ++j) acc[j / 8][j % 8] += lds.joined[wave][j][lane];
       store(a, acc);
     }
     __syncthreads();
   });
-  if (p.there != nullptr || wave >= 4 || c0 >= side.C) return;
+  if (p.there != nullptr || wave >= 4 || !on) return;
   const f4 zero[RT][8] = {};
   each(~0u, [&](int a) { store(a, zero); });      // adapters without rows
 }
@@ -885,7 +889,7 @@ struct Side {                 // a narrow product
 };
 
 struct Plan {
-  int tm, turns, run, few, mixed;   // run: many rows; few: one launch; mixed: rows of several adapters to a tile
+  int tm, turns, run, few, mixed, fine;   // run: many rows; few: one launch; mixed: rows of several adapters to a tile; fine: 32 r a block of `narrow`
   Side h, g;
   int steps, tiles, splits, per_split, rt, outer_turns;
   size_t da_bytes, db_bytes, there_bytes, total;
@@ -921,7 +925,11 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   if (p.turns > a.n) p.turns = a.n;
   if (p.turns > a.requests) p.turns = a.requests;
   const int tiles = div_up(a.rows, tile);
-  cut(tiles, p.turns, a.K, div_up(a.R, 128), p.run && !backward, p.h);
+  // Long ranks over more blocks where there are few: up to 128 r a block load their weights in turns (130 rows of 416 columns, rank 88, 12.0 -> 6.2 us, 1860 of
+  // 2568, rank 80, 351 blocks, 27 -> 19; but 4000 of 2560, rank 64, 500 blocks, 11.3 -> 14.7: each reads the rows again).
+  p.fine = a.R > 32 && (int64_t)tiles * p.turns * div_up(a.R, 32) <= HDMOE_NUM_CU * 3 / 2;
+  const int rblocks = div_up(a.R, p.fine ? 32 : 128);
+  cut(tiles, p.turns, a.K, rblocks, p.run && !backward, p.h);
   p.steps = div_up(a.R, 32), p.tiles = div_up(a.R, 16);
   const size_t part = (size_t)a.rows * a.R * sizeof(float), rank = (size_t)div_up(a.rows, 16) * p.steps * 2048;
   const size_t rows = (size_t)div_up(a.rows, STAGE) * (STAGE / 32) * p.tiles * 2048;
@@ -936,7 +944,7 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
     p.total = p.h.part + p.h.rank;
     return p;
   }
-  cut(tiles, p.turns, a.N, div_up(a.R, 128), false, p.g);
+  cut(tiles, p.turns, a.N, rblocks, false, p.g);
   p.h.part = p.h.slices > 1 ? bytes_of(part * p.h.slices) : 0;
   p.g.part = p.g.slices > 1 ? bytes_of(part * p.g.slices) : 0;
   p.h.rows = p.g.rows = rows;
@@ -976,9 +984,9 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   return p;
 }
 
-// f(r tiles of 16, mode and r tiles of the turned product, tokens of a tile in 16) as constants; PAIR: both products run
+// f(r tiles of 16, mode and r tiles of the turned product, tokens of a tile in 16) as constants; fine: 32 r a block at most; PAIR: both products run
 template <bool PAIR, class F>
-void narrow_shape(int R, int tm, F f) {
+void narrow_shape(int R, bool fine, int tm, F f) {
   using std::integral_constant;
   auto tokens = [&](auto rt, auto mode, auto rtg) {
     constexpr int most = decltype(rt)::value > 4 || (PAIR && decltype(rtg)::value > 4) ? 2 : 4;
@@ -991,7 +999,7 @@ void narrow_shape(int R, int tm, F f) {
   const integral_constant<int, 2> two;
   const integral_constant<int, 8> eight;
   if (R <= 16) tokens(integral_constant<int, 1>(), narrow, two);
-  else if (R <= 32) tokens(two, narrow, two);
+  else if (R <= 32 || fine) tokens(two, narrow, two);
   else if (R <= 64) tokens(integral_constant<int, 4>(), wide, eight);
   else tokens(eight, wide, eight);
 }
@@ -1101,7 +1109,7 @@ extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t st
       else hipLaunchKernelGGL((few_kernel<A, 4>), grid, dim3(NARROW_WAVES * 64), 0, s, np, wp);
       return;
     }
-    narrow_shape<false>(a->R, plan.tm, [&](auto rt, auto, auto, auto tm) {
+    narrow_shape<false>(a->R, plan.fine, plan.tm, [&](auto rt, auto, auto, auto tm) {
       constexpr int RT = decltype(rt)::value, TM = decltype(tm)::value;
       hipLaunchKernelGGL((narrow_kernel<A, RT, TM>), dim3(narrow_blocks(np, TM), div_up(a->R, 16 * RT)), dim3(NARROW_WAVES * 64), 0, s, np);
     });
@@ -1156,10 +1164,10 @@ extern "C" int hdmoe_add_adapters_backward(const hdmoe_adapter_args* a, hdmoe_st
   const dim3 grid(op.side[0].blocks + op.side[1].blocks, plan.outer_turns * div_up(a->R, 16 * plan.rt), plan.splits);
   typed(a->dtype, [&](auto t) {
     typedef decltype(t) A;
-    narrow_shape<true>(a->R, plan.tm, [&](auto rt, auto mode, auto rtg, auto tm) {
+    narrow_shape<true>(a->R, plan.fine, plan.tm, [&](auto rt, auto mode, auto rtg, auto tm) {
       constexpr int RT = decltype(rt)::value, MODE = decltype(mode)::value, RTG = decltype(rtg)::value, TM = decltype(tm)::value;
       const int nh = narrow_blocks(hp, TM), ng = narrow_blocks(gp, TM);
-      hipLaunchKernelGGL((narrow_pair_kernel<A, MODE, RT, RTG, TM>), dim3(nh + ng, div_up(a->R, 128)), dim3(NARROW_WAVES * 64), 0, s, hp, gp, ng);
+      hipLaunchKernelGGL((narrow_pair_kernel<A, MODE, RT, RTG, TM>), dim3(nh + ng, div_up(a->R, MODE == ACROSS32 ? 32 : 128)), dim3(NARROW_WAVES * 64), 0, s, hp, gp, ng);
     });
     if (h != nullptr || g != nullptr)
       hipLaunchKernelGGL(join_kernel, dim3(div_up((int64_t)a->rows * plan.steps * 4, 64), 2), dim3(64), 0, s, jp);
