@@ -239,3 +239,11 @@ def test_long_ranks_over_runs_of_every_length(R):
 def test_parts_that_are_too_many_to_be_cut_as_finely(n, R):
     """Adapters whose gradients, times the runs that the rows alone would be cut into, pass what the parts may take."""
     check(problem(n + R, 2, 1500, 72, 1032, n, R, torch.bfloat16, torch.tensor([5, n - 1])))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K,N", [(120, 128), (129, 255), (136, 1160), (1025, 511), (2048, 640)])
+def test_columns_that_end_inside_a_wave(dtype, K, N):
+    """Waves that have the last 128 columns over again, or too few columns for that: short and long ranks, one adapter and rows of many."""
+    for requests, per, n, R in ((2, 300, 2, 40), (1, 900, 1, 88), (1, 600, 1, 256), (40, 1, 5, 104), (3, 50, 2, 72)):
+        check(problem(K + N + R, requests, per, K, N, n, R, dtype, None))
