@@ -15,7 +15,8 @@ Linears share a supported storage dtype (bf16, or float8_e4m3fn with fp8 matrix 
 in bf16). Linears with a scale for each block of 128 (ops.block_fp8_ops) run as two launches for all experts
 and the shared one between gate, dispatch and combine. Otherwise it composes the same HIP stages per expert through the Linear modules, which
 needs the per-expert row counts on the host (one sync, as the reference's mask indexing).
-Inputs must be bf16 HIP tensors: there is no CPU path.
+Inputs must be bf16 HIP tensors: there is no CPU path. A Linear with adapters (ops.Adapters) is called by itself, so its
+layer is composed. MoEGate.route is the gate with its balance loss, for training.
 """
 from typing import Optional
 

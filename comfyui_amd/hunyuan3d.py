@@ -8,7 +8,8 @@ and erf-GELU epilogue for the experts.
   MoEGate       hunyuandit.py:73-112  softmax scores, top-k of E unsorted, not renormalised
   MoEBlock      hunyuandit.py:114-188 experts on their tokens, weighted index_add_ in expert order, + shared expert
 
-Inference only (the reference's training branch and auxiliary loss are not part of this path). A token meets at
+Inference only, but for MoEGate.route (the gate with the auxiliary loss and gradients; the reference's training branch of the block is not part
+of this path). A token meets at
 most two experts, so the index_add_ accumulation bf16(bf16(w_a y_a) + bf16(w_b y_b)) is the same two-term sum the
 HiDream combine forms. Inputs must be bf16 or fp16 HIP tensors (fp16 is what model_management.unet_dtype picks for
 this model family on a device with fp16 support, supported_models_base.py:46): there is no CPU path. With fp16
@@ -21,7 +22,8 @@ Three ways through the experts:
     of them and the GELU between;
   * anything else the `operations` argument brings (scaled-fp8 Linears with or without the fp8 matrix multiply,
     manual-cast or offloaded weights, weight functions): one expert at a time through the Linear modules' own
-    forward, the GELU as an elementwise kernel, with the same gate, dispatch and combine kernels around them.
+    forward, the GELU as an elementwise kernel, with the same gate, dispatch and combine kernels around them; so are Linears with
+    adapters (ops.Adapters).
 """
 import torch
 import torch.nn as nn

@@ -1,6 +1,6 @@
 """Operation classes with the attribute and method contract of ComfyUI's comfy.ops,
-restricted to what the HiDream MoE feed-forward uses (Linear), computing on the
-MI355X through libhdmoe.
+restricted to what the HiDream MoE feed-forward uses (Linear, LayerNorm), computing on the
+MI355X through libhdmoe, and low-rank adapters beside a Linear (Adapters).
 
 Reference (paths under /root/reference/comfy): ops.py:61-95 cast_bias_weight,
 :97-100 CastWeightBiasOp, :103-115 disable_weight_init.Linear, :282-284
