@@ -281,8 +281,14 @@ __global__ __launch_bounds__(WAVES * 64, 2) void gate_balance_backward_kernel(Ba
 #pragma unroll
             for (int i = 0; i < 4; ++i) dp[i] += e == i ? d : 0.0f;
           }
+      }
+      // Less the first expert's dp: a softmax's gradient does not change by what all dp of a token have in common, and the sum of s is a rounding away from
+      // 1. Where all dp are the same, as with every expert chosen by every token, the gradient is 0.
+      const float common = __shfl(dp[0], lane & ~3, 64);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dot = __builtin_fmaf(s[i], dp[i], dot);
+      for (int i = 0; i < 4; ++i) {
+        dp[i] -= common;
+        dot = __builtin_fmaf(s[i], dp[i], dot);
       }
       dot += __shfl_xor(dot, 1, 64);
       dot += __shfl_xor(dot, 2, 64);
