@@ -7,6 +7,10 @@
 // variance is that of the differences from its mean (nothing cancels), and the backward pass takes mean and r from x again instead of
 // reading what a forward pass would have stored. All sums are fp32; every output is rounded once.
 //
+// A sum of D values times 1 / D is a few roundings off the mean, of the values' size: for equal values that alone would be their variance, and r up to
+// 1 / sqrt(eps) times it (1000 values of 29952, eps 1e-5: y of 0.5 instead of 0). The sum of the differences f = x - mean goes beside that of their squares and
+// says what the mean lacks: c = sum f / D, mean + c, var = sum f^2 / D - c^2, sum g (f - c) = sum g f - c sum g. Equal values then have differences of 0.
+//
 // The sums over rows of dw and db: a wave keeps them for its columns over all rows that it takes, the waves of a block add theirs up in
 // LDS, and a second kernel adds the blocks' up, each in one fixed order (no atomics). Modulated: a block's rows are of one sequence.
 #include <type_traits>
@@ -79,8 +83,9 @@ __device__ __forceinline__ void wave_sums(float (&v)[N]) {
 
 // The same over the W waves of a block that share a row. `turn` alternates between calls: a wave may be in the next one while another
 // still reads this one's.
-template <int W, int N>
-__device__ __forceinline__ void row_sums(float (&v)[N], float (*lds)[W][N], int& turn) {
+template <int W, int M, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*lds)[W][M], int& turn) {
+  static_assert(N <= M);
   wave_sums(v);
   if constexpr (W > 1) {
     const int wave = threadIdx.x >> 6;
@@ -96,6 +101,12 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*lds)[W][N], int&
     }
     turn ^= 1;
   }
+}
+
+// r from v = sum f^2 / D and c. Past the largest number v says so and c^2 nothing.
+__device__ __forceinline__ float inverse_deviation(float v, float c, float eps) {
+  if (v < __builtin_inff()) v = fmaxf(__builtin_fmaf(-c, c, v), 0.0f);
+  return 1.0f / __builtin_sqrtf(v + eps);
 }
 
 struct Gain {
@@ -127,7 +138,7 @@ constexpr int threads(int W) { return W > 4 ? W * 64 : 256; }
 template <class A, int W, int C, bool FULL>
 __global__ __launch_bounds__(threads(W)) void layer_norm_kernel(const typename A::type* __restrict__ x, Gain gain, int64_t rows, int D, float eps,
                                                          typename A::type* __restrict__ out) {
-  __shared__ float lds[2][W][1];
+  __shared__ float lds[2][W][2];
   int turn = 0;
   constexpr int TEAMS = W > 4 ? 1 : 4 / W;
   const int lane = threadIdx.x & (W * 64 - 1);
@@ -147,16 +158,17 @@ __global__ __launch_bounds__(threads(W)) void layer_norm_kernel(const typename A
       for (int j = 0; j < V; ++j) f[c][j] = raw[c].at(j), s[0] += f[c][j];
     row_sums<W>(s, lds, turn);
     const float mean = s[0] * inv;
-    s[0] = 0.0f;
+    float q[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         f[c][j] = FULL || j < have[c] ? f[c][j] - mean : 0.0f;
-        s[0] = __builtin_fmaf(f[c][j], f[c][j], s[0]);
+        q[0] = __builtin_fmaf(f[c][j], f[c][j], q[0]);
+        q[1] += f[c][j];
       }
-    row_sums<W>(s, lds, turn);
-    const float r = 1.0f / __builtin_sqrtf(s[0] * inv + eps);
+    row_sums<W>(q, lds, turn);
+    const float lacks = q[1] / (float)D, r = inverse_deviation(q[0] * inv, lacks, eps);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (c * W * 64 + lane) * V;
@@ -165,7 +177,7 @@ __global__ __launch_bounds__(threads(W)) void layer_norm_kernel(const typename A
       if (gain.b != nullptr) gains<A>(b, gain.b, gain.f32, col, have[c]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        y[j] = f[c][j] * r;
+        y[j] = (f[c][j] - lacks) * r;
         if (gain.w != nullptr) y[j] *= w[j];
         if (gain.b != nullptr) y[j] += b[j];
       }
@@ -195,7 +207,7 @@ template <class A, int W, int C, bool FULL>
 __global__ __launch_bounds__(threads(W), 2) void layer_norm_backward_kernel(NormGrad p) {
   constexpr int TEAMS = W > 4 ? 1 : 4 / W;
   constexpr int WIDTH = W * 64 * V * C;
-  __shared__ float lds[2][W][2];
+  __shared__ float lds[2][W][3];
   __shared__ __attribute__((aligned(16))) float joined[TEAMS][TEAMS > 1 ? WIDTH : 1];
   int turn = 0;
   const int lane = threadIdx.x & (W * 64 - 1), team = threadIdx.x / (W * 64), D = p.D;
@@ -232,24 +244,25 @@ __global__ __launch_bounds__(threads(W), 2) void layer_norm_backward_kernel(Norm
     }
     row_sums<W>(s, lds, turn);
     const float mean = s[0] * inv, mg = s[1] * inv;
-    s[0] = s[1] = 0.0f;
+    float q[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         f[c][j] = FULL || j < have[c] ? f[c][j] - mean : 0.0f;
-        s[0] = __builtin_fmaf(f[c][j], f[c][j], s[0]);
-        s[1] = __builtin_fmaf(f[c][j], g[c][j], s[1]);
+        q[0] = __builtin_fmaf(f[c][j], f[c][j], q[0]);
+        q[1] = __builtin_fmaf(f[c][j], g[c][j], q[1]);
+        q[2] += f[c][j];
       }
-    row_sums<W>(s, lds, turn);
-    const float r = 1.0f / __builtin_sqrtf(s[0] * inv + p.eps);
-    const float mgn = s[1] * r * inv;   // mean(g n)
+    row_sums<W>(q, lds, turn);
+    const float lacks = q[2] / (float)D, r = inverse_deviation(q[0] * inv, lacks, p.eps);
+    const float mgn = __builtin_fmaf(-lacks, s[1], q[1]) * r * inv;   // mean(g n)
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       float o[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float n = f[c][j] * r, d = ry[c].at(j);
+        const float n = (f[c][j] - lacks) * r, d = ry[c].at(j);
         o[j] = r * (g[c][j] - mg - n * mgn);
         aw[c][j] = __builtin_fmaf(d, n, aw[c][j]);
         ab[c][j] += d;
