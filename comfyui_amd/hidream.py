@@ -267,7 +267,8 @@ class FeedForwardSwiGLU(nn.Module):
             if y is not None:
                 return y
         # per-Linear composition (also the place where a CPU tensor is refused)
-        return self.w2(HF.silu_mul(self.w1(x), self.w3(x)))
+        call = amd_ops.call_linear
+        return call(self.w2, HF.silu_mul(call(self.w1, x), call(self.w3, x)))
 
     def forward_branch(self, x, shift, scale, gate, eps=1e-6):
         """The whole feed-forward branch of a block around a dense feed-forward (the text stream's `ff_t`, or `ff_i`

@@ -62,7 +62,7 @@ class GELU(nn.Module):
         x2 = hidden_states.reshape(-1, hidden_states.shape[-1]).contiguous()
         _need(x2)
         if not _plain_bf16(self.proj, x2):
-            return HF.gelu(self.proj(x2).contiguous()).view(*hidden_states.shape[:-1], self.proj.weight.shape[0])
+            return HF.gelu(amd_ops.call_linear(self.proj, x2).contiguous()).view(*hidden_states.shape[:-1], self.proj.weight.shape[0])
         _, y = HF.grouped_linear(x2[:0], None, [], a_static=x2, shared=(self.proj.weight, self.proj.bias), act="gelu",
                                  fixed_k_cut=amd_ops._batch_invariant(self.proj))
         return y.view(*hidden_states.shape[:-1], self.proj.weight.shape[0])
@@ -123,7 +123,7 @@ class FeedForward(nn.Module):
         _need(x2)
         stages = _stages(self, x2)
         if stages is None:
-            y = self.net[2](self.net[0](x2))     # net[1] is Dropout, the identity at inference
+            y = amd_ops.call_linear(self.net[2], self.net[0](x2))     # net[1] is Dropout, the identity at inference
             return y.view(*hidden_states.shape[:-1], y.shape[-1])
         w_in, w_out = stages
         _, h = HF.grouped_linear(x2[:0], None, [], a_static=x2, shared=w_in, act="gelu",

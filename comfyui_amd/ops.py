@@ -19,6 +19,7 @@ Every forward needs HIP tensors; a CPU tensor raises (the package has no CPU pat
 """
 import contextlib
 import logging
+import types
 
 import weakref
 
@@ -208,7 +209,7 @@ def _linear_upcast(lin, input, scale):
 
 
 class Adapters(torch.nn.Module):
-    """Low-rank adapters of many requests beside a Linear: set as `linear.adapters`, they join each result of its forward. a [n, R, in], b [n, out, R] in the
+    """Low-rank adapters of many requests beside a Linear of this package: set as `linear.adapters`, they join each result of its forward, between its hooks. a [n, R, in], b [n, out, R] in the
     activations' type, scale [n] fp32 (the usual alpha / rank times the strength). `index`, set before a forward, is int32 on the device with the
     adapter of each request in the batch (-1: none), each request having as many rows as the others. Not in the reference, which patches a
     LoRA into the weights: these differ between the requests of one batch, and the weights stay as they are. One forward of a model at a time: `index` is
@@ -220,6 +221,7 @@ class Adapters(torch.nn.Module):
         self.a, self.b = (torch.nn.Parameter(t, requires_grad=False) for t in (a, b))
         self.register_buffer("scale", scale)
         self.index = None
+        self._joined = 0       # results so far
         self._rows = None      # an index for each row, while a routed expert is called (functional.dispatch's order)
 
     @classmethod
@@ -238,7 +240,9 @@ class Adapters(torch.nn.Module):
         index = self.index if self._rows is None else self._rows
         if index is None:
             raise RuntimeError("comfyui_amd.ops.Adapters: set `index`, the adapter of each request, before the forward")
-        return HF.add_adapters(base.contiguous(), x.contiguous(), self.a, self.b, self.scale, index)
+        out = HF.add_adapters(base.contiguous(), x.contiguous(), self.a, self.b, self.scale, index)
+        self._joined += 1
+        return out
 
 
 def adapters_of(lin):
@@ -251,7 +255,7 @@ class routed_adapters:
     perm[r] // 2."""
 
     def __init__(self, module, T, perm):
-        self.on = [ad for ad in (adapters_of(l) for l in module.modules() if isinstance(l, torch.nn.Linear)) if ad is not None]
+        self.on = [ad for ad in (adapters_of(l) for l in module.modules() if isinstance(l, torch.nn.Linear)) if isinstance(ad, Adapters)]
         self.T, self.perm = T, perm
 
     def __enter__(self):
@@ -265,9 +269,40 @@ class routed_adapters:
             ad._rows = None
 
 
-def _with_adapters(lin, input, out):
+class _Forward:
+    """The `forward` of a Linear class: of a module it takes the adapters with it, so that pre-hooks have their say about the input of both and hooks see the
+    whole result. Of the class (`Linear.forward`) it is the function itself, the product alone."""
+
+    def __init__(self, own):
+        self.own = own
+
+    def __get__(self, lin, cls=None):
+        return self.own if lin is None else types.MethodType(self, lin)
+
+    def __call__(self, lin, *args, **kwargs):
+        if not args and "input" in kwargs:
+            args = (kwargs.pop("input"),)
+        out = self.own(lin, *args, **kwargs)
+        ad = adapters_of(lin)
+        if ad is None or next(c.__dict__["forward"] for c in type(lin).__mro__ if "forward" in c.__dict__) is not self:
+            return out      # (a subclass's forward has called its parent's: they join the outer one's result)
+        return ad(out, args[0])
+
+
+def call_linear(lin, input):
+    """lin(input) of a Linear that may be of another operations class, which knows nothing of Adapters: one that leaves them out is refused."""
     ad = adapters_of(lin)
-    return out if ad is None else ad(out, input)
+    if ad is None or isinstance(lin, disable_weight_init.Linear):
+        return lin(input)
+    return _with_adapters(lin, ad, lin, input)
+
+
+def _with_adapters(lin, ad, call, *args, **kwargs):
+    before = getattr(ad, "_joined", None)
+    out = call(*args, **kwargs)
+    if before is not None and ad._joined == before:
+        raise RuntimeError(f"comfyui_amd.ops.Adapters: beside a {type(lin).__module__}.{type(lin).__qualname__} whose forward leaves them out")
+    return out
 
 
 class disable_weight_init:
@@ -300,8 +335,17 @@ class disable_weight_init:
         def reset_parameters(self):
             return None
 
-        def __call__(self, input, *args, **kwargs):
-            return _with_adapters(self, input, super().__call__(input, *args, **kwargs))
+        def __init_subclass__(cls, **kwargs):
+            super().__init_subclass__(**kwargs)
+            own = cls.__dict__.get("forward")
+            if isinstance(own, types.FunctionType):
+                cls.forward = _Forward(own)
+
+        def __call__(self, *args, **kwargs):
+            ad = adapters_of(self)
+            if ad is None:
+                return super().__call__(*args, **kwargs)
+            return _with_adapters(self, ad, super().__call__, *args, **kwargs)     # (a module's or class's `forward` may have been replaced)
 
         def _load_from_state_dict(self, *args, **kwargs):
             invalidate_scale_cache()   # load_state_dict copies into the Parameters in place
@@ -313,6 +357,7 @@ class disable_weight_init:
             weight, bias = cast_bias_weight(self, input)
             return _linear_bf16(input, weight, bias, **_fixed_k_cut(self))
 
+        @_Forward
         def forward(self, *args, **kwargs):
             if self.comfy_cast_weights or len(self.weight_function) > 0 or len(self.bias_function) > 0:
                 return self.forward_comfy_cast_weights(*args, **kwargs)
