@@ -284,9 +284,13 @@ class _Forward:
             args = (kwargs.pop("input"),)
         out = self.own(lin, *args, **kwargs)
         ad = adapters_of(lin)
-        if ad is None or next(c.__dict__["forward"] for c in type(lin).__mro__ if "forward" in c.__dict__) is not self:
+        if ad is None or _class_forward(type(lin)) is not self:
             return out      # (a subclass's forward has called its parent's: they join the outer one's result)
-        return ad(out, args[0])
+        return ad(out, args[0] if args else next(iter(kwargs.values())))
+
+
+def _class_forward(cls):
+    return next(c.__dict__["forward"] for c in cls.__mro__ if "forward" in c.__dict__)
 
 
 def call_linear(lin, input):
@@ -337,8 +341,8 @@ class disable_weight_init:
 
         def __init_subclass__(cls, **kwargs):
             super().__init_subclass__(**kwargs)
-            own = cls.__dict__.get("forward")
-            if isinstance(own, types.FunctionType):
+            own = _class_forward(cls)
+            if not isinstance(own, _Forward):
                 cls.forward = _Forward(own)
 
         def __call__(self, *args, **kwargs):

@@ -78,7 +78,15 @@ def test_subclasses():
         def forward(self, x):
             return x * 5
 
+    class Mixin:
+        def forward(self, x):
+            return super().forward(x) * 2
+
+    class Mixed(Mixin, ops.manual_cast.Linear):
+        pass
+
     with torch.no_grad():
+        assert torch.equal(identity(Mixed)(ONE), 3 * ONE) and torch.equal(identity(Twice)(x=ONE), 3 * ONE)
         assert torch.equal(identity(Twice)(ONE), 3 * ONE)          # they join the outer result
         assert torch.equal(identity(Twice)(input=ONE), 3 * ONE)
         assert torch.equal(identity(Own)(ONE), 6 * ONE) and torch.equal(identity(Own).forward(ONE), 6 * ONE)
