@@ -224,6 +224,14 @@ class Adapters(torch.nn.Module):
         self._joined = 0       # results so far
         self._rows = None      # an index for each row, while a routed expert is called (functional.dispatch's order)
 
+    def _apply(self, fn, recurse=True):
+        """module.to(dtype) moves the scales and leaves their type: they are fp32 beside adapters of any."""
+        scale = self.scale
+        super()._apply(fn, recurse)
+        if self.scale.dtype != scale.dtype:
+            self.scale = scale.to(self.scale.device)
+        return self
+
     @classmethod
     def stack(cls, adapters, dtype=None, device=None):
         """Of [(a [r, in], b [out, r], scale)], whose ranks may differ: those below the largest are filled up with zeros."""

@@ -170,3 +170,21 @@ def test_linears_of_other_classes_in_hunyuan3d(monkeypatch):
                 ff(x)
             del lin.adapters
         assert ff(x).shape == (3, 16)
+
+
+def test_a_cast_of_the_model_leaves_the_scales_fp32():
+    scale = torch.tensor([0.1, 1.0 / 3.0])
+    ad = ops.Adapters(torch.ones((2, 4, 16)), torch.ones((2, 16, 4)), scale.clone())
+    lin = identity()
+    lin.adapters = ad
+    for cast in (lambda m: m.to(BF16), lambda m: m.half(), lambda m: m.to(torch.device("cpu"), torch.bfloat16), lambda m: m.bfloat16().float()):
+        cast(lin)
+        assert ad.scale.dtype == torch.float32 and torch.equal(ad.scale, scale) and ad.a.dtype == lin.weight.dtype and "scale" in ad.state_dict()
+    lin.to(BF16)
+    with torch.no_grad():
+        ad.index = torch.ones(1, dtype=torch.int32)
+        assert lin(ONE.to(BF16)).isfinite().all()
+    lin.to("meta")
+    assert ad.scale.device.type == "meta" and ad.scale.dtype == torch.float32
+    lin.to(torch.float16).to_empty(device="cpu")
+    assert ad.scale.device.type == "cpu" and ad.scale.dtype == torch.float32
