@@ -270,7 +270,9 @@ class routed_adapters:
         for ad in self.on:
             if ad.index is None or ad.index.numel() == 0 or self.T % ad.index.numel() != 0:
                 raise RuntimeError(f"comfyui_amd.ops.Adapters: `index` must be set and divide the {self.T} tokens of the layer")
-            ad._rows = ad.index.reshape(-1)[self.perm // (HF.TOPK * (self.T // ad.index.numel()))]
+        rows = [ad.index.reshape(-1)[self.perm // (HF.TOPK * (self.T // ad.index.numel()))] for ad in self.on]
+        for ad, r in zip(self.on, rows):      # all or, where one of them has no such rows, none: __exit__ follows the former alone
+            ad._rows = r
 
     def __exit__(self, *exc):
         for ad in self.on:

@@ -188,3 +188,22 @@ def test_a_cast_of_the_model_leaves_the_scales_fp32():
     assert ad.scale.device.type == "meta" and ad.scale.dtype == torch.float32
     lin.to(torch.float16).to_empty(device="cpu")
     assert ad.scale.device.type == "cpu" and ad.scale.dtype == torch.float32
+
+
+def test_routed_rows_of_all_adapters_or_none():
+    first, second = identity(), identity()
+    first.adapters.index = torch.tensor([0, -1], dtype=torch.int32)
+    for bad in (None, torch.zeros(3, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)):
+        second.adapters.index = bad
+        with pytest.raises(RuntimeError, match="index"), ops.routed_adapters(torch.nn.ModuleList([first, second]), 4, torch.tensor([7, 0])):
+            pass
+        assert first.adapters._rows is None and second.adapters._rows is None
+    with torch.no_grad():
+        assert torch.equal(first(ONE), torch.cat([2 * ONE[:1], ONE[1:]]))       # by `index`, not by rows of an earlier call
+    second.adapters.index = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(IndexError), ops.routed_adapters(torch.nn.ModuleList([first, second]), 4, torch.tensor([7, 800])):
+        pass
+    assert first.adapters._rows is None
+    with ops.routed_adapters(torch.nn.ModuleList([first, second]), 4, torch.tensor([7, 0])):
+        assert first.adapters._rows.tolist() == [-1, 0] and second.adapters._rows.tolist() == [0, 0]
+    assert first.adapters._rows is None and second.adapters._rows is None
