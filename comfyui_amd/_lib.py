@@ -135,7 +135,7 @@ class BalanceArgs(ctypes.Structure):
 
 class AdapterArgs(ctypes.Structure):
     """hdmoe_adapter_args"""
-    _fields_ = [(n, c_int) for n in ("dtype", "rows", "requests", "K", "N", "n", "R")] + [
+    _fields_ = [(n, c_int) for n in ("dtype", "rows", "requests", "K", "N", "n", "R", "fixed_k_cut")] + [
         (n, c_void_p) for n in ("x", "a", "b", "scale", "index", "base", "out", "dy", "dx", "da", "db", "workspace")] + [
         ("workspace_bytes", c_size_t)]
 

@@ -908,7 +908,8 @@ constexpr int64_t FEW_BYTES = 64 << 20;   // that the blocks of `few` may read
 constexpr int64_t LANES_MAX = (int64_t)1 << 32;
 constexpr int MANY_ROWS = 512;            // from here on `wide` keeps its weights over runs of tokens
 
-// The contraction is cut over blocks until the card has about one a CU, in slices of a block of each wave at least; `whole`: not at all.
+// The contraction is cut over blocks until the card has about one a CU, in slices of a block of each wave at least; `whole`: not at all. A whole one has one
+// order of its additions in every kernel here (each wave's blocks of 128 k in turn, the waves' sums by halves), and so have the sums over the rank.
 void cut(int tiles, int turns, int K, int rblocks, bool whole, Side& s) {
   const int most = div_up(K, NARROW_WAVES * K_BLOCK);
   int want = whole ? 1 : div_up(HDMOE_NUM_CU, (int64_t)tiles * turns * rblocks);
@@ -934,7 +935,7 @@ Plan plan_of(const hdmoe_adapter_args& a, bool backward) {
   // 2568, rank 80, 351 blocks, 27 -> 19; but 4000 of 2560, rank 64, 500 blocks, 11.3 -> 14.7: each reads the rows again).
   p.fine = a.R > 32 && (int64_t)tiles * p.turns * div_up(a.R, 32) <= HDMOE_NUM_CU * 3 / 2;
   const int rblocks = div_up(a.R, p.fine ? 32 : 128);
-  cut(tiles, p.turns, a.K, rblocks, p.run && !backward, p.h);
+  cut(tiles, p.turns, a.K, rblocks, !backward && (p.run || a.fixed_k_cut), p.h);
   p.steps = div_up(a.R, 32), p.tiles = div_up(a.R, 16);
   const size_t part = (size_t)a.rows * a.R * sizeof(float), rank = (size_t)div_up(a.rows, 16) * p.steps * 2048;
   const size_t rows = (size_t)div_up(a.rows, STAGE) * (STAGE / 32) * p.tiles * 2048;

@@ -295,15 +295,18 @@ struct Adapters {
   }
 };
 
-// (base, x, a, b, scale, index, out, stream)
+// (base, x, a, b, scale, index, out, fixed_k_cut, stream)
 PyObject* do_add_adapters(PyObject*, PyObject* const* o, Py_ssize_t count) {
-  HDMOE_ARGUMENTS(8)
+  HDMOE_ARGUMENTS(9)
   return answer([&]() -> PyObject* {
     Adapters c(o[1], o[2], o[3], o[4], o[5]);
     const at::Tensor& base = tensor(o[0]);
     c.beside(base);
     if (o[6] != Py_None) c.beside(tensor(o[6]));
-    void* const stream = stream_of(o[7]);
+    const int fixed = PyObject_IsTrue(o[7]);
+    need(fixed >= 0);
+    c.p.fixed_k_cut = fixed;
+    void* const stream = stream_of(o[8]);
     at::Tensor out = optional(o[6]);
     int rc;
     {

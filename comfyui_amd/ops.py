@@ -179,7 +179,7 @@ def _linear_bf16(input, weight, bias, fixed_k_cut=False):
 
 
 def _batch_invariant(module):
-    """`module.batch_invariant = True` on a Linear: its contraction is never cut along K by the number of rows, so that a row's
+    """`module.batch_invariant = True` on a Linear: its contraction, and that of its adapters, is never cut along K by the number of rows, so that a row's
     bytes do not depend on which rows come with it. Not an attribute of the reference classes."""
     return module.__dict__.get("batch_invariant", False)
 
@@ -242,13 +242,13 @@ class Adapters(torch.nn.Module):
         scale = torch.tensor([float(s) for _, _, s in adapters], dtype=torch.float32)
         return cls(a.to(device=device, dtype=dtype).contiguous(), b.to(device=device, dtype=dtype).contiguous(), scale.to(device))
 
-    def forward(self, base, x):
+    def forward(self, base, x, fixed_k_cut=False):
         if torch.is_grad_enabled() and (self.a.requires_grad or self.b.requires_grad):
             raise RuntimeError("comfyui_amd.ops.Adapters: a Linear with adapters is inference only; autograd.add_adapters has the gradients")
         index = self.index if self._rows is None else self._rows
         if index is None:
             raise RuntimeError("comfyui_amd.ops.Adapters: set `index`, the adapter of each request, before the forward")
-        out = HF.add_adapters(base.contiguous(), x.contiguous(), self.a, self.b, self.scale, index)
+        out = HF.add_adapters(base.contiguous(), x.contiguous(), self.a, self.b, self.scale, index, fixed_k_cut=fixed_k_cut)
         self._joined += 1
         return out
 
@@ -296,7 +296,7 @@ class _Forward:
         ad = adapters_of(lin)
         if ad is None or _class_forward(type(lin)) is not self:
             return out      # (a subclass's forward has called its parent's: they join the outer one's result)
-        return ad(out, args[0] if args else next(iter(kwargs.values())))
+        return ad(out, args[0] if args else next(iter(kwargs.values())), **_fixed_k_cut(lin))
 
 
 def _class_forward(cls):

@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define HDMOE_VERSION 119
+#define HDMOE_VERSION 120
 
 #define HDMOE_OK 0
 #define HDMOE_E_NULL (-1)      /* required pointer is NULL */
@@ -439,7 +439,9 @@ int hdmoe_gate_balance_backward(const hdmoe_balance_args* args, hdmoe_stream_t s
  * rows of out are those of base. x [rows, K], base and out [rows, N] of dtype (bf16 or fp16), a [n, R, K], b [n, N, R] of the same; scale [n] fp32,
  * index [requests] int32, requests a divisor of rows (every request has as many rows; requests = rows: an index for each). R from 1 to
  * HDMOE_ADAPTER_MAX_RANK (adapters of a smaller rank are filled up with zeros), any K and N, n up to HDMOE_ADAPTER_MAX. a . x is held in fp32, and
- * enters the second product with 16 significant bits; sums are fp32, out is rounded once. out may be base.
+ * enters the second product with 16 significant bits; sums are fp32, out is rounded once. out may be base. a . x is cut over blocks where rows are few; fixed_k_cut = 1
+ * leaves it whole whatever the sizes: a row of out then has the same bytes whatever rows, requests and adapters come with it (48 rows of 40 adapters, 6912 x 2560, rank 32,
+ * 14.2 -> 18.8 us). The gradients do not look at it.
  *
  * The gradients, from dy [rows, N], that of out (and of base):
  *   dx [rows, K] = scale dy b a (0 for rows without an adapter), da [n, R, K], db [n, N, R]: sums over the rows of each adapter, fp32 in one
@@ -452,6 +454,7 @@ int hdmoe_gate_balance_backward(const hdmoe_balance_args* args, hdmoe_stream_t s
 #define HDMOE_ADAPTER_MAX_RANK 256
 typedef struct hdmoe_adapter_args {
   int dtype, rows, requests, K, N, n, R;
+  int fixed_k_cut;           /* hdmoe_add_adapters; 0 is the usual choice */
   const void *x, *a, *b;
   const float* scale;
   const int32_t* index;
