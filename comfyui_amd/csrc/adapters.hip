@@ -1039,7 +1039,8 @@ void launch_wide(const WideArgs& p, hipStream_t s) {
   hipLaunchKernelGGL((wide_kernel<A, TURNED>), grid, dim3(WIDE_WAVES * 64), bytes, s, p);
 }
 
-int check_args(const hdmoe_adapter_args* a, const char* what) {
+// Sizes alone: what the workspace depends on
+int check_sizes(const hdmoe_adapter_args* a, const char* what) {
   if (a == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: args is NULL", what);
   if (a->dtype != HDMOE_T_BF16 && a->dtype != HDMOE_T_F16) return hdmoe_fail(HDMOE_E_SHAPE, "%s: dtype=%d", what, a->dtype);
   if (a->rows < 0 || a->K < 1 || a->N < 1 || a->n < 1 || a->n > HDMOE_ADAPTER_MAX || a->R < 1 || a->R > HDMOE_ADAPTER_MAX_RANK ||
@@ -1048,9 +1049,7 @@ int check_args(const hdmoe_adapter_args* a, const char* what) {
                       a->n, HDMOE_ADAPTER_MAX, a->R, HDMOE_ADAPTER_MAX_RANK);
   if (a->K > (1 << 24) || a->N > (1 << 24) || a->rows > (1 << 30))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%d (at most 2^30) K=%d N=%d (at most 2^24)", what, a->rows, a->K, a->N);
-  if (a->a == nullptr || a->b == nullptr || a->scale == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: a, b or scale is NULL", what);
   if (a->rows == 0) return HDMOE_OK;
-  if (a->x == nullptr || a->index == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: x or index is NULL", what);
   // A launch has fewer than 2^32 threads, along each of its dimensions: both narrow products of a pair, the planes' groups, and the products back where
   // tiles have a block for each adapter that they can hold.
   const int64_t rows_per = a->rows / a->requests, tiles = div_up(a->rows, 16), most = rows_per < 16 ? 16 : 1;
@@ -1058,6 +1057,13 @@ int check_args(const hdmoe_adapter_args* a, const char* what) {
   const int64_t wide = tiles * turns * div_up(a->K > a->N ? a->K : a->N, 128 * WIDE_WAVES) * WIDE_WAVES * 64, join = (int64_t)a->rows * div_up(a->R, 32) * 4 + 64;
   if (narrow >= LANES_MAX || join >= LANES_MAX || ((rows_per < 16 || a->rows < MANY_ROWS) && wide >= LANES_MAX))
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: rows=%d requests=%d K=%d N=%d: more threads than a launch has", what, a->rows, a->requests, a->K, a->N);
+  return HDMOE_OK;
+}
+
+int check_args(const hdmoe_adapter_args* a, const char* what) {
+  if (int rc = check_sizes(a, what)) return rc;
+  if (a->a == nullptr || a->b == nullptr || a->scale == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: a, b or scale is NULL", what);
+  if (a->rows > 0 && (a->x == nullptr || a->index == nullptr)) return hdmoe_fail(HDMOE_E_NULL, "%s: x or index is NULL", what);
   return HDMOE_OK;
 }
 
@@ -1074,7 +1080,7 @@ const uint16_t* bits(const void* p) { return static_cast<const uint16_t*>(p); }
 }  // namespace
 
 extern "C" size_t hdmoe_adapters_workspace_bytes(const hdmoe_adapter_args* a, int backward) {
-  if (check_args(a, "hdmoe_adapters_workspace_bytes") != HDMOE_OK || a->rows == 0) return 0;
+  if (check_sizes(a, "hdmoe_adapters_workspace_bytes") != HDMOE_OK || a->rows == 0) return 0;
   return plan_of(*a, backward != 0).total;
 }
 

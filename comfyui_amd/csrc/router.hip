@@ -396,7 +396,8 @@ int balance_split(int T, int D) {
   return each;
 }
 
-int check_balance(const hdmoe_balance_args* a, const char* what) {
+// Sizes alone: what the workspace depends on, beside whether there is a mask
+int check_sizes(const hdmoe_balance_args* a, const char* what) {
   if (a == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: args is NULL", what);
   if (a->dtype != HDMOE_T_BF16 && a->dtype != HDMOE_T_F16) return hdmoe_fail(HDMOE_E_SHAPE, "%s: dtype=%d", what, a->dtype);
   if (a->T < 0 || a->T > (1 << 30) || a->D < 8 || a->D % 8 != 0 || a->D > (1 << 24) || a->E < 1 || a->E > HDMOE_MAX_EXPERTS || a->k < 1 || a->k > HDMOE_MAX_EXPERTS ||
@@ -406,6 +407,11 @@ int check_balance(const hdmoe_balance_args* a, const char* what) {
   const int length = a->T / a->sequences;
   if ((int64_t)a->sequences * (div_up(length, balance_tile(length, a->sequences)) + 1) * SCORE_WAVES * 64 >= (int64_t)1 << 32)      // threads of a launch
     return hdmoe_fail(HDMOE_E_SHAPE, "%s: T=%d sequences=%d: too many", what, a->T, a->sequences);
+  return HDMOE_OK;
+}
+
+int check_balance(const hdmoe_balance_args* a, const char* what) {
+  if (int rc = check_sizes(a, what)) return rc;
   if (a->gate_w == nullptr || a->counts == nullptr) return hdmoe_fail(HDMOE_E_NULL, "%s: gate_w or counts is NULL", what);
   if (a->T > 0 && (a->x == nullptr || a->topk_idx == nullptr || a->scores == nullptr))
     return hdmoe_fail(HDMOE_E_NULL, "%s: x, topk_idx or scores is NULL", what);
@@ -430,7 +436,7 @@ void typed(int dtype, F f) {
 }  // namespace
 
 extern "C" size_t hdmoe_gate_balance_workspace_bytes(const hdmoe_balance_args* a, int backward) {
-  return check_balance(a, "hdmoe_gate_balance_workspace_bytes") == HDMOE_OK ? balance_bytes(a, backward != 0) : 0;
+  return check_sizes(a, "hdmoe_gate_balance_workspace_bytes") == HDMOE_OK ? balance_bytes(a, backward != 0) : 0;
 }
 
 static int check_workspace(const hdmoe_balance_args* a, bool backward, const char* what) {

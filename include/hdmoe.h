@@ -413,7 +413,8 @@ int hdmoe_layer_norm_backward(const hdmoe_norm_grad_args* args, hdmoe_stream_t s
  * The gradients, from dloss (one fp32 on the device; counts carry none) and, unless NULL, dweight [T, k] of dtype, that of the chosen scores
  * scores[t, topk_idx[t, j]]: dx [T, D] and dgate_w [E, D] of dtype. scores and counts are those of the forward call. Sums over tokens are
  * fp32 in an order that depends on the sizes alone. Outputs may not overlap inputs; rows start on any address of their type. workspace:
- * hdmoe_gate_balance_workspace_bytes (backward 0 or 1; it looks at mask for NULL), on 16 bytes, device. */
+ * hdmoe_gate_balance_workspace_bytes (backward 0 or 1; it looks at the sizes and whether mask is NULL, and answers 0 for sizes that the calls refuse, too), on 16
+ * bytes, device. */
 typedef struct hdmoe_balance_args {
   int dtype, T, sequences, D, E, k;
   float alpha;
@@ -449,7 +450,8 @@ int hdmoe_gate_balance_backward(const hdmoe_balance_args* args, hdmoe_stream_t s
  *
  * What rows of other adapters hold, NaN among it, never reaches a row or a gradient. (Infinities in a row's own values or adapter can come out as NaN.)
  * Rows of one adapter next to each other are fastest; the gradients look through all rows once for each adapter among them. Outputs may not overlap
- * inputs but for out and base. Rows start on any address of their type; workspace: hdmoe_adapters_workspace_bytes (backward 0 or 1), on 16 bytes, device. */
+ * inputs but for out and base. Rows start on any address of their type; workspace: hdmoe_adapters_workspace_bytes (backward 0 or 1; it looks at the sizes and
+ * fixed_k_cut alone, and answers 0 for sizes that the calls refuse, too), on 16 bytes, device. */
 #define HDMOE_ADAPTER_MAX 4096
 #define HDMOE_ADAPTER_MAX_RANK 256
 typedef struct hdmoe_adapter_args {
