@@ -1104,7 +1104,7 @@ extern "C" int hdmoe_add_adapters(const hdmoe_adapter_args* a, hdmoe_stream_t st
     return at < out + out_bytes && out < at + bytes;
   };
   if (meets(a->x, rows * a->K * value) || meets(a->a, (size_t)a->n * a->R * a->K * value) || meets(a->b, (size_t)a->n * a->R * a->N * value) ||
-      (a->base != a->out && meets(a->base, out_bytes)))
+      meets(a->scale, a->n * sizeof(float)) || meets(a->index, a->requests * sizeof(int32_t)) || (a->base != a->out && meets(a->base, out_bytes)))
     return hdmoe_fail(HDMOE_E_SHAPE, "hdmoe_add_adapters: out overlaps an input (it may be base, as a whole)");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Requests q = requests_of(a);
