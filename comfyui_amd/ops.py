@@ -343,7 +343,7 @@ class disable_weight_init:
         def forward(self, *args, **kwargs):
             if self.comfy_cast_weights or len(self.weight_function) > 0 or len(self.bias_function) > 0:
                 return self.forward_comfy_cast_weights(*args, **kwargs)
-            return self._norm(args[0], self.weight, self.bias)
+            return self._norm(*args, **kwargs, weight=self.weight, bias=self.bias)
 
     class Linear(torch.nn.Linear, CastWeightBiasOp):
         def reset_parameters(self):
