@@ -248,6 +248,8 @@ class Adapters(torch.nn.Module):
         index = self.index if self._rows is None else self._rows
         if index is None:
             raise RuntimeError("comfyui_amd.ops.Adapters: set `index`, the adapter of each request, before the forward")
+        if x.dim() == 1:      # a row, as the Linear takes it
+            return self.forward(base[None], x[None], fixed_k_cut)[0]
         out = HF.add_adapters(base.contiguous(), x.contiguous(), self.a, self.b, self.scale, index, fixed_k_cut=fixed_k_cut)
         self._joined += 1
         return out

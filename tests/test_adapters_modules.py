@@ -12,6 +12,7 @@ BF16 = torch.bfloat16
 @pytest.fixture(autouse=True)
 def on_the_cpu(monkeypatch):
     def add_adapters(base, x, a, b, scale, index, **kwargs):
+        assert x.dim() >= 2 and base.shape[:-1] == x.shape[:-1]
         out = base.clone().reshape(-1, base.shape[-1])
         per = x.numel() // x.shape[-1] // index.numel()
         for t, row in enumerate(x.reshape(-1, x.shape[-1])):
@@ -207,3 +208,10 @@ def test_routed_rows_of_all_adapters_or_none():
     with ops.routed_adapters(torch.nn.ModuleList([first, second]), 4, torch.tensor([7, 0])):
         assert first.adapters._rows.tolist() == [-1, 0] and second.adapters._rows.tolist() == [0, 0]
     assert first.adapters._rows is None and second.adapters._rows is None
+
+
+def test_a_single_row_without_an_axis_of_its_own():
+    lin = identity()
+    with torch.no_grad():
+        y = lin(ONE[0])
+    assert y.shape == (16,) and torch.equal(y, 2 * ONE[0])
