@@ -286,19 +286,19 @@ class _Forward:
     whole result. Of the class (`Linear.forward`) it is the function itself, the product alone."""
 
     def __init__(self, own):
-        self.own = own
+        def joined(lin, *args, **kwargs):
+            if not args and "input" in kwargs:
+                args = (kwargs.pop("input"),)
+            out = own(lin, *args, **kwargs)
+            ad = adapters_of(lin)
+            if ad is None or _class_forward(type(lin)) is not self:
+                return out      # (a subclass's forward has called its parent's: they join the outer one's result)
+            return ad(out, args[0] if args else next(iter(kwargs.values())), **_fixed_k_cut(lin))
+
+        self.own, self.joined = own, joined
 
     def __get__(self, lin, cls=None):
-        return self.own if lin is None else types.MethodType(self, lin)
-
-    def __call__(self, lin, *args, **kwargs):
-        if not args and "input" in kwargs:
-            args = (kwargs.pop("input"),)
-        out = self.own(lin, *args, **kwargs)
-        ad = adapters_of(lin)
-        if ad is None or _class_forward(type(lin)) is not self:
-            return out      # (a subclass's forward has called its parent's: they join the outer one's result)
-        return ad(out, args[0] if args else next(iter(kwargs.values())), **_fixed_k_cut(lin))
+        return self.own if lin is None else types.MethodType(self.joined, lin)
 
 
 def _class_forward(cls):
