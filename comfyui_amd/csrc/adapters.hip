@@ -1016,8 +1016,9 @@ template <class A, bool TURNED>
 void launch_wide_run(const WideArgs& p, hipStream_t s) {
   auto go = [&](auto steps, auto groups) {
     constexpr int STEPS = decltype(steps)::value, GROUPS = decltype(groups)::value;
-    // The shortest runs that leave no more blocks than the card holds at once: two a CU, or three without a base (8192 x 2560, rank 32: 235 blocks 20.8 us, 430
-    // 15.1, 640 12.8, 855 14.2).
+    // The shortest runs that leave no more blocks than two a CU, or three without a base (8192 x 2560, rank 32: 235 blocks 20.8 us, 430 15.1, 640 12.8, 855
+    // 14.2). That is what the card holds at once of bf16 up to rank 64 with a base and up to 32 without; by their registers it holds two of the other instances
+    // without a base (fp16 over 64: one), and one with a base of fp16 over 32 and of all over 64, whose blocks then come in two turns or more.
     constexpr int HELD = (TURNED ? 3 : 2) * HDMOE_NUM_CU;
     const int chunks = div_up(p.C, WAVES * Wide<A, TURNED>::COLS), most = chunks < HELD ? HELD / chunks : 1;
     int run = div_up(p.q.T, (int64_t)16 * most) * 16;
