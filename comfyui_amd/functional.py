@@ -1172,7 +1172,8 @@ def add_adapters(base, x, a, b, scale, index, out=None, fixed_k_cut=False):
     smaller rank filled up with zeros; scale [n] fp32. index: int32, one for each request, each of as many rows of x in turn (x [B, S, K] with index [B]; an
     index for each row: index [rows]); negative or from n on: no adapter, and the row is base's. Sums are fp32, the narrow product between the two
     keeps 16 significant bits, the result is rounded once; infinities in a row's own values or adapter, or in the narrow product, can come out as NaN. `out`: takes the result, base itself if it is to be
-    added in place; it overlaps nothing else. fixed_k_cut: a row's bytes do not depend on the rows, requests and adapters that come with it (a @ x is otherwise cut by their number)."""
+    added in place; it overlaps nothing else. fixed_k_cut: a row's bytes do not depend on the rows, requests and adapters that come with it (a @ x is otherwise
+    cut by their number)."""
     r = _row_call("add_adapters", x, base, x, a, b, scale, index, out, fixed_k_cut)
     if r is not None:
         return r

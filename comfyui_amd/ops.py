@@ -209,12 +209,12 @@ def _linear_upcast(lin, input, scale):
 
 
 class Adapters(torch.nn.Module):
-    """Low-rank adapters of many requests beside a Linear of this package: set as `linear.adapters`, they join each result of its forward, between its hooks. a [n, R, in], b [n, out, R] in the
-    activations' type, scale [n] fp32 (the usual alpha / rank times the strength). `index`, set before a forward, is int32 on the device with the
-    adapter of each request in the batch (-1: none), each request having as many rows as the others. Not in the reference, which patches a
-    LoRA into the weights: these differ between the requests of one batch, and the weights stay as they are. One forward of a model at a time: `index` is
-    the module's. Inference only, as the Linear is; autograd.add_adapters
-    has the gradients."""
+    """Low-rank adapters of many requests beside a Linear of this package: set as `linear.adapters`, they join each result of its forward, after its
+    pre-hooks and before its hooks. a [n, R, in], b [n, out, R] in the activations' type, scale [n] fp32 (the usual alpha / rank times the strength),
+    whatever the model is cast to. `index`, set before a forward, is int32 on the device with the adapter of each request in the batch (-1: none), each
+    request having as many rows as the others. Not in the reference, which patches a LoRA into the weights: these differ between the requests of one
+    batch, and the weights stay as they are. One forward of a model at a time: `index` is the module's. Inference only, as the Linear is;
+    autograd.add_adapters has the gradients."""
 
     def __init__(self, a, b, scale):
         super().__init__()

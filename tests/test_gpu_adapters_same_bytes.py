@@ -65,7 +65,7 @@ def test_routed_experts_among_others():
 
 
 def test_the_functions_own_flag():
-    """functional.add_adapters(fixed_k_cut=True) with and without the compiled call, and the gradient of it is not touched."""
+    """functional.add_adapters(fixed_k_cut=True) with and without the compiled call."""
     from comfyui_amd import functional as HF
     from tests.test_gpu_adapters import problem
     p = problem(3, 600, 1, 6912, 256, 3, 16, BF16)
